@@ -16,6 +16,7 @@ MAX_BLOCKS = 16
 FMT_TRELLIS_3INST = 0
 FMT_E8_SHELL = 1
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
+MX4_MXFP4, MX4_NVFP4 = 0, 1
 
 EXPORTS = [
     "glqb_plan_create", "glqb_plan_workspace_bytes", "glqb_plan_code_bytes", "glqb_plan_flops",
@@ -29,7 +30,16 @@ EXPORTS = [
     "glqb_comm_create", "glqb_comm_handle", "glqb_comm_connect", "glqb_comm_connect_local", "glqb_comm_set_timeout_ms",
     "glqb_comm_max_floats", "glqb_comm_all_reduce", "glqb_comm_status", "glqb_comm_epoch", "glqb_comm_destroy",
     "glqb_plan_set_comm",
+    "glqb_mx4_quantize", "glqb_mx4_dequantize", "glqb_mx4_image_bytes", "glqb_mx4_pack", "glqb_mx4_workspace_bytes",
+    "glqb_mx4_product", "glqb_mx4_status",
 ]
+
+
+class Mx4WeightDesc(C.Structure):
+    _fields_ = [
+        ("image", C.c_void_p), ("tensor_scale", C.c_void_p),
+        ("format", C.c_int32), ("experts", C.c_int32), ("m", C.c_int32), ("n", C.c_int32),
+    ]
 
 
 class MoeDesc(C.Structure):
@@ -177,6 +187,20 @@ def load() -> C.CDLL:
     lib.glqb_comm_destroy.restype = None
     lib.glqb_plan_set_comm.argtypes = [vp, vp]
     lib.glqb_plan_set_comm.restype = C.c_int
+    lib.glqb_mx4_quantize.argtypes = [vp, i32, i64, i64, i32, i32, vp, vp, vp, vp, vp]
+    lib.glqb_mx4_quantize.restype = C.c_int
+    lib.glqb_mx4_dequantize.argtypes = [vp, vp, vp, i64, i64, i32, i32, vp, i32, vp]
+    lib.glqb_mx4_dequantize.restype = C.c_int
+    lib.glqb_mx4_image_bytes.argtypes = [i32, i32, i32, i32]
+    lib.glqb_mx4_image_bytes.restype = sz
+    lib.glqb_mx4_pack.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp]
+    lib.glqb_mx4_pack.restype = C.c_int
+    lib.glqb_mx4_workspace_bytes.argtypes = [C.POINTER(Mx4WeightDesc), i64, i64, vp, i32]
+    lib.glqb_mx4_workspace_bytes.restype = sz
+    lib.glqb_mx4_product.argtypes = [C.POINTER(Mx4WeightDesc), vp, i32, i64, i64, vp, i32, i32, vp, vp, i32, i64, i32, i32, vp, sz, vp]
+    lib.glqb_mx4_product.restype = C.c_int
+    lib.glqb_mx4_status.argtypes = [C.POINTER(i32)]
+    lib.glqb_mx4_status.restype = C.c_int
     lib.glqb_last_error.argtypes = []
     lib.glqb_last_error.restype = C.c_char_p
     lib.glqb_version.argtypes = []

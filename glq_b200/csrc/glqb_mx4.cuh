@@ -1,0 +1,210 @@
+// Microscaled 4-bit floating point: formats, the weight image, and the conversions every kernel of glqb_mx4*.cu shares.
+//
+// A value is e2m1 (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) times the scale of its block:
+//   MXFP4  32 values share 2^(s - 127), s one byte (255: not a number)
+//   NVFP4  16 values share an e4m3 number, and a tensor (or expert) one fp32 number
+// Rows are stored as checkpoints store them: two codes to a byte, the even value in the low nibble, and one byte per block.
+//
+// The image of a weight matrix is those bytes in the order the products read them: tiles of 128 rows x 256 values,
+// [row tile][value tile], each 16 KiB of codes as a K-major tile with the 128-byte swizzle of the tensor core (so one bulk copy
+// brings what tcgen05.mma reads), then the scales of the tile, 512 bytes per four blocks: byte (r % 32) * 16 + (r / 32) * 4 + i
+// is block i of row r, which is how tcgen05.cp hands scales to tensor memory.  The eight codes of a 32-bit word lie in the order
+// 0 2 4 6 1 3 5 7: values 2i and 2i + 1 are nibbles i and i + 4, so that one shift and mask bring a pair to the halves of
+// a register.  (The 4-bit products do not see it: both operands have that order, and a word never leaves its block.)
+// Behind the tiles: for MXFP4 one byte per row, the largest scale of the row (see mx4_operand_scale).
+#pragma once
+#include "glqb_internal.h"
+#include <cuda_fp8.h>
+
+namespace glqb {
+
+constexpr int MX4_ROWS = 128, MX4_K = 256;                    // a tile
+constexpr int MX4_CODE_BYTES = MX4_ROWS * MX4_K / 2;          // 16 KiB
+
+template <int FMT> struct Mx4Fmt;
+template <> struct Mx4Fmt<GLQB_MX4_MXFP4> { static constexpr int BLOCK = 32; };
+template <> struct Mx4Fmt<GLQB_MX4_NVFP4> { static constexpr int BLOCK = 16; };
+__host__ __device__ constexpr int mx4_block(int fmt) { return fmt == GLQB_MX4_MXFP4 ? 32 : 16; }
+__host__ __device__ constexpr int mx4_scale_bytes(int fmt) { return MX4_ROWS * (MX4_K / mx4_block(fmt)); }   // of a tile
+__host__ __device__ constexpr int mx4_tile_bytes(int fmt) { return MX4_CODE_BYTES + mx4_scale_bytes(fmt); }
+
+// byte of the 32-bit word that holds value k (0..255) of row r of a tile
+__host__ __device__ __forceinline__ int mx4_word_offset(int r, int k) {
+  return (r >> 3) * 1024 + (r & 7) * 128 + (((k >> 5) ^ (r & 7)) << 4) + ((k >> 3) & 3) * 4;
+}
+// byte of the scale of block b (of a tile) of row r, behind the codes
+__host__ __device__ __forceinline__ int mx4_scale_offset(int r, int b) {
+  return (b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3);
+}
+
+#ifdef __CUDACC__
+// 0 1 2 3 4 5 6 7 -> 0 2 4 6 1 3 5 7
+__device__ __forceinline__ uint32_t mx4_interleave(uint32_t w) {
+  uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;            // even values, odd values, a byte each
+  lo = (lo | (lo >> 4)) & 0x00FF00FFu;
+  hi = (hi | (hi >> 4)) & 0x00FF00FFu;
+  return (lo | (lo >> 8)) & 0xFFFFu | ((hi | (hi >> 8)) << 16);
+}
+// Eight floats to e2m1, round to nearest even, saturating; `image`: in the image's order of nibbles.
+template <bool IMAGE>
+__device__ __forceinline__ uint32_t mx4_codes8(const float (&v)[8]) {
+  uint32_t r;
+  // (the first source of the conversion is the high nibble)
+  if constexpr (IMAGE)
+    asm("{ .reg .b8 a, b, c, d; cvt.rn.satfinite.e2m1x2.f32 a, %3, %1; cvt.rn.satfinite.e2m1x2.f32 b, %7, %5; "
+        "cvt.rn.satfinite.e2m1x2.f32 c, %4, %2; cvt.rn.satfinite.e2m1x2.f32 d, %8, %6; mov.b32 %0, {a, b, c, d}; }"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  else
+    asm("{ .reg .b8 a, b, c, d; cvt.rn.satfinite.e2m1x2.f32 a, %2, %1; cvt.rn.satfinite.e2m1x2.f32 b, %4, %3; "
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5; cvt.rn.satfinite.e2m1x2.f32 d, %8, %7; mov.b32 %0, {a, b, c, d}; }"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+__device__ __forceinline__ float mx4_magnitude(uint32_t code) {           // of the low three bits
+  const uint32_t e = (code >> 1) & 3u, m = code & 1u;
+  return e ? __uint_as_float((126u + e) << 23 | m << 22) : 0.5f * (float)m;
+}
+__device__ __forceinline__ float mx4_value(uint32_t code) {               // of a nibble
+  const float v = mx4_magnitude(code);
+  return code & 8u ? -v : v;
+}
+__device__ __forceinline__ float mx4_e4m3(uint32_t byte) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+}
+__device__ __forceinline__ float mx4_e8m0(uint32_t byte) {                // 2^(byte - 127)
+  return byte == 255u ? __uint_as_float(0x7FC00000u) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
+}
+template <int FMT>
+__device__ __forceinline__ float mx4_scale_value(uint32_t byte) {
+  if constexpr (FMT == GLQB_MX4_MXFP4) return mx4_e8m0(byte);
+  else return mx4_e4m3(byte);
+}
+
+// ---- quantisation ---------------------------------------------------------------------------------
+// The definition is in real numbers: the scale of an NVFP4 block is the e4m3 number nearest to amax / (6 t), a code the e2m1
+// number nearest to x / (s t), ties to even.  fp32 quotients can land on the wrong side of a border, so the conversion is done
+// for the quotient a little smaller and a little larger (its error is below 1.5 * 2^-22, the margin 2^-21); where the two disagree
+// the side is taken from an exact comparison: border * s and border * 6 have at most eight bits, so fma(-p, t, x) has the
+// sign of x - border * s * t.  (MXFP4 divides by powers of two: nothing to decide.)
+constexpr float MX4_BELOW = 1.0f - 0x1p-21f, MX4_ABOVE = 1.0f + 0x1p-21f;
+// Steps below 2^-100 would lose bits in that product, and their reciprocal's range ends: 64 bits there.
+constexpr float MX4_TINY = 0x1p-100f;
+
+__device__ __forceinline__ uint32_t mx4_nv_scale(float amax, float t) {
+  const float q = __fdividef(amax, 6.0f * t);
+  uint16_t both;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(both) : "f"(q * MX4_ABOVE), "f"(q * MX4_BELOW));
+  const uint32_t lo = both & 0xFFu, hi = both >> 8;
+  const bool tiny = t < MX4_TINY || t > 0x1p100f;
+  if (lo == hi && !tiny) return lo;
+  if (tiny) {
+    // amax / (6 t) to the nearest, by its distance to the neighbours of the value that fp32 arithmetic of 64 bits gives
+    const double d = fmin((double)amax / (6.0 * (double)t), 448.0);
+    uint32_t s = __nv_cvt_double_to_fp8(d, __NV_SATFINITE, __NV_E4M3) & 0x7Fu;
+    while (s < 126u && 2.0 * d > (double)mx4_e4m3(s) + (double)mx4_e4m3(s + 1u)) ++s;
+    while (s > 0u && 2.0 * d < (double)mx4_e4m3(s) + (double)mx4_e4m3(s - 1u)) --s;
+    if (s < 126u && (s & 1u) && 2.0 * d == (double)mx4_e4m3(s) + (double)mx4_e4m3(s + 1u)) ++s;
+    else if (s > 0u && (s & 1u) && 2.0 * d == (double)mx4_e4m3(s) + (double)mx4_e4m3(s - 1u)) --s;
+    return s;
+  }
+  const float middle = 0.5f * (mx4_e4m3(lo) + mx4_e4m3(hi)), rest = fmaf(-(middle * 6.0f), t, amax);
+  return rest > 0.0f ? hi : rest < 0.0f ? lo : (lo & 1u) ? hi : lo;
+}
+// magnitude code of |x| / (s t), from the codes of a slightly smaller and a slightly larger quotient
+__device__ __forceinline__ uint32_t mx4_decide(uint32_t lo, uint32_t hi, float x, float s, float t) {
+  if (lo == hi) return lo;
+  const float border = 0.5f * (mx4_magnitude(lo) + mx4_magnitude(hi)), rest = fmaf(-(border * s), t, x);
+  return rest > 0.0f ? hi : rest < 0.0f ? lo : (lo & 1u) ? hi : lo;
+}
+__device__ __noinline__ uint32_t mx4_decide_tiny(float x, float s, float t) {
+  const double d = (double)s * (double)t, a = (double)x;      // (31 bits: products with the borders are exact)
+  return (uint32_t)((a > 0.25 * d) + (a >= 0.75 * d) + (a > 1.25 * d) + (a >= 1.75 * d) + (a > 2.5 * d) + (a >= 3.5 * d) + (a > 5.0 * d));
+}
+
+// Eight consecutive values of a row per thread; the BLOCK / 8 threads of a block are neighbours in a warp (all 32 lanes take
+// part).  Returns the eight codes; `scale`: the block's byte, the same in its threads.  A block with an infinity or NaN
+// gets the scale NaN and codes of zero.
+template <int FMT, bool IMAGE>
+__device__ __forceinline__ uint32_t mx4_quantize8(const float (&v)[8], float t, uint32_t& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int d = 1; d < Mx4Fmt<FMT>::BLOCK / 8; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  const bool broken = top >= 0x7F800000u;
+  if constexpr (FMT == GLQB_MX4_MXFP4) {
+    const uint32_t e = top >> 23;
+    scale = broken ? 255u : e > 2u ? e - 2u : 0u;
+    if (broken) return 0u;
+    const float r = __uint_as_float((254u - scale) << 23);
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = v[i] * r;
+    return mx4_codes8<IMAGE>(q);
+  } else {
+    scale = broken ? 0x7Fu : mx4_nv_scale(__uint_as_float(top), t);
+    if (broken) return 0u;
+    const float s = mx4_e4m3(scale), step = s * t;
+    float lo[8], hi[8];
+    if (step >= MX4_TINY) {
+      const float r = __frcp_rn(step), rl = r * MX4_BELOW, rh = r * MX4_ABOVE;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { lo[i] = v[i] * rl; hi[i] = v[i] * rh; }
+      const uint32_t a = mx4_codes8<IMAGE>(lo), b = mx4_codes8<IMAGE>(hi);
+      if (a == b) return a;
+      uint32_t c = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = IMAGE ? (i >> 1) + 4 * (i & 1) : i;
+        const uint32_t l = (a >> (4 * at)) & 15u, h = (b >> (4 * at)) & 15u;
+        c |= (mx4_decide(l & 7u, h & 7u, fabsf(v[i]), s, t) | (l & 8u)) << (4 * at);
+      }
+      return c;
+    }
+    uint32_t c = 0;
+    if (scale != 0u) {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const int at = IMAGE ? (i >> 1) + 4 * (i & 1) : i;
+        float x = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) x = i == j ? v[j] : x;
+        c |= (mx4_decide_tiny(fabsf(x), s, t) | (x < 0.0f ? 8u : 0u)) << (4 * at);
+      }
+    }
+    return c;
+  }
+}
+
+// the fp32 scale of a tensor whose largest finite value is `amax`: the top of both levels, 448 * 6
+__device__ __forceinline__ float mx4_tensor_scale(float amax) { return fmaxf(__fdiv_rn(amax, 2688.0f), 0x1p-126f); }
+
+// ---- loads of activations -------------------------------------------------------------------------
+// values col .. col + 7 of a row as fp32, zeros from `cols` on; `vec`: rows start on 16 bytes
+template <typename T>
+__device__ __forceinline__ void mx4_load8(const T* row, int col, int cols, bool vec, float (&v)[8]) {
+  if (vec && col + 8 <= cols) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(row + col), b = *reinterpret_cast<const float4*>(row + col + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + col);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (__is_same(T, __half)) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        } else {
+          v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? (float)row[col + i] : 0.0f;
+  }
+}
+#endif  // __CUDACC__
+
+}  // namespace glqb

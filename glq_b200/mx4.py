@@ -1,0 +1,306 @@
+"""Microscaled 4-bit floating point: quantisation, and products with weights held in it.
+
+Two formats.  ``"mxfp4"``: e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign) under one power of two per 32 consecutive
+values of a row.  ``"nvfp4"``: e2m1 values under one e4m3 scale per 16 consecutive values and one fp32 scale per tensor (or
+expert).  Rows are stored as checkpoints hold them: two codes to a byte, the even value in the low nibble, and one scale byte
+per block.  ``mx4_pack`` lays weights out once for the products; ``mx4_linear`` multiplies a layer, ``mx4_grouped_linear`` one
+matrix per expert with ragged numbers of rows.  The operators run on the current stream of their tensors' device, take a
+workspace from torch's allocator where they need one, read nothing back and can be captured into a CUDA graph.  They have no
+gradients.  No counterpart in the reference, whose formats are the E8 shell and the trellis code.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+_FORMATS = {"mxfp4": _lib.MX4_MXFP4, "nvfp4": _lib.MX4_NVFP4}
+_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_RAN_ON: set = set()                # devices whose status word a product may have set
+_DTYPES = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
+
+
+class Mx4Tensor(NamedTuple):
+    """Values in 4 bits: ``codes`` uint8 (..., ceil(cols / 2)), ``scales`` uint8 (..., ceil(cols / block)), both dense; for
+    "nvfp4" ``tensor_scale``, fp32: one, or one per matrix of a three-dimensional tensor."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    format: str
+    cols: int
+    tensor_scale: Optional[torch.Tensor] = None
+
+
+class Mx4Weight:
+    """Weights laid out for the products (``mx4_pack``): (out_features, in_features), or one such matrix per expert."""
+    __slots__ = ("image", "tensor_scale", "format", "experts", "out_features", "in_features", "_desc", "_ref")
+
+    def __init__(self, image, tensor_scale, format, experts, out_features, in_features):
+        self.image, self.tensor_scale, self.format, self.experts = image, tensor_scale, format, experts
+        self.out_features, self.in_features = out_features, in_features
+        self._desc = _lib.Mx4WeightDesc(image.data_ptr(), tensor_scale.data_ptr() if tensor_scale is not None else 0,
+                                        _FORMATS[format], experts or 1, out_features, in_features)
+        self._ref = C.byref(self._desc)
+
+
+class _on:
+    """The device of a call made current: kernels of another device's tensors are launched there."""
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.before)
+        return False
+
+
+def _format(format):
+    if format not in _FORMATS:
+        raise ValueError(f'glq_b200: format is "mxfp4" or "nvfp4", not {format!r}')
+    return _FORMATS[format]
+
+
+def _cuda(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"glq_b200: {name} must be a CUDA tensor (there is no CPU path)")
+
+
+def _same_device(t, x, name):
+    _cuda(t, name)
+    if t.get_device() != x.get_device():
+        raise ValueError(f"glq_b200: {name} is on {t.device}, expected {x.device}")
+
+
+def _dtype(dtype, what):
+    d = _DTYPES.get(dtype)
+    if d is None:
+        raise ValueError(f"glq_b200: {what} is bf16, fp16 or fp32, not {dtype}")
+    return d
+
+
+def _scale_ptr(t, x, name, count=1):
+    _same_device(t, x, name)
+    if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"glq_b200: {name} must be {count} fp32 value{'s' if count > 1 else ''}, got {tuple(t.shape)} of {t.dtype}")
+    return t.data_ptr()
+
+
+def _rows(x, cols):
+    """x (..., cols) as rows of consecutive values; rows that overlap (an expanded tensor) are copied."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, cols)
+    if (cols > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < cols):
+        x2 = x2.contiguous()
+    return x2
+
+
+def mx4_quantize(x, format="mxfp4", tensor_scale=None) -> Mx4Tensor:
+    """x (..., cols) of bf16, fp16 or fp32 to 4 bits, each value to the nearest (ties to the even code) of its block's scale.
+    "mxfp4": the scale is 2^(floor(log2 amax) - 2), values above six times it saturate.  "nvfp4": the block's scale is the
+    e4m3 number nearest to amax / (6 t), with t the one fp32 value ``tensor_scale`` (positive), or, without it,
+    max(largest finite |x| / 2688, 2^-126), found by a first pass.  A block with an infinity or NaN becomes NaN."""
+    fmt = _format(format)
+    _cuda(x, "x")
+    dt = _dtype(x.dtype, "x")
+    if x.dim() == 0:
+        raise ValueError("glq_b200: x needs at least one dimension")
+    cols = x.shape[-1]
+    x2 = _rows(x, cols) if x.numel() else x.reshape(0, max(cols, 1))
+    codes = torch.empty(x.shape[:-1] + ((cols + 1) // 2,), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.shape[:-1] + (-(-cols // _BLOCK[format]),), dtype=torch.uint8, device=x.device)
+    given = own = None
+    if format == "nvfp4":
+        if tensor_scale is None:
+            own = torch.empty(2, dtype=torch.float32, device=x.device)
+        else:
+            given = _scale_ptr(tensor_scale, x, "tensor_scale")
+    elif tensor_scale is not None:
+        raise ValueError('glq_b200: "mxfp4" has no tensor_scale')
+    if x.numel():
+        with _on(x.get_device()) as stream:
+            _lib.check(_lib.load().glqb_mx4_quantize(x2.data_ptr(), dt, x2.stride(0), x2.shape[0], cols, fmt, given,
+                                                     own.data_ptr() if own is not None else None, codes.data_ptr(),
+                                                     scales.data_ptr(), stream), "mx4_quantize")
+    elif own is not None:
+        own.fill_(2.0 ** -126)
+    return Mx4Tensor(codes, scales, format, cols, own[:1] if own is not None else tensor_scale)
+
+
+def _checked(q: Mx4Tensor):
+    """(format, rows, values per row, matrices) of an Mx4Tensor."""
+    fmt = _format(q.format)
+    _cuda(q.codes, "codes")
+    _same_device(q.scales, q.codes, "scales")
+    cols, lead = int(q.cols), q.codes.shape[:-1]
+    if q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8 or q.codes.dim() < 1:
+        raise ValueError("glq_b200: codes and scales are uint8 tensors of stored rows")
+    if q.codes.shape[-1] != (cols + 1) // 2 or q.scales.shape != lead + (-(-cols // _BLOCK[q.format]),):
+        raise ValueError(f"glq_b200: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} are not {q.format} rows of {cols} values")
+    rows = 1
+    for d in lead:
+        rows *= d
+    scales = 0
+    if q.format == "nvfp4":
+        if q.tensor_scale is None:
+            raise ValueError('glq_b200: "nvfp4" needs its tensor_scale')
+        scales = q.tensor_scale.numel()
+        if scales != 1 and not (len(lead) == 2 and scales == lead[0]):
+            raise ValueError(f"glq_b200: {scales} tensor scales for rows of {tuple(lead)}")
+        _scale_ptr(q.tensor_scale, q.codes, "tensor_scale", scales)
+    return fmt, rows, cols, scales
+
+
+def mx4_dequantize(q: Mx4Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values (..., cols) an ``Mx4Tensor`` stands for, formed in fp32 and rounded to ``dtype``."""
+    fmt, rows, cols, scales = _checked(q)
+    dt = _dtype(dtype, "dtype")
+    codes, sc = q.codes.contiguous(), q.scales.contiguous()
+    out = torch.empty(codes.shape[:-1] + (cols,), dtype=dtype, device=codes.device)
+    if out.numel():
+        with _on(codes.get_device()) as stream:
+            _lib.check(_lib.load().glqb_mx4_dequantize(codes.data_ptr(), sc.data_ptr(),
+                                                       q.tensor_scale.data_ptr() if scales else None, rows // max(scales, 1),
+                                                       rows, cols, fmt, out.data_ptr(), dt, stream), "mx4_dequantize")
+    return out
+
+
+def mx4_pack(q: Mx4Tensor) -> Mx4Weight:
+    """Weights (m, n), or (experts, m, n), laid out for ``mx4_linear`` / ``mx4_grouped_linear``: once, when they are loaded.
+    The image has the size of codes and scales, rows rounded up to 128 and values to 256."""
+    fmt, rows, n, scales = _checked(q)
+    if q.codes.dim() not in (2, 3):
+        raise ValueError(f"glq_b200: weights are (m, n) or (experts, m, n), got codes of {tuple(q.codes.shape)}")
+    experts, m = (q.codes.shape[0] if q.codes.dim() == 3 else None), q.codes.shape[-2]
+    if rows == 0 or n == 0:
+        raise ValueError(f"glq_b200: empty weights, codes of {tuple(q.codes.shape)}")
+    codes, sc = q.codes.contiguous(), q.scales.contiguous()
+    lib = _lib.load()
+    image = torch.empty(lib.glqb_mx4_image_bytes(fmt, experts or 1, m, n), dtype=torch.uint8, device=codes.device)
+    with _on(codes.get_device()) as stream:
+        _lib.check(lib.glqb_mx4_pack(codes.data_ptr(), sc.data_ptr(), fmt, experts or 1, m, n, image.data_ptr(), stream), "mx4_pack")
+    t = q.tensor_scale
+    if scales:
+        t = t.reshape(1).expand(experts or 1).contiguous() if scales == 1 else t.reshape(-1)
+    return Mx4Weight(image, t, q.format, experts, m, n)
+
+
+def _overlap(a, b):
+    def span(t):
+        first = t.data_ptr()
+        return first, first + (sum((d - 1) * s for d, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _product(x, w, offsets, quantize_input, input_scale, y, accumulate, clear_rest):
+    """The call itself: x and y two-dimensional with consecutive values in a row."""
+    dt = _DTYPES[x.dtype]
+    xs = None
+    if input_scale is not None:
+        if not quantize_input or w.format != "nvfp4":
+            raise ValueError('glq_b200: input_scale belongs to quantize_input with "nvfp4" weights')
+        xs = _scale_ptr(input_scale, x, "input_scale")
+    if x.shape[0] == 0:
+        return
+    lib = _lib.load()
+    with _on(x.get_device()) as stream:
+        size = lib.glqb_mx4_workspace_bytes(w._ref, x.shape[0], x.stride(0), x.data_ptr(), quantize_input)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        rc = lib.glqb_mx4_product(w._ref, x.data_ptr(), dt, x.stride(0), x.shape[0], offsets.data_ptr() if offsets is not None else None,
+                                  offsets is not None and offsets.dtype == torch.int64, quantize_input, xs, y.data_ptr(),
+                                  _DTYPES[y.dtype], y.stride(0), accumulate, clear_rest, ws.data_ptr() if size else None, size, stream)
+    if rc:
+        _lib.check(rc, "mx4_product")
+    _RAN_ON.add(x.get_device())
+
+
+def _input(x, w, quantize_input):
+    if not isinstance(w, Mx4Weight):
+        raise ValueError("glq_b200: weight is what mx4_pack returns")
+    _cuda(x, "x")
+    if x.get_device() != w.image.get_device():
+        raise ValueError(f"glq_b200: x is on {x.device}, the weight on {w.image.device}")
+    _dtype(x.dtype, "x")
+    if x.dtype == torch.float32 and not quantize_input:
+        raise ValueError("glq_b200: x is bf16 or fp16 (fp32 with quantize_input only)")
+    if x.dim() < 1 or x.shape[-1] != w.in_features:
+        raise ValueError(f"glq_b200: x of {tuple(x.shape)} for a weight of {w.in_features} inputs")
+
+
+def mx4_linear(x, weight: Mx4Weight, *, quantize_input=False, input_scale=None, out_dtype=None, accumulate_into=None):
+    """x (..., n) times a packed (m, n) weight: (..., m), sums in fp32 and one rounding.  x is bf16 or fp16 and is taken as it is; with
+    ``quantize_input`` (then fp32 too) it is brought to the weight's format first, as ``mx4_quantize`` does ("nvfp4": by
+    ``input_scale``, one fp32 value, or by the scale of the whole of x), and the tensor cores multiply 4-bit values, at four times
+    their 16-bit rate.  ``accumulate_into`` adds the result to that dense (..., m) tensor in place (residual add, before the
+    rounding) and returns it."""
+    _input(x, weight, quantize_input)
+    if weight.experts is not None:
+        raise ValueError("glq_b200: mx4_linear takes one matrix, not one per expert")
+    n, m = weight.in_features, weight.out_features
+    rows = x.numel() // n
+    if accumulate_into is not None:
+        _same_device(accumulate_into, x, "accumulate_into")
+        out = accumulate_into
+        if out_dtype not in (None, out.dtype):
+            raise ValueError(f"glq_b200: accumulate_into is {out.dtype}, out_dtype {out_dtype}")
+        if out.dim() < 1 or out.shape[-1] != m or out.numel() != rows * m or not out.is_contiguous():
+            raise RuntimeError("glq_b200: accumulate_into must be a dense (tokens, out_features) tensor")
+    else:
+        out = torch.empty(x.shape[:-1] + (m,), dtype=out_dtype or x.dtype, device=x.device)
+    _dtype(out.dtype, "the result")
+    if rows:
+        x2 = _rows(x, n)
+        if accumulate_into is not None and _overlap(x2, out):
+            raise ValueError("glq_b200: accumulate_into overlaps x")
+        _product(x2, weight, None, bool(quantize_input), input_scale, out.view(rows, m), accumulate_into is not None, False)
+    return out
+
+
+def mx4_grouped_linear(x, weight: Mx4Weight, offsets, *, quantize_input=False, input_scale=None, out_dtype=None, out=None):
+    """Products grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of x (rows, n) times matrix e of a packed
+    (experts, m, n) weight: (rows, m).  ``offsets``: experts + 1 ascending integers (int32 or int64) on the device, any number of
+    rows per expert, none included; nothing is read back.  Rows of no expert (in front of offsets[0], behind offsets[experts])
+    are zero in a new result and stay as they are in a given ``out`` (rows, m), whose rows may lie apart.  Offsets outside
+    0 .. rows are held to that range, and an expert whose range ends before it begins has no rows.  The other arguments as for
+    ``mx4_linear``; "nvfp4" inputs without ``input_scale`` take the scale of rows offsets[0] .. offsets[experts] - 1."""
+    _input(x, weight, quantize_input)
+    if weight.experts is None:
+        raise ValueError("glq_b200: mx4_grouped_linear takes one matrix per expert")
+    if x.dim() != 2:
+        raise ValueError(f"glq_b200: x is (rows, n), got {tuple(x.shape)}")
+    _same_device(offsets, x, "offsets")
+    if offsets.dtype not in (torch.int32, torch.int64) or offsets.dim() != 1 or offsets.numel() != weight.experts + 1 or not offsets.is_contiguous():
+        raise ValueError(f"glq_b200: offsets must be {weight.experts + 1} int32 or int64 values, got {tuple(offsets.shape)} of {offsets.dtype}")
+    rows, m = x.shape[0], weight.out_features
+    fresh = out is None
+    if fresh:
+        out = torch.empty(rows, m, dtype=out_dtype or x.dtype, device=x.device)
+    else:
+        _same_device(out, x, "out")
+        if out_dtype not in (None, out.dtype):
+            raise ValueError(f"glq_b200: out is {out.dtype}, out_dtype {out_dtype}")
+        if out.shape != (rows, m) or (m > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < m):
+            raise ValueError(f"glq_b200: out must be ({rows}, {m}) with consecutive values in a row, got {tuple(out.shape)}")
+    _dtype(out.dtype, "the result")
+    if rows:
+        x2 = _rows(x, weight.in_features)
+        if not fresh and _overlap(x2, out):
+            raise ValueError("glq_b200: out overlaps x")
+        _product(x2, weight, offsets, bool(quantize_input), input_scale, out, False, fresh)
+    return out
+
+
+def mx4_check_status() -> None:
+    """Synchronise the devices that products ran on and raise RuntimeError (code GLQB_E_DEVICE) if a bounded wait in one of them
+    gave up since the last call: the results of that run are invalid."""
+    for index in sorted(_RAN_ON):
+        with _on(index):
+            _lib.check(_lib.load().glqb_mx4_status(None), "mx4 status")

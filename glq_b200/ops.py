@@ -21,6 +21,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
+from .mx4 import (Mx4Tensor, Mx4Weight, mx4_check_status, mx4_dequantize, mx4_grouped_linear, mx4_linear,  # noqa: F401
+                  mx4_pack, mx4_quantize)
 from .plan import LinearSpec, Plan, block_decompose
 
 DECODE_MAX_TOKENS = 64
@@ -139,6 +141,7 @@ def check_device_status() -> None:
     for p in list(_PLAN_CACHE.values()):
         if hasattr(p, "check_status"):
             p.check_status()
+    mx4_check_status()
 
 
 def clear_caches() -> None:

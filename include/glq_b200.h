@@ -292,6 +292,55 @@ int glqb_trellis_linear_noalloc(const void* x, int32_t x_dtype, void* y, int32_t
                                 int32_t n_blocks_m, void* stream);
 size_t glqb_noalloc_scratch_bytes(void);
 
+/*
+ * Microscaled 4-bit floating point ("mx4"): e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) under a scale per
+ * block of consecutive values of a row.  No counterpart in the reference.
+ *   GLQB_MX4_MXFP4  blocks of 32, the scale byte s stands for 2^(s - 127), 255 for NaN
+ *   GLQB_MX4_NVFP4  blocks of 16, the scale byte is an e4m3 number (>= 0), times one fp32 number per tensor (or expert)
+ * Stored rows: codes two to a byte, the even value in the low nibble, ceil(cols / 2) bytes; ceil(cols / block) scale bytes.
+ * All entry points enqueue on `stream` and neither allocate nor synchronise, unless stated.
+ */
+#define GLQB_MX4_MXFP4 0
+#define GLQB_MX4_NVFP4 1
+
+/* rows x cols values (x_stride elements apart) to stored rows, each rounded to nearest even from the real quotient by its
+ * block's scale: MXFP4 2^(floor(log2 amax) - 2), saturating at 6; NVFP4 e4m3(amax / (6 t)), t = *tensor_scale (positive), or,
+ * with tensor_scale NULL, max(largest finite |x| / 2688, 2^-126), which is left in own_scale[0] (own_scale: two floats,
+ * needed then).  A block with an infinity or NaN gets the scale NaN and codes of zero. */
+int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows, int32_t cols, int32_t format,
+                      const float* tensor_scale, float* own_scale, void* codes, void* scales, void* stream);
+/* The values stored rows stand for; row r takes tensor_scale[r / rows_per_scale] (NVFP4). */
+int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tensor_scale, int64_t rows_per_scale, int64_t rows,
+                        int32_t cols, int32_t format, void* out, int32_t out_dtype, void* stream);
+
+/* A matrix (m x n), or one per expert, laid out for the products; see glqb_mx4_pack. */
+typedef struct GlqbMx4Weight {
+  const void* image;                     /* glqb_mx4_image_bytes bytes, 128-byte aligned */
+  const float* tensor_scale;             /* NVFP4: fp32 per expert; MXFP4: NULL */
+  int32_t format, experts, m, n;
+} GlqbMx4Weight;
+size_t glqb_mx4_image_bytes(int32_t format, int32_t experts, int32_t m, int32_t n);
+/* stored rows (experts * m of them, n values each) into an image */
+int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t experts, int32_t m, int32_t n, void* image,
+                  void* stream);
+
+/* y[r] = x[r] W_e^T, fp32 sums rounded once.  offsets NULL: one matrix, all rows.  Else device integers (int64 with
+ * offsets_are_int64, else int32), experts + 1 of them: rows offsets[e] .. offsets[e + 1] - 1 of x and y belong to expert e.  They
+ * are read on the device and held to 0 .. rows; a range that ends before it begins is empty.  Rows of no expert keep what y
+ * holds, or are zeroed with clear_rest.
+ * quantize: x is brought to the weights' format first, as glqb_mx4_quantize does (NVFP4: by *x_scale, or, with x_scale NULL, by the
+ * scale of rows offsets[0] .. offsets[experts] - 1), and 4-bit values are multiplied.  Without it x is fp16 or bf16 and stays so.
+ * MXFP4 weights are held relative to the largest scale of their row: under fp16 activations a block more than 2^24 below it
+ * loses bits, 2^132 under bf16.
+ * accumulate: y <- y + result, added before the rounding.  A bounded wait that gives up sets the device's status word. */
+size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize);
+int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows,
+                     const void* offsets, int32_t offsets_are_int64, int32_t quantize, const float* x_scale,
+                     void* y, int32_t y_dtype, int64_t y_stride, int32_t accumulate, int32_t clear_rest,
+                     void* workspace, size_t workspace_bytes, void* stream);
+/* Synchronising read of the current device's status word, which it clears: GLQB_E_DEVICE if a wait gave up since the last. */
+int glqb_mx4_status(int32_t* status_out);
+
 const char* glqb_last_error(void);
 const char* glqb_version(void);
 

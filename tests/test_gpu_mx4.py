@@ -1,0 +1,493 @@
+"""Microscaled 4-bit floating point on the GPU against 64-bit numpy.
+
+Tolerances.  Quantisation and dequantisation are exact up to the output's one rounding.  Products: n fp32 additions, each off by
+at most 2^-23 of what has been summed (the tensor cores cut off instead of rounding), so n * 2^-23 * sum |x w|; then the result's
+rounding, half a step: finfo.eps / 2 relative to the value (and half its smallest subnormal).
+"""
+import numpy as np
+import pytest
+import torch
+
+import mx4_oracle as O
+from glq_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+FORMATS = ["mxfp4", "nvfp4"]
+
+
+def host(t):
+    return t.detach().double().cpu().numpy()
+
+
+def to_cuda(a, dtype=torch.float32):
+    return torch.from_numpy(np.ascontiguousarray(a)).to("cuda").to(dtype)
+
+
+def check_quantized(x, fmt, t=None):
+    """quantise x on the GPU and compare codes, scales and the tensor's scale with the oracle, bit for bit."""
+    given = None if t is None else torch.tensor([t], dtype=torch.float32, device="cuda")
+    q = ops.mx4_quantize(x, fmt, given)
+    v = host(x).reshape(-1, x.shape[-1])
+    if fmt == "nvfp4":
+        ts = np.float32(O.tensor_scale(v)) if t is None else np.float32(t)
+        assert q.tensor_scale.item() == ts
+    else:
+        ts = None
+    code, byte = O.quantize(v, fmt, ts)
+    got = O.unpack_nibbles(q.codes.cpu().numpy().reshape(len(v), -1), x.shape[-1])
+    scales = q.scales.cpu().numpy().reshape(len(v), -1)
+    assert np.array_equal(scales, byte)
+    # (zeros may carry either sign)
+    assert np.array_equal(np.where(got & 7, got, 0), np.where(code & 7, code, 0))
+    if x.shape[-1] % 2:
+        assert not (q.codes.cpu().numpy().reshape(len(v), -1)[:, -1] & 0xF0).any()
+    return q
+
+
+# ---- quantisation ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (2, 8), (5, 15), (1, 16), (4, 17), (3, 32), (2, 33), (7, 100), (64, 256), (13, 1000), (1, 2048), (300, 4100)])
+def test_quantize_matches_definition(fmt, dtype, rows, cols):
+    g = np.random.default_rng(rows * 10007 + cols)
+    x = to_cuda(g.standard_normal((rows, cols)) * np.exp(g.standard_normal((rows, 1)) * 3), DT[dtype])
+    q = check_quantized(x, fmt)
+    assert q.codes.shape == (rows, (cols + 1) // 2) and q.cols == cols
+
+
+@pytest.mark.parametrize("t", [1.0, 0.37, 2.0 ** -20, 1e-31, 3e-38, 1e30, 5e34])
+def test_nvfp4_given_scale_and_ties(t):
+    """Values on the borders of codes and of block scales: multiples of an eighth of the scale."""
+    g = np.random.default_rng(5)
+    x = (g.integers(-64, 65, (64, 160)) * 0.125) * np.float64(t)
+    x[:, ::16] = np.float64(t) * 6 * O.E4M3[g.integers(40, 90, (64, 10))] * g.choice([1.0, 1.0625, 1.03125, 0.96875], (64, 10))
+    check_quantized(to_cuda(x), "nvfp4", t)
+
+
+def test_nvfp4_every_block_scale_border():
+    """A block whose largest value lies on the middle between two e4m3 scales, and one fp32 step to either side."""
+    middle = (O.E4M3[1:] + O.E4M3[:-1]) / 2
+    for t in (1.0, 0.7):
+        top = (6.0 * middle * np.float64(np.float32(t))).astype(np.float32)
+        x = np.zeros((3 * len(top), 16), np.float32)
+        x[0::3, 3], x[1::3, 3], x[2::3, 3] = top, np.nextafter(top, np.float32(0)), -np.nextafter(top, np.float32(np.inf))
+        check_quantized(to_cuda(x), "nvfp4", t)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_extremes(fmt):
+    x = np.zeros((10, 64), np.float32)
+    x[0, 5] = np.inf
+    x[1, 40] = np.nan
+    x[2, :] = 3.4e38
+    x[3, :] = np.float32(1e-45)
+    x[4, ::3] = 1.1754944e-38
+    x[5, 7] = -7.99
+    x[6] = np.linspace(-6, 6, 64)
+    x[7, 3], x[7, 4] = 1e30, 1e-30
+    x[8, 0], x[8, 1] = -np.inf, np.nan
+    for rows in (x, x[3:5], x[9:], x[5:7]):
+        check_quantized(to_cuda(rows), fmt, None)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_strides_alignment_and_shapes(fmt):
+    g = np.random.default_rng(1)
+    base = to_cuda(g.standard_normal((40, 531)), torch.bfloat16)
+    check_quantized(base[3:, 5:517], fmt)                       # rows that start on odd addresses
+    check_quantized(base[:, :512], fmt)
+    check_quantized(base[::2, 3:100], fmt)
+    check_quantized(base.t(), fmt)                              # values apart
+    check_quantized(base[0].expand(7, 531), fmt)                # the same row again
+    check_quantized(base[:, :520].reshape(5, 8, 520), fmt)
+    check_quantized(base[0], fmt)
+    for shape in ((0, 64), (3, 0), (0,), (2, 0, 5)):
+        q = ops.mx4_quantize(torch.zeros(shape, device="cuda"), fmt)
+        assert q.codes.shape[:-1] == shape[:-1] and q.codes.numel() == 0
+        assert ops.mx4_dequantize(q).shape == shape
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 33), (8, 64), (5, 1001), (3, 4, 80)])
+def test_dequantize_every_byte(fmt, dtype, shape):
+    g = np.random.default_rng(shape[-1])
+    cols, lead = shape[-1], shape[:-1]
+    code = g.integers(0, 16, shape, dtype=np.uint8)
+    byte = g.integers(0, 256 if fmt == "mxfp4" else 128, lead + (-(-cols // O.BLOCK[fmt]),), dtype=np.uint8)
+    per = lead[0] if len(lead) == 2 else 1
+    t = np.float32(g.uniform(0.1, 3, per)) if fmt == "nvfp4" else None
+    q = ops.Mx4Tensor(to_cuda(O.pack_nibbles(code), torch.uint8), to_cuda(byte, torch.uint8), fmt, cols, to_cuda(t) if t is not None else None)
+    got = ops.mx4_dequantize(q, DT[dtype])
+    want = O.values(code, byte, fmt)
+    if t is not None:
+        want = (want.astype(np.float32) * t.reshape((per,) + (1,) * (want.ndim - 1))) if per > 1 else want.astype(np.float32) * t[0]
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(want.astype(np.float32)).to(DT[dtype])
+    assert torch.equal(torch.nan_to_num(got.cpu(), nan=7.5), torch.nan_to_num(want, nan=7.5))
+
+
+# ---- products --------------------------------------------------------------------------------------------------
+def make_weight(g, shape, fmt, spread=1.0):
+    """(packed weight, values in 64 bits (E, m, n) or (m, n))."""
+    n = shape[-1]
+    w = g.standard_normal(shape) * np.exp(g.standard_normal(shape[:-1] + (1,)) * spread) / np.sqrt(n)
+    flat = w.reshape(-1, n)
+    if fmt == "nvfp4":
+        groups = shape[0] if len(shape) == 3 else 1
+        t = np.array([O.tensor_scale(p) for p in flat.reshape(groups, -1, n)], np.float32)
+        parts = [O.quantize(p, fmt, ti) for p, ti in zip(flat.reshape(groups, -1, n), t)]
+        code, byte = np.concatenate([p[0] for p in parts]), np.concatenate([p[1] for p in parts])
+        vals = np.concatenate([O.values(*p, fmt, ti) for p, ti in zip(parts, t)])
+    else:
+        t = None
+        code, byte = O.quantize(flat, fmt)
+        vals = O.values(code, byte, fmt)
+    lead = shape[:-1]
+    q = ops.Mx4Tensor(to_cuda(O.pack_nibbles(code).reshape(lead + (-1,)), torch.uint8), to_cuda(byte.reshape(lead + (-1,)), torch.uint8), fmt, n,
+                      to_cuda(t) if t is not None else None)
+    return ops.mx4_pack(q), vals.reshape(shape)
+
+
+def quantized_values(x, fmt, t=None):
+    ts = None if fmt == "mxfp4" else np.float32(O.tensor_scale(x) if t is None else t)
+    return O.values(*O.quantize(x, fmt, ts), fmt, ts)
+
+
+def tolerance(x, w, want, dtype):
+    f = torch.finfo(dtype)
+    return x.shape[-1] * 2.0 ** -23 * (np.abs(x) @ np.abs(w).T) + f.eps / 2 * np.abs(want) + f.smallest_normal * f.eps / 2
+
+
+def check_product(got, x, w, dtype, add=None):
+    want = x @ w.T
+    tol = tolerance(x, w, want if add is None else np.abs(want) + np.abs(add), dtype)
+    if add is not None:
+        want = want + add
+    err = np.abs(host(got) - want)
+    assert np.all(err <= tol), f"off by {np.nanmax(err / tol):.3g} tolerances at {np.unravel_index(np.argmax(err / tol), err.shape)}"
+
+
+SIZES = [(1, 1, 1), (1, 128, 256), (1, 64, 64), (2, 130, 96), (1, 200, 1024), (3, 17, 33), (5, 300, 520), (8, 128, 2048), (9, 256, 256), (16, 384, 640),
+         (17, 129, 257), (31, 128, 512), (33, 500, 1000), (64, 256, 768), (65, 128, 320), (100, 640, 512), (129, 130, 300), (192, 128, 256),
+         (193, 257, 264), (300, 384, 1536), (513, 200, 144)]
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tokens,m,n", SIZES)
+def test_linear(fmt, dtype, quantize, tokens, m, n):
+    g = np.random.default_rng(tokens * 1000003 + m * 1009 + n)
+    weight, w = make_weight(g, (m, n), fmt)
+    x = to_cuda(g.standard_normal((tokens, n)), DT[dtype])
+    y = ops.mx4_linear(x, weight, quantize_input=quantize)
+    assert y.shape == (tokens, m) and y.dtype == DT[dtype]
+    xv = host(x)
+    check_product(y, quantized_values(xv, fmt) if quantize else xv, w, DT[dtype])
+    assert torch.equal(y, ops.mx4_linear(x, weight, quantize_input=quantize))      # no result depends on timing
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("tokens", [1, 20, 150])
+@pytest.mark.parametrize("out", ["bf16", "fp16", "fp32"])
+def test_linear_output_types_and_residual(fmt, quantize, tokens, out):
+    g = np.random.default_rng(tokens)
+    weight, w = make_weight(g, (272, 416), fmt)
+    x = to_cuda(g.standard_normal((2, tokens, 416)), torch.bfloat16)
+    xv = host(x).reshape(-1, 416)
+    xq = quantized_values(xv, fmt) if quantize else xv
+    y = ops.mx4_linear(x, weight, quantize_input=quantize, out_dtype=DT[out])
+    assert y.shape == (2, tokens, 272) and y.dtype == DT[out]
+    check_product(y.reshape(-1, 272), xq, w, DT[out])
+    add = to_cuda(g.standard_normal((2, tokens, 272)), DT[out])
+    before = host(add).reshape(-1, 272)
+    r = ops.mx4_linear(x, weight, quantize_input=quantize, accumulate_into=add)
+    assert r is add
+    check_product(add.reshape(-1, 272), xq, w, DT[out], add=before)
+
+
+@pytest.mark.parametrize("tokens", [2, 40, 200])
+@pytest.mark.parametrize("quantize", [False, True])
+def test_linear_strided_and_unaligned_rows(tokens, quantize):
+    g = np.random.default_rng(tokens)
+    weight, w = make_weight(g, (160, 328), "mxfp4")
+    base = to_cuda(g.standard_normal((tokens, 700)), torch.bfloat16)
+    for x in (base[:, :328], base[:, 8:336], base[:, 3:331], base[:, 1:657:2], base.t()[:328].t(), base[:1, :328].expand(tokens, 328)):
+        xv = host(x)
+        check_product(ops.mx4_linear(x, weight, quantize_input=quantize), quantized_values(xv, "mxfp4") if quantize else xv, w, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("tokens", [3, 140])
+def test_quantized_input_with_given_scale(dtype, tokens):
+    g = np.random.default_rng(tokens)
+    weight, w = make_weight(g, (144, 272), "nvfp4")
+    x = to_cuda(g.standard_normal((tokens, 272)), DT[dtype])
+    t = torch.tensor([0.0021], device="cuda")
+    y = ops.mx4_linear(x, weight, quantize_input=True, input_scale=t)
+    check_product(y, quantized_values(host(x), "nvfp4", t.item()), w, DT[dtype])
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("tokens", [1, 24, 160])
+def test_mxfp4_scales_over_the_whole_range(quantize, tokens):
+    """Rows whose blocks have any exponent: 2^20 within a row, rows from 2^-127 to 2^100, a row of zeros, blocks that are NaN."""
+    g = np.random.default_rng(3)
+    m, n = 136, 512
+    code = g.integers(0, 16, (m, n), dtype=np.uint8)
+    base = np.linspace(0, 220, m).astype(int)[:, None]
+    byte = np.clip(base + g.integers(0, 21, (m, n // 32)), 0, 254).astype(np.uint8)
+    code[7] = 0
+    byte[9, 3] = byte[m - 1, 15] = 255
+    weight = ops.mx4_pack(ops.Mx4Tensor(to_cuda(O.pack_nibbles(code), torch.uint8), to_cuda(byte, torch.uint8), "mxfp4", n))
+    w = O.values(code, byte, "mxfp4")
+    for dtype in (torch.bfloat16, torch.float16):
+        x = to_cuda(g.standard_normal((tokens, n)) * 2.0 ** -3, dtype)
+        xv = quantized_values(host(x), "mxfp4") if quantize else host(x)
+        y = ops.mx4_linear(x, weight, quantize_input=quantize, out_dtype=torch.float32)
+        got = host(y)
+        nan = np.zeros(m, bool)
+        nan[[9, m - 1]] = True
+        assert np.isnan(got[:, nan]).all() and np.isfinite(got[:, ~nan]).all()
+        # (sums of the smallest rows are subnormal in fp32: each addition may lose half of 2^-149; half of them are cut off)
+        wz = np.where(nan[:, None], 0.0, w)
+        want = xv @ wz.T
+        tol = tolerance(xv, wz, want, torch.float32) + n * 2.0 ** -149
+        # products below 2^-126 may be taken as zero by the matrix instructions
+        tol = tol + n * 2.0 ** -126 * (np.abs(w).max(1, initial=0.0, where=~np.isnan(w)) < 2.0 ** -100)
+        assert np.all(np.abs(got - want)[:, ~nan] <= tol[:, ~nan])
+
+
+# ---- grouped by expert ------------------------------------------------------------------------------------------
+def counts_to_offsets(counts, first=0, dtype=torch.int32):
+    return torch.tensor(np.concatenate([[first], first + np.cumsum(counts)]), dtype=dtype, device="cuda")
+
+
+COUNTS = {
+    "one_each": [1] * 7,
+    "some_empty": [0, 3, 0, 0, 17, 1, 0],
+    "one_takes_all": [0, 0, 70, 0],
+    "none": [0, 0, 0],
+    "ragged": [5, 130, 16, 64, 1, 33, 193, 2],
+    "one_expert": [50],
+    "many": [1, 0, 2, 0, 3] * 30,
+    "large": [300, 0, 129, 260],
+}
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("name", list(COUNTS))
+def test_grouped(fmt, quantize, name):
+    counts = COUNTS[name]
+    g = np.random.default_rng(len(counts))
+    m, n = (200, 352) if len(counts) < 20 else (130, 96)
+    dtype = torch.bfloat16 if fmt == "mxfp4" else torch.float16
+    weight, w = make_weight(g, (len(counts), m, n), fmt)
+    first, behind = 3, 5
+    rows = sum(counts) + first + behind
+    xh = g.standard_normal((rows, n))
+    xh[:first] = np.nan                                          # rows of no expert are not read into anything
+    xh[rows - behind:] = 1e4
+    x = to_cuda(xh, dtype)
+    off = counts_to_offsets(counts, first, torch.int64 if len(counts) % 2 else torch.int32)
+    y = ops.mx4_grouped_linear(x, weight, off, quantize_input=quantize)
+    at = off.tolist()
+    assert not y[:first].any() and not y[at[-1]:].any()
+    xv = host(x)[first:at[-1]]
+    if quantize and len(xv):
+        xv = quantized_values(xv, fmt)
+    for e in range(len(counts)):
+        if counts[e]:
+            check_product(y[at[e]:at[e + 1]], xv[at[e] - first:at[e + 1] - first], w[e], dtype)
+    # a given result keeps the rows of no expert, also with rows that lie apart
+    out = torch.full((rows, m + 9), 7.0, dtype=dtype, device="cuda")
+    r = ops.mx4_grouped_linear(x, weight, off, quantize_input=quantize, out=out[:, 4:4 + m])
+    assert r.data_ptr() == out[:, 4:].data_ptr()
+    assert torch.equal(out[first:at[-1], 4:4 + m], y[first:at[-1]])
+    out[first:at[-1], 4:4 + m] = 7.0
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+def test_grouped_offsets_that_make_no_sense_stay_in_bounds(quantize):
+    g = np.random.default_rng(2)
+    weight, w = make_weight(g, (4, 144, 160), "mxfp4")
+    x = to_cuda(g.standard_normal((60, 160)), torch.bfloat16)
+    xv = quantized_values(host(x), "mxfp4") if quantize else host(x)
+    for off in ([-5, 10, 10, 30, 1000], [0, 40, 20, 60, 60], [100, 200, 300, 400, 500], [-9, -8, -7, -6, -5], [0, 2 ** 40, 2 ** 41, 5, 60]):
+        y = ops.mx4_grouped_linear(x, weight, torch.tensor(off, dtype=torch.int64, device="cuda"), quantize_input=quantize)
+        seen = np.zeros(60, bool)
+        for e in range(4):
+            b, f = (min(max(v, 0), 60) for v in off[e:e + 2])
+            alone = [k for k in range(b, f) if sum(min(max(off[i], 0), 60) <= k < min(max(off[i + 1], 0), 60) for i in range(4)) == 1]
+            if alone:
+                check_product(y[alone], xv[alone], w[e], torch.bfloat16)
+            seen[b:max(b, f)] = True
+        assert not host(y)[~seen].any()
+
+
+def test_grouped_matches_linear_per_expert():
+    g = np.random.default_rng(8)
+    counts = [40, 0, 25, 90]
+    weight, w = make_weight(g, (4, 256, 512), "nvfp4")
+    x = to_cuda(g.standard_normal((sum(counts), 512)), torch.bfloat16)
+    off = counts_to_offsets(counts)
+    y = ops.mx4_grouped_linear(x, weight, off, out_dtype=torch.float32)
+    at = off.tolist()
+    for e in range(4):
+        if counts[e]:
+            check_product(y[at[e]:at[e + 1]], host(x)[at[e]:at[e + 1]], w[e], torch.float32)
+
+
+# ---- streams, graphs, together ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("tokens", [1, 30, 140])
+def test_captured_and_replayed_with_new_inputs(quantize, tokens):
+    g = np.random.default_rng(4)
+    weight, w = make_weight(g, (256, 384), "nvfp4")
+    experts, we = make_weight(g, (3, 256, 384), "nvfp4")
+    x = to_cuda(g.standard_normal((tokens, 384)), torch.bfloat16)
+    off = torch.zeros(4, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        for _ in range(2):                                       # two graphs of the same calls, replayed at once below
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                y = ops.mx4_linear(x, weight, quantize_input=quantize)
+                z = ops.mx4_grouped_linear(x, experts, off, quantize_input=quantize)
+                v = ops.mx4_dequantize(ops.mx4_quantize(x, "nvfp4"), torch.float32)
+            graphs.append((graph, y, z, v))
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(3):
+        x.copy_(to_cuda(g.standard_normal((tokens, 384)) * (k + 1), torch.bfloat16))
+        cut = sorted(g.integers(0, tokens + 1, 2).tolist())
+        off.copy_(torch.tensor([0] + cut + [tokens], dtype=torch.int32))
+        torch.cuda.synchronize()
+        other = torch.cuda.Stream()
+        graphs[0][0].replay()
+        with torch.cuda.stream(other):
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        xv = host(x)
+        xq = quantized_values(xv, "nvfp4")
+        for _, y, z, v in graphs:
+            check_product(y, xq if quantize else xv, w, torch.bfloat16)
+            at = [0] + cut + [tokens]
+            for e in range(3):
+                if at[e] < at[e + 1]:
+                    check_product(z[at[e]:at[e + 1]], (xq if quantize else xv)[at[e]:at[e + 1]], we[e], torch.bfloat16)
+            assert np.allclose(host(v), xq, rtol=2.0 ** -23, atol=0)
+    ops.check_device_status()
+
+
+def test_calls_on_several_streams_at_once():
+    g = np.random.default_rng(6)
+    weight, w = make_weight(g, (512, 1024), "mxfp4")
+    xs = [to_cuda(g.standard_normal((t, 1024)), torch.bfloat16) for t in (1, 7, 48, 130, 300)]
+    torch.cuda.synchronize()
+    for quantize in (False, True):
+        alone = [ops.mx4_linear(x, weight, quantize_input=quantize) for x in xs]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in xs]
+        got = [[] for _ in xs]
+        for _ in range(10):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(ops.mx4_linear(xs[i], weight, quantize_input=quantize))
+        torch.cuda.synchronize()
+        for i in range(len(xs)):
+            assert all(torch.equal(y, alone[i]) for y in got[i])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_experts_layer_of_a_decoder(fmt):
+    """The operators as they are used together: a dense block with residual, then routed experts over sorted rows."""
+    g = np.random.default_rng(9)
+    hidden, inter, experts, tokens, top = 256, 192, 6, 50, 2
+    up, wu = make_weight(g, (2 * inter, hidden), fmt, spread=0.2)
+    down, wd = make_weight(g, (hidden, inter), fmt, spread=0.2)
+    w13, v13 = make_weight(g, (experts, 2 * inter, hidden), fmt, spread=0.2)
+    w2, v2 = make_weight(g, (experts, hidden, inter), fmt, spread=0.2)
+    x = to_cuda(g.standard_normal((tokens, hidden)), torch.bfloat16)
+
+    def act(h):
+        return torch.nn.functional.silu(h[:, :inter]) * h[:, inter:]
+
+    res = x.clone()
+    h = ops.mx4_linear(x, up, out_dtype=torch.float32)
+    check_product(h, host(x), wu, torch.float32)
+    a = act(h).to(torch.bfloat16)
+    before = host(res)
+    ops.mx4_linear(a, down, accumulate_into=res)
+    check_product(res, host(a), wd, torch.bfloat16, add=before)
+    ids = torch.from_numpy(np.stack([g.permutation(experts)[:top] for _ in range(tokens)])).cuda()
+    weights = torch.rand(tokens, top, device="cuda")
+    order = torch.argsort(ids.flatten(), stable=True)
+    token = order // top
+    off = torch.cat((ids.new_zeros(1), torch.bincount(ids.flatten(), minlength=experts).cumsum(0))).to(torch.int32)
+    rows = res[token]
+    h = ops.mx4_grouped_linear(rows, w13, off, out_dtype=torch.float32)
+    a = act(h).to(torch.bfloat16)
+    y = ops.mx4_grouped_linear(a, w2, off, out_dtype=torch.float32)
+    out = torch.zeros(tokens, hidden, device="cuda").index_add_(0, token, y * weights.flatten()[order, None])
+    want = np.zeros((tokens, hidden))
+    at = off.tolist()
+    for e in range(experts):
+        r = slice(at[e], at[e + 1])
+        check_product(h[r], host(rows)[r], v13[e], torch.float32)
+        part = host(a)[r] @ v2[e].T
+        check_product(y[r], host(a)[r], v2[e], torch.float32)
+        np.add.at(want, token[r].cpu().numpy(), part * host(weights.flatten()[order][r])[:, None])
+    assert np.allclose(host(out), want, rtol=1e-4, atol=1e-4 * np.abs(want).max())
+    ops.check_device_status()
+
+
+# ---- refusals ----------------------------------------------------------------------------------------------------
+def test_refusals():
+    g = np.random.default_rng(0)
+    weight, _ = make_weight(g, (64, 96), "mxfp4")
+    nv, _ = make_weight(g, (64, 96), "nvfp4")
+    experts, _ = make_weight(g, (2, 64, 96), "mxfp4")
+    x = torch.zeros(4, 96, dtype=torch.bfloat16, device="cuda")
+    off = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    one = torch.ones(1, device="cuda")
+
+    def refuse(match, call, kind=(ValueError, RuntimeError)):
+        with pytest.raises(kind, match=match):
+            call()
+
+    refuse("inputs", lambda: ops.mx4_linear(x[:, :64], weight))
+    refuse("fp32", lambda: ops.mx4_linear(x.float(), weight))
+    refuse("not torch.int32", lambda: ops.mx4_linear(x.int(), weight))
+    refuse("one per expert", lambda: ops.mx4_linear(x, experts))
+    refuse("one matrix per expert", lambda: ops.mx4_grouped_linear(x, weight, off))
+    refuse("3 int32 or int64", lambda: ops.mx4_grouped_linear(x, experts, off[:2]))
+    refuse("3 int32 or int64", lambda: ops.mx4_grouped_linear(x, experts, off.float()))
+    refuse("CUDA tensor", lambda: ops.mx4_grouped_linear(x, experts, off.cpu()))
+    refuse("CUDA tensor", lambda: ops.mx4_linear(x.cpu(), weight))
+    refuse("rows, n", lambda: ops.mx4_grouped_linear(x[None], experts, off))
+    refuse("out must be", lambda: ops.mx4_grouped_linear(x, experts, off, out=torch.zeros(4, 63, device="cuda")))
+    refuse("out overlaps", lambda: ops.mx4_grouped_linear(x, experts, off, out=x[:, :64]))
+    refuse("input_scale", lambda: ops.mx4_linear(x, weight, quantize_input=True, input_scale=one))
+    refuse("input_scale", lambda: ops.mx4_linear(x, nv, input_scale=one))
+    refuse("1 fp32 value", lambda: ops.mx4_linear(x, nv, quantize_input=True, input_scale=one.double()))
+    refuse("dense", lambda: ops.mx4_linear(x, weight, accumulate_into=torch.zeros(4, 70, device="cuda")[:, :64]))
+    refuse("out_dtype", lambda: ops.mx4_linear(x, weight, accumulate_into=torch.zeros(4, 64, device="cuda"), out_dtype=torch.bfloat16))
+    square, _ = make_weight(g, (96, 96), "mxfp4")
+    refuse("overlaps x", lambda: ops.mx4_linear(x, square, accumulate_into=x))
+    refuse("tensor_scale", lambda: ops.mx4_quantize(x, "mxfp4", one))
+    refuse("not torch.float64", lambda: ops.mx4_quantize(x.double()))
+    q = ops.mx4_quantize(x)
+    refuse("are not mxfp4 rows", lambda: ops.mx4_pack(q._replace(cols=64)))
+    refuse("needs its tensor_scale", lambda: ops.mx4_pack(ops.mx4_quantize(x, "nvfp4")._replace(tensor_scale=None)))
+    refuse("tensor scales", lambda: ops.mx4_pack(ops.mx4_quantize(x, "nvfp4")._replace(tensor_scale=torch.ones(3, device="cuda"))))
+    refuse("uint8", lambda: ops.mx4_dequantize(q._replace(codes=q.codes.int())))
+    refuse("empty", lambda: ops.mx4_pack(ops.mx4_quantize(x[:0])))
+    assert ops.mx4_linear(x[:0], weight).shape == (0, 64)
+    assert ops.mx4_grouped_linear(x[:0], experts, off * 0).shape == (0, 64)

@@ -1,0 +1,113 @@
+"""Microscaled 4-bit floating point without a GPU: the oracle against itself, the ABI's structure, the refusals."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import mx4_oracle as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_oracle_rounds_to_the_nearest_value_and_to_even_codes():
+    x = np.array([[0.0, 0.25, 0.26, 0.74, 0.75, 1.25, 1.75, 2.5, 2.6, 3.5, 5.0, 5.01, 6.0, -0.25, -5.0, 4.0]])
+    code, byte = O.quantize(x, "nvfp4", 1.0)
+    assert byte.tolist() == [[56]]                              # 6 / 6 = 1.0 in e4m3
+    assert O.MAGNITUDES[code & 7].tolist() == [[0, 0, 0.5, 0.5, 1, 1, 2, 2, 3, 4, 4, 6, 6, 0, 4, 4]]
+    code, byte = O.quantize(np.array([[7.9, 4.0, -0.5] + [0.0] * 29]), "mxfp4")
+    assert byte.tolist() == [[127]] and O.values(code, byte, "mxfp4")[0, :3].tolist() == [6.0, 4.0, -0.5]
+    assert O.quantize(np.zeros((1, 32)), "mxfp4")[1].tolist() == [[0]]
+    assert O.quantize(np.full((1, 32), np.inf), "mxfp4")[1].tolist() == [[255]]
+
+
+def test_oracle_nibbles_round_trip():
+    code = np.random.default_rng(0).integers(0, 16, (3, 7), dtype=np.uint8)
+    assert np.array_equal(O.unpack_nibbles(O.pack_nibbles(code), 7), code)
+
+
+def test_e4m3_table_is_torchs():
+    assert np.array_equal(torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy(), O.E4M3)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from glq_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def test_struct_layout_matches_header(tmp_path):
+    from glq_b200 import _lib
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include "glq_b200.h"\nint main(){printf("%zu %zu %zu %zu\\n", sizeof(GlqbMx4Weight),'
+                   '__builtin_offsetof(GlqbMx4Weight, tensor_scale), __builtin_offsetof(GlqbMx4Weight, format), __builtin_offsetof(GlqbMx4Weight, n));}')
+    exe = tmp_path / "s"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    out = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    D = _lib.Mx4WeightDesc
+    assert out == [ctypes.sizeof(D), D.tensor_scale.offset, D.format.offset, D.n.offset]
+
+
+def test_image_sizes(lib):
+    # tiles of 128 x 256: 16 KiB of codes and 1 (blocks of 32) or 2 KiB (of 16) of scales, MXFP4 a byte per row behind them
+    assert lib.glqb_mx4_image_bytes(0, 1, 128, 256) == 16384 + 1024 + 128
+    assert lib.glqb_mx4_image_bytes(1, 1, 128, 256) == 16384 + 2048
+    assert lib.glqb_mx4_image_bytes(1, 5, 129, 257) == 5 * 4 * (16384 + 2048)
+    assert lib.glqb_mx4_image_bytes(2, 1, 128, 256) == 0 and lib.glqb_mx4_image_bytes(0, 0, 128, 256) == 0
+
+
+def test_c_entries_refuse_before_any_cuda_call(lib):
+    from glq_b200 import _lib
+    p = 4096                                                    # never dereferenced: each call is refused
+
+    def refused(rc, code, text):
+        assert rc == code and text in lib.glqb_last_error().decode(), (rc, lib.glqb_last_error())
+
+    refused(lib.glqb_mx4_quantize(p, 0, 32, 1, 32, 2, None, None, p, p, None), -1, "format")
+    refused(lib.glqb_mx4_quantize(p, 3, 32, 1, 32, 0, None, None, p, p, None), -1, "dtype")
+    refused(lib.glqb_mx4_quantize(p, 0, 32, -1, 32, 0, None, None, p, p, None), -1, "-1 x 32")
+    refused(lib.glqb_mx4_quantize(p, 0, 31, 2, 32, 0, None, None, p, p, None), -1, "apart")
+    refused(lib.glqb_mx4_quantize(p, 0, 32, 1, 32, 1, None, None, p, p, None), -1, "tensor_scale")
+    refused(lib.glqb_mx4_quantize(None, 0, 32, 1, 32, 0, None, None, p, p, None), -1, "null")
+    assert lib.glqb_mx4_quantize(None, 0, 32, 0, 32, 0, None, None, None, None, None) == 0
+    refused(lib.glqb_mx4_dequantize(p, p, None, 1, 1, 32, 1, p, 0, None), -1, "tensor_scale")
+    refused(lib.glqb_mx4_dequantize(p, p, None, 1, 1, 32, 0, p, 7, None), -1, "dtype")
+    refused(lib.glqb_mx4_pack(p, p, 0, 1, 0, 32, p, None), -1, "1 x 0 x 32")
+    refused(lib.glqb_mx4_pack(p, p, 0, 1, 32, 32, p + 64, None), -1, "aligned")
+    refused(lib.glqb_mx4_pack(p, p, 0, 65536, 65536, 65536, p, None), -1, "tiles")
+
+    def product(w, x=p, xd=1, xs=64, rows=2, offsets=None, q=0, y=p, yd=1, ys=64, ws=None, size=0, xscale=None):
+        return lib.glqb_mx4_product(ctypes.byref(w), x, xd, xs, rows, offsets, 0, q, xscale, y, yd, ys, 0, 0, ws, size, None)
+
+    w = _lib.Mx4WeightDesc(p, None, 0, 1, 64, 64)
+    refused(product(_lib.Mx4WeightDesc(p, None, 5, 1, 64, 64)), -1, "format")
+    refused(product(_lib.Mx4WeightDesc(p, None, 0, 2, 64, 64)), -1, "offsets")
+    refused(product(_lib.Mx4WeightDesc(p, None, 1, 1, 64, 64)), -1, "null")
+    refused(product(w, xd=2), -1, "fp32")
+    refused(product(w, yd=4), -1, "dtype")
+    refused(product(w, rows=1 << 31), -1, "rows")
+    refused(product(w, xs=63), -1, "overlap")
+    refused(product(w, ys=63), -1, "overlap")
+    refused(product(w, y=None), -1, "null")
+    refused(product(w, q=1), -3, "workspace")
+    assert product(w, rows=0) == 0
+
+
+def test_operators_refuse_host_tensors_and_wrong_arguments():
+    from glq_b200 import ops
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.mx4_quantize(x)
+    with pytest.raises(ValueError, match="mxfp4"):
+        ops.mx4_quantize(x, "fp4")
+    q = ops.Mx4Tensor(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), "mxfp4", 64)
+    for call in (ops.mx4_dequantize, ops.mx4_pack):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call(q)
+    with pytest.raises(ValueError, match="mx4_pack"):
+        ops.mx4_linear(x, q)
+    with pytest.raises(ValueError, match="mx4_pack"):
+        ops.mx4_grouped_linear(x, q, torch.zeros(3, dtype=torch.int32))
