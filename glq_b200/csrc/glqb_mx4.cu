@@ -1,6 +1,7 @@
 // Microscaled 4-bit floating point: quantisation and back, the weight image, and the C entry points (include/glq_b200.h).
-#include "glqb_mx4.cuh"
+#include "glqb_mx4_gemm.cuh"
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -23,6 +24,8 @@ int mx4_launched(const char* what) {
 
 constexpr int QT_THREADS = 256;
 
+__device__ int g_mx4_status;   // 0, or what gave up (ST_GAVE_UP_*): products have no plan to keep it in
+
 // Rows and columns of a call.  Rows that follow one another without a gap and end on whole blocks are one long row: their
 // codes and scales do too.
 struct Mx4Rows {
@@ -32,7 +35,7 @@ struct Mx4Rows {
   bool vec;
 };
 
-// The rows that belong to an expert: offsets[0] .. offsets[experts] - 1, held to those there are.
+// Rows offsets[0] .. offsets[experts] - 1, held to those there are.
 struct Mx4Range {
   const void* offsets;        // null: all
   int wide, experts;
@@ -202,74 +205,71 @@ __global__ void __launch_bounds__(256) mx4_row_top_kernel(const uint8_t* __restr
   if (threadIdx.x % 32 == 0) tops[row] = (uint8_t)top;
 }
 
-// ---- the product, plainly: a warp sums eight rows of x against one row of the matrix in fp32 -------
-template <int FMT, typename T>
-__global__ void __launch_bounds__(256)
-mx4_plain_kernel(const uint8_t* __restrict__ image, const float* __restrict__ tensor_scale, int m, int n, int k_tiles, int m_tiles,
-                 const T* __restrict__ x, long long x_stride, long long rows, const void* offsets, int wide, const float* x_scale,
-                 uint8_t* y, int y_dtype, long long y_stride, int accumulate) {
-  constexpr int BLOCK = Mx4Fmt<FMT>::BLOCK;
-  const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32, e = blockIdx.z;
-  if (row >= m) return;
-  long long begin = 0, end = rows;
-  if (offsets) {
-    begin = wide ? reinterpret_cast<const long long*>(offsets)[e] : reinterpret_cast<const int*>(offsets)[e];
-    end = wide ? reinterpret_cast<const long long*>(offsets)[e + 1] : reinterpret_cast<const int*>(offsets)[e + 1];
-    begin = max(0ll, min(rows, begin));
-    end = max(0ll, min(rows, end));
+// ---- activations of the products ------------------------------------------------------------------
+// Rows that TMA cannot read (not on 16 bytes) are copied, to rows of a multiple of eight values.
+__global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* __restrict__ x, long long x_stride, long long rows, int n, int n_pad,
+                                                        uint16_t* __restrict__ out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * n_pad; i += (long long)gridDim.x * 256) {
+    const long long r = i / n_pad;
+    const int c = (int)(i - r * n_pad);
+    out[i] = c < n ? x[r * x_stride + c] : (uint16_t)0;
   }
-  const uint8_t* tiles = image + ((long long)e * m_tiles + row / MX4_ROWS) * k_tiles * mx4_tile_bytes(FMT);
-  const int r = row % MX4_ROWS;
-  float scale = 1.0f;
-  if constexpr (FMT == GLQB_MX4_NVFP4) scale = tensor_scale[e] * (x_scale ? *x_scale : 1.0f);
-  for (long long t0 = begin + blockIdx.y * 8ll; t0 < end; t0 += gridDim.y * 8ll) {
-    float acc[8] = {};
-    for (int k = lane * 8; k < n; k += 256) {
-      const uint8_t* tile = tiles + (long long)(k / MX4_K) * mx4_tile_bytes(FMT);
-      const int kk = k % MX4_K;
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + mx4_word_offset(r, kk));
-      const float s = mx4_scale_value<FMT>(tile[MX4_CODE_BYTES + mx4_scale_offset(r, kk / BLOCK)]);
-      for (int j = 0; j < 8 && k + j < n; ++j) {
-        const float v = mx4_value(w >> (4 * ((j >> 1) + 4 * (j & 1))) & 15u) * s;
-        for (int t = 0; t < 8; ++t)
-          if (t0 + t < end) acc[t] += v * (float)x[(t0 + t) * x_stride + k + j];
-      }
-    }
-    for (int t = 0; t < 8; ++t) {
-      float a = acc[t];
-      for (int d = 16; d; d >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, d);
-      if (lane || t0 + t >= end) continue;
-      a *= scale;
-      const long long at = (t0 + t) * y_stride + row;
-      if (y_dtype == GLQB_DT_F32) {
-        float* o = reinterpret_cast<float*>(y) + at;
-        *o = accumulate ? *o + a : a;
-      } else if (y_dtype == GLQB_DT_F16) {
-        __half* o = reinterpret_cast<__half*>(y) + at;
-        *o = __float2half_rn(accumulate ? __half2float(*o) + a : a);
-      } else {
-        __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(y) + at;
-        *o = __float2bfloat16_rn(accumulate ? __bfloat162float(*o) + a : a);
-      }
+}
+
+// Rows of x in 4 bits, as the tiles the 4-bit product fetches (per token tile, per 256 values: tn rows of 128 bytes with the
+// 128-byte swizzle, then the scales, 128 rows at a time as in the weight image).  A warp takes a row, 256 values at a time;
+// values past the row are zeros, rows past a tile's are left out (their columns are not stored).
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, const float* amax, float* own_scale,
+                                                          int x_scales, bool vec) {
+  extern __shared__ int lists[];
+  int* eff = lists;
+  int* pre = lists + J.experts + 1;
+  mx4_groups(J, eff, pre);
+  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
+  float t = 1.0f;
+  if constexpr (FMT == GLQB_MX4_NVFP4) {
+    t = x_scale ? *x_scale : mx4_tensor_scale(*amax);
+    if (!x_scale && blockIdx.x == 0 && threadIdx.x == 0) *own_scale = t;
+  }
+  const int lane = threadIdx.x & 31, end = eff[J.experts];
+  const long long stage = (long long)J.tn * 128 + x_scales;
+  for (int row = eff[0] + blockIdx.x * 8 + (threadIdx.x >> 5); row < end; row += gridDim.x * 8) {
+    const int e = J.experts == 1 ? 0 : mx4_find(eff, J.experts, row), in = row - eff[e];
+    const int per = mx4_per_tile(eff[e + 1] - eff[e], pre[e + 1] - pre[e]), tile = pre[e] + in / per, r = in % per;
+    if (tile >= J.max_tiles) continue;
+    uint8_t* at = J.x_image + (long long)tile * J.k_tiles * stage;
+    uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+    uint8_t* scales = at + J.tn * 128 + (r >> 7) * mx4_scale_bytes(FMT) + mx4_scale_offset(r & 127, lane / PER);
+    const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
+    for (int k = 0; k < J.k_tiles; ++k, codes += stage, scales += stage) {
+      float v[8];
+      mx4_load8(src, k * MX4_K + lane * 8, J.n, vec, v);
+      uint32_t s;
+      *reinterpret_cast<uint32_t*>(codes) = mx4_quantize8<FMT, true>(v, t, s);
+      if (lane % PER == 0) *scales = (uint8_t)s;
     }
   }
 }
 
-// rows of no expert
-__global__ void __launch_bounds__(256) mx4_clear_kernel(const void* offsets, int wide, int experts, long long rows, int m, uint8_t* y, int size,
-                                                        long long y_stride) {
-  const long long row = blockIdx.x;
-  __shared__ int owned;
-  if (threadIdx.x == 0) owned = 0;
-  __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-    const long long b = wide ? reinterpret_cast<const long long*>(offsets)[e] : reinterpret_cast<const int*>(offsets)[e];
-    const long long f = wide ? reinterpret_cast<const long long*>(offsets)[e + 1] : reinterpret_cast<const int*>(offsets)[e + 1];
-    if (row >= b && row < f) owned = 1;
+// Rows of no expert are zeroed.  (Offsets as mx4_groups takes them: the experts' rows are one range.)
+__global__ void __launch_bounds__(256) mx4_clear_kernel(const __grid_constant__ Mx4Job J) {
+  extern __shared__ int lists[];
+  int* eff = lists;
+  mx4_groups(J, eff, lists + J.experts + 1);
+  const int first = eff[0], last = eff[J.experts], size = J.y_dtype == GLQB_DT_F32 ? 4 : 2;
+  for (int row = blockIdx.x; row < J.rows; row += gridDim.x) {
+    if (row >= first && row < last) {
+      // (to the next row of this CTA behind the experts')
+      row += (last - row - 1) / (int)gridDim.x * (int)gridDim.x;
+      continue;
+    }
+    uint8_t* p = reinterpret_cast<uint8_t*>(J.y) + row * J.y_stride * size;
+    for (int i = threadIdx.x; i < J.m; i += 256) {
+      if (size == 4) reinterpret_cast<uint32_t*>(p)[i] = 0u;
+      else reinterpret_cast<uint16_t*>(p)[i] = 0;
+    }
   }
-  __syncthreads();
-  if (owned) return;
-  for (int i = threadIdx.x; i < m * size; i += blockDim.x) y[row * y_stride * size + i] = 0;
 }
 
 Mx4Rows rows_of(long long rows, int cols, long long stride, int format, const void* base, int elem) {
@@ -288,18 +288,24 @@ bool one_row(long long rows, int cols, long long stride, int format) {
 }
 int grid_for(long long total) { return (int)std::min<long long>((total + QT_THREADS - 1) / QT_THREADS, 148 * 64); }
 
+// the largest finite |x| of the range's rows
+int amax_launch(const void* x, int x_dtype, const Mx4Rows& q, const Mx4Range& range, float* amax, cudaStream_t stream) {
+  const cudaError_t e = cudaMemsetAsync(amax, 0, 4, stream);
+  if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4 amax: %s", cudaGetErrorString(e));
+  const long long n = q.rows * ((q.cols + 7) / 8);
+  const int grid = (int)std::min<long long>((n + QT_THREADS - 1) / QT_THREADS, 148 * 8);
+  if (x_dtype == GLQB_DT_F16) mx4_amax_kernel<__half><<<grid, QT_THREADS, 0, stream>>>((const __half*)x, q, range, amax);
+  else if (x_dtype == GLQB_DT_BF16) mx4_amax_kernel<__nv_bfloat16><<<grid, QT_THREADS, 0, stream>>>((const __nv_bfloat16*)x, q, range, amax);
+  else mx4_amax_kernel<float><<<grid, QT_THREADS, 0, stream>>>((const float*)x, q, range, amax);
+  return GLQB_OK;
+}
 template <int FMT>
-int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const Mx4Range& range, const float* tensor_scale, float* own_scale, uint8_t* codes,
-                    uint8_t* scales, cudaStream_t stream) {
+int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const float* tensor_scale, float* own_scale, uint8_t* codes, uint8_t* scales,
+                    cudaStream_t stream) {
   const long long total = q.rows * q.chunks;
   if (FMT == GLQB_MX4_NVFP4 && !tensor_scale) {
-    const cudaError_t e = cudaMemsetAsync(own_scale + 1, 0, 4, stream);
-    if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4_quantize: %s", cudaGetErrorString(e));
-    const long long n = q.rows * ((q.cols + 7) / 8);
-    const int grid = (int)std::min<long long>((n + QT_THREADS - 1) / QT_THREADS, 148 * 8);
-    if (x_dtype == GLQB_DT_F16) mx4_amax_kernel<__half><<<grid, QT_THREADS, 0, stream>>>((const __half*)x, q, range, own_scale + 1);
-    else if (x_dtype == GLQB_DT_BF16) mx4_amax_kernel<__nv_bfloat16><<<grid, QT_THREADS, 0, stream>>>((const __nv_bfloat16*)x, q, range, own_scale + 1);
-    else mx4_amax_kernel<float><<<grid, QT_THREADS, 0, stream>>>((const float*)x, q, range, own_scale + 1);
+    const int rc = amax_launch(x, x_dtype, q, Mx4Range{nullptr, 0, 0}, own_scale + 1, stream);
+    if (rc) return rc;
   }
   const int grid = grid_for(total);
   if (x_dtype == GLQB_DT_F16)
@@ -322,8 +328,8 @@ using namespace glqb;
 
 extern "C" {
 
-static int quantize_rows(const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows, int32_t cols, int32_t format, const Mx4Range& range,
-                         const float* tensor_scale, float* own_scale, void* codes, void* scales, void* stream_) {
+int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows, int32_t cols, int32_t format,
+                      const float* tensor_scale, float* own_scale, void* codes, void* scales, void* stream_) {
   if (!format_ok(format)) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: format %d", format);
   if (!dtype_ok(x_dtype)) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: dtype %d", x_dtype);
   if (rows < 0 || cols < 0) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: %lld x %d", (long long)rows, cols);
@@ -332,16 +338,11 @@ static int quantize_rows(const void* x, int32_t x_dtype, int64_t x_stride, int64
   if (!x || !codes || !scales) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: null argument");
   if (x_stride < cols && rows > 1) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: rows of %d values %lld apart", cols, (long long)x_stride);
   Mx4Rows q = rows_of(rows, cols, x_stride, format, x, size_of(x_dtype));
-  if (!range.offsets && one_row(rows, cols, x_stride, format)) { q.cols = rows * cols; q.chunks = (int)(q.cols / 8); q.rows = 1; q.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0; }
+  if (one_row(rows, cols, x_stride, format)) { q.cols = rows * cols; q.chunks = (int)(q.cols / 8); q.rows = 1; q.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0; }
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
-    return quantize_launch<GLQB_MX4_MXFP4>(x, x_dtype, q, range, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
-  return quantize_launch<GLQB_MX4_NVFP4>(x, x_dtype, q, range, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
-}
-
-int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows, int32_t cols, int32_t format,
-                      const float* tensor_scale, float* own_scale, void* codes, void* scales, void* stream_) {
-  return quantize_rows(x, x_dtype, x_stride, rows, cols, format, Mx4Range{nullptr, 0, 0}, tensor_scale, own_scale, codes, scales, stream_);
+    return quantize_launch<GLQB_MX4_MXFP4>(x, x_dtype, q, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
+  return quantize_launch<GLQB_MX4_NVFP4>(x, x_dtype, q, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
 }
 
 int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tensor_scale, int64_t rows_per_scale, int64_t rows,
@@ -395,20 +396,47 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
   return mx4_launched("mx4_pack");
 }
 
-// quantised activations: codes, scales, the tensor's scale
-static size_t x_bytes(const GlqbMx4Weight* w, int64_t rows, size_t* scales_at, size_t* own_at, size_t* back_at) {
-  const size_t codes = ((size_t)rows * ((w->n + 1) / 2) + 255) / 256 * 256;
-  const size_t scales = ((size_t)rows * ((w->n + mx4_block(w->format) - 1) / mx4_block(w->format)) + 255) / 256 * 256;
-  *scales_at = codes;
-  *own_at = codes + scales;
-  *back_at = codes + scales + 256;
-  return *back_at + (size_t)rows * w->n * 4;
+// What a call launches, by its sizes alone.
+struct Form {
+  int tn, max_tiles, split, x_scales, n_pad;
+  bool align;
+  size_t image, bytes;        // of the workspace: x in 4 bits or aligned, then two floats
+};
+static int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, int sms) {
+  Form f = {};
+  const int most = quantize ? (w->format == GLQB_MX4_MXFP4 ? 192 : 160) : 192, per = (int)((rows + w->experts - 1) / w->experts);
+  // token tiles: a matrix's rows split evenly; of experts up to twice their average, so that most have one tile
+  if (w->experts == 1) f.tn = (int)(((rows + (rows + most - 1) / most - 1) / ((rows + most - 1) / most) + 15) / 16 * 16);
+  else f.tn = std::min(most, (2 * per + 15) / 16 * 16);
+  f.max_tiles = w->experts == 1 ? (int)((rows + f.tn - 1) / f.tn) : (int)(rows / f.tn + std::min<long long>(w->experts, rows));
+  const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K, tiles = f.max_tiles * mt;
+  f.split = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, kt), sms / std::max<long long>(1, tiles)));
+  if (quantize) {
+    f.x_scales = mx4_x_scale_bytes(w->format, f.tn);
+    f.image = (size_t)f.max_tiles * kt * ((size_t)f.tn * 128 + f.x_scales);
+    f.bytes = f.image + 256;
+  } else if (reinterpret_cast<uintptr_t>(x) % 16 || (rows > 1 && x_stride % 8)) {
+    f.align = true;
+    f.n_pad = (w->n + 7) / 8 * 8;
+    f.bytes = (size_t)rows * f.n_pad * 2;
+  }
+  return f;
 }
 
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize) {
-  if (!w || !format_ok(w->format) || rows < 0 || !quantize) return 0;
-  size_t a, b, c;
-  return x_bytes(w, rows, &a, &b, &c);
+  if (!w || !format_ok(w->format) || rows <= 0 || rows >= (1ll << 31) || w->experts < 1 || w->m < 1 || w->n < 1) return 0;
+  return form_of(w, rows, x_stride, x, quantize, sm_count()).bytes;
 }
 
 int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows,
@@ -416,7 +444,8 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
                      void* y, int32_t y_dtype, int64_t y_stride, int32_t accumulate, int32_t clear_rest,
                      void* workspace, size_t workspace_bytes, void* stream_) {
   if (!w || !format_ok(w->format)) return mx4_fail(GLQB_E_INVALID, "mx4_product: format");
-  if (w->experts < 1 || w->m < 1 || w->n < 1) return mx4_fail(GLQB_E_INVALID, "mx4_product: %d x %d x %d", w->experts, w->m, w->n);
+  if (w->experts < 1 || w->experts > MX4_MAX_EXPERTS || w->m < 1 || w->n < 1)
+    return mx4_fail(GLQB_E_INVALID, "mx4_product: %d x %d x %d (at most %d experts)", w->experts, w->m, w->n, MX4_MAX_EXPERTS);
   if (!offsets && w->experts != 1) return mx4_fail(GLQB_E_INVALID, "mx4_product: %d experts need offsets", w->experts);
   if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return mx4_fail(GLQB_E_INVALID, "mx4_product: dtype");
   if (!quantize && x_dtype == GLQB_DT_F32) return mx4_fail(GLQB_E_INVALID, "mx4_product: fp32 activations are served quantised only");
@@ -424,48 +453,81 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   if (rows == 0) return GLQB_OK;
   if (!w->image || !x || !y || (w->format == GLQB_MX4_NVFP4 && !w->tensor_scale)) return mx4_fail(GLQB_E_INVALID, "mx4_product: null argument");
   if (rows > 1 && (x_stride < w->n || y_stride < w->m)) return mx4_fail(GLQB_E_INVALID, "mx4_product: rows overlap");
-  if (workspace_bytes < glqb_mx4_workspace_bytes(w, rows, x_stride, x, quantize) || (quantize && !workspace))
-    return mx4_fail(GLQB_E_WORKSPACE, "mx4_product: workspace of %zu bytes, %zu needed", workspace_bytes, glqb_mx4_workspace_bytes(w, rows, x_stride, x, quantize));
+  const int sms = sm_count();
+  const Form f = form_of(w, rows, x_stride, x, quantize, sms);
+  if (workspace_bytes < f.bytes || (f.bytes && !workspace))
+    return mx4_fail(GLQB_E_WORKSPACE, "mx4_product: workspace of %zu bytes, %zu needed", workspace_bytes, f.bytes);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const int mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K;
-  if (offsets && clear_rest)
-    mx4_clear_kernel<<<(unsigned)rows, 256, 0, stream>>>(offsets, offsets_are_int64, w->experts, rows, w->m, (uint8_t*)y, size_of(y_dtype), y_stride);
-  const float* xs = nullptr;
-  if (quantize) {
-    size_t scales_at, own_at, back_at;
-    x_bytes(w, rows, &scales_at, &own_at, &back_at);
-    uint8_t* ws = (uint8_t*)workspace;
-    float* own = (float*)(ws + own_at);
-    int rc = quantize_rows(x, x_dtype, x_stride, rows, w->n, w->format, Mx4Range{offsets, offsets_are_int64, w->experts}, x_scale, own, ws, ws + scales_at, stream_);
-    if (rc) return rc;
-    xs = x_scale ? x_scale : own;
-    rc = glqb_mx4_dequantize(ws, ws + scales_at, xs, rows, rows, w->n, w->format, ws + back_at, GLQB_DT_F32, stream_);
-    if (rc) return rc;
-    x = ws + back_at;
-    x_stride = w->n;
-    x_dtype = GLQB_DT_F32;
+  int* status = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_mx4_status);
+  if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4_product: %s", cudaGetErrorString(e));
+  Mx4Job J = {};
+  J.m = w->m;
+  J.n = w->n;
+  J.m_tiles = (w->m + MX4_ROWS - 1) / MX4_ROWS;
+  J.k_tiles = (w->n + MX4_K - 1) / MX4_K;
+  J.image = (const uint8_t*)w->image;
+  J.tops = J.image + (size_t)w->experts * J.m_tiles * J.k_tiles * mx4_tile_bytes(w->format);
+  J.w_scale = w->tensor_scale;
+  J.offsets = offsets;
+  J.wide = offsets_are_int64;
+  J.experts = w->experts;
+  J.rows = (int)rows;
+  J.tn = f.tn;
+  J.max_tiles = f.max_tiles;
+  J.split = f.split;
+  J.y = y;
+  J.y_stride = y_stride;
+  J.y_dtype = y_dtype;
+  J.accumulate = accumulate;
+  J.x = x;
+  J.x_stride = x_stride;
+  J.status = status;
+  const size_t lists = (size_t)(J.experts + 1) * 8;
+  if (offsets && clear_rest) mx4_clear_kernel<<<(unsigned)std::min<long long>(rows, 148), 256, lists, stream>>>(J);
+  if (!quantize) {
+    if (f.align) {
+      mx4_align_kernel<<<grid_for(rows * f.n_pad), 256, 0, stream>>>((const uint16_t*)x, x_stride, rows, w->n, f.n_pad, (uint16_t*)workspace);
+      J.x = workspace;
+      J.x_stride = f.n_pad;
+    }
+    const char* what = nullptr;
+    e = mx4_gemm16_launch(w->format, x_dtype == GLQB_DT_BF16, J, sms, stream, &what);
+    if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4_product: %s", what ? what : cudaGetErrorString(e));
+    return mx4_launched("mx4_product");
   }
-  const dim3 grid((unsigned)((w->m + 7) / 8), (unsigned)std::min<long long>((rows + 7) / 8, 1024), (unsigned)w->experts);
-  auto launch = [&](auto fmt) {
+  J.x_image = (uint8_t*)workspace;
+  float* own = (float*)((uint8_t*)workspace + f.image);
+  J.x_scale = x_scale ? x_scale : own;
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_stride * size_of(x_dtype) % 16 == 0);
+  if (w->format == GLQB_MX4_NVFP4 && !x_scale) {
+    const Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, x, size_of(x_dtype));
+    const int rc = amax_launch(x, x_dtype, q, Mx4Range{offsets, offsets_are_int64, w->experts}, own + 1, stream);
+    if (rc) return rc;
+  }
+  const int grid = (int)std::min<long long>((rows + 7) / 8, 148 * 8);
+  auto image = [&](auto fmt) {
     constexpr int FMT = decltype(fmt)::value;
-    if (x_dtype == GLQB_DT_F16)
-      mx4_plain_kernel<FMT, __half><<<grid, 256, 0, stream>>>((const uint8_t*)w->image, w->tensor_scale, w->m, w->n, kt, mt, (const __half*)x, x_stride, rows, offsets,
-                                                              offsets_are_int64, nullptr, (uint8_t*)y, y_dtype, y_stride, accumulate);
-    else if (x_dtype == GLQB_DT_BF16)
-      mx4_plain_kernel<FMT, __nv_bfloat16><<<grid, 256, 0, stream>>>((const uint8_t*)w->image, w->tensor_scale, w->m, w->n, kt, mt, (const __nv_bfloat16*)x, x_stride, rows,
-                                                                     offsets, offsets_are_int64, nullptr, (uint8_t*)y, y_dtype, y_stride, accumulate);
-    else
-      mx4_plain_kernel<FMT, float><<<grid, 256, 0, stream>>>((const uint8_t*)w->image, w->tensor_scale, w->m, w->n, kt, mt, (const float*)x, x_stride, rows, offsets,
-                                                             offsets_are_int64, nullptr, (uint8_t*)y, y_dtype, y_stride, accumulate);
+    if (x_dtype == GLQB_DT_F16) mx4_x_image_kernel<__half, FMT><<<grid, 256, lists, stream>>>(J, x_scale, own + 1, own, f.x_scales, vec);
+    else if (x_dtype == GLQB_DT_BF16) mx4_x_image_kernel<__nv_bfloat16, FMT><<<grid, 256, lists, stream>>>(J, x_scale, own + 1, own, f.x_scales, vec);
+    else mx4_x_image_kernel<float, FMT><<<grid, 256, lists, stream>>>(J, x_scale, own + 1, own, f.x_scales, vec);
   };
-  if (w->format == GLQB_MX4_MXFP4) launch(std::integral_constant<int, GLQB_MX4_MXFP4>());
-  else launch(std::integral_constant<int, GLQB_MX4_NVFP4>());
+  if (w->format == GLQB_MX4_MXFP4) image(std::integral_constant<int, GLQB_MX4_MXFP4>());
+  else image(std::integral_constant<int, GLQB_MX4_NVFP4>());
+  e = mx4_gemm4_launch(w->format, J, sms, stream);
+  if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4_product: %s", cudaGetErrorString(e));
   return mx4_launched("mx4_product");
 }
 
 int glqb_mx4_status(int32_t* status_out) {
-  if (status_out) *status_out = 0;
-  return GLQB_OK;
+  int code = 0;
+  const int zero = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&code, g_mx4_status, sizeof code);
+  if (e == cudaSuccess && code) e = cudaMemcpyToSymbol(g_mx4_status, &zero, sizeof zero);
+  if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4_status: %s", cudaGetErrorString(e));
+  if (status_out) *status_out = code;
+  return code ? mx4_fail(GLQB_E_DEVICE, "a bounded wait in a 4-bit product gave up (status %d): results are invalid", code) : GLQB_OK;
 }
 
 }  // extern "C"

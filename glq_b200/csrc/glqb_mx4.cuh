@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t mx4_decide(uint32_t lo, uint32_t hi, float x
   const float border = 0.5f * (mx4_magnitude(lo) + mx4_magnitude(hi)), rest = fmaf(-(border * s), t, x);
   return rest > 0.0f ? hi : rest < 0.0f ? lo : (lo & 1u) ? hi : lo;
 }
-__device__ __noinline__ uint32_t mx4_decide_tiny(float x, float s, float t) {
+static __device__ __noinline__ uint32_t mx4_decide_tiny(float x, float s, float t) {
   const double d = (double)s * (double)t, a = (double)x;      // (31 bits: products with the borders are exact)
   return (uint32_t)((a > 0.25 * d) + (a >= 0.75 * d) + (a > 1.25 * d) + (a >= 1.75 * d) + (a > 2.5 * d) + (a >= 3.5 * d) + (a > 5.0 * d));
 }
@@ -176,8 +176,8 @@ __device__ __forceinline__ uint32_t mx4_quantize8(const float (&v)[8], float t, 
   }
 }
 
-// the fp32 scale of a tensor whose largest finite value is `amax`: the top of both levels, 448 * 6
-__device__ __forceinline__ float mx4_tensor_scale(float amax) { return fmaxf(__fdiv_rn(amax, 2688.0f), 0x1p-126f); }
+// The fp32 scale of a tensor whose largest finite value is `amax`: the top of both levels, 448 * 6, by its fp32 reciprocal.
+__device__ __forceinline__ float mx4_tensor_scale(float amax) { return fmaxf(amax * (1.0f / 2688.0f), 0x1p-126f); }
 
 // ---- loads of activations -------------------------------------------------------------------------
 // values col .. col + 7 of a row as fp32, zeros from `cols` on; `vec`: rows start on 16 bytes

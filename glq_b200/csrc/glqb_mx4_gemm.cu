@@ -1,0 +1,533 @@
+// Products of microscaled 4-bit weights on the tensor cores (tcgen05.mma, accumulators in tensor memory).
+//
+// One CTA computes 128 weight rows x up to tn rows of x at a time and takes such tiles in turn; accumulators alternate, so
+// that one is drained while the other fills.  A tile's sum over the values may be shared by the CTAs of a cluster (few
+// tiles: decode batches, small layers): each sums its part of the values, and the parts are added in rank order through the
+// cluster's shared memory.  Every wait is bounded: on expiry the status word is set, tensor memory is freed and the kernel
+// returns.
+#include "glqb_mx4_gemm.cuh"
+#include "glqb_launch.h"
+#include <cuda.h>
+#include <algorithm>
+
+namespace glqb {
+namespace {
+
+// ---- PTX ------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+               "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// A from tensor memory, B from shared memory
+__device__ __forceinline__ void umma16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
+               "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+// both from shared memory, 4-bit, scales of blocks in tensor memory
+template <int FMT>
+__device__ __forceinline__ void umma4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  if constexpr (FMT == GLQB_MX4_MXFP4)
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0; tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+                 : "memory");
+  else
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0; tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+                 : "memory");
+}
+// 512 bytes of scales (32 rows of 16) to four columns of tensor memory, the same in all four quarters
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// rows of 16 bytes, eight of them 128 bytes after the eight before, no swizzle
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+
+// fp32 accumulator, both operands K-major, M = 128; `type` 0: fp16, 1: bf16
+__device__ __forceinline__ uint32_t idesc16(int type, int cols) {
+  return (1u << 4) | (uint32_t)type << 7 | (uint32_t)type << 10 | (uint32_t)(cols >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+// e2m1 operands, K = 64; scales e8m0 or e4m3, `sf`: the first of a word's four bytes that an instruction takes
+template <int FMT>
+__device__ __forceinline__ uint32_t idesc4(int cols, uint32_t sf) {
+  return sf << 4 | 1u << 7 | 1u << 10 | (uint32_t)(cols >> 3) << 17 | (FMT == GLQB_MX4_MXFP4 ? 1u << 23 : 0u) | (uint32_t)(128 >> 7) << 27 | sf << 29;
+}
+
+// ---- parts of both kernels ------------------------------------------------------------------------
+struct Bars {                  // in shared memory
+  uint64_t full_w[8], empty_w[8], full_x[8], empty_x[8], full_a[2], empty_a[2], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  volatile int abort;
+};
+
+// Columns of a finished accumulator to y, or (a cluster's CTA) to shared memory as [column][row].
+template <int FMT, typename T, bool QUANT>
+__device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, int mt, uint32_t acc, int quarter, int lane, float* red) {
+  const int r = quarter * 32 + lane, row = mt * MX4_ROWS + r;
+  Mx4Factor f{1.0f, 1.0f};
+  if (!red && row < J.m) {
+    if constexpr (!QUANT) f = mx4_row_factor<FMT, T>(J, t.expert, row);
+    else if constexpr (FMT == GLQB_MX4_NVFP4) f = Mx4Factor{J.w_scale[t.expert], *J.x_scale};
+  }
+#pragma unroll 1
+  for (int c0 = 0; c0 < t.rows; c0 += 32) {
+    uint32_t v[32];
+    tmem_ld32(acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0, v);
+    tmem_ld_wait();
+    if (red) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c0 + i < t.rows) red[(c0 + i) * MX4_ROWS + r] = __uint_as_float(v[i]);
+    } else if (row < J.m) {
+      const long long at = (long long)(t.row0 + c0) * J.y_stride + row;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c0 + i < t.rows) mx4_put(J, at + i * J.y_stride, __uint_as_float(v[i]) * f.a * f.b);
+    }
+  }
+}
+// The cluster's parts of a tile, added in rank order; the columns are shared out over the CTAs.
+template <int FMT, typename T, bool QUANT>
+__device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int mt, float* red, int rank) {
+  const int r = threadIdx.x % MX4_ROWS, row = mt * MX4_ROWS + r;
+  if (row >= J.m) return;
+  Mx4Factor f{1.0f, 1.0f};
+  if constexpr (!QUANT) f = mx4_row_factor<FMT, T>(J, t.expert, row);
+  else if constexpr (FMT == GLQB_MX4_NVFP4) f = Mx4Factor{J.w_scale[t.expert], *J.x_scale};
+  const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
+  for (int c = rank + J.split * (int)(threadIdx.x / MX4_ROWS); c < t.rows; c += J.split * (int)(blockDim.x / MX4_ROWS)) {
+    float v = 0.0f;
+    for (int s = 0; s < J.split; ++s) v += ld_cluster(base + (uint32_t)(c * MX4_ROWS * 4), s);
+    mx4_put(J, (long long)(t.row0 + c) * J.y_stride + row, v * f.a * f.b);
+  }
+}
+
+// ---- 16-bit activations ---------------------------------------------------------------------------
+// Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by eight warps straight into tensor memory as
+// the A operand (thread = row, 64 values = 32 columns), activations by TMA as 64-value boxes with the 128-byte swizzle.  A step
+// is 128 values: eight MMAs.  Warp 0 issues MMAs, warp 1 loads, warps 4-7 drain, warps 8-15 decode.
+constexpr int G16_THREADS = 512, G16_W_STAGES = 3, G16_MAX_TN = 192;
+constexpr int G16_A0 = 2 * G16_MAX_TN;             // tensor memory: two accumulators, then two stages of A of 64 columns
+
+struct Mx4Ring { int x_stages, box_rows, x_half; };  // stages of x, rows per box, bytes of 64 values of a tile
+
+template <int FMT, typename T>
+__global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid_constant__ Mx4Job J, const __grid_constant__ CUtensorMap map, Mx4Ring R) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* w_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* x_base = w_base + G16_W_STAGES * mx4_tile_bytes(FMT);
+  Bars& B = *reinterpret_cast<Bars*>(x_base + R.x_stages * 2 * R.x_half);
+  int* eff = reinterpret_cast<int*>(&B + 1);
+  int* pre = eff + J.experts + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < G16_W_STAGES; ++s) { mbar_init(&B.full_w[s], 1); mbar_init(&B.empty_w[s], 8); }
+    for (int s = 0; s < R.x_stages; ++s) { mbar_init(&B.full_x[s], 1); mbar_init(&B.empty_x[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&B.full_a[s], 8); mbar_init(&B.empty_a[s], 1); mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], 4); }
+    mbar_init(&B.drain, 1);
+    B.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&B.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  mx4_groups(J, eff, pre);                         // (ends with a block barrier)
+  tc_fence_after();
+  const uint32_t tmem = B.tmem;
+  const int tiles = min(pre[J.experts], J.max_tiles) * J.m_tiles;
+  const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
+  const int k0 = rank * J.k_tiles / J.split, k1 = (rank + 1) * J.k_tiles / J.split;      // this CTA's tiles of 256 values
+  const int steps = min(2 * k1, (J.n + 127) / 128) - 2 * k0;                             // of 128
+  uint32_t loads_w = 0, loads_x = 0;
+  bool ok = true;
+
+  if (warp == 0) {
+    uint32_t q = 0, seq = 0;
+    const uint32_t x0 = smem_u32(x_base);
+    for (int i = first; i < tiles && ok; i += step, ++seq) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+      const uint32_t idesc = idesc16(__is_same(T, __half) ? 0 : 1, (t.rows + 15) & ~15), d = tmem + (seq & 1u) * G16_MAX_TN;
+      if (!mbar_wait(&B.acc_empty[seq & 1u], ((seq >> 1) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
+      tc_fence_after();
+      for (int k = 0; k < steps; ++k, ++q) {
+        const uint32_t sa = q & 1u, sx = q % R.x_stages;
+        if (!mbar_wait(&B.full_x[sx], (q / R.x_stages) & 1u, &B.abort) || !mbar_wait(&B.full_a[sa], (q >> 1) & 1u, &B.abort)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t a = tmem + G16_A0 + sa * 64u, b = x0 + sx * 2u * R.x_half;
+          const uint64_t d0 = umma_desc_sw128(b), d1 = umma_desc_sw128(b + R.x_half);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma16(d, a + 8u * j, d0 + 2u * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma16(d, a + 32u + 8u * j, d1 + 2u * j, idesc, 1u);
+          umma_commit(&B.empty_x[sx]);
+          umma_commit(&B.empty_a[sa]);
+          if (k + 1 == steps) umma_commit(&B.acc_full[seq & 1u]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int i = first; i < tiles && ok; i += step) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + i % J.m_tiles) * J.k_tiles + k0) * mx4_tile_bytes(FMT);
+        const int boxes = (t.rows + R.box_rows - 1) / R.box_rows;
+        for (int k = 0; k < steps && ok; ++k, ++loads_x) {
+          if ((k & 1) == 0) {
+            const uint32_t s = loads_w % G16_W_STAGES;
+            if (!mbar_wait(&B.empty_w[s], ((loads_w / G16_W_STAGES) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
+            mbar_expect_tx(&B.full_w[s], mx4_tile_bytes(FMT));
+            bulk_g2s(w_base + s * mx4_tile_bytes(FMT), src + (long long)(k >> 1) * mx4_tile_bytes(FMT), mx4_tile_bytes(FMT), &B.full_w[s]);
+            ++loads_w;
+          }
+          const uint32_t s = loads_x % R.x_stages;
+          if (!mbar_wait(&B.empty_x[s], ((loads_x / R.x_stages) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
+          mbar_expect_tx(&B.full_x[s], (uint32_t)(2 * boxes * R.box_rows * 128));
+          uint8_t* dst = x_base + s * 2 * R.x_half;
+          for (int b = 0; b < boxes; ++b) {
+            tma_load_2d(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, t.row0 + b * R.box_rows, &B.full_x[s]);
+            tma_load_2d(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, t.row0 + b * R.box_rows, &B.full_x[s]);
+          }
+        }
+      }
+      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+    }
+  } else if (warp >= 8) {
+    // warps 8-11 take the first 64 values of a step, 12-15 the others; a warp the 32 rows of its quarter of tensor memory
+    const int half = (warp - 8) >> 2, r = (warp & 3) * 32 + lane;
+    uint32_t q = 0, wq = 0;
+    for (int i = first; i < tiles && ok; i += step) {
+      int top = 0;
+      if constexpr (FMT == GLQB_MX4_MXFP4) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+        top = J.tops[((long long)t.expert * J.m_tiles + i % J.m_tiles) * MX4_ROWS + r];
+      }
+      for (int k = 0; k < steps; ++k, ++q) {
+        const uint32_t s = wq % G16_W_STAGES, sa = q & 1u;
+        if ((k & 1) == 0 && !mbar_wait(&B.full_w[s], (wq / G16_W_STAGES) & 1u, &B.abort)) { ok = false; break; }
+        const uint8_t* tile = w_base + s * mx4_tile_bytes(FMT);
+        const int c = (k & 1) * 4 + half * 2;      // 16-byte units of a row: two of them
+        uint32_t a[32];
+        const uint8_t* codes = tile + (r >> 3) * 1024 + (r & 7) * 128;
+        const uint8_t* sc = tile + MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4;
+        uint32_t sw;
+        if constexpr (FMT == GLQB_MX4_MXFP4) sw = *reinterpret_cast<const uint32_t*>(sc + (c >> 2) * 512) >> (8 * (c & 3));
+        else sw = *reinterpret_cast<const uint32_t*>(sc + (c >> 1) * 512);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 v = *reinterpret_cast<const uint4*>(codes + (((c + u) ^ (r & 7)) << 4));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t m0, m1;
+          if constexpr (FMT == GLQB_MX4_MXFP4) m0 = m1 = mx4_multiplier<FMT, T>((sw >> (8 * u)) & 0xFFu, top);
+          else {
+            m0 = mx4_multiplier<FMT, T>((sw >> (16 * u)) & 0xFFu, 0);
+            m1 = mx4_multiplier<FMT, T>((sw >> (16 * u + 8)) & 0xFFu, 0);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) a[u * 16 + j * 4 + p] = mx4_mul2<T>(mx4_pair<T>(w[j], p), j < 2 ? m0 : m1);
+        }
+        if ((k & 1) == 1 || k + 1 == steps) {      // done with this tile of weights
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.empty_w[s]);
+          ++wq;
+        }
+        if (!mbar_wait(&B.empty_a[sa], ((q >> 1) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
+        __syncwarp();
+        tc_fence_after();
+        tmem_st32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + G16_A0 + sa * 64u + half * 32u, a);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.full_a[sa]);
+      }
+    }
+    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER); }
+  } else if (warp >= 4) {
+    uint32_t seq = 0;
+    for (int i = first; i < tiles && ok; i += step, ++seq) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+      if (!mbar_wait(&B.acc_full[seq & 1u], (seq >> 1) & 1u, &B.abort)) { ok = false; break; }
+      __syncwarp();
+      tc_fence_after();
+      drain_tile<FMT, T, false>(J, t, i % J.m_tiles, tmem + (seq & 1u) * G16_MAX_TN, warp & 3, lane, J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.acc_empty[seq & 1u]);
+    }
+    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
+  }
+  // ---- every thread arrives here, also after a wait gave up
+  __syncwarp();
+  if (J.split > 1) {                               // (one tile per cluster)
+    cluster_sync();
+    if (first < tiles) add_parts<FMT, T, false>(J, mx4_tile(J, eff, pre, first / J.m_tiles), first % J.m_tiles, reinterpret_cast<float*>(x_base), rank);
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (B.abort) {
+    // what may still be in flight: the copies armed last, and the MMAs issued so far
+    if (warp == 1 && lane == 0) {
+      for (uint32_t n = 0; n < min(loads_w, (uint32_t)G16_W_STAGES); ++n) {
+        const uint32_t u = loads_w - 1 - n;
+        mbar_wait(&B.full_w[u % G16_W_STAGES], (u / G16_W_STAGES) & 1u);
+      }
+      for (uint32_t n = 0; n < min(loads_x, (uint32_t)R.x_stages); ++n) {
+        const uint32_t u = loads_x - 1 - n;
+        mbar_wait(&B.full_x[u % R.x_stages], (u / R.x_stages) & 1u);
+      }
+    }
+    if (warp == 0 && elect_one()) {
+      umma_commit(&B.drain);
+      mbar_wait(&B.drain, 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- 4-bit activations ----------------------------------------------------------------------------
+// Both operands as they lie in their images; a stage is 256 values: four MMAs, whose scales one thread copies to tensor memory
+// in front of them.  Warp 0 issues, warp 1 loads, warps 4-7 drain.
+constexpr int G4_THREADS = 256;
+template <int FMT> struct G4 {
+  static constexpr int ATOMS = mx4_scale_bytes(FMT) / 512;         // 512-byte pieces of scales per 128 rows x 256 values
+  static constexpr int MAX_TN = FMT == GLQB_MX4_MXFP4 ? 192 : 160;
+  static constexpr int SF_COLS = ATOMS * 12;                       // tensor memory of a stage: weights 4, activations 8 per piece
+  static constexpr int STAGES = (512 - 2 * MAX_TN) / SF_COLS;      // MXFP4 5, NVFP4 4: tensor memory, and shared memory
+};
+
+template <int FMT>
+__global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_constant__ Mx4Job J, int stages, int x_scales) {
+  using C = G4<FMT>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int stage_bytes = mx4_tile_bytes(FMT) + J.tn * 128 + x_scales;
+  Bars& B = *reinterpret_cast<Bars*>(base + stages * stage_bytes);
+  int* eff = reinterpret_cast<int*>(&B + 1);
+  int* pre = eff + J.experts + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&B.full_x[s], 1); mbar_init(&B.empty_x[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], 4); }
+    mbar_init(&B.drain, 1);
+    B.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&B.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  mx4_groups(J, eff, pre);
+  tc_fence_after();
+  const uint32_t tmem = B.tmem;
+  const int tiles = min(pre[J.experts], J.max_tiles) * J.m_tiles;
+  const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
+  const int k0 = rank * J.k_tiles / J.split, steps = (rank + 1) * J.k_tiles / J.split - k0;
+  uint32_t loads = 0;
+  bool ok = true;
+
+  if (warp == 0) {
+    uint32_t q = 0, seq = 0;
+    for (int i = first; i < tiles && ok; i += step, ++seq) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+      const int cols = (t.rows + 15) & ~15;
+      const uint32_t d = tmem + (seq & 1u) * C::MAX_TN;
+      if (!mbar_wait(&B.acc_empty[seq & 1u], ((seq >> 1) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
+      tc_fence_after();
+      for (int k = 0; k < steps; ++k, ++q) {
+        const uint32_t s = q % stages;
+        if (!mbar_wait(&B.full_x[s], (q / stages) & 1u, &B.abort)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t w = smem_u32(base) + s * stage_bytes, x = w + mx4_tile_bytes(FMT);
+          const uint32_t sa = tmem + 2 * C::MAX_TN + s * C::SF_COLS, sb = sa + 4 * C::ATOMS;
+          const uint64_t dws = scale_desc(w + MX4_CODE_BYTES), dxs = scale_desc(x + J.tn * 128);
+          // (copies and MMAs of one thread run in the order they are issued in)
+#pragma unroll
+          for (int j = 0; j < C::ATOMS; ++j) {
+            tmem_copy_scales(sa + 4u * j, dws + 32u * j);
+            tmem_copy_scales(sb + 8u * j, dxs + 32u * j);
+            if (cols > 128) tmem_copy_scales(sb + 8u * j + 4u, dxs + 32u * (j + C::ATOMS));
+          }
+          const uint64_t da = umma_desc_sw128(w), db = umma_desc_sw128(x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t atom = j * C::ATOMS / 4, sf = C::ATOMS == 2 ? 2u * (j & 1) : 0u;
+            umma4<FMT>(d, da + 2u * j, db + 2u * j, idesc4<FMT>(cols, sf), sa + 4u * atom, sb + 8u * atom, (k > 0 || j > 0) ? 1u : 0u);
+          }
+          umma_commit(&B.empty_x[s]);
+          if (k + 1 == steps) umma_commit(&B.acc_full[seq & 1u]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const int x_stage = J.tn * 128 + x_scales;
+      for (int i = first; i < tiles && ok; i += step) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+        const uint32_t x_codes = (uint32_t)((t.rows + 15) & ~15) * 128u;
+        const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + i % J.m_tiles) * J.k_tiles + k0) * mx4_tile_bytes(FMT);
+        const uint8_t* xsrc = J.x_image + ((long long)(i / J.m_tiles) * J.k_tiles + k0) * x_stage;
+        for (int k = 0; k < steps; ++k, ++loads) {
+          const uint32_t s = loads % stages;
+          if (!mbar_wait(&B.empty_x[s], ((loads / stages) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
+          uint8_t* w = base + s * stage_bytes;
+          mbar_expect_tx(&B.full_x[s], mx4_tile_bytes(FMT) + x_codes + x_scales);
+          bulk_g2s(w, wsrc + (long long)k * mx4_tile_bytes(FMT), mx4_tile_bytes(FMT), &B.full_x[s]);
+          bulk_g2s(w + mx4_tile_bytes(FMT), xsrc + (long long)k * x_stage, x_codes, &B.full_x[s]);
+          bulk_g2s(w + mx4_tile_bytes(FMT) + J.tn * 128, xsrc + (long long)k * x_stage + J.tn * 128, x_scales, &B.full_x[s]);
+        }
+      }
+      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+    }
+  } else if (warp >= 4) {
+    uint32_t seq = 0;
+    for (int i = first; i < tiles && ok; i += step, ++seq) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+      if (!mbar_wait(&B.acc_full[seq & 1u], (seq >> 1) & 1u, &B.abort)) { ok = false; break; }
+      __syncwarp();
+      tc_fence_after();
+      drain_tile<FMT, __half, true>(J, t, i % J.m_tiles, tmem + (seq & 1u) * C::MAX_TN, warp & 3, lane, J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.acc_empty[seq & 1u]);
+    }
+    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
+  }
+  __syncwarp();
+  if (J.split > 1) {
+    cluster_sync();
+    if (first < tiles) add_parts<FMT, __half, true>(J, mx4_tile(J, eff, pre, first / J.m_tiles), first % J.m_tiles, reinterpret_cast<float*>(base), rank);
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (B.abort) {
+    if (warp == 1 && lane == 0)
+      for (uint32_t n = 0; n < min(loads, (uint32_t)stages); ++n) {
+        const uint32_t u = loads - 1 - n;
+        mbar_wait(&B.full_x[u % stages], (u / stages) & 1u);
+      }
+    if (warp == 0 && elect_one()) {
+      umma_commit(&B.drain);
+      mbar_wait(&B.drain, 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
+  // (per device and idempotent: a word of the runtime, no synchronisation)
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// More than half of an SM's shared memory, whatever a launch needs: two CTAs on an SM would wait for each other's tensor memory,
+// and clusters that do so in turn would wait for ever.
+constexpr size_t ONE_PER_SM = 120 * 1024;
+
+size_t groups_bytes(const Mx4Job& J) { return sizeof(Bars) + (size_t)(J.experts + 1) * 8; }
+
+}  // namespace
+
+cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count, cudaStream_t stream, const char** what) {
+  Mx4Ring R;
+  R.box_rows = std::min(J.tn, 32);
+  const int rows = (J.tn + R.box_rows - 1) / R.box_rows * R.box_rows;
+  R.x_half = rows * 128;
+  const size_t fixed = 1024 + G16_W_STAGES * (size_t)mx4_tile_bytes(format) + groups_bytes(J);
+  R.x_stages = (int)std::min<size_t>(8, (227 * 1024 - fixed) / (2 * (size_t)R.x_half));
+  const size_t smem = std::max(ONE_PER_SM, fixed + (size_t)R.x_stages * 2 * R.x_half);
+  CUtensorMap map;
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) { *what = "cuTensorMapEncodeTiled not found"; return cudaErrorNotSupported; }
+  const cuuint64_t dims[2] = {(cuuint64_t)J.n, (cuuint64_t)J.rows}, strides[1] = {(cuuint64_t)(J.rows == 1 ? (J.n * 2 + 15) / 16 * 16 : J.x_stride * 2)};
+  const cuuint32_t box[2] = {64, (cuuint32_t)R.box_rows}, ones[2] = {1, 1};
+  const CUresult r = encode(&map, x_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(J.x), dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { *what = "cuTensorMapEncodeTiled refused the activations"; return cudaErrorInvalidValue; }
+  const long long tiles = (long long)J.max_tiles * J.m_tiles;
+  const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
+  auto run = [&](auto* kernel) { return launch(kernel, grid, G16_THREADS, smem, J.split, stream, J, map, R); };
+  if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(mx4_gemm16_kernel<GLQB_MX4_MXFP4, __nv_bfloat16>) : run(mx4_gemm16_kernel<GLQB_MX4_MXFP4, __half>);
+  return x_bf16 ? run(mx4_gemm16_kernel<GLQB_MX4_NVFP4, __nv_bfloat16>) : run(mx4_gemm16_kernel<GLQB_MX4_NVFP4, __half>);
+}
+
+cudaError_t mx4_gemm4_launch(int format, const Mx4Job& J, int sm_count, cudaStream_t stream) {
+  const int x_scales = mx4_x_scale_bytes(format, J.tn), most = format == GLQB_MX4_MXFP4 ? G4<GLQB_MX4_MXFP4>::STAGES : G4<GLQB_MX4_NVFP4>::STAGES;
+  const size_t fixed = 1024 + groups_bytes(J), stage = (size_t)mx4_tile_bytes(format) + J.tn * 128 + x_scales;
+  const int stages = (int)std::min<size_t>(most, (227 * 1024 - fixed) / stage);
+  const long long tiles = (long long)J.max_tiles * J.m_tiles;
+  const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
+  const size_t smem = std::max(ONE_PER_SM, fixed + stages * stage);
+  auto run = [&](auto* kernel) { return launch(kernel, grid, G4_THREADS, smem, J.split, stream, J, stages, x_scales); };
+  return format == GLQB_MX4_MXFP4 ? run(mx4_gemm4_kernel<GLQB_MX4_MXFP4>) : run(mx4_gemm4_kernel<GLQB_MX4_NVFP4>);
+}
+
+}  // namespace glqb

@@ -1,0 +1,156 @@
+// What the products of microscaled 4-bit weights share: the job, the token tiles of experts, the results.
+#pragma once
+#include "glqb_mx4.cuh"
+#include "glqb_ptx.cuh"
+
+namespace glqb {
+
+constexpr int MX4_MAX_EXPERTS = 1024;
+
+struct Mx4Job {
+  const uint8_t* image;
+  const uint8_t* tops;        // MXFP4: largest scale byte of every row (experts x m_tiles * 128)
+  const float* w_scale;       // NVFP4: fp32 scale per expert
+  const float* x_scale;       // 4-bit activations, NVFP4: theirs
+  const void* offsets;        // null: one matrix, all rows
+  int wide, experts, rows, m, n, m_tiles, k_tiles;
+  int tn;                     // most rows of x per token tile, a multiple of 16
+  int max_tiles;              // bound of the token tiles
+  int split;                  // CTAs of a cluster that share a tile's sum
+  void* y;
+  long long y_stride;
+  int y_dtype, accumulate;
+  const void* x;              // 16-bit activations
+  long long x_stride;
+  uint8_t* x_image;           // 4-bit activations: per token tile, per 256 values: tn rows of 128 bytes, then the scales
+  int* status;
+};
+
+#ifdef __CUDACC__
+// Rows of every expert and the token tiles in front of it.  offsets are held to 0 .. rows and to ascend (each at least
+// the largest before it), so that whatever they hold, experts do not overlap and the tiles are no more than max_tiles.
+// Called by all threads; `eff` and `pre` have experts + 1 entries in shared memory.
+__device__ __forceinline__ void mx4_groups(const Mx4Job& J, int* eff, int* pre) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    if (!J.offsets) {
+      if (lane == 0) { eff[0] = 0; eff[1] = J.rows; pre[0] = 0; pre[1] = (J.rows + J.tn - 1) / J.tn; }
+    } else {
+      int top = 0, tiles = 0;
+      for (int b = 0; b <= J.experts; b += 32) {
+        const int e = min(b + lane, J.experts);
+        const long long o = J.wide ? reinterpret_cast<const long long*>(J.offsets)[e] : reinterpret_cast<const int*>(J.offsets)[e];
+        int v = (int)max(0ll, min((long long)J.rows, o));
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+          if (lane >= d) v = max(v, u);
+        }
+        v = max(v, top);
+        int before = __shfl_up_sync(0xFFFFFFFFu, v, 1);
+        if (lane == 0) before = b == 0 ? v : top;
+        int t = (v - before + J.tn - 1) / J.tn;        // tiles of expert e - 1
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int u = __shfl_up_sync(0xFFFFFFFFu, t, d);
+          if (lane >= d) t += u;
+        }
+        t += tiles;
+        if (b + lane <= J.experts) { eff[e] = v; pre[e] = t; }
+        top = __shfl_sync(0xFFFFFFFFu, v, 31);
+        tiles = __shfl_sync(0xFFFFFFFFu, t, 31);
+      }
+    }
+  }
+  __syncthreads();
+}
+// the last e with list[e] <= v (list ascends, list[0] <= v < list[experts]): the expert that has tile, or row, v
+__device__ __forceinline__ int mx4_find(const int* list, int experts, int v) {
+  int lo = 0, hi = experts;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (list[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+// Token tile t: an expert's rows are split evenly over as few tiles as they need, in steps of 16 (no tile is empty: the tiles
+// before the last hold fewer than the expert has).
+struct Mx4Tile { int expert, row0, rows; };
+__device__ __forceinline__ int mx4_per_tile(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) & ~15; }
+__device__ __forceinline__ Mx4Tile mx4_tile(const Mx4Job& J, const int* eff, const int* pre, int t) {
+  const int e = J.experts == 1 ? 0 : mx4_find(pre, J.experts, t);
+  const int rows = eff[e + 1] - eff[e], per = mx4_per_tile(rows, pre[e + 1] - pre[e]), at = (t - pre[e]) * per;
+  return Mx4Tile{e, eff[e] + at, min(per, rows - at)};
+}
+
+__device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) {
+  if (J.y_dtype == GLQB_DT_BF16) {
+    __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(J.y) + at;
+    *p = __float2bfloat16_rn(J.accumulate ? __bfloat162float(*p) + v : v);
+  } else if (J.y_dtype == GLQB_DT_F16) {
+    __half* p = reinterpret_cast<__half*>(J.y) + at;
+    *p = __float2half_rn(J.accumulate ? __half2float(*p) + v : v);
+  } else {
+    float* p = reinterpret_cast<float*>(J.y) + at;
+    *p = J.accumulate ? *p + v : v;
+  }
+}
+
+// ---- 4-bit weights as 16-bit operands -------------------------------------------------------------
+// The bits of a code are moved to sign, exponent and first mantissa bit of a 16-bit number, where they read as the value times
+// 2^-126 (bf16) or 2^-14 (fp16), subnormals included; one multiplication by a power of two, or by an e4m3 number, times what
+// brings that back gives the operand exactly.  So that the multiplier stays in range, operands are
+//   MXFP4  value * 2^(s - top) (bf16), value * 2^(s - top + 1) (fp16), top the largest scale byte of the row
+//   NVFP4  value * s * 2^-7
+// and mx4_row_factor is what the sums are multiplied by.
+template <typename T>
+__device__ __forceinline__ uint32_t mx4_pair(uint32_t w, int i) {       // values 2i, 2i + 1 of a word
+  const uint32_t x = (i == 3 ? w : w << (12 - 4 * i)) & 0xF000F000u;
+  if constexpr (__is_same(T, __half)) return (x | x >> 3) & 0x8E008E00u;
+  else return (x | x >> 6) & 0x81C081C0u;
+}
+template <int FMT, typename T>
+__device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {   // in both halves
+  uint32_t h;
+  if constexpr (FMT == GLQB_MX4_MXFP4) {
+    const int d = (int)s - top;
+    if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : d > -30 ? (uint32_t)(d + 30) << 10 : d >= -39 ? 1u << (d + 39) : 0u;
+    else h = s == 255u ? 0x7FC0u : d > -253 ? (uint32_t)(d + 253) << 7 : 0u;
+  } else {
+    const float f = mx4_e4m3(s);
+    if constexpr (__is_same(T, __half)) h = __half_as_ushort(__float2half_rn(f * 128.0f));
+    else h = __float_as_uint(f * 0x1p119f) >> 16;
+  }
+  return h | h << 16;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t mx4_mul2(uint32_t a, uint32_t b) {
+  if constexpr (__is_same(T, __half)) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+struct Mx4Factor { float a, b; };     // two factors: 2^-127 and 2^127 have no single one
+template <int FMT, typename T>
+__device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert, int row) {
+  if constexpr (FMT == GLQB_MX4_MXFP4) {
+    const int p = (int)J.tops[(long long)expert * J.m_tiles * MX4_ROWS + row] - (__is_same(T, __half) ? 128 : 127), h = p >> 1;
+    return Mx4Factor{__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(p - h + 127) << 23)};
+  } else {
+    return Mx4Factor{128.0f, J.w_scale[expert]};
+  }
+}
+#endif  // __CUDACC__
+
+// ---- glqb_mx4_gemm.cu
+// `x_bf16`: type of 16-bit activations.  Rows of x start on 16 bytes.
+cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& job, int sm_count, cudaStream_t stream, const char** what);
+cudaError_t mx4_gemm4_launch(int format, const Mx4Job& job, int sm_count, cudaStream_t stream);
+// scales of a token tile per 256 values, in bytes
+inline int mx4_x_scale_bytes(int format, int tn) { return mx4_scale_bytes(format) * ((tn + 127) / 128); }
+
+}  // namespace glqb

@@ -106,7 +106,7 @@ def mx4_quantize(x, format="mxfp4", tensor_scale=None) -> Mx4Tensor:
     """x (..., cols) of bf16, fp16 or fp32 to 4 bits, each value to the nearest (ties to the even code) of its block's scale.
     "mxfp4": the scale is 2^(floor(log2 amax) - 2), values above six times it saturate.  "nvfp4": the block's scale is the
     e4m3 number nearest to amax / (6 t), with t the one fp32 value ``tensor_scale`` (positive), or, without it,
-    max(largest finite |x| / 2688, 2^-126), found by a first pass.  A block with an infinity or NaN becomes NaN."""
+    max(largest finite |x| * fp32(1 / 2688), 2^-126), found by a first pass.  A block with an infinity or NaN becomes NaN."""
     fmt = _format(format)
     _cuda(x, "x")
     dt = _dtype(x.dtype, "x")
@@ -269,7 +269,7 @@ def mx4_grouped_linear(x, weight: Mx4Weight, offsets, *, quantize_input=False, i
     (experts, m, n) weight: (rows, m).  ``offsets``: experts + 1 ascending integers (int32 or int64) on the device, any number of
     rows per expert, none included; nothing is read back.  Rows of no expert (in front of offsets[0], behind offsets[experts])
     are zero in a new result and stay as they are in a given ``out`` (rows, m), whose rows may lie apart.  Offsets outside
-    0 .. rows are held to that range, and an expert whose range ends before it begins has no rows.  The other arguments as for
+    0 .. rows are held to that range, and one that is less than the one before it counts as that one.  At most 1024 experts.  The other arguments as for
     ``mx4_linear``; "nvfp4" inputs without ``input_scale`` take the scale of rows offsets[0] .. offsets[experts] - 1."""
     _input(x, weight, quantize_input)
     if weight.experts is None:

@@ -305,7 +305,7 @@ size_t glqb_noalloc_scratch_bytes(void);
 
 /* rows x cols values (x_stride elements apart) to stored rows, each rounded to nearest even from the real quotient by its
  * block's scale: MXFP4 2^(floor(log2 amax) - 2), saturating at 6; NVFP4 e4m3(amax / (6 t)), t = *tensor_scale (positive), or,
- * with tensor_scale NULL, max(largest finite |x| / 2688, 2^-126), which is left in own_scale[0] (own_scale: two floats,
+ * with tensor_scale NULL, max(largest finite |x| * fp32(1 / 2688), 2^-126), which is left in own_scale[0] (own_scale: two floats,
  * needed then).  A block with an infinity or NaN gets the scale NaN and codes of zero. */
 int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows, int32_t cols, int32_t format,
                       const float* tensor_scale, float* own_scale, void* codes, void* scales, void* stream);
@@ -326,8 +326,8 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
 
 /* y[r] = x[r] W_e^T, fp32 sums rounded once.  offsets NULL: one matrix, all rows.  Else device integers (int64 with
  * offsets_are_int64, else int32), experts + 1 of them: rows offsets[e] .. offsets[e + 1] - 1 of x and y belong to expert e.  They
- * are read on the device and held to 0 .. rows; a range that ends before it begins is empty.  Rows of no expert keep what y
- * holds, or are zeroed with clear_rest.
+ * ascend; they are read on the device, where each is held to 0 .. rows and to no less than the one before it.  Rows of no expert
+ * keep what y holds, or are zeroed with clear_rest.  At most 1024 experts.
  * quantize: x is brought to the weights' format first, as glqb_mx4_quantize does (NVFP4: by *x_scale, or, with x_scale NULL, by the
  * scale of rows offsets[0] .. offsets[experts] - 1), and 4-bit values are multiplied.  Without it x is fp16 or bf16 and stays so.
  * MXFP4 weights are held relative to the largest scale of their row: under fp16 activations a block more than 2^24 below it

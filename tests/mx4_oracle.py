@@ -18,7 +18,7 @@ def nearest(value, table):
 def tensor_scale(x):
     a = np.abs(x[np.isfinite(x)])
     top = np.float32(a.max() if a.size else 0.0)
-    return max(np.float32(top / np.float32(2688.0)), np.float32(2.0 ** -126))
+    return max(np.float32(top * np.float32(1.0 / 2688.0)), np.float32(2.0 ** -126))
 
 
 def quantize(x, fmt, t=None):
