@@ -480,6 +480,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.y_stride = y_stride;
   J.y_dtype = y_dtype;
   J.accumulate = accumulate;
+  J.y_wide = y_dtype != GLQB_DT_F32 && !accumulate && reinterpret_cast<uintptr_t>(y) % 16 == 0 && (rows == 1 || y_stride % 8 == 0);
   J.x = x;
   J.x_stride = x_stride;
   J.status = status;

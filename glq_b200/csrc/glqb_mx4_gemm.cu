@@ -29,6 +29,19 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
 // A from tensor memory, B from shared memory
 __device__ __forceinline__ void umma16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
@@ -77,36 +90,74 @@ __device__ __forceinline__ uint32_t idesc4(int cols, uint32_t sf) {
 }
 
 // ---- parts of both kernels ------------------------------------------------------------------------
-struct Bars {                  // in shared memory
+struct __align__(16) Bars {     // in shared memory
+  uint8_t turn[4][2048];       // results on their way out, per draining warp
   uint64_t full_w[8], empty_w[8], full_x[8], empty_x[8], full_a[2], empty_a[2], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   volatile int abort;
 };
 
-// Columns of a finished accumulator to y, or (a cluster's CTA) to shared memory as [column][row].
 template <int FMT, typename T, bool QUANT>
-__device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, int mt, uint32_t acc, int quarter, int lane, float* red) {
+__device__ __forceinline__ Mx4Factor row_factor(const Mx4Job& J, int expert, int row) {
+  if constexpr (!QUANT) return mx4_row_factor<FMT, T>(J, expert, row);
+  else if constexpr (FMT == GLQB_MX4_NVFP4) return Mx4Factor{J.w_scale[expert], *J.x_scale};
+  else return Mx4Factor{1.0f, 1.0f};
+}
+// Columns of a finished accumulator to y, or (a cluster's CTA) to shared memory as [column][row].  A thread has a row of
+// weights, so its values lie y_stride apart: 32 rows x 32 columns are turned in the warp's 2 KiB of shared memory and stored 16
+// bytes per lane.  (A 2-byte store per value took 4000 clocks per 32 columns, 24,000 per tile of 192, which is a mainloop of
+// 4096 values; most of it instruction fetches of the unrolled stores.)  Other results go eight columns at a time.
+template <int FMT, typename T, bool QUANT>
+__device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, int mt, uint32_t acc, int quarter, int lane, uint8_t* stage, float* red) {
   const int r = quarter * 32 + lane, row = mt * MX4_ROWS + r;
-  Mx4Factor f{1.0f, 1.0f};
-  if (!red && row < J.m) {
-    if constexpr (!QUANT) f = mx4_row_factor<FMT, T>(J, t.expert, row);
-    else if constexpr (FMT == GLQB_MX4_NVFP4) f = Mx4Factor{J.w_scale[t.expert], *J.x_scale};
+  acc += (uint32_t)(quarter * 32) << 16;
+  if (red) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < t.rows; c0 += 16) {
+      uint32_t v[16];
+      tmem_ld16(acc + (uint32_t)c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) red[(c0 + i) * MX4_ROWS + r] = __uint_as_float(v[i]);    // (room for whole sixteens)
+    }
+    return;
+  }
+  const Mx4Factor f = row < J.m ? row_factor<FMT, T, QUANT>(J, t.expert, row) : Mx4Factor{1.0f, 1.0f};
+  if (J.y_wide && mt * MX4_ROWS + quarter * 32 + 32 <= J.m) {
+    uint16_t* put = reinterpret_cast<uint16_t*>(stage) + lane;
+    const uint8_t* get = stage + lane * 16;
+    uint16_t* y = reinterpret_cast<uint16_t*>(J.y) + (long long)(t.row0 + (lane >> 2)) * J.y_stride + mt * MX4_ROWS + quarter * 32 + (lane & 3) * 8;
+    const bool bf16 = J.y_dtype == GLQB_DT_BF16;
+#pragma unroll 1
+    for (int c0 = 0; c0 < t.rows; c0 += 32) {
+      uint32_t v[32];
+      tmem_ld32(acc + (uint32_t)c0, v);
+      tmem_ld_wait();
+      __syncwarp();
+      if (bf16) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) put[i * 32] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(v[i]) * f.a * f.b));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) put[i * 32] = __half_as_ushort(__float2half_rn(__uint_as_float(v[i]) * f.a * f.b));
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + i * 8 + (lane >> 2) < t.rows) *reinterpret_cast<uint4*>(y + (long long)(c0 + i * 8) * J.y_stride) = *reinterpret_cast<const uint4*>(get + i * 512);
+    }
+    return;
   }
 #pragma unroll 1
-  for (int c0 = 0; c0 < t.rows; c0 += 32) {
-    uint32_t v[32];
-    tmem_ld32(acc + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0, v);
+  for (int c0 = 0; c0 < t.rows; c0 += 8) {
+    uint32_t v[8];
+    tmem_ld8(acc + (uint32_t)c0, v);
     tmem_ld_wait();
-    if (red) {
+    if (row >= J.m) continue;
+    const long long at = (long long)(t.row0 + c0) * J.y_stride + row;
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c0 + i < t.rows) red[(c0 + i) * MX4_ROWS + r] = __uint_as_float(v[i]);
-    } else if (row < J.m) {
-      const long long at = (long long)(t.row0 + c0) * J.y_stride + row;
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c0 + i < t.rows) mx4_put(J, at + i * J.y_stride, __uint_as_float(v[i]) * f.a * f.b);
-    }
+    for (int i = 0; i < 8; ++i)
+      if (c0 + i < t.rows) mx4_put(J, at + i * J.y_stride, __uint_as_float(v[i]) * f.a * f.b);
   }
 }
 // The cluster's parts of a tile, added in rank order; the columns are shared out over the CTAs.
@@ -114,9 +165,7 @@ template <int FMT, typename T, bool QUANT>
 __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int mt, float* red, int rank) {
   const int r = threadIdx.x % MX4_ROWS, row = mt * MX4_ROWS + r;
   if (row >= J.m) return;
-  Mx4Factor f{1.0f, 1.0f};
-  if constexpr (!QUANT) f = mx4_row_factor<FMT, T>(J, t.expert, row);
-  else if constexpr (FMT == GLQB_MX4_NVFP4) f = Mx4Factor{J.w_scale[t.expert], *J.x_scale};
+  const Mx4Factor f = row_factor<FMT, T, QUANT>(J, t.expert, row);
   const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
   for (int c = rank + J.split * (int)(threadIdx.x / MX4_ROWS); c < t.rows; c += J.split * (int)(blockDim.x / MX4_ROWS)) {
     float v = 0.0f;
@@ -277,7 +326,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       if (!mbar_wait(&B.acc_full[seq & 1u], (seq >> 1) & 1u, &B.abort)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      drain_tile<FMT, T, false>(J, t, i % J.m_tiles, tmem + (seq & 1u) * G16_MAX_TN, warp & 3, lane, J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
+      drain_tile<FMT, T, false>(J, t, i % J.m_tiles, tmem + (seq & 1u) * G16_MAX_TN, warp & 3, lane, B.turn[warp & 3], J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.acc_empty[seq & 1u]);
@@ -423,7 +472,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
       if (!mbar_wait(&B.acc_full[seq & 1u], (seq >> 1) & 1u, &B.abort)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      drain_tile<FMT, __half, true>(J, t, i % J.m_tiles, tmem + (seq & 1u) * C::MAX_TN, warp & 3, lane, J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
+      drain_tile<FMT, __half, true>(J, t, i % J.m_tiles, tmem + (seq & 1u) * C::MAX_TN, warp & 3, lane, B.turn[warp & 3], J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.acc_empty[seq & 1u]);

@@ -20,6 +20,7 @@ struct Mx4Job {
   void* y;
   long long y_stride;
   int y_dtype, accumulate;
+  bool y_wide;                // 16-bit results whose rows lie on 16 bytes, nothing to add
   const void* x;              // 16-bit activations
   long long x_stride;
   uint8_t* x_image;           // 4-bit activations: per token tile, per 256 values: tn rows of 128 bytes, then the scales
