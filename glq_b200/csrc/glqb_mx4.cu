@@ -399,7 +399,7 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
 // What a call launches, by its sizes alone.
 struct Form {
   int tn, max_tiles, split, x_scales, n_pad;
-  bool align;
+  bool align, mv;
   size_t image, bytes;        // of the workspace: x in 4 bits or aligned, then two floats
 };
 static int sm_count() {
@@ -413,12 +413,16 @@ static int sm_count() {
   }
   return n;
 }
+constexpr int MV_MAX_ROWS = 16;     // rows (an expert's, on average) up to which the streaming kernel runs
 static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, int sms) {
   Form f = {};
-  const int most = quantize ? (w->format == GLQB_MX4_MXFP4 ? 192 : 160) : 192, per = (int)((rows + w->experts - 1) / w->experts);
+  const int avg = (int)((rows + w->experts - 1) / w->experts);
+  f.mv = !quantize && avg <= MV_MAX_ROWS;
+  const int most = quantize ? (w->format == GLQB_MX4_MXFP4 ? 192 : 160) : 192;
   // token tiles: a matrix's rows split evenly; of experts up to twice their average, so that most have one tile
-  if (w->experts == 1) f.tn = (int)(((rows + (rows + most - 1) / most - 1) / ((rows + most - 1) / most) + 15) / 16 * 16);
-  else f.tn = std::min(most, (2 * per + 15) / 16 * 16);
+  if (f.mv) f.tn = avg > (w->experts == 1 ? 8 : 4) ? 16 : 8;
+  else if (w->experts == 1) f.tn = (int)(((rows + (rows + most - 1) / most - 1) / ((rows + most - 1) / most) + 15) / 16 * 16);
+  else f.tn = std::min(most, (2 * avg + 15) / 16 * 16);
   f.max_tiles = w->experts == 1 ? (int)((rows + f.tn - 1) / f.tn) : (int)(rows / f.tn + std::min<long long>(w->experts, rows));
   const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K, tiles = f.max_tiles * mt;
   f.split = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, kt), sms / std::max<long long>(1, tiles)));
@@ -426,7 +430,7 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
     f.x_scales = mx4_x_scale_bytes(w->format, f.tn);
     f.image = (size_t)f.max_tiles * kt * ((size_t)f.tn * 128 + f.x_scales);
     f.bytes = f.image + 256;
-  } else if (reinterpret_cast<uintptr_t>(x) % 16 || (rows > 1 && x_stride % 8)) {
+  } else if (reinterpret_cast<uintptr_t>(x) % 16 || (rows > 1 && x_stride % 8) || (f.mv && w->n % 8)) {
     f.align = true;
     f.n_pad = (w->n + 7) / 8 * 8;
     f.bytes = (size_t)rows * f.n_pad * 2;
@@ -491,6 +495,11 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
       mx4_align_kernel<<<grid_for(rows * f.n_pad), 256, 0, stream>>>((const uint16_t*)x, x_stride, rows, w->n, f.n_pad, (uint16_t*)workspace);
       J.x = workspace;
       J.x_stride = f.n_pad;
+    }
+    if (f.mv) {
+      if (f.align) J.n = f.n_pad;
+      e = mx4_mv_launch(w->format, x_dtype == GLQB_DT_BF16, J, sms, stream);
+      return e == cudaSuccess ? GLQB_OK : mx4_fail(GLQB_E_CUDA, "mx4_product: %s", cudaGetErrorString(e));
     }
     const char* what = nullptr;
     e = mx4_gemm16_launch(w->format, x_dtype == GLQB_DT_BF16, J, sms, stream, &what);

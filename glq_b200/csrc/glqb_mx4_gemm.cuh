@@ -147,6 +147,9 @@ __device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert,
 }
 #endif  // __CUDACC__
 
+// ---- glqb_mx4_mv.cu
+// Few rows of x (tn 8 or 16), which start on 16 bytes and end on whole eights of values.
+cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& job, int sm_count, cudaStream_t stream);
 // ---- glqb_mx4_gemm.cu
 // `x_bf16`: type of 16-bit activations.  Rows of x start on 16 bytes.
 cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& job, int sm_count, cudaStream_t stream, const char** what);
