@@ -189,20 +189,23 @@ __global__ void __launch_bounds__(256) mx4_pack_kernel(const uint8_t* __restrict
     tile[MX4_CODE_BYTES + mx4_scale_offset(r, b)] = row < m && col < scale_row ? scales[(e * m + row) * scale_row + col] : 0;
   }
 }
-// MXFP4: the largest scale byte of every row that is a number
+// MXFP4: the largest scale byte of every row that is a number; + 256 for rows that have one that is none, or so large a one that a
+// multiplier by 2^(s - largest) may leave the exponents of bf16
 __global__ void __launch_bounds__(256) mx4_row_top_kernel(const uint8_t* __restrict__ scales, long long rows, int m, int m_pad, int scale_row,
-                                                          uint8_t* __restrict__ tops) {
+                                                          uint16_t* __restrict__ tops) {
   const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;          // of experts x m_pad
   if (row >= rows) return;
   const int r = (int)(row % m_pad);
-  uint32_t top = 0;
+  uint32_t top = 0, nan = 0;
   if (r < m)
     for (int c = threadIdx.x % 32; c < scale_row; c += 32) {
       const uint32_t s = scales[(row / m_pad * m + r) * scale_row + c];
       top = s < 255u ? max(top, s) : top;
+      nan |= s == 255u;
     }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
-  if (threadIdx.x % 32 == 0) tops[row] = (uint8_t)top;
+  nan = __any_sync(0xFFFFFFFFu, nan);
+  if (threadIdx.x % 32 == 0) tops[row] = (uint16_t)(top | (nan || top > 252u ? 256u : 0u));
 }
 
 // ---- activations of the products ------------------------------------------------------------------
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(256) mx4_x_image_kernel(const __grid_constant_
   const long long stage = (long long)J.tn * 128 + x_scales;
   for (int row = eff[0] + blockIdx.x * 8 + (threadIdx.x >> 5); row < end; row += gridDim.x * 8) {
     const int e = J.experts == 1 ? 0 : mx4_find(eff, J.experts, row), in = row - eff[e];
-    const int per = mx4_per_tile(eff[e + 1] - eff[e], pre[e + 1] - pre[e]), tile = pre[e] + in / per, r = in % per;
+    const int per = mx4_per_tile(J.tn, eff[e + 1] - eff[e], pre[e + 1] - pre[e]), tile = pre[e] + in / per, r = in % per;
     if (tile >= J.max_tiles) continue;
     uint8_t* at = J.x_image + (long long)tile * J.k_tiles * stage;
     uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
@@ -372,7 +375,7 @@ int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tens
 size_t glqb_mx4_image_bytes(int32_t format, int32_t experts, int32_t m, int32_t n) {
   if (!format_ok(format) || experts < 1 || m < 1 || n < 1) return 0;
   const size_t mt = ((size_t)m + MX4_ROWS - 1) / MX4_ROWS, kt = ((size_t)n + MX4_K - 1) / MX4_K;
-  return (size_t)experts * mt * (kt * mx4_tile_bytes(format) + (format == GLQB_MX4_MXFP4 ? MX4_ROWS : 0));
+  return (size_t)experts * mt * (kt * mx4_tile_bytes(format) + (format == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0));
 }
 
 int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t experts, int32_t m, int32_t n, void* image,
@@ -389,7 +392,7 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
     mx4_pack_kernel<GLQB_MX4_MXFP4><<<(unsigned)tiles, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, m, n, kt, mt, (uint8_t*)image);
     const long long rows = (long long)experts * mt * MX4_ROWS;
     mx4_row_top_kernel<<<(unsigned)(rows / 8), 256, 0, stream>>>((const uint8_t*)scales, rows, m, mt * MX4_ROWS, (n + 31) / 32,
-                                                                 (uint8_t*)image + tiles * mx4_tile_bytes(format));
+                                                                 (uint16_t*)((uint8_t*)image + tiles * mx4_tile_bytes(format)));
   } else {
     mx4_pack_kernel<GLQB_MX4_NVFP4><<<(unsigned)tiles, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, m, n, kt, mt, (uint8_t*)image);
   }
@@ -425,7 +428,8 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
   else f.tn = std::min(most, (2 * avg + 15) / 16 * 16);
   f.max_tiles = w->experts == 1 ? (int)((rows + f.tn - 1) / f.tn) : (int)(rows / f.tn + std::min<long long>(w->experts, rows));
   const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K, tiles = f.max_tiles * mt;
-  f.split = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, kt), sms / std::max<long long>(1, tiles)));
+  // CTAs that share a tile's sum: as many as the SMs hold at once
+  f.split = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, kt), (f.mv ? 2 : 1) * sms / std::max<long long>(1, tiles)));
   if (quantize) {
     f.x_scales = mx4_x_scale_bytes(w->format, f.tn);
     f.image = (size_t)f.max_tiles * kt * ((size_t)f.tn * 128 + f.x_scales);
@@ -471,7 +475,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.m_tiles = (w->m + MX4_ROWS - 1) / MX4_ROWS;
   J.k_tiles = (w->n + MX4_K - 1) / MX4_K;
   J.image = (const uint8_t*)w->image;
-  J.tops = J.image + (size_t)w->experts * J.m_tiles * J.k_tiles * mx4_tile_bytes(w->format);
+  J.tops = (const uint16_t*)(J.image + (size_t)w->experts * J.m_tiles * J.k_tiles * mx4_tile_bytes(w->format));
   J.w_scale = w->tensor_scale;
   J.offsets = offsets;
   J.wide = offsets_are_int64;

@@ -11,7 +11,7 @@
 // is block i of row r, which is how tcgen05.cp hands scales to tensor memory.  The eight codes of a 32-bit word lie in the order
 // 0 2 4 6 1 3 5 7: values 2i and 2i + 1 are nibbles i and i + 4, so that one shift and mask bring a pair to the halves of
 // a register.  (The 4-bit products do not see it: both operands have that order, and a word never leaves its block.)
-// Behind the tiles: for MXFP4 one byte per row, the largest scale of the row (see mx4_operand_scale).
+// Behind the tiles: for MXFP4 two bytes per row, the largest scale of the row, which 16-bit operands are held relative to.
 #pragma once
 #include "glqb_internal.h"
 #include <cuda_fp8.h>

@@ -68,17 +68,6 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) 
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
   return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
-}
-
 // fp32 accumulator, both operands K-major, M = 128; `type` 0: fp16, 1: bf16
 __device__ __forceinline__ uint32_t idesc16(int type, int cols) {
   return (1u << 4) | (uint32_t)type << 7 | (uint32_t)type << 10 | (uint32_t)(cols >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
@@ -168,8 +157,7 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int
   const Mx4Factor f = row_factor<FMT, T, QUANT>(J, t.expert, row);
   const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
   for (int c = rank + J.split * (int)(threadIdx.x / MX4_ROWS); c < t.rows; c += J.split * (int)(blockDim.x / MX4_ROWS)) {
-    float v = 0.0f;
-    for (int s = 0; s < J.split; ++s) v += ld_cluster(base + (uint32_t)(c * MX4_ROWS * 4), s);
+    const float v = sum_cluster(base + (uint32_t)(c * MX4_ROWS * 4), J.split);
     mx4_put(J, (long long)(t.row0 + c) * J.y_stride + row, v * f.a * f.b);
   }
 }
@@ -205,6 +193,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     tmem_relinquish();
   }
   tc_fence_before();
+  if (J.offsets) pdl_wait();
   mx4_groups(J, eff, pre);                         // (ends with a block barrier)
   tc_fence_after();
   const uint32_t tmem = B.tmem;
@@ -256,6 +245,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
             bulk_g2s(w_base + s * mx4_tile_bytes(FMT), src + (long long)(k >> 1) * mx4_tile_bytes(FMT), mx4_tile_bytes(FMT), &B.full_w[s]);
             ++loads_w;
           }
+          if (loads_x == 0) pdl_wait();            // (the weights do not depend on what runs in front of this call)
           const uint32_t s = loads_x % R.x_stages;
           if (!mbar_wait(&B.empty_x[s], ((loads_x / R.x_stages) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
           mbar_expect_tx(&B.full_x[s], (uint32_t)(2 * boxes * R.box_rows * 128));
@@ -276,7 +266,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       int top = 0;
       if constexpr (FMT == GLQB_MX4_MXFP4) {
         const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-        top = J.tops[((long long)t.expert * J.m_tiles + i % J.m_tiles) * MX4_ROWS + r];
+        top = J.tops[((long long)t.expert * J.m_tiles + i % J.m_tiles) * MX4_ROWS + r] & 0xFF;
       }
       for (int k = 0; k < steps; ++k, ++q) {
         const uint32_t s = wq % G16_W_STAGES, sa = q & 1u;
@@ -300,9 +290,12 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
             m1 = mx4_multiplier<FMT, T>((sw >> (16 * u + 8)) & 0xFFu, 0);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j) {
+            uint32_t r[4];
+            mx4_pairs<T>(w[j], r);
 #pragma unroll
-            for (int p = 0; p < 4; ++p) a[u * 16 + j * 4 + p] = mx4_mul2<T>(mx4_pair<T>(w[j], p), j < 2 ? m0 : m1);
+            for (int p = 0; p < 4; ++p) a[u * 16 + j * 4 + p] = mx4_mul2<T>(r[p], j < 2 ? m0 : m1);
+          }
         }
         if ((k & 1) == 1 || k + 1 == steps) {      // done with this tile of weights
           __syncwarp();
@@ -320,6 +313,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     }
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER); }
   } else if (warp >= 4) {
+    pdl_wait();                                    // (y may still be in use)
     uint32_t seq = 0;
     for (int i = first; i < tiles && ok; i += step, ++seq) {
       const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
@@ -400,6 +394,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
     tmem_relinquish();
   }
   tc_fence_before();
+  pdl_wait();
   mx4_groups(J, eff, pre);
   tc_fence_after();
   const uint32_t tmem = B.tmem;
@@ -506,25 +501,6 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   }
 }
 
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
-  // (per device and idempotent: a word of the runtime, no synchronisation)
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
@@ -563,7 +539,7 @@ cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_c
   if (r != CUDA_SUCCESS) { *what = "cuTensorMapEncodeTiled refused the activations"; return cudaErrorInvalidValue; }
   const long long tiles = (long long)J.max_tiles * J.m_tiles;
   const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
-  auto run = [&](auto* kernel) { return launch(kernel, grid, G16_THREADS, smem, J.split, stream, J, map, R); };
+  auto run = [&](auto* kernel) { return mx4_launch(kernel, grid, G16_THREADS, smem, J.split, stream, J, map, R); };
   if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(mx4_gemm16_kernel<GLQB_MX4_MXFP4, __nv_bfloat16>) : run(mx4_gemm16_kernel<GLQB_MX4_MXFP4, __half>);
   return x_bf16 ? run(mx4_gemm16_kernel<GLQB_MX4_NVFP4, __nv_bfloat16>) : run(mx4_gemm16_kernel<GLQB_MX4_NVFP4, __half>);
 }
@@ -575,7 +551,7 @@ cudaError_t mx4_gemm4_launch(int format, const Mx4Job& J, int sm_count, cudaStre
   const long long tiles = (long long)J.max_tiles * J.m_tiles;
   const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
   const size_t smem = std::max(ONE_PER_SM, fixed + stages * stage);
-  auto run = [&](auto* kernel) { return launch(kernel, grid, G4_THREADS, smem, J.split, stream, J, stages, x_scales); };
+  auto run = [&](auto* kernel) { return mx4_launch(kernel, grid, G4_THREADS, smem, J.split, stream, J, stages, x_scales); };
   return format == GLQB_MX4_MXFP4 ? run(mx4_gemm4_kernel<GLQB_MX4_MXFP4>) : run(mx4_gemm4_kernel<GLQB_MX4_NVFP4>);
 }
 

@@ -2,6 +2,7 @@
 #pragma once
 #include "glqb_mx4.cuh"
 #include "glqb_ptx.cuh"
+#include "glqb_launch.h"
 
 namespace glqb {
 
@@ -9,7 +10,7 @@ constexpr int MX4_MAX_EXPERTS = 1024;
 
 struct Mx4Job {
   const uint8_t* image;
-  const uint8_t* tops;        // MXFP4: largest scale byte of every row (experts x m_tiles * 128)
+  const uint16_t* tops;       // MXFP4: of every row (experts x m_tiles * 128) the largest scale byte, + 256: see mx4_row_top_kernel
   const float* w_scale;       // NVFP4: fp32 scale per expert
   const float* x_scale;       // 4-bit activations, NVFP4: theirs
   const void* offsets;        // null: one matrix, all rows
@@ -28,6 +29,27 @@ struct Mx4Job {
 };
 
 #ifdef __CUDACC__
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+
+// a value of every CTA of the cluster, added in rank order (all loads before the first sum)
+__device__ __forceinline__ float sum_cluster(uint32_t addr, int ranks) {
+  float v[8];
+#pragma unroll
+  for (int s = 0; s < 8; ++s) v[s] = s < ranks ? ld_cluster(addr, s) : 0.0f;
+  float sum = v[0];
+#pragma unroll
+  for (int s = 1; s < 8; ++s) sum += v[s];
+  return sum;
+}
 // Rows of every expert and the token tiles in front of it.  offsets are held to 0 .. rows and to ascend (each at least
 // the largest before it), so that whatever they hold, experts do not overlap and the tiles are no more than max_tiles.
 // Called by all threads; `eff` and `pre` have experts + 1 entries in shared memory.
@@ -78,10 +100,10 @@ __device__ __forceinline__ int mx4_find(const int* list, int experts, int v) {
 // Token tile t: an expert's rows are split evenly over as few tiles as they need, in steps of 16 (no tile is empty: the tiles
 // before the last hold fewer than the expert has).
 struct Mx4Tile { int expert, row0, rows; };
-__device__ __forceinline__ int mx4_per_tile(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) & ~15; }
+__device__ __forceinline__ int mx4_per_tile(int tn, int rows, int tiles) { return tn <= 16 ? tn : ((rows + tiles - 1) / tiles + 15) & ~15; }
 __device__ __forceinline__ Mx4Tile mx4_tile(const Mx4Job& J, const int* eff, const int* pre, int t) {
   const int e = J.experts == 1 ? 0 : mx4_find(pre, J.experts, t);
-  const int rows = eff[e + 1] - eff[e], per = mx4_per_tile(rows, pre[e + 1] - pre[e]), at = (t - pre[e]) * per;
+  const int rows = eff[e + 1] - eff[e], per = mx4_per_tile(J.tn, rows, pre[e + 1] - pre[e]), at = (t - pre[e]) * per;
   return Mx4Tile{e, eff[e] + at, min(per, rows - at)};
 }
 
@@ -105,19 +127,33 @@ __device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) 
 //   MXFP4  value * 2^(s - top) (bf16), value * 2^(s - top + 1) (fp16), top the largest scale byte of the row
 //   NVFP4  value * s * 2^-7
 // and mx4_row_factor is what the sums are multiplied by.
+// The four pairs of a word, unscaled: r[i] holds values 2i and 2i + 1.  Logic and right shifts issue at half an instruction a clock,
+// and so do integer products (left shifts), on a pipe of their own.  In bf16 two of the pairs are therefore brought to bits 9:6 of
+// each half and copied to 15:12 by a product with 65, the others masked at 15:12 and shifted down: ten instructions on the one
+// pipe and four on the other per word, where all pairs the second way are twelve and three.  In fp16 the two places share a bit,
+// which a product would carry out of.
 template <typename T>
-__device__ __forceinline__ uint32_t mx4_pair(uint32_t w, int i) {       // values 2i, 2i + 1 of a word
-  const uint32_t x = (i == 3 ? w : w << (12 - 4 * i)) & 0xF000F000u;
-  if constexpr (__is_same(T, __half)) return (x | x >> 3) & 0x8E008E00u;
-  else return (x | x >> 6) & 0x81C081C0u;
+__device__ __forceinline__ void mx4_pairs(uint32_t w, uint32_t (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (__is_same(T, __half)) {
+      const uint32_t x = (i == 3 ? w : w << (12 - 4 * i)) & 0xF000F000u;
+      r[i] = (x | x >> 3) & 0x8E008E00u;
+    } else if (i < 2) {
+      r[i] = (((w << (6 - 4 * i)) & 0x03C003C0u) * 65u) & 0x81C081C0u;
+    } else {
+      const uint32_t x = (i == 3 ? w : w << 4) & 0xF000F000u;
+      r[i] = (x | x >> 6) & 0x81C081C0u;
+    }
+  }
 }
 template <int FMT, typename T>
 __device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {   // in both halves
   uint32_t h;
   if constexpr (FMT == GLQB_MX4_MXFP4) {
     const int d = (int)s - top;
-    if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : d > -30 ? (uint32_t)(d + 30) << 10 : d >= -39 ? 1u << (d + 39) : 0u;
-    else h = s == 255u ? 0x7FC0u : d > -253 ? (uint32_t)(d + 253) << 7 : 0u;
+    if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : (uint32_t)max(d + 30, 0) << 10;
+    else h = s == 255u ? 0x7FC0u : (uint32_t)max(d + 253, 0) << 7;
   } else {
     const float f = mx4_e4m3(s);
     if constexpr (__is_same(T, __half)) h = __half_as_ushort(__float2half_rn(f * 128.0f));
@@ -139,13 +175,35 @@ struct Mx4Factor { float a, b; };     // two factors: 2^-127 and 2^127 have no s
 template <int FMT, typename T>
 __device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert, int row) {
   if constexpr (FMT == GLQB_MX4_MXFP4) {
-    const int p = (int)J.tops[(long long)expert * J.m_tiles * MX4_ROWS + row] - (__is_same(T, __half) ? 128 : 127), h = p >> 1;
+    const int p = (int)(J.tops[(long long)expert * J.m_tiles * MX4_ROWS + row] & 0xFFu) - (__is_same(T, __half) ? 128 : 127), h = p >> 1;
     return Mx4Factor{__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(p - h + 127) << 23)};
   } else {
     return Mx4Factor{128.0f, J.w_scale[expert]};
   }
 }
 #endif  // __CUDACC__
+
+// Chained to the kernel in front (launch_chained), `cluster` CTAs per cluster.
+template <typename... P, typename... A>
+inline cudaError_t mx4_launch(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
+  // (per device and idempotent: a word of the runtime, no synchronisation)
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 
 // ---- glqb_mx4_mv.cu
 // Few rows of x (tn 8 or 16), which start on 16 bytes and end on whole eights of values.

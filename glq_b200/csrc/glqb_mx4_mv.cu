@@ -1,11 +1,14 @@
 // Products of microscaled 4-bit weights with few rows of x: decode steps, experts of few tokens.
 //
-// What bounds these is the weights' way from HBM and, close behind, the instructions that make 16-bit operands of them.  A warp
-// streams 16 rows x 256 values at a time (four 16-byte loads per lane, the next four under way), turns them into fragments of
-// mma.sync.m16n8k16 in registers (five instructions per two weights) and multiplies them with 8 NB rows of x.  The MMA's order
-// of values is free as long as both operands have it: lane t of a quad takes the 16-byte unit t of a weight row, 32 values, and
-// of each row of x the same 32 values, so nothing is exchanged.  The eight warps of a CTA share out the values of a strip of 16
-// rows; their sums are added in warp order.  A CTA takes strips in turn, its loads running ahead over the strips' borders.
+// What bounds these is the weights' way from HBM and, close behind, the instructions that make 16-bit operands of them (about
+// 430 per warp for 16 rows x 256 values, five per two weights).  A CTA takes 128 weight rows x 8 NB rows of x; one warp brings
+// tiles of 128 x 256 weights with the rows of x that belong to them into a ring of stages (bulk copies), and runs ahead over the
+// borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile into fragments of mma.sync.m16n8k16 in registers and
+// multiply.  The MMA's order of values is free as long as both operands have it: lane t of a quad takes word t of a 16-byte unit, eight
+// values, and of x the same eight, so nothing is exchanged and every shared-memory access is free of conflicts.  Where there
+// are few tiles the CTAs of a cluster share out the values and add their parts in rank order.
+// Lanes that read weights from global memory (a CTA's warps sharing out the values): one token of 14336 x 4096 14.5 us,
+// sixteen 25.4, 256 rows over 128 experts of 1536 x 2048 83 us: rows of x came from L1 with sixteen lines per load.
 #include "glqb_mx4_gemm.cuh"
 #include "glqb_launch.h"
 #include <algorithm>
@@ -13,193 +16,222 @@
 namespace glqb {
 namespace {
 
-constexpr int MV4_WARPS = 8, MV4_THREADS = MV4_WARPS * 32, MV4_ROWS = 16;
+constexpr int MV4_WARPS = 8, MV4_THREADS = (MV4_WARPS + 1) * 32;
+constexpr int MV4_X_ROW = MX4_K * 2 + 64;        // bytes of a row of x in a stage: eight rows in all the banks
+template <int FMT, int NB> struct Mv4 {
+  static constexpr int STAGE = mx4_tile_bytes(FMT) + 8 * NB * MV4_X_ROW;
+  static constexpr int STAGES = NB == 1 ? 4 : 3;                       // two CTAs per SM
+};
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (__is_same(T, __half))
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 
-// The token tile of a CTA: an expert and up to tn of its rows.  All threads; a range that ends before it begins is empty.
-__device__ __forceinline__ bool mv4_tile(const Mx4Job& J, int tile, Mx4Tile& t) {
-  if (!J.offsets) {
-    t = Mx4Tile{0, tile * J.tn, min(J.tn, J.rows - tile * J.tn)};
-    return t.rows > 0;
-  }
-  __shared__ int sums[MV4_WARPS], found[3];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int begin[4], rows[4], mine = 0;                       // four experts per thread: MX4_MAX_EXPERTS
-  const int e0 = threadIdx.x * 4;
+// The multipliers of a row's blocks that lane t meets in the 16-byte units 2i and 2i + 1, from the word of scales that holds them.
+// MXFP4: bytes 2i % 4 and + 1.  NVFP4: bytes t / 2 and t / 2 + 2 of word i.
+template <int FMT, typename T>
+__device__ __forceinline__ void multipliers(uint32_t word, int i, int top, bool odd, uint32_t pick, uint32_t (&m)[2]) {
+  if constexpr (FMT == GLQB_MX4_MXFP4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    begin[i] = rows[i] = 0;
-    const int e = e0 + i;
-    if (e < J.experts) {
-      const long long b = J.wide ? reinterpret_cast<const long long*>(J.offsets)[e] : reinterpret_cast<const int*>(J.offsets)[e];
-      const long long f = J.wide ? reinterpret_cast<const long long*>(J.offsets)[e + 1] : reinterpret_cast<const int*>(J.offsets)[e + 1];
-      begin[i] = (int)max(0ll, min((long long)J.rows, b));
-      rows[i] = (int)max(0ll, min((long long)J.rows, f)) - begin[i];
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t s = (word >> (8 * (2 * (i & 1) + u))) & 0xFFu;
+      if (__is_same(T, __half) || odd) m[u] = mx4_multiplier<FMT, T>(s, top);
+      else m[u] = s * 0x00800080u + (uint32_t)(253 - top) * 0x00800080u;
     }
-    mine += (max(rows[i], 0) + J.tn - 1) / J.tn;
-  }
-  int upto = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int u = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-    if (lane >= d) upto += u;
-  }
-  if (lane == 31) sums[warp] = upto;
-  if (threadIdx.x == 0) found[2] = 0;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) upto += sums[w];
-  int at = tile - (upto - mine);
-  if (at >= 0 && at < mine) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = (max(rows[i], 0) + J.tn - 1) / J.tn;
-      if (at >= 0 && at < n) {
-        found[0] = e0 + i;
-        found[1] = begin[i] + at * J.tn;
-        found[2] = min(J.tn, rows[i] - at * J.tn);
-      }
-      at -= n;
+  } else {
+    const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)__byte_perm(word, 0, pick), __NV_E4M3));
+    if constexpr (__is_same(T, __half)) {
+      const __half2 r = __hmul2(h, __float2half2_rn(128.0f));
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(&r);
+      m[0] = __byte_perm(b, 0, 0x1010);
+      m[1] = __byte_perm(b, 0, 0x3232);
+    } else {
+      const float2 f = __half22float2(h);
+      m[0] = __byte_perm(__float_as_uint(f.x * 0x1p119f), 0, 0x3232);
+      m[1] = __byte_perm(__float_as_uint(f.y * 0x1p119f), 0, 0x3232);
     }
   }
-  __syncthreads();
-  t = Mx4Tile{found[0], found[1], found[2]};
-  return t.rows > 0;
 }
-
-template <int FMT>
-struct Mv4Item {               // 16 rows x 256 values: rows g and g + 8, 16-byte units t and t + 4, and their scales
-  uint4 w[2][2];
-  uint32_t s[2][2];
-  __device__ __forceinline__ void load(const uint8_t* tile, int r, int t) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = r + 8 * h;
-      const uint8_t* codes = tile + (row >> 3) * 1024 + (row & 7) * 128;
-      const uint8_t* scales = tile + MX4_CODE_BYTES + (row & 31) * 16 + (row >> 5) * 4;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        w[h][u] = ld_stream(codes + (((t + 4 * u) ^ (row & 7)) << 4));
-        if constexpr (FMT == GLQB_MX4_MXFP4) s[h][u] = __ldg(scales + u * 512 + t);
-        else s[h][u] = __ldg(reinterpret_cast<const uint16_t*>(scales + (2 * u + (t >> 1)) * 512 + (t & 1) * 2));
-      }
-    }
-  }
-};
 
 template <int FMT, typename T, int NB>
-__global__ void __launch_bounds__(MV4_THREADS, NB == 1 ? 3 : 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J, int strips) {
-  __shared__ float red[2][MV4_WARPS][8 * NB][MV4_ROWS];
-  Mx4Tile tile;
-  if (!mv4_tile(J, blockIdx.y, tile)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint8_t* image = J.image + (long long)tile.expert * J.m_tiles * J.k_tiles * mx4_tile_bytes(FMT);
-  const T* x = reinterpret_cast<const T*>(J.x) + (long long)tile.row0 * J.x_stride;
-  auto tile_of = [&](int strip, int k) -> const uint8_t* { return image + ((long long)(strip >> 3) * J.k_tiles + k) * mx4_tile_bytes(FMT); };
-
-  int strip = blockIdx.x, k = warp;
-  Mv4Item<FMT> next;
-  if (k < J.k_tiles) next.load(tile_of(strip, k), (strip & 7) * MV4_ROWS + g, t);
-  for (int turn = 0; strip < strips; ++turn) {
-    float acc[NB][4] = {};
-    int top[2] = {0, 0};
-    if constexpr (FMT == GLQB_MX4_MXFP4) {
-      const uint8_t* p = J.tops + ((long long)tile.expert * J.m_tiles * MX4_ROWS) + strip * MV4_ROWS + g;
-      top[0] = p[0];
-      top[1] = p[8];
-    }
-    const int after = strip + gridDim.x;
-#pragma unroll 1
-    for (; k < J.k_tiles; ) {
-      Mv4Item<FMT> it = next;
-      const int kt = k;
-      k += MV4_WARPS;
-      if (k < J.k_tiles) next.load(tile_of(strip, k), (strip & 7) * MV4_ROWS + g, t);
-      else if (after < strips) next.load(tile_of(after, warp), (after & 7) * MV4_ROWS + g, t);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int col = kt * MX4_K + (t + 4 * u) * 32;
-        uint32_t m[2][2];                                // multipliers of rows g and g + 8, of the first and last 16 values
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (FMT == GLQB_MX4_MXFP4) m[h][0] = m[h][1] = mx4_multiplier<FMT, T>(it.s[h][u], top[h]);
-          else {
-            m[h][0] = mx4_multiplier<FMT, T>(it.s[h][u] & 0xFFu, 0);
-            m[h][1] = mx4_multiplier<FMT, T>(it.s[h][u] >> 8, 0);
-          }
-        }
-        const uint32_t w[2][4] = {{it.w[0][u].x, it.w[0][u].y, it.w[0][u].z, it.w[0][u].w}, {it.w[1][u].x, it.w[1][u].y, it.w[1][u].z, it.w[1][u].w}};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                    // eight values: two MMAs
-          uint4 b[NB];
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            b[i] = make_uint4(0, 0, 0, 0);
-            if (i * 8 + g < tile.rows && col + j * 8 < J.n) b[i] = *reinterpret_cast<const uint4*>(x + (long long)(i * 8 + g) * J.x_stride + col + j * 8);
-          }
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            uint32_t a[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) a[q] = mx4_mul2<T>(mx4_pair<T>(w[q & 1][j], 2 * p + (q >> 1)), m[q & 1][j >> 1]);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) mma16816<T>(acc[i], a, p ? b[i].z : b[i].x, p ? b[i].w : b[i].y);
-          }
-        }
-      }
-    }
-    // (two buffers in turn: a strip's sums are read before the barrier of the next one's)
-    auto& mine = red[turn & 1];
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) mine[warp][i * 8 + 2 * t + (q & 1)][g + 8 * (q >> 1)] = acc[i][q];
-    __syncthreads();
-    for (int o = threadIdx.x; o < tile.rows * MV4_ROWS; o += MV4_THREADS) {
-      const int r = o % MV4_ROWS, c = o / MV4_ROWS, row = strip * MV4_ROWS + r;
-      float v = 0.0f;
-#pragma unroll
-      for (int s = 0; s < MV4_WARPS; ++s) v += mine[s][c][r];
-      if (row < J.m) {
-        const Mx4Factor f = mx4_row_factor<FMT, T>(J, tile.expert, row);
-        mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, v * f.a * f.b);
-      }
-    }
-    strip = after;
-    k = warp;
+__global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J) {
+  constexpr int TILE = mx4_tile_bytes(FMT), STAGE = Mv4<FMT, NB>::STAGE, STAGES = Mv4<FMT, NB>::STAGES;
+  extern __shared__ __align__(128) uint8_t ring[];
+  float* red = reinterpret_cast<float*>(ring + STAGES * STAGE);                      // [8 NB][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(red + 8 * NB * MX4_ROWS);
+  uint64_t* empty = full + STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
+  int* eff = const_cast<int*>(abort_flag) + 2;
+  int* pre = eff + J.experts + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); }
+    *abort_flag = 0;
+    fence_mbar_init();
   }
+  if (J.offsets) pdl_wait();
+  mx4_groups(J, eff, pre);                               // (ends with a block barrier)
+  pdl_trigger();
+  const int tiles = min(pre[J.experts], J.max_tiles) * J.m_tiles;
+  const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
+  const int k0 = rank * J.k_tiles / J.split, k1 = (rank + 1) * J.k_tiles / J.split;
+  uint32_t q = 0;                                        // stages so far
+  bool ok = true, waited = false;
+
+  if (warp == MV4_WARPS) {
+    for (int i = first; i < tiles && ok; i += step) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
+      const uint8_t* w = J.image + ((long long)t.expert * J.m_tiles + i % J.m_tiles) * J.k_tiles * TILE;
+      const uint8_t* x = reinterpret_cast<const uint8_t*>(J.x) + (long long)(t.row0 + min(lane, t.rows - 1)) * J.x_stride * 2;
+      for (int k = k0; k < k1; ++k, ++q) {
+        const uint32_t s = q % STAGES, x_bytes = (uint32_t)min(MX4_K, J.n - k * MX4_K) * 2u;
+        if (!mbar_wait(&empty[s], ((q / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        uint8_t* to = ring + s * STAGE;
+        if (lane == 0) {
+          mbar_expect_tx(&full[s], TILE + (uint32_t)t.rows * x_bytes);
+          bulk_g2s(to, w + (long long)k * TILE, TILE, &full[s]);
+        }
+        __syncwarp();
+        if (!waited) pdl_wait();                         // (the weights do not depend on what runs in front of this call)
+        waited = true;
+        if (lane < t.rows) bulk_g2s(to + TILE + lane * MV4_X_ROW, x + (long long)k * MX4_K * 2, x_bytes, &full[s]);
+      }
+    }
+    if (!ok) { *abort_flag = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+  } else {
+    pdl_wait();                                          // (y may still be in use)
+    const int g = lane >> 2, t = lane & 3, r = warp * 16 + g;
+    const uint32_t codes0 = (uint32_t)(warp * 2048 + g * 128 + (g << 4) + t * 4);
+    const uint32_t scales0 = (uint32_t)(MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4);
+    const uint32_t pick = (uint32_t)(t >> 1) | (uint32_t)((t >> 1) + 2) << 4;
+    constexpr int WORDS = FMT == GLQB_MX4_MXFP4 ? 2 : 4;
+    // (a warp whose wait gave up goes through the rest without waiting: the others meet it at the barriers)
+    for (int i = first; i < tiles; i += step) {
+      const Mx4Tile tile = mx4_tile(J, eff, pre, i / J.m_tiles);
+      const int mt = i % J.m_tiles;
+      int top[2] = {0, 0};
+      bool odd = false;                                  // rows that the short form of the multiplier does not cover
+      if constexpr (FMT == GLQB_MX4_MXFP4) {
+        const uint16_t* p = J.tops + ((long long)tile.expert * J.m_tiles + mt) * MX4_ROWS + r;
+        top[0] = p[0];
+        top[1] = p[8];
+        odd = __any_sync(0xFFFFFFFFu, ((top[0] | top[1]) & 256) != 0);
+        top[0] &= 255;
+        top[1] &= 255;
+      }
+      float acc[NB][2][4] = {};                          // two chains of MMAs
+      for (int k = k0; k < k1 && ok; ++k, ++q) {
+        const uint32_t s = q % STAGES;
+        if (!mbar_wait(&full[s], (q / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; break; }
+        const uint8_t* stage = ring + s * STAGE;
+        uint32_t sw[2][WORDS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int a = 0; a < WORDS; ++a) sw[h][a] = *reinterpret_cast<const uint32_t*>(stage + scales0 + 128 * h + 512 * a);
+        const uint8_t* xs = stage + TILE + g * MV4_X_ROW + t * 16;
+        const int left = J.n - k * MX4_K - t * 8;        // values of x from this lane's first on
+        auto units = [&](auto plain) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {                  // two units of 16 bytes
+            uint32_t m[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) multipliers<FMT, T>(sw[h][FMT == GLQB_MX4_MXFP4 ? p >> 1 : p], p, top[h], !decltype(plain)::value, pick, m[h]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int j = 2 * p + u;
+              const uint8_t* c = stage + (codes0 ^ (uint32_t)(j << 4));
+              const uint32_t w[2] = {*reinterpret_cast<const uint32_t*>(c), *reinterpret_cast<const uint32_t*>(c + 1024)};
+              uint4 b[NB];
+#pragma unroll
+              for (int n = 0; n < NB; ++n) {
+                b[n] = *reinterpret_cast<const uint4*>(xs + n * 8 * MV4_X_ROW + j * 64);
+                if (!decltype(plain)::value && j * 32 >= left) b[n] = make_uint4(0, 0, 0, 0);
+              }
+              uint32_t r[2][4];
+              mx4_pairs<T>(w[0], r[0]);
+              mx4_pairs<T>(w[1], r[1]);
+#pragma unroll
+              for (int v = 0; v < 2; ++v) {
+                uint32_t a[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = mx4_mul2<T>(r[e & 1][2 * v + (e >> 1)], m[e & 1][u]);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) mma16816<T>(acc[n][v], a, v ? b[n].z : b[n].x, v ? b[n].w : b[n].y);
+              }
+            }
+          }
+        };
+        if (!odd && (k + 1) * MX4_K <= J.n) units(std::true_type());
+        else units(std::false_type());
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][0][e] + acc[n][1][e];
+      if (J.split == 1) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int row = mt * MX4_ROWS + (threadIdx.x & 127);
+        if (row < J.m) {
+          const Mx4Factor f = mx4_row_factor<FMT, T>(J, tile.expert, row);
+          for (int c = threadIdx.x >> 7; c < tile.rows; c += 2)
+            mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, red[c * MX4_ROWS + (threadIdx.x & 127)] * f.a * f.b);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER);
+  }
+  __syncwarp();
+  if (J.split > 1) {                                     // (one tile per cluster)
+    cluster_sync();
+    if (first < tiles && warp < MV4_WARPS) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, first / J.m_tiles);
+      const int r = threadIdx.x & 127, row = first % J.m_tiles * MX4_ROWS + r;
+      if (row < J.m) {
+        const Mx4Factor f = mx4_row_factor<FMT, T>(J, t.expert, row);
+        const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
+        for (int c = rank + J.split * (int)(threadIdx.x >> 7); c < t.rows; c += 2 * J.split) {
+          const float v = sum_cluster(base + (uint32_t)(c * MX4_ROWS * 4), J.split);
+          mx4_put(J, (long long)(t.row0 + c) * J.y_stride + row, v * f.a * f.b);
+        }
+      }
+    }
+    cluster_sync();
+  }
+  __syncthreads();
+  if (*abort_flag && warp == MV4_WARPS && lane == 0)     // copies still under way
+    for (uint32_t n = 0; n < min(q, (uint32_t)STAGES); ++n) mbar_wait(&full[(q - 1 - n) % STAGES], ((q - 1 - n) / STAGES) & 1u);
 }
 
 }  // namespace
 
 cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count, cudaStream_t stream) {
-  const int strips = (J.m + MV4_ROWS - 1) / MV4_ROWS, nb = J.tn / 8;
-  // as many CTAs as the SMs hold, each with the same number of strips
-  const long long room = std::max<long long>(1, (long long)sm_count * (nb == 1 ? 3 : 2) / J.max_tiles), turns = (strips + room - 1) / room;
-  const dim3 grid((unsigned)((strips + turns - 1) / turns), (unsigned)J.max_tiles);
-  auto run = [&](auto* kernel) { kernel<<<grid, MV4_THREADS, 0, stream>>>(J, strips); return cudaGetLastError(); };
-  auto of = [&](auto fmt, auto type) {
+  const int nb = J.tn / 8;
+  const long long tiles = (long long)J.max_tiles * J.m_tiles;
+  const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, 2ll * sm_count);
+  auto run = [&](auto fmt, auto type, auto blocks) {
     using T = decltype(type);
-    constexpr int F = decltype(fmt)::value;
-    return nb == 1 ? run(mx4_mv_kernel<F, T, 1>) : run(mx4_mv_kernel<F, T, 2>);
+    constexpr int F = decltype(fmt)::value, NB = decltype(blocks)::value;
+    using C = Mv4<F, NB>;
+    const size_t smem = (size_t)C::STAGES * C::STAGE + 8 * NB * MX4_ROWS * 4 + C::STAGES * 16 + 8 + (size_t)(J.experts + 1) * 8;
+    return mx4_launch(mx4_mv_kernel<F, T, NB>, grid, MV4_THREADS, smem, J.split, stream, J);
   };
   using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
   using N = std::integral_constant<int, GLQB_MX4_NVFP4>;
-  if (format == GLQB_MX4_MXFP4) return x_bf16 ? of(M(), __nv_bfloat16()) : of(M(), __half());
-  return x_bf16 ? of(N(), __nv_bfloat16()) : of(N(), __half());
+  auto of = [&](auto blocks) {
+    if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(M(), __nv_bfloat16(), blocks) : run(M(), __half(), blocks);
+    return x_bf16 ? run(N(), __nv_bfloat16(), blocks) : run(N(), __half(), blocks);
+  };
+  return nb == 1 ? of(std::integral_constant<int, 1>()) : of(std::integral_constant<int, 2>());
 }
 
 }  // namespace glqb

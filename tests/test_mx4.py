@@ -52,8 +52,8 @@ def test_struct_layout_matches_header(tmp_path):
 
 
 def test_image_sizes(lib):
-    # tiles of 128 x 256: 16 KiB of codes and 1 (blocks of 32) or 2 KiB (of 16) of scales, MXFP4 a byte per row behind them
-    assert lib.glqb_mx4_image_bytes(0, 1, 128, 256) == 16384 + 1024 + 128
+    # tiles of 128 x 256: 16 KiB of codes and 1 (blocks of 32) or 2 KiB (of 16) of scales, MXFP4 two bytes per row behind them
+    assert lib.glqb_mx4_image_bytes(0, 1, 128, 256) == 16384 + 1024 + 256
     assert lib.glqb_mx4_image_bytes(1, 1, 128, 256) == 16384 + 2048
     assert lib.glqb_mx4_image_bytes(1, 5, 129, 257) == 5 * 4 * (16384 + 2048)
     assert lib.glqb_mx4_image_bytes(2, 1, 128, 256) == 0 and lib.glqb_mx4_image_bytes(0, 0, 128, 256) == 0
