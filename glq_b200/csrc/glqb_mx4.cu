@@ -163,7 +163,7 @@ mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 // One thread per 32-bit word of a tile's codes, then one per scale byte; rows and values past the matrix are zeros.
 template <int FMT>
 __global__ void __launch_bounds__(256) mx4_pack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int m, int n,
-                                                       int k_tiles, int m_tiles, uint8_t* __restrict__ image) {
+                                                       int k_tiles, int m_tiles, uint8_t* __restrict__ image, const uint16_t* __restrict__ tops) {
   constexpr int BLOCK = Mx4Fmt<FMT>::BLOCK, PER = MX4_K / BLOCK;
   const int kt = blockIdx.x % k_tiles;
   const long long at = blockIdx.x / k_tiles;                  // (expert, row tile)
@@ -186,26 +186,44 @@ __global__ void __launch_bounds__(256) mx4_pack_kernel(const uint8_t* __restrict
   for (int i = threadIdx.x; i < mx4_scale_bytes(FMT); i += blockDim.x) {
     const int r = i / PER, b = i % PER, row = mt * MX4_ROWS + r;
     const long long col = (long long)kt * PER + b;
-    tile[MX4_CODE_BYTES + mx4_scale_offset(r, b)] = row < m && col < scale_row ? scales[(e * m + row) * scale_row + col] : 0;
+    const bool in = row < m && col < scale_row;
+    uint32_t byte = in ? scales[(e * m + row) * scale_row + col] : 0u;
+    if constexpr (FMT == GLQB_MX4_MXFP4) {
+      // A block of zeros (past the matrix, or of a quantised zero, whose byte is 0) gets the row's largest scale: it stays zero, and
+      // the operands' scales lie close together.
+      uint32_t any = 0;
+      if (in) {
+        const int first = kt * (MX4_K / 2) + b * (BLOCK / 2);
+        const uint8_t* p = codes + (e * m + row) * code_row;
+        for (int j = first; j < min(first + BLOCK / 2, (int)code_row); ++j) any |= p[j] & (2 * j + 1 < n ? 0x77u : 0x07u);
+      }
+      if (byte != 255u && !any) byte = row < m ? tops[(e * m_tiles + mt) * MX4_ROWS + r] & 0xFFu : 0u;
+    }
+    tile[MX4_CODE_BYTES + mx4_scale_offset(r, b)] = (uint8_t)byte;
   }
 }
-// MXFP4: the largest scale byte of every row that is a number; + 256 for rows that have one that is none, or so large a one that a
-// multiplier by 2^(s - largest) may leave the exponents of bf16
-__global__ void __launch_bounds__(256) mx4_row_top_kernel(const uint8_t* __restrict__ scales, long long rows, int m, int m_pad, int scale_row,
-                                                          uint16_t* __restrict__ tops) {
+// MXFP4: the largest scale byte of every row's blocks that are numbers and not zero; + 256 for rows that have a block that is no number,
+// or one so far below the largest that 2^(s - largest + 13) is no normal fp16 number.
+__global__ void __launch_bounds__(256) mx4_row_top_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long rows, int m,
+                                                          int m_pad, int n, uint16_t* __restrict__ tops) {
   const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;          // of experts x m_pad
   if (row >= rows) return;
-  const int r = (int)(row % m_pad);
-  uint32_t top = 0, nan = 0;
-  if (r < m)
+  const int r = (int)(row % m_pad), scale_row = (n + 31) / 32, code_row = (n + 1) / 2;
+  uint32_t top = 0, low = 255, nan = 0;
+  if (r < m) {
+    const long long at = row / m_pad * m + r;
     for (int c = threadIdx.x % 32; c < scale_row; c += 32) {
-      const uint32_t s = scales[(row / m_pad * m + r) * scale_row + c];
-      top = s < 255u ? max(top, s) : top;
-      nan |= s == 255u;
+      const uint32_t s = scales[at * scale_row + c];
+      uint32_t any = 0;
+      for (int j = c * 16; j < min(c * 16 + 16, code_row); ++j) any |= codes[at * code_row + j] & (2 * j + 1 < n ? 0x77u : 0x07u);
+      if (s == 255u) nan = 1u;
+      else if (any) { top = max(top, s); low = min(low, s); }
     }
+  }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
+  low = __reduce_min_sync(0xFFFFFFFFu, low);
   nan = __any_sync(0xFFFFFFFFu, nan);
-  if (threadIdx.x % 32 == 0) tops[row] = (uint16_t)(top | (nan || top > 252u ? 256u : 0u));
+  if (threadIdx.x % 32 == 0) tops[row] = (uint16_t)(top | (nan || top > low + 27u ? 256u : 0u));
 }
 
 // ---- activations of the products ------------------------------------------------------------------
@@ -389,12 +407,12 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
   if (tiles >= (1ll << 31)) return mx4_fail(GLQB_E_INVALID, "mx4_pack: %d x %d x %d is more than 2^31 tiles", experts, m, n);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4) {
-    mx4_pack_kernel<GLQB_MX4_MXFP4><<<(unsigned)tiles, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, m, n, kt, mt, (uint8_t*)image);
     const long long rows = (long long)experts * mt * MX4_ROWS;
-    mx4_row_top_kernel<<<(unsigned)(rows / 8), 256, 0, stream>>>((const uint8_t*)scales, rows, m, mt * MX4_ROWS, (n + 31) / 32,
-                                                                 (uint16_t*)((uint8_t*)image + tiles * mx4_tile_bytes(format)));
+    uint16_t* tops = (uint16_t*)((uint8_t*)image + tiles * mx4_tile_bytes(format));
+    mx4_row_top_kernel<<<(unsigned)(rows / 8), 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, rows, m, mt * MX4_ROWS, n, tops);
+    mx4_pack_kernel<GLQB_MX4_MXFP4><<<(unsigned)tiles, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, m, n, kt, mt, (uint8_t*)image, tops);
   } else {
-    mx4_pack_kernel<GLQB_MX4_NVFP4><<<(unsigned)tiles, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, m, n, kt, mt, (uint8_t*)image);
+    mx4_pack_kernel<GLQB_MX4_NVFP4><<<(unsigned)tiles, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, m, n, kt, mt, (uint8_t*)image, nullptr);
   }
   return mx4_launched("mx4_pack");
 }

@@ -54,6 +54,13 @@ __device__ __forceinline__ float sum_cluster(uint32_t addr, int ranks) {
 // the largest before it), so that whatever they hold, experts do not overlap and the tiles are no more than max_tiles.
 // Called by all threads; `eff` and `pre` have experts + 1 entries in shared memory.
 __device__ __forceinline__ void mx4_groups(const Mx4Job& J, int* eff, int* pre) {
+  if (J.offsets) {
+    for (int e = threadIdx.x; e <= J.experts; e += blockDim.x) {
+      const long long o = J.wide ? reinterpret_cast<const long long*>(J.offsets)[e] : reinterpret_cast<const int*>(J.offsets)[e];
+      eff[e] = (int)max(0ll, min((long long)J.rows, o));
+    }
+    __syncthreads();
+  }
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     if (!J.offsets) {
@@ -62,8 +69,7 @@ __device__ __forceinline__ void mx4_groups(const Mx4Job& J, int* eff, int* pre) 
       int top = 0, tiles = 0;
       for (int b = 0; b <= J.experts; b += 32) {
         const int e = min(b + lane, J.experts);
-        const long long o = J.wide ? reinterpret_cast<const long long*>(J.offsets)[e] : reinterpret_cast<const int*>(J.offsets)[e];
-        int v = (int)max(0ll, min((long long)J.rows, o));
+        int v = eff[e];
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
@@ -121,25 +127,21 @@ __device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) 
 }
 
 // ---- 4-bit weights as 16-bit operands -------------------------------------------------------------
-// The bits of a code are moved to sign, exponent and first mantissa bit of a 16-bit number, where they read as the value times
-// 2^-126 (bf16) or 2^-14 (fp16), subnormals included; one multiplication by a power of two, or by an e4m3 number, times what
-// brings that back gives the operand exactly.  So that the multiplier stays in range, operands are
-//   MXFP4  value * 2^(s - top) (bf16), value * 2^(s - top + 1) (fp16), top the largest scale byte of the row
-//   NVFP4  value * s * 2^-7
+// fp16: cvt takes two codes of a byte to fp16.  bf16 has no such instruction: the bits of a code are moved to sign, exponent and
+// first mantissa bit of a 16-bit number, where they read as the value times 2^-126, subnormals included.  One multiplication by
+// the scale then gives the operand exactly.  So that multiplier and operand stay in range, operands are
+//   MXFP4  value * 2^(s - top + 13) (fp16), value * 2^(s - top) (bf16), top the largest scale byte of the row
+//   NVFP4  value * s (fp16), value * s * 2^-7 (bf16)
 // and mx4_row_factor is what the sums are multiplied by.
-// The four pairs of a word, unscaled: r[i] holds values 2i and 2i + 1.  Logic and right shifts issue at half an instruction a clock,
-// and so do integer products (left shifts), on a pipe of their own.  In bf16 two of the pairs are therefore brought to bits 9:6 of
+//
+// bf16: the four pairs of a word, unscaled, r[i] holds values 2i and 2i + 1.  Logic and right shifts issue at half an instruction a
+// clock, and so do integer products (left shifts), on a pipe of their own.  Two of the pairs are therefore brought to bits 9:6 of
 // each half and copied to 15:12 by a product with 65, the others masked at 15:12 and shifted down: ten instructions on the one
-// pipe and four on the other per word, where all pairs the second way are twelve and three.  In fp16 the two places share a bit,
-// which a product would carry out of.
-template <typename T>
-__device__ __forceinline__ void mx4_pairs(uint32_t w, uint32_t (&r)[4]) {
+// pipe and four on the other per word, where all pairs the second way are twelve and three.
+__device__ __forceinline__ void mx4_pairs_bf16(uint32_t w, uint32_t (&r)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (__is_same(T, __half)) {
-      const uint32_t x = (i == 3 ? w : w << (12 - 4 * i)) & 0xF000F000u;
-      r[i] = (x | x >> 3) & 0x8E008E00u;
-    } else if (i < 2) {
+    if (i < 2) {
       r[i] = (((w << (6 - 4 * i)) & 0x03C003C0u) * 65u) & 0x81C081C0u;
     } else {
       const uint32_t x = (i == 3 ? w : w << 4) & 0xF000F000u;
@@ -147,17 +149,32 @@ __device__ __forceinline__ void mx4_pairs(uint32_t w, uint32_t (&r)[4]) {
     }
   }
 }
+// fp16: the bytes of a word, two values each
+__device__ __forceinline__ void mx4_bytes_f16(uint32_t w, uint32_t (&r)[4]) {
+  asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; "
+      "cvt.rn.f16x2.e2m1x2 %3, d; }" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+}
+// the pairs of a word in the order of the values
+template <typename T>
+__device__ __forceinline__ void mx4_pairs(uint32_t w, uint32_t (&r)[4]) {
+  if constexpr (__is_same(T, __half)) {
+    // nibbles 0 2 4 6 1 3 5 7 -> bytes (0 1) (2 3) (4 5) (6 7)
+    const uint32_t v = w >> 16, a = (w & 0x0F0Fu) | ((v & 0x0F0Fu) << 4), b = ((w >> 4) & 0x0F0Fu) | (v & 0xF0F0u);
+    mx4_bytes_f16(__byte_perm(a, b, 0x5140), r);
+  } else {
+    mx4_pairs_bf16(w, r);
+  }
+}
 template <int FMT, typename T>
 __device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {   // in both halves
   uint32_t h;
   if constexpr (FMT == GLQB_MX4_MXFP4) {
     const int d = (int)s - top;
-    if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : (uint32_t)max(d + 30, 0) << 10;
+    if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : d > -28 ? (uint32_t)(d + 28) << 10 : d >= -37 ? 1u << (d + 37) : 0u;
     else h = s == 255u ? 0x7FC0u : (uint32_t)max(d + 253, 0) << 7;
   } else {
-    const float f = mx4_e4m3(s);
-    if constexpr (__is_same(T, __half)) h = __half_as_ushort(__float2half_rn(f * 128.0f));
-    else h = __float_as_uint(f * 0x1p119f) >> 16;
+    if constexpr (__is_same(T, __half)) h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)s, __NV_E4M3).x;
+    else h = __float_as_uint(mx4_e4m3(s) * 0x1p119f) >> 16;
   }
   return h | h << 16;
 }
@@ -172,14 +189,15 @@ __device__ __forceinline__ uint32_t mx4_mul2(uint32_t a, uint32_t b) {
   }
 }
 struct Mx4Factor { float a, b; };     // two factors: 2^-127 and 2^127 have no single one
+template <typename T>
+__device__ __forceinline__ Mx4Factor mx4_power(uint32_t top) {          // MXFP4, from a row's entry in `tops`
+  const int p = (int)(top & 0xFFu) - (__is_same(T, __half) ? 140 : 127), h = p >> 1;
+  return Mx4Factor{__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(p - h + 127) << 23)};
+}
 template <int FMT, typename T>
 __device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert, int row) {
-  if constexpr (FMT == GLQB_MX4_MXFP4) {
-    const int p = (int)(J.tops[(long long)expert * J.m_tiles * MX4_ROWS + row] & 0xFFu) - (__is_same(T, __half) ? 128 : 127), h = p >> 1;
-    return Mx4Factor{__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(p - h + 127) << 23)};
-  } else {
-    return Mx4Factor{128.0f, J.w_scale[expert]};
-  }
+  if constexpr (FMT == GLQB_MX4_MXFP4) return mx4_power<T>(J.tops[(long long)expert * J.m_tiles * MX4_ROWS + row]);
+  else return Mx4Factor{__is_same(T, __half) ? 1.0f : 128.0f, J.w_scale[expert]};
 }
 #endif  // __CUDACC__
 

@@ -1,14 +1,17 @@
 // Products of microscaled 4-bit weights with few rows of x: decode steps, experts of few tokens.
 //
-// What bounds these is the weights' way from HBM and, close behind, the instructions that make 16-bit operands of them (about
-// 430 per warp for 16 rows x 256 values, five per two weights).  A CTA takes 128 weight rows x 8 NB rows of x; one warp brings
-// tiles of 128 x 256 weights with the rows of x that belong to them into a ring of stages (bulk copies), and runs ahead over the
-// borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile into fragments of mma.sync.m16n8k16 in registers and
-// multiply.  The MMA's order of values is free as long as both operands have it: lane t of a quad takes word t of a 16-byte unit, eight
-// values, and of x the same eight, so nothing is exchanged and every shared-memory access is free of conflicts.  Where there
-// are few tiles the CTAs of a cluster share out the values and add their parts in rank order.
-// Lanes that read weights from global memory (a CTA's warps sharing out the values): one token of 14336 x 4096 14.5 us,
-// sixteen 25.4, 256 rows over 128 experts of 1536 x 2048 83 us: rows of x came from L1 with sixteen lines per load.
+// What bounds these is the weights' way from HBM and, close behind, the instructions that make 16-bit operands of them.  A CTA
+// takes 128 weight rows x 8 NB rows of x; one warp brings tiles of 128 x 256 weights with the rows of x that belong to them into a
+// ring of stages (bulk copies), and runs ahead over the borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile
+// into fragments of mma.sync.m16n8k16 in registers and multiply.  The MMA's order of values is free as long as both operands have it:
+// lane t of a quad takes word t of a 16-byte unit, eight values, and of x the same eight, so nothing is exchanged and every
+// shared-memory access is free of conflicts.  Where there are few tiles the CTAs of a cluster share out the values and add
+// their parts in rank order.
+//
+// Operands are fp16, because two codes become fp16 in one instruction and bf16 in four (as bf16: 505 instructions per warp
+// for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  bf16 rows of x are brought to fp16 in shared memory, 256
+// values at a time, by the power of two that takes the largest finite one to 2^14 .. 2^15; the sums of a tile are multiplied back in
+// fp32.  Values of at least 2^-32 of the largest are exact, smaller ones off by at most 2^-40 of it.
 #include "glqb_mx4_gemm.cuh"
 #include "glqb_launch.h"
 #include <algorithm>
@@ -19,43 +22,67 @@ namespace {
 constexpr int MV4_WARPS = 8, MV4_THREADS = (MV4_WARPS + 1) * 32;
 constexpr int MV4_X_ROW = MX4_K * 2 + 64;        // bytes of a row of x in a stage: eight rows in all the banks
 template <int FMT, int NB> struct Mv4 {
-  static constexpr int STAGE = mx4_tile_bytes(FMT) + 8 * NB * MV4_X_ROW;
+  static constexpr int TOPS = mx4_tile_bytes(FMT) + 8 * NB * MV4_X_ROW;     // MXFP4: the rows' largest scales, with a tile's first stage
+  static constexpr int STAGE = TOPS + (FMT == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0);
   static constexpr int STAGES = NB == 1 ? 4 : 3;                       // two CTAs per SM
 };
 
-template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (__is_same(T, __half))
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // The multipliers of a row's blocks that lane t meets in the 16-byte units 2i and 2i + 1, from the word of scales that holds them.
-// MXFP4: bytes 2i % 4 and + 1.  NVFP4: bytes t / 2 and t / 2 + 2 of word i.
-template <int FMT, typename T>
-__device__ __forceinline__ void multipliers(uint32_t word, int i, int top, bool odd, uint32_t pick, uint32_t (&m)[2]) {
+// MXFP4: bytes 2i % 4 and + 1 (`plain`: all numbers, within 2^27 of the largest).  NVFP4: bytes t / 2 and t / 2 + 2 of word i.
+template <int FMT>
+__device__ __forceinline__ void multipliers(uint32_t word, int i, int top, bool plain, uint32_t pick, uint32_t (&m)[2]) {
   if constexpr (FMT == GLQB_MX4_MXFP4) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t s = (word >> (8 * (2 * (i & 1) + u))) & 0xFFu;
-      if (__is_same(T, __half) || odd) m[u] = mx4_multiplier<FMT, T>(s, top);
-      else m[u] = s * 0x00800080u + (uint32_t)(253 - top) * 0x00800080u;
+      m[u] = plain ? s * 0x04000400u + (uint32_t)(28 - top) * 0x04000400u : mx4_multiplier<FMT, __half>(s, top);
     }
   } else {
-    const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)__byte_perm(word, 0, pick), __NV_E4M3));
-    if constexpr (__is_same(T, __half)) {
-      const __half2 r = __hmul2(h, __float2half2_rn(128.0f));
-      const uint32_t b = *reinterpret_cast<const uint32_t*>(&r);
-      m[0] = __byte_perm(b, 0, 0x1010);
-      m[1] = __byte_perm(b, 0, 0x3232);
-    } else {
-      const float2 f = __half22float2(h);
-      m[0] = __byte_perm(__float_as_uint(f.x * 0x1p119f), 0, 0x3232);
-      m[1] = __byte_perm(__float_as_uint(f.y * 0x1p119f), 0, 0x3232);
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)__byte_perm(word, 0, pick), __NV_E4M3);
+    const uint32_t b = (uint32_t)h.x | (uint32_t)h.y << 16;
+    m[0] = __byte_perm(b, 0, 0x1010);
+    m[1] = __byte_perm(b, 0, 0x3232);
+  }
+}
+
+// A row's eight values of a lane, bf16 or fp16, to fp16 in the order 0 2 4 6 1 3 5 7; bf16 times a power of two: returned is
+// what the sums are multiplied by, its inverse (MXFP4: and the 2^-13 that fp16 operands carry).  `left`: values there are; the others become zeros.
+template <int FMT, typename T>
+__device__ __forceinline__ float convert8(uint8_t* p, int left) {
+  uint4 v = *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if (left < 8) {                                        // (n is a multiple of eight: all or none)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 0u;
+  }
+  if constexpr (__is_same(T, __half)) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632),
+                                              __byte_perm(w[2], w[3], 0x7632));
+    return 1.0f;
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = w[i] & 0x7FFFu, hi = (w[i] >> 16) & 0x7FFFu;
+      top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
     }
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    const int e = max((int)(top >> 7), 15);              // biased exponent of the largest; 2^(141 - e) takes it to 2^14
+    const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16) * up;
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u) * up;
+    }
+    auto pack = [](float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); };
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack(f[0], f[2]), pack(f[4], f[6]), pack(f[1], f[3]), pack(f[5], f[7]));
+    return __uint_as_float((uint32_t)(e - 14) << 23) * (FMT == GLQB_MX4_MXFP4 ? 0x1p-13f : 1.0f);
   }
 }
 
@@ -63,15 +90,17 @@ template <int FMT, typename T, int NB>
 __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J) {
   constexpr int TILE = mx4_tile_bytes(FMT), STAGE = Mv4<FMT, NB>::STAGE, STAGES = Mv4<FMT, NB>::STAGES;
   extern __shared__ __align__(128) uint8_t ring[];
-  float* red = reinterpret_cast<float*>(ring + STAGES * STAGE);                      // [8 NB][128]
-  uint64_t* full = reinterpret_cast<uint64_t*>(red + 8 * NB * MX4_ROWS);
+  float* red = reinterpret_cast<float*>(ring + STAGES * STAGE);                      // [2][8 NB][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(red + 2 * 8 * NB * MX4_ROWS);
   uint64_t* empty = full + STAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
+  uint64_t* ready = empty + STAGES;                                                  // x as fp16
+  float* x_scale = reinterpret_cast<float*>(ready + STAGES);                         // [STAGES][8 NB]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(x_scale + STAGES * 8 * NB);
   int* eff = const_cast<int*>(abort_flag) + 2;
   int* pre = eff + J.experts + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); mbar_init(&ready[s], MV4_WARPS); }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -94,7 +123,9 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
         if (!mbar_wait(&empty[s], ((q / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
         uint8_t* to = ring + s * STAGE;
         if (lane == 0) {
-          mbar_expect_tx(&full[s], TILE + (uint32_t)t.rows * x_bytes);
+          const uint32_t tops = FMT == GLQB_MX4_MXFP4 && k == k0 ? 2 * MX4_ROWS : 0;
+          mbar_expect_tx(&full[s], TILE + tops + (uint32_t)t.rows * x_bytes);
+          if (tops) bulk_g2s(to + Mv4<FMT, NB>::TOPS, J.tops + ((long long)t.expert * J.m_tiles + i % J.m_tiles) * MX4_ROWS, tops, &full[s]);
           bulk_g2s(to, w + (long long)k * TILE, TILE, &full[s]);
         }
         __syncwarp();
@@ -110,82 +141,105 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     const uint32_t codes0 = (uint32_t)(warp * 2048 + g * 128 + (g << 4) + t * 4);
     const uint32_t scales0 = (uint32_t)(MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4);
     const uint32_t pick = (uint32_t)(t >> 1) | (uint32_t)((t >> 1) + 2) << 4;
+    int turn = 0;
     constexpr int WORDS = FMT == GLQB_MX4_MXFP4 ? 2 : 4;
+    // This warp's rows of x in stage `u`, which holds values k * 256 on of `rows` rows.  Done one stage ahead of the products.
+    auto convert = [&](uint32_t u, int rows, int k) {
+      const uint32_t s = u % STAGES;
+      if (!ok || !mbar_wait(&full[s], (u / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; return; }
+      for (int row = warp; row < rows; row += MV4_WARPS) {
+        const float down = convert8<FMT, T>(ring + s * STAGE + TILE + row * MV4_X_ROW + lane * 16, J.n - k * MX4_K - lane * 8);
+        if (lane == 0) x_scale[s * 8 * NB + row] = down;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ready[s]);
+    };
+    if (first < tiles) convert(0, mx4_tile(J, eff, pre, first / J.m_tiles).rows, k0);
     // (a warp whose wait gave up goes through the rest without waiting: the others meet it at the barriers)
     for (int i = first; i < tiles; i += step) {
       const Mx4Tile tile = mx4_tile(J, eff, pre, i / J.m_tiles);
       const int mt = i % J.m_tiles;
       int top[2] = {0, 0};
-      bool odd = false;                                  // rows that the short form of the multiplier does not cover
-      if constexpr (FMT == GLQB_MX4_MXFP4) {
-        const uint16_t* p = J.tops + ((long long)tile.expert * J.m_tiles + mt) * MX4_ROWS + r;
-        top[0] = p[0];
-        top[1] = p[8];
-        odd = __any_sync(0xFFFFFFFFu, ((top[0] | top[1]) & 256) != 0);
-        top[0] &= 255;
-        top[1] &= 255;
-      }
-      float acc[NB][2][4] = {};                          // two chains of MMAs
-      for (int k = k0; k < k1 && ok; ++k, ++q) {
+      bool plain = true;                                 // rows that the short form of the multiplier covers
+      Mx4Factor f{1.0f, 1.0f};
+      if constexpr (FMT == GLQB_MX4_NVFP4) f.b = __ldg(J.w_scale + tile.expert);
+      float acc[NB][4] = {};
+      for (int k = k0; k < k1; ++k, ++q) {
+        if (k + 1 < k1) convert(q + 1, tile.rows, k + 1);
+        else if (i + step < tiles) convert(q + 1, mx4_tile(J, eff, pre, (i + step) / J.m_tiles).rows, k0);
         const uint32_t s = q % STAGES;
-        if (!mbar_wait(&full[s], (q / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; break; }
+        if (!ok || !mbar_wait(&ready[s], (q / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; continue; }
         const uint8_t* stage = ring + s * STAGE;
+        if constexpr (FMT == GLQB_MX4_MXFP4) {
+          if (k == k0) {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(stage + Mv4<FMT, NB>::TOPS);
+            top[0] = p[r];
+            top[1] = p[r + 8];
+            plain = !__any_sync(0xFFFFFFFFu, ((top[0] | top[1]) & 256) != 0);
+            top[0] &= 255;
+            top[1] &= 255;
+            f = mx4_power<T>(p[threadIdx.x & 127]);
+          }
+        }
         uint32_t sw[2][WORDS];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int a = 0; a < WORDS; ++a) sw[h][a] = *reinterpret_cast<const uint32_t*>(stage + scales0 + 128 * h + 512 * a);
         const uint8_t* xs = stage + TILE + g * MV4_X_ROW + t * 16;
-        const int left = J.n - k * MX4_K - t * 8;        // values of x from this lane's first on
-        auto units = [&](auto plain) {
+        float d[NB][2][4] = {};                          // two chains of MMAs
+        auto units = [&](auto is_plain) {
 #pragma unroll
           for (int p = 0; p < 4; ++p) {                  // two units of 16 bytes
             uint32_t m[2][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) multipliers<FMT, T>(sw[h][FMT == GLQB_MX4_MXFP4 ? p >> 1 : p], p, top[h], !decltype(plain)::value, pick, m[h]);
+            for (int h = 0; h < 2; ++h) multipliers<FMT>(sw[h][FMT == GLQB_MX4_MXFP4 ? p >> 1 : p], p, top[h], decltype(is_plain)::value, pick, m[h]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const int j = 2 * p + u;
               const uint8_t* c = stage + (codes0 ^ (uint32_t)(j << 4));
-              const uint32_t w[2] = {*reinterpret_cast<const uint32_t*>(c), *reinterpret_cast<const uint32_t*>(c + 1024)};
+              uint32_t w[2][4];
+              mx4_bytes_f16(*reinterpret_cast<const uint32_t*>(c), w[0]);
+              mx4_bytes_f16(*reinterpret_cast<const uint32_t*>(c + 1024), w[1]);
               uint4 b[NB];
 #pragma unroll
-              for (int n = 0; n < NB; ++n) {
-                b[n] = *reinterpret_cast<const uint4*>(xs + n * 8 * MV4_X_ROW + j * 64);
-                if (!decltype(plain)::value && j * 32 >= left) b[n] = make_uint4(0, 0, 0, 0);
-              }
-              uint32_t r[2][4];
-              mx4_pairs<T>(w[0], r[0]);
-              mx4_pairs<T>(w[1], r[1]);
+              for (int n = 0; n < NB; ++n) b[n] = *reinterpret_cast<const uint4*>(xs + n * 8 * MV4_X_ROW + j * 64);
 #pragma unroll
               for (int v = 0; v < 2; ++v) {
                 uint32_t a[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = mx4_mul2<T>(r[e & 1][2 * v + (e >> 1)], m[e & 1][u]);
+                for (int e = 0; e < 4; ++e) a[e] = mx4_mul2<__half>(w[e & 1][2 * v + (e >> 1)], m[e & 1][u]);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) mma16816<T>(acc[n][v], a, v ? b[n].z : b[n].x, v ? b[n].w : b[n].y);
+                for (int n = 0; n < NB; ++n) mma16816(d[n][v], a, v ? b[n].z : b[n].x, v ? b[n].w : b[n].y);
               }
             }
           }
         };
-        if (!odd && (k + 1) * MX4_K <= J.n) units(std::true_type());
+        if (plain) units(std::true_type());
         else units(std::false_type());
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          float2 down = make_float2(1.0f, 1.0f);
+          if constexpr (!__is_same(T, __half)) down = *reinterpret_cast<const float2*>(x_scale + s * 8 * NB + n * 8 + 2 * t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(d[n][0][e] + d[n][1][e], e & 1 ? down.y : down.x, acc[n][e]);
+        }
+        fence_async_smem();                              // (x was written here: the next copy into the stage comes behind)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }
+      // (two buffers in turn: a tile's sums are read before the barrier of the next one's)
+      float* sums = red + (turn++ & 1) * (8 * NB * MX4_ROWS);
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) red[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][0][e] + acc[n][1][e];
+        for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][e];
       if (J.split == 1) {
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const int row = mt * MX4_ROWS + (threadIdx.x & 127);
-        if (row < J.m) {
-          const Mx4Factor f = mx4_row_factor<FMT, T>(J, tile.expert, row);
+        if (row < J.m)
           for (int c = threadIdx.x >> 7; c < tile.rows; c += 2)
-            mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, red[c * MX4_ROWS + (threadIdx.x & 127)] * f.a * f.b);
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+            mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, sums[c * MX4_ROWS + (threadIdx.x & 127)] * f.a * f.b);
       }
     }
     if (!ok && lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER);
@@ -197,7 +251,9 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
       const Mx4Tile t = mx4_tile(J, eff, pre, first / J.m_tiles);
       const int r = threadIdx.x & 127, row = first % J.m_tiles * MX4_ROWS + r;
       if (row < J.m) {
-        const Mx4Factor f = mx4_row_factor<FMT, T>(J, t.expert, row);
+        Mx4Factor f{1.0f, 1.0f};
+        if constexpr (FMT == GLQB_MX4_MXFP4) f = mx4_power<T>(J.tops[((long long)t.expert * J.m_tiles) * MX4_ROWS + row]);
+        else f.b = J.w_scale[t.expert];
         const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
         for (int c = rank + J.split * (int)(threadIdx.x >> 7); c < t.rows; c += 2 * J.split) {
           const float v = sum_cluster(base + (uint32_t)(c * MX4_ROWS * 4), J.split);
@@ -222,7 +278,7 @@ cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count
     using T = decltype(type);
     constexpr int F = decltype(fmt)::value, NB = decltype(blocks)::value;
     using C = Mv4<F, NB>;
-    const size_t smem = (size_t)C::STAGES * C::STAGE + 8 * NB * MX4_ROWS * 4 + C::STAGES * 16 + 8 + (size_t)(J.experts + 1) * 8;
+    const size_t smem = (size_t)C::STAGES * C::STAGE + 2 * 8 * NB * MX4_ROWS * 4 + C::STAGES * (24 + 8 * NB * 4) + 8 + (size_t)(J.experts + 1) * 8;
     return mx4_launch(mx4_mv_kernel<F, T, NB>, grid, MV4_THREADS, smem, J.split, stream, J);
   };
   using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
