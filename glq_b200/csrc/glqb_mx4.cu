@@ -423,16 +423,20 @@ struct Form {
   bool align, mv;
   size_t image, bytes;        // of the workspace: x in 4 bits or aligned, then two floats
 };
-static int sm_count() {
-  static std::atomic<int> known[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  int n = known[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
-    known[dev].store(n, std::memory_order_relaxed);
+struct Device { std::atomic<int> sms; std::atomic<int*> status; };
+static Device* device() {
+  static Device known[64];
+  Device& d = known[mx4_device()];
+  if (d.sms.load(std::memory_order_acquire) == 0) {
+    int n = 0;
+    int* p = nullptr;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, mx4_device()) != cudaSuccess || n < 1 ||
+        cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_mx4_status) != cudaSuccess)
+      return nullptr;
+    d.status.store(p, std::memory_order_relaxed);
+    d.sms.store(n, std::memory_order_release);
   }
-  return n;
+  return &d;
 }
 constexpr int MV_MAX_ROWS = 16;     // rows (an expert's, on average) up to which the streaming kernel runs
 static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, int sms) {
@@ -462,7 +466,7 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
 
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize) {
   if (!w || !format_ok(w->format) || rows <= 0 || rows >= (1ll << 31) || w->experts < 1 || w->m < 1 || w->n < 1) return 0;
-  return form_of(w, rows, x_stride, x, quantize, sm_count()).bytes;
+  return form_of(w, rows, x_stride, x, quantize, 1).bytes;      // (what a call needs does not depend on the SMs)
 }
 
 int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows,
@@ -479,14 +483,14 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   if (rows == 0) return GLQB_OK;
   if (!w->image || !x || !y || (w->format == GLQB_MX4_NVFP4 && !w->tensor_scale)) return mx4_fail(GLQB_E_INVALID, "mx4_product: null argument");
   if (rows > 1 && (x_stride < w->n || y_stride < w->m)) return mx4_fail(GLQB_E_INVALID, "mx4_product: rows overlap");
-  const int sms = sm_count();
+  const Device* d = device();
+  const int sms = d ? d->sms.load(std::memory_order_relaxed) : 1;      // (the workspace does not depend on it)
   const Form f = form_of(w, rows, x_stride, x, quantize, sms);
   if (workspace_bytes < f.bytes || (f.bytes && !workspace))
     return mx4_fail(GLQB_E_WORKSPACE, "mx4_product: workspace of %zu bytes, %zu needed", workspace_bytes, f.bytes);
+  if (!d) return mx4_fail(GLQB_E_CUDA, "mx4_product: no device");
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  int* status = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&status), g_mx4_status);
-  if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4_product: %s", cudaGetErrorString(e));
+  cudaError_t e = cudaSuccess;
   Mx4Job J = {};
   J.m = w->m;
   J.n = w->n;
@@ -509,7 +513,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.y_wide = y_dtype != GLQB_DT_F32 && !accumulate && reinterpret_cast<uintptr_t>(y) % 16 == 0 && (rows == 1 || y_stride % 8 == 0);
   J.x = x;
   J.x_stride = x_stride;
-  J.status = status;
+  J.status = d->status.load(std::memory_order_relaxed);
   const size_t lists = (size_t)(J.experts + 1) * 8;
   if (offsets && clear_rest) mx4_clear_kernel<<<(unsigned)std::min<long long>(rows, 148), 256, lists, stream>>>(J);
   if (!quantize) {

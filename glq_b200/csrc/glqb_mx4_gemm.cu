@@ -539,9 +539,14 @@ cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_c
   if (r != CUDA_SUCCESS) { *what = "cuTensorMapEncodeTiled refused the activations"; return cudaErrorInvalidValue; }
   const long long tiles = (long long)J.max_tiles * J.m_tiles;
   const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
-  auto run = [&](auto* kernel) { return mx4_launch(kernel, grid, G16_THREADS, smem, J.split, stream, J, map, R); };
-  if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(mx4_gemm16_kernel<GLQB_MX4_MXFP4, __nv_bfloat16>) : run(mx4_gemm16_kernel<GLQB_MX4_MXFP4, __half>);
-  return x_bf16 ? run(mx4_gemm16_kernel<GLQB_MX4_NVFP4, __nv_bfloat16>) : run(mx4_gemm16_kernel<GLQB_MX4_NVFP4, __half>);
+  auto run = [&](auto fmt, auto type) {
+    constexpr auto K = mx4_gemm16_kernel<decltype(fmt)::value, decltype(type)>;
+    return mx4_launch<K>(K, grid, G16_THREADS, smem, J.split, stream, J, map, R);
+  };
+  using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
+  using N = std::integral_constant<int, GLQB_MX4_NVFP4>;
+  if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(M(), __nv_bfloat16()) : run(M(), __half());
+  return x_bf16 ? run(N(), __nv_bfloat16()) : run(N(), __half());
 }
 
 cudaError_t mx4_gemm4_launch(int format, const Mx4Job& J, int sm_count, cudaStream_t stream) {
@@ -551,8 +556,11 @@ cudaError_t mx4_gemm4_launch(int format, const Mx4Job& J, int sm_count, cudaStre
   const long long tiles = (long long)J.max_tiles * J.m_tiles;
   const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
   const size_t smem = std::max(ONE_PER_SM, fixed + stages * stage);
-  auto run = [&](auto* kernel) { return mx4_launch(kernel, grid, G4_THREADS, smem, J.split, stream, J, stages, x_scales); };
-  return format == GLQB_MX4_MXFP4 ? run(mx4_gemm4_kernel<GLQB_MX4_MXFP4>) : run(mx4_gemm4_kernel<GLQB_MX4_NVFP4>);
+  auto run = [&](auto fmt) {
+    constexpr auto K = mx4_gemm4_kernel<decltype(fmt)::value>;
+    return mx4_launch<K>(K, grid, G4_THREADS, smem, J.split, stream, J, stages, x_scales);
+  };
+  return format == GLQB_MX4_MXFP4 ? run(std::integral_constant<int, GLQB_MX4_MXFP4>()) : run(std::integral_constant<int, GLQB_MX4_NVFP4>());
 }
 
 }  // namespace glqb

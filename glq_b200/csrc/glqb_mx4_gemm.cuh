@@ -3,6 +3,7 @@
 #include "glqb_mx4.cuh"
 #include "glqb_ptx.cuh"
 #include "glqb_launch.h"
+#include <atomic>
 
 namespace glqb {
 
@@ -40,6 +41,11 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
   return v;
 }
 
+__device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
 // a value of every CTA of the cluster, added in rank order (all loads before the first sum)
 __device__ __forceinline__ float sum_cluster(uint32_t addr, int ranks) {
   float v[8];
@@ -202,11 +208,19 @@ __device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert,
 #endif  // __CUDACC__
 
 // Chained to the kernel in front (launch_chained), `cluster` CTAs per cluster.
-template <typename... P, typename... A>
+inline int mx4_device() {       // the current one, 0..63
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
+}
+template <auto K, typename... P, typename... A>
 inline cudaError_t mx4_launch(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
-  // (per device and idempotent: a word of the runtime, no synchronisation)
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
+  static std::atomic<int> limit[64];     // per device: the shared memory the kernel may have (raised, never lowered)
+  std::atomic<int>& most = limit[mx4_device()];
+  if (most.load(std::memory_order_relaxed) < (int)smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return e;
+    most.store(227 * 1024, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)threads);

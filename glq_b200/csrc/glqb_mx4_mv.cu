@@ -1,16 +1,15 @@
 // Products of microscaled 4-bit weights with few rows of x: decode steps, experts of few tokens.
 //
 // What bounds these is the weights' way from HBM and, close behind, the instructions that make 16-bit operands of them.  A CTA
-// takes 128 weight rows x 8 NB rows of x; one warp brings tiles of 128 x 256 weights with the rows of x that belong to them into a
-// ring of stages (bulk copies), and runs ahead over the borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile
-// into fragments of mma.sync.m16n8k16 in registers and multiply.  The MMA's order of values is free as long as both operands have it:
-// lane t of a quad takes word t of a 16-byte unit, eight values, and of x the same eight, so nothing is exchanged and every
-// shared-memory access is free of conflicts.  Where there are few tiles the CTAs of a cluster share out the values and add
-// their parts in rank order.
+// takes 128 weight rows x 8 NB rows of x; one warp brings tiles of 128 x 256 weights into a ring of stages (bulk copies) and runs
+// ahead over the borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile into fragments of mma.sync.m16n8k16 in
+// registers and multiply.  The MMA's order of values is free as long as both operands have it: lane t of a quad takes word t of a
+// 16-byte unit, eight values, and of x the same eight, so nothing is exchanged and every shared-memory access is free of
+// conflicts.  Where there are few tiles the CTAs of a cluster share out the values and add their parts in rank order.
 //
 // Operands are fp16, because two codes become fp16 in one instruction and bf16 in four (as bf16: 505 instructions per warp
-// for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  bf16 rows of x are brought to fp16 in shared memory, 256
-// values at a time, by the power of two that takes the largest finite one to 2^14 .. 2^15; the sums of a tile are multiplied back in
+// for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  Rows of x are loaded two
+// tiles ahead and put to shared memory one ahead, bf16 as fp16, 256 values at a time, by the power of two that takes the largest finite one to 2^14 .. 2^15; the sums of a tile are multiplied back in
 // fp32.  Values of at least 2^-32 of the largest are exact, smaller ones off by at most 2^-40 of it.
 #include "glqb_mx4_gemm.cuh"
 #include "glqb_launch.h"
@@ -20,11 +19,11 @@ namespace glqb {
 namespace {
 
 constexpr int MV4_WARPS = 8, MV4_THREADS = (MV4_WARPS + 1) * 32;
-constexpr int MV4_X_ROW = MX4_K * 2 + 64;        // bytes of a row of x in a stage: eight rows in all the banks
+constexpr int MV4_X_ROW = MX4_K * 2 + 64;        // bytes of a row of x: two rows in different banks
+constexpr int MV4_X_STAGES = 3;                  // of x: being written, being read, and read by warps that lag behind
 template <int FMT, int NB> struct Mv4 {
-  static constexpr int TOPS = mx4_tile_bytes(FMT) + 8 * NB * MV4_X_ROW;     // MXFP4: the rows' largest scales, with a tile's first stage
-  static constexpr int STAGE = TOPS + (FMT == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0);
-  static constexpr int STAGES = NB == 1 ? 4 : 3;                       // two CTAs per SM
+  static constexpr int STAGE = mx4_tile_bytes(FMT) + (FMT == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0);   // (the rows' largest scales)
+  static constexpr int STAGES = NB == 1 ? 4 : 3, X_STAGE = 8 * NB * MV4_X_ROW;                     // two CTAs per SM
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -50,16 +49,11 @@ __device__ __forceinline__ void multipliers(uint32_t word, int i, int top, bool 
   }
 }
 
-// A row's eight values of a lane, bf16 or fp16, to fp16 in the order 0 2 4 6 1 3 5 7; bf16 times a power of two: returned is
-// what the sums are multiplied by, its inverse (MXFP4: and the 2^-13 that fp16 operands carry).  `left`: values there are; the others become zeros.
+// A row's eight values of a lane to `p` as fp16 in the order 0 2 4 6 1 3 5 7; bf16 times a power of two: returned is what the sums are
+// multiplied by, its inverse (MXFP4: and the 2^-13 that fp16 operands carry).
 template <int FMT, typename T>
-__device__ __forceinline__ float convert8(uint8_t* p, int left) {
-  uint4 v = *reinterpret_cast<const uint4*>(p);
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  if (left < 8) {                                        // (n is a multiple of eight: all or none)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = 0u;
-  }
+__device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   if constexpr (__is_same(T, __half)) {
     *reinterpret_cast<uint4*>(p) = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632),
                                               __byte_perm(w[2], w[3], 0x7632));
@@ -90,17 +84,19 @@ template <int FMT, typename T, int NB>
 __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J) {
   constexpr int TILE = mx4_tile_bytes(FMT), STAGE = Mv4<FMT, NB>::STAGE, STAGES = Mv4<FMT, NB>::STAGES;
   extern __shared__ __align__(128) uint8_t ring[];
-  float* red = reinterpret_cast<float*>(ring + STAGES * STAGE);                      // [2][8 NB][128]
-  uint64_t* full = reinterpret_cast<uint64_t*>(red + 2 * 8 * NB * MX4_ROWS);
+  uint8_t* xs = ring + STAGES * STAGE;                                               // [X_STAGES][8 NB] rows of fp16
+  float* red = reinterpret_cast<float*>(xs + MV4_X_STAGES * Mv4<FMT, NB>::X_STAGE);  // [2][8 NB][128]
+  float* x_scale = red + 2 * 8 * NB * MX4_ROWS;                                      // [X_STAGES][8 NB]
+  uint64_t* full = reinterpret_cast<uint64_t*>(x_scale + MV4_X_STAGES * 8 * NB);
   uint64_t* empty = full + STAGES;
-  uint64_t* ready = empty + STAGES;                                                  // x as fp16
-  float* x_scale = reinterpret_cast<float*>(ready + STAGES);                         // [STAGES][8 NB]
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(x_scale + STAGES * 8 * NB);
+  uint64_t* ready = empty + STAGES;                                                  // [X_STAGES]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ready + MV4_X_STAGES);
   int* eff = const_cast<int*>(abort_flag) + 2;
   int* pre = eff + J.experts + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); mbar_init(&ready[s], MV4_WARPS); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); }
+    for (int s = 0; s < MV4_X_STAGES; ++s) mbar_init(&ready[s], MV4_WARPS);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -111,30 +107,26 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
   const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
   const int k0 = rank * J.k_tiles / J.split, k1 = (rank + 1) * J.k_tiles / J.split;
   uint32_t q = 0;                                        // stages so far
-  bool ok = true, waited = false;
+  bool ok = true;
+  Mx4Factor factor{1.0f, 1.0f};
+  if (J.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   if (warp == MV4_WARPS) {
-    for (int i = first; i < tiles && ok; i += step) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-      const uint8_t* w = J.image + ((long long)t.expert * J.m_tiles + i % J.m_tiles) * J.k_tiles * TILE;
-      const uint8_t* x = reinterpret_cast<const uint8_t*>(J.x) + (long long)(t.row0 + min(lane, t.rows - 1)) * J.x_stride * 2;
-      for (int k = k0; k < k1; ++k, ++q) {
-        const uint32_t s = q % STAGES, x_bytes = (uint32_t)min(MX4_K, J.n - k * MX4_K) * 2u;
-        if (!mbar_wait(&empty[s], ((q / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-        uint8_t* to = ring + s * STAGE;
-        if (lane == 0) {
-          const uint32_t tops = FMT == GLQB_MX4_MXFP4 && k == k0 ? 2 * MX4_ROWS : 0;
-          mbar_expect_tx(&full[s], TILE + tops + (uint32_t)t.rows * x_bytes);
-          if (tops) bulk_g2s(to + Mv4<FMT, NB>::TOPS, J.tops + ((long long)t.expert * J.m_tiles + i % J.m_tiles) * MX4_ROWS, tops, &full[s]);
-          bulk_g2s(to, w + (long long)k * TILE, TILE, &full[s]);
+    if (lane == 0) {                                     // (the weights do not depend on what runs in front of this call)
+      for (int i = first; i < tiles && ok; i += step) {
+        const int e = mx4_tile(J, eff, pre, i / J.m_tiles).expert;
+        const long long at = (long long)e * J.m_tiles + i % J.m_tiles;
+        for (int k = k0; k < k1; ++k, ++q) {
+          const uint32_t s = q % STAGES, tops = FMT == GLQB_MX4_MXFP4 && k == k0 ? 2 * MX4_ROWS : 0;
+          if (!mbar_wait(&empty[s], ((q / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&full[s], TILE + tops);
+          bulk_g2s(ring + s * STAGE, J.image + (at * J.k_tiles + k) * TILE, TILE, &full[s]);
+          if (tops) bulk_g2s(ring + s * STAGE + TILE, J.tops + at * MX4_ROWS, tops, &full[s]);
         }
-        __syncwarp();
-        if (!waited) pdl_wait();                         // (the weights do not depend on what runs in front of this call)
-        waited = true;
-        if (lane < t.rows) bulk_g2s(to + TILE + lane * MV4_X_ROW, x + (long long)k * MX4_K * 2, x_bytes, &full[s]);
       }
+      if (!ok) { *abort_flag = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
-    if (!ok) { *abort_flag = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+    pdl_wait();                                          // (a grid ends behind the one in front of it)
   } else {
     pdl_wait();                                          // (y may still be in use)
     const int g = lane >> 2, t = lane & 3, r = warp * 16 + g;
@@ -143,18 +135,44 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     const uint32_t pick = (uint32_t)(t >> 1) | (uint32_t)((t >> 1) + 2) << 4;
     int turn = 0;
     constexpr int WORDS = FMT == GLQB_MX4_MXFP4 ? 2 : 4;
-    // This warp's rows of x in stage `u`, which holds values k * 256 on of `rows` rows.  Done one stage ahead of the products.
-    auto convert = [&](uint32_t u, int rows, int k) {
-      const uint32_t s = u % STAGES;
-      if (!ok || !mbar_wait(&full[s], (u / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; return; }
-      for (int row = warp; row < rows; row += MV4_WARPS) {
-        const float down = convert8<FMT, T>(ring + s * STAGE + TILE + row * MV4_X_ROW + lane * 16, J.n - k * MX4_K - lane * 8);
+    // This warp's rows of x, a tile at a time: fetch() loads those of the next tile, put() writes what was loaded to buffer u % 3.  When a
+    // warp puts tile q + 1 all have put tile q, which each did with its products of tile q - 2 behind it: the buffer is free.
+    int next = first, next_k = k0, rows = 0;
+    Mx4Tile ahead{0, 0, 0};
+    if (first < tiles) ahead = mx4_tile(J, eff, pre, first / J.m_tiles);
+    uint4 raw[NB];
+    auto fetch = [&]() {
+      rows = next < tiles ? ahead.rows : 0;
+      if (!rows) return;
+      const int col = next_k * MX4_K + lane * 8;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int row = warp + 8 * n;
+        raw[n] = make_uint4(0, 0, 0, 0);
+        if (row < rows && col < J.n) raw[n] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(J.x) + (ahead.row0 + row) * J.x_stride + col);
+      }
+      if (++next_k == k1) {
+        next_k = k0;
+        next += step;
+        if (next < tiles) ahead = mx4_tile(J, eff, pre, next / J.m_tiles);
+      }
+    };
+    auto put = [&](uint32_t u) {
+      if (!rows) return;
+      const uint32_t s = u % MV4_X_STAGES;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int row = warp + 8 * n;
+        if (row >= rows) break;
+        const float down = put8<FMT, T>(xs + s * Mv4<FMT, NB>::X_STAGE + row * MV4_X_ROW + lane * 16, raw[n]);
         if (lane == 0) x_scale[s * 8 * NB + row] = down;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ready[s]);
     };
-    if (first < tiles) convert(0, mx4_tile(J, eff, pre, first / J.m_tiles).rows, k0);
+    fetch();
+    put(0);
+    fetch();
     // (a warp whose wait gave up goes through the rest without waiting: the others meet it at the barriers)
     for (int i = first; i < tiles; i += step) {
       const Mx4Tile tile = mx4_tile(J, eff, pre, i / J.m_tiles);
@@ -165,14 +183,15 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
       if constexpr (FMT == GLQB_MX4_NVFP4) f.b = __ldg(J.w_scale + tile.expert);
       float acc[NB][4] = {};
       for (int k = k0; k < k1; ++k, ++q) {
-        if (k + 1 < k1) convert(q + 1, tile.rows, k + 1);
-        else if (i + step < tiles) convert(q + 1, mx4_tile(J, eff, pre, (i + step) / J.m_tiles).rows, k0);
-        const uint32_t s = q % STAGES;
-        if (!ok || !mbar_wait(&ready[s], (q / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; continue; }
+        const uint32_t s = q % STAGES, xq = q % MV4_X_STAGES;
+        if (!ok || !mbar_wait(&ready[xq], (q / MV4_X_STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; continue; }
+        put(q + 1);
+        fetch();
+        if (!mbar_wait(&full[s], (q / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; continue; }
         const uint8_t* stage = ring + s * STAGE;
         if constexpr (FMT == GLQB_MX4_MXFP4) {
           if (k == k0) {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(stage + Mv4<FMT, NB>::TOPS);
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(stage + TILE);
             top[0] = p[r];
             top[1] = p[r + 8];
             plain = !__any_sync(0xFFFFFFFFu, ((top[0] | top[1]) & 256) != 0);
@@ -186,7 +205,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int a = 0; a < WORDS; ++a) sw[h][a] = *reinterpret_cast<const uint32_t*>(stage + scales0 + 128 * h + 512 * a);
-        const uint8_t* xs = stage + TILE + g * MV4_X_ROW + t * 16;
+        const uint8_t* xr = xs + xq * Mv4<FMT, NB>::X_STAGE + g * MV4_X_ROW + t * 16;
         float d[NB][2][4] = {};                          // two chains of MMAs
         auto units = [&](auto is_plain) {
 #pragma unroll
@@ -203,7 +222,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
               mx4_bytes_f16(*reinterpret_cast<const uint32_t*>(c + 1024), w[1]);
               uint4 b[NB];
 #pragma unroll
-              for (int n = 0; n < NB; ++n) b[n] = *reinterpret_cast<const uint4*>(xs + n * 8 * MV4_X_ROW + j * 64);
+              for (int n = 0; n < NB; ++n) b[n] = *reinterpret_cast<const uint4*>(xr + n * 8 * MV4_X_ROW + j * 64);
 #pragma unroll
               for (int v = 0; v < 2; ++v) {
                 uint32_t a[4];
@@ -220,13 +239,26 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           float2 down = make_float2(1.0f, 1.0f);
-          if constexpr (!__is_same(T, __half)) down = *reinterpret_cast<const float2*>(x_scale + s * 8 * NB + n * 8 + 2 * t);
+          if constexpr (!__is_same(T, __half)) down = *reinterpret_cast<const float2*>(x_scale + xq * 8 * NB + n * 8 + 2 * t);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(d[n][0][e] + d[n][1][e], e & 1 ? down.y : down.x, acc[n][e]);
         }
-        fence_async_smem();                              // (x was written here: the next copy into the stage comes behind)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      if (J.split > 1) {
+        // Each column of a shared tile has a CTA that adds it up: the parts go to its memory, part by part.
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all have begun)
+        const int owned = (8 * NB + J.split - 1) / J.split;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = n * 8 + 2 * t + (e & 1);
+            st_cluster(smem_u32(red) + (uint32_t)((rank * owned + c / J.split) * MX4_ROWS + r + 8 * (e >> 1)) * 4u, c % J.split, acc[n][e]);
+          }
+        factor = f;
+        continue;
       }
       // (two buffers in turn: a tile's sums are read before the barrier of the next one's)
       float* sums = red + (turn++ & 1) * (8 * NB * MX4_ROWS);
@@ -234,34 +266,30 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][e];
-      if (J.split == 1) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const int row = mt * MX4_ROWS + (threadIdx.x & 127);
-        if (row < J.m)
-          for (int c = threadIdx.x >> 7; c < tile.rows; c += 2)
-            mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, sums[c * MX4_ROWS + (threadIdx.x & 127)] * f.a * f.b);
-      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const int row = mt * MX4_ROWS + (threadIdx.x & 127);
+      if (row < J.m)
+        for (int c = threadIdx.x >> 7; c < tile.rows; c += 2)
+          mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, sums[c * MX4_ROWS + (threadIdx.x & 127)] * f.a * f.b);
     }
     if (!ok && lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER);
   }
   __syncwarp();
   if (J.split > 1) {                                     // (one tile per cluster)
+    if (first >= tiles || warp == MV4_WARPS) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster_sync();
     if (first < tiles && warp < MV4_WARPS) {
       const Mx4Tile t = mx4_tile(J, eff, pre, first / J.m_tiles);
-      const int r = threadIdx.x & 127, row = first % J.m_tiles * MX4_ROWS + r;
-      if (row < J.m) {
-        Mx4Factor f{1.0f, 1.0f};
-        if constexpr (FMT == GLQB_MX4_MXFP4) f = mx4_power<T>(J.tops[((long long)t.expert * J.m_tiles) * MX4_ROWS + row]);
-        else f.b = J.w_scale[t.expert];
-        const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
-        for (int c = rank + J.split * (int)(threadIdx.x >> 7); c < t.rows; c += 2 * J.split) {
-          const float v = sum_cluster(base + (uint32_t)(c * MX4_ROWS * 4), J.split);
-          mx4_put(J, (long long)(t.row0 + c) * J.y_stride + row, v * f.a * f.b);
+      const int r = threadIdx.x & 127, row = first % J.m_tiles * MX4_ROWS + r, owned = (8 * NB + J.split - 1) / J.split;
+      if (row < J.m)
+        for (int c = threadIdx.x >> 7; c * J.split + rank < t.rows; c += 2) {
+          float v = 0.0f;
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            if (s < J.split) v += red[(s * owned + c) * MX4_ROWS + r];
+          mx4_put(J, (long long)(t.row0 + c * J.split + rank) * J.y_stride + row, v * factor.a * factor.b);
         }
-      }
     }
-    cluster_sync();
   }
   __syncthreads();
   if (*abort_flag && warp == MV4_WARPS && lane == 0)     // copies still under way
@@ -278,8 +306,9 @@ cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count
     using T = decltype(type);
     constexpr int F = decltype(fmt)::value, NB = decltype(blocks)::value;
     using C = Mv4<F, NB>;
-    const size_t smem = (size_t)C::STAGES * C::STAGE + 2 * 8 * NB * MX4_ROWS * 4 + C::STAGES * (24 + 8 * NB * 4) + 8 + (size_t)(J.experts + 1) * 8;
-    return mx4_launch(mx4_mv_kernel<F, T, NB>, grid, MV4_THREADS, smem, J.split, stream, J);
+    const size_t smem = (size_t)C::STAGES * (C::STAGE + 16) + MV4_X_STAGES * (C::X_STAGE + 8 * NB * 4 + 8) + 2 * 8 * NB * MX4_ROWS * 4 + 8 + (size_t)(J.experts + 1) * 8;
+    constexpr auto K = mx4_mv_kernel<F, T, NB>;
+    return mx4_launch<K>(K, grid, MV4_THREADS, smem, J.split, stream, J);
   };
   using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
   using N = std::integral_constant<int, GLQB_MX4_NVFP4>;

@@ -11,6 +11,7 @@ gradients.  No counterpart in the reference, whose formats are the E8 shell and 
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -35,7 +36,7 @@ class Mx4Tensor(NamedTuple):
 
 class Mx4Weight:
     """Weights laid out for the products (``mx4_pack``): (out_features, in_features), or one such matrix per expert."""
-    __slots__ = ("image", "tensor_scale", "format", "experts", "out_features", "in_features", "_desc", "_ref")
+    __slots__ = ("image", "tensor_scale", "format", "experts", "out_features", "in_features", "_desc", "_ref", "_index")
 
     def __init__(self, image, tensor_scale, format, experts, out_features, in_features):
         self.image, self.tensor_scale, self.format, self.experts = image, tensor_scale, format, experts
@@ -43,24 +44,25 @@ class Mx4Weight:
         self._desc = _lib.Mx4WeightDesc(image.data_ptr(), tensor_scale.data_ptr() if tensor_scale is not None else 0,
                                         _FORMATS[format], experts or 1, out_features, in_features)
         self._ref = C.byref(self._desc)
+        self._index = image.get_device()
 
 
-class _on:
-    """The device of a call made current: kernels of another device's tensors are launched there."""
+_get_device, _set_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_setDevice, torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, index):
-        self.index = index
 
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch._C._cuda_setDevice(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch._C._cuda_setDevice(self.before)
-        return False
+def _call(index, what, fn, *args):
+    """fn(*args, current stream) with the tensors' device current: its kernels are launched there."""
+    before = _get_device()
+    if before == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        _set_device(index)
+        try:
+            rc = fn(*args, _raw_stream(index))
+        finally:
+            _set_device(before)
+    if rc:
+        _lib.check(rc, what)
 
 
 def _format(format):
@@ -97,7 +99,8 @@ def _scale_ptr(t, x, name, count=1):
 def _rows(x, cols):
     """x (..., cols) as rows of consecutive values; rows that overlap (an expanded tensor) are copied."""
     x2 = x if x.dim() == 2 else x.reshape(-1, cols)
-    if (cols > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < cols):
+    apart, step = x2.stride()
+    if (step != 1 and cols > 1) or (apart < cols and x2.shape[0] > 1):
         x2 = x2.contiguous()
     return x2
 
@@ -110,65 +113,61 @@ def mx4_quantize(x, format="mxfp4", tensor_scale=None) -> Mx4Tensor:
     fmt = _format(format)
     _cuda(x, "x")
     dt = _dtype(x.dtype, "x")
-    if x.dim() == 0:
+    shape = x.shape
+    if not shape:
         raise ValueError("glq_b200: x needs at least one dimension")
-    cols = x.shape[-1]
-    x2 = _rows(x, cols) if x.numel() else x.reshape(0, max(cols, 1))
-    codes = torch.empty(x.shape[:-1] + ((cols + 1) // 2,), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(x.shape[:-1] + (-(-cols // _BLOCK[format]),), dtype=torch.uint8, device=x.device)
+    cols, lead, some = shape[-1], shape[:-1], x.numel() > 0
+    codes = x.new_empty(lead + ((cols + 1) // 2,), dtype=torch.uint8)
+    scales = x.new_empty(lead + (-(-cols // _BLOCK[format]),), dtype=torch.uint8)
     given = own = None
     if format == "nvfp4":
         if tensor_scale is None:
-            own = torch.empty(2, dtype=torch.float32, device=x.device)
+            own = x.new_empty((2,), dtype=torch.float32)
         else:
             given = _scale_ptr(tensor_scale, x, "tensor_scale")
     elif tensor_scale is not None:
         raise ValueError('glq_b200: "mxfp4" has no tensor_scale')
-    if x.numel():
-        with _on(x.get_device()) as stream:
-            _lib.check(_lib.load().glqb_mx4_quantize(x2.data_ptr(), dt, x2.stride(0), x2.shape[0], cols, fmt, given,
-                                                     own.data_ptr() if own is not None else None, codes.data_ptr(),
-                                                     scales.data_ptr(), stream), "mx4_quantize")
+    if some:
+        x2 = _rows(x, cols)
+        _call(x.get_device(), "mx4_quantize", _lib.load().glqb_mx4_quantize, x2.data_ptr(), dt, x2.stride(0), x2.shape[0], cols, fmt, given,
+              own.data_ptr() if own is not None else None, codes.data_ptr(), scales.data_ptr())
     elif own is not None:
         own.fill_(2.0 ** -126)
     return Mx4Tensor(codes, scales, format, cols, own[:1] if own is not None else tensor_scale)
 
 
 def _checked(q: Mx4Tensor):
-    """(format, rows, values per row, matrices) of an Mx4Tensor."""
-    fmt = _format(q.format)
-    _cuda(q.codes, "codes")
-    _same_device(q.scales, q.codes, "scales")
-    cols, lead = int(q.cols), q.codes.shape[:-1]
-    if q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8 or q.codes.dim() < 1:
+    """(format, rows, values per row, scales of the whole) of an Mx4Tensor."""
+    codes, scales, format, cols, t = q
+    fmt = _format(format)
+    _cuda(codes, "codes")
+    _same_device(scales, codes, "scales")
+    shape = codes.shape
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not shape:
         raise ValueError("glq_b200: codes and scales are uint8 tensors of stored rows")
-    if q.codes.shape[-1] != (cols + 1) // 2 or q.scales.shape != lead + (-(-cols // _BLOCK[q.format]),):
-        raise ValueError(f"glq_b200: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} are not {q.format} rows of {cols} values")
-    rows = 1
-    for d in lead:
-        rows *= d
-    scales = 0
-    if q.format == "nvfp4":
-        if q.tensor_scale is None:
+    lead = shape[:-1]
+    if shape[-1] != (cols + 1) // 2 or scales.shape != lead + (-(-cols // _BLOCK[format]),):
+        raise ValueError(f"glq_b200: codes {tuple(shape)} and scales {tuple(scales.shape)} are not {format} rows of {cols} values")
+    count = 0
+    if format == "nvfp4":
+        if t is None:
             raise ValueError('glq_b200: "nvfp4" needs its tensor_scale')
-        scales = q.tensor_scale.numel()
-        if scales != 1 and not (len(lead) == 2 and scales == lead[0]):
-            raise ValueError(f"glq_b200: {scales} tensor scales for rows of {tuple(lead)}")
-        _scale_ptr(q.tensor_scale, q.codes, "tensor_scale", scales)
-    return fmt, rows, cols, scales
+        count = t.numel()
+        if count != 1 and not (len(lead) == 2 and count == lead[0]):
+            raise ValueError(f"glq_b200: {count} tensor scales for rows of {tuple(lead)}")
+        _scale_ptr(t, codes, "tensor_scale", count)
+    return fmt, math.prod(lead), cols, count
 
 
 def mx4_dequantize(q: Mx4Tensor, dtype=torch.bfloat16) -> torch.Tensor:
     """The values (..., cols) an ``Mx4Tensor`` stands for, formed in fp32 and rounded to ``dtype``."""
-    fmt, rows, cols, scales = _checked(q)
+    fmt, rows, cols, count = _checked(q)
     dt = _dtype(dtype, "dtype")
     codes, sc = q.codes.contiguous(), q.scales.contiguous()
-    out = torch.empty(codes.shape[:-1] + (cols,), dtype=dtype, device=codes.device)
-    if out.numel():
-        with _on(codes.get_device()) as stream:
-            _lib.check(_lib.load().glqb_mx4_dequantize(codes.data_ptr(), sc.data_ptr(),
-                                                       q.tensor_scale.data_ptr() if scales else None, rows // max(scales, 1),
-                                                       rows, cols, fmt, out.data_ptr(), dt, stream), "mx4_dequantize")
+    out = codes.new_empty(codes.shape[:-1] + (cols,), dtype=dtype)
+    if rows and cols:
+        _call(codes.get_device(), "mx4_dequantize", _lib.load().glqb_mx4_dequantize, codes.data_ptr(), sc.data_ptr(),
+              q.tensor_scale.data_ptr() if count else None, rows // (count or 1), rows, cols, fmt, out.data_ptr(), dt)
     return out
 
 
@@ -183,9 +182,8 @@ def mx4_pack(q: Mx4Tensor) -> Mx4Weight:
         raise ValueError(f"glq_b200: empty weights, codes of {tuple(q.codes.shape)}")
     codes, sc = q.codes.contiguous(), q.scales.contiguous()
     lib = _lib.load()
-    image = torch.empty(lib.glqb_mx4_image_bytes(fmt, experts or 1, m, n), dtype=torch.uint8, device=codes.device)
-    with _on(codes.get_device()) as stream:
-        _lib.check(lib.glqb_mx4_pack(codes.data_ptr(), sc.data_ptr(), fmt, experts or 1, m, n, image.data_ptr(), stream), "mx4_pack")
+    image = codes.new_empty((lib.glqb_mx4_image_bytes(fmt, experts or 1, m, n),))
+    _call(codes.get_device(), "mx4_pack", lib.glqb_mx4_pack, codes.data_ptr(), sc.data_ptr(), fmt, experts or 1, m, n, image.data_ptr())
     t = q.tensor_scale
     if scales:
         t = t.reshape(1).expand(experts or 1).contiguous() if scales == 1 else t.reshape(-1)
@@ -200,39 +198,38 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
-def _product(x, w, offsets, quantize_input, input_scale, y, accumulate, clear_rest):
-    """The call itself: x and y two-dimensional with consecutive values in a row."""
-    dt = _DTYPES[x.dtype]
-    xs = None
-    if input_scale is not None:
-        if not quantize_input or w.format != "nvfp4":
-            raise ValueError('glq_b200: input_scale belongs to quantize_input with "nvfp4" weights')
-        xs = _scale_ptr(input_scale, x, "input_scale")
-    if x.shape[0] == 0:
-        return
-    lib = _lib.load()
-    with _on(x.get_device()) as stream:
-        size = lib.glqb_mx4_workspace_bytes(w._ref, x.shape[0], x.stride(0), x.data_ptr(), quantize_input)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        rc = lib.glqb_mx4_product(w._ref, x.data_ptr(), dt, x.stride(0), x.shape[0], offsets.data_ptr() if offsets is not None else None,
-                                  offsets is not None and offsets.dtype == torch.int64, quantize_input, xs, y.data_ptr(),
-                                  _DTYPES[y.dtype], y.stride(0), accumulate, clear_rest, ws.data_ptr() if size else None, size, stream)
-    if rc:
-        _lib.check(rc, "mx4_product")
-    _RAN_ON.add(x.get_device())
-
-
-def _input(x, w, quantize_input):
-    if not isinstance(w, Mx4Weight):
+def _input(x, w, quantize_input, input_scale):
+    """Checks of x and the weight; (x's type, pointer of its scale)."""
+    if w.__class__ is not Mx4Weight:
         raise ValueError("glq_b200: weight is what mx4_pack returns")
     _cuda(x, "x")
-    if x.get_device() != w.image.get_device():
+    if x.get_device() != w._index:
         raise ValueError(f"glq_b200: x is on {x.device}, the weight on {w.image.device}")
-    _dtype(x.dtype, "x")
-    if x.dtype == torch.float32 and not quantize_input:
+    dt = _dtype(x.dtype, "x")
+    if dt == _lib.DT_F32 and not quantize_input:
         raise ValueError("glq_b200: x is bf16 or fp16 (fp32 with quantize_input only)")
-    if x.dim() < 1 or x.shape[-1] != w.in_features:
-        raise ValueError(f"glq_b200: x of {tuple(x.shape)} for a weight of {w.in_features} inputs")
+    shape = x.shape
+    if not shape or shape[-1] != w.in_features:
+        raise ValueError(f"glq_b200: x of {tuple(shape)} for a weight of {w.in_features} inputs")
+    if input_scale is None:
+        return dt, None
+    if not quantize_input or w.format != "nvfp4":
+        raise ValueError('glq_b200: input_scale belongs to quantize_input with "nvfp4" weights')
+    return dt, _scale_ptr(input_scale, x, "input_scale")
+
+
+def _product(x, dt, w, offsets, quantize_input, xs, y, y_dt, y_stride, accumulate, clear_rest):
+    """The call itself: x and y two-dimensional with consecutive values in a row."""
+    lib, rows, apart, at = _lib.load(), x.shape[0], x.stride(0), x.data_ptr()
+    ws, size = None, 0
+    if quantize_input or at & 15 or apart & 7 or w.in_features & 7:
+        size = lib.glqb_mx4_workspace_bytes(w._ref, rows, apart, at, quantize_input)
+        if size:
+            ws = x.new_empty((size,), dtype=torch.uint8)
+    _call(w._index, "mx4_product", lib.glqb_mx4_product, w._ref, at, dt, apart, rows, offsets.data_ptr() if offsets is not None else None,
+          offsets is not None and offsets.dtype is torch.int64, quantize_input, xs, y.data_ptr(), y_dt, y_stride, accumulate, clear_rest,
+          ws.data_ptr() if size else None, size)
+    _RAN_ON.add(w._index)
 
 
 def mx4_linear(x, weight: Mx4Weight, *, quantize_input=False, input_scale=None, out_dtype=None, accumulate_into=None):
@@ -241,26 +238,26 @@ def mx4_linear(x, weight: Mx4Weight, *, quantize_input=False, input_scale=None, 
     ``input_scale``, one fp32 value, or by the scale of the whole of x), and the tensor cores multiply 4-bit values, at four times
     their 16-bit rate.  ``accumulate_into`` adds the result to that dense (..., m) tensor in place (residual add, before the
     rounding) and returns it."""
-    _input(x, weight, quantize_input)
+    dt, xs = _input(x, weight, quantize_input, input_scale)
     if weight.experts is not None:
         raise ValueError("glq_b200: mx4_linear takes one matrix, not one per expert")
-    n, m = weight.in_features, weight.out_features
-    rows = x.numel() // n
-    if accumulate_into is not None:
-        _same_device(accumulate_into, x, "accumulate_into")
+    m, shape = weight.out_features, x.shape
+    x2 = _rows(x, weight.in_features)
+    rows = x2.shape[0]
+    if accumulate_into is None:
+        out = x.new_empty(shape[:-1] + (m,)) if out_dtype is None else x.new_empty(shape[:-1] + (m,), dtype=out_dtype)
+    else:
         out = accumulate_into
+        _same_device(out, x, "accumulate_into")
         if out_dtype not in (None, out.dtype):
             raise ValueError(f"glq_b200: accumulate_into is {out.dtype}, out_dtype {out_dtype}")
         if out.dim() < 1 or out.shape[-1] != m or out.numel() != rows * m or not out.is_contiguous():
             raise RuntimeError("glq_b200: accumulate_into must be a dense (tokens, out_features) tensor")
-    else:
-        out = torch.empty(x.shape[:-1] + (m,), dtype=out_dtype or x.dtype, device=x.device)
-    _dtype(out.dtype, "the result")
-    if rows:
-        x2 = _rows(x, n)
-        if accumulate_into is not None and _overlap(x2, out):
+        if rows and _overlap(x2, out):
             raise ValueError("glq_b200: accumulate_into overlaps x")
-        _product(x2, weight, None, bool(quantize_input), input_scale, out.view(rows, m), accumulate_into is not None, False)
+    y_dt = _dtype(out.dtype, "the result")
+    if rows:
+        _product(x2, dt, weight, None, bool(quantize_input), xs, out, y_dt, m, accumulate_into is not None, False)
     return out
 
 
@@ -269,32 +266,33 @@ def mx4_grouped_linear(x, weight: Mx4Weight, offsets, *, quantize_input=False, i
     (experts, m, n) weight: (rows, m).  ``offsets``: experts + 1 ascending integers (int32 or int64) on the device, any number of
     rows per expert, none included; nothing is read back.  Rows of no expert (in front of offsets[0], behind offsets[experts])
     are zero in a new result and stay as they are in a given ``out`` (rows, m), whose rows may lie apart.  Offsets outside
-    0 .. rows are held to that range, and one that is less than the one before it counts as that one.  At most 1024 experts.  The other arguments as for
-    ``mx4_linear``; "nvfp4" inputs without ``input_scale`` take the scale of rows offsets[0] .. offsets[experts] - 1."""
-    _input(x, weight, quantize_input)
+    0 .. rows are held to that range, and one that is less than the one before it counts as that one.  At most 1024 experts.
+    The other arguments as for ``mx4_linear``; "nvfp4" inputs without ``input_scale`` take the scale of rows
+    offsets[0] .. offsets[experts] - 1."""
+    dt, xs = _input(x, weight, quantize_input, input_scale)
     if weight.experts is None:
         raise ValueError("glq_b200: mx4_grouped_linear takes one matrix per expert")
     if x.dim() != 2:
         raise ValueError(f"glq_b200: x is (rows, n), got {tuple(x.shape)}")
     _same_device(offsets, x, "offsets")
-    if offsets.dtype not in (torch.int32, torch.int64) or offsets.dim() != 1 or offsets.numel() != weight.experts + 1 or not offsets.is_contiguous():
+    if offsets.dtype not in (torch.int32, torch.int64) or offsets.shape != (weight.experts + 1,) or not offsets.is_contiguous():
         raise ValueError(f"glq_b200: offsets must be {weight.experts + 1} int32 or int64 values, got {tuple(offsets.shape)} of {offsets.dtype}")
     rows, m = x.shape[0], weight.out_features
+    x2 = _rows(x, weight.in_features)
     fresh = out is None
     if fresh:
-        out = torch.empty(rows, m, dtype=out_dtype or x.dtype, device=x.device)
+        out = x.new_empty((rows, m)) if out_dtype is None else x.new_empty((rows, m), dtype=out_dtype)
     else:
         _same_device(out, x, "out")
         if out_dtype not in (None, out.dtype):
             raise ValueError(f"glq_b200: out is {out.dtype}, out_dtype {out_dtype}")
         if out.shape != (rows, m) or (m > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < m):
             raise ValueError(f"glq_b200: out must be ({rows}, {m}) with consecutive values in a row, got {tuple(out.shape)}")
-    _dtype(out.dtype, "the result")
-    if rows:
-        x2 = _rows(x, weight.in_features)
-        if not fresh and _overlap(x2, out):
+        if rows and _overlap(x2, out):
             raise ValueError("glq_b200: out overlaps x")
-        _product(x2, weight, offsets, bool(quantize_input), input_scale, out, False, fresh)
+    y_dt = _dtype(out.dtype, "the result")
+    if rows:
+        _product(x2, dt, weight, offsets, bool(quantize_input), xs, out, y_dt, out.stride(0), False, fresh)
     return out
 
 
@@ -302,5 +300,4 @@ def mx4_check_status() -> None:
     """Synchronise the devices that products ran on and raise RuntimeError (code GLQB_E_DEVICE) if a bounded wait in one of them
     gave up since the last call: the results of that run are invalid."""
     for index in sorted(_RAN_ON):
-        with _on(index):
-            _lib.check(_lib.load().glqb_mx4_status(None), "mx4 status")
+        _call(index, "mx4 status", lambda stream: _lib.load().glqb_mx4_status(None))
