@@ -419,7 +419,7 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
 
 // What a call launches, by its sizes alone.
 struct Form {
-  int tn, max_tiles, split, x_scales, n_pad;
+  int tn, max_tiles, split, pair, x_scales, n_pad;
   bool align, mv;
   size_t image, bytes;        // of the workspace: x in 4 bits or aligned, then two floats
 };
@@ -452,6 +452,7 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
   const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K, tiles = f.max_tiles * mt;
   // CTAs that share a tile's sum: as many as the SMs hold at once
   f.split = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, kt), (f.mv ? 2 : 1) * sms / std::max<long long>(1, tiles)));
+  f.pair = !quantize && !f.mv && f.split == 1 && f.tn >= 96 && mt > 1;
   if (quantize) {
     f.x_scales = mx4_x_scale_bytes(w->format, f.tn);
     f.image = (size_t)f.max_tiles * kt * ((size_t)f.tn * 128 + f.x_scales);
@@ -506,6 +507,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.tn = f.tn;
   J.max_tiles = f.max_tiles;
   J.split = f.split;
+  J.pair = f.pair;
   J.y = y;
   J.y_stride = y_stride;
   J.y_dtype = y_dtype;

@@ -42,11 +42,68 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
                : "r"(taddr)
                : "memory");
 }
-// A from tensor memory, B from shared memory
+// A from tensor memory, B from shared memory; of a pair of CTAs: 128 rows from each one's tensor memory, half of the columns from each
+// one's shared memory
+template <bool PAIR>
 __device__ __forceinline__ void umma16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
-               "r"(idesc), "r"(accumulate)
-               : "memory");
+  if constexpr (PAIR)
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+  else
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// arrives at the barrier (of a pair: of both CTAs) when the MMAs issued so far are done
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+                 : "memory");
+  else
+    umma_commit(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void alloc_all(uint32_t* slot) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, 512);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void dealloc_all(uint32_t taddr) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+  else tmem_dealloc(taddr, 512);
+}
+// arrives at the first CTA's barrier, from either CTA of a pair
+template <bool PAIR>
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  if constexpr (PAIR) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+  } else {
+    mbar_arrive(bar);
+  }
+}
+// mbar_wait for what the other CTA of a pair has released
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t it = 0; it < GM_SPIN_LIMIT; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 63u) == 63u && *abort_flag) return false;
+  }
+  return false;
 }
 // both from shared memory, 4-bit, scales of blocks in tensor memory
 template <int FMT>
@@ -68,9 +125,9 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) 
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
   return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
-// fp32 accumulator, both operands K-major, M = 128; `type` 0: fp16, 1: bf16
-__device__ __forceinline__ uint32_t idesc16(int type, int cols) {
-  return (1u << 4) | (uint32_t)type << 7 | (uint32_t)type << 10 | (uint32_t)(cols >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+// fp32 accumulator, both operands K-major; `type` 0: fp16, 1: bf16
+__device__ __forceinline__ uint32_t idesc16(int type, int rows, int cols) {
+  return (1u << 4) | (uint32_t)type << 7 | (uint32_t)type << 10 | (uint32_t)(cols >> 3) << 17 | (uint32_t)(rows >> 4) << 24;
 }
 // e2m1 operands, K = 64; scales e8m0 or e4m3, `sf`: the first of a word's four bytes that an instruction takes
 template <int FMT>
@@ -81,7 +138,7 @@ __device__ __forceinline__ uint32_t idesc4(int cols, uint32_t sf) {
 // ---- parts of both kernels ------------------------------------------------------------------------
 struct __align__(16) Bars {     // in shared memory
   uint8_t turn[4][2048];       // results on their way out, per draining warp
-  uint64_t full_w[8], empty_w[8], full_x[8], empty_x[8], full_a[2], empty_a[2], acc_full[2], acc_empty[2], drain;
+  uint64_t full_w[8], empty_w[8], full_x[8], empty_x[8], full_a[4], empty_a[4], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   volatile int abort;
 };
@@ -163,175 +220,220 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int
 }
 
 // ---- 16-bit activations ---------------------------------------------------------------------------
-// Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by eight warps straight into tensor memory as
+// Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by sixteen warps straight into tensor memory as
 // the A operand (thread = row, 64 values = 32 columns), activations by TMA as 64-value boxes with the 128-byte swizzle.  A step
-// is 128 values: eight MMAs.  Warp 0 issues MMAs, warp 1 loads, warps 4-7 drain, warps 8-15 decode.
-constexpr int G16_THREADS = 512, G16_W_STAGES = 3, G16_MAX_TN = 192;
-constexpr int G16_A0 = 2 * G16_MAX_TN;             // tensor memory: two accumulators, then two stages of A of 64 columns
+// is 128 values, eight MMAs; two groups of eight warps decode the steps in turn.  Warp 0 issues MMAs, warp 1 loads, warp 2 of a
+// pair's second CTA reports its activations, warps 4-7 drain, 8-23 decode.
+//
+// With wide tiles what bounds one CTA is shared memory: of 128 bytes a clock, writing and reading the activations of 192 rows takes
+// 125 (2048 tokens of 14336 x 4096 317 us; without the loads 202).  Two CTAs therefore share a tile of 256 weight rows (PAIR): each
+// brings half of the activations, the first one's thread issues for both.  What is to arrive at the issuing thread comes from
+// both CTAs; what it releases goes to both.
+constexpr int G16_THREADS = 768, G16_W_STAGES = 3, G16_MAX_TN = 192, G16_PRODUCERS = 8;
 
-struct Mx4Ring { int x_stages, box_rows, x_half; };  // stages of x, rows per box, bytes of 64 values of a tile
+struct Mx4Ring { int x_stages, box_rows, x_half, a_stages, acc_cols; };  // stages of x, rows per box, bytes of 64 values of a CTA's rows
 
-template <int FMT, typename T>
+struct Pos {                   // a place in a ring, and the parity of its round
+  uint32_t s = 0, phase = 0;
+  __device__ __forceinline__ void add(uint32_t d, uint32_t n) {
+    s += d;
+    while (s >= n) { s -= n; phase ^= 1u; }
+  }
+  __device__ __forceinline__ void back(uint32_t n) {
+    if (s == 0) { s = n; phase ^= 1u; }
+    --s;
+  }
+};
+
+template <int FMT, typename T, bool PAIR>
 __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid_constant__ Mx4Job J, const __grid_constant__ CUtensorMap map, Mx4Ring R) {
+  constexpr int TILE = mx4_tile_bytes(FMT);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* w_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* x_base = w_base + G16_W_STAGES * mx4_tile_bytes(FMT);
+  uint8_t* x_base = w_base + G16_W_STAGES * TILE;
   Bars& B = *reinterpret_cast<Bars*>(x_base + R.x_stages * 2 * R.x_half);
   int* eff = reinterpret_cast<int*>(&B + 1);
   int* pre = eff + J.experts + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a CTA's place among those that work on one tile: of a pair (weight rows), or of a split (values)
+  const int ranks = PAIR ? 2 : J.split, first = blockIdx.x / ranks, step = gridDim.x / ranks, rank = blockIdx.x % ranks;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < G16_W_STAGES; ++s) { mbar_init(&B.full_w[s], 1); mbar_init(&B.empty_w[s], 8); }
+    for (int s = 0; s < G16_W_STAGES; ++s) { mbar_init(&B.full_w[s], 1); mbar_init(&B.empty_w[s], 2 * G16_PRODUCERS); }
     for (int s = 0; s < R.x_stages; ++s) { mbar_init(&B.full_x[s], 1); mbar_init(&B.empty_x[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&B.full_a[s], 8); mbar_init(&B.empty_a[s], 1); mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], 4); }
+    for (int s = 0; s < R.a_stages; ++s) { mbar_init(&B.full_a[s], PAIR ? 2 * G16_PRODUCERS + 1 : G16_PRODUCERS); mbar_init(&B.empty_a[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], PAIR ? 8 : 4); }
     mbar_init(&B.drain, 1);
     B.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 0) {
-    tmem_alloc(&B.tmem, 512);
-    tmem_relinquish();
-  }
+  if (warp == 0) alloc_all<PAIR>(&B.tmem);
   tc_fence_before();
   if (J.offsets) pdl_wait();
   mx4_groups(J, eff, pre);                         // (ends with a block barrier)
+  if constexpr (PAIR) cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = B.tmem;
-  const int tiles = min(pre[J.experts], J.max_tiles) * J.m_tiles;
-  const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
-  const int k0 = rank * J.k_tiles / J.split, k1 = (rank + 1) * J.k_tiles / J.split;      // this CTA's tiles of 256 values
-  const int steps = min(2 * k1, (J.n + 127) / 128) - 2 * k0;                             // of 128
+  const uint32_t tmem = B.tmem, tmem_a = tmem + 2 * R.acc_cols;
+  const int m_tiles = PAIR ? (J.m_tiles + 1) / 2 : J.m_tiles;
+  const int tiles = min(pre[J.experts], J.max_tiles) * m_tiles;
+  const int k0 = PAIR ? 0 : rank * J.k_tiles / J.split, k1 = PAIR ? J.k_tiles : (rank + 1) * J.k_tiles / J.split;     // tiles of 256 values
+  const int steps = min(2 * k1, (J.n + 127) / 128) - 2 * k0;                                                          // of 128
+  // this CTA's row tile (the second CTA of a pair may have none: it computes the one before again and stores nothing)
+  auto row_tile = [&](int i) { return PAIR ? 2 * (i % m_tiles) + rank : i % m_tiles; };
+  auto cols_of = [&](const Mx4Tile& t) { return PAIR ? (t.rows + 31) & ~31 : (t.rows + 15) & ~15; };
   uint32_t loads_w = 0, loads_x = 0;
   bool ok = true;
 
   if (warp == 0) {
-    uint32_t q = 0, seq = 0;
-    const uint32_t x0 = smem_u32(x_base);
-    for (int i = first; i < tiles && ok; i += step, ++seq) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-      const uint32_t idesc = idesc16(__is_same(T, __half) ? 0 : 1, (t.rows + 15) & ~15), d = tmem + (seq & 1u) * G16_MAX_TN;
-      if (!mbar_wait(&B.acc_empty[seq & 1u], ((seq >> 1) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
-      tc_fence_after();
-      for (int k = 0; k < steps; ++k, ++q) {
-        const uint32_t sa = q & 1u, sx = q % R.x_stages;
-        if (!mbar_wait(&B.full_x[sx], (q / R.x_stages) & 1u, &B.abort) || !mbar_wait(&B.full_a[sa], (q >> 1) & 1u, &B.abort)) { ok = false; break; }
+    if (!PAIR || rank == 0) {
+      Pos a, x, acc;
+      const uint32_t x0 = smem_u32(x_base);
+      for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+        const uint32_t idesc = idesc16(__is_same(T, __half) ? 0 : 1, PAIR ? 256 : 128, cols_of(t)), d = tmem + acc.s * R.acc_cols;
+        if (!(PAIR ? mbar_wait_cluster(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort) : mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort))) { ok = false; break; }
         tc_fence_after();
-        if (elect_one()) {
-          const uint32_t a = tmem + G16_A0 + sa * 64u, b = x0 + sx * 2u * R.x_half;
-          const uint64_t d0 = umma_desc_sw128(b), d1 = umma_desc_sw128(b + R.x_half);
+        for (int k = 0; k < steps; ++k, a.add(1, R.a_stages), x.add(1, R.x_stages)) {
+          if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) ||
+              !(PAIR ? mbar_wait_cluster(&B.full_a[a.s], a.phase, &B.abort) : mbar_wait(&B.full_a[a.s], a.phase, &B.abort))) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t at = tmem_a + a.s * 64u, b = x0 + x.s * 2u * R.x_half;
+            const uint64_t d0 = umma_desc_sw128(b), d1 = umma_desc_sw128(b + R.x_half);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma16(d, a + 8u * j, d0 + 2u * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
+            for (int j = 0; j < 4; ++j) umma16<PAIR>(d, at + 8u * j, d0 + 2u * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma16(d, a + 32u + 8u * j, d1 + 2u * j, idesc, 1u);
-          umma_commit(&B.empty_x[sx]);
-          umma_commit(&B.empty_a[sa]);
-          if (k + 1 == steps) umma_commit(&B.acc_full[seq & 1u]);
+            for (int j = 0; j < 4; ++j) umma16<PAIR>(d, at + 32u + 8u * j, d1 + 2u * j, idesc, 1u);
+            commit<PAIR>(&B.empty_x[x.s]);
+            commit<PAIR>(&B.empty_a[a.s]);
+            if (k + 1 == steps) commit<PAIR>(&B.acc_full[acc.s]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
+      if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
     }
-    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
   } else if (warp == 1) {
     if (lane == 0) {
+      Pos w, x;
       for (int i = first; i < tiles && ok; i += step) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + i % J.m_tiles) * J.k_tiles + k0) * mx4_tile_bytes(FMT);
-        const int boxes = (t.rows + R.box_rows - 1) / R.box_rows;
-        for (int k = 0; k < steps && ok; ++k, ++loads_x) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
+        const int rows = PAIR ? cols_of(t) / 2 : t.rows, row0 = t.row0 + (PAIR ? rank * rows : 0), boxes = (rows + R.box_rows - 1) / R.box_rows;
+        for (int k = 0; k < steps && ok; ++k, ++loads_x, x.add(1, R.x_stages)) {
           if ((k & 1) == 0) {
-            const uint32_t s = loads_w % G16_W_STAGES;
-            if (!mbar_wait(&B.empty_w[s], ((loads_w / G16_W_STAGES) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
-            mbar_expect_tx(&B.full_w[s], mx4_tile_bytes(FMT));
-            bulk_g2s(w_base + s * mx4_tile_bytes(FMT), src + (long long)(k >> 1) * mx4_tile_bytes(FMT), mx4_tile_bytes(FMT), &B.full_w[s]);
+            if (!mbar_wait(&B.empty_w[w.s], w.phase ^ 1u, &B.abort)) { ok = false; break; }
+            mbar_expect_tx(&B.full_w[w.s], TILE);
+            bulk_g2s(w_base + w.s * TILE, src + (long long)(k >> 1) * TILE, TILE, &B.full_w[w.s]);
             ++loads_w;
+            w.add(1, G16_W_STAGES);
           }
           if (loads_x == 0) pdl_wait();            // (the weights do not depend on what runs in front of this call)
-          const uint32_t s = loads_x % R.x_stages;
-          if (!mbar_wait(&B.empty_x[s], ((loads_x / R.x_stages) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
-          mbar_expect_tx(&B.full_x[s], (uint32_t)(2 * boxes * R.box_rows * 128));
-          uint8_t* dst = x_base + s * 2 * R.x_half;
+          if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
+          mbar_expect_tx(&B.full_x[x.s], (uint32_t)(2 * boxes * R.box_rows * 128));
+          uint8_t* dst = x_base + x.s * 2 * R.x_half;
           for (int b = 0; b < boxes; ++b) {
-            tma_load_2d(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, t.row0 + b * R.box_rows, &B.full_x[s]);
-            tma_load_2d(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, t.row0 + b * R.box_rows, &B.full_x[s]);
+            tma_load_2d(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, row0 + b * R.box_rows, &B.full_x[x.s]);
+            tma_load_2d(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, row0 + b * R.box_rows, &B.full_x[x.s]);
           }
         }
       }
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
+  } else if (warp == 2) {
+    if (PAIR && rank == 1 && lane == 0) {
+      Pos a, x;
+      for (int i = first; i < tiles && ok; i += step)
+        for (int k = 0; k < steps; ++k, a.add(1, R.a_stages), x.add(1, R.x_stages)) {
+          // (the stage of A first: its barrier is in the round that this arrival counts for)
+          if (!mbar_wait(&B.empty_a[a.s], a.phase ^ 1u, &B.abort) || !mbar_wait(&B.full_x[x.s], x.phase, &B.abort)) { ok = false; break; }
+          arrive_first<PAIR>(&B.full_a[a.s]);
+        }
+      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+    }
   } else if (warp >= 8) {
-    // warps 8-11 take the first 64 values of a step, 12-15 the others; a warp the 32 rows of its quarter of tensor memory
-    const int half = (warp - 8) >> 2, r = (warp & 3) * 32 + lane;
-    uint32_t q = 0, wq = 0;
+    // of a group's eight warps four take the first 64 values of a step, four the others; a warp the 32 rows of its quarter of tensor memory
+    const int group = (warp - 8) >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
+    const uint32_t to = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + half * 32u;
+    Pos a, w;
+    a.add(group, R.a_stages);
     for (int i = first; i < tiles && ok; i += step) {
       int top = 0;
       if constexpr (FMT == GLQB_MX4_MXFP4) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-        top = J.tops[((long long)t.expert * J.m_tiles + i % J.m_tiles) * MX4_ROWS + r] & 0xFF;
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+        top = J.tops[((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * MX4_ROWS + r] & 0xFF;
       }
-      for (int k = 0; k < steps; ++k, ++q) {
-        const uint32_t s = wq % G16_W_STAGES, sa = q & 1u;
-        if ((k & 1) == 0 && !mbar_wait(&B.full_w[s], (wq / G16_W_STAGES) & 1u, &B.abort)) { ok = false; break; }
-        const uint8_t* tile = w_base + s * mx4_tile_bytes(FMT);
-        const int c = (k & 1) * 4 + half * 2;      // 16-byte units of a row: two of them
-        uint32_t a[32];
-        const uint8_t* codes = tile + (r >> 3) * 1024 + (r & 7) * 128;
-        const uint8_t* sc = tile + MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4;
-        uint32_t sw;
-        if constexpr (FMT == GLQB_MX4_MXFP4) sw = *reinterpret_cast<const uint32_t*>(sc + (c >> 2) * 512) >> (8 * (c & 3));
-        else sw = *reinterpret_cast<const uint32_t*>(sc + (c >> 1) * 512);
+      for (int k = group; k < steps + group; k += 2, w.add(1, G16_W_STAGES)) {
+        if (!mbar_wait(&B.full_w[w.s], w.phase, &B.abort)) { ok = false; break; }
+        const uint8_t* tile = w_base + w.s * TILE;
+        uint32_t v[32];
+        if (k < steps) {
+          const int c = group * 4 + half * 2;      // 16-byte units of a row: two of them
+          const uint8_t* codes = tile + (r >> 3) * 1024 + (r & 7) * 128;
+          const uint8_t* sc = tile + MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4;
+          uint32_t sw;
+          if constexpr (FMT == GLQB_MX4_MXFP4) sw = *reinterpret_cast<const uint32_t*>(sc + (c >> 2) * 512) >> (8 * (c & 3));
+          else sw = *reinterpret_cast<const uint32_t*>(sc + (c >> 1) * 512);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint4 v = *reinterpret_cast<const uint4*>(codes + (((c + u) ^ (r & 7)) << 4));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t m0, m1;
-          if constexpr (FMT == GLQB_MX4_MXFP4) m0 = m1 = mx4_multiplier<FMT, T>((sw >> (8 * u)) & 0xFFu, top);
-          else {
-            m0 = mx4_multiplier<FMT, T>((sw >> (16 * u)) & 0xFFu, 0);
-            m1 = mx4_multiplier<FMT, T>((sw >> (16 * u + 8)) & 0xFFu, 0);
-          }
+          for (int u = 0; u < 2; ++u) {
+            const uint4 q = *reinterpret_cast<const uint4*>(codes + (((c + u) ^ (r & 7)) << 4));
+            const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+            uint32_t m0, m1;
+            if constexpr (FMT == GLQB_MX4_MXFP4) m0 = m1 = mx4_multiplier<FMT, T>((sw >> (8 * u)) & 0xFFu, top);
+            else {
+              m0 = mx4_multiplier<FMT, T>((sw >> (16 * u)) & 0xFFu, 0);
+              m1 = mx4_multiplier<FMT, T>((sw >> (16 * u + 8)) & 0xFFu, 0);
+            }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t r[4];
-            mx4_pairs<T>(w[j], r);
+            for (int j = 0; j < 4; ++j) {
+              uint32_t p[4];
+              mx4_pairs<T>(words[j], p);
 #pragma unroll
-            for (int p = 0; p < 4; ++p) a[u * 16 + j * 4 + p] = mx4_mul2<T>(r[p], j < 2 ? m0 : m1);
+              for (int e = 0; e < 4; ++e) v[u * 16 + j * 4 + e] = mx4_mul2<T>(p[e], j < 2 ? m0 : m1);
+            }
           }
         }
-        if ((k & 1) == 1 || k + 1 == steps) {      // done with this tile of weights
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.empty_w[w.s]);
+        if (k < steps) {
+          if (!mbar_wait(&B.empty_a[a.s], a.phase ^ 1u, &B.abort)) { ok = false; break; }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&B.empty_w[s]);
-          ++wq;
+          tc_fence_after();
+          tmem_st32(to + a.s * 64u, v);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first<PAIR>(&B.full_a[a.s]);
+          a.add(2, R.a_stages);
         }
-        if (!mbar_wait(&B.empty_a[sa], ((q >> 1) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
-        __syncwarp();
-        tc_fence_after();
-        tmem_st32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + G16_A0 + sa * 64u + half * 32u, a);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B.full_a[sa]);
+      }
+      // (the place of the next tile's first step, or second: an odd number of steps puts the groups on the other one's)
+      if (steps & 1) {
+        if (group) a.add(1, R.a_stages);
+        else a.back(R.a_stages);
       }
     }
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER); }
   } else if (warp >= 4) {
     pdl_wait();                                    // (y may still be in use)
-    uint32_t seq = 0;
-    for (int i = first; i < tiles && ok; i += step, ++seq) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-      if (!mbar_wait(&B.acc_full[seq & 1u], (seq >> 1) & 1u, &B.abort)) { ok = false; break; }
+    Pos acc;
+    for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      drain_tile<FMT, T, false>(J, t, i % J.m_tiles, tmem + (seq & 1u) * G16_MAX_TN, warp & 3, lane, B.turn[warp & 3], J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
+      const int mt = row_tile(i);
+      if (!PAIR || mt < J.m_tiles)
+        drain_tile<FMT, T, false>(J, t, mt, tmem + acc.s * R.acc_cols, warp & 3, lane, B.turn[warp & 3], !PAIR && J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B.acc_empty[seq & 1u]);
+      if (lane == 0) arrive_first<PAIR>(&B.acc_empty[acc.s]);
     }
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
   }
   // ---- every thread arrives here, also after a wait gave up
   __syncwarp();
-  if (J.split > 1) {                               // (one tile per cluster)
+  if (!PAIR && J.split > 1) {                      // (one tile per cluster)
     cluster_sync();
-    if (first < tiles) add_parts<FMT, T, false>(J, mx4_tile(J, eff, pre, first / J.m_tiles), first % J.m_tiles, reinterpret_cast<float*>(x_base), rank);
+    if (first < tiles) add_parts<FMT, T, false>(J, mx4_tile(J, eff, pre, first / m_tiles), first % m_tiles, reinterpret_cast<float*>(x_base), rank);
     cluster_sync();
   }
   tc_fence_before();
@@ -348,16 +450,17 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
         mbar_wait(&B.full_x[u % R.x_stages], (u / R.x_stages) & 1u);
       }
     }
-    if (warp == 0 && elect_one()) {
-      umma_commit(&B.drain);
+    if (warp == 0 && (!PAIR || rank == 0) && elect_one()) {
+      commit<PAIR>(&B.drain);
       mbar_wait(&B.drain, 0);
     }
     tc_fence_before();
     __syncthreads();
   }
+  if constexpr (PAIR) cluster_sync();              // (neither CTA's memory goes while the other still works on it)
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    dealloc_all<PAIR>(tmem);
   }
 }
 
@@ -523,9 +626,11 @@ size_t groups_bytes(const Mx4Job& J) { return sizeof(Bars) + (size_t)(J.experts 
 
 cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count, cudaStream_t stream, const char** what) {
   Mx4Ring R;
-  R.box_rows = std::min(J.tn, 32);
-  const int rows = (J.tn + R.box_rows - 1) / R.box_rows * R.box_rows;
-  R.x_half = rows * 128;
+  const int own = J.pair ? (J.tn + 31) / 32 * 16 : J.tn;       // rows of x that a CTA brings
+  R.box_rows = std::min(own, 32);
+  R.x_half = (own + R.box_rows - 1) / R.box_rows * R.box_rows * 128;
+  R.acc_cols = (J.tn + 31) / 32 * 32;
+  R.a_stages = std::min(4, (512 - 2 * R.acc_cols) / 64);
   const size_t fixed = 1024 + G16_W_STAGES * (size_t)mx4_tile_bytes(format) + groups_bytes(J);
   R.x_stages = (int)std::min<size_t>(8, (227 * 1024 - fixed) / (2 * (size_t)R.x_half));
   const size_t smem = std::max(ONE_PER_SM, fixed + (size_t)R.x_stages * 2 * R.x_half);
@@ -537,16 +642,20 @@ cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_c
   const CUresult r = encode(&map, x_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(J.x), dims, strides, box, ones,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { *what = "cuTensorMapEncodeTiled refused the activations"; return cudaErrorInvalidValue; }
-  const long long tiles = (long long)J.max_tiles * J.m_tiles;
-  const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
-  auto run = [&](auto fmt, auto type) {
-    constexpr auto K = mx4_gemm16_kernel<decltype(fmt)::value, decltype(type)>;
-    return mx4_launch<K>(K, grid, G16_THREADS, smem, J.split, stream, J, map, R);
+  const int ranks = J.pair ? 2 : J.split;
+  const long long tiles = (long long)J.max_tiles * (J.pair ? (J.m_tiles + 1) / 2 : J.m_tiles);
+  const int grid = J.split > 1 ? (int)(tiles * ranks) : (int)std::min<long long>(tiles, sm_count / ranks) * ranks;
+  auto run = [&](auto fmt, auto type, auto pair) {
+    constexpr auto K = mx4_gemm16_kernel<decltype(fmt)::value, decltype(type), decltype(pair)::value>;
+    return mx4_launch<K>(K, grid, G16_THREADS, smem, ranks, stream, J, map, R);
   };
   using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
   using N = std::integral_constant<int, GLQB_MX4_NVFP4>;
-  if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(M(), __nv_bfloat16()) : run(M(), __half());
-  return x_bf16 ? run(N(), __nv_bfloat16()) : run(N(), __half());
+  auto of = [&](auto pair) {
+    if (format == GLQB_MX4_MXFP4) return x_bf16 ? run(M(), __nv_bfloat16(), pair) : run(M(), __half(), pair);
+    return x_bf16 ? run(N(), __nv_bfloat16(), pair) : run(N(), __half(), pair);
+  };
+  return J.pair ? of(std::true_type()) : of(std::false_type());
 }
 
 cudaError_t mx4_gemm4_launch(int format, const Mx4Job& J, int sm_count, cudaStream_t stream) {

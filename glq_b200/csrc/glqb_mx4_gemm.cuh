@@ -19,6 +19,7 @@ struct Mx4Job {
   int tn;                     // most rows of x per token tile, a multiple of 16
   int max_tiles;              // bound of the token tiles
   int split;                  // CTAs of a cluster that share a tile's sum
+  int pair;                   // two CTAs share a tile of 256 weight rows (16-bit activations, split 1)
   void* y;
   long long y_stride;
   int y_dtype, accumulate;
