@@ -14,7 +14,17 @@ namespace glqb {
 namespace {
 
 // ---- PTX ------------------------------------------------------------------------------------------
+// `bar`: of this CTA, or (PAIR) its namesake in the pair's first CTA
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  if constexpr (PAIR) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(bar)));
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(at)
+                 : "memory");
+    return;
+  }
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
                "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
                : "memory");
@@ -79,31 +89,17 @@ __device__ __forceinline__ void dealloc_all(uint32_t taddr) {
   if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
   else tmem_dealloc(taddr, 512);
 }
-// arrives at the first CTA's barrier, from either CTA of a pair
+// Arrives at the first CTA's barrier, from either CTA of a pair.  What it hands over is tensor memory, which the tcgen05 fences order; a
+// release of all memory at cluster scope took a thousand clocks.
 template <bool PAIR>
 __device__ __forceinline__ void arrive_first(uint64_t* bar) {
   if constexpr (PAIR) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
   } else {
     mbar_arrive(bar);
   }
-}
-// mbar_wait for what the other CTA of a pair has released
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t it = 0; it < GM_SPIN_LIMIT; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((it & 63u) == 63u && *abort_flag) return false;
-  }
-  return false;
 }
 // both from shared memory, 4-bit, scales of blocks in tensor memory
 template <int FMT>
@@ -222,14 +218,14 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int
 // ---- 16-bit activations ---------------------------------------------------------------------------
 // Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by sixteen warps straight into tensor memory as
 // the A operand (thread = row, 64 values = 32 columns), activations by TMA as 64-value boxes with the 128-byte swizzle.  A step
-// is 128 values, eight MMAs; two groups of eight warps decode the steps in turn.  Warp 0 issues MMAs, warp 1 loads, warp 2 of a
-// pair's second CTA reports its activations, warps 4-7 drain, 8-23 decode.
+// is 128 values, eight MMAs; two groups of eight warps decode the steps in turn.  Warp 0 issues MMAs, warp 1 loads, warps 4-7
+// drain, 8-23 decode.
 //
 // With wide tiles what bounds one CTA is shared memory: of 128 bytes a clock, writing and reading the activations of 192 rows takes
 // 125 (2048 tokens of 14336 x 4096 317 us; without the loads 202).  Two CTAs therefore share a tile of 256 weight rows (PAIR): each
 // brings half of the activations, the first one's thread issues for both.  What is to arrive at the issuing thread comes from
 // both CTAs; what it releases goes to both.
-constexpr int G16_THREADS = 768, G16_W_STAGES = 3, G16_MAX_TN = 192, G16_PRODUCERS = 8;
+constexpr int G16_THREADS = 768, G16_W_STAGES = 3, G16_PRODUCERS = 8;
 
 struct Mx4Ring { int x_stages, box_rows, x_half, a_stages, acc_cols; };  // stages of x, rows per box, bytes of 64 values of a CTA's rows
 
@@ -260,7 +256,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   if (threadIdx.x == 0) {
     for (int s = 0; s < G16_W_STAGES; ++s) { mbar_init(&B.full_w[s], 1); mbar_init(&B.empty_w[s], 2 * G16_PRODUCERS); }
     for (int s = 0; s < R.x_stages; ++s) { mbar_init(&B.full_x[s], 1); mbar_init(&B.empty_x[s], 1); }
-    for (int s = 0; s < R.a_stages; ++s) { mbar_init(&B.full_a[s], PAIR ? 2 * G16_PRODUCERS + 1 : G16_PRODUCERS); mbar_init(&B.empty_a[s], 1); }
+    for (int s = 0; s < R.a_stages; ++s) { mbar_init(&B.full_a[s], PAIR ? 2 * G16_PRODUCERS : G16_PRODUCERS); mbar_init(&B.empty_a[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], PAIR ? 8 : 4); }
     mbar_init(&B.drain, 1);
     B.abort = 0;
@@ -290,11 +286,10 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
         const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
         const uint32_t idesc = idesc16(__is_same(T, __half) ? 0 : 1, PAIR ? 256 : 128, cols_of(t)), d = tmem + acc.s * R.acc_cols;
-        if (!(PAIR ? mbar_wait_cluster(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort) : mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort))) { ok = false; break; }
+        if (!mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort)) { ok = false; break; }
         tc_fence_after();
         for (int k = 0; k < steps; ++k, a.add(1, R.a_stages), x.add(1, R.x_stages)) {
-          if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) ||
-              !(PAIR ? mbar_wait_cluster(&B.full_a[a.s], a.phase, &B.abort) : mbar_wait(&B.full_a[a.s], a.phase, &B.abort))) { ok = false; break; }
+          if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) || !mbar_wait(&B.full_a[a.s], a.phase, &B.abort)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
             const uint32_t at = tmem_a + a.s * 64u, b = x0 + x.s * 2u * R.x_half;
@@ -329,25 +324,14 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
           }
           if (loads_x == 0) pdl_wait();            // (the weights do not depend on what runs in front of this call)
           if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
-          mbar_expect_tx(&B.full_x[x.s], (uint32_t)(2 * boxes * R.box_rows * 128));
+          if (!PAIR || rank == 0) mbar_expect_tx(&B.full_x[x.s], (uint32_t)((PAIR ? 4 : 2) * boxes * R.box_rows * 128));
           uint8_t* dst = x_base + x.s * 2 * R.x_half;
           for (int b = 0; b < boxes; ++b) {
-            tma_load_2d(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, row0 + b * R.box_rows, &B.full_x[x.s]);
-            tma_load_2d(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, row0 + b * R.box_rows, &B.full_x[x.s]);
+            tma_load_2d<PAIR>(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, row0 + b * R.box_rows, &B.full_x[x.s]);
+            tma_load_2d<PAIR>(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, row0 + b * R.box_rows, &B.full_x[x.s]);
           }
         }
       }
-      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
-    }
-  } else if (warp == 2) {
-    if (PAIR && rank == 1 && lane == 0) {
-      Pos a, x;
-      for (int i = first; i < tiles && ok; i += step)
-        for (int k = 0; k < steps; ++k, a.add(1, R.a_stages), x.add(1, R.x_stages)) {
-          // (the stage of A first: its barrier is in the round that this arrival counts for)
-          if (!mbar_wait(&B.empty_a[a.s], a.phase ^ 1u, &B.abort) || !mbar_wait(&B.full_x[x.s], x.phase, &B.abort)) { ok = false; break; }
-          arrive_first<PAIR>(&B.full_a[a.s]);
-        }
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
   } else if (warp >= 8) {
@@ -445,10 +429,11 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
         const uint32_t u = loads_w - 1 - n;
         mbar_wait(&B.full_w[u % G16_W_STAGES], (u / G16_W_STAGES) & 1u);
       }
-      for (uint32_t n = 0; n < min(loads_x, (uint32_t)R.x_stages); ++n) {
-        const uint32_t u = loads_x - 1 - n;
-        mbar_wait(&B.full_x[u % R.x_stages], (u / R.x_stages) & 1u);
-      }
+      if (!PAIR || rank == 0)                      // (a pair's first CTA for both: they end together)
+        for (uint32_t n = 0; n < min(loads_x, (uint32_t)R.x_stages); ++n) {
+          const uint32_t u = loads_x - 1 - n;
+          mbar_wait(&B.full_x[u % R.x_stages], (u / R.x_stages) & 1u);
+        }
     }
     if (warp == 0 && (!PAIR || rank == 0) && elect_one()) {
       commit<PAIR>(&B.drain);
