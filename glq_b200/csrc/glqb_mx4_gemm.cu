@@ -218,14 +218,14 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int
 // ---- 16-bit activations ---------------------------------------------------------------------------
 // Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by sixteen warps straight into tensor memory as
 // the A operand (thread = row, 64 values = 32 columns), activations by TMA as 64-value boxes with the 128-byte swizzle.  A step
-// is 128 values, eight MMAs; two groups of eight warps decode the steps in turn.  Warp 0 issues MMAs, warp 1 loads, warps 4-7
-// drain, 8-23 decode.
+// is 128 values, eight MMAs; two groups of eight warps decode the steps in turn.  Warp 0 issues MMAs, warp 1 loads
+// activations, warp 2 weights, warps 4-7 drain, 8-23 decode.
 //
 // With wide tiles what bounds one CTA is shared memory: of 128 bytes a clock, writing and reading the activations of 192 rows takes
 // 125 (2048 tokens of 14336 x 4096 317 us; without the loads 202).  Two CTAs therefore share a tile of 256 weight rows (PAIR): each
 // brings half of the activations, the first one's thread issues for both.  What is to arrive at the issuing thread comes from
 // both CTAs; what it releases goes to both.
-constexpr int G16_THREADS = 768, G16_W_STAGES = 3, G16_PRODUCERS = 8;
+constexpr int G16_THREADS = 768, G16_W_STAGES = 4, G16_PRODUCERS = 8;
 
 struct Mx4Ring { int x_stages, box_rows, x_half, a_stages, acc_cols; };  // stages of x, rows per box, bytes of 64 values of a CTA's rows
 
@@ -309,20 +309,12 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      Pos w, x;
+      pdl_wait();
+      Pos x;
       for (int i = first; i < tiles && ok; i += step) {
         const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
-        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
         const int rows = PAIR ? cols_of(t) / 2 : t.rows, row0 = t.row0 + (PAIR ? rank * rows : 0), boxes = (rows + R.box_rows - 1) / R.box_rows;
-        for (int k = 0; k < steps && ok; ++k, ++loads_x, x.add(1, R.x_stages)) {
-          if ((k & 1) == 0) {
-            if (!mbar_wait(&B.empty_w[w.s], w.phase ^ 1u, &B.abort)) { ok = false; break; }
-            mbar_expect_tx(&B.full_w[w.s], TILE);
-            bulk_g2s(w_base + w.s * TILE, src + (long long)(k >> 1) * TILE, TILE, &B.full_w[w.s]);
-            ++loads_w;
-            w.add(1, G16_W_STAGES);
-          }
-          if (loads_x == 0) pdl_wait();            // (the weights do not depend on what runs in front of this call)
+        for (int k = 0; k < steps; ++k, ++loads_x, x.add(1, R.x_stages)) {
           if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
           if (!PAIR || rank == 0) mbar_expect_tx(&B.full_x[x.s], (uint32_t)((PAIR ? 4 : 2) * boxes * R.box_rows * 128));
           uint8_t* dst = x_base + x.s * 2 * R.x_half;
@@ -330,6 +322,20 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
             tma_load_2d<PAIR>(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, row0 + b * R.box_rows, &B.full_x[x.s]);
             tma_load_2d<PAIR>(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, row0 + b * R.box_rows, &B.full_x[x.s]);
           }
+        }
+      }
+      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {                               // (the weights do not depend on what runs in front of this call)
+      Pos w;
+      for (int i = first; i < tiles && ok; i += step) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
+        for (int k = k0; k < k1; ++k, ++loads_w, src += TILE, w.add(1, G16_W_STAGES)) {
+          if (!mbar_wait(&B.empty_w[w.s], w.phase ^ 1u, &B.abort)) { ok = false; break; }
+          mbar_expect_tx(&B.full_w[w.s], TILE);
+          bulk_g2s(w_base + w.s * TILE, src, TILE, &B.full_w[w.s]);
         }
       }
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
@@ -424,11 +430,12 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   __syncthreads();
   if (B.abort) {
     // what may still be in flight: the copies armed last, and the MMAs issued so far
-    if (warp == 1 && lane == 0) {
+    if (warp == 2 && lane == 0)
       for (uint32_t n = 0; n < min(loads_w, (uint32_t)G16_W_STAGES); ++n) {
         const uint32_t u = loads_w - 1 - n;
         mbar_wait(&B.full_w[u % G16_W_STAGES], (u / G16_W_STAGES) & 1u);
       }
+    if (warp == 1 && lane == 0) {
       if (!PAIR || rank == 0)                      // (a pair's first CTA for both: they end together)
         for (uint32_t n = 0; n < min(loads_x, (uint32_t)R.x_stages); ++n) {
           const uint32_t u = loads_x - 1 - n;
