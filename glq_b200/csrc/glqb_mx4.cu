@@ -31,8 +31,8 @@ __device__ int g_mx4_status;   // 0, or what gave up (ST_GAVE_UP_*): products ha
 struct Mx4Rows {
   long long rows, stride;     // elements between rows
   long long cols;
-  int chunks;                 // eights of values per row, whole blocks
-  bool vec;
+  long long chunks;           // eights of values per row, whole blocks
+  bool vec;                   // rows start on 16 bytes
 };
 
 // Rows offsets[0] .. offsets[experts] - 1, held to those there are.
@@ -50,111 +50,178 @@ struct Mx4Range {
   }
 };
 
+// Eights of values that a thread takes at once, their loads in front of everything else.  I: the type of an eight's index (64-bit
+// divisions only where there are more than 2^31).
+constexpr int QT_BATCH = 4;
+template <typename I>
+__device__ __forceinline__ void place(const Mx4Rows& q, I i, I& row, I& c) {
+  row = q.rows == 1 ? (I)0 : i / (I)q.chunks;
+  c = i - row * (I)q.chunks;
+}
+
 // ---- largest finite magnitude ---------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(QT_THREADS) mx4_amax_kernel(const T* __restrict__ x, Mx4Rows q, Mx4Range range, float* amax) {
+// A part per CTA; those who need the whole reduce the parts (no atomics, nothing to clear beforehand).
+constexpr int AMAX_PARTS = 256, AMAX_THREADS = 1024;
+static_assert(AMAX_PARTS + 1 == GLQB_MX4_SCALE_FLOATS, "");
+template <typename T, typename I>
+__global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* __restrict__ x, Mx4Rows q, Mx4Range range, float* __restrict__ parts) {
   uint32_t top = 0;
-  const long long chunks = (q.cols + 7) / 8;
   long long first, last;
   range.get(q.rows, first, last);
-  const long long total = last * chunks;
-  for (long long i = first * chunks + (long long)blockIdx.x * QT_THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * QT_THREADS) {
-    const long long row = q.rows == 1 ? 0 : i / chunks, c = i - row * chunks;
-    const long long left = q.cols - c * 8;
-    float v[8];
-    mx4_load8(x + row * q.stride + c * 8, 0, (int)min(left, 8ll), q.vec, v);
+  const I end = (I)(last * q.chunks), step = (I)gridDim.x * AMAX_THREADS;
+  for (I b = (I)(first * q.chunks) + (I)blockIdx.x * AMAX_THREADS + threadIdx.x; b < end; b += step * QT_BATCH) {
+    Mx4Raw<T> raw[QT_BATCH];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-      top = b < 0x7F800000u ? max(top, b) : top;
+    for (int j = 0; j < QT_BATCH; ++j) {
+      const I i = b + j * step;
+      I row, c;
+      place(q, i, row, c);
+      const long long left = i < end ? q.cols - (long long)c * 8 : 0;
+      raw[j].load(x + (long long)row * q.stride + (long long)c * 8, 0, (int)max(0ll, min(left, 8ll)), q.vec);
+    }
+#pragma unroll
+    for (int j = 0; j < QT_BATCH; ++j) {
+      float v[8];
+      raw[j].get(v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t w = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+        top = w < 0x7F800000u ? max(top, w) : top;
+      }
     }
   }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
-  // (non-negative floats order as their bits do; the largest does not depend on the order)
-  if ((threadIdx.x & 31) == 0 && top) atomicMax(reinterpret_cast<unsigned*>(amax), top);
+  __shared__ uint32_t tops[AMAX_THREADS / 32];
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    top = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x < AMAX_THREADS / 32 ? tops[threadIdx.x] : 0u);
+    if (threadIdx.x == 0) parts[blockIdx.x] = __uint_as_float(top);
+  }
+}
+// The tensor's scale for all threads of a block of 256: given, or from the parts; the first block leaves it in own_scale[0].
+__device__ __forceinline__ float whole_scale(const float* given, float* own_scale, int parts) {
+  if (given) return *given;
+  uint32_t top = threadIdx.x < parts ? __float_as_uint(own_scale[1 + threadIdx.x]) : 0u;      // (non-negative: ordered as their bits)
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  __shared__ uint32_t tops[QT_THREADS / 32];
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < QT_THREADS / 32; ++i) top = max(top, tops[i]);
+  const float t = mx4_tensor_scale(__uint_as_float(top));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *own_scale = t;
+  return t;
 }
 
 // ---- quantisation ---------------------------------------------------------------------------------
-template <typename T, int FMT>
+// HBM bound: 2 or 4 bytes in and 0.53 or 0.56 out per value.
+template <typename T, int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
-mx4_quantize_kernel(const T* __restrict__ x, Mx4Rows q, long long total, const float* tensor_scale, const float* amax, float* own_scale,
-                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+mx4_quantize_kernel(const T* __restrict__ x, Mx4Rows q, const float* tensor_scale, float* own_scale, int parts, uint8_t* __restrict__ codes,
+                    uint8_t* __restrict__ scales) {
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
   float t = 1.0f;
-  if constexpr (FMT == GLQB_MX4_NVFP4) {
-    t = tensor_scale ? *tensor_scale : mx4_tensor_scale(*amax);
-    if (!tensor_scale && blockIdx.x == 0 && threadIdx.x == 0) *own_scale = t;
-  }
+  if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(tensor_scale, own_scale, parts);
   const long long code_row = (q.cols + 1) / 2, scale_row = q.chunks / PER;
-  // (whole warps: the threads of a block exchange their largest value)
-  const long long first = (long long)blockIdx.x * QT_THREADS + threadIdx.x, warp_first = first - (threadIdx.x & 31);
-  for (long long w = warp_first, i = first; w < total; w += (long long)gridDim.x * QT_THREADS, i += (long long)gridDim.x * QT_THREADS) {
-    float v[8];
-    const bool live = i < total;
-    const long long row = q.rows == 1 ? 0 : live ? i / q.chunks : 0, c = live ? i - row * q.chunks : 0;
-    const long long left = live ? q.cols - c * 8 : 0;
-    if (left > 0) mx4_load8(x + row * q.stride + c * 8, 0, (int)min(left, 8ll), q.vec, v);
-    else {
+  const I total = (I)(q.rows * q.chunks);
+  Mx4Raw<T> raw[QT_BATCH];
+  I row[QT_BATCH], c[QT_BATCH];
+  int left[QT_BATCH];                                                // values from the eight's first on, at most eight; -8 and less: no eight
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    }
+  for (int j = 0; j < QT_BATCH; ++j) {
+    const I i = (I)blockIdx.x * (QT_THREADS * QT_BATCH) + j * QT_THREADS + threadIdx.x;
+    place(q, i, row[j], c[j]);
+    left[j] = i < total ? (int)max(-7ll, min(8ll, q.cols - (long long)c[j] * 8)) : -8;
+    raw[j].load(x + (long long)row[j] * q.stride + (long long)c[j] * 8, 0, max(0, left[j]), q.vec);
+  }
+#pragma unroll
+  for (int j = 0; j < QT_BATCH; ++j) {
     uint32_t s;
-    const uint32_t word = mx4_quantize8<FMT, false>(v, t, s);
-    if (!live) continue;
-    uint8_t* p = codes + row * code_row + c * 4;
-    if (left >= 8 && (code_row & 3) == 0) *reinterpret_cast<uint32_t*>(p) = word;
-    else {
-      for (int j = 0; j < 4; ++j)
-        if (2 * j < left) p[j] = (uint8_t)(word >> (8 * j));
+    float v[8];
+    raw[j].get(v);
+    const uint32_t word = mx4_quantize8<FMT, false>(v, t, s);     // (all lanes: the threads of a block exchange their largest value)
+    if (left[j] <= -8) continue;
+    uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 4;
+    const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(p);
+    if (left[j] >= 8 && (at & 3u) == 0) *reinterpret_cast<uint32_t*>(p) = word;
+    else if (left[j] >= 8 && (at & 1u) == 0) {
+      reinterpret_cast<uint16_t*>(p)[0] = (uint16_t)word;
+      reinterpret_cast<uint16_t*>(p)[1] = (uint16_t)(word >> 16);
+    } else {
+      for (int b = 0; b < 4; ++b)
+        if (2 * b < left[j]) p[b] = (uint8_t)(word >> (8 * b));
     }
-    if (c % PER == 0) scales[row * scale_row + c / PER] = (uint8_t)s;
+    if (c[j] % PER == 0) scales[(long long)row[j] * scale_row + (long long)(c[j] / PER)] = (uint8_t)s;
   }
 }
 
-template <int FMT>
+template <int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
 mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale,
-                      long long rows_per_scale, Mx4Rows q, long long total, void* __restrict__ out, int out_dtype) {
+                      long long rows_per_scale, Mx4Rows q, void* __restrict__ out, int out_dtype) {
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
   const long long code_row = (q.cols + 1) / 2, scale_row = q.chunks / PER;
-  for (long long i = (long long)blockIdx.x * QT_THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * QT_THREADS) {
-    const long long row = q.rows == 1 ? 0 : i / q.chunks, c = i - row * q.chunks;
-    const long long left = q.cols - c * 8;
-    if (left <= 0) continue;
-    const uint8_t* p = codes + row * code_row + c * 4;
-    uint32_t word = 0;
-    if (left >= 8 && (code_row & 3) == 0) word = *reinterpret_cast<const uint32_t*>(p);
-    else {
-      for (int j = 0; j < 4; ++j)
-        if (2 * j < left) word |= (uint32_t)p[j] << (8 * j);
-    }
-    const float s = mx4_scale_value<FMT>(scales[row * scale_row + c / PER]);
-    float t = 1.0f;
-    if constexpr (FMT == GLQB_MX4_NVFP4) t = tensor_scale[row / rows_per_scale];
-    float v[8];
+  const I total = (I)(q.rows * q.chunks);
+  const bool one_scale = FMT != GLQB_MX4_NVFP4 || rows_per_scale >= q.rows;
+  float t0 = 1.0f;
+  if (FMT == GLQB_MX4_NVFP4 && one_scale) t0 = *tensor_scale;
+  uint32_t word[QT_BATCH], byte[QT_BATCH];
+  I row[QT_BATCH], c[QT_BATCH];
+  int left[QT_BATCH];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mx4_value((word >> (4 * j)) & 15u) * s * t;
-    const long long at = row * q.cols + c * 8;
-    const bool whole = left >= 8 && q.vec;
+  for (int j = 0; j < QT_BATCH; ++j) {
+    const I i = (I)blockIdx.x * (QT_THREADS * QT_BATCH) + j * QT_THREADS + threadIdx.x;
+    place(q, i, row[j], c[j]);
+    left[j] = i < total ? (int)max(0ll, min(8ll, q.cols - (long long)c[j] * 8)) : 0;
+    word[j] = byte[j] = 0;
+    if (left[j] <= 0) continue;
+    const uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 4;
+    const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(p);
+    if (left[j] >= 8 && (at & 3u) == 0) word[j] = *reinterpret_cast<const uint32_t*>(p);
+    else if (left[j] >= 8 && (at & 1u) == 0) word[j] = reinterpret_cast<const uint16_t*>(p)[0] | (uint32_t)reinterpret_cast<const uint16_t*>(p)[1] << 16;
+    else {
+      for (int b = 0; b < 4; ++b)
+        if (2 * b < left[j]) word[j] |= (uint32_t)p[b] << (8 * b);
+    }
+    byte[j] = scales[(long long)row[j] * scale_row + (long long)(c[j] / PER)];
+  }
+#pragma unroll
+  for (int j = 0; j < QT_BATCH; ++j) {
+    if (left[j] <= 0) continue;
+    const float s = mx4_scale_value<FMT>(byte[j]);
+    const float t = one_scale ? t0 : tensor_scale[(long long)row[j] / rows_per_scale];
+    float v[8];
+    mx4_values8(word[j], v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = FMT == GLQB_MX4_NVFP4 ? v[e] * s * t : v[e] * s;
+    const long long at = (long long)row[j] * q.cols + (long long)c[j] * 8;
+    const bool whole = left[j] >= 8 && q.vec;
     if (out_dtype == GLQB_DT_F32) {
       float* o = reinterpret_cast<float*>(out) + at;
       if (whole) {
         reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
         reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
       } else
-        for (int j = 0; j < 8; ++j)
-          if (j < left) o[j] = v[j];
+        for (int e = 0; e < 8; ++e)
+          if (e < left[j]) o[e] = v[e];
     } else {
-      uint16_t h[8];
+      uint32_t h[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        h[j] = out_dtype == GLQB_DT_F16 ? __half_as_ushort(__float2half_rn(v[j])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
+      for (int e = 0; e < 4; ++e) {
+        if (out_dtype == GLQB_DT_F16) {
+          const __half2 r = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+          h[e] = *reinterpret_cast<const uint32_t*>(&r);
+        } else {
+          const __nv_bfloat162 r = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+          h[e] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+      }
       uint16_t* o = reinterpret_cast<uint16_t*>(out) + at;
-      if (whole)
-        *reinterpret_cast<uint4*>(o) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+      if (whole) *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
       else
-        for (int j = 0; j < 8; ++j)
-          if (j < left) o[j] = h[j];
+        for (int e = 0; e < 8; ++e)
+          if (e < left[j]) o[e] = (uint16_t)(h[e >> 1] >> (16 * (e & 1)));
     }
   }
 }
@@ -238,57 +305,45 @@ __global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* __restri
 }
 
 // Rows of x in 4 bits, as the tiles the 4-bit product fetches (per token tile, per 256 values: tn rows of 128 bytes with the
-// 128-byte swizzle, then the scales, 128 rows at a time as in the weight image).  A warp takes a row, 256 values at a time;
-// values past the row are zeros, rows past a tile's are left out (their columns are not stored).
+// 128-byte swizzle, then the scales, 128 rows at a time as in the weight image).  A warp takes `batches` times 1024 values of a row
+// (with many rows all of a row: finding its tile takes as long as a thousand values); values past the row are zeros, rows past a
+// tile's are left out (their columns are not stored).
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, const float* amax, float* own_scale,
-                                                          int x_scales, bool vec) {
+__global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
+                                                                 int x_scales, bool vec, int batches) {
   extern __shared__ int lists[];
   int* eff = lists;
   int* pre = lists + J.experts + 1;
   mx4_groups(J, eff, pre);
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
   float t = 1.0f;
-  if constexpr (FMT == GLQB_MX4_NVFP4) {
-    t = x_scale ? *x_scale : mx4_tensor_scale(*amax);
-    if (!x_scale && blockIdx.x == 0 && threadIdx.x == 0) *own_scale = t;
-  }
-  const int lane = threadIdx.x & 31, end = eff[J.experts];
-  const long long stage = (long long)J.tn * 128 + x_scales;
-  for (int row = eff[0] + blockIdx.x * 8 + (threadIdx.x >> 5); row < end; row += gridDim.x * 8) {
+  if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(x_scale, own_scale, parts);
+  const int lane = threadIdx.x & 31, first = eff[0], end = eff[J.experts], per_row = (J.k_tiles + QT_BATCH * batches - 1) / (QT_BATCH * batches);
+  const long long stage = (long long)J.tn * 128 + x_scales, items = (long long)(end - first) * per_row;
+  for (long long i = (long long)blockIdx.x * (QT_THREADS / 32) + (threadIdx.x >> 5); i < items; i += (long long)gridDim.x * (QT_THREADS / 32)) {
+    const int at_row = per_row == 1 ? (int)i : (int)((unsigned long long)i / (unsigned)per_row), row = first + at_row;
+    int k0 = (int)(i - (long long)at_row * per_row) * QT_BATCH * batches;
+    const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
     const int e = J.experts == 1 ? 0 : mx4_find(eff, J.experts, row), in = row - eff[e];
     const int per = mx4_per_tile(J.tn, eff[e + 1] - eff[e], pre[e + 1] - pre[e]), tile = pre[e] + in / per, r = in % per;
     if (tile >= J.max_tiles) continue;
-    uint8_t* at = J.x_image + (long long)tile * J.k_tiles * stage;
+    uint8_t* at = J.x_image + ((long long)tile * J.k_tiles + k0) * stage;
     uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
     uint8_t* scales = at + J.tn * 128 + (r >> 7) * mx4_scale_bytes(FMT) + mx4_scale_offset(r & 127, lane / PER);
-    const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
-    for (int k = 0; k < J.k_tiles; ++k, codes += stage, scales += stage) {
-      float v[8];
-      mx4_load8(src, k * MX4_K + lane * 8, J.n, vec, v);
-      uint32_t s;
-      *reinterpret_cast<uint32_t*>(codes) = mx4_quantize8<FMT, true>(v, t, s);
-      if (lane % PER == 0) *scales = (uint8_t)s;
-    }
-  }
-}
-
-// Rows of no expert are zeroed.  (Offsets as mx4_groups takes them: the experts' rows are one range.)
-__global__ void __launch_bounds__(256) mx4_clear_kernel(const __grid_constant__ Mx4Job J) {
-  extern __shared__ int lists[];
-  int* eff = lists;
-  mx4_groups(J, eff, lists + J.experts + 1);
-  const int first = eff[0], last = eff[J.experts], size = J.y_dtype == GLQB_DT_F32 ? 4 : 2;
-  for (int row = blockIdx.x; row < J.rows; row += gridDim.x) {
-    if (row >= first && row < last) {
-      // (to the next row of this CTA behind the experts')
-      row += (last - row - 1) / (int)gridDim.x * (int)gridDim.x;
-      continue;
-    }
-    uint8_t* p = reinterpret_cast<uint8_t*>(J.y) + row * J.y_stride * size;
-    for (int i = threadIdx.x; i < J.m; i += 256) {
-      if (size == 4) reinterpret_cast<uint32_t*>(p)[i] = 0u;
-      else reinterpret_cast<uint16_t*>(p)[i] = 0;
+    for (const int k1 = min(J.k_tiles, k0 + QT_BATCH * batches); k0 < k1; k0 += QT_BATCH) {
+      Mx4Raw<T> raw[QT_BATCH];
+#pragma unroll
+      for (int j = 0; j < QT_BATCH; ++j) raw[j].load(src, (k0 + j) * MX4_K + lane * 8, J.n, vec);
+#pragma unroll
+      for (int j = 0; j < QT_BATCH; ++j, codes += stage, scales += stage) {
+        uint32_t s;
+        float v[8];
+        raw[j].get(v);
+        const uint32_t word = mx4_quantize8<FMT, true>(v, t, s);
+        if (k0 + j >= k1) continue;
+        *reinterpret_cast<uint32_t*>(codes) = word;
+        if (lane % PER == 0) *scales = (uint8_t)s;
+      }
     }
   }
 }
@@ -299,43 +354,53 @@ Mx4Rows rows_of(long long rows, int cols, long long stride, int format, const vo
   q.rows = rows;
   q.cols = cols;
   q.stride = stride;
-  q.chunks = (cols + block - 1) / block * (block / 8);
+  q.chunks = ((long long)cols + block - 1) / block * (block / 8);
   q.vec = reinterpret_cast<uintptr_t>(base) % 16 == 0 && (stride * elem % 16 == 0 || rows == 1);
+  if (stride == cols && cols % block == 0) {       // whole blocks, no gaps: one row
+    q.cols = rows * cols;
+    q.chunks = q.cols / 8;
+    q.rows = 1;
+    q.vec = reinterpret_cast<uintptr_t>(base) % 16 == 0;
+  }
   return q;
 }
-// Whole blocks, no gaps: one row (of up to 2^31 eights: what a row's count of them holds).
-bool one_row(long long rows, int cols, long long stride, int format) {
-  return stride == cols && cols % mx4_block(format) == 0 && rows * (cols / 8) < (1ll << 31);
-}
-int grid_for(long long total) { return (int)std::min<long long>((total + QT_THREADS - 1) / QT_THREADS, 148 * 64); }
+bool small(const Mx4Rows& q) { return q.rows * q.chunks < (1ll << 31) - QT_THREADS * QT_BATCH; }
+unsigned grid_for(const Mx4Rows& q) { return (unsigned)((q.rows * q.chunks + QT_THREADS * QT_BATCH - 1) / (QT_THREADS * QT_BATCH)); }
 
-// the largest finite |x| of the range's rows
-int amax_launch(const void* x, int x_dtype, const Mx4Rows& q, const Mx4Range& range, float* amax, cudaStream_t stream) {
-  const cudaError_t e = cudaMemsetAsync(amax, 0, 4, stream);
-  if (e != cudaSuccess) return mx4_fail(GLQB_E_CUDA, "mx4 amax: %s", cudaGetErrorString(e));
-  const long long n = q.rows * ((q.cols + 7) / 8);
-  const int grid = (int)std::min<long long>((n + QT_THREADS - 1) / QT_THREADS, 148 * 8);
-  if (x_dtype == GLQB_DT_F16) mx4_amax_kernel<__half><<<grid, QT_THREADS, 0, stream>>>((const __half*)x, q, range, amax);
-  else if (x_dtype == GLQB_DT_BF16) mx4_amax_kernel<__nv_bfloat16><<<grid, QT_THREADS, 0, stream>>>((const __nv_bfloat16*)x, q, range, amax);
-  else mx4_amax_kernel<float><<<grid, QT_THREADS, 0, stream>>>((const float*)x, q, range, amax);
-  return GLQB_OK;
+// the largest finite |x| of the range's rows, in parts; their number
+int amax_launch(const void* x, int x_dtype, const Mx4Rows& q, const Mx4Range& range, float* parts, cudaStream_t stream) {
+  const int grid = (int)std::min<long long>((q.rows * q.chunks + AMAX_THREADS - 1) / AMAX_THREADS, AMAX_PARTS);
+  auto run = [&](auto type, auto index) {
+    using T = decltype(type);
+    mx4_amax_kernel<T, decltype(index)><<<grid, AMAX_THREADS, 0, stream>>>((const T*)x, q, range, parts);
+  };
+  auto of = [&](auto type) { q.rows * q.chunks < (1ll << 31) - (long long)AMAX_PARTS * AMAX_THREADS * QT_BATCH ? run(type, (uint32_t)0) : run(type, (uint64_t)0); };
+  if (x_dtype == GLQB_DT_F16) of(__half());
+  else if (x_dtype == GLQB_DT_BF16) of(__nv_bfloat16());
+  else of(float());
+  return grid;
 }
 template <int FMT>
 int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const float* tensor_scale, float* own_scale, uint8_t* codes, uint8_t* scales,
                     cudaStream_t stream) {
-  const long long total = q.rows * q.chunks;
-  if (FMT == GLQB_MX4_NVFP4 && !tensor_scale) {
-    const int rc = amax_launch(x, x_dtype, q, Mx4Range{nullptr, 0, 0}, own_scale + 1, stream);
-    if (rc) return rc;
-  }
-  const int grid = grid_for(total);
-  if (x_dtype == GLQB_DT_F16)
-    mx4_quantize_kernel<__half, FMT><<<grid, QT_THREADS, 0, stream>>>((const __half*)x, q, total, tensor_scale, own_scale + 1, own_scale, codes, scales);
-  else if (x_dtype == GLQB_DT_BF16)
-    mx4_quantize_kernel<__nv_bfloat16, FMT><<<grid, QT_THREADS, 0, stream>>>((const __nv_bfloat16*)x, q, total, tensor_scale, own_scale + 1, own_scale, codes, scales);
-  else
-    mx4_quantize_kernel<float, FMT><<<grid, QT_THREADS, 0, stream>>>((const float*)x, q, total, tensor_scale, own_scale + 1, own_scale, codes, scales);
+  int parts = 0;
+  if (FMT == GLQB_MX4_NVFP4 && !tensor_scale) parts = amax_launch(x, x_dtype, q, Mx4Range{nullptr, 0, 0}, own_scale + 1, stream);
+  auto run = [&](auto type, auto index) {
+    using T = decltype(type);
+    mx4_quantize_kernel<T, FMT, decltype(index)><<<grid_for(q), QT_THREADS, 0, stream>>>((const T*)x, q, tensor_scale, own_scale, parts, codes, scales);
+  };
+  auto of = [&](auto type) { small(q) ? run(type, (uint32_t)0) : run(type, (uint64_t)0); };
+  if (x_dtype == GLQB_DT_F16) of(__half());
+  else if (x_dtype == GLQB_DT_BF16) of(__nv_bfloat16());
+  else of(float());
   return mx4_launched("mx4_quantize");
+}
+template <int FMT>
+int dequantize_launch(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, const Mx4Rows& q, void* out,
+                      int out_dtype, cudaStream_t stream) {
+  if (small(q)) mx4_dequantize_kernel<FMT, uint32_t><<<grid_for(q), QT_THREADS, 0, stream>>>(codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
+  else mx4_dequantize_kernel<FMT, uint64_t><<<grid_for(q), QT_THREADS, 0, stream>>>(codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
+  return mx4_launched("mx4_dequantize");
 }
 
 bool dtype_ok(int d) { return d == GLQB_DT_F16 || d == GLQB_DT_BF16 || d == GLQB_DT_F32; }
@@ -358,8 +423,7 @@ int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t 
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!x || !codes || !scales) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: null argument");
   if (x_stride < cols && rows > 1) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: rows of %d values %lld apart", cols, (long long)x_stride);
-  Mx4Rows q = rows_of(rows, cols, x_stride, format, x, size_of(x_dtype));
-  if (one_row(rows, cols, x_stride, format)) { q.cols = rows * cols; q.chunks = (int)(q.cols / 8); q.rows = 1; q.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0; }
+  const Mx4Rows q = rows_of(rows, cols, x_stride, format, x, size_of(x_dtype));
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
     return quantize_launch<GLQB_MX4_MXFP4>(x, x_dtype, q, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
@@ -375,19 +439,15 @@ int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tens
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!codes || !scales || !out) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: null argument");
   Mx4Rows q = rows_of(rows, cols, cols, format, out, size_of(out_dtype));
-  if (one_row(rows, cols, cols, format) && (format == GLQB_MX4_MXFP4 || rows_per_scale >= rows)) {
-    q.cols = rows * cols;
-    q.chunks = (int)(q.cols / 8);
-    q.rows = 1;
-    q.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  if (q.rows == 1 && rows > 1 && format == GLQB_MX4_NVFP4 && rows_per_scale < rows) {     // (rows under scales of their own)
+    q.rows = rows;
+    q.cols = cols;
+    q.chunks = cols / 8;
   }
-  const long long total = q.rows * q.chunks;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
-    mx4_dequantize_kernel<GLQB_MX4_MXFP4><<<grid_for(total), QT_THREADS, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, nullptr, 1, q, total, out, out_dtype);
-  else
-    mx4_dequantize_kernel<GLQB_MX4_NVFP4><<<grid_for(total), QT_THREADS, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, tensor_scale, rows_per_scale, q, total, out, out_dtype);
-  return mx4_launched("mx4_dequantize");
+    return dequantize_launch<GLQB_MX4_MXFP4>((const uint8_t*)codes, (const uint8_t*)scales, nullptr, rows, q, out, out_dtype, stream);
+  return dequantize_launch<GLQB_MX4_NVFP4>((const uint8_t*)codes, (const uint8_t*)scales, tensor_scale, rows_per_scale, q, out, out_dtype, stream);
 }
 
 size_t glqb_mx4_image_bytes(int32_t format, int32_t experts, int32_t m, int32_t n) {
@@ -456,7 +516,7 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
   if (quantize) {
     f.x_scales = mx4_x_scale_bytes(w->format, f.tn);
     f.image = (size_t)f.max_tiles * kt * ((size_t)f.tn * 128 + f.x_scales);
-    f.bytes = f.image + 256;
+    f.bytes = f.image + GLQB_MX4_SCALE_FLOATS * 4;
   } else if (reinterpret_cast<uintptr_t>(x) % 16 || (rows > 1 && x_stride % 8) || (f.mv && w->n % 8)) {
     f.align = true;
     f.n_pad = (w->n + 7) / 8 * 8;
@@ -517,10 +577,10 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.x_stride = x_stride;
   J.status = d->status.load(std::memory_order_relaxed);
   const size_t lists = (size_t)(J.experts + 1) * 8;
-  if (offsets && clear_rest) mx4_clear_kernel<<<(unsigned)std::min<long long>(rows, 148), 256, lists, stream>>>(J);
+  J.clear = offsets && clear_rest;
   if (!quantize) {
     if (f.align) {
-      mx4_align_kernel<<<grid_for(rows * f.n_pad), 256, 0, stream>>>((const uint16_t*)x, x_stride, rows, w->n, f.n_pad, (uint16_t*)workspace);
+      mx4_align_kernel<<<(unsigned)std::min<long long>((rows * f.n_pad + 255) / 256, 148 * 32), 256, 0, stream>>>((const uint16_t*)x, x_stride, rows, w->n, f.n_pad, (uint16_t*)workspace);
       J.x = workspace;
       J.x_stride = f.n_pad;
     }
@@ -538,17 +598,20 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   float* own = (float*)((uint8_t*)workspace + f.image);
   J.x_scale = x_scale ? x_scale : own;
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_stride * size_of(x_dtype) % 16 == 0);
+  int parts = 0;
   if (w->format == GLQB_MX4_NVFP4 && !x_scale) {
-    const Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, x, size_of(x_dtype));
-    const int rc = amax_launch(x, x_dtype, q, Mx4Range{offsets, offsets_are_int64, w->experts}, own + 1, stream);
-    if (rc) return rc;
+    Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, x, size_of(x_dtype));
+    if (offsets && q.rows == 1) { q.rows = rows; q.cols = w->n; q.chunks = w->n / 8; }
+    parts = amax_launch(x, x_dtype, q, Mx4Range{offsets, offsets_are_int64, w->experts}, own + 1, stream);
   }
-  const int grid = (int)std::min<long long>((rows + 7) / 8, 148 * 8);
+  const long long warps = (long long)sms * 64, batches = (J.k_tiles + QT_BATCH - 1) / QT_BATCH;
+  const int at_once = (int)std::max<long long>(1, std::min(batches, rows * batches / warps));
+  const int grid = (int)std::min<long long>((rows * ((batches + at_once - 1) / at_once) + 7) / 8, (long long)sms * 8);
   auto image = [&](auto fmt) {
     constexpr int FMT = decltype(fmt)::value;
-    if (x_dtype == GLQB_DT_F16) mx4_x_image_kernel<__half, FMT><<<grid, 256, lists, stream>>>(J, x_scale, own + 1, own, f.x_scales, vec);
-    else if (x_dtype == GLQB_DT_BF16) mx4_x_image_kernel<__nv_bfloat16, FMT><<<grid, 256, lists, stream>>>(J, x_scale, own + 1, own, f.x_scales, vec);
-    else mx4_x_image_kernel<float, FMT><<<grid, 256, lists, stream>>>(J, x_scale, own + 1, own, f.x_scales, vec);
+    if (x_dtype == GLQB_DT_F16) mx4_x_image_kernel<__half, FMT><<<grid, QT_THREADS, lists, stream>>>(J, x_scale, own, parts, f.x_scales, vec, at_once);
+    else if (x_dtype == GLQB_DT_BF16) mx4_x_image_kernel<__nv_bfloat16, FMT><<<grid, QT_THREADS, lists, stream>>>(J, x_scale, own, parts, f.x_scales, vec, at_once);
+    else mx4_x_image_kernel<float, FMT><<<grid, QT_THREADS, lists, stream>>>(J, x_scale, own, parts, f.x_scales, vec, at_once);
   };
   if (w->format == GLQB_MX4_MXFP4) image(std::integral_constant<int, GLQB_MX4_MXFP4>());
   else image(std::integral_constant<int, GLQB_MX4_NVFP4>());

@@ -15,6 +15,7 @@
 #pragma once
 #include "glqb_internal.h"
 #include <cuda_fp8.h>
+#include <type_traits>
 
 namespace glqb {
 
@@ -64,9 +65,17 @@ __device__ __forceinline__ float mx4_magnitude(uint32_t code) {           // of 
   const uint32_t e = (code >> 1) & 3u, m = code & 1u;
   return e ? __uint_as_float((126u + e) << 23 | m << 22) : 0.5f * (float)m;
 }
-__device__ __forceinline__ float mx4_value(uint32_t code) {               // of a nibble
-  const float v = mx4_magnitude(code);
-  return code & 8u ? -v : v;
+// the eight values of a stored word
+__device__ __forceinline__ void mx4_values8(uint32_t w, float (&v)[8]) {
+  uint32_t r[4];
+  asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; "
+      "cvt.rn.f16x2.e2m1x2 %3, d; }" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 __device__ __forceinline__ float mx4_e4m3(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
@@ -180,31 +189,46 @@ __device__ __forceinline__ uint32_t mx4_quantize8(const float (&v)[8], float t, 
 __device__ __forceinline__ float mx4_tensor_scale(float amax) { return fmaxf(amax * (1.0f / 2688.0f), 0x1p-126f); }
 
 // ---- loads of activations -------------------------------------------------------------------------
-// values col .. col + 7 of a row as fp32, zeros from `cols` on; `vec`: rows start on 16 bytes
+// Values col .. col + 7 of a row as they lie, zeros from `cols` on (`vec`: rows start on 16 bytes), and as fp32.
 template <typename T>
-__device__ __forceinline__ void mx4_load8(const T* row, int col, int cols, bool vec, float (&v)[8]) {
-  if (vec && col + 8 <= cols) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(row + col), b = *reinterpret_cast<const float4*>(row + col + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(row + col);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Mx4Raw {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, int col, int cols, bool vec) {
+    if (vec && col + 8 <= cols) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (__is_same(T, __half)) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(row + col)[i];
+    } else {
+      using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+      const U* p = reinterpret_cast<const U*>(row);
+      uint32_t h[sizeof(T) * 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) * 2; ++i) h[i] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < cols) h[i * sizeof(T) / 4] |= (uint32_t)p[col + i] << (sizeof(T) == 4 ? 0 : 16 * (i & 1));
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint32_t h[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) v[4 * i + j] = __uint_as_float(h[j]);
+        else if constexpr (__is_same(T, __half)) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+          v[2 * j] = f.x;
+          v[2 * j + 1] = f.y;
         } else {
-          v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+          v[2 * j] = __uint_as_float(h[j] << 16);
+          v[2 * j + 1] = __uint_as_float(h[j] & 0xFFFF0000u);
         }
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? (float)row[col + i] : 0.0f;
   }
-}
+};
 #endif  // __CUDACC__
 
 }  // namespace glqb

@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER); }
   } else if (warp >= 4) {
     pdl_wait();                                    // (y may still be in use)
+    mx4_clear_rest(J, eff, threadIdx.x - 128, 128);
     Pos acc;
     for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
       const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
@@ -556,6 +557,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
   } else if (warp >= 4) {
+    mx4_clear_rest(J, eff, threadIdx.x - 128, 128);
     uint32_t seq = 0;
     for (int i = first; i < tiles && ok; i += step, ++seq) {
       const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);

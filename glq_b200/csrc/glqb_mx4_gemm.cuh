@@ -23,6 +23,7 @@ struct Mx4Job {
   void* y;
   long long y_stride;
   int y_dtype, accumulate;
+  int clear;                  // rows of no expert are zeroed
   bool y_wide;                // 16-bit results whose rows lie on 16 bytes, nothing to add
   const void* x;              // 16-bit activations
   long long x_stride;
@@ -130,6 +131,23 @@ __device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) 
   } else {
     float* p = reinterpret_cast<float*>(J.y) + at;
     *p = J.accumulate ? *p + v : v;
+  }
+}
+
+// Rows of no expert (the experts' rows are one range: mx4_groups) are zeroed: by `threads` threads of each CTA.
+__device__ __forceinline__ void mx4_clear_rest(const Mx4Job& J, const int* eff, int thread, int threads) {
+  if (!J.clear) return;
+  const int first = eff[0], last = eff[J.experts], rest = J.rows - (last - first), size = J.y_dtype == GLQB_DT_F32 ? 4 : 2;
+  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+    uint8_t* p = reinterpret_cast<uint8_t*>(J.y) + (long long)(i < first ? i : i + (last - first)) * J.y_stride * size;
+    if (J.y_wide && J.m % 8 == 0) {
+      for (int c = thread; c < J.m / 8; c += threads) reinterpret_cast<uint4*>(p)[c] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int c = thread; c < J.m; c += threads) {
+        if (size == 4) reinterpret_cast<uint32_t*>(p)[c] = 0u;
+        else reinterpret_cast<uint16_t*>(p)[c] = 0;
+      }
+    }
   }
 }
 

@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     pdl_wait();                                          // (a grid ends behind the one in front of it)
   } else {
     pdl_wait();                                          // (y may still be in use)
+    mx4_clear_rest(J, eff, threadIdx.x, MV4_WARPS * 32);
     const int g = lane >> 2, t = lane & 3, r = warp * 16 + g;
     const uint32_t codes0 = (uint32_t)(warp * 2048 + g * 128 + (g << 4) + t * 4);
     const uint32_t scales0 = (uint32_t)(MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4);

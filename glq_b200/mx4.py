@@ -122,7 +122,7 @@ def mx4_quantize(x, format="mxfp4", tensor_scale=None) -> Mx4Tensor:
     given = own = None
     if format == "nvfp4":
         if tensor_scale is None:
-            own = x.new_empty((2,), dtype=torch.float32)
+            own = x.new_empty((_lib.MX4_SCALE_FLOATS,), dtype=torch.float32)
         else:
             given = _scale_ptr(tensor_scale, x, "tensor_scale")
     elif tensor_scale is not None:

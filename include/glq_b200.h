@@ -302,11 +302,12 @@ size_t glqb_noalloc_scratch_bytes(void);
  */
 #define GLQB_MX4_MXFP4 0
 #define GLQB_MX4_NVFP4 1
+#define GLQB_MX4_SCALE_FLOATS 257     /* a tensor's scale, and what it is found with */
 
 /* rows x cols values (x_stride elements apart) to stored rows, each rounded to nearest even from the real quotient by its
  * block's scale: MXFP4 2^(floor(log2 amax) - 2), saturating at 6; NVFP4 e4m3(amax / (6 t)), t = *tensor_scale (positive), or,
- * with tensor_scale NULL, max(largest finite |x| * fp32(1 / 2688), 2^-126), which is left in own_scale[0] (own_scale: two floats,
- * needed then).  A block with an infinity or NaN gets the scale NaN and codes of zero. */
+ * with tensor_scale NULL, max(largest finite |x| * fp32(1 / 2688), 2^-126), which is left in own_scale[0] (own_scale:
+ * GLQB_MX4_SCALE_FLOATS floats, needed then).  A block with an infinity or NaN gets the scale NaN and codes of zero. */
 int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows, int32_t cols, int32_t format,
                       const float* tensor_scale, float* own_scale, void* codes, void* scales, void* stream);
 /* The values stored rows stand for; row r takes tensor_scale[r / rows_per_scale] (NVFP4). */
