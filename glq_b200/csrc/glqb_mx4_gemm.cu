@@ -102,20 +102,27 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
   }
 }
 // both from shared memory, 4-bit, scales of blocks in tensor memory
-template <int FMT>
+template <int FMT, bool PAIR>
 __device__ __forceinline__ void umma4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  if constexpr (FMT == GLQB_MX4_MXFP4)
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0; tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-                 : "memory");
-  else
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0; tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-                 : "memory");
+#define GLQB_UMMA4(GROUP, KIND)                                                                                                              \
+  asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0; tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d), \
+               "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                                                                   \
+               : "memory")
+  if constexpr (FMT == GLQB_MX4_MXFP4) {
+    if constexpr (PAIR) GLQB_UMMA4("2", "mxf4.block_scale.scale_vec::2X");
+    else GLQB_UMMA4("1", "mxf4.block_scale.scale_vec::2X");
+  } else {
+    if constexpr (PAIR) GLQB_UMMA4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    else GLQB_UMMA4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  }
+#undef GLQB_UMMA4
 }
-// 512 bytes of scales (32 rows of 16) to four columns of tensor memory, the same in all four quarters
+// 512 bytes of scales (32 rows of 16) to four columns of tensor memory, the same in all four quarters; of a pair: in each CTA from its
+// own shared memory
+template <bool PAIR>
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 // rows of 16 bytes, eight of them 128 bytes after the eight before, no swizzle
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
@@ -127,8 +134,8 @@ __device__ __forceinline__ uint32_t idesc16(int type, int rows, int cols) {
 }
 // e2m1 operands, K = 64; scales e8m0 or e4m3, `sf`: the first of a word's four bytes that an instruction takes
 template <int FMT>
-__device__ __forceinline__ uint32_t idesc4(int cols, uint32_t sf) {
-  return sf << 4 | 1u << 7 | 1u << 10 | (uint32_t)(cols >> 3) << 17 | (FMT == GLQB_MX4_MXFP4 ? 1u << 23 : 0u) | (uint32_t)(128 >> 7) << 27 | sf << 29;
+__device__ __forceinline__ uint32_t idesc4(int rows, int cols, uint32_t sf) {
+  return sf << 4 | 1u << 7 | 1u << 10 | (uint32_t)(cols >> 3) << 17 | (FMT == GLQB_MX4_MXFP4 ? 1u << 23 : 0u) | (uint32_t)(rows >> 7) << 27 | sf << 29;
 }
 
 // ---- parts of both kernels ------------------------------------------------------------------------
@@ -215,6 +222,18 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int
   }
 }
 
+struct Pos {                   // a place in a ring, and the parity of its round
+  uint32_t s = 0, phase = 0;
+  __device__ __forceinline__ void add(uint32_t d, uint32_t n) {
+    s += d;
+    while (s >= n) { s -= n; phase ^= 1u; }
+  }
+  __device__ __forceinline__ void back(uint32_t n) {
+    if (s == 0) { s = n; phase ^= 1u; }
+    --s;
+  }
+};
+
 // ---- 16-bit activations ---------------------------------------------------------------------------
 // Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by sixteen warps straight into tensor memory as
 // the A operand (thread = row, 64 values = 32 columns), activations by TMA as 64-value boxes with the 128-byte swizzle.  A step
@@ -228,18 +247,6 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int
 constexpr int G16_THREADS = 768, G16_W_STAGES = 4, G16_PRODUCERS = 8;
 
 struct Mx4Ring { int x_stages, box_rows, x_half, a_stages, acc_cols; };  // stages of x, rows per box, bytes of 64 values of a CTA's rows
-
-struct Pos {                   // a place in a ring, and the parity of its round
-  uint32_t s = 0, phase = 0;
-  __device__ __forceinline__ void add(uint32_t d, uint32_t n) {
-    s += d;
-    while (s >= n) { s -= n; phase ^= 1u; }
-  }
-  __device__ __forceinline__ void back(uint32_t n) {
-    if (s == 0) { s = n; phase ^= 1u; }
-    --s;
-  }
-};
 
 template <int FMT, typename T, bool PAIR>
 __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid_constant__ Mx4Job J, const __grid_constant__ CUtensorMap map, Mx4Ring R) {
@@ -458,8 +465,11 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
 }
 
 // ---- 4-bit activations ----------------------------------------------------------------------------
-// Both operands as they lie in their images; a stage is 256 values: four MMAs, whose scales one thread copies to tensor memory
-// in front of them.  Warp 0 issues, warp 1 loads, warps 4-7 drain.
+// Both operands as they lie in their images; a stage is 256 values: four MMAs, whose scales the issuing thread copies to tensor memory
+// in front of them.  Warp 0 issues (in a pair's second CTA it reports the stages that have arrived), warp 1 loads, warps 4-7 drain.
+//
+// What bounds it is shared memory: per stage of 192 columns one CTA writes 43 KiB and the MMAs read 40, where they take 384 clocks at
+// 128 bytes each.  Two CTAs that share a tile of 256 weight rows (PAIR) bring and read half of the activations each.
 constexpr int G4_THREADS = 256;
 template <int FMT> struct G4 {
   static constexpr int ATOMS = mx4_scale_bytes(FMT) / 512;         // 512-byte pieces of scales per 128 rows x 256 values
@@ -468,113 +478,126 @@ template <int FMT> struct G4 {
   static constexpr int STAGES = (512 - 2 * MAX_TN) / SF_COLS;      // MXFP4 5, NVFP4 4: tensor memory, and shared memory
 };
 
-template <int FMT>
+template <int FMT, bool PAIR>
 __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_constant__ Mx4Job J, int stages, int x_scales) {
   using C = G4<FMT>;
+  constexpr int TILE = mx4_tile_bytes(FMT);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int stage_bytes = mx4_tile_bytes(FMT) + J.tn * 128 + x_scales;
+  const int own = PAIR ? J.tn / 2 : J.tn, stage_bytes = TILE + (own + 7) / 8 * 1024 + x_scales;      // (a multiple of 1024: whole groups of eight rows)
   Bars& B = *reinterpret_cast<Bars*>(base + stages * stage_bytes);
   int* eff = reinterpret_cast<int*>(&B + 1);
   int* pre = eff + J.experts + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ranks = PAIR ? 2 : J.split, first = blockIdx.x / ranks, step = gridDim.x / ranks, rank = blockIdx.x % ranks;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) { mbar_init(&B.full_x[s], 1); mbar_init(&B.empty_x[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], 4); }
+    // (full_w of the first CTA of a pair: the second one's stages)
+    for (int s = 0; s < stages; ++s) { mbar_init(&B.full_x[s], 1); mbar_init(&B.empty_x[s], 1); mbar_init(&B.full_w[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&B.acc_full[s], 1); mbar_init(&B.acc_empty[s], PAIR ? 8 : 4); }
     mbar_init(&B.drain, 1);
     B.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 0) {
-    tmem_alloc(&B.tmem, 512);
-    tmem_relinquish();
-  }
+  if (warp == 0) alloc_all<PAIR>(&B.tmem);
   tc_fence_before();
   pdl_wait();
   mx4_groups(J, eff, pre);
+  if constexpr (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = B.tmem;
-  const int tiles = min(pre[J.experts], J.max_tiles) * J.m_tiles;
-  const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
-  const int k0 = rank * J.k_tiles / J.split, steps = (rank + 1) * J.k_tiles / J.split - k0;
+  const int m_tiles = PAIR ? (J.m_tiles + 1) / 2 : J.m_tiles;
+  const int tiles = min(pre[J.experts], J.max_tiles) * m_tiles;
+  const int k0 = PAIR ? 0 : rank * J.k_tiles / J.split, steps = PAIR ? J.k_tiles : (rank + 1) * J.k_tiles / J.split - k0;
+  auto row_tile = [&](int i) { return PAIR ? 2 * (i % m_tiles) + rank : i % m_tiles; };
   uint32_t loads = 0;
   bool ok = true;
 
   if (warp == 0) {
-    uint32_t q = 0, seq = 0;
-    for (int i = first; i < tiles && ok; i += step, ++seq) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-      const int cols = (t.rows + 15) & ~15;
-      const uint32_t d = tmem + (seq & 1u) * C::MAX_TN;
-      if (!mbar_wait(&B.acc_empty[seq & 1u], ((seq >> 1) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
-      tc_fence_after();
-      for (int k = 0; k < steps; ++k, ++q) {
-        const uint32_t s = q % stages;
-        if (!mbar_wait(&B.full_x[s], (q / stages) & 1u, &B.abort)) { ok = false; break; }
+    Pos x, acc;
+    if (!PAIR || rank == 0) {
+      for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+        const int cols = (t.rows + 15) & ~15;
+        const uint32_t d = tmem + acc.s * C::MAX_TN;
+        if (!mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort)) { ok = false; break; }
         tc_fence_after();
-        if (elect_one()) {
-          const uint32_t w = smem_u32(base) + s * stage_bytes, x = w + mx4_tile_bytes(FMT);
-          const uint32_t sa = tmem + 2 * C::MAX_TN + s * C::SF_COLS, sb = sa + 4 * C::ATOMS;
-          const uint64_t dws = scale_desc(w + MX4_CODE_BYTES), dxs = scale_desc(x + J.tn * 128);
-          // (copies and MMAs of one thread run in the order they are issued in)
+        for (int k = 0; k < steps; ++k, x.add(1, stages)) {
+          if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) || (PAIR && !mbar_wait(&B.full_w[x.s], x.phase, &B.abort))) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t w = smem_u32(base) + x.s * stage_bytes, xs = w + TILE, sc = xs + (own + 7) / 8 * 1024;
+            const uint32_t sa = tmem + 2 * C::MAX_TN + x.s * C::SF_COLS, sb = sa + 4 * C::ATOMS;
+            const uint64_t dws = scale_desc(w + MX4_CODE_BYTES), dxs = scale_desc(sc);
+            // (copies and MMAs of one thread run in the order they are issued in)
 #pragma unroll
-          for (int j = 0; j < C::ATOMS; ++j) {
-            tmem_copy_scales(sa + 4u * j, dws + 32u * j);
-            tmem_copy_scales(sb + 8u * j, dxs + 32u * j);
-            if (cols > 128) tmem_copy_scales(sb + 8u * j + 4u, dxs + 32u * (j + C::ATOMS));
-          }
-          const uint64_t da = umma_desc_sw128(w), db = umma_desc_sw128(x);
+            for (int j = 0; j < C::ATOMS; ++j) {
+              tmem_copy_scales<PAIR>(sa + 4u * j, dws + 32u * j);
+              tmem_copy_scales<PAIR>(sb + 8u * j, dxs + 32u * j);
+              if (cols > 128) tmem_copy_scales<PAIR>(sb + 8u * j + 4u, dxs + 32u * (j + C::ATOMS));
+            }
+            const uint64_t da = umma_desc_sw128(w), db = umma_desc_sw128(xs);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t atom = j * C::ATOMS / 4, sf = C::ATOMS == 2 ? 2u * (j & 1) : 0u;
-            umma4<FMT>(d, da + 2u * j, db + 2u * j, idesc4<FMT>(cols, sf), sa + 4u * atom, sb + 8u * atom, (k > 0 || j > 0) ? 1u : 0u);
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t atom = j * C::ATOMS / 4, sf = C::ATOMS == 2 ? 2u * (j & 1) : 0u;
+              umma4<FMT, PAIR>(d, da + 2u * j, db + 2u * j, idesc4<FMT>(PAIR ? 256 : 128, cols, sf), sa + 4u * atom, sb + 8u * atom, (k > 0 || j > 0) ? 1u : 0u);
+            }
+            commit<PAIR>(&B.empty_x[x.s]);
+            if (k + 1 == steps) commit<PAIR>(&B.acc_full[acc.s]);
           }
-          umma_commit(&B.empty_x[s]);
-          if (k + 1 == steps) umma_commit(&B.acc_full[seq & 1u]);
+          __syncwarp();
         }
-        __syncwarp();
       }
+      if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
+    } else if (lane == 0) {
+      for (int i = first; i < tiles && ok; i += step)
+        for (int k = 0; k < steps; ++k, x.add(1, stages)) {
+          if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort)) { ok = false; break; }
+          arrive_first<PAIR>(&B.full_w[x.s]);
+        }
+      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
-    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
   } else if (warp == 1) {
     if (lane == 0) {
       const int x_stage = J.tn * 128 + x_scales;
+      Pos x;
       for (int i = first; i < tiles && ok; i += step) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-        const uint32_t x_codes = (uint32_t)((t.rows + 15) & ~15) * 128u;
-        const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + i % J.m_tiles) * J.k_tiles + k0) * mx4_tile_bytes(FMT);
-        const uint8_t* xsrc = J.x_image + ((long long)(i / J.m_tiles) * J.k_tiles + k0) * x_stage;
-        for (int k = 0; k < steps; ++k, ++loads) {
-          const uint32_t s = loads % stages;
-          if (!mbar_wait(&B.empty_x[s], ((loads / stages) & 1u) ^ 1u, &B.abort)) { ok = false; break; }
-          uint8_t* w = base + s * stage_bytes;
-          mbar_expect_tx(&B.full_x[s], mx4_tile_bytes(FMT) + x_codes + x_scales);
-          bulk_g2s(w, wsrc + (long long)k * mx4_tile_bytes(FMT), mx4_tile_bytes(FMT), &B.full_x[s]);
-          bulk_g2s(w + mx4_tile_bytes(FMT), xsrc + (long long)k * x_stage, x_codes, &B.full_x[s]);
-          bulk_g2s(w + mx4_tile_bytes(FMT) + J.tn * 128, xsrc + (long long)k * x_stage + J.tn * 128, x_scales, &B.full_x[s]);
+        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+        const uint32_t x_codes = (uint32_t)((t.rows + 15) & ~15) * (PAIR ? 64u : 128u);
+        const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
+        const uint8_t* xsrc = J.x_image + ((long long)(i / m_tiles) * J.k_tiles + k0) * x_stage;
+        for (int k = 0; k < steps; ++k, ++loads, x.add(1, stages), wsrc += TILE, xsrc += x_stage) {
+          if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
+          uint8_t* w = base + x.s * stage_bytes;
+          mbar_expect_tx(&B.full_x[x.s], TILE + x_codes + x_scales);
+          bulk_g2s(w, wsrc, TILE, &B.full_x[x.s]);
+          bulk_g2s(w + TILE, xsrc + (PAIR ? rank * x_codes : 0u), x_codes, &B.full_x[x.s]);
+          bulk_g2s(w + TILE + (own + 7) / 8 * 1024, xsrc + J.tn * 128, x_scales, &B.full_x[x.s]);
         }
       }
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
   } else if (warp >= 4) {
     mx4_clear_rest(J, eff, threadIdx.x - 128, 128);
-    uint32_t seq = 0;
-    for (int i = first; i < tiles && ok; i += step, ++seq) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / J.m_tiles);
-      if (!mbar_wait(&B.acc_full[seq & 1u], (seq >> 1) & 1u, &B.abort)) { ok = false; break; }
+    Pos acc;
+    for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
+      const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      drain_tile<FMT, __half, true>(J, t, i % J.m_tiles, tmem + (seq & 1u) * C::MAX_TN, warp & 3, lane, B.turn[warp & 3], J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
+      const int mt = row_tile(i);
+      if (!PAIR || mt < J.m_tiles)
+        drain_tile<FMT, __half, true>(J, t, mt, tmem + acc.s * C::MAX_TN, warp & 3, lane, B.turn[warp & 3], !PAIR && J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B.acc_empty[seq & 1u]);
+      if (lane == 0) arrive_first<PAIR>(&B.acc_empty[acc.s]);
     }
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
   }
+  // ---- every thread arrives here, also after a wait gave up
   __syncwarp();
-  if (J.split > 1) {
+  if (!PAIR && J.split > 1) {
     cluster_sync();
-    if (first < tiles) add_parts<FMT, __half, true>(J, mx4_tile(J, eff, pre, first / J.m_tiles), first % J.m_tiles, reinterpret_cast<float*>(base), rank);
+    if (first < tiles) add_parts<FMT, __half, true>(J, mx4_tile(J, eff, pre, first / m_tiles), first % m_tiles, reinterpret_cast<float*>(base), rank);
     cluster_sync();
   }
   tc_fence_before();
@@ -585,16 +608,17 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
         const uint32_t u = loads - 1 - n;
         mbar_wait(&B.full_x[u % stages], (u / stages) & 1u);
       }
-    if (warp == 0 && elect_one()) {
-      umma_commit(&B.drain);
+    if (warp == 0 && (!PAIR || rank == 0) && elect_one()) {
+      commit<PAIR>(&B.drain);
       mbar_wait(&B.drain, 0);
     }
     tc_fence_before();
     __syncthreads();
   }
+  if constexpr (PAIR) cluster_sync();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    dealloc_all<PAIR>(tmem);
   }
 }
 
@@ -654,16 +678,18 @@ cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_c
 
 cudaError_t mx4_gemm4_launch(int format, const Mx4Job& J, int sm_count, cudaStream_t stream) {
   const int x_scales = mx4_x_scale_bytes(format, J.tn), most = format == GLQB_MX4_MXFP4 ? G4<GLQB_MX4_MXFP4>::STAGES : G4<GLQB_MX4_NVFP4>::STAGES;
-  const size_t fixed = 1024 + groups_bytes(J), stage = (size_t)mx4_tile_bytes(format) + J.tn * 128 + x_scales;
+  const int ranks = J.pair ? 2 : J.split, own = J.pair ? J.tn / 2 : J.tn;
+  const size_t fixed = 1024 + groups_bytes(J), stage = (size_t)mx4_tile_bytes(format) + (own + 7) / 8 * 1024 + x_scales;
   const int stages = (int)std::min<size_t>(most, (227 * 1024 - fixed) / stage);
-  const long long tiles = (long long)J.max_tiles * J.m_tiles;
-  const int grid = J.split > 1 ? (int)(tiles * J.split) : (int)std::min<long long>(tiles, sm_count);
+  const long long tiles = (long long)J.max_tiles * (J.pair ? (J.m_tiles + 1) / 2 : J.m_tiles);
+  const int grid = J.split > 1 ? (int)(tiles * ranks) : (int)std::min<long long>(tiles, sm_count / ranks) * ranks;
   const size_t smem = std::max(ONE_PER_SM, fixed + stages * stage);
-  auto run = [&](auto fmt) {
-    constexpr auto K = mx4_gemm4_kernel<decltype(fmt)::value>;
-    return mx4_launch<K>(K, grid, G4_THREADS, smem, J.split, stream, J, stages, x_scales);
+  auto run = [&](auto fmt, auto pair) {
+    constexpr auto K = mx4_gemm4_kernel<decltype(fmt)::value, decltype(pair)::value>;
+    return mx4_launch<K>(K, grid, G4_THREADS, smem, ranks, stream, J, stages, x_scales);
   };
-  return format == GLQB_MX4_MXFP4 ? run(std::integral_constant<int, GLQB_MX4_MXFP4>()) : run(std::integral_constant<int, GLQB_MX4_NVFP4>());
+  auto of = [&](auto fmt) { return J.pair ? run(fmt, std::true_type()) : run(fmt, std::false_type()); };
+  return format == GLQB_MX4_MXFP4 ? of(std::integral_constant<int, GLQB_MX4_MXFP4>()) : of(std::integral_constant<int, GLQB_MX4_NVFP4>());
 }
 
 }  // namespace glqb
