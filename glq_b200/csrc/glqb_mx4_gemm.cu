@@ -52,6 +52,17 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
                : "r"(taddr)
                : "memory");
 }
+// 16 lanes x 32 columns as fragments of 16 x 8 values: r[4g + 0, 1] columns 8g + 2t, + 1 of row l / 4 (t = l % 4), r[4g + 2, 3] of row l / 4 + 8
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void stmatrix_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 // A from tensor memory, B from shared memory; of a pair of CTAs: 128 rows from each one's tensor memory, half of the columns from each
 // one's shared memory
 template <bool PAIR>
@@ -140,7 +151,7 @@ __device__ __forceinline__ uint32_t idesc4(int rows, int cols, uint32_t sf) {
 
 // ---- parts of both kernels ------------------------------------------------------------------------
 struct __align__(16) Bars {     // in shared memory
-  uint8_t turn[4][2048];       // results on their way out, per draining warp
+  uint8_t turn[4][32 * 80];    // results on their way out, per draining warp
   uint64_t full_w[8], empty_w[8], full_x[8], empty_x[8], full_a[4], empty_a[4], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   volatile int abort;
@@ -152,10 +163,57 @@ __device__ __forceinline__ Mx4Factor row_factor(const Mx4Job& J, int expert, int
   else if constexpr (FMT == GLQB_MX4_NVFP4) return Mx4Factor{J.w_scale[expert], *J.x_scale};
   else return Mx4Factor{1.0f, 1.0f};
 }
-// Columns of a finished accumulator to y, or (a cluster's CTA) to shared memory as [column][row].  A thread has a row of
-// weights, so its values lie y_stride apart: 32 rows x 32 columns are turned in the warp's 2 KiB of shared memory and stored 16
-// bytes per lane.  (A 2-byte store per value took 4000 clocks per 32 columns, 24,000 per tile of 192, which is a mainloop of
-// 4096 values; most of it instruction fetches of the unrolled stores.)  Other results go eight columns at a time.
+// Columns of a finished accumulator to y, or (a cluster's CTA) to shared memory as [column][row].  Rows of y lie across the
+// accumulator's columns: 32 rows x 32 columns come as fragments, are turned by stmatrix in the warp's shared memory (columns TURN bytes
+// apart, so that eight of them are in different banks) and are stored 16 bytes per lane, the next 16 rows on their way.  (A
+// 2-byte store per value took 4000 clocks per 32 columns, 24,000 per tile of 192, which is a mainloop of 4096 values; turned by 2-byte
+// stores 1050.)  Other results go eight columns at a time.
+constexpr int TURN = 80;
+template <int FMT, bool QUANT, bool BF16>
+__device__ __forceinline__ void drain_wide(const Mx4Job& J, const Mx4Tile& t, int row, uint32_t acc, int lane, uint8_t* stage, const Mx4Factor& own) {
+  // factors of rows lane / 4 + 8 i
+  float fa[4], fb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    fa[i] = __shfl_sync(0xFFFFFFFFu, own.a, (lane >> 2) + 8 * i);
+    fb[i] = __shfl_sync(0xFFFFFFFFu, own.b, (lane >> 2) + 8 * i);
+  }
+  const uint32_t put = smem_u32(stage) + (uint32_t)(((lane >> 4) * 8 + (lane & 7)) * TURN + ((lane >> 3) & 1) * 16);
+  const uint8_t* get = stage + (lane >> 2) * TURN + (lane & 3) * 16;
+  uint16_t* y = reinterpret_cast<uint16_t*>(J.y) + (long long)(t.row0 + (lane >> 2)) * J.y_stride + row + (lane & 3) * 8;
+  auto pack = [&](uint32_t a, uint32_t b, int i) -> uint32_t {
+    const float u = __uint_as_float(a) * fa[i] * fb[i], v = __uint_as_float(b) * fa[i] * fb[i];
+    if constexpr (BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(u, v);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(u, v);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    }
+  };
+  auto turn = [&](const uint32_t (&v)[16], int h) {      // rows 16 h .. 16 h + 15
+#pragma unroll
+    for (int g = 0; g < 4; g += 2)
+      stmatrix_trans(put + (uint32_t)(g * 8 * TURN + h * 32), pack(v[4 * g], v[4 * g + 1], 2 * h), pack(v[4 * g + 2], v[4 * g + 3], 2 * h + 1),
+                     pack(v[4 * g + 4], v[4 * g + 5], 2 * h), pack(v[4 * g + 6], v[4 * g + 7], 2 * h + 1));
+  };
+  uint32_t upper[16], lower[16];
+  tmem_ld_frag(acc, upper);
+#pragma unroll 1
+  for (int c0 = 0; c0 < t.rows; c0 += 32) {
+    tmem_ld_wait();
+    tmem_ld_frag(acc + (16u << 16) + (uint32_t)c0, lower);
+    __syncwarp();
+    turn(upper, 0);
+    tmem_ld_wait();
+    if (c0 + 32 < t.rows) tmem_ld_frag(acc + (uint32_t)c0 + 32u, upper);
+    turn(lower, 1);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c0 + i * 8 + (lane >> 2) < t.rows) *reinterpret_cast<uint4*>(y + (long long)(c0 + i * 8) * J.y_stride) = *reinterpret_cast<const uint4*>(get + i * 8 * TURN);
+  }
+}
 template <int FMT, typename T, bool QUANT>
 __device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, int mt, uint32_t acc, int quarter, int lane, uint8_t* stage, float* red) {
   const int r = quarter * 32 + lane, row = mt * MX4_ROWS + r;
@@ -173,28 +231,9 @@ __device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, in
   }
   const Mx4Factor f = row < J.m ? row_factor<FMT, T, QUANT>(J, t.expert, row) : Mx4Factor{1.0f, 1.0f};
   if (J.y_wide && mt * MX4_ROWS + quarter * 32 + 32 <= J.m) {
-    uint16_t* put = reinterpret_cast<uint16_t*>(stage) + lane;
-    const uint8_t* get = stage + lane * 16;
-    uint16_t* y = reinterpret_cast<uint16_t*>(J.y) + (long long)(t.row0 + (lane >> 2)) * J.y_stride + mt * MX4_ROWS + quarter * 32 + (lane & 3) * 8;
-    const bool bf16 = J.y_dtype == GLQB_DT_BF16;
-#pragma unroll 1
-    for (int c0 = 0; c0 < t.rows; c0 += 32) {
-      uint32_t v[32];
-      tmem_ld32(acc + (uint32_t)c0, v);
-      tmem_ld_wait();
-      __syncwarp();
-      if (bf16) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) put[i * 32] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(v[i]) * f.a * f.b));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) put[i * 32] = __half_as_ushort(__float2half_rn(__uint_as_float(v[i]) * f.a * f.b));
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c0 + i * 8 + (lane >> 2) < t.rows) *reinterpret_cast<uint4*>(y + (long long)(c0 + i * 8) * J.y_stride) = *reinterpret_cast<const uint4*>(get + i * 512);
-    }
+    const int row0 = mt * MX4_ROWS + quarter * 32;
+    if (J.y_dtype == GLQB_DT_BF16) drain_wide<FMT, QUANT, true>(J, t, row0, acc, lane, stage, f);
+    else drain_wide<FMT, QUANT, false>(J, t, row0, acc, lane, stage, f);
     return;
   }
 #pragma unroll 1
