@@ -312,20 +312,19 @@ template <typename T, int FMT>
 __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
                                                                  int x_scales, bool vec, int batches) {
   extern __shared__ int lists[];
-  int* eff = lists;
-  int* pre = lists + J.experts + 1;
-  mx4_groups(J, eff, pre);
+  const Mx4Lists L(lists, J.experts);
+  mx4_groups(J, L);
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
   float t = 1.0f;
   if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(x_scale, own_scale, parts);
-  const int lane = threadIdx.x & 31, first = eff[0], end = eff[J.experts], per_row = (J.k_tiles + QT_BATCH * batches - 1) / (QT_BATCH * batches);
+  const int lane = threadIdx.x & 31, first = L.eff[0], end = L.eff[J.experts], per_row = (J.k_tiles + QT_BATCH * batches - 1) / (QT_BATCH * batches);
   const long long stage = (long long)J.tn * 128 + x_scales, items = (long long)(end - first) * per_row;
   for (long long i = (long long)blockIdx.x * (QT_THREADS / 32) + (threadIdx.x >> 5); i < items; i += (long long)gridDim.x * (QT_THREADS / 32)) {
     const int at_row = per_row == 1 ? (int)i : (int)((unsigned long long)i / (unsigned)per_row), row = first + at_row;
     int k0 = (int)(i - (long long)at_row * per_row) * QT_BATCH * batches;
     const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
-    const int e = J.experts == 1 ? 0 : mx4_find(eff, J.experts, row), in = row - eff[e];
-    const int per = mx4_per_tile(J.tn, eff[e + 1] - eff[e], pre[e + 1] - pre[e]), tile = pre[e] + in / per, r = in % per;
+    const int e = J.experts == 1 ? 0 : mx4_find(L.eff, J.experts, row), in = row - L.eff[e];
+    const int per = L.per[e], tile = L.pre[e] + in / per, r = in % per;
     if (tile >= J.max_tiles) continue;
     uint8_t* at = J.x_image + ((long long)tile * J.k_tiles + k0) * stage;
     uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
@@ -579,7 +578,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.x = x;
   J.x_stride = x_stride;
   J.status = d->status.load(std::memory_order_relaxed);
-  const size_t lists = (size_t)(J.experts + 1) * 8;
+  const size_t lists = (size_t)(J.experts + 1) * 12;
   J.clear = offsets && clear_rest;
   if (!quantize) {
     if (f.align) {

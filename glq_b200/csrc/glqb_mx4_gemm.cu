@@ -170,7 +170,7 @@ __device__ __forceinline__ Mx4Factor row_factor(const Mx4Job& J, int expert, int
 // stores 1050.)  Other results go eight columns at a time.
 constexpr int TURN = 80;
 template <int FMT, bool QUANT, bool BF16>
-__device__ __forceinline__ void drain_wide(const Mx4Job& J, const Mx4Tile& t, int row, uint32_t acc, int lane, uint8_t* stage, const Mx4Factor& own) {
+__device__ __forceinline__ void drain_wide(const Mx4Job& J, const Mx4Walk& t, int row, uint32_t acc, int lane, uint8_t* stage, const Mx4Factor& own) {
   // factors of rows lane / 4 + 8 i
   float fa[4], fb[4];
 #pragma unroll
@@ -215,7 +215,7 @@ __device__ __forceinline__ void drain_wide(const Mx4Job& J, const Mx4Tile& t, in
   }
 }
 template <int FMT, typename T, bool QUANT>
-__device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, int mt, uint32_t acc, int quarter, int lane, uint8_t* stage, float* red) {
+__device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Walk& t, int mt, const Mx4Factor& f, uint32_t acc, int quarter, int lane, uint8_t* stage, float* red) {
   const int r = quarter * 32 + lane, row = mt * MX4_ROWS + r;
   acc += (uint32_t)(quarter * 32) << 16;
   if (red) {
@@ -229,7 +229,6 @@ __device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, in
     }
     return;
   }
-  const Mx4Factor f = row < J.m ? row_factor<FMT, T, QUANT>(J, t.expert, row) : Mx4Factor{1.0f, 1.0f};
   if (J.y_wide && mt * MX4_ROWS + quarter * 32 + 32 <= J.m) {
     const int row0 = mt * MX4_ROWS + quarter * 32;
     if (J.y_dtype == GLQB_DT_BF16) drain_wide<FMT, QUANT, true>(J, t, row0, acc, lane, stage, f);
@@ -250,14 +249,20 @@ __device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Tile& t, in
 }
 // The cluster's parts of a tile, added in rank order; the columns are shared out over the CTAs.
 template <int FMT, typename T, bool QUANT>
-__device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Tile& t, int mt, float* red, int rank) {
-  const int r = threadIdx.x % MX4_ROWS, row = mt * MX4_ROWS + r;
+__device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Walk& t, float* red, int rank) {
+  const int r = threadIdx.x % MX4_ROWS, row = t.mt * MX4_ROWS + r;
   if (row >= J.m) return;
   const Mx4Factor f = row_factor<FMT, T, QUANT>(J, t.expert, row);
   const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
-  for (int c = rank + J.split * (int)(threadIdx.x / MX4_ROWS); c < t.rows; c += J.split * (int)(blockDim.x / MX4_ROWS)) {
-    const float v = sum_cluster(base + (uint32_t)(c * MX4_ROWS * 4), J.split);
-    mx4_put(J, (long long)(t.row0 + c) * J.y_stride + row, v * f.a * f.b);
+  const int groups = blockDim.x / MX4_ROWS, own = J.split * groups;
+#pragma unroll 1
+  for (int c = rank + J.split * (int)(threadIdx.x / MX4_ROWS); c < t.rows; c += 4 * own) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i * own < t.rows ? sum_cluster(base + (uint32_t)((c + i * own) * MX4_ROWS * 4), J.split) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i * own < t.rows) mx4_put(J, (long long)(t.row0 + c + i * own) * J.y_stride + row, v[i] * f.a * f.b);
   }
 }
 
@@ -294,8 +299,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   uint8_t* w_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* x_base = w_base + G16_W_STAGES * TILE;
   Bars& B = *reinterpret_cast<Bars*>(x_base + R.x_stages * 2 * R.x_half);
-  int* eff = reinterpret_cast<int*>(&B + 1);
-  int* pre = eff + J.experts + 1;
+  const Mx4Lists L(reinterpret_cast<int*>(&B + 1), J.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a CTA's place among those that work on one tile: of a pair (weight rows), or of a split (values)
   const int ranks = PAIR ? 2 : J.split, first = blockIdx.x / ranks, step = gridDim.x / ranks, rank = blockIdx.x % ranks;
@@ -311,17 +315,17 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   if (warp == 0) alloc_all<PAIR>(&B.tmem);
   tc_fence_before();
   if (J.offsets) pdl_wait();
-  mx4_groups(J, eff, pre);                         // (ends with a block barrier)
+  mx4_groups(J, L);                         // (ends with a block barrier)
   if constexpr (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = B.tmem, tmem_a = tmem + 2 * R.acc_cols;
   const int m_tiles = PAIR ? (J.m_tiles + 1) / 2 : J.m_tiles;
-  const int tiles = min(pre[J.experts], J.max_tiles) * m_tiles;
+  const int tiles = min(L.pre[J.experts], J.max_tiles) * m_tiles;
   const int k0 = PAIR ? 0 : rank * J.k_tiles / J.split, k1 = PAIR ? J.k_tiles : (rank + 1) * J.k_tiles / J.split;     // tiles of 256 values
   const int steps = min(2 * k1, (J.n + 127) / 128) - 2 * k0;                                                          // of 128
   // this CTA's row tile (the second CTA of a pair may have none: it computes the one before again and stores nothing)
-  auto row_tile = [&](int i) { return PAIR ? 2 * (i % m_tiles) + rank : i % m_tiles; };
-  auto cols_of = [&](const Mx4Tile& t) { return PAIR ? (t.rows + 31) & ~31 : (t.rows + 15) & ~15; };
+  auto row_tile = [&](const Mx4Walk& t) { return PAIR ? 2 * t.mt + rank : t.mt; };
+  auto cols_of = [&](const Mx4Walk& t) { return PAIR ? (t.rows + 31) & ~31 : (t.rows + 15) & ~15; };
   uint32_t loads_w = 0, loads_x = 0;
   bool ok = true;
 
@@ -329,8 +333,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     if (!PAIR || rank == 0) {
       Pos a, x, acc;
       const uint32_t x0 = smem_u32(x_base);
-      for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+      for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
         const uint32_t idesc = idesc16(__is_same(T, __half) ? 0 : 1, PAIR ? 256 : 128, cols_of(t)), d = tmem + acc.s * R.acc_cols;
         if (!mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort)) { ok = false; break; }
         tc_fence_after();
@@ -354,30 +357,27 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      pdl_wait();
-      Pos x;
-      for (int i = first; i < tiles && ok; i += step) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
-        const int rows = PAIR ? cols_of(t) / 2 : t.rows, row0 = t.row0 + (PAIR ? rank * rows : 0), boxes = (rows + R.box_rows - 1) / R.box_rows;
-        for (int k = 0; k < steps; ++k, ++loads_x, x.add(1, R.x_stages)) {
-          if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
-          if (!PAIR || rank == 0) mbar_expect_tx(&B.full_x[x.s], (uint32_t)((PAIR ? 4 : 2) * boxes * R.box_rows * 128));
-          uint8_t* dst = x_base + x.s * 2 * R.x_half;
-          for (int b = 0; b < boxes; ++b) {
-            tma_load_2d<PAIR>(dst + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128, row0 + b * R.box_rows, &B.full_x[x.s]);
-            tma_load_2d<PAIR>(dst + R.x_half + b * R.box_rows * 128, &map, k0 * MX4_K + k * 128 + 64, row0 + b * R.box_rows, &B.full_x[x.s]);
-          }
-        }
+    // (a box per lane: one thread that issues them in turn is late among the warps that decode)
+    pdl_wait();
+    Pos x;
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
+      const int rows = PAIR ? cols_of(t) / 2 : t.rows, row0 = t.row0 + (PAIR ? rank * rows : 0), boxes = (rows + R.box_rows - 1) / R.box_rows;
+      const int box = lane >> 1, half = lane & 1, to = half * R.x_half + box * R.box_rows * 128;
+      for (int k = 0; k < steps; ++k, ++loads_x, x.add(1, R.x_stages)) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort));
+        if (!ok) break;
+        if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(&B.full_x[x.s], (uint32_t)((PAIR ? 4 : 2) * boxes * R.box_rows * 128));
+        __syncwarp();
+        if (box < boxes)
+          tma_load_2d<PAIR>(x_base + x.s * 2 * R.x_half + to, &map, k0 * MX4_K + k * 128 + half * 64, row0 + box * R.box_rows, &B.full_x[x.s]);
       }
-      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
+    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
   } else if (warp == 2) {
     if (lane == 0) {                               // (the weights do not depend on what runs in front of this call)
       Pos w;
-      for (int i = first; i < tiles && ok; i += step) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
-        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
+      for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
+        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
         for (int k = k0; k < k1; ++k, ++loads_w, src += TILE, w.add(1, G16_W_STAGES)) {
           if (!mbar_wait(&B.empty_w[w.s], w.phase ^ 1u, &B.abort)) { ok = false; break; }
           mbar_expect_tx(&B.full_w[w.s], TILE);
@@ -392,11 +392,10 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     const uint32_t to = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + half * 32u;
     Pos a, w;
     a.add(group, R.a_stages);
-    for (int i = first; i < tiles && ok; i += step) {
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
       int top = 0;
       if constexpr (FMT == GLQB_MX4_MXFP4) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
-        top = J.tops[((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * MX4_ROWS + r] & 0xFF;
+        top = J.tops[((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * MX4_ROWS + r] & 0xFF;
       }
       for (int k = group; k < steps + group; k += 2, w.add(1, G16_W_STAGES)) {
         if (!mbar_wait(&B.full_w[w.s], w.phase, &B.abort)) { ok = false; break; }
@@ -450,16 +449,17 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER); }
   } else if (warp >= 4) {
     pdl_wait();                                    // (y may still be in use)
-    mx4_clear_rest(J, eff, threadIdx.x - 128, 128);
+    mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
     Pos acc;
-    for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
+      const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
+      Mx4Factor f{1.0f, 1.0f};
+      if (row < J.m) f = row_factor<FMT, T, false>(J, t.expert, row);
       if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      const int mt = row_tile(i);
       if (!PAIR || mt < J.m_tiles)
-        drain_tile<FMT, T, false>(J, t, mt, tmem + acc.s * R.acc_cols, warp & 3, lane, B.turn[warp & 3], !PAIR && J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
+        drain_tile<FMT, T, false>(J, t, mt, f, tmem + acc.s * R.acc_cols, warp & 3, lane, B.turn[warp & 3], !PAIR && J.split > 1 ? reinterpret_cast<float*>(x_base) : nullptr);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_first<PAIR>(&B.acc_empty[acc.s]);
@@ -470,7 +470,8 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   __syncwarp();
   if (!PAIR && J.split > 1) {                      // (one tile per cluster)
     cluster_sync();
-    if (first < tiles) add_parts<FMT, T, false>(J, mx4_tile(J, eff, pre, first / m_tiles), first % m_tiles, reinterpret_cast<float*>(x_base), rank);
+    const Mx4Walk t(L, J.experts, first, step, tiles, m_tiles);
+    if (t.more()) add_parts<FMT, T, false>(J, t, reinterpret_cast<float*>(x_base), rank);
     cluster_sync();
   }
   tc_fence_before();
@@ -525,8 +526,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int own = PAIR ? J.tn / 2 : J.tn, stage_bytes = TILE + (own + 7) / 8 * 1024 + x_scales;      // (a multiple of 1024: whole groups of eight rows)
   Bars& B = *reinterpret_cast<Bars*>(base + stages * stage_bytes);
-  int* eff = reinterpret_cast<int*>(&B + 1);
-  int* pre = eff + J.experts + 1;
+  const Mx4Lists L(reinterpret_cast<int*>(&B + 1), J.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ranks = PAIR ? 2 : J.split, first = blockIdx.x / ranks, step = gridDim.x / ranks, rank = blockIdx.x % ranks;
   if (threadIdx.x == 0) {
@@ -540,22 +540,21 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   if (warp == 0) alloc_all<PAIR>(&B.tmem);
   tc_fence_before();
   pdl_wait();
-  mx4_groups(J, eff, pre);
+  mx4_groups(J, L);
   if constexpr (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = B.tmem;
   const int m_tiles = PAIR ? (J.m_tiles + 1) / 2 : J.m_tiles;
-  const int tiles = min(pre[J.experts], J.max_tiles) * m_tiles;
+  const int tiles = min(L.pre[J.experts], J.max_tiles) * m_tiles;
   const int k0 = PAIR ? 0 : rank * J.k_tiles / J.split, steps = PAIR ? J.k_tiles : (rank + 1) * J.k_tiles / J.split - k0;
-  auto row_tile = [&](int i) { return PAIR ? 2 * (i % m_tiles) + rank : i % m_tiles; };
+  auto row_tile = [&](const Mx4Walk& t) { return PAIR ? 2 * t.mt + rank : t.mt; };
   uint32_t loads = 0;
   bool ok = true;
 
   if (warp == 0) {
     Pos x, acc;
     if (!PAIR || rank == 0) {
-      for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+      for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
         const int cols = (t.rows + 15) & ~15;
         const uint32_t d = tmem + acc.s * C::MAX_TN;
         if (!mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort)) { ok = false; break; }
@@ -599,11 +598,10 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
     if (lane == 0) {
       const int x_stage = J.tn * 128 + x_scales;
       Pos x;
-      for (int i = first; i < tiles && ok; i += step) {
-        const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+      for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
         const uint32_t x_codes = (uint32_t)((t.rows + 15) & ~15) * (PAIR ? 64u : 128u);
-        const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(i), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
-        const uint8_t* xsrc = J.x_image + ((long long)(i / m_tiles) * J.k_tiles + k0) * x_stage;
+        const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
+        const uint8_t* xsrc = J.x_image + ((long long)t.tt * J.k_tiles + k0) * x_stage;
         for (int k = 0; k < steps; ++k, ++loads, x.add(1, stages), wsrc += TILE, xsrc += x_stage) {
           if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
           uint8_t* w = base + x.s * stage_bytes;
@@ -616,16 +614,17 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
   } else if (warp >= 4) {
-    mx4_clear_rest(J, eff, threadIdx.x - 128, 128);
+    mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
     Pos acc;
-    for (int i = first; i < tiles && ok; i += step, acc.add(1, 2)) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, i / m_tiles);
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
+      const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
+      Mx4Factor f{1.0f, 1.0f};
+      if (row < J.m) f = row_factor<FMT, __half, true>(J, t.expert, row);
       if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; break; }
       __syncwarp();
       tc_fence_after();
-      const int mt = row_tile(i);
       if (!PAIR || mt < J.m_tiles)
-        drain_tile<FMT, __half, true>(J, t, mt, tmem + acc.s * C::MAX_TN, warp & 3, lane, B.turn[warp & 3], !PAIR && J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
+        drain_tile<FMT, __half, true>(J, t, mt, f, tmem + acc.s * C::MAX_TN, warp & 3, lane, B.turn[warp & 3], !PAIR && J.split > 1 ? reinterpret_cast<float*>(base) : nullptr);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_first<PAIR>(&B.acc_empty[acc.s]);
@@ -636,7 +635,8 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   __syncwarp();
   if (!PAIR && J.split > 1) {
     cluster_sync();
-    if (first < tiles) add_parts<FMT, __half, true>(J, mx4_tile(J, eff, pre, first / m_tiles), first % m_tiles, reinterpret_cast<float*>(base), rank);
+    const Mx4Walk t(L, J.experts, first, step, tiles, m_tiles);
+    if (t.more()) add_parts<FMT, __half, true>(J, t, reinterpret_cast<float*>(base), rank);
     cluster_sync();
   }
   tc_fence_before();
@@ -677,7 +677,7 @@ EncodeTiled encode_tiled() {
 // and clusters that do so in turn would wait for ever.
 constexpr size_t ONE_PER_SM = 120 * 1024;
 
-size_t groups_bytes(const Mx4Job& J) { return sizeof(Bars) + (size_t)(J.experts + 1) * 8; }
+size_t groups_bytes(const Mx4Job& J) { return sizeof(Bars) + (size_t)(J.experts + 1) * 12; }
 
 }  // namespace
 

@@ -60,8 +60,13 @@ __device__ __forceinline__ float sum_cluster(uint32_t addr, int ranks) {
 }
 // Rows of every expert and the token tiles in front of it.  offsets are held to 0 .. rows and to ascend (each at least
 // the largest before it), so that whatever they hold, experts do not overlap and the tiles are no more than max_tiles.
-// Called by all threads; `eff` and `pre` have experts + 1 entries in shared memory.
-__device__ __forceinline__ void mx4_groups(const Mx4Job& J, int* eff, int* pre) {
+// Called by all threads; the lists have experts + 1 entries each, in shared memory.
+struct Mx4Lists {
+  int *eff, *pre, *per;       // an expert's first row, the token tiles in front of it, the rows of its tiles
+  __device__ __forceinline__ Mx4Lists(int* at, int experts) : eff(at), pre(at + experts + 1), per(at + 2 * (experts + 1)) {}
+};
+__device__ __forceinline__ void mx4_groups(const Mx4Job& J, const Mx4Lists& L) {
+  int *eff = L.eff, *pre = L.pre;
   if (J.offsets) {
     for (int e = threadIdx.x; e <= J.experts; e += blockDim.x) {
       const long long o = J.wide ? reinterpret_cast<const long long*>(J.offsets)[e] : reinterpret_cast<const int*>(J.offsets)[e];
@@ -100,6 +105,13 @@ __device__ __forceinline__ void mx4_groups(const Mx4Job& J, int* eff, int* pre) 
     }
   }
   __syncthreads();
+  // An expert's rows are split evenly over as few tiles as they need, in steps of 16 (no tile is empty: the tiles before the last
+  // hold fewer than the expert has).
+  for (int e = threadIdx.x; e < J.experts; e += blockDim.x) {
+    const int rows = eff[e + 1] - eff[e], tiles = max(pre[e + 1] - pre[e], 1);
+    L.per[e] = J.tn <= 16 ? J.tn : ((rows + tiles - 1) / tiles + 15) & ~15;
+  }
+  __syncthreads();
 }
 // the last e with list[e] <= v (list ascends, list[0] <= v < list[experts]): the expert that has tile, or row, v
 __device__ __forceinline__ int mx4_find(const int* list, int experts, int v) {
@@ -111,15 +123,37 @@ __device__ __forceinline__ int mx4_find(const int* list, int experts, int v) {
   }
   return lo;
 }
-// Token tile t: an expert's rows are split evenly over as few tiles as they need, in steps of 16 (no tile is empty: the tiles
-// before the last hold fewer than the expert has).
-struct Mx4Tile { int expert, row0, rows; };
-__device__ __forceinline__ int mx4_per_tile(int tn, int rows, int tiles) { return tn <= 16 ? tn : ((rows + tiles - 1) / tiles + 15) & ~15; }
-__device__ __forceinline__ Mx4Tile mx4_tile(const Mx4Job& J, const int* eff, const int* pre, int t) {
-  const int e = J.experts == 1 ? 0 : mx4_find(pre, J.experts, t);
-  const int rows = eff[e + 1] - eff[e], per = mx4_per_tile(J.tn, rows, pre[e + 1] - pre[e]), at = (t - pre[e]) * per;
-  return Mx4Tile{e, eff[e] + at, min(per, rows - at)};
-}
+// The tiles of a CTA, one after the other: number `i` of (token tile, row tile), rows first.  (A search and three divisions per tile and
+// role took 1550 clocks among the warps that decode.)
+struct Mx4Walk {
+  int i, mt, expert, row0, rows;
+  int tt, tiles, m_tiles, step, dt, dm;
+  __device__ __forceinline__ Mx4Walk(const Mx4Lists& L, int experts, int first, int step, int tiles, int m_tiles)
+      : i(first), tt(first / m_tiles), tiles(tiles), m_tiles(m_tiles), step(step) {
+    mt = first - tt * m_tiles;
+    dt = step / m_tiles;
+    dm = step - dt * m_tiles;
+    expert = row0 = rows = 0;
+    if (!more()) return;
+    if (experts > 1) expert = mx4_find(L.pre, experts, tt);
+    place(L);
+  }
+  __device__ __forceinline__ bool more() const { return i < tiles; }
+  __device__ __forceinline__ void place(const Mx4Lists& L) {
+    const int per = L.per[expert], at = (tt - L.pre[expert]) * per;
+    row0 = L.eff[expert] + at;
+    rows = min(per, L.eff[expert + 1] - row0);
+  }
+  __device__ __forceinline__ void next(const Mx4Lists& L) {
+    i += step;
+    tt += dt;
+    mt += dm;
+    if (mt >= m_tiles) { mt -= m_tiles; ++tt; }
+    if (!more()) return;
+    while (L.pre[expert + 1] <= tt) ++expert;
+    place(L);
+  }
+};
 
 __device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) {
   if (J.y_dtype == GLQB_DT_BF16) {

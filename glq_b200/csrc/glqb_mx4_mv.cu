@@ -91,8 +91,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
   uint64_t* empty = full + STAGES;
   uint64_t* ready = empty + STAGES;                                                  // [X_STAGES]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(ready + MV4_X_STAGES);
-  int* eff = const_cast<int*>(abort_flag) + 2;
-  int* pre = eff + J.experts + 1;
+  const Mx4Lists L(const_cast<int*>(abort_flag) + 2, J.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); }
@@ -101,9 +100,9 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     fence_mbar_init();
   }
   if (J.offsets) pdl_wait();
-  mx4_groups(J, eff, pre);                               // (ends with a block barrier)
+  mx4_groups(J, L);                               // (ends with a block barrier)
   pdl_trigger();
-  const int tiles = min(pre[J.experts], J.max_tiles) * J.m_tiles;
+  const int tiles = min(L.pre[J.experts], J.max_tiles) * J.m_tiles;
   const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
   const int k0 = rank * J.k_tiles / J.split, k1 = (rank + 1) * J.k_tiles / J.split;
   uint32_t q = 0;                                        // stages so far
@@ -113,9 +112,8 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
 
   if (warp == MV4_WARPS) {
     if (lane == 0) {                                     // (the weights do not depend on what runs in front of this call)
-      for (int i = first; i < tiles && ok; i += step) {
-        const int e = mx4_tile(J, eff, pre, i / J.m_tiles).expert;
-        const long long at = (long long)e * J.m_tiles + i % J.m_tiles;
+      for (Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles); t.more() && ok; t.next(L)) {
+        const long long at = (long long)t.expert * J.m_tiles + t.mt;
         for (int k = k0; k < k1; ++k, ++q) {
           const uint32_t s = q % STAGES, tops = FMT == GLQB_MX4_MXFP4 && k == k0 ? 2 * MX4_ROWS : 0;
           if (!mbar_wait(&empty[s], ((q / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
@@ -129,7 +127,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     pdl_wait();                                          // (a grid ends behind the one in front of it)
   } else {
     pdl_wait();                                          // (y may still be in use)
-    mx4_clear_rest(J, eff, threadIdx.x, MV4_WARPS * 32);
+    mx4_clear_rest(J, L.eff, threadIdx.x, MV4_WARPS * 32);
     const int g = lane >> 2, t = lane & 3, r = warp * 16 + g;
     const uint32_t codes0 = (uint32_t)(warp * 2048 + g * 128 + (g << 4) + t * 4);
     const uint32_t scales0 = (uint32_t)(MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4);
@@ -138,12 +136,11 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     constexpr int WORDS = FMT == GLQB_MX4_MXFP4 ? 2 : 4;
     // This warp's rows of x, a tile at a time: fetch() loads those of the next tile, put() writes what was loaded to buffer u % 3.  When a
     // warp puts tile q + 1 all have put tile q, which each did with its products of tile q - 2 behind it: the buffer is free.
-    int next = first, next_k = k0, rows = 0;
-    Mx4Tile ahead{0, 0, 0};
-    if (first < tiles) ahead = mx4_tile(J, eff, pre, first / J.m_tiles);
+    int next_k = k0, rows = 0;
+    Mx4Walk ahead(L, J.experts, first, step, tiles, J.m_tiles);
     uint4 raw[NB];
     auto fetch = [&]() {
-      rows = next < tiles ? ahead.rows : 0;
+      rows = ahead.more() ? ahead.rows : 0;
       if (!rows) return;
       const int col = next_k * MX4_K + lane * 8;
 #pragma unroll
@@ -154,8 +151,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
       }
       if (++next_k == k1) {
         next_k = k0;
-        next += step;
-        if (next < tiles) ahead = mx4_tile(J, eff, pre, next / J.m_tiles);
+        ahead.next(L);
       }
     };
     auto put = [&](uint32_t u) {
@@ -175,9 +171,8 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     put(0);
     fetch();
     // (a warp whose wait gave up goes through the rest without waiting: the others meet it at the barriers)
-    for (int i = first; i < tiles; i += step) {
-      const Mx4Tile tile = mx4_tile(J, eff, pre, i / J.m_tiles);
-      const int mt = i % J.m_tiles;
+    for (Mx4Walk tile(L, J.experts, first, step, tiles, J.m_tiles); tile.more(); tile.next(L)) {
+      const int mt = tile.mt;
       int top[2] = {0, 0};
       bool plain = true;                                 // rows that the short form of the multiplier covers
       Mx4Factor f{1.0f, 1.0f};
@@ -280,8 +275,8 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
     if (first >= tiles || warp == MV4_WARPS) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster_sync();
     if (first < tiles && warp < MV4_WARPS) {
-      const Mx4Tile t = mx4_tile(J, eff, pre, first / J.m_tiles);
-      const int r = threadIdx.x & 127, row = first % J.m_tiles * MX4_ROWS + r, owned = (8 * NB + J.split - 1) / J.split;
+      const Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles);
+      const int r = threadIdx.x & 127, row = t.mt * MX4_ROWS + r, owned = (8 * NB + J.split - 1) / J.split;
       if (row < J.m)
         for (int c = threadIdx.x >> 7; c * J.split + rank < t.rows; c += 2) {
           float v = 0.0f;
@@ -307,7 +302,7 @@ cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count
     using T = decltype(type);
     constexpr int F = decltype(fmt)::value, NB = decltype(blocks)::value;
     using C = Mv4<F, NB>;
-    const size_t smem = (size_t)C::STAGES * (C::STAGE + 16) + MV4_X_STAGES * (C::X_STAGE + 8 * NB * 4 + 8) + 2 * 8 * NB * MX4_ROWS * 4 + 8 + (size_t)(J.experts + 1) * 8;
+    const size_t smem = (size_t)C::STAGES * (C::STAGE + 16) + MV4_X_STAGES * (C::X_STAGE + 8 * NB * 4 + 8) + 2 * 8 * NB * MX4_ROWS * 4 + 8 + (size_t)(J.experts + 1) * 12;
     constexpr auto K = mx4_mv_kernel<F, T, NB>;
     return mx4_launch<K>(K, grid, MV4_THREADS, smem, J.split, stream, J);
   };
