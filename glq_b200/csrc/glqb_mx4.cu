@@ -4,6 +4,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 namespace glqb {
 namespace {
@@ -485,26 +486,35 @@ struct Form {
   bool align, mv;
   size_t image, bytes;        // of the workspace: x in 4 bits or aligned, then two floats
 };
-struct Device { std::atomic<int> sms; std::atomic<int*> status; };
-static Device* device() {
+struct Device {
+  std::atomic<int> sms{0};
+  int* status = nullptr;
+  int mv[9] = {}, gemm[9] = {};       // clusters that are there at once, by their CTAs
+};
+static const Device* device() {
   static Device known[64];
+  static std::mutex building;
   Device& d = known[mx4_device()];
   if (d.sms.load(std::memory_order_acquire) == 0) {
+    std::lock_guard<std::mutex> lock(building);
     int n = 0;
-    int* p = nullptr;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, mx4_device()) != cudaSuccess || n < 1 ||
-        cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_mx4_status) != cudaSuccess)
-      return nullptr;
-    d.status.store(p, std::memory_order_relaxed);
-    d.sms.store(n, std::memory_order_release);
+    if (d.sms.load(std::memory_order_relaxed) == 0) {
+      if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, mx4_device()) != cudaSuccess || n < 1 ||
+          cudaGetSymbolAddress(reinterpret_cast<void**>(&d.status), g_mx4_status) != cudaSuccess)
+        return nullptr;
+      for (int s = 2; s <= 8; ++s) { d.mv[s] = mx4_mv_clusters(s); d.gemm[s] = mx4_gemm_clusters(s); }
+      d.sms.store(n, std::memory_order_release);
+    }
   }
   return &d;
 }
-constexpr int MV_MAX_ROWS = 16;     // rows (an expert's, on average) up to which the streaming kernel runs
-static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, int sms) {
+// Rows (an expert's, on average) up to which the streaming kernel runs.  Above / below, in a graph: 12 tokens of 4096 x 14336 19.8 / 17.3 us, of
+// 2048 x 2048 13.8 / 5.4, 16 of 14336 x 4096 19.8 / 20.5; 128 experts of 1536 x 2048, 600 rows 96 / 89, 1400 rows 98 / 108.
+constexpr int MV_MAX_ROWS = 16, MV_MAX_EXPERT_ROWS = 8;
+static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, const Device* d) {
   Form f = {};
   const int avg = (int)((rows + w->experts - 1) / w->experts);
-  f.mv = !quantize && avg <= MV_MAX_ROWS;
+  f.mv = !quantize && avg <= (w->experts == 1 ? MV_MAX_ROWS : MV_MAX_EXPERT_ROWS);
   const int most = quantize ? (w->format == GLQB_MX4_MXFP4 ? 192 : 160) : 192;
   // token tiles: a matrix's rows split evenly; of experts up to twice their average, so that most have one tile
   if (f.mv) f.tn = avg > (w->experts == 1 ? 8 : 4) ? 16 : 8;
@@ -512,8 +522,10 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
   else f.tn = std::min(most, (2 * avg + 15) / 16 * 16);
   f.max_tiles = w->experts == 1 ? (int)((rows + f.tn - 1) / f.tn) : (int)(rows / f.tn + std::min<long long>(w->experts, rows));
   const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K, tiles = f.max_tiles * mt;
-  // CTAs that share a tile's sum: as many as the SMs hold at once
-  f.split = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, kt), (f.mv ? 2 : 1) * sms / std::max<long long>(1, tiles)));
+  // CTAs that share a tile's sum: as many as leave all tiles there at once
+  f.split = 1;
+  for (int s = 2; d && s <= std::min<long long>(8, kt); ++s)
+    if (tiles <= (f.mv ? d->mv : d->gemm)[s]) f.split = s;
   f.pair = !f.mv && f.split == 1 && f.tn >= 96 && mt > 1;
   if (quantize) {
     f.x_scales = mx4_x_scale_bytes(w->format, f.tn);
@@ -529,7 +541,7 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
 
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize) {
   if (!w || !format_ok(w->format) || rows <= 0 || rows >= (1ll << 31) || w->experts < 1 || w->m < 1 || w->n < 1) return 0;
-  return form_of(w, rows, x_stride, x, quantize, 1).bytes;      // (what a call needs does not depend on the SMs)
+  return form_of(w, rows, x_stride, x, quantize, nullptr).bytes;      // (what a call needs does not depend on the device)
 }
 
 int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows,
@@ -547,11 +559,11 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   if (!w->image || !x || !y || (w->format == GLQB_MX4_NVFP4 && !w->tensor_scale)) return mx4_fail(GLQB_E_INVALID, "mx4_product: null argument");
   if (rows > 1 && (x_stride < w->n || y_stride < w->m)) return mx4_fail(GLQB_E_INVALID, "mx4_product: rows overlap");
   const Device* d = device();
-  const int sms = d ? d->sms.load(std::memory_order_relaxed) : 1;      // (the workspace does not depend on it)
-  const Form f = form_of(w, rows, x_stride, x, quantize, sms);
+  const Form f = form_of(w, rows, x_stride, x, quantize, d);
   if (workspace_bytes < f.bytes || (f.bytes && !workspace))
     return mx4_fail(GLQB_E_WORKSPACE, "mx4_product: workspace of %zu bytes, %zu needed", workspace_bytes, f.bytes);
   if (!d) return mx4_fail(GLQB_E_CUDA, "mx4_product: no device");
+  const int sms = d->sms.load(std::memory_order_relaxed);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   cudaError_t e = cudaSuccess;
   Mx4Job J = {};
@@ -577,7 +589,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.y_wide = y_dtype != GLQB_DT_F32 && !accumulate && reinterpret_cast<uintptr_t>(y) % 16 == 0 && (rows == 1 || y_stride % 8 == 0);
   J.x = x;
   J.x_stride = x_stride;
-  J.status = d->status.load(std::memory_order_relaxed);
+  J.status = d->status;
   const size_t lists = (size_t)(J.experts + 1) * 12;
   J.clear = offsets && clear_rest;
   if (!quantize) {

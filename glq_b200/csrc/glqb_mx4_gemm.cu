@@ -266,18 +266,6 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Walk& t, flo
   }
 }
 
-struct Pos {                   // a place in a ring, and the parity of its round
-  uint32_t s = 0, phase = 0;
-  __device__ __forceinline__ void add(uint32_t d, uint32_t n) {
-    s += d;
-    while (s >= n) { s -= n; phase ^= 1u; }
-  }
-  __device__ __forceinline__ void back(uint32_t n) {
-    if (s == 0) { s = n; phase ^= 1u; }
-    --s;
-  }
-};
-
 // ---- 16-bit activations ---------------------------------------------------------------------------
 // Weights come as they lie, 17 KiB per 128 x 256 (bulk copies), are decoded by sixteen warps straight into tensor memory as
 // the A operand (thread = row, 64 values = 32 columns), activations by TMA as 64-value boxes with the 128-byte swizzle.  A step
@@ -331,7 +319,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
 
   if (warp == 0) {
     if (!PAIR || rank == 0) {
-      Pos a, x, acc;
+      Mx4Pos a, x, acc;
       const uint32_t x0 = smem_u32(x_base);
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
         const uint32_t idesc = idesc16(__is_same(T, __half) ? 0 : 1, PAIR ? 256 : 128, cols_of(t)), d = tmem + acc.s * R.acc_cols;
@@ -359,7 +347,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   } else if (warp == 1) {
     // (a box per lane: one thread that issues them in turn is late among the warps that decode)
     pdl_wait();
-    Pos x;
+    Mx4Pos x;
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
       const int rows = PAIR ? cols_of(t) / 2 : t.rows, row0 = t.row0 + (PAIR ? rank * rows : 0), boxes = (rows + R.box_rows - 1) / R.box_rows;
       const int box = lane >> 1, half = lane & 1, to = half * R.x_half + box * R.box_rows * 128;
@@ -375,7 +363,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
   } else if (warp == 2) {
     if (lane == 0) {                               // (the weights do not depend on what runs in front of this call)
-      Pos w;
+      Mx4Pos w;
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
         const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
         for (int k = k0; k < k1; ++k, ++loads_w, src += TILE, w.add(1, G16_W_STAGES)) {
@@ -390,7 +378,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     // of a group's eight warps four take the first 64 values of a step, four the others; a warp the 32 rows of its quarter of tensor memory
     const int group = (warp - 8) >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t to = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + half * 32u;
-    Pos a, w;
+    Mx4Pos a, w;
     a.add(group, R.a_stages);
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
       int top = 0;
@@ -450,7 +438,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   } else if (warp >= 4) {
     pdl_wait();                                    // (y may still be in use)
     mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
-    Pos acc;
+    Mx4Pos acc;
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
       const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
       Mx4Factor f{1.0f, 1.0f};
@@ -552,7 +540,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   bool ok = true;
 
   if (warp == 0) {
-    Pos x, acc;
+    Mx4Pos x, acc;
     if (!PAIR || rank == 0) {
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
         const int cols = (t.rows + 15) & ~15;
@@ -597,7 +585,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   } else if (warp == 1) {
     if (lane == 0) {
       const int x_stage = J.tn * 128 + x_scales;
-      Pos x;
+      Mx4Pos x;
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
         const uint32_t x_codes = (uint32_t)((t.rows + 15) & ~15) * (PAIR ? 64u : 128u);
         const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
@@ -615,7 +603,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
     }
   } else if (warp >= 4) {
     mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
-    Pos acc;
+    Mx4Pos acc;
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
       const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
       Mx4Factor f{1.0f, 1.0f};
@@ -680,6 +668,8 @@ constexpr size_t ONE_PER_SM = 120 * 1024;
 size_t groups_bytes(const Mx4Job& J) { return sizeof(Bars) + (size_t)(J.experts + 1) * 12; }
 
 }  // namespace
+
+int mx4_gemm_clusters(int split) { return mx4_clusters(mx4_gemm4_kernel<GLQB_MX4_MXFP4, false>, G4_THREADS, ONE_PER_SM, split); }
 
 cudaError_t mx4_gemm16_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count, cudaStream_t stream, const char** what) {
   Mx4Ring R;

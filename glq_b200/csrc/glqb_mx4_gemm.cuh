@@ -155,6 +155,18 @@ struct Mx4Walk {
   }
 };
 
+struct Mx4Pos {                   // a place in a ring, and the parity of its round
+  uint32_t s = 0, phase = 0;
+  __device__ __forceinline__ void add(uint32_t d, uint32_t n) {
+    s += d;
+    while (s >= n) { s -= n; phase ^= 1u; }
+  }
+  __device__ __forceinline__ void back(uint32_t n) {
+    if (s == 0) { s = n; phase ^= 1u; }
+    --s;
+  }
+};
+
 __device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) {
   if (J.y_dtype == GLQB_DT_BF16) {
     __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(J.y) + at;
@@ -290,6 +302,26 @@ inline cudaError_t mx4_launch(void (*kernel)(P...), int grid, int threads, size_
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+// Clusters of `cluster` CTAs that the device holds at once (SMs come in groups whose size no cluster divides: 132 CTAs of 148 in clusters
+// of four, 120 of eight; a launch of more takes twice as long).
+template <typename... P>
+inline int mx4_clusters(void (*kernel)(P...), int threads, size_t smem, int cluster) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess ? n : 0;
+}
+int mx4_mv_clusters(int split);
+int mx4_gemm_clusters(int split);
 // ---- glqb_mx4_mv.cu
 // Few rows of x (tn 8 or 16), which start on 16 bytes and end on whole eights of values.
 cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& job, int sm_count, cudaStream_t stream);

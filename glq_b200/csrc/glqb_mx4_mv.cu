@@ -1,15 +1,15 @@
 // Products of microscaled 4-bit weights with few rows of x: decode steps, experts of few tokens.
 //
 // What bounds these is the weights' way from HBM and, close behind, the instructions that make 16-bit operands of them.  A CTA
-// takes 128 weight rows x 8 NB rows of x; one warp brings tiles of 128 x 256 weights into a ring of stages (bulk copies) and runs
-// ahead over the borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile into fragments of mma.sync.m16n8k16 in
+// takes 128 weight rows x 8 NB rows of x; one warp brings tiles of 128 x 256 weights into a ring of stages (bulk copies), two or four bring the
+// values of x that belong to them, and they run ahead over the borders of the CTA's work.  Eight warps take 16 weight rows each, turn a tile into fragments of mma.sync.m16n8k16 in
 // registers and multiply.  The MMA's order of values is free as long as both operands have it: lane t of a quad takes word t of a
 // 16-byte unit, eight values, and of x the same eight, so nothing is exchanged and every shared-memory access is free of
 // conflicts.  Where there are few tiles the CTAs of a cluster share out the values and add their parts in rank order.
 //
 // Operands are fp16, because two codes become fp16 in one instruction and bf16 in four (as bf16: 505 instructions per warp
-// for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  Rows of x are loaded two
-// tiles ahead and put to shared memory one ahead, bf16 as fp16, 256 values at a time, by the power of two that takes the largest finite one to 2^14 .. 2^15; the sums of a tile are multiplied back in
+// for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  bf16 rows of x are brought to
+// fp16 on their way to shared memory, 256 values at a time, by the power of two that takes the largest finite one to 2^14 .. 2^15; the sums of a tile are multiplied back in
 // fp32.  Values of at least 2^-32 of the largest are exact, smaller ones off by at most 2^-40 of it.
 #include "glqb_mx4_gemm.cuh"
 #include "glqb_launch.h"
@@ -18,12 +18,13 @@
 namespace glqb {
 namespace {
 
-constexpr int MV4_WARPS = 8, MV4_THREADS = (MV4_WARPS + 1) * 32;
+constexpr int MV4_WARPS = 8;
 constexpr int MV4_X_ROW = MX4_K * 2 + 64;        // bytes of a row of x: two rows in different banks
-constexpr int MV4_X_STAGES = 3;                  // of x: being written, being read, and read by warps that lag behind
 template <int FMT, int NB> struct Mv4 {
-  static constexpr int STAGE = mx4_tile_bytes(FMT) + (FMT == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0);   // (the rows' largest scales)
-  static constexpr int STAGES = NB == 1 ? 4 : 3, X_STAGE = 8 * NB * MV4_X_ROW;                     // two CTAs per SM
+  static constexpr int X = mx4_tile_bytes(FMT) + (FMT == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0);       // of a stage: weights, their rows' largest scales,
+  static constexpr int X_SCALE = X + 8 * NB * MV4_X_ROW, STAGE = X_SCALE + 128;                    // x, what its sums are multiplied by
+  static constexpr int STAGES = NB == 1 ? 4 : 3;                                                   // two CTAs per SM
+  static constexpr int X_WARPS = 2 * NB, THREADS = (MV4_WARPS + 1 + X_WARPS) * 32;
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -81,119 +82,132 @@ __device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
 }
 
 template <int FMT, typename T, int NB>
-__global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J) {
-  constexpr int TILE = mx4_tile_bytes(FMT), STAGE = Mv4<FMT, NB>::STAGE, STAGES = Mv4<FMT, NB>::STAGES;
+__global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J) {
+  using C = Mv4<FMT, NB>;
+  constexpr int TILE = mx4_tile_bytes(FMT), STAGE = C::STAGE, STAGES = C::STAGES;
   extern __shared__ __align__(128) uint8_t ring[];
-  uint8_t* xs = ring + STAGES * STAGE;                                               // [X_STAGES][8 NB] rows of fp16
-  float* red = reinterpret_cast<float*>(xs + MV4_X_STAGES * Mv4<FMT, NB>::X_STAGE);  // [2][8 NB][128]
-  float* x_scale = red + 2 * 8 * NB * MX4_ROWS;                                      // [X_STAGES][8 NB]
-  uint64_t* full = reinterpret_cast<uint64_t*>(x_scale + MV4_X_STAGES * 8 * NB);
+  float* red = reinterpret_cast<float*>(ring + STAGES * STAGE);                      // [2][8 NB][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(red + 2 * 8 * NB * MX4_ROWS);
   uint64_t* empty = full + STAGES;
-  uint64_t* ready = empty + STAGES;                                                  // [X_STAGES]
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(ready + MV4_X_STAGES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
   const Mx4Lists L(const_cast<int*>(abort_flag) + 2, J.experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], MV4_WARPS); }
-    for (int s = 0; s < MV4_X_STAGES; ++s) mbar_init(&ready[s], MV4_WARPS);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1 + C::X_WARPS); mbar_init(&empty[s], MV4_WARPS); }
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (J.offsets) pdl_wait();
-  mx4_groups(J, L);                               // (ends with a block barrier)
+  mx4_groups(J, L);                                      // (ends with a block barrier)
   pdl_trigger();
   const int tiles = min(L.pre[J.experts], J.max_tiles) * J.m_tiles;
   const int first = blockIdx.x / J.split, step = gridDim.x / J.split, rank = blockIdx.x % J.split;
   const int k0 = rank * J.k_tiles / J.split, k1 = (rank + 1) * J.k_tiles / J.split;
-  uint32_t q = 0;                                        // stages so far
+  uint32_t loads = 0;
   bool ok = true;
   Mx4Factor factor{1.0f, 1.0f};
   if (J.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   if (warp == MV4_WARPS) {
     if (lane == 0) {                                     // (the weights do not depend on what runs in front of this call)
+      Mx4Pos p;
       for (Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles); t.more() && ok; t.next(L)) {
         const long long at = (long long)t.expert * J.m_tiles + t.mt;
-        for (int k = k0; k < k1; ++k, ++q) {
-          const uint32_t s = q % STAGES, tops = FMT == GLQB_MX4_MXFP4 && k == k0 ? 2 * MX4_ROWS : 0;
-          if (!mbar_wait(&empty[s], ((q / STAGES) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-          mbar_expect_tx(&full[s], TILE + tops);
-          bulk_g2s(ring + s * STAGE, J.image + (at * J.k_tiles + k) * TILE, TILE, &full[s]);
-          if (tops) bulk_g2s(ring + s * STAGE + TILE, J.tops + at * MX4_ROWS, tops, &full[s]);
+        const uint8_t* src = J.image + (at * J.k_tiles + k0) * TILE;
+        for (int k = k0; k < k1; ++k, ++loads, src += TILE, p.add(1, STAGES)) {
+          const uint32_t tops = FMT == GLQB_MX4_MXFP4 && k == k0 ? 2 * MX4_ROWS : 0;
+          if (!mbar_wait(&empty[p.s], p.phase ^ 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&full[p.s], TILE + tops);
+          bulk_g2s(ring + p.s * STAGE, src, TILE, &full[p.s]);
+          if (tops) bulk_g2s(ring + p.s * STAGE + TILE, J.tops + at * MX4_ROWS, tops, &full[p.s]);
         }
       }
       if (!ok) { *abort_flag = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
     pdl_wait();                                          // (a grid ends behind the one in front of it)
+  } else if (warp > MV4_WARPS) {
+    // four rows of x each: those of the next tile are on their way while the last ones are written
+    pdl_wait();
+    constexpr int OWN = 8 * NB / C::X_WARPS;
+    const int mine = warp - MV4_WARPS - 1;
+    Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles);
+    int k = k0, rows = 0;
+    const T* at = nullptr;                               // of row `mine`
+    auto place = [&]() {
+      rows = t.more() ? t.rows : 0;
+      at = reinterpret_cast<const T*>(J.x) + (long long)(t.row0 + mine) * J.x_stride + k0 * MX4_K + lane * 8;
+    };
+    auto fetch = [&](uint4 (&raw)[OWN]) {
+      const bool in = k * MX4_K + lane * 8 < J.n;        // (n is a multiple of eight)
+#pragma unroll
+      for (int n = 0; n < OWN; ++n) {
+        raw[n] = make_uint4(0, 0, 0, 0);
+        if (mine + C::X_WARPS * n < rows && in) raw[n] = *reinterpret_cast<const uint4*>(at + C::X_WARPS * n * J.x_stride);
+      }
+      at += MX4_K;
+    };
+    auto put = [&](const uint4 (&raw)[OWN], int there, const Mx4Pos& p) -> bool {
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty[p.s], p.phase ^ 1u, abort_flag))) return false;
+      uint8_t* stage = ring + p.s * STAGE;
+#pragma unroll
+      for (int n = 0; n < OWN; ++n) {
+        const int row = mine + C::X_WARPS * n;
+        if (row >= there) break;
+        const float down = put8<FMT, T>(stage + C::X + row * MV4_X_ROW + lane * 16, raw[n]);
+        if (lane == 0) *reinterpret_cast<float*>(stage + C::X_SCALE + row * 4) = down;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[p.s]);
+      return true;
+    };
+    Mx4Pos p;
+    uint4 now[OWN];
+    place();
+    if (rows) fetch(now);
+    while (rows && ok) {
+      const int there = rows;
+      if (++k == k1) {
+        k = k0;
+        t.next(L);
+        place();
+      }
+      uint4 next[OWN];
+      if (rows) fetch(next);
+      ok = put(now, there, p);
+#pragma unroll
+      for (int n = 0; n < OWN; ++n) now[n] = next[n];
+      p.add(1, STAGES);
+    }
+    if (!ok) { *abort_flag = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
   } else {
     pdl_wait();                                          // (y may still be in use)
     mx4_clear_rest(J, L.eff, threadIdx.x, MV4_WARPS * 32);
     const int g = lane >> 2, t = lane & 3, r = warp * 16 + g;
     const uint32_t codes0 = (uint32_t)(warp * 2048 + g * 128 + (g << 4) + t * 4);
-    const uint32_t scales0 = (uint32_t)(MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4);
+    const uint32_t scales0 = (uint32_t)(MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4), x0 = (uint32_t)(C::X + g * MV4_X_ROW + t * 16);
     const uint32_t pick = (uint32_t)(t >> 1) | (uint32_t)((t >> 1) + 2) << 4;
-    int turn = 0;
     constexpr int WORDS = FMT == GLQB_MX4_MXFP4 ? 2 : 4;
-    // This warp's rows of x, a tile at a time: fetch() loads those of the next tile, put() writes what was loaded to buffer u % 3.  When a
-    // warp puts tile q + 1 all have put tile q, which each did with its products of tile q - 2 behind it: the buffer is free.
-    int next_k = k0, rows = 0;
-    Mx4Walk ahead(L, J.experts, first, step, tiles, J.m_tiles);
-    uint4 raw[NB];
-    auto fetch = [&]() {
-      rows = ahead.more() ? ahead.rows : 0;
-      if (!rows) return;
-      const int col = next_k * MX4_K + lane * 8;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int row = warp + 8 * n;
-        raw[n] = make_uint4(0, 0, 0, 0);
-        if (row < rows && col < J.n) raw[n] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(J.x) + (ahead.row0 + row) * J.x_stride + col);
-      }
-      if (++next_k == k1) {
-        next_k = k0;
-        ahead.next(L);
-      }
-    };
-    auto put = [&](uint32_t u) {
-      if (!rows) return;
-      const uint32_t s = u % MV4_X_STAGES;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int row = warp + 8 * n;
-        if (row >= rows) break;
-        const float down = put8<FMT, T>(xs + s * Mv4<FMT, NB>::X_STAGE + row * MV4_X_ROW + lane * 16, raw[n]);
-        if (lane == 0) x_scale[s * 8 * NB + row] = down;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ready[s]);
-    };
-    fetch();
-    put(0);
-    fetch();
+    int turn = 0;
+    Mx4Pos p;
     // (a warp whose wait gave up goes through the rest without waiting: the others meet it at the barriers)
     for (Mx4Walk tile(L, J.experts, first, step, tiles, J.m_tiles); tile.more(); tile.next(L)) {
-      const int mt = tile.mt;
       int top[2] = {0, 0};
       bool plain = true;                                 // rows that the short form of the multiplier covers
       Mx4Factor f{1.0f, 1.0f};
       if constexpr (FMT == GLQB_MX4_NVFP4) f.b = __ldg(J.w_scale + tile.expert);
       float acc[NB][4] = {};
-      for (int k = k0; k < k1; ++k, ++q) {
-        const uint32_t s = q % STAGES, xq = q % MV4_X_STAGES;
-        if (!ok || !mbar_wait(&ready[xq], (q / MV4_X_STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; continue; }
-        put(q + 1);
-        fetch();
-        if (!mbar_wait(&full[s], (q / STAGES) & 1u, abort_flag)) { ok = false; *abort_flag = 1; continue; }
-        const uint8_t* stage = ring + s * STAGE;
+      for (int k = k0; k < k1; ++k, p.add(1, STAGES)) {
+        if (!ok || !mbar_wait(&full[p.s], p.phase, abort_flag)) { ok = false; *abort_flag = 1; continue; }
+        const uint8_t* stage = ring + p.s * STAGE;
         if constexpr (FMT == GLQB_MX4_MXFP4) {
           if (k == k0) {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(stage + TILE);
-            top[0] = p[r];
-            top[1] = p[r + 8];
+            const uint16_t* tops = reinterpret_cast<const uint16_t*>(stage + TILE);
+            top[0] = tops[r];
+            top[1] = tops[r + 8];
             plain = !__any_sync(0xFFFFFFFFu, ((top[0] | top[1]) & 256) != 0);
             top[0] &= 255;
             top[1] &= 255;
-            f = mx4_power<T>(p[threadIdx.x & 127]);
+            f = mx4_power<T>(tops[threadIdx.x & 127]);
           }
         }
         uint32_t sw[2][WORDS];
@@ -201,24 +215,23 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int a = 0; a < WORDS; ++a) sw[h][a] = *reinterpret_cast<const uint32_t*>(stage + scales0 + 128 * h + 512 * a);
-        const uint8_t* xr = xs + xq * Mv4<FMT, NB>::X_STAGE + g * MV4_X_ROW + t * 16;
         float d[NB][2][4] = {};                          // two chains of MMAs
         auto units = [&](auto is_plain) {
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {                  // two units of 16 bytes
+          for (int i = 0; i < 4; ++i) {                  // two units of 16 bytes
             uint32_t m[2][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) multipliers<FMT>(sw[h][FMT == GLQB_MX4_MXFP4 ? p >> 1 : p], p, top[h], decltype(is_plain)::value, pick, m[h]);
+            for (int h = 0; h < 2; ++h) multipliers<FMT>(sw[h][FMT == GLQB_MX4_MXFP4 ? i >> 1 : i], i, top[h], decltype(is_plain)::value, pick, m[h]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const int j = 2 * p + u;
+              const int j = 2 * i + u;
               const uint8_t* c = stage + (codes0 ^ (uint32_t)(j << 4));
               uint32_t w[2][4];
               mx4_bytes_f16(*reinterpret_cast<const uint32_t*>(c), w[0]);
               mx4_bytes_f16(*reinterpret_cast<const uint32_t*>(c + 1024), w[1]);
               uint4 b[NB];
 #pragma unroll
-              for (int n = 0; n < NB; ++n) b[n] = *reinterpret_cast<const uint4*>(xr + n * 8 * MV4_X_ROW + j * 64);
+              for (int n = 0; n < NB; ++n) b[n] = *reinterpret_cast<const uint4*>(stage + x0 + n * 8 * MV4_X_ROW + j * 64);
 #pragma unroll
               for (int v = 0; v < 2; ++v) {
                 uint32_t a[4];
@@ -235,12 +248,12 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           float2 down = make_float2(1.0f, 1.0f);
-          if constexpr (!__is_same(T, __half)) down = *reinterpret_cast<const float2*>(x_scale + xq * 8 * NB + n * 8 + 2 * t);
+          if constexpr (!__is_same(T, __half)) down = *reinterpret_cast<const float2*>(stage + C::X_SCALE + (n * 8 + 2 * t) * 4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(d[n][0][e] + d[n][1][e], e & 1 ? down.y : down.x, acc[n][e]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
+        if (lane == 0) mbar_arrive(&empty[p.s]);
       }
       if (J.split > 1) {
         // Each column of a shared tile has a CTA that adds it up: the parts go to its memory, part by part.
@@ -263,7 +276,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][e];
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const int row = mt * MX4_ROWS + (threadIdx.x & 127);
+      const int row = tile.mt * MX4_ROWS + (threadIdx.x & 127);
       if (row < J.m)
         for (int c = threadIdx.x >> 7; c < tile.rows; c += 2)
           mx4_put(J, (long long)(tile.row0 + c) * J.y_stride + row, sums[c * MX4_ROWS + (threadIdx.x & 127)] * f.a * f.b);
@@ -272,7 +285,7 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
   }
   __syncwarp();
   if (J.split > 1) {                                     // (one tile per cluster)
-    if (first >= tiles || warp == MV4_WARPS) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (first >= tiles || warp >= MV4_WARPS) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster_sync();
     if (first < tiles && warp < MV4_WARPS) {
       const Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles);
@@ -289,10 +302,17 @@ __global__ void __launch_bounds__(MV4_THREADS, 2) mx4_mv_kernel(const __grid_con
   }
   __syncthreads();
   if (*abort_flag && warp == MV4_WARPS && lane == 0)     // copies still under way
-    for (uint32_t n = 0; n < min(q, (uint32_t)STAGES); ++n) mbar_wait(&full[(q - 1 - n) % STAGES], ((q - 1 - n) / STAGES) & 1u);
+    for (uint32_t n = 0; n < min(loads, (uint32_t)STAGES); ++n) mbar_wait(&full[(loads - 1 - n) % STAGES], ((loads - 1 - n) / STAGES) & 1u);
 }
 
 }  // namespace
+
+template <int F, typename T, int NB>
+static size_t mv_smem(int experts) {
+  using C = Mv4<F, NB>;
+  return (size_t)C::STAGES * (C::STAGE + 16) + 2 * 8 * NB * MX4_ROWS * 4 + 8 + (size_t)(experts + 1) * 12;
+}
+int mx4_mv_clusters(int split) { return mx4_clusters(mx4_mv_kernel<GLQB_MX4_MXFP4, __half, 1>, Mv4<GLQB_MX4_MXFP4, 1>::THREADS, mv_smem<GLQB_MX4_MXFP4, __half, 1>(1), split); }
 
 cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count, cudaStream_t stream) {
   const int nb = J.tn / 8;
@@ -301,10 +321,8 @@ cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count
   auto run = [&](auto fmt, auto type, auto blocks) {
     using T = decltype(type);
     constexpr int F = decltype(fmt)::value, NB = decltype(blocks)::value;
-    using C = Mv4<F, NB>;
-    const size_t smem = (size_t)C::STAGES * (C::STAGE + 16) + MV4_X_STAGES * (C::X_STAGE + 8 * NB * 4 + 8) + 2 * 8 * NB * MX4_ROWS * 4 + 8 + (size_t)(J.experts + 1) * 12;
     constexpr auto K = mx4_mv_kernel<F, T, NB>;
-    return mx4_launch<K>(K, grid, MV4_THREADS, smem, J.split, stream, J);
+    return mx4_launch<K>(K, grid, Mv4<F, NB>::THREADS, mv_smem<F, T, NB>(J.experts), J.split, stream, J);
   };
   using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
   using N = std::integral_constant<int, GLQB_MX4_NVFP4>;
