@@ -17,7 +17,7 @@ FMT_TRELLIS_3INST = 0
 FMT_E8_SHELL = 1
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 MX4_MXFP4, MX4_NVFP4 = 0, 1
-MX4_SCALE_FLOATS = 257
+MX4_SCALE_FLOATS = 297
 
 EXPORTS = [
     "glqb_plan_create", "glqb_plan_workspace_bytes", "glqb_plan_code_bytes", "glqb_plan_flops",

@@ -24,6 +24,7 @@ int mx4_launched(const char* what) {
 }
 
 constexpr int QT_THREADS = 256;
+constexpr int MX4_MAX_SIZE = 1 << 30, MX4_MAX_ROWS = 0x7FFF0000;   // (sums with a tile's size stay 32-bit)
 
 __device__ int g_mx4_status;   // 0, or what gave up (ST_GAVE_UP_*): products have no plan to keep it in
 
@@ -62,10 +63,12 @@ __device__ __forceinline__ void place(const Mx4Rows& q, I i, I& row, I& c) {
 
 // ---- largest finite magnitude ---------------------------------------------------------------------
 // A part per CTA; those who need the whole reduce the parts (no atomics, nothing to clear beforehand).
-constexpr int AMAX_PARTS = 256, AMAX_THREADS = 1024;
+constexpr int AMAX_PARTS = 296, AMAX_THREADS = 1024;      // (two CTAs on each of 148 SMs)
 static_assert(AMAX_PARTS + 1 == GLQB_MX4_SCALE_FLOATS, "");
 template <typename T, typename I>
-__global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* __restrict__ x, Mx4Rows q, Mx4Range range, float* __restrict__ parts) {
+__global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* x, Mx4Rows q, Mx4Range range, float* parts) {
+  pdl_wait();
+  pdl_trigger();
   uint32_t top = 0;
   long long first, last;
   range.get(q.rows, first, last);
@@ -103,7 +106,8 @@ __global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* __restr
 // The tensor's scale for all threads of a block of 256: given, or from the parts; the first block leaves it in own_scale[0].
 __device__ __forceinline__ float whole_scale(const float* given, float* own_scale, int parts) {
   if (given) return *given;
-  uint32_t top = threadIdx.x < parts ? __float_as_uint(own_scale[1 + threadIdx.x]) : 0u;      // (non-negative: ordered as their bits)
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < parts; i += QT_THREADS) top = max(top, __float_as_uint(own_scale[1 + i]));      // (non-negative: ordered as their bits)
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   __shared__ uint32_t tops[QT_THREADS / 32];
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
@@ -119,9 +123,11 @@ __device__ __forceinline__ float whole_scale(const float* given, float* own_scal
 // HBM bound: 2 or 4 bytes in and 0.53 or 0.56 out per value.
 template <typename T, int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
-mx4_quantize_kernel(const T* __restrict__ x, Mx4Rows q, const float* tensor_scale, float* own_scale, int parts, uint8_t* __restrict__ codes,
-                    uint8_t* __restrict__ scales) {
+mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own_scale, int parts, uint8_t* codes,
+                    uint8_t* scales) {
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
+  pdl_wait();
+  pdl_trigger();
   float t = 1.0f;
   if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(tensor_scale, own_scale, parts);
   const long long code_row = (q.cols + 1) / 2, scale_row = q.chunks / PER;
@@ -159,9 +165,11 @@ mx4_quantize_kernel(const T* __restrict__ x, Mx4Rows q, const float* tensor_scal
 
 template <int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
-mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale,
-                      long long rows_per_scale, Mx4Rows q, void* __restrict__ out, int out_dtype) {
+mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, Mx4Rows q, void* out,
+                      int out_dtype) {
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
+  pdl_wait();
+  pdl_trigger();
   const long long code_row = (q.cols + 1) / 2, scale_row = q.chunks / PER;
   const I total = (I)(q.rows * q.chunks);
   const bool one_scale = FMT != GLQB_MX4_NVFP4 || rows_per_scale >= q.rows;
@@ -296,8 +304,9 @@ __global__ void __launch_bounds__(256) mx4_row_top_kernel(const uint8_t* __restr
 
 // ---- activations of the products ------------------------------------------------------------------
 // Rows that TMA cannot read (not on 16 bytes) are copied, to rows of a multiple of eight values.
-__global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* __restrict__ x, long long x_stride, long long rows, int n, int n_pad,
-                                                        uint16_t* __restrict__ out) {
+__global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* x, long long x_stride, long long rows, int n, int n_pad, uint16_t* out) {
+  pdl_wait();
+  pdl_trigger();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * n_pad; i += (long long)gridDim.x * 256) {
     const long long r = i / n_pad;
     const int c = (int)(i - r * n_pad);
@@ -314,6 +323,8 @@ __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_co
                                                                  int x_scales, bool vec, int batches) {
   extern __shared__ int lists[];
   const Mx4Lists L(lists, J.experts);
+  pdl_wait();
+  pdl_trigger();
   mx4_groups(J, L);
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
   float t = 1.0f;
@@ -375,7 +386,7 @@ int amax_launch(const void* x, int x_dtype, const Mx4Rows& q, const Mx4Range& ra
   const int grid = (int)std::min<long long>((q.rows * q.chunks + AMAX_THREADS - 1) / AMAX_THREADS, AMAX_PARTS);
   auto run = [&](auto type, auto index) {
     using T = decltype(type);
-    mx4_amax_kernel<T, decltype(index)><<<grid, AMAX_THREADS, 0, stream>>>((const T*)x, q, range, parts);
+    launch_chained(true, mx4_amax_kernel<T, decltype(index)>, grid, AMAX_THREADS, 0, stream, (const T*)x, q, range, parts);
   };
   auto of = [&](auto type) { q.rows * q.chunks < (1ll << 31) - (long long)AMAX_PARTS * AMAX_THREADS * QT_BATCH ? run(type, (uint32_t)0) : run(type, (uint64_t)0); };
   if (x_dtype == GLQB_DT_F16) of(__half());
@@ -390,7 +401,8 @@ int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const float* t
   if (FMT == GLQB_MX4_NVFP4 && !tensor_scale) parts = amax_launch(x, x_dtype, q, Mx4Range{nullptr, 0, 0}, own_scale + 1, stream);
   auto run = [&](auto type, auto index) {
     using T = decltype(type);
-    mx4_quantize_kernel<T, FMT, decltype(index)><<<grid_for(q), QT_THREADS, 0, stream>>>((const T*)x, q, tensor_scale, own_scale, parts, codes, scales);
+    launch_chained(true, mx4_quantize_kernel<T, FMT, decltype(index)>, (int)grid_for(q), QT_THREADS, 0, stream, (const T*)x, q, tensor_scale, own_scale, parts, codes,
+                   scales);
   };
   auto of = [&](auto type) { small(q) ? run(type, (uint32_t)0) : run(type, (uint64_t)0); };
   if (x_dtype == GLQB_DT_F16) of(__half());
@@ -401,8 +413,8 @@ int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const float* t
 template <int FMT>
 int dequantize_launch(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, const Mx4Rows& q, void* out,
                       int out_dtype, cudaStream_t stream) {
-  if (small(q)) mx4_dequantize_kernel<FMT, uint32_t><<<grid_for(q), QT_THREADS, 0, stream>>>(codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
-  else mx4_dequantize_kernel<FMT, uint64_t><<<grid_for(q), QT_THREADS, 0, stream>>>(codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
+  auto* kernel = small(q) ? mx4_dequantize_kernel<FMT, uint32_t> : mx4_dequantize_kernel<FMT, uint64_t>;
+  launch_chained(true, kernel, (int)grid_for(q), QT_THREADS, 0, stream, codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
   return mx4_launched("mx4_dequantize");
 }
 
@@ -462,7 +474,7 @@ size_t glqb_mx4_image_bytes(int32_t format, int32_t experts, int32_t m, int32_t 
 int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t experts, int32_t m, int32_t n, void* image,
                   void* stream_) {
   if (!format_ok(format)) return mx4_fail(GLQB_E_INVALID, "mx4_pack: format %d", format);
-  if (experts < 1 || m < 1 || n < 1) return mx4_fail(GLQB_E_INVALID, "mx4_pack: %d x %d x %d", experts, m, n);
+  if (experts < 1 || m < 1 || n < 1 || m > MX4_MAX_SIZE || n > MX4_MAX_SIZE) return mx4_fail(GLQB_E_INVALID, "mx4_pack: %d x %d x %d", experts, m, n);
   if (!codes || !scales || !image) return mx4_fail(GLQB_E_INVALID, "mx4_pack: null argument");
   if (reinterpret_cast<uintptr_t>(image) % 128) return mx4_fail(GLQB_E_INVALID, "mx4_pack: the image must be 128-byte aligned");
   const int mt = (m + MX4_ROWS - 1) / MX4_ROWS, kt = (n + MX4_K - 1) / MX4_K;
@@ -540,7 +552,7 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
 }
 
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize) {
-  if (!w || !format_ok(w->format) || rows <= 0 || rows >= (1ll << 31) || w->experts < 1 || w->m < 1 || w->n < 1) return 0;
+  if (!w || !format_ok(w->format) || rows <= 0 || rows > MX4_MAX_ROWS || w->experts < 1 || w->m < 1 || w->n < 1) return 0;
   return form_of(w, rows, x_stride, x, quantize, nullptr).bytes;      // (what a call needs does not depend on the device)
 }
 
@@ -551,11 +563,14 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   if (!w || !format_ok(w->format)) return mx4_fail(GLQB_E_INVALID, "mx4_product: format");
   if (w->experts < 1 || w->experts > MX4_MAX_EXPERTS || w->m < 1 || w->n < 1)
     return mx4_fail(GLQB_E_INVALID, "mx4_product: %d x %d x %d (at most %d experts)", w->experts, w->m, w->n, MX4_MAX_EXPERTS);
+  if (w->m > MX4_MAX_SIZE || w->n > MX4_MAX_SIZE) return mx4_fail(GLQB_E_INVALID, "mx4_product: %d x %d", w->m, w->n);
   if (!offsets && w->experts != 1) return mx4_fail(GLQB_E_INVALID, "mx4_product: %d experts need offsets", w->experts);
   if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return mx4_fail(GLQB_E_INVALID, "mx4_product: dtype");
   if (!quantize && x_dtype == GLQB_DT_F32) return mx4_fail(GLQB_E_INVALID, "mx4_product: fp32 activations are served quantised only");
-  if (rows < 0 || rows >= (1ll << 31)) return mx4_fail(GLQB_E_INVALID, "mx4_product: %lld rows", (long long)rows);
+  if (rows < 0 || rows > MX4_MAX_ROWS) return mx4_fail(GLQB_E_INVALID, "mx4_product: %lld rows", (long long)rows);
   if (rows == 0) return GLQB_OK;
+  if ((rows + w->experts) * ((w->m + MX4_ROWS - 1) / MX4_ROWS) >= 1ll << 30)       // (tiles are counted in 31 bits)
+    return mx4_fail(GLQB_E_INVALID, "mx4_product: %lld rows of %d results are too many for one call", (long long)rows, w->m);
   if (!w->image || !x || !y || (w->format == GLQB_MX4_NVFP4 && !w->tensor_scale)) return mx4_fail(GLQB_E_INVALID, "mx4_product: null argument");
   if (rows > 1 && (x_stride < w->n || y_stride < w->m)) return mx4_fail(GLQB_E_INVALID, "mx4_product: rows overlap");
   const Device* d = device();
@@ -594,7 +609,8 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.clear = offsets && clear_rest;
   if (!quantize) {
     if (f.align) {
-      mx4_align_kernel<<<(unsigned)std::min<long long>((rows * f.n_pad + 255) / 256, 148 * 32), 256, 0, stream>>>((const uint16_t*)x, x_stride, rows, w->n, f.n_pad, (uint16_t*)workspace);
+      launch_chained(true, mx4_align_kernel, (int)std::min<long long>((rows * f.n_pad + 255) / 256, 148 * 32), 256, 0, stream, (const uint16_t*)x, x_stride, rows, w->n,
+                     f.n_pad, (uint16_t*)workspace);
       J.x = workspace;
       J.x_stride = f.n_pad;
     }
@@ -623,9 +639,9 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   const int grid = (int)std::min<long long>((rows * ((batches + at_once - 1) / at_once) + 7) / 8, (long long)sms * 8);
   auto image = [&](auto fmt) {
     constexpr int FMT = decltype(fmt)::value;
-    if (x_dtype == GLQB_DT_F16) mx4_x_image_kernel<__half, FMT><<<grid, QT_THREADS, lists, stream>>>(J, x_scale, own, parts, f.x_scales, vec, at_once);
-    else if (x_dtype == GLQB_DT_BF16) mx4_x_image_kernel<__nv_bfloat16, FMT><<<grid, QT_THREADS, lists, stream>>>(J, x_scale, own, parts, f.x_scales, vec, at_once);
-    else mx4_x_image_kernel<float, FMT><<<grid, QT_THREADS, lists, stream>>>(J, x_scale, own, parts, f.x_scales, vec, at_once);
+    if (x_dtype == GLQB_DT_F16) launch_chained(true, mx4_x_image_kernel<__half, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, vec, at_once);
+    else if (x_dtype == GLQB_DT_BF16) launch_chained(true, mx4_x_image_kernel<__nv_bfloat16, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, vec, at_once);
+    else launch_chained(true, mx4_x_image_kernel<float, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, vec, at_once);
   };
   if (w->format == GLQB_MX4_MXFP4) image(std::integral_constant<int, GLQB_MX4_MXFP4>());
   else image(std::integral_constant<int, GLQB_MX4_NVFP4>());

@@ -276,7 +276,7 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Walk& t, flo
 // 125 (2048 tokens of 14336 x 4096 317 us; without the loads 202).  Two CTAs therefore share a tile of 256 weight rows (PAIR): each
 // brings half of the activations, the first one's thread issues for both.  What is to arrive at the issuing thread comes from
 // both CTAs; what it releases goes to both.
-constexpr int G16_THREADS = 768, G16_W_STAGES = 4, G16_PRODUCERS = 8;
+constexpr int G16_THREADS = 768, G16_W_STAGES = 3, G16_PRODUCERS = 8;
 
 struct Mx4Ring { int x_stages, box_rows, x_half, a_stages, acc_cols; };  // stages of x, rows per box, bytes of 64 values of a CTA's rows
 
@@ -362,10 +362,17 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     }
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
   } else if (warp == 2) {
-    if (lane == 0) {                               // (the weights do not depend on what runs in front of this call)
+    if (lane == 0) {
       Mx4Pos w;
+      auto weights = [&](const Mx4Walk& t) { return J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE; };
+      if (!J.offsets) {                            // on their way to L2 while the kernel in front ends (which may write them: none is read)
+        const Mx4Walk t(L, J.experts, first, step, tiles, m_tiles);
+        if (t.more())
+          for (int k = 0; k < min(G16_W_STAGES, k1 - k0); ++k) bulk_prefetch_l2(weights(t) + k * TILE, TILE);
+      }
+      pdl_wait();
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
-        const uint8_t* src = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
+        const uint8_t* src = weights(t);
         for (int k = k0; k < k1; ++k, ++loads_w, src += TILE, w.add(1, G16_W_STAGES)) {
           if (!mbar_wait(&B.empty_w[w.s], w.phase ^ 1u, &B.abort)) { ok = false; break; }
           mbar_expect_tx(&B.full_w[w.s], TILE);
@@ -375,6 +382,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
   } else if (warp >= 8) {
+    pdl_wait();
     // of a group's eight warps four take the first 64 values of a step, four the others; a warp the 32 rows of its quarter of tensor memory
     const int group = (warp - 8) >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t to = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + half * 32u;
@@ -527,7 +535,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   }
   if (warp == 0) alloc_all<PAIR>(&B.tmem);
   tc_fence_before();
-  pdl_wait();
+  if (J.offsets) pdl_wait();
   mx4_groups(J, L);
   if constexpr (PAIR) cluster_sync();
   tc_fence_after();
@@ -586,22 +594,34 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
     if (lane == 0) {
       const int x_stage = J.tn * 128 + x_scales;
       Mx4Pos x;
+      int early = 0;                               // stages whose weights went out before x was there (x's kernel began behind all that may write them)
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
         const uint32_t x_codes = (uint32_t)((t.rows + 15) & ~15) * (PAIR ? 64u : 128u);
         const uint8_t* wsrc = J.image + (((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * J.k_tiles + k0) * TILE;
         const uint8_t* xsrc = J.x_image + ((long long)t.tt * J.k_tiles + k0) * x_stage;
         for (int k = 0; k < steps; ++k, ++loads, x.add(1, stages), wsrc += TILE, xsrc += x_stage) {
           if (!mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort)) { ok = false; break; }
+          if (loads == 0) {
+            for (; early < min(stages, steps); ++early) {
+              mbar_expect_tx(&B.full_x[early], TILE + x_codes + x_scales);
+              bulk_g2s(base + early * stage_bytes, wsrc + (long long)early * TILE, TILE, &B.full_x[early]);
+            }
+            pdl_wait();
+          }
           uint8_t* w = base + x.s * stage_bytes;
-          mbar_expect_tx(&B.full_x[x.s], TILE + x_codes + x_scales);
-          bulk_g2s(w, wsrc, TILE, &B.full_x[x.s]);
+          if (loads >= early) {
+            mbar_expect_tx(&B.full_x[x.s], TILE + x_codes + x_scales);
+            bulk_g2s(w, wsrc, TILE, &B.full_x[x.s]);
+          }
           bulk_g2s(w + TILE, xsrc + (PAIR ? rank * x_codes : 0u), x_codes, &B.full_x[x.s]);
           bulk_g2s(w + TILE + (own + 7) / 8 * 1024, xsrc + J.tn * 128, x_scales, &B.full_x[x.s]);
         }
       }
+      loads = max(loads, (uint32_t)early);
       if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
   } else if (warp >= 4) {
+    pdl_wait();                                    // (y may still be in use)
     mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
     Mx4Pos acc;
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {

@@ -16,10 +16,10 @@ struct Mx4Job {
   const float* x_scale;       // 4-bit activations, NVFP4: theirs
   const void* offsets;        // null: one matrix, all rows
   int wide, experts, rows, m, n, m_tiles, k_tiles;
-  int tn;                     // most rows of x per token tile, a multiple of 16
+  int tn;                     // most rows of x per token tile: a multiple of 16, or 8
   int max_tiles;              // bound of the token tiles
   int split;                  // CTAs of a cluster that share a tile's sum
-  int pair;                   // two CTAs share a tile of 256 weight rows (16-bit activations, split 1)
+  int pair;                   // two CTAs share a tile of 256 weight rows (split 1)
   void* y;
   long long y_stride;
   int y_dtype, accumulate;
@@ -272,11 +272,11 @@ __device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert,
 }
 #endif  // __CUDACC__
 
-// Chained to the kernel in front (launch_chained), `cluster` CTAs per cluster.
 inline int mx4_device() {       // the current one, 0..63
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
 }
+// Chained to the kernel in front (launch_chained), `cluster` CTAs per cluster.
 template <auto K, typename... P, typename... A>
 inline cudaError_t mx4_launch(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
   static std::atomic<int> limit[64];     // per device: the shared memory the kernel may have (raised, never lowered)

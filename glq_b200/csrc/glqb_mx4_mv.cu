@@ -109,8 +109,14 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
   if (J.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   if (warp == MV4_WARPS) {
-    if (lane == 0) {                                     // (the weights do not depend on what runs in front of this call)
+    if (lane == 0) {
       Mx4Pos p;
+      if (!J.offsets) {                                  // on their way to L2 while the kernel in front ends (which may write them: none is read)
+        const Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles);
+        if (t.more())
+          for (int k = k0; k < min(k0 + STAGES, k1); ++k) bulk_prefetch_l2(J.image + (((long long)t.expert * J.m_tiles + t.mt) * J.k_tiles + k) * TILE, TILE);
+      }
+      pdl_wait();
       for (Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles); t.more() && ok; t.next(L)) {
         const long long at = (long long)t.expert * J.m_tiles + t.mt;
         const uint8_t* src = J.image + (at * J.k_tiles + k0) * TILE;
@@ -124,7 +130,6 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
       }
       if (!ok) { *abort_flag = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
     }
-    pdl_wait();                                          // (a grid ends behind the one in front of it)
   } else if (warp > MV4_WARPS) {
     // four rows of x each: those of the next tile are on their way while the last ones are written
     pdl_wait();
@@ -194,7 +199,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
       int top[2] = {0, 0};
       bool plain = true;                                 // rows that the short form of the multiplier covers
       Mx4Factor f{1.0f, 1.0f};
-      if constexpr (FMT == GLQB_MX4_NVFP4) f.b = __ldg(J.w_scale + tile.expert);
+      if constexpr (FMT == GLQB_MX4_NVFP4) f.b = J.w_scale[tile.expert];
       float acc[NB][4] = {};
       for (int k = k0; k < k1; ++k, p.add(1, STAGES)) {
         if (!ok || !mbar_wait(&full[p.s], p.phase, abort_flag)) { ok = false; *abort_flag = 1; continue; }

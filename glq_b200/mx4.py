@@ -35,16 +35,19 @@ class Mx4Tensor(NamedTuple):
 
 
 class Mx4Weight:
-    """Weights laid out for the products (``mx4_pack``): (out_features, in_features), or one such matrix per expert."""
+    """Weights laid out for the products (``mx4_pack``): (out_features, in_features), or one such matrix per expert.  The
+    attributes cannot be set (a new image, or one on another device, is a new weight)."""
     __slots__ = ("image", "tensor_scale", "format", "experts", "out_features", "in_features", "_desc", "_ref", "_index")
 
     def __init__(self, image, tensor_scale, format, experts, out_features, in_features):
-        self.image, self.tensor_scale, self.format, self.experts = image, tensor_scale, format, experts
-        self.out_features, self.in_features = out_features, in_features
-        self._desc = _lib.Mx4WeightDesc(image.data_ptr(), tensor_scale.data_ptr() if tensor_scale is not None else 0,
-                                        _FORMATS[format], experts or 1, out_features, in_features)
-        self._ref = C.byref(self._desc)
-        self._index = image.get_device()
+        desc = _lib.Mx4WeightDesc(image.data_ptr(), tensor_scale.data_ptr() if tensor_scale is not None else 0,
+                                  _FORMATS[format], experts or 1, out_features, in_features)
+        values = (image, tensor_scale, format, experts, out_features, in_features, desc, C.byref(desc), image.get_device())
+        for name, value in zip(self.__slots__, values):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"glq_b200: {name} of a packed weight cannot be set")
 
 
 _get_device, _set_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_setDevice, torch._C._cuda_getCurrentRawStream
@@ -186,7 +189,7 @@ def mx4_pack(q: Mx4Tensor) -> Mx4Weight:
     _call(codes.get_device(), "mx4_pack", lib.glqb_mx4_pack, codes.data_ptr(), sc.data_ptr(), fmt, experts or 1, m, n, image.data_ptr())
     t = q.tensor_scale
     if scales:
-        t = t.reshape(1).expand(experts or 1).contiguous() if scales == 1 else t.reshape(-1)
+        t = t.reshape(-1).expand(experts or 1).clone(memory_format=torch.contiguous_format)
     return Mx4Weight(image, t, q.format, experts, m, n)
 
 
@@ -233,7 +236,7 @@ def _product(x, dt, w, offsets, quantize_input, xs, y, y_dt, y_stride, accumulat
 
 
 def mx4_linear(x, weight: Mx4Weight, *, quantize_input=False, input_scale=None, out_dtype=None, accumulate_into=None):
-    """x (..., n) times a packed (m, n) weight: (..., m), sums in fp32 and one rounding.  x is bf16 or fp16 and is taken as it is; with
+    """x (..., n) times a packed (m, n) weight: (..., m), sums in fp32 and one rounding.  x is bf16 or fp16; with
     ``quantize_input`` (then fp32 too) it is brought to the weight's format first, as ``mx4_quantize`` does ("nvfp4": by
     ``input_scale``, one fp32 value, or by the scale of the whole of x), and the tensor cores multiply 4-bit values, at four times
     their 16-bit rate.  ``accumulate_into`` adds the result to that dense (..., m) tensor in place (residual add, before the

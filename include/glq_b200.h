@@ -302,7 +302,7 @@ size_t glqb_noalloc_scratch_bytes(void);
  */
 #define GLQB_MX4_MXFP4 0
 #define GLQB_MX4_NVFP4 1
-#define GLQB_MX4_SCALE_FLOATS 257     /* a tensor's scale, and what it is found with */
+#define GLQB_MX4_SCALE_FLOATS 297     /* a tensor's scale, and what it is found with */
 
 /* rows x cols values (x_stride elements apart) to stored rows, each rounded to nearest even from the real quotient by its
  * block's scale: MXFP4 2^(floor(log2 amax) - 2), saturating at 6; NVFP4 e4m3(amax / (6 t)), t = *tensor_scale (positive), or,
@@ -331,8 +331,8 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
  * keep what y holds, or are zeroed with clear_rest.  At most 1024 experts.
  * quantize: x is brought to the weights' format first, as glqb_mx4_quantize does (NVFP4: by *x_scale, or, with x_scale NULL, by the
  * scale of rows offsets[0] .. offsets[experts] - 1), and 4-bit values are multiplied.  Without it x is fp16 or bf16 and stays so.
- * MXFP4 weights are held relative to the largest scale of their row: under fp16 activations a block more than 2^24 below it
- * loses bits, 2^132 under bf16.
+ * Under 16-bit activations MXFP4 weights are multiplied relative to the largest scale of their row: a block whose scale lies more
+ * than 2^36 below it loses bits.  m and n up to 2^30, rows up to 2^31 - 2^16.
  * accumulate: y <- y + result, added before the rounding.  A bounded wait that gives up sets the device's status word. */
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize);
 int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows,
