@@ -179,3 +179,89 @@ class GLQLinear(nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
                 f"m_pad={self.m_pad}, n_pad={self.n_pad}, trellis={self._is_trellis}")
+
+
+class Mx4Linear(nn.Module):
+    """A linear layer whose weight is held in microscaled 4-bit floating point ("mxfp4" or "nvfp4"), as checkpoints store it:
+    ``codes`` (out, ceil(in / 2)) and ``scales`` (out, ceil(in / block)) uint8, for "nvfp4" ``tensor_scale`` (fp32, one), ``bias``.
+    They are laid out for the products (``weight``) at the first forward, and again after they were loaded, moved or written.
+    ``quantize_input``: activations are brought to the format as well and 4-bit values are multiplied.  No counterpart in the
+    reference.  There is no CPU path: on a CPU tensor ``forward`` raises."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, format: str = "mxfp4",
+                 quantize_input: bool = False):
+        super().__init__()
+        if format not in ("mxfp4", "nvfp4"):
+            raise ValueError(f'format is "mxfp4" or "nvfp4", not {format!r}')
+        self.in_features, self.out_features, self.format, self.quantize_input = in_features, out_features, format, quantize_input
+        block = 32 if format == "mxfp4" else 16
+        self.register_buffer("codes", torch.zeros(out_features, (in_features + 1) // 2, dtype=torch.uint8))
+        self.register_buffer("scales", torch.zeros(out_features, -(-in_features // block), dtype=torch.uint8))
+        if format == "nvfp4":
+            self.register_buffer("tensor_scale", torch.ones(1, dtype=torch.float32))
+        else:
+            self.tensor_scale = None
+        if bias:
+            self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32))
+        else:
+            self.bias = None
+        self._packed = None           # (what the stored rows were when they were packed, the packed weight)
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias=None, format: str = "mxfp4", quantize_input: bool = False) -> "Mx4Linear":
+        """The layer of a dense (out, in) weight on a GPU, quantised here."""
+        m, n = weight.shape
+        layer = cls(n, m, bias is not None, format, quantize_input)
+        q = ops.mx4_quantize(weight.detach(), format)
+        layer.codes, layer.scales = q.codes, q.scales
+        if format == "nvfp4":
+            layer.tensor_scale = q.tensor_scale.clone()
+        if bias is not None:
+            layer.bias = bias.detach().float()
+        return layer
+
+    def _apply(self, fn, *args, **kwargs):
+        # (half() and bfloat16() are for activations: the tensor's scale and the bias stay fp32)
+        kept = {name: t for name in ("tensor_scale", "bias") if (t := getattr(self, name)) is not None}
+        super()._apply(fn, *args, **kwargs)
+        for name, t in kept.items():
+            now = getattr(self, name)
+            if now.dtype != torch.float32:
+                setattr(self, name, t.to(now.device))
+        self._packed = None
+        return self
+
+    def __getstate__(self):
+        return {**self.__dict__, "_packed": None}
+
+    def _rows(self) -> "ops.Mx4Tensor":
+        return ops.Mx4Tensor(self.codes, self.scales, self.format, self.in_features, self.tensor_scale)
+
+    @property
+    def weight(self) -> "ops.Mx4Weight":
+        """The packed weight (``ops.mx4_pack``).  Buffers created under inference mode do not count their changes: after writing to
+        one in place, call ``repack``."""
+        held = [t for t in (self.codes, self.scales, self.tensor_scale) if t is not None]
+        now = [0 if t.is_inference() else t._version for t in held]
+        if self._packed is None or self._packed[0] != now or any(a is not b for a, b in zip(self._packed[1], held)):
+            if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("glq_b200: the weight is packed at the first forward: run one before capturing a graph")
+            self._packed = (now, held, ops.mx4_pack(self._rows()))
+        return self._packed[2]
+
+    def repack(self) -> None:
+        self._packed = None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not x.is_cuda:
+            raise RuntimeError("glq_b200.Mx4Linear has no CPU path")
+        y = ops.mx4_linear(x, self.weight, quantize_input=self.quantize_input)
+        return y if self.bias is None else y + self.bias.to(y.dtype)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """Dense (out_features, in_features) weight."""
+        return ops.mx4_dequantize(self._rows(), dtype)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"format={self.format}, quantize_input={self.quantize_input}")

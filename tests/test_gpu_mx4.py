@@ -448,6 +448,177 @@ def test_experts_layer_of_a_decoder(fmt):
     ops.check_device_status()
 
 
+# ---- forms that only larger calls take ---------------------------------------------------------------------------
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tokens,m,n", [(1500, 1024, 384), (1921, 1100, 640), (2048, 1153, 96), (3000, 900, 264)])
+def test_linear_of_many_tokens(fmt, dtype, quantize, tokens, m, n):
+    """Two CTAs to a tile of 256 weight rows, also an odd number of them, with values that end inside a step."""
+    g = np.random.default_rng(tokens + m + n)
+    weight, w = make_weight(g, (m, n), fmt)
+    x = to_cuda(g.standard_normal((tokens, n)), DT[dtype])
+    y = ops.mx4_linear(x, weight, quantize_input=quantize)
+    xv = quantized_values(host(x), fmt) if quantize else host(x)
+    check_product(y, xv, w, DT[dtype])
+    assert torch.equal(y, ops.mx4_linear(x, weight, quantize_input=quantize))
+    add = torch.zeros_like(y)
+    ops.mx4_linear(x, weight, quantize_input=quantize, accumulate_into=add)
+    assert torch.equal(add, y)
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("experts,per,m,n", [(100, 20, 300, 160), (40, 90, 270, 96), (12, 300, 1100, 128), (1024, 1, 130, 64), (1024, 11, 16, 40)])
+def test_grouped_many_experts(fmt, quantize, experts, per, m, n):
+    """More tiles than CTAs, by one CTA each and by two, with counts from none to four times the average."""
+    g = np.random.default_rng(experts)
+    weight, w = make_weight(g, (experts, m, n), fmt)
+    counts = g.multinomial(experts * per, g.dirichlet(np.full(experts, 1.5)))
+    counts[[0, 5]] = 0
+    x = to_cuda(g.standard_normal((int(counts.sum()), n)), torch.bfloat16)
+    off = counts_to_offsets(counts)
+    y = ops.mx4_grouped_linear(x, weight, off, quantize_input=quantize)
+    xv = quantized_values(host(x), fmt) if quantize else host(x)
+    at = off.tolist()
+    for e in range(experts):
+        if counts[e]:
+            check_product(y[at[e]:at[e + 1]], xv[at[e]:at[e + 1]], w[e], torch.bfloat16)
+    assert torch.equal(y, ops.mx4_grouped_linear(x, weight, off, quantize_input=quantize))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens", [1, 7, 16, 40, 250])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_activations_of_any_size(fmt, tokens, dtype):
+    """Rows of x between 2^-100 and 2^100 (fp16: 2^-14 and 2^12), mixed magnitudes in a row, infinities and NaN, which stay in their rows."""
+    g = np.random.default_rng(tokens)
+    m, n = 200, 600
+    weight, w = make_weight(g, (m, n), fmt, spread=0.1)
+    span = np.linspace(-100, 100, tokens) if dtype == "bf16" else np.linspace(-14, 8, tokens)
+    x = g.standard_normal((tokens, n)) * 2.0 ** span[:, None] * 2.0 ** g.integers(-12, 1, (tokens, n))
+    bad = sorted({0, tokens // 2, tokens - 1}) if tokens > 1 else []
+    for r, value in zip(bad, (np.inf, -np.inf, np.nan)):
+        x[r, 300 + r % 200] = value
+    if tokens > 6:
+        x[3] = 0.0
+    xd = to_cuda(x, DT[dtype])
+    xv = host(xd)
+    y = host(ops.mx4_linear(xd, weight, out_dtype=torch.float32))
+    clean = np.setdiff1d(np.arange(tokens), bad)
+    want = xv[clean] @ w.T
+    # bf16 values may be multiplied as fp16 under a power of two per 256 of them: off by 2^-40 of the largest
+    low = 2.0 ** -40 * n * np.abs(xv[clean]).max(1, keepdims=True, initial=0) * np.abs(w).max(1)
+    assert np.all(np.abs(y[clean] - want) <= tolerance(xv[clean], w, want, torch.float32) + low)
+    for r in bad:
+        with np.errstate(invalid="ignore"):
+            terms = xv[r] * w
+            want_bad = terms.sum(1)
+        assert np.array_equal(np.isnan(y[r]), np.isnan(want_bad)) and np.array_equal(np.isposinf(y[r]), np.isposinf(want_bad))
+
+
+def test_stored_rows_that_start_anywhere():
+    """Codes and scales in views that begin on odd addresses."""
+    g = np.random.default_rng(4)
+    for fmt in FORMATS:
+        q = ops.mx4_quantize(to_cuda(g.standard_normal((37, 203))), fmt)
+        for shift in (1, 2, 5):
+            codes, scales = (torch.zeros(t.numel() + shift, dtype=torch.uint8, device="cuda")[shift:].view(t.shape).copy_(t) for t in (q.codes, q.scales))
+            moved = q._replace(codes=codes, scales=scales)
+            assert torch.equal(ops.mx4_dequantize(moved), ops.mx4_dequantize(q))
+            assert torch.equal(ops.mx4_pack(moved).image, ops.mx4_pack(q).image)
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("tokens", [1, 60])
+def test_weights_packed_right_in_front_of_the_product(quantize, tokens):
+    """Weights written by the launch in front of a product are the ones it multiplies, eager and in a graph."""
+    g = np.random.default_rng(6)
+    m, n = 1024, 2048
+    dense = [to_cuda(g.standard_normal((m, n)), torch.bfloat16) for _ in range(3)]
+    x = to_cuda(g.standard_normal((tokens, n)), torch.bfloat16)
+    want = []
+    for d in dense:
+        w = ops.mx4_pack(ops.mx4_quantize(d))
+        torch.cuda.synchronize()
+        want.append(ops.mx4_linear(x, w, quantize_input=quantize))
+    images = [ops.mx4_pack(ops.mx4_quantize(d)).image for d in dense]
+    assert not torch.equal(want[0], want[1])
+    source = dense[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.mx4_linear(x, ops.mx4_pack(ops.mx4_quantize(source)), quantize_input=quantize)
+    w = ops.mx4_pack(ops.mx4_quantize(dense[0]))
+    for _ in range(5):
+        for d, image, right in zip(dense, images, want):
+            assert torch.equal(ops.mx4_linear(x, ops.mx4_pack(ops.mx4_quantize(d)), quantize_input=quantize), right)
+            w.image.copy_(image)
+            assert torch.equal(ops.mx4_linear(x, w, quantize_input=quantize), right)
+            source.copy_(d)
+            graph.replay()
+            assert torch.equal(y, right)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values in x and in the result."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    g = np.random.default_rng(1)
+    rows, cols = 135000, 16384
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    tail = to_cuda(g.standard_normal((70, cols)), torch.bfloat16)
+    x[-70:] = tail
+    for fmt in FORMATS:
+        q, alone = ops.mx4_quantize(x, fmt), ops.mx4_quantize(tail, fmt)
+        assert torch.equal(q.codes[-70:], alone.codes) and torch.equal(q.scales[-70:], alone.scales)
+        assert torch.equal(ops.mx4_dequantize(q)[-70:], ops.mx4_dequantize(alone))
+        assert not q.codes[:-70].any()
+        del q
+    weight, w = make_weight(g, (128, cols), "mxfp4")
+    for quantize in (False, True):
+        y = ops.mx4_linear(x, weight, quantize_input=quantize)
+        check_product(y[-70:], quantized_values(host(tail), "mxfp4") if quantize else host(tail), w, torch.bfloat16)
+        assert not y[:-70].any()
+    del x, y
+    torch.cuda.empty_cache()
+    weight, w = make_weight(g, (cols, 64), "nvfp4")
+    x = torch.zeros(rows, 64, dtype=torch.bfloat16, device="cuda")
+    x[-70:] = tail[:, :64]
+    for quantize in (False, True):
+        y = ops.mx4_linear(x, weight, quantize_input=quantize)
+        check_product(y[-70:], quantized_values(host(tail[:, :64]), "nvfp4") if quantize else host(tail[:, :64]), w, torch.bfloat16)
+        assert not y[:-70].any()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_layer_of_4_bit_weights(fmt):
+    import copy
+    from glq_b200.linear import Mx4Linear
+    g = np.random.default_rng(12)
+    dense, bias = to_cuda(g.standard_normal((96, 160)) / 12), to_cuda(g.standard_normal(96))
+    layer = Mx4Linear.from_weight(dense, bias, fmt)
+    x = to_cuda(g.standard_normal((3, 5, 160)), torch.bfloat16)
+    y = layer(x)
+    assert y.shape == (3, 5, 96)
+    direct = ops.mx4_linear(x, ops.mx4_pack(ops.mx4_quantize(dense, fmt)))
+    assert torch.equal(y, direct + bias.to(torch.bfloat16))
+    assert torch.equal(layer.dequantize(), ops.mx4_dequantize(ops.mx4_quantize(dense, fmt), torch.float32))
+    assert layer.weight is layer.weight and not layer.codes.is_cpu
+    # another layer loads it, after it has run with what it held before
+    other = Mx4Linear(160, 96, bias=True, format=fmt).cuda()
+    assert torch.equal(other(x), torch.zeros_like(y))
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other(x), y)
+    other.codes[:48].zero_()
+    assert torch.equal(other(x)[..., :48], torch.zeros_like(y[..., :48]) + bias[:48].to(torch.bfloat16))
+    twin = copy.deepcopy(layer)
+    assert torch.equal(twin(x), y) and twin.weight is not layer.weight
+    twin.quantize_input = True
+    assert torch.equal(twin(x.float()), ops.mx4_linear(x.float(), layer.weight, quantize_input=True) + bias)
+    twin.half()
+    assert twin.bias.dtype == torch.float32 and torch.equal(layer(x), y)
+
+
 # ---- refusals ----------------------------------------------------------------------------------------------------
 def test_refusals():
     g = np.random.default_rng(0)
@@ -491,3 +662,9 @@ def test_refusals():
     refuse("empty", lambda: ops.mx4_pack(ops.mx4_quantize(x[:0])))
     assert ops.mx4_linear(x[:0], weight).shape == (0, 64)
     assert ops.mx4_grouped_linear(x[:0], experts, off * 0).shape == (0, 64)
+    with pytest.raises(AttributeError, match="cannot be set"):
+        weight.image = weight.image.clone()
+    scale = torch.tensor([0.5], device="cuda")
+    own = ops.mx4_pack(ops.mx4_quantize(x, "nvfp4", scale))
+    scale.fill_(2.0)
+    assert own.tensor_scale.item() == 0.5

@@ -111,3 +111,38 @@ def test_operators_refuse_host_tensors_and_wrong_arguments():
         ops.mx4_linear(x, q)
     with pytest.raises(ValueError, match="mx4_pack"):
         ops.mx4_grouped_linear(x, q, torch.zeros(3, dtype=torch.int32))
+
+
+def test_sizes_beyond_what_is_counted_are_refused(lib):
+    from glq_b200 import _lib
+    p, big = 4096, (1 << 30) + 1
+
+    def product(w, rows, offsets=None, stride=1 << 40):
+        return lib.glqb_mx4_product(ctypes.byref(w), p, 1, stride, rows, offsets, 0, 0, None, p, 1, stride, 0, 0, None, 0, None), lib.glqb_last_error().decode()
+
+    for w, rows, offsets, text in ((_lib.Mx4WeightDesc(p, None, 0, 1025, 64, 64), 2, p, "at most 1024"),
+                                   (_lib.Mx4WeightDesc(p, None, 0, 1, big, 64), 2, None, str(big)),
+                                   (_lib.Mx4WeightDesc(p, None, 0, 1, 64, big), 2, None, str(big)),
+                                   (_lib.Mx4WeightDesc(p, None, 0, 1, 64, 64), 0x7FFF0001, None, "rows"),
+                                   (_lib.Mx4WeightDesc(p, None, 0, 1, 1 << 20, 64), 1 << 18, None, "too many")):
+        rc, said = product(w, rows, offsets)
+        assert rc == -1 and text in said, said
+    for m, n in ((big, 1), (1, big)):
+        assert lib.glqb_mx4_pack(p, p, 0, 1, m, n, p, None) == -1
+
+
+def test_layer_of_4_bit_weights_on_the_host():
+    from glq_b200.linear import Mx4Linear
+    layer = Mx4Linear(50, 33, bias=True, format="nvfp4")
+    shapes = {k: (tuple(v.shape), v.dtype) for k, v in layer.state_dict().items()}
+    assert shapes == {"codes": ((33, 25), torch.uint8), "scales": ((33, 4), torch.uint8), "tensor_scale": ((1,), torch.float32),
+                      "bias": ((33,), torch.float32)}
+    layer.half()
+    assert layer.tensor_scale.dtype == layer.bias.dtype == torch.float32 and layer.codes.dtype == torch.uint8
+    layer.load_state_dict({**layer.state_dict(), "tensor_scale": torch.full((1,), 0.25)})
+    assert layer.tensor_scale.item() == 0.25
+    assert set(Mx4Linear(64, 8).state_dict()) == {"codes", "scales"}
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        layer(torch.zeros(1, 50))
+    with pytest.raises(ValueError, match="mxfp4"):
+        Mx4Linear(8, 8, format="fp4")
