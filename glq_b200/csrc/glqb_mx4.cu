@@ -33,8 +33,11 @@ __device__ int g_mx4_status;   // 0, or what gave up (ST_GAVE_UP_*): products ha
 struct Mx4Rows {
   long long rows, stride;     // elements between rows
   long long cols;
-  long long chunks;           // eights of values per row, whole blocks
-  bool vec;                   // rows start on 16 bytes
+  long long chunks;           // sixteens of values per row, whole blocks
+  long long full;             // those that have all sixteen
+  uint32_t magic;             // i / chunks = i * magic / 2^(32 + shift) for i < 2^31 (see rows_of)
+  int rest, shift;            // values behind the full ones
+  int vec;                    // rows start on 32 bytes (2), on 16 (1), or anywhere (0)
 };
 
 // Rows offsets[0] .. offsets[experts] - 1, held to those there are.
@@ -52,14 +55,19 @@ struct Mx4Range {
   }
 };
 
-// Eights of values that a thread takes at once, their loads in front of everything else.  I: the type of an eight's index (64-bit
-// divisions only where there are more than 2^31).
-constexpr int QT_BATCH = 4;
+// Sixteens of values that a thread takes at once, their loads in front of everything else.  I: the type of a sixteenth's index (64-bit
+// divisions only where there are more than 2^31).  What bounds these kernels next to HBM is the instructions around the values
+// (by eights 112 per warp and eight for MXFP4, half of them addresses and scales): sixteens share them out further.
+constexpr int QT_BATCH = 2;
 template <typename I>
 __device__ __forceinline__ void place(const Mx4Rows& q, I i, I& row, I& c) {
-  row = q.rows == 1 ? (I)0 : i / (I)q.chunks;
+  if constexpr (sizeof(I) == 4) row = q.chunks == 1 ? i : __umulhi(i, q.magic) >> q.shift;
+  else row = q.rows == 1 ? (I)0 : i / (I)q.chunks;
   c = i - row * (I)q.chunks;
 }
+// values of a row from its sixteen c on, at most sixteen
+template <typename I>
+__device__ __forceinline__ int values_at(const Mx4Rows& q, I c) { return c < (I)q.full ? 16 : c == (I)q.full ? q.rest : 0; }
 
 // ---- largest finite magnitude ---------------------------------------------------------------------
 // A part per CTA; those who need the whole reduce the parts (no atomics, nothing to clear beforehand).
@@ -80,17 +88,20 @@ __global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* x, Mx4R
       const I i = b + j * step;
       I row, c;
       place(q, i, row, c);
-      const long long left = i < end ? q.cols - (long long)c * 8 : 0;
-      raw[j].load(x + (long long)row * q.stride + (long long)c * 8, 0, (int)max(0ll, min(left, 8ll)), q.vec);
+      raw[j].load(x + (long long)row * q.stride + (long long)c * 16, i < end ? values_at(q, c) : 0, q.vec);
     }
 #pragma unroll
     for (int j = 0; j < QT_BATCH; ++j) {
-      float v[8];
-      raw[j].get(v);
+      const uint32_t all = raw[j].top();
+      if (all < 0x7F800000u) top = max(top, all);
+      else {                                                        // the finite ones among them
+        float v[16];
+        raw[j].get(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t w = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-        top = w < 0x7F800000u ? max(top, w) : top;
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t w = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+          top = w < 0x7F800000u ? max(top, w) : top;
+        }
       }
     }
   }
@@ -124,50 +135,60 @@ __device__ __forceinline__ float whole_scale(const float* given, float* own_scal
 template <typename T, int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
 mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own_scale, int parts, uint8_t* codes,
-                    uint8_t* scales) {
-  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
+                    uint8_t* scales, int unit) {
+  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 16;
   pdl_wait();
   pdl_trigger();
-  float t = 1.0f;
-  if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(tensor_scale, own_scale, parts);
   const long long code_row = (q.cols + 1) / 2, scale_row = q.chunks / PER;
   const I total = (I)(q.rows * q.chunks);
   Mx4Raw<T> raw[QT_BATCH];
   I row[QT_BATCH], c[QT_BATCH];
-  int left[QT_BATCH];                                                // values from the eight's first on, at most eight; -8 and less: no eight
+  int left[QT_BATCH];                                                // -1: behind the last row
 #pragma unroll
   for (int j = 0; j < QT_BATCH; ++j) {
     const I i = (I)blockIdx.x * (QT_THREADS * QT_BATCH) + j * QT_THREADS + threadIdx.x;
     place(q, i, row[j], c[j]);
-    left[j] = i < total ? (int)max(-7ll, min(8ll, q.cols - (long long)c[j] * 8)) : -8;
-    raw[j].load(x + (long long)row[j] * q.stride + (long long)c[j] * 8, 0, max(0, left[j]), q.vec);
+    left[j] = i < total ? values_at(q, c[j]) : -1;
+    raw[j].load(x + (long long)row[j] * q.stride + (long long)c[j] * 16, left[j], q.vec);
   }
+  float t = 1.0f;
+  if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(tensor_scale, own_scale, parts);       // (while the values are on their way)
 #pragma unroll
   for (int j = 0; j < QT_BATCH; ++j) {
     uint32_t s;
-    float v[8];
+    float v[16];
     raw[j].get(v);
-    const uint32_t word = mx4_quantize8<FMT, false>(v, t, s);     // (all lanes: the threads of a block exchange their largest value)
-    if (left[j] <= -8) continue;
-    uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 4;
-    const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(p);
-    if (left[j] >= 8 && (at & 3u) == 0) *reinterpret_cast<uint32_t*>(p) = word;
-    else if (left[j] >= 8 && (at & 1u) == 0) {
-      reinterpret_cast<uint16_t*>(p)[0] = (uint16_t)word;
-      reinterpret_cast<uint16_t*>(p)[1] = (uint16_t)(word >> 16);
+    const uint2 word = mx4_quantize16<FMT, false>(v, raw[j].top(), t, s);     // (all lanes: the threads of a block exchange their largest value)
+    if (left[j] < 0) continue;
+    uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 8;
+    if (left[j] == 16 && unit == 8) *reinterpret_cast<uint2*>(p) = word;
+    else if (left[j] == 16 && unit == 4) {
+      reinterpret_cast<uint32_t*>(p)[0] = word.x;
+      reinterpret_cast<uint32_t*>(p)[1] = word.y;
+    } else if (left[j] == 16 && unit == 2) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) reinterpret_cast<uint16_t*>(p)[b] = (uint16_t)((b < 2 ? word.x : word.y) >> (16 * (b & 1)));
     } else {
-      for (int b = 0; b < 4; ++b)
-        if (2 * b < left[j]) p[b] = (uint8_t)(word >> (8 * b));
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        if (2 * b < left[j]) p[b] = (uint8_t)((b < 4 ? word.x : word.y) >> (8 * (b & 3)));
     }
     if (c[j] % PER == 0) scales[(long long)row[j] * scale_row + (long long)(c[j] / PER)] = (uint8_t)s;
   }
 }
 
+__device__ __forceinline__ void put32(void* p, const uint4& a, const uint4& b, int vec) {
+  if (vec == 2) mx4_store32(p, a, b);
+  else {
+    reinterpret_cast<uint4*>(p)[0] = a;
+    reinterpret_cast<uint4*>(p)[1] = b;
+  }
+}
 template <int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
 mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, Mx4Rows q, void* out,
-                      int out_dtype) {
-  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
+                      int out_dtype, int unit) {
+  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 16;
   pdl_wait();
   pdl_trigger();
   const long long code_row = (q.cols + 1) / 2, scale_row = q.chunks / PER;
@@ -175,23 +196,31 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
   const bool one_scale = FMT != GLQB_MX4_NVFP4 || rows_per_scale >= q.rows;
   float t0 = 1.0f;
   if (FMT == GLQB_MX4_NVFP4 && one_scale) t0 = *tensor_scale;
-  uint32_t word[QT_BATCH], byte[QT_BATCH];
+  uint32_t part[QT_BATCH][4], byte[QT_BATCH];                        // (parts of codes as they are loaded: nothing waits for them here)
   I row[QT_BATCH], c[QT_BATCH];
   int left[QT_BATCH];
 #pragma unroll
   for (int j = 0; j < QT_BATCH; ++j) {
     const I i = (I)blockIdx.x * (QT_THREADS * QT_BATCH) + j * QT_THREADS + threadIdx.x;
     place(q, i, row[j], c[j]);
-    left[j] = i < total ? (int)max(0ll, min(8ll, q.cols - (long long)c[j] * 8)) : 0;
-    word[j] = byte[j] = 0;
+    left[j] = i < total ? values_at(q, c[j]) : 0;
+    byte[j] = part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0;
     if (left[j] <= 0) continue;
-    const uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 4;
-    const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(p);
-    if (left[j] >= 8 && (at & 3u) == 0) word[j] = *reinterpret_cast<const uint32_t*>(p);
-    else if (left[j] >= 8 && (at & 1u) == 0) word[j] = reinterpret_cast<const uint16_t*>(p)[0] | (uint32_t)reinterpret_cast<const uint16_t*>(p)[1] << 16;
-    else {
-      for (int b = 0; b < 4; ++b)
-        if (2 * b < left[j]) word[j] |= (uint32_t)p[b] << (8 * b);
+    const uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 8;
+    if (left[j] == 16 && unit == 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      part[j][0] = w.x;
+      part[j][2] = w.y;
+    } else if (left[j] == 16 && unit == 4) {
+      part[j][0] = reinterpret_cast<const uint32_t*>(p)[0];
+      part[j][2] = reinterpret_cast<const uint32_t*>(p)[1];
+    } else if (left[j] == 16 && unit == 2) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) part[j][b] = reinterpret_cast<const uint16_t*>(p)[b];
+    } else {
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        if (2 * b < left[j]) part[j][b >> 1] |= (uint32_t)p[b] << (8 * (b & 1));
     }
     byte[j] = scales[(long long)row[j] * scale_row + (long long)(c[j] / PER)];
   }
@@ -200,24 +229,34 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
     if (left[j] <= 0) continue;
     const float s = mx4_scale_value<FMT>(byte[j]);
     const float t = one_scale ? t0 : tensor_scale[(long long)row[j] / rows_per_scale];
-    float v[8];
-    mx4_values8(word[j], v);
+    float v[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = FMT == GLQB_MX4_NVFP4 ? v[e] * s * t : v[e] * s;
-    const long long at = (long long)row[j] * q.cols + (long long)c[j] * 8;
-    const bool whole = left[j] >= 8 && q.vec;
+    for (int w = 0; w < 2; ++w) {
+      float u[8];
+      mx4_values8(part[j][2 * w] | part[j][2 * w + 1] << 16, u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[8 * w + e] = FMT == GLQB_MX4_NVFP4 ? u[e] * s * t : u[e] * s;
+    }
+    const long long at = (long long)row[j] * q.cols + (long long)c[j] * 16;
+    const bool whole = left[j] == 16 && q.vec;
     if (out_dtype == GLQB_DT_F32) {
       float* o = reinterpret_cast<float*>(out) + at;
       if (whole) {
-        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else
-        for (int e = 0; e < 8; ++e)
-          if (e < left[j]) o[e] = v[e];
-    } else {
-      uint32_t h[4];
+        uint4 h[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e)
+          h[e] = make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+        put32(o, h[0], h[1], q.vec);
+        put32(o + 8, h[2], h[3], q.vec);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (e < left[j]) o[e] = v[e];
+      }
+    } else {
+      uint32_t h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
         if (out_dtype == GLQB_DT_F16) {
           const __half2 r = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
           h[e] = *reinterpret_cast<const uint32_t*>(&r);
@@ -227,10 +266,12 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
         }
       }
       uint16_t* o = reinterpret_cast<uint16_t*>(out) + at;
-      if (whole) *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
-      else
-        for (int e = 0; e < 8; ++e)
+      if (whole) put32(o, make_uint4(h[0], h[1], h[2], h[3]), make_uint4(h[4], h[5], h[6], h[7]), q.vec);
+      else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
           if (e < left[j]) o[e] = (uint16_t)(h[e >> 1] >> (16 * (e & 1)));
+      }
     }
   }
 }
@@ -318,65 +359,91 @@ __global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* x, long 
 // 128-byte swizzle, then the scales, 128 rows at a time as in the weight image).  A warp takes `batches` times 1024 values of a row
 // (with many rows all of a row: finding its tile takes as long as a thousand values); values past the row are zeros, rows past a
 // tile's are left out (their columns are not stored).
+constexpr int X_TILES = 2 * QT_BATCH;              // of 256 values: what a warp takes at once
 template <typename T, int FMT>
 __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
-                                                                 int x_scales, bool vec, int batches) {
+                                                                 int x_scales, int vec, int batches) {
   extern __shared__ int lists[];
   const Mx4Lists L(lists, J.experts);
   pdl_wait();
   pdl_trigger();
   mx4_groups(J, L);
-  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 8;
+  constexpr int PER = Mx4Fmt<FMT>::BLOCK / 16;
   float t = 1.0f;
   if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(x_scale, own_scale, parts);
-  const int lane = threadIdx.x & 31, first = L.eff[0], end = L.eff[J.experts], per_row = (J.k_tiles + QT_BATCH * batches - 1) / (QT_BATCH * batches);
+  const int lane = threadIdx.x & 31, first = L.eff[0], end = L.eff[J.experts], per_row = (J.k_tiles + X_TILES * batches - 1) / (X_TILES * batches);
+  const int half = lane >> 4, c = lane & 15;                // a step's second tile, sixteen of a tile
   const long long stage = (long long)J.tn * 128 + x_scales, items = (long long)(end - first) * per_row;
   for (long long i = (long long)blockIdx.x * (QT_THREADS / 32) + (threadIdx.x >> 5); i < items; i += (long long)gridDim.x * (QT_THREADS / 32)) {
     const int at_row = per_row == 1 ? (int)i : (int)((unsigned long long)i / (unsigned)per_row), row = first + at_row;
-    int k0 = (int)(i - (long long)at_row * per_row) * QT_BATCH * batches;
+    int k0 = (int)(i - (long long)at_row * per_row) * X_TILES * batches;
     const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
     const int e = J.experts == 1 ? 0 : mx4_find(L.eff, J.experts, row), in = row - L.eff[e];
     const int per = L.per[e], tile = L.pre[e] + in / per, r = in % per;
     if (tile >= J.max_tiles) continue;
-    uint8_t* at = J.x_image + ((long long)tile * J.k_tiles + k0) * stage;
-    uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
-    uint8_t* scales = at + J.tn * 128 + (r >> 7) * mx4_scale_bytes(FMT) + mx4_scale_offset(r & 127, lane / PER);
-    for (const int k1 = min(J.k_tiles, k0 + QT_BATCH * batches); k0 < k1; k0 += QT_BATCH) {
+    uint8_t* at = J.x_image + ((long long)tile * J.k_tiles + k0 + half) * stage;
+    uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+    uint8_t* scales = at + J.tn * 128 + (r >> 7) * mx4_scale_bytes(FMT) + mx4_scale_offset(r & 127, c / PER);
+    for (const int k1 = min(J.k_tiles, k0 + X_TILES * batches); k0 < k1; k0 += X_TILES) {
       Mx4Raw<T> raw[QT_BATCH];
 #pragma unroll
-      for (int j = 0; j < QT_BATCH; ++j) raw[j].load(src, (k0 + j) * MX4_K + lane * 8, J.n, vec);
+      for (int j = 0; j < QT_BATCH; ++j) {
+        const long long col = (long long)(k0 + 2 * j + half) * MX4_K + c * 16;
+        raw[j].load(src + col, (int)max(0ll, min(16ll, J.n - col)), vec);
+      }
 #pragma unroll
-      for (int j = 0; j < QT_BATCH; ++j, codes += stage, scales += stage) {
+      for (int j = 0; j < QT_BATCH; ++j, codes += 2 * stage, scales += 2 * stage) {
         uint32_t s;
-        float v[8];
+        float v[16];
         raw[j].get(v);
-        const uint32_t word = mx4_quantize8<FMT, true>(v, t, s);
+        const uint2 word = mx4_quantize16<FMT, true>(v, raw[j].top(), t, s);
         // four blocks' scales lie together: one store (a store per byte took a sixth of the kernel's time)
         s |= __shfl_down_sync(0xFFFFFFFFu, s, PER) << 8;
         s |= __shfl_down_sync(0xFFFFFFFFu, s, 2 * PER) << 16;
-        if (k0 + j >= k1) continue;
-        *reinterpret_cast<uint32_t*>(codes) = word;
-        if (lane % (4 * PER) == 0) *reinterpret_cast<uint32_t*>(scales) = s;
+        if (k0 + 2 * j + half >= k1) continue;
+        *reinterpret_cast<uint2*>(codes) = word;
+        if (c % (4 * PER) == 0) *reinterpret_cast<uint32_t*>(scales) = s;
       }
     }
   }
 }
 
-Mx4Rows rows_of(long long rows, int cols, long long stride, int format, const void* base, int elem) {
+// rows on 32 bytes, on 16, or anywhere
+int vec_of(const void* base, long long rows, long long stride_bytes) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(base) | (rows == 1 ? 0 : (uintptr_t)stride_bytes);
+  return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
+}
+Mx4Rows rows_of(long long rows, int cols, long long stride, int format, const void* base, int elem, bool join) {
   const int block = mx4_block(format);
   Mx4Rows q;
   q.rows = rows;
   q.cols = cols;
   q.stride = stride;
-  q.chunks = ((long long)cols + block - 1) / block * (block / 8);
-  q.vec = reinterpret_cast<uintptr_t>(base) % 16 == 0 && (stride * elem % 16 == 0 || rows == 1);
-  if (stride == cols && cols % block == 0) {       // whole blocks, no gaps: one row
+  q.chunks = ((long long)cols + block - 1) / block * (block / 16);
+  q.vec = vec_of(base, rows, stride * elem);
+  if (join && stride == cols && cols % block == 0) {       // whole blocks, no gaps: one row
     q.cols = rows * cols;
-    q.chunks = q.cols / 8;
+    q.chunks = q.cols / 16;
     q.rows = 1;
-    q.vec = reinterpret_cast<uintptr_t>(base) % 16 == 0;
+    q.vec = vec_of(base, 1, 0);
   }
+  q.full = q.cols / 16;
+  q.rest = (int)(q.cols % 16);
+  // Division by a multiplication: with 2^(l - 1) < chunks <= 2^l and magic = ceil(2^(31 + l) / chunks), less than
+  // 2^32, magic * chunks is above 2^(31 + l) by less than 2^l, so that i * magic / 2^(31 + l) is off by less than 1 / chunks for i < 2^31.
+  q.magic = 0;
+  q.shift = 0;
+  if (q.chunks < 2 || q.chunks >= 1ll << 31) return q;
+  int l = 1;
+  while ((1ll << l) < q.chunks) ++l;
+  q.magic = (uint32_t)(((1ull << (31 + l)) + (uint64_t)q.chunks - 1) / (uint64_t)q.chunks);
+  q.shift = l - 1;
   return q;
+}
+// widest stores and loads of codes, in bytes
+int unit_of(const uint8_t* codes, const Mx4Rows& q) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(codes) | (q.rows == 1 ? 0 : (uintptr_t)((q.cols + 1) / 2));
+  return bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
 }
 bool small(const Mx4Rows& q) { return q.rows * q.chunks < (1ll << 31) - QT_THREADS * QT_BATCH; }
 unsigned grid_for(const Mx4Rows& q) { return (unsigned)((q.rows * q.chunks + QT_THREADS * QT_BATCH - 1) / (QT_THREADS * QT_BATCH)); }
@@ -402,7 +469,7 @@ int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const float* t
   auto run = [&](auto type, auto index) {
     using T = decltype(type);
     launch_chained(true, mx4_quantize_kernel<T, FMT, decltype(index)>, (int)grid_for(q), QT_THREADS, 0, stream, (const T*)x, q, tensor_scale, own_scale, parts, codes,
-                   scales);
+                   scales, unit_of(codes, q));
   };
   auto of = [&](auto type) { small(q) ? run(type, (uint32_t)0) : run(type, (uint64_t)0); };
   if (x_dtype == GLQB_DT_F16) of(__half());
@@ -414,7 +481,7 @@ template <int FMT>
 int dequantize_launch(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, const Mx4Rows& q, void* out,
                       int out_dtype, cudaStream_t stream) {
   auto* kernel = small(q) ? mx4_dequantize_kernel<FMT, uint32_t> : mx4_dequantize_kernel<FMT, uint64_t>;
-  launch_chained(true, kernel, (int)grid_for(q), QT_THREADS, 0, stream, codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
+  launch_chained(true, kernel, (int)grid_for(q), QT_THREADS, 0, stream, codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype, unit_of(codes, q));
   return mx4_launched("mx4_dequantize");
 }
 
@@ -438,7 +505,7 @@ int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t 
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!x || !codes || !scales) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: null argument");
   if (x_stride < cols && rows > 1) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: rows of %d values %lld apart", cols, (long long)x_stride);
-  const Mx4Rows q = rows_of(rows, cols, x_stride, format, x, size_of(x_dtype));
+  const Mx4Rows q = rows_of(rows, cols, x_stride, format, x, size_of(x_dtype), true);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
     return quantize_launch<GLQB_MX4_MXFP4>(x, x_dtype, q, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
@@ -453,12 +520,7 @@ int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tens
   if (format == GLQB_MX4_NVFP4 && (!tensor_scale || rows_per_scale < 1)) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: nvfp4 needs tensor_scale");
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!codes || !scales || !out) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: null argument");
-  Mx4Rows q = rows_of(rows, cols, cols, format, out, size_of(out_dtype));
-  if (q.rows == 1 && rows > 1 && format == GLQB_MX4_NVFP4 && rows_per_scale < rows) {     // (rows under scales of their own)
-    q.rows = rows;
-    q.cols = cols;
-    q.chunks = cols / 8;
-  }
+  const Mx4Rows q = rows_of(rows, cols, cols, format, out, size_of(out_dtype), format == GLQB_MX4_MXFP4 || rows_per_scale >= rows);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
     return dequantize_launch<GLQB_MX4_MXFP4>((const uint8_t*)codes, (const uint8_t*)scales, nullptr, rows, q, out, out_dtype, stream);
@@ -627,14 +689,13 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.x_image = (uint8_t*)workspace;
   float* own = (float*)((uint8_t*)workspace + f.image);
   J.x_scale = x_scale ? x_scale : own;
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_stride * size_of(x_dtype) % 16 == 0);
+  const int vec = vec_of(x, rows, x_stride * size_of(x_dtype));
   int parts = 0;
   if (w->format == GLQB_MX4_NVFP4 && !x_scale) {
-    Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, x, size_of(x_dtype));
-    if (offsets && q.rows == 1) { q.rows = rows; q.cols = w->n; q.chunks = w->n / 8; }
+    const Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, x, size_of(x_dtype), !offsets);
     parts = amax_launch(x, x_dtype, q, Mx4Range{offsets, offsets_are_int64, w->experts}, own + 1, stream);
   }
-  const long long warps = (long long)sms * 64, batches = (J.k_tiles + QT_BATCH - 1) / QT_BATCH;
+  const long long warps = (long long)sms * 64, batches = (J.k_tiles + X_TILES - 1) / X_TILES;
   const int at_once = (int)std::max<long long>(1, std::min(batches, rows * batches / warps));
   const int grid = (int)std::min<long long>((rows * ((batches + at_once - 1) / at_once) + 7) / 8, (long long)sms * 8);
   auto image = [&](auto fmt) {

@@ -130,100 +130,137 @@ static __device__ __noinline__ uint32_t mx4_decide_tiny(float x, float s, float 
   return (uint32_t)((a > 0.25 * d) + (a >= 0.75 * d) + (a > 1.25 * d) + (a >= 1.75 * d) + (a > 2.5 * d) + (a >= 3.5 * d) + (a > 5.0 * d));
 }
 
-// Eight consecutive values of a row per thread; the BLOCK / 8 threads of a block are neighbours in a warp (all 32 lanes take
-// part).  Returns the eight codes; `scale`: the block's byte, the same in its threads.  A block with an infinity or NaN
-// gets the scale NaN and codes of zero.
+// Sixteen consecutive values of a row per thread, `top` the bits of their largest magnitude; the BLOCK / 16 threads of a block are
+// neighbours in a warp (all 32 lanes take part).  Returns the codes; `scale`: the block's byte, the same in its threads.  A
+// block with an infinity or NaN gets the scale NaN and codes of zero.
 template <int FMT, bool IMAGE>
-__device__ __forceinline__ uint32_t mx4_quantize8(const float (&v)[8], float t, uint32_t& scale) {
-  uint32_t top = 0;
+__device__ __forceinline__ uint2 mx4_quantize16(const float (&v)[16], uint32_t top, float t, uint32_t& scale) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int d = 1; d < Mx4Fmt<FMT>::BLOCK / 8; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  for (int d = 1; d < Mx4Fmt<FMT>::BLOCK / 16; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
   const bool broken = top >= 0x7F800000u;
+  uint32_t c[2];
   if constexpr (FMT == GLQB_MX4_MXFP4) {
     const uint32_t e = top >> 23;
     scale = broken ? 255u : e > 2u ? e - 2u : 0u;
-    if (broken) return 0u;
+    if (broken) return make_uint2(0u, 0u);
     const float r = __uint_as_float((254u - scale) << 23);
-    float q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] * r;
-    return mx4_codes8<IMAGE>(q);
+    for (int w = 0; w < 2; ++w) {
+      float q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = v[8 * w + i] * r;
+      c[w] = mx4_codes8<IMAGE>(q);
+    }
   } else {
     scale = broken ? 0x7Fu : mx4_nv_scale(__uint_as_float(top), t);
-    if (broken) return 0u;
+    if (broken) return make_uint2(0u, 0u);
     const float s = mx4_e4m3(scale), step = s * t;
-    float lo[8], hi[8];
     if (step >= MX4_TINY) {
       const float r = __frcp_rn(step), rl = r * MX4_BELOW, rh = r * MX4_ABOVE;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { lo[i] = v[i] * rl; hi[i] = v[i] * rh; }
-      const uint32_t a = mx4_codes8<IMAGE>(lo), b = mx4_codes8<IMAGE>(hi);
-      if (a == b) return a;
-      uint32_t c = 0;
+      for (int w = 0; w < 2; ++w) {
+        float lo[8], hi[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = IMAGE ? (i >> 1) + 4 * (i & 1) : i;
-        const uint32_t l = (a >> (4 * at)) & 15u, h = (b >> (4 * at)) & 15u;
-        c |= (mx4_decide(l & 7u, h & 7u, fabsf(v[i]), s, t) | (l & 8u)) << (4 * at);
+        for (int i = 0; i < 8; ++i) { lo[i] = v[8 * w + i] * rl; hi[i] = v[8 * w + i] * rh; }
+        const uint32_t a = mx4_codes8<IMAGE>(lo), b = mx4_codes8<IMAGE>(hi);
+        c[w] = a;
+        if (a != b) {
+          c[w] = 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = IMAGE ? (i >> 1) + 4 * (i & 1) : i;
+            const uint32_t l = (a >> (4 * at)) & 15u, h = (b >> (4 * at)) & 15u;
+            c[w] |= (mx4_decide(l & 7u, h & 7u, fabsf(v[8 * w + i]), s, t) | (l & 8u)) << (4 * at);
+          }
+        }
       }
-      return c;
-    }
-    uint32_t c = 0;
-    if (scale != 0u) {
+    } else {
+      c[0] = c[1] = 0u;
+      if (scale != 0u) {
 #pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
-        const int at = IMAGE ? (i >> 1) + 4 * (i & 1) : i;
-        float x = v[0];
+        for (int i = 0; i < 16; ++i) {
+          const int at = IMAGE ? ((i & 7) >> 1) + 4 * (i & 1) : i & 7;
+          float x = v[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) x = i == j ? v[j] : x;
-        c |= (mx4_decide_tiny(fabsf(x), s, t) | (x < 0.0f ? 8u : 0u)) << (4 * at);
+          for (int j = 1; j < 16; ++j) x = i == j ? v[j] : x;
+          const uint32_t code = (mx4_decide_tiny(fabsf(x), s, t) | (x < 0.0f ? 8u : 0u)) << (4 * at);
+          c[0] |= i < 8 ? code : 0u;
+          c[1] |= i < 8 ? 0u : code;
+        }
       }
     }
-    return c;
   }
+  return make_uint2(c[0], c[1]);
 }
 
 // The fp32 scale of a tensor whose largest finite value is `amax`: the top of both levels, 448 * 6, by its fp32 reciprocal.
 __device__ __forceinline__ float mx4_tensor_scale(float amax) { return fmaxf(amax * (1.0f / 2688.0f), 0x1p-126f); }
 
 // ---- loads of activations -------------------------------------------------------------------------
-// Values col .. col + 7 of a row as they lie, zeros from `cols` on (`vec`: rows start on 16 bytes), and as fp32.
+// 32 bytes at once, from and to addresses on 32 bytes.
+__device__ __forceinline__ void mx4_load32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void mx4_store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+}
+// Sixteen values of a row as they lie, zeros from the `left`-th on, and as fp32.  `vec`: rows start on 32 bytes (2), on 16 (1) or anywhere.
 template <typename T>
 struct Mx4Raw {
-  uint4 w[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* row, int col, int cols, bool vec) {
-    if (vec && col + 8 <= cols) {
+  uint4 w[sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, int left, int vec) {
+    if (left >= 16 && vec == 2) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(row + col)[i];
+      for (int i = 0; i < (int)sizeof(T); i += 2) mx4_load32(reinterpret_cast<const uint4*>(p) + i, w[i], w[i + 1]);
+    } else if (left >= 16 && vec) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
       using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
-      const U* p = reinterpret_cast<const U*>(row);
-      uint32_t h[sizeof(T) * 2];
+      const U* u = reinterpret_cast<const U*>(p);
+      uint32_t h[sizeof(T) * 4];
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) * 2; ++i) h[i] = 0u;
+      for (int i = 0; i < (int)sizeof(T) * 4; ++i) h[i] = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < cols) h[i * sizeof(T) / 4] |= (uint32_t)p[col + i] << (sizeof(T) == 4 ? 0 : 16 * (i & 1));
+      for (int i = 0; i < 16; ++i)
+        if (i < left) h[i * sizeof(T) / 4] |= (uint32_t)u[i] << (sizeof(T) == 4 ? 0 : 16 * (i & 1));
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      for (int i = 0; i < (int)sizeof(T); ++i) w[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
     }
   }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+  // bits, as fp32, of the largest magnitude (16-bit types: two at a time, their bits without the sign are ordered as they are)
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      for (int i = 0; i < 4; ++i)
+        m = max(max(m, max(w[i].x & 0x7FFFFFFFu, w[i].y & 0x7FFFFFFFu)), max(w[i].z & 0x7FFFFFFFu, w[i].w & 0x7FFFFFFFu));
+      return m;
+    } else {
+      constexpr uint32_t M = 0x7FFF7FFFu;
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) m = __vmaxu2(__vmaxu2(m, __vmaxu2(w[i].x & M, w[i].y & M)), __vmaxu2(w[i].z & M, w[i].w & M));
+      if constexpr (__is_same(T, __half)) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xFFFFu, m >> 16))));
+      else return max(m << 16, m & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[16]) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) {
       const uint32_t h[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (sizeof(T) == 4) v[4 * i + j] = __uint_as_float(h[j]);
         else if constexpr (__is_same(T, __half)) {
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-          v[2 * j] = f.x;
-          v[2 * j + 1] = f.y;
+          v[8 * i + 2 * j] = f.x;
+          v[8 * i + 2 * j + 1] = f.y;
         } else {
-          v[2 * j] = __uint_as_float(h[j] << 16);
-          v[2 * j + 1] = __uint_as_float(h[j] & 0xFFFF0000u);
+          v[8 * i + 2 * j] = __uint_as_float(h[j] << 16);
+          v[8 * i + 2 * j + 1] = __uint_as_float(h[j] & 0xFFFF0000u);
         }
       }
     }
