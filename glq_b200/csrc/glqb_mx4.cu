@@ -37,7 +37,6 @@ struct Mx4Rows {
   long long full;             // those that have all sixteen
   uint32_t magic;             // i / chunks = i * magic / 2^(32 + shift) for i < 2^31 (see rows_of)
   int rest, shift;            // values behind the full ones
-  int vec;                    // rows start on 32 bytes (2), on 16 (1), or anywhere (0)
 };
 
 // Rows offsets[0] .. offsets[experts] - 1, held to those there are.
@@ -88,7 +87,7 @@ __global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* x, Mx4R
       const I i = b + j * step;
       I row, c;
       place(q, i, row, c);
-      raw[j].load(x + (long long)row * q.stride + (long long)c * 16, i < end ? values_at(q, c) : 0, q.vec);
+      raw[j].load(x + (long long)row * q.stride + (long long)c * 16, i < end ? values_at(q, c) : 0);
     }
 #pragma unroll
     for (int j = 0; j < QT_BATCH; ++j) {
@@ -135,7 +134,7 @@ __device__ __forceinline__ float whole_scale(const float* given, float* own_scal
 template <typename T, int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
 mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own_scale, int parts, uint8_t* codes,
-                    uint8_t* scales, int unit) {
+                    uint8_t* scales) {
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 16;
   pdl_wait();
   pdl_trigger();
@@ -149,7 +148,7 @@ mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own
     const I i = (I)blockIdx.x * (QT_THREADS * QT_BATCH) + j * QT_THREADS + threadIdx.x;
     place(q, i, row[j], c[j]);
     left[j] = i < total ? values_at(q, c[j]) : -1;
-    raw[j].load(x + (long long)row[j] * q.stride + (long long)c[j] * 16, left[j], q.vec);
+    raw[j].load(x + (long long)row[j] * q.stride + (long long)c[j] * 16, left[j]);
   }
   float t = 1.0f;
   if constexpr (FMT == GLQB_MX4_NVFP4) t = whole_scale(tensor_scale, own_scale, parts);       // (while the values are on their way)
@@ -161,13 +160,15 @@ mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own
     const uint2 word = mx4_quantize16<FMT, false>(v, raw[j].top(), t, s);     // (all lanes: the threads of a block exchange their largest value)
     if (left[j] < 0) continue;
     uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 8;
-    if (left[j] == 16 && unit == 8) *reinterpret_cast<uint2*>(p) = word;
-    else if (left[j] == 16 && unit == 4) {
+    const uint32_t at = left[j] == 16 ? (uint32_t)reinterpret_cast<uintptr_t>(p) : 1u;
+    if ((at & 7u) == 0) *reinterpret_cast<uint2*>(p) = word;
+    else if ((at & 3u) == 0) {
       reinterpret_cast<uint32_t*>(p)[0] = word.x;
       reinterpret_cast<uint32_t*>(p)[1] = word.y;
-    } else if (left[j] == 16 && unit == 2) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b) reinterpret_cast<uint16_t*>(p)[b] = (uint16_t)((b < 2 ? word.x : word.y) >> (16 * (b & 1)));
+    } else if ((at & 1u) == 0) {
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)word.x;
+      *reinterpret_cast<uint32_t*>(p + 2) = __funnelshift_r(word.x, word.y, 16);
+      *reinterpret_cast<uint16_t*>(p + 6) = (uint16_t)(word.y >> 16);
     } else {
 #pragma unroll
       for (int b = 0; b < 8; ++b)
@@ -177,17 +178,10 @@ mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own
   }
 }
 
-__device__ __forceinline__ void put32(void* p, const uint4& a, const uint4& b, int vec) {
-  if (vec == 2) mx4_store32(p, a, b);
-  else {
-    reinterpret_cast<uint4*>(p)[0] = a;
-    reinterpret_cast<uint4*>(p)[1] = b;
-  }
-}
 template <int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
 mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, Mx4Rows q, void* out,
-                      int out_dtype, int unit) {
+                      int out_dtype) {
   constexpr int PER = Mx4Fmt<FMT>::BLOCK / 16;
   pdl_wait();
   pdl_trigger();
@@ -207,20 +201,22 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
     byte[j] = part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0;
     if (left[j] <= 0) continue;
     const uint8_t* p = codes + (long long)row[j] * code_row + (long long)c[j] * 8;
-    if (left[j] == 16 && unit == 8) {
+    const uint32_t at = left[j] == 16 ? (uint32_t)reinterpret_cast<uintptr_t>(p) : 1u;
+    if ((at & 7u) == 0) {
       const uint2 w = *reinterpret_cast<const uint2*>(p);
       part[j][0] = w.x;
       part[j][2] = w.y;
-    } else if (left[j] == 16 && unit == 4) {
+    } else if ((at & 3u) == 0) {
       part[j][0] = reinterpret_cast<const uint32_t*>(p)[0];
       part[j][2] = reinterpret_cast<const uint32_t*>(p)[1];
-    } else if (left[j] == 16 && unit == 2) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b) part[j][b] = reinterpret_cast<const uint16_t*>(p)[b];
+    } else if ((at & 1u) == 0) {
+      part[j][0] = *reinterpret_cast<const uint16_t*>(p);
+      part[j][1] = *reinterpret_cast<const uint32_t*>(p + 2);
+      part[j][3] = *reinterpret_cast<const uint16_t*>(p + 6);
     } else {
 #pragma unroll
       for (int b = 0; b < 8; ++b)
-        if (2 * b < left[j]) part[j][b >> 1] |= (uint32_t)p[b] << (8 * (b & 1));
+        if (2 * b < left[j]) part[j][b >> 2 << 1] |= (uint32_t)p[b] << (8 * (b & 3));
     }
     byte[j] = scales[(long long)row[j] * scale_row + (long long)(c[j] / PER)];
   }
@@ -229,26 +225,23 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
     if (left[j] <= 0) continue;
     const float s = mx4_scale_value<FMT>(byte[j]);
     const float t = one_scale ? t0 : tensor_scale[(long long)row[j] / rows_per_scale];
+    const uint32_t words[2] = {part[j][0] | part[j][1] << 16, part[j][2] | part[j][1] >> 16 | part[j][3] << 16};
     float v[16];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       float u[8];
-      mx4_values8(part[j][2 * w] | part[j][2 * w + 1] << 16, u);
+      mx4_values8(words[w], u);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[8 * w + e] = FMT == GLQB_MX4_NVFP4 ? u[e] * s * t : u[e] * s;
     }
     const long long at = (long long)row[j] * q.cols + (long long)c[j] * 16;
-    const bool whole = left[j] == 16 && q.vec;
     if (out_dtype == GLQB_DT_F32) {
       float* o = reinterpret_cast<float*>(out) + at;
-      if (whole) {
-        uint4 h[4];
+      uint32_t h[16];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          h[e] = make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
-        put32(o, h[0], h[1], q.vec);
-        put32(o + 8, h[2], h[3], q.vec);
-      } else {
+      for (int e = 0; e < 16; ++e) h[e] = __float_as_uint(v[e]);
+      if (left[j] == 16) mx4_put_words(o, h);
+      else {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (e < left[j]) o[e] = v[e];
@@ -266,7 +259,7 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
         }
       }
       uint16_t* o = reinterpret_cast<uint16_t*>(out) + at;
-      if (whole) put32(o, make_uint4(h[0], h[1], h[2], h[3]), make_uint4(h[4], h[5], h[6], h[7]), q.vec);
+      if (left[j] == 16) mx4_put_words(o, h);
       else {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -362,7 +355,7 @@ __global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* x, long 
 constexpr int X_TILES = 2 * QT_BATCH;              // of 256 values: what a warp takes at once
 template <typename T, int FMT>
 __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
-                                                                 int x_scales, int vec, int batches) {
+                                                                 int x_scales, int batches) {
   extern __shared__ int lists[];
   const Mx4Lists L(lists, J.experts);
   pdl_wait();
@@ -374,13 +367,30 @@ __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_co
   const int lane = threadIdx.x & 31, first = L.eff[0], end = L.eff[J.experts], per_row = (J.k_tiles + X_TILES * batches - 1) / (X_TILES * batches);
   const int half = lane >> 4, c = lane & 15;                // a step's second tile, sixteen of a tile
   const long long stage = (long long)J.tn * 128 + x_scales, items = (long long)(end - first) * per_row;
-  for (long long i = (long long)blockIdx.x * (QT_THREADS / 32) + (threadIdx.x >> 5); i < items; i += (long long)gridDim.x * (QT_THREADS / 32)) {
-    const int at_row = per_row == 1 ? (int)i : (int)((unsigned long long)i / (unsigned)per_row), row = first + at_row;
-    int k0 = (int)(i - (long long)at_row * per_row) * X_TILES * batches;
-    const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
-    const int e = J.experts == 1 ? 0 : mx4_find(L.eff, J.experts, row), in = row - L.eff[e];
-    const int per = L.per[e], tile = L.pre[e] + in / per, r = in % per;
+  const long long warps = (long long)gridDim.x * (QT_THREADS / 32), w = (long long)blockIdx.x * (QT_THREADS / 32) + (threadIdx.x >> 5);
+  const long long i0 = w * items / warps, i1 = (w + 1) * items / warps;
+  if (i0 == i1) return;
+  // a warp's items follow one another: the expert and the tile of a row come from those of the row before
+  int row = first + (int)(i0 / per_row), part = (int)(i0 % per_row);
+  int e = J.experts == 1 ? 0 : mx4_find(L.eff, J.experts, row), per = L.per[e];
+  int tile = L.pre[e] + (row - L.eff[e]) / per, r = (row - L.eff[e]) % per;
+  for (long long i = i0; i < i1; ++i) {
+    if (i > i0 && ++part == per_row) {
+      part = 0;
+      ++row;
+      if (row >= L.eff[e + 1]) {
+        while (row >= L.eff[e + 1]) ++e;
+        per = L.per[e];
+        tile = L.pre[e];
+        r = 0;
+      } else if (++r == per) {
+        ++tile;
+        r = 0;
+      }
+    }
     if (tile >= J.max_tiles) continue;
+    int k0 = part * X_TILES * batches;
+    const T* src = reinterpret_cast<const T*>(J.x) + row * J.x_stride;
     uint8_t* at = J.x_image + ((long long)tile * J.k_tiles + k0 + half) * stage;
     uint8_t* codes = at + (r >> 3) * 1024 + (r & 7) * 128 + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
     uint8_t* scales = at + J.tn * 128 + (r >> 7) * mx4_scale_bytes(FMT) + mx4_scale_offset(r & 127, c / PER);
@@ -388,8 +398,8 @@ __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_co
       Mx4Raw<T> raw[QT_BATCH];
 #pragma unroll
       for (int j = 0; j < QT_BATCH; ++j) {
-        const long long col = (long long)(k0 + 2 * j + half) * MX4_K + c * 16;
-        raw[j].load(src + col, (int)max(0ll, min(16ll, J.n - col)), vec);
+        const int col = (k0 + 2 * j + half) * MX4_K + c * 16;
+        raw[j].load(src + col, max(0, min(16, J.n - col)));
       }
 #pragma unroll
       for (int j = 0; j < QT_BATCH; ++j, codes += 2 * stage, scales += 2 * stage) {
@@ -408,24 +418,17 @@ __global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_co
   }
 }
 
-// rows on 32 bytes, on 16, or anywhere
-int vec_of(const void* base, long long rows, long long stride_bytes) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(base) | (rows == 1 ? 0 : (uintptr_t)stride_bytes);
-  return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
-}
-Mx4Rows rows_of(long long rows, int cols, long long stride, int format, const void* base, int elem, bool join) {
+Mx4Rows rows_of(long long rows, int cols, long long stride, int format, bool join) {
   const int block = mx4_block(format);
   Mx4Rows q;
   q.rows = rows;
   q.cols = cols;
   q.stride = stride;
   q.chunks = ((long long)cols + block - 1) / block * (block / 16);
-  q.vec = vec_of(base, rows, stride * elem);
   if (join && stride == cols && cols % block == 0) {       // whole blocks, no gaps: one row
     q.cols = rows * cols;
     q.chunks = q.cols / 16;
     q.rows = 1;
-    q.vec = vec_of(base, 1, 0);
   }
   q.full = q.cols / 16;
   q.rest = (int)(q.cols % 16);
@@ -439,11 +442,6 @@ Mx4Rows rows_of(long long rows, int cols, long long stride, int format, const vo
   q.magic = (uint32_t)(((1ull << (31 + l)) + (uint64_t)q.chunks - 1) / (uint64_t)q.chunks);
   q.shift = l - 1;
   return q;
-}
-// widest stores and loads of codes, in bytes
-int unit_of(const uint8_t* codes, const Mx4Rows& q) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(codes) | (q.rows == 1 ? 0 : (uintptr_t)((q.cols + 1) / 2));
-  return bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
 }
 bool small(const Mx4Rows& q) { return q.rows * q.chunks < (1ll << 31) - QT_THREADS * QT_BATCH; }
 unsigned grid_for(const Mx4Rows& q) { return (unsigned)((q.rows * q.chunks + QT_THREADS * QT_BATCH - 1) / (QT_THREADS * QT_BATCH)); }
@@ -469,7 +467,7 @@ int quantize_launch(const void* x, int x_dtype, const Mx4Rows& q, const float* t
   auto run = [&](auto type, auto index) {
     using T = decltype(type);
     launch_chained(true, mx4_quantize_kernel<T, FMT, decltype(index)>, (int)grid_for(q), QT_THREADS, 0, stream, (const T*)x, q, tensor_scale, own_scale, parts, codes,
-                   scales, unit_of(codes, q));
+                   scales);
   };
   auto of = [&](auto type) { small(q) ? run(type, (uint32_t)0) : run(type, (uint64_t)0); };
   if (x_dtype == GLQB_DT_F16) of(__half());
@@ -481,13 +479,12 @@ template <int FMT>
 int dequantize_launch(const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, long long rows_per_scale, const Mx4Rows& q, void* out,
                       int out_dtype, cudaStream_t stream) {
   auto* kernel = small(q) ? mx4_dequantize_kernel<FMT, uint32_t> : mx4_dequantize_kernel<FMT, uint64_t>;
-  launch_chained(true, kernel, (int)grid_for(q), QT_THREADS, 0, stream, codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype, unit_of(codes, q));
+  launch_chained(true, kernel, (int)grid_for(q), QT_THREADS, 0, stream, codes, scales, tensor_scale, rows_per_scale, q, out, out_dtype);
   return mx4_launched("mx4_dequantize");
 }
 
 bool dtype_ok(int d) { return d == GLQB_DT_F16 || d == GLQB_DT_BF16 || d == GLQB_DT_F32; }
 bool format_ok(int f) { return f == GLQB_MX4_MXFP4 || f == GLQB_MX4_NVFP4; }
-int size_of(int dtype) { return dtype == GLQB_DT_F32 ? 4 : 2; }
 
 }  // namespace
 }  // namespace glqb
@@ -505,7 +502,7 @@ int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t 
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!x || !codes || !scales) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: null argument");
   if (x_stride < cols && rows > 1) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: rows of %d values %lld apart", cols, (long long)x_stride);
-  const Mx4Rows q = rows_of(rows, cols, x_stride, format, x, size_of(x_dtype), true);
+  const Mx4Rows q = rows_of(rows, cols, x_stride, format, true);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
     return quantize_launch<GLQB_MX4_MXFP4>(x, x_dtype, q, tensor_scale, own_scale, (uint8_t*)codes, (uint8_t*)scales, stream);
@@ -520,7 +517,7 @@ int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tens
   if (format == GLQB_MX4_NVFP4 && (!tensor_scale || rows_per_scale < 1)) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: nvfp4 needs tensor_scale");
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!codes || !scales || !out) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: null argument");
-  const Mx4Rows q = rows_of(rows, cols, cols, format, out, size_of(out_dtype), format == GLQB_MX4_MXFP4 || rows_per_scale >= rows);
+  const Mx4Rows q = rows_of(rows, cols, cols, format, format == GLQB_MX4_MXFP4 || rows_per_scale >= rows);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
     return dequantize_launch<GLQB_MX4_MXFP4>((const uint8_t*)codes, (const uint8_t*)scales, nullptr, rows, q, out, out_dtype, stream);
@@ -689,20 +686,19 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   J.x_image = (uint8_t*)workspace;
   float* own = (float*)((uint8_t*)workspace + f.image);
   J.x_scale = x_scale ? x_scale : own;
-  const int vec = vec_of(x, rows, x_stride * size_of(x_dtype));
   int parts = 0;
   if (w->format == GLQB_MX4_NVFP4 && !x_scale) {
-    const Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, x, size_of(x_dtype), !offsets);
+    const Mx4Rows q = rows_of(rows, w->n, x_stride, w->format, !offsets);
     parts = amax_launch(x, x_dtype, q, Mx4Range{offsets, offsets_are_int64, w->experts}, own + 1, stream);
   }
-  const long long warps = (long long)sms * 64, batches = (J.k_tiles + X_TILES - 1) / X_TILES;
+  const long long warps = (long long)sms * 32, batches = (J.k_tiles + X_TILES - 1) / X_TILES;
   const int at_once = (int)std::max<long long>(1, std::min(batches, rows * batches / warps));
-  const int grid = (int)std::min<long long>((rows * ((batches + at_once - 1) / at_once) + 7) / 8, (long long)sms * 8);
+  const int grid = (int)std::min<long long>((rows * ((batches + at_once - 1) / at_once) + 7) / 8, (long long)sms * 4);
   auto image = [&](auto fmt) {
     constexpr int FMT = decltype(fmt)::value;
-    if (x_dtype == GLQB_DT_F16) launch_chained(true, mx4_x_image_kernel<__half, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, vec, at_once);
-    else if (x_dtype == GLQB_DT_BF16) launch_chained(true, mx4_x_image_kernel<__nv_bfloat16, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, vec, at_once);
-    else launch_chained(true, mx4_x_image_kernel<float, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, vec, at_once);
+    if (x_dtype == GLQB_DT_F16) launch_chained(true, mx4_x_image_kernel<__half, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, at_once);
+    else if (x_dtype == GLQB_DT_BF16) launch_chained(true, mx4_x_image_kernel<__nv_bfloat16, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, at_once);
+    else launch_chained(true, mx4_x_image_kernel<float, FMT>, grid, QT_THREADS, lists, stream, J, x_scale, own, parts, f.x_scales, at_once);
   };
   if (w->format == GLQB_MX4_MXFP4) image(std::integral_constant<int, GLQB_MX4_MXFP4>());
   else image(std::integral_constant<int, GLQB_MX4_NVFP4>());

@@ -206,28 +206,65 @@ __device__ __forceinline__ void mx4_store32(void* p, const uint4& a, const uint4
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
 }
-// Sixteen values of a row as they lie, zeros from the `left`-th on, and as fp32.  `vec`: rows start on 32 bytes (2), on 16 (1) or anywhere.
+// 32-bit words to any address that the values allow, in the widest stores that lie on their size.  (A sector that is written in two
+// halves costs as much as two: where 64 bytes start in the middle of a sector, its other half comes from the neighbour.)
+template <int WORDS>
+__device__ __forceinline__ void mx4_put_words(void* p, const uint32_t (&h)[WORDS]) {
+  const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(p);
+  auto four = [&](int i) { return make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]); };
+  uint4* p4 = reinterpret_cast<uint4*>(p);
+  if ((at & 31u) == 0) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 8) mx4_store32(p4 + i / 4, four(i), four(i + 4));
+  } else if ((at & 15u) == 0) {
+    p4[0] = four(0);
+#pragma unroll
+    for (int i = 4; i + 8 < WORDS; i += 8) mx4_store32(p4 + i / 4, four(i), four(i + 4));
+    p4[WORDS / 4 - 1] = four(WORDS - 4);
+  } else if ((at & 3u) == 0) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint32_t*>(p)[i] = h[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2 * WORDS; ++i) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(h[i >> 1] >> (16 * (i & 1)));
+  }
+}
+// Sixteen values of a row as they lie, zeros from the `left`-th on, and as fp32.
 template <typename T>
 struct Mx4Raw {
   uint4 w[sizeof(T)];
-  __device__ __forceinline__ void load(const T* p, int left, int vec) {
-    if (left >= 16 && vec == 2) {
+  __device__ __forceinline__ void load(const T* p, int left) {
+    constexpr int N = sizeof(T);
+    const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(p);
+    const uint4* p4 = reinterpret_cast<const uint4*>(p);
+    if (left >= 16 && (at & 31u) == 0) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T); i += 2) mx4_load32(reinterpret_cast<const uint4*>(p) + i, w[i], w[i + 1]);
-    } else if (left >= 16 && vec) {
+      for (int i = 0; i < N; i += 2) mx4_load32(p4 + i, w[i], w[i + 1]);
+    } else if (left >= 16 && (at & 15u) == 0) {
+      w[0] = p4[0];
+      if constexpr (N == 4) mx4_load32(p4 + 1, w[1], w[2]);
+      w[N - 1] = p4[N - 1];
+    } else if (left >= 16 && (at & 7u) == 0) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+      for (int i = 0; i < N; ++i) {
+        const uint2 a = reinterpret_cast<const uint2*>(p)[2 * i], b = reinterpret_cast<const uint2*>(p)[2 * i + 1];
+        w[i] = make_uint4(a.x, a.y, b.x, b.y);
+      }
+    } else if (left >= 16 && (at & 3u) == 0) {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
     } else {
-      using U = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+      using U = std::conditional_t<N == 4, uint32_t, uint16_t>;
       const U* u = reinterpret_cast<const U*>(p);
-      uint32_t h[sizeof(T) * 4];
+      uint32_t e[16];
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) * 4; ++i) h[i] = 0u;
+      for (int i = 0; i < 16; ++i) e[i] = i < left ? (uint32_t)u[i] : 0u;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < left) h[i * sizeof(T) / 4] |= (uint32_t)u[i] << (sizeof(T) == 4 ? 0 : 16 * (i & 1));
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T); ++i) w[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      for (int i = 0; i < N; ++i) {
+        if constexpr (N == 4) w[i] = make_uint4(e[4 * i], e[4 * i + 1], e[4 * i + 2], e[4 * i + 3]);
+        else w[i] = make_uint4(e[8 * i] | e[8 * i + 1] << 16, e[8 * i + 2] | e[8 * i + 3] << 16, e[8 * i + 4] | e[8 * i + 5] << 16, e[8 * i + 6] | e[8 * i + 7] << 16);
+      }
     }
   }
   // bits, as fp32, of the largest magnitude (16-bit types: two at a time, their bits without the sign are ordered as they are)
