@@ -247,22 +247,38 @@ __device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Walk& t, in
       if (c0 + i < t.rows) mx4_put(J, at + i * J.y_stride, __uint_as_float(v[i]) * f.a * f.b);
   }
 }
-// The cluster's parts of a tile, added in rank order; the columns are shared out over the CTAs.
+// The cluster's parts of a tile, added in rank order; the columns are shared out over the CTAs, then over their warps, a lane four rows
+// of 16 bytes.  (By 4-byte loads and 2-byte stores this took 3.5 us of 26 for 333 tokens of 2048 x 11008, four CTAs to a tile.)
 template <int FMT, typename T, bool QUANT>
 __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Walk& t, float* red, int rank) {
-  const int r = threadIdx.x % MX4_ROWS, row = t.mt * MX4_ROWS + r;
+  const int r = (threadIdx.x & 31) * 4, row = t.mt * MX4_ROWS + r, warps = blockDim.x >> 5;
   if (row >= J.m) return;
-  const Mx4Factor f = row_factor<FMT, T, QUANT>(J, t.expert, row);
+  Mx4Factor f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = row_factor<FMT, T, QUANT>(J, t.expert, min(row + i, J.m - 1));
   const uint32_t base = smem_u32(red) + (uint32_t)r * 4u;
-  const int groups = blockDim.x / MX4_ROWS, own = J.split * groups;
-#pragma unroll 1
-  for (int c = rank + J.split * (int)(threadIdx.x / MX4_ROWS); c < t.rows; c += 4 * own) {
-    float v[4];
+  for (int c = rank + J.split * (int)(threadIdx.x >> 5); c < t.rows; c += J.split * warps) {
+    const float4 s = sum_cluster4(base + (uint32_t)(c * MX4_ROWS * 4), J.split);
+    const float v[4] = {s.x * f[0].a * f[0].b, s.y * f[1].a * f[1].b, s.z * f[2].a * f[2].b, s.w * f[3].a * f[3].b};
+    const long long at = (long long)(t.row0 + c) * J.y_stride + row;
+    if (J.y_wide && row + 4 <= J.m) {
+      uint32_t h[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i * own < t.rows ? sum_cluster(base + (uint32_t)((c + i * own) * MX4_ROWS * 4), J.split) : 0.0f;
+      for (int i = 0; i < 2; ++i) {
+        if (J.y_dtype == GLQB_DT_BF16) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          h[i] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+          h[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(J.y) + at) = make_uint2(h[0], h[1]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i * own < t.rows) mx4_put(J, (long long)(t.row0 + c + i * own) * J.y_stride + row, v[i] * f.a * f.b);
+      for (int i = 0; i < 4; ++i)
+        if (row + i < J.m) mx4_put(J, at + i, v[i]);
+    }
   }
 }
 
@@ -301,9 +317,11 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     fence_mbar_init();
   }
   if (warp == 0) alloc_all<PAIR>(&B.tmem);
+  if (threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
   tc_fence_before();
   if (J.offsets) pdl_wait();
   mx4_groups(J, L);                         // (ends with a block barrier)
+  pdl_trigger();
   if constexpr (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = B.tmem, tmem_a = tmem + 2 * R.acc_cols;
@@ -537,6 +555,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   tc_fence_before();
   if (J.offsets) pdl_wait();
   mx4_groups(J, L);
+  pdl_trigger();
   if constexpr (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = B.tmem;

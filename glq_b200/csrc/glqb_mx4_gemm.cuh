@@ -35,11 +35,11 @@ struct Mx4Job {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {
   uint32_t a;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
 
@@ -48,14 +48,14 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float v) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
-// a value of every CTA of the cluster, added in rank order (all loads before the first sum)
-__device__ __forceinline__ float sum_cluster(uint32_t addr, int ranks) {
-  float v[8];
+// four values of every CTA of the cluster, added in rank order (all loads before the first sum)
+__device__ __forceinline__ float4 sum_cluster4(uint32_t addr, int ranks) {
+  float4 v[8];
 #pragma unroll
-  for (int s = 0; s < 8; ++s) v[s] = s < ranks ? ld_cluster(addr, s) : 0.0f;
-  float sum = v[0];
+  for (int s = 0; s < 8; ++s) v[s] = s < ranks ? ld_cluster4(addr, s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 sum = v[0];
 #pragma unroll
-  for (int s = 1; s < 8; ++s) sum += v[s];
+  for (int s = 1; s < 8; ++s) sum = make_float4(sum.x + v[s].x, sum.y + v[s].y, sum.z + v[s].z, sum.w + v[s].w);
   return sum;
 }
 // Rows of every expert and the token tiles in front of it.  offsets are held to 0 .. rows and to ascend (each at least
