@@ -538,7 +538,8 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
   if (reinterpret_cast<uintptr_t>(image) % 128) return mx4_fail(GLQB_E_INVALID, "mx4_pack: the image must be 128-byte aligned");
   const int mt = (m + MX4_ROWS - 1) / MX4_ROWS, kt = (n + MX4_K - 1) / MX4_K;
   const long long tiles = (long long)experts * mt * kt;
-  if (tiles >= (1ll << 31)) return mx4_fail(GLQB_E_INVALID, "mx4_pack: %d x %d x %d is more than 2^31 tiles", experts, m, n);
+  if (tiles >= (1ll << 31) || experts > MX4_MAX_EXPERTS || (long long)experts * mt >= 1ll << 27)
+    return mx4_fail(GLQB_E_INVALID, "mx4_pack: %d x %d x %d: too many tiles (at most %d experts)", experts, m, n, MX4_MAX_EXPERTS);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4) {
     const long long rows = (long long)experts * mt * MX4_ROWS;

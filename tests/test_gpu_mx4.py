@@ -517,6 +517,55 @@ def test_activations_of_any_size(fmt, tokens, dtype):
         assert np.array_equal(np.isnan(y[r]), np.isnan(want_bad)) and np.array_equal(np.isposinf(y[r]), np.isposinf(want_bad))
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens,m", [(1, 200), (40, 200), (250, 200), (1700, 1100)])
+def test_quantized_activations_with_infinities_and_nan(fmt, tokens, m):
+    """A block that holds one becomes NaN, and with it its row of the result; the others are what they are without it."""
+    g = np.random.default_rng(tokens)
+    n = 328
+    weight, w = make_weight(g, (m, n), fmt)
+    x = g.standard_normal((tokens, n))
+    bad = sorted({0, tokens // 3, tokens - 1})
+    for r, value in zip(bad, (np.nan, np.inf, -np.inf)):
+        x[r, (r * 7) % n] = value
+    xd = to_cuda(x, torch.bfloat16)
+    y = host(ops.mx4_linear(xd, weight, quantize_input=True, out_dtype=torch.float32))
+    assert np.isnan(y[bad]).all()
+    clean = np.setdiff1d(np.arange(tokens), bad)
+    if len(clean):
+        xv = quantized_values(host(xd), fmt)[clean]
+        want = xv @ w.T
+        assert np.all(np.abs(y[clean] - want) <= tolerance(xv, w, want, torch.float32))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_weights_with_nan_blocks_and_an_expert_of_zeros(fmt):
+    """NaN blocks of weights stay in their rows, in every form; an expert whose weights are all zero gives zeros."""
+    g = np.random.default_rng(2)
+    experts, m, n = 3, 140, 288
+    dense = g.standard_normal((experts, m, n))
+    dense[1] = 0.0
+    dense[0, 5, 40] = np.nan
+    dense[2, 139, 287] = np.inf
+    q = ops.mx4_quantize(to_cuda(dense), fmt)
+    weight = ops.mx4_pack(q)
+    nan = np.zeros((experts, m), bool)
+    nan[0, 5] = nan[2, 139] = True
+    w = host(ops.mx4_dequantize(q, torch.float32))
+    assert np.array_equal(np.isnan(w).any(-1), nan)
+    for per in (3, 50, 200):
+        off = counts_to_offsets([per] * experts)
+        x = to_cuda(g.standard_normal((experts * per, n)), torch.bfloat16)
+        for quantize in (False, True):
+            y = host(ops.mx4_grouped_linear(x, weight, off, quantize_input=quantize, out_dtype=torch.float32))
+            xv = quantized_values(host(x), fmt) if quantize else host(x)
+            for e in range(experts):
+                r = slice(e * per, (e + 1) * per)
+                assert np.isnan(y[r][:, nan[e]]).all()
+                want = xv[r] @ w[e][~nan[e]].T
+                assert np.all(np.abs(y[r][:, ~nan[e]] - want) <= tolerance(xv[r], w[e][~nan[e]], want, torch.float32))
+
+
 def test_stored_rows_that_start_anywhere():
     """Codes and scales in views that begin on odd addresses."""
     g = np.random.default_rng(4)
@@ -588,6 +637,25 @@ def test_offsets_beyond_32_bits():
         y = ops.mx4_linear(x, weight, quantize_input=quantize)
         check_product(y[-70:], quantized_values(host(tail[:, :64]), "nvfp4") if quantize else host(tail[:, :64]), w, torch.bfloat16)
         assert not y[:-70].any()
+
+
+def test_more_sixteens_than_31_bits():
+    """Rows whose sixteens of values are counted in 64 bits."""
+    rows, cols = 8330000, 4100
+    if torch.cuda.mem_get_info()[0] < 110 << 30:
+        pytest.skip("needs 110 GB")
+    g = np.random.default_rng(1)
+    tail = to_cuda(g.standard_normal((9, cols)), torch.bfloat16)
+    for fmt in FORMATS:
+        x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+        x[-9:] = tail
+        q, alone = ops.mx4_quantize(x, fmt), ops.mx4_quantize(tail, fmt)
+        del x
+        assert torch.equal(q.codes[-9:], alone.codes) and torch.equal(q.scales[-9:], alone.scales)
+        y = ops.mx4_dequantize(q)
+        assert torch.equal(y[-9:], ops.mx4_dequantize(alone)) and not y[-10].any() and not y[0].any()
+        del y, q
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("fmt", FORMATS)

@@ -129,6 +129,8 @@ def test_sizes_beyond_what_is_counted_are_refused(lib):
         assert rc == -1 and text in said, said
     for m, n in ((big, 1), (1, big)):
         assert lib.glqb_mx4_pack(p, p, 0, 1, m, n, p, None) == -1
+    assert lib.glqb_mx4_pack(p, p, 0, 1025, 8, 8, p, None) == -1 and "1024 experts" in lib.glqb_last_error().decode()
+    assert lib.glqb_mx4_pack(p, p, 0, 1024, 1 << 26, 1, p, None) == -1
 
 
 def test_layer_of_4_bit_weights_on_the_host():
