@@ -232,7 +232,12 @@ mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, const float* 
       float u[8];
       mx4_values8(words[w], u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 * w + e] = FMT == GLQB_MX4_NVFP4 ? u[e] * s * t : u[e] * s;
+      for (int e = 0; e < 8; e += 2) {
+        mx4_mul_f32x2(u[e], u[e + 1], s, s);
+        if constexpr (FMT == GLQB_MX4_NVFP4) mx4_mul_f32x2(u[e], u[e + 1], t, t);
+        v[8 * w + e] = u[e];
+        v[8 * w + e + 1] = u[e + 1];
+      }
     }
     const long long at = (long long)row[j] * q.cols + (long long)c[j] * 16;
     if (out_dtype == GLQB_DT_F32) {

@@ -89,6 +89,11 @@ __device__ __forceinline__ float mx4_scale_value(uint32_t byte) {
   else return mx4_e4m3(byte);
 }
 
+// Two products at once: (a x, b y).
+__device__ __forceinline__ void mx4_mul_f32x2(float& a, float& b, float x, float y) {
+  asm("{ .reg .b64 u, v; mov.b64 u, {%0, %1}; mov.b64 v, {%2, %3}; mul.rn.f32x2 u, u, v; mov.b64 {%0, %1}, u; }" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+
 // ---- quantisation ---------------------------------------------------------------------------------
 // The definition is in real numbers: the scale of an NVFP4 block is the e4m3 number nearest to amax / (6 t), a code the e2m1
 // number nearest to x / (s t), ties to even.  fp32 quotients can land on the wrong side of a border, so the conversion is done
@@ -148,7 +153,9 @@ __device__ __forceinline__ uint2 mx4_quantize16(const float (&v)[16], uint32_t t
     for (int w = 0; w < 2; ++w) {
       float q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = v[8 * w + i] * r;
+      for (int i = 0; i < 8; ++i) q[i] = v[8 * w + i];
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) mx4_mul_f32x2(q[i], q[i + 1], r, r);
       c[w] = mx4_codes8<IMAGE>(q);
     }
   } else {
@@ -161,7 +168,12 @@ __device__ __forceinline__ uint2 mx4_quantize16(const float (&v)[16], uint32_t t
       for (int w = 0; w < 2; ++w) {
         float lo[8], hi[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { lo[i] = v[8 * w + i] * rl; hi[i] = v[8 * w + i] * rh; }
+        for (int i = 0; i < 8; ++i) lo[i] = hi[i] = v[8 * w + i];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          mx4_mul_f32x2(lo[i], lo[i + 1], rl, rl);
+          mx4_mul_f32x2(hi[i], hi[i + 1], rh, rh);
+        }
         const uint32_t a = mx4_codes8<IMAGE>(lo), b = mx4_codes8<IMAGE>(hi);
         c[w] = a;
         if (a != b) {

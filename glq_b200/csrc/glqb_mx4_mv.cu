@@ -67,20 +67,27 @@ __device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
                                               __byte_perm(w[2], w[3], 0x7632));
     return 1.0f;
   } else {
-    uint32_t top = 0;
+    constexpr uint32_t M = 0x7FFF7FFFu;
+    const uint32_t both = __vmaxu2(__vmaxu2(w[0] & M, w[1] & M), __vmaxu2(w[2] & M, w[3] & M));
+    uint32_t top = max(both & 0xFFFFu, both >> 16);
+    if (top >= 0x7F80u) {                                // an infinity or NaN: the largest of the others
+      top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = w[i] & 0x7FFFu, hi = (w[i] >> 16) & 0x7FFFu;
-      top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = w[i] & 0x7FFFu, hi = (w[i] >> 16) & 0x7FFFu;
+        top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+      }
     }
+    __syncwarp();
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     const int e = max((int)(top >> 7), 15);              // biased exponent of the largest; 2^(141 - e) takes it to 2^14
     const float up = __uint_as_float((uint32_t)(268 - e) << 23);
     float f[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16) * up;
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u) * up;
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      mx4_mul_f32x2(f[2 * i], f[2 * i + 1], up, up);
     }
     auto pack = [](float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); };
     *reinterpret_cast<uint4*>(p) = make_uint4(pack(f[0], f[2]), pack(f[4], f[6]), pack(f[1], f[3]), pack(f[5], f[7]));
