@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* x, long 
 // tile's are left out (their columns are not stored).
 constexpr int X_TILES = 2 * QT_BATCH;              // of 256 values: what a warp takes at once
 template <typename T, int FMT>
-__global__ void __launch_bounds__(QT_THREADS) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
+__global__ void __launch_bounds__(QT_THREADS, 4) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
                                                                  int x_scales, int batches) {
   extern __shared__ int lists[];
   const Mx4Lists L(lists, J.experts);
