@@ -585,20 +585,25 @@ static const Device* device() {
   }
   return &d;
 }
-// Rows (an expert's, on average) up to which the streaming kernel runs.  Above / below, in a graph: 12 tokens of 4096 x 14336 19.8 / 17.3 us, of
-// 2048 x 2048 13.8 / 5.4, 16 of 14336 x 4096 19.8 / 20.5; 128 experts of 1536 x 2048, 600 rows 96 / 89, 1400 rows 98 / 108.
-constexpr int MV_MAX_ROWS = 16, MV_MAX_EXPERT_ROWS = 8;
+// Rows (an expert's, on average) up to which the streaming kernel runs; of small layers twice as many: its passes over the weights cost
+// less than the tensor-core form's start.  Streaming / tensor cores in a graph, us: 16 tokens of 4096 x 14336 17.2 / 19.4, of 2048 x 2048
+// 5.5 / 7.8, of 14336 x 4096 18.9 / 18.9, 24 30.6 / 19.4; 32 tokens of 2048 x 2048 6.3 / 8.3, of 2048 x 4096 8.1 / 9.6, of 8192 x 1024 8.3 / 8.7,
+// but of 1024 x 8192 11.0 / 9.9 and of 4096 x 4096 11.7 / 11.1; 128 experts of 1536 x 2048, 600 rows 80 / 94, 1000 82 / 94, 1400 93 / 94; of
+// 2048 x 768, 2000 rows 63 / 56.
+constexpr int MV_MAX_ROWS = 16, MV_MAX_EXPERT_ROWS = 8, MV_SMALL_TILES = 256, MV_SMALL_K = 16;
 static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, const Device* d) {
   Form f = {};
   const int avg = (int)((rows + w->experts - 1) / w->experts);
-  f.mv = !quantize && avg <= (w->experts == 1 ? MV_MAX_ROWS : MV_MAX_EXPERT_ROWS);
+  const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K;
+  const bool small = kt <= MV_SMALL_K && mt * kt <= MV_SMALL_TILES;
+  f.mv = !quantize && avg <= (w->experts != 1 ? MV_MAX_EXPERT_ROWS : small ? 2 * MV_MAX_ROWS : MV_MAX_ROWS);
   const int most = quantize ? (w->format == GLQB_MX4_MXFP4 ? 192 : 160) : 192;
   // token tiles: a matrix's rows split evenly; of experts up to twice their average, so that most have one tile
   if (f.mv) f.tn = avg > (w->experts == 1 ? 8 : 4) ? 16 : 8;
   else if (w->experts == 1) f.tn = (int)(((rows + (rows + most - 1) / most - 1) / ((rows + most - 1) / most) + 15) / 16 * 16);
   else f.tn = std::min(most, (2 * avg + 15) / 16 * 16);
   f.max_tiles = w->experts == 1 ? (int)((rows + f.tn - 1) / f.tn) : (int)(rows / f.tn + std::min<long long>(w->experts, rows));
-  const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K, tiles = f.max_tiles * mt;
+  const long long tiles = f.max_tiles * mt;
   // CTAs that share a tile's sum: as many as leave all tiles there at once
   f.split = 1;
   for (int s = 2; d && s <= std::min<long long>(8, kt); ++s)

@@ -171,7 +171,8 @@ def check_product(got, x, w, dtype, add=None):
 
 SIZES = [(1, 1, 1), (1, 128, 256), (1, 64, 64), (2, 130, 96), (1, 200, 1024), (3, 17, 33), (5, 300, 520), (8, 128, 2048), (9, 256, 256), (16, 384, 640),
          (17, 129, 257), (31, 128, 512), (33, 500, 1000), (64, 256, 768), (65, 128, 320), (100, 640, 512), (129, 130, 300), (192, 128, 256),
-         (193, 257, 264), (300, 384, 1536), (513, 200, 144)]
+         (193, 257, 264), (300, 384, 1536), (513, 200, 144),
+         (17, 256, 4400), (24, 130, 5000), (32, 2048, 1024), (32, 4300, 2100), (26, 136, 72)]
 
 
 @pytest.mark.parametrize("quantize", [False, True])
