@@ -427,11 +427,8 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
             const uint4 q = *reinterpret_cast<const uint4*>(codes + (((c + u) ^ (r & 7)) << 4));
             const uint32_t words[4] = {q.x, q.y, q.z, q.w};
             uint32_t m0, m1;
-            if constexpr (FMT == GLQB_MX4_MXFP4) m0 = m1 = mx4_multiplier<FMT, T>((sw >> (8 * u)) & 0xFFu, top);
-            else {
-              m0 = mx4_multiplier<FMT, T>((sw >> (16 * u)) & 0xFFu, 0);
-              m1 = mx4_multiplier<FMT, T>((sw >> (16 * u + 8)) & 0xFFu, 0);
-            }
+            if constexpr (FMT == GLQB_MX4_MXFP4) m0 = m1 = mx4_multiplier<T>((sw >> (8 * u)) & 0xFFu, top);
+            else mx4_multipliers<T>((sw >> (16 * u)) & 0xFFFFu, m0, m1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t p[4];

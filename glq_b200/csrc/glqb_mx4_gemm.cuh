@@ -236,18 +236,30 @@ __device__ __forceinline__ void mx4_pairs(uint32_t w, uint32_t (&r)[4]) {
     mx4_pairs_bf16(w, r);
   }
 }
-template <int FMT, typename T>
-__device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {   // in both halves
+// MXFP4: what a block's codes are multiplied by, in both halves
+template <typename T>
+__device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {
+  const int d = (int)s - top;
   uint32_t h;
-  if constexpr (FMT == GLQB_MX4_MXFP4) {
-    const int d = (int)s - top;
-    if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : d > -28 ? (uint32_t)(d + 28) << 10 : d >= -37 ? 1u << (d + 37) : 0u;
-    else h = s == 255u ? 0x7FC0u : (uint32_t)max(d + 253, 0) << 7;
-  } else {
-    if constexpr (__is_same(T, __half)) h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)s, __NV_E4M3).x;
-    else h = __float_as_uint(mx4_e4m3(s) * 0x1p119f) >> 16;
-  }
+  if constexpr (__is_same(T, __half)) h = s == 255u ? 0x7E00u : d > -28 ? (uint32_t)(d + 28) << 10 : d >= -37 ? 1u << (d + 37) : 0u;
+  else h = s == 255u ? 0x7FC0u : (uint32_t)max(d + 253, 0) << 7;
   return h | h << 16;
+}
+// NVFP4: the same of two neighbouring blocks, from their bytes
+template <typename T>
+__device__ __forceinline__ void mx4_multipliers(uint32_t two, uint32_t& m0, uint32_t& m1) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  if constexpr (__is_same(T, __half)) {
+    const uint32_t b = (uint32_t)h.x | (uint32_t)h.y << 16;
+    m0 = __byte_perm(b, 0, 0x1010);
+    m1 = __byte_perm(b, 0, 0x3232);
+  } else {
+    const float2 f = __half22float2(__half2(h));
+    float a = f.x, b = f.y;
+    mx4_mul_f32x2(a, b, 0x1p119f, 0x1p119f);
+    m0 = __byte_perm(__float_as_uint(a), 0, 0x3232);
+    m1 = __byte_perm(__float_as_uint(b), 0, 0x3232);
+  }
 }
 template <typename T>
 __device__ __forceinline__ uint32_t mx4_mul2(uint32_t a, uint32_t b) {
