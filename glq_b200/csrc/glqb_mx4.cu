@@ -69,8 +69,8 @@ template <typename I>
 __device__ __forceinline__ int values_at(const Mx4Rows& q, I c) { return c < (I)q.full ? 16 : c == (I)q.full ? q.rest : 0; }
 
 // ---- largest finite magnitude ---------------------------------------------------------------------
-// A part per CTA; those who need the whole reduce the parts (no atomics, nothing to clear beforehand).
-constexpr int AMAX_PARTS = 296, AMAX_THREADS = 1024;      // (two CTAs on each of 148 SMs)
+// A part per CTA; those who need the whole reduce the parts (no atomics, nothing to clear beforehand).  HBM bound: 88 MB of fp32 in 20 us.
+constexpr int AMAX_PARTS = 296, AMAX_THREADS = 1024;      // (two for each of 148 SMs)
 static_assert(AMAX_PARTS + 1 == GLQB_MX4_SCALE_FLOATS, "");
 template <typename T, typename I>
 __global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* x, Mx4Rows q, Mx4Range range, float* parts) {
@@ -130,7 +130,8 @@ __device__ __forceinline__ float whole_scale(const float* given, float* own_scal
 }
 
 // ---- quantisation ---------------------------------------------------------------------------------
-// HBM bound: 2 or 4 bytes in and 0.53 or 0.56 out per value.
+// 2 or 4 bytes in and 0.53 or 0.56 out per value: 2048 x 14336 bf16 to MXFP4 and back 24.9 us = 6.0 TB/s; to NVFP4 the instructions of
+// the scales and of two conversions per value count as well (5376 x 4100 fp32 25 us of 101 MB).
 template <typename T, int FMT, typename I>
 __global__ void __launch_bounds__(QT_THREADS)
 mx4_quantize_kernel(const T* x, Mx4Rows q, const float* tensor_scale, float* own_scale, int parts, uint8_t* codes,
@@ -356,7 +357,8 @@ __global__ void __launch_bounds__(256) mx4_align_kernel(const uint16_t* x, long 
 // Rows of x in 4 bits, as the tiles the 4-bit product fetches (per token tile, per 256 values: tn rows of 128 bytes with the
 // 128-byte swizzle, then the scales, 128 rows at a time as in the weight image).  A warp takes `batches` times 1024 values of a row
 // (with many rows all of a row: finding its tile takes as long as a thousand values); values past the row are zeros, rows past a
-// tile's are left out (their columns are not stored).
+// tile's are left out (their columns are not stored).  32768 rows of 2048 bf16 values to MXFP4 38 us (170 MB): the instructions around the
+// values bound it, 88 per warp for eight of a lane.  (The next step's values in registers meanwhile: three CTAs per SM for four, 44 us.)
 constexpr int X_TILES = 2 * QT_BATCH;              // of 256 values: what a warp takes at once
 template <typename T, int FMT>
 __global__ void __launch_bounds__(QT_THREADS, 4) mx4_x_image_kernel(const __grid_constant__ Mx4Job J, const float* x_scale, float* own_scale, int parts,
@@ -561,7 +563,7 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
 struct Form {
   int tn, max_tiles, split, pair, x_scales, n_pad;
   bool align, mv;
-  size_t image, bytes;        // of the workspace: x in 4 bits or aligned, then two floats
+  size_t image, bytes;        // of the workspace: x in 4 bits, then the floats of its scale; or x on 16 bytes
 };
 struct Device {
   std::atomic<int> sms{0};
