@@ -99,6 +99,13 @@ def _scale_ptr(t, x, name, count=1):
     return t.data_ptr()
 
 
+def _new(x, lead, cols, dtype):
+    """An empty dense (..., cols) tensor beside x (the two-dimensional case by the call that costs the host least)."""
+    if len(lead) == 1:
+        return torch.empty_strided((lead[0], cols), (cols, 1), dtype=dtype, device=x.device)
+    return x.new_empty(lead + (cols,), dtype=dtype)
+
+
 def _rows(x, cols):
     """x (..., cols) as rows of consecutive values; rows that overlap (an expanded tensor) are copied."""
     x2 = x if x.dim() == 2 else x.reshape(-1, cols)
@@ -120,8 +127,8 @@ def mx4_quantize(x, format="mxfp4", tensor_scale=None) -> Mx4Tensor:
     if not shape:
         raise ValueError("glq_b200: x needs at least one dimension")
     cols, lead, some = shape[-1], shape[:-1], x.numel() > 0
-    codes = x.new_empty(lead + ((cols + 1) // 2,), dtype=torch.uint8)
-    scales = x.new_empty(lead + (-(-cols // _BLOCK[format]),), dtype=torch.uint8)
+    codes = _new(x, lead, (cols + 1) // 2, torch.uint8)
+    scales = _new(x, lead, -(-cols // _BLOCK[format]), torch.uint8)
     given = own = None
     if format == "nvfp4":
         if tensor_scale is None:
@@ -167,7 +174,7 @@ def mx4_dequantize(q: Mx4Tensor, dtype=torch.bfloat16) -> torch.Tensor:
     fmt, rows, cols, count = _checked(q)
     dt = _dtype(dtype, "dtype")
     codes, sc = q.codes.contiguous(), q.scales.contiguous()
-    out = codes.new_empty(codes.shape[:-1] + (cols,), dtype=dtype)
+    out = _new(codes, codes.shape[:-1], cols, dtype)
     if rows and cols:
         _call(codes.get_device(), "mx4_dequantize", _lib.load().glqb_mx4_dequantize, codes.data_ptr(), sc.data_ptr(),
               q.tensor_scale.data_ptr() if count else None, rows // (count or 1), rows, cols, fmt, out.data_ptr(), dt)
@@ -248,7 +255,7 @@ def mx4_linear(x, weight: Mx4Weight, *, quantize_input=False, input_scale=None, 
     x2 = _rows(x, weight.in_features)
     rows = x2.shape[0]
     if accumulate_into is None:
-        out = x.new_empty(shape[:-1] + (m,)) if out_dtype is None else x.new_empty(shape[:-1] + (m,), dtype=out_dtype)
+        out = _new(x, shape[:-1], m, x.dtype if out_dtype is None else out_dtype)
     else:
         out = accumulate_into
         _same_device(out, x, "accumulate_into")
@@ -284,7 +291,7 @@ def mx4_grouped_linear(x, weight: Mx4Weight, offsets, *, quantize_input=False, i
     x2 = _rows(x, weight.in_features)
     fresh = out is None
     if fresh:
-        out = x.new_empty((rows, m)) if out_dtype is None else x.new_empty((rows, m), dtype=out_dtype)
+        out = _new(x, (rows,), m, x.dtype if out_dtype is None else out_dtype)
     else:
         _same_device(out, x, "out")
         if out_dtype not in (None, out.dtype):
