@@ -595,7 +595,7 @@ static const Device* device() {
 constexpr int MV_MAX_ROWS = 16, MV_MAX_EXPERT_ROWS = 8, MV_SMALL_TILES = 256, MV_SMALL_K = 16;
 static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, const void* x, int quantize, const Device* d) {
   Form f = {};
-  const int avg = (int)((rows + w->experts - 1) / w->experts);
+  const int avg = (int)((rows + w->experts - 1) / w->experts);          // (below 2^30: countable)
   const long long mt = (w->m + MX4_ROWS - 1) / MX4_ROWS, kt = (w->n + MX4_K - 1) / MX4_K;
   const bool small = kt <= MV_SMALL_K && mt * kt <= MV_SMALL_TILES;
   f.mv = !quantize && avg <= (w->experts != 1 ? MV_MAX_EXPERT_ROWS : small ? 2 * MV_MAX_ROWS : MV_MAX_ROWS);
@@ -623,8 +623,13 @@ static Form form_of(const GlqbMx4Weight* w, long long rows, long long x_stride, 
   return f;
 }
 
+// (token tiles are counted in 31 bits)
+static bool countable(const GlqbMx4Weight* w, long long rows) { return (rows + w->experts) * ((w->m + MX4_ROWS - 1) / MX4_ROWS) < 1ll << 30; }
+
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize) {
-  if (!w || !format_ok(w->format) || rows <= 0 || rows > MX4_MAX_ROWS || w->experts < 1 || w->m < 1 || w->n < 1) return 0;
+  if (!w || !format_ok(w->format) || rows <= 0 || rows > MX4_MAX_ROWS || w->experts < 1 || w->experts > MX4_MAX_EXPERTS || w->m < 1 ||
+      w->m > MX4_MAX_SIZE || w->n < 1 || w->n > MX4_MAX_SIZE || !countable(w, rows))
+    return 0;
   return form_of(w, rows, x_stride, x, quantize, nullptr).bytes;      // (what a call needs does not depend on the device)
 }
 
@@ -641,7 +646,7 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
   if (!quantize && x_dtype == GLQB_DT_F32) return mx4_fail(GLQB_E_INVALID, "mx4_product: fp32 activations are served quantised only");
   if (rows < 0 || rows > MX4_MAX_ROWS) return mx4_fail(GLQB_E_INVALID, "mx4_product: %lld rows", (long long)rows);
   if (rows == 0) return GLQB_OK;
-  if ((rows + w->experts) * ((w->m + MX4_ROWS - 1) / MX4_ROWS) >= 1ll << 30)       // (tiles are counted in 31 bits)
+  if (!countable(w, rows))
     return mx4_fail(GLQB_E_INVALID, "mx4_product: %lld rows of %d results are too many for one call", (long long)rows, w->m);
   if (!w->image || !x || !y || (w->format == GLQB_MX4_NVFP4 && !w->tensor_scale)) return mx4_fail(GLQB_E_INVALID, "mx4_product: null argument");
   if (rows > 1 && (x_stride < w->n || y_stride < w->m)) return mx4_fail(GLQB_E_INVALID, "mx4_product: rows overlap");

@@ -127,6 +127,10 @@ def test_sizes_beyond_what_is_counted_are_refused(lib):
                                    (_lib.Mx4WeightDesc(p, None, 0, 1, 1 << 20, 64), 1 << 18, None, "too many")):
         rc, said = product(w, rows, offsets)
         assert rc == -1 and text in said, said
+        assert lib.glqb_mx4_workspace_bytes(ctypes.byref(w), rows, 1 << 40, p, 1) == 0
+    two = _lib.Mx4WeightDesc(p, None, 0, 2, 64, 64)
+    assert lib.glqb_mx4_workspace_bytes(ctypes.byref(two), 0x7FFF0000, 64, p, 1) == 0 and product(two, 0x7FFF0000, p)[0] == -1
+    assert lib.glqb_mx4_workspace_bytes(ctypes.byref(two), 1000, 64, p, 1) > 1000 * 32
     for m, n in ((big, 1), (1, big)):
         assert lib.glqb_mx4_pack(p, p, 0, 1, m, n, p, None) == -1
     assert lib.glqb_mx4_pack(p, p, 0, 1025, 8, 8, p, None) == -1 and "1024 experts" in lib.glqb_last_error().decode()
