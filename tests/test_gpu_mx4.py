@@ -406,6 +406,40 @@ def test_calls_on_several_streams_at_once():
             assert all(torch.equal(y, alone[i]) for y in got[i])
 
 
+def test_calls_of_every_form_behind_one_another():
+    """Chained launches of all forms in changing order, on one stream and on three: the bits of each call alone."""
+    g = np.random.default_rng(21)
+    torch.manual_seed(21)
+    sizes = ((512, 1024), (2048, 2048), (1100, 648))
+    weights = {(f, s): ops.mx4_pack(ops.mx4_quantize(torch.randn(s, device="cuda"), f)) for f in FORMATS for s in sizes + ((16, 640, 512),)}
+
+    def job(fmt, quantize, tokens, dtype):
+        if g.random() < 0.3:
+            counts = g.integers(0, max(1, tokens // 8) + 1, 16)
+            off, x = counts_to_offsets(counts), torch.randn(int(counts.sum()) + 2, 512, device="cuda", dtype=dtype)
+            return lambda: ops.mx4_grouped_linear(x, weights[fmt, (16, 640, 512)], off, quantize_input=quantize)
+        m, n = sizes[g.integers(len(sizes))]
+        x = torch.randn(tokens, n, device="cuda", dtype=dtype)
+        return lambda: ops.mx4_linear(x, weights[fmt, (m, n)], quantize_input=quantize)
+
+    jobs = [job(f, q, t, d) for f in FORMATS for q in (False, True) for t in (1, 16, 20, 33, 150, 2100) for d in (torch.bfloat16, torch.float16)]
+    alone = []
+    for j in jobs:
+        alone.append(j())
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(10):
+        got = {int(i): jobs[i]() for i in g.permutation(len(jobs))}
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[i], alone[i]) for i in got)
+        for i in g.permutation(len(jobs)):
+            with torch.cuda.stream(streams[i % 3]):
+                got[int(i)] = jobs[i]()
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[i], alone[i]) for i in got)
+    ops.check_device_status()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_experts_layer_of_a_decoder(fmt):
     """The operators as they are used together: a dense block with residual, then routed experts over sorted rows."""
