@@ -39,18 +39,28 @@ struct Mx4Rows {
   int rest, shift;            // values behind the full ones
 };
 
-// Rows offsets[0] .. offsets[experts] - 1, held to those there are.
+// The rows of the experts: from offsets[0] up to the largest offset, held to those there are.  (mx4_groups counts an offset below one before
+// it as that one: its experts end at the largest, wherever that stands.)
 struct Mx4Range {
   const void* offsets;        // null: all
   int wide, experts;
-  __device__ void get(long long rows, long long& first, long long& last) const {
+  __device__ long long at(int e, long long rows) const {
+    const long long o = wide ? reinterpret_cast<const long long*>(offsets)[e] : reinterpret_cast<const int*>(offsets)[e];
+    return max(0ll, min(rows, o));
+  }
+  // By all threads of a block; tops: a word per warp.  (rows < 2^31)
+  __device__ void get(long long rows, long long& first, long long& last, uint32_t* tops) const {
     first = 0;
     last = rows;
     if (!offsets) return;
-    first = wide ? reinterpret_cast<const long long*>(offsets)[0] : reinterpret_cast<const int*>(offsets)[0];
-    last = wide ? reinterpret_cast<const long long*>(offsets)[experts] : reinterpret_cast<const int*>(offsets)[experts];
-    first = max(0ll, min(rows, first));
-    last = max(0ll, min(rows, last));
+    uint32_t top = 0;
+    for (int e = threadIdx.x; e <= experts; e += blockDim.x) top = max(top, (uint32_t)at(e, rows));
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    last = __reduce_max_sync(0xFFFFFFFFu, (threadIdx.x & 31) < blockDim.x / 32 ? tops[threadIdx.x & 31] : 0u);
+    first = at(0, rows);
+    __syncthreads();          // (tops is used again)
   }
 };
 
@@ -76,9 +86,10 @@ template <typename T, typename I>
 __global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* x, Mx4Rows q, Mx4Range range, float* parts) {
   pdl_wait();
   pdl_trigger();
+  __shared__ uint32_t tops[AMAX_THREADS / 32];
   uint32_t top = 0;
   long long first, last;
-  range.get(q.rows, first, last);
+  range.get(q.rows, first, last, tops);
   const I end = (I)(last * q.chunks), step = (I)gridDim.x * AMAX_THREADS;
   for (I b = (I)(first * q.chunks) + (I)blockIdx.x * AMAX_THREADS + threadIdx.x; b < end; b += step * QT_BATCH) {
     Mx4Raw<T> raw[QT_BATCH];
@@ -105,7 +116,6 @@ __global__ void __launch_bounds__(AMAX_THREADS) mx4_amax_kernel(const T* x, Mx4R
     }
   }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
-  __shared__ uint32_t tops[AMAX_THREADS / 32];
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
   __syncthreads();
   if (threadIdx.x < 32) {

@@ -277,8 +277,8 @@ def mx4_grouped_linear(x, weight: Mx4Weight, offsets, *, quantize_input=False, i
     rows per expert, none included; nothing is read back.  Rows of no expert (in front of offsets[0], behind offsets[experts])
     are zero in a new result and stay as they are in a given ``out`` (rows, m), whose rows may lie apart.  Offsets outside
     0 .. rows are held to that range, and one that is less than the one before it counts as that one.  At most 1024 experts.
-    The other arguments as for ``mx4_linear``; "nvfp4" inputs without ``input_scale`` take the scale of rows
-    offsets[0] .. offsets[experts] - 1."""
+    The other arguments as for ``mx4_linear``; "nvfp4" inputs without ``input_scale`` take the scale of the
+    experts' rows (offsets[0] up to the largest offset, held to 0 .. rows)."""
     dt, xs = _input(x, weight, quantize_input, input_scale)
     if weight.experts is None:
         raise ValueError("glq_b200: mx4_grouped_linear takes one matrix per expert")

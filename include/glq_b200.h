@@ -330,7 +330,7 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
  * ascend; they are read on the device, where each is held to 0 .. rows and to no less than the one before it.  Rows of no expert
  * keep what y holds, or are zeroed with clear_rest.  At most 1024 experts.
  * quantize: x is brought to the weights' format first, as glqb_mx4_quantize does (NVFP4: by *x_scale, or, with x_scale NULL, by the
- * scale of rows offsets[0] .. offsets[experts] - 1), and 4-bit values are multiplied.  Without it x is fp16 or bf16 and stays so.
+ * scale of the experts' rows, offsets[0] up to the largest offset), and 4-bit values are multiplied.  Without it x is fp16 or bf16 and stays so.
  * Under 16-bit activations MXFP4 weights are multiplied relative to the largest scale of their row: a block whose scale lies more
  * than 2^36 below it may lose bits; few bf16 rows are multiplied as fp16 under a power of two per 256 values (exact from 2^-32 of the
  * largest of them on).  m and n up to 2^30, rows up to 2^31 - 2^16, (rows + experts) * ceil(m / 128) below 2^30.

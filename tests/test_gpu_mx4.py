@@ -771,3 +771,28 @@ def test_refusals():
     own = ops.mx4_pack(ops.mx4_quantize(x, "nvfp4", scale))
     scale.fill_(2.0)
     assert own.tensor_scale.item() == 0.5
+
+
+# ---- offsets out of order, and the scale of 4-bit activations ------------------------------------------------------
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+@pytest.mark.parametrize("off", [[0, 20, 60, 50], [5, 60, 10, 0], [0, 0, 40, -3], [70, 10, 20, 30], [0, 30, 45, 60], [9, 9, 9, 9]])
+def test_scale_of_grouped_inputs_is_that_of_the_rows_multiplied(off, wide):
+    """An offset below one before it counts as that one: rows behind the last offset as it is written are some expert's, and the
+    largest values among them set the scale.  Rows of no expert do not."""
+    g = np.random.default_rng(14)
+    weight, w = make_weight(g, (3, 144, 160), "nvfp4")
+    xh = g.standard_normal((64, 160))
+    edge = np.maximum.accumulate(np.clip(off, 0, 64))
+    xh[edge[-1]:] = 1e3                                           # of no expert
+    xh[:edge[0]] = -1e3
+    if edge[-1] > edge[0]:
+        xh[edge[-1] - 1, 7] = 60.0
+    x = to_cuda(xh, torch.bfloat16)
+    y = ops.mx4_grouped_linear(x, weight, torch.tensor(off, dtype=wide, device="cuda"), quantize_input=True)
+    assert not y[:edge[0]].any() and not y[edge[-1]:].any()
+    if edge[-1] == edge[0]:
+        return
+    xv = quantized_values(host(x)[edge[0]:edge[-1]], "nvfp4")
+    for e in range(3):
+        if edge[e] < edge[e + 1]:
+            check_product(y[edge[e]:edge[e + 1]], xv[edge[e] - edge[0]:edge[e + 1] - edge[0]], w[e], torch.bfloat16)
