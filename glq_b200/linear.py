@@ -7,6 +7,8 @@ calls by name.  There is no CPU path: on a CPU tensor ``forward`` raises.
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 import torch.nn as nn
 
@@ -181,6 +183,9 @@ class GLQLinear(nn.Module):
                 f"m_pad={self.m_pad}, n_pad={self.n_pad}, trellis={self._is_trellis}")
 
 
+_PACKING = threading.Lock()          # of layers of 4-bit weights: one host thread at a time
+
+
 class Mx4Linear(nn.Module):
     """A linear layer whose weight is held in microscaled 4-bit floating point ("mxfp4" or "nvfp4"), as checkpoints store it:
     ``codes`` (out, ceil(in / 2)) and ``scales`` (out, ceil(in / block)) uint8, for "nvfp4" ``tensor_scale`` (fp32, one), ``bias``.
@@ -205,7 +210,7 @@ class Mx4Linear(nn.Module):
             self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32))
         else:
             self.bias = None
-        self._packed = None           # (what the stored rows were when they were packed, the packed weight)
+        self._packed = None           # (versions of the stored rows when they were packed, the rows, the packed weight, the stream)
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, bias=None, format: str = "mxfp4", quantize_input: bool = False) -> "Mx4Linear":
@@ -228,7 +233,7 @@ class Mx4Linear(nn.Module):
             now = getattr(self, name)
             if now.dtype != torch.float32:
                 setattr(self, name, t.to(now.device))
-        self._packed = None
+        self._let_go()
         return self
 
     def __getstate__(self):
@@ -239,23 +244,52 @@ class Mx4Linear(nn.Module):
 
     @property
     def weight(self) -> "ops.Mx4Weight":
-        """The packed weight (``ops.mx4_pack``).  Buffers created under inference mode do not count their changes: after writing to
-        one in place, call ``repack``."""
+        """The packed weight (``ops.mx4_pack``), complete: the host has waited for the stream that packed it, so that any stream may
+        read it.  Buffers created under inference mode do not count their changes: after writing to one in place, call ``repack``."""
+        return self._ready()[2]
+
+    def _ready(self):
         held = [t for t in (self.codes, self.scales, self.tensor_scale) if t is not None]
         now = [0 if t.is_inference() else t._version for t in held]
-        if self._packed is None or self._packed[0] != now or any(a is not b for a, b in zip(self._packed[1], held)):
+
+        def current(packed):
+            return packed is not None and packed[0] == now and all(a is b for a, b in zip(packed[1], held))
+
+        packed = self._packed
+        if current(packed):
+            return packed
+        with _PACKING, torch.cuda.device(self.codes.get_device()):
+            if current(self._packed):             # (by another thread meanwhile)
+                return self._packed
             if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("glq_b200: the weight is packed at the first forward: run one before capturing a graph")
-            self._packed = (now, held, ops.mx4_pack(self._rows()))
-        return self._packed[2]
+            self._let_go()
+            weight = ops.mx4_pack(self._rows())
+            stream = torch.cuda.current_stream()
+            stream.synchronize()
+            self._packed = packed = (now, held, weight, stream.cuda_stream)
+        return packed
+
+    def _let_go(self) -> None:
+        """Drops the packed weight, behind whatever still reads it: its memory belongs to the stream that packed it, not to those."""
+        if self._packed is not None:
+            torch.cuda.synchronize(self._packed[2].image.device)
+            self._packed = None
 
     def repack(self) -> None:
-        self._packed = None
+        self._let_go()
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:
             raise RuntimeError("glq_b200.Mx4Linear has no CPU path")
-        y = ops.mx4_linear(x, self.weight, quantize_input=self.quantize_input)
+        _, _, w, packed_on = self._ready()
+        y = ops.mx4_linear(x, w, quantize_input=self.quantize_input)
+        if ops._stream(x) != packed_on and not torch.cuda.is_current_stream_capturing():
+            # (the layer may go while another stream than the packing one has yet to read the weight)
+            stream = torch.cuda.current_stream(x.device)
+            for t in (w.image, w.tensor_scale):
+                if t is not None:
+                    t.record_stream(stream)
         return y if self.bias is None else y + self.bias.to(y.dtype)
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:

@@ -796,3 +796,63 @@ def test_scale_of_grouped_inputs_is_that_of_the_rows_multiplied(off, wide):
     for e in range(3):
         if edge[e] < edge[e + 1]:
             check_product(y[edge[e]:edge[e + 1]], xv[edge[e] - edge[0]:edge[e + 1] - edge[0]], w[e], torch.bfloat16)
+
+
+# ---- the layer on several streams ------------------------------------------------------------------------------------
+DELAY = 40_000_000                  # clocks that a stream is kept busy: some 20 ms
+
+
+def layers_and_input(fmt="mxfp4", seed=15):
+    """Two layers of the same sizes and their results for x, each alone."""
+    from glq_b200.linear import Mx4Linear
+    g = np.random.default_rng(seed)
+    layers = [Mx4Linear.from_weight(to_cuda(g.standard_normal((1024, 2048)) / 45), None, fmt) for _ in range(2)]
+    x = to_cuda(g.standard_normal((20, 2048)), torch.bfloat16)
+    want = [ops.mx4_linear(x, ops.mx4_pack(layer._rows())) for layer in layers]
+    torch.cuda.synchronize()
+    assert not torch.equal(*want)
+    return layers, x, want
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_layer_packed_on_one_stream_and_read_on_another(fmt):
+    (layer, other), x, want = layers_and_input(fmt)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(DELAY)
+        ya = layer(x)
+    with torch.cuda.stream(b):
+        yb = layer(x)
+    torch.cuda.synchronize()
+    assert torch.equal(ya, want[0]) and torch.equal(yb, want[0])
+    # b is late: what it reads must still be there after the layer has been packed again, and after it has gone
+    for change in (lambda: layer.load_state_dict(other.state_dict()), lambda: layer.codes.copy_(other.codes), layer.half, layer.repack):
+        layer.load_state_dict(layers_and_input(fmt)[0][0].state_dict())
+        layer(x)
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(DELAY)
+            yb = layer(x)
+        with torch.cuda.stream(a):
+            change()
+            ya = layer(x)
+            junk = torch.full_like(layer.weight.image, 0x55)
+        torch.cuda.synchronize()
+        assert torch.equal(yb, want[0])
+        assert torch.equal(ya, ops.mx4_linear(x, ops.mx4_pack(layer._rows())))
+        del junk
+
+
+def test_layer_that_goes_while_another_stream_reads_it():
+    (layer, _), x, want = layers_and_input()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        size = layer.weight.image.numel()
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(DELAY)
+        y = layer(x)
+    del layer
+    with torch.cuda.stream(a):
+        junk = [torch.full((size,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[0])
+    del junk

@@ -152,3 +152,29 @@ def test_layer_of_4_bit_weights_on_the_host():
         layer(torch.zeros(1, 50))
     with pytest.raises(ValueError, match="mxfp4"):
         Mx4Linear(8, 8, format="fp4")
+
+
+def test_layer_waits_for_its_packing_and_for_its_readers(monkeypatch):
+    """Whoever is given the packed weight finds it complete, whatever stream they run on; a weight that is packed again goes when nothing
+    reads it any more.  (The order of the host's calls, without a GPU.)"""
+    import contextlib
+    import types
+    from glq_b200 import linear
+    calls = []
+
+    def pack(rows, out=None):
+        calls.append("pack")
+        return types.SimpleNamespace(image=types.SimpleNamespace(device="device"), tensor_scale=None)
+
+    monkeypatch.setattr(linear.ops, "mx4_pack", pack)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: types.SimpleNamespace(synchronize=lambda: calls.append("wait"), cuda_stream=7))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: calls.append("all"))
+    layer = linear.Mx4Linear(64, 8)
+    first = layer.weight
+    assert calls == ["pack", "wait"] and layer.weight is first and calls == ["pack", "wait"]
+    for change in (lambda: layer.codes.add_(1), layer.half, layer.repack, lambda: layer.load_state_dict(layer.state_dict())):
+        calls.clear()
+        change()
+        assert layer.weight is not None
+        assert calls == ["all", "pack", "wait"], calls
