@@ -210,7 +210,7 @@ class Mx4Linear(nn.Module):
             self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32))
         else:
             self.bias = None
-        self._packed = None           # (versions of the stored rows when they were packed, the rows, the packed weight, the stream)
+        self._packed = None           # (versions of the stored rows when they were packed, the rows, the packed weight, its memory's stream)
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, bias=None, format: str = "mxfp4", quantize_input: bool = False) -> "Mx4Linear":
@@ -233,7 +233,10 @@ class Mx4Linear(nn.Module):
             now = getattr(self, name)
             if now.dtype != torch.float32:
                 setattr(self, name, t.to(now.device))
-        self._let_go()
+        if self._packed is not None and self._packed[2].image.device != self.codes.device:
+            torch.cuda.synchronize(self._packed[2].image.device)      # (its readers' streams are not the one its memory goes back to)
+            self._packed = None
+        self.repack()
         return self
 
     def __getstate__(self):
@@ -245,7 +248,8 @@ class Mx4Linear(nn.Module):
     @property
     def weight(self) -> "ops.Mx4Weight":
         """The packed weight (``ops.mx4_pack``), complete: the host has waited for the stream that packed it, so that any stream may
-        read it.  Buffers created under inference mode do not count their changes: after writing to one in place, call ``repack``."""
+        read it.  Packed again it keeps its memory, so that captured graphs go on with the new weights; a layer that went to another
+        device has a new one, and has to be captured again.  Buffers created under inference mode do not count their changes: after writing to one in place, call ``repack``."""
         return self._ready()[2]
 
     def _ready(self):
@@ -263,21 +267,21 @@ class Mx4Linear(nn.Module):
                 return self._packed
             if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("glq_b200: the weight is packed at the first forward: run one before capturing a graph")
-            self._let_go()
-            weight = ops.mx4_pack(self._rows())
-            stream = torch.cuda.current_stream()
+            rows, stream, before = self._rows(), torch.cuda.current_stream(), self._packed
+            weight, packed_on = None, stream.cuda_stream
+            if before is not None:                # the same memory takes the new weights, behind whatever reads the old ones
+                torch.cuda.synchronize(before[2].image.device)
+                if before[2].image.device == self.codes.device and before[2]._holds(rows):
+                    weight, packed_on = before[2:]
+            weight = ops.mx4_pack(rows, out=weight)
             stream.synchronize()
-            self._packed = packed = (now, held, weight, stream.cuda_stream)
+            self._packed = packed = (now, held, weight, packed_on)
         return packed
 
-    def _let_go(self) -> None:
-        """Drops the packed weight, behind whatever still reads it: its memory belongs to the stream that packed it, not to those."""
-        if self._packed is not None:
-            torch.cuda.synchronize(self._packed[2].image.device)
-            self._packed = None
-
     def repack(self) -> None:
-        self._let_go()
+        """The next forward packs the stored rows again."""
+        if self._packed is not None:
+            self._packed = (None, ()) + self._packed[2:]
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:

@@ -36,7 +36,7 @@ class Mx4Tensor(NamedTuple):
 
 class Mx4Weight:
     """Weights laid out for the products (``mx4_pack``): (out_features, in_features), or one such matrix per expert.  The
-    attributes cannot be set (a new image, or one on another device, is a new weight)."""
+    attributes cannot be set (a new image, or one on another device, is a new weight; ``mx4_pack(..., out=)`` fills the same one)."""
     __slots__ = ("image", "tensor_scale", "format", "experts", "out_features", "in_features", "_desc", "_ref", "_index")
 
     def __init__(self, image, tensor_scale, format, experts, out_features, in_features):
@@ -48,6 +48,11 @@ class Mx4Weight:
 
     def __setattr__(self, name, value):
         raise AttributeError(f"glq_b200: {name} of a packed weight cannot be set")
+
+    def _holds(self, q: Mx4Tensor) -> bool:
+        """Are q's rows of these sizes, format and device?"""
+        lead = (self.out_features,) if self.experts is None else (self.experts, self.out_features)
+        return (self.format, self.in_features, self._index, lead) == (q.format, q.cols, q.codes.get_device(), tuple(q.codes.shape[:-1]))
 
 
 _get_device, _set_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_setDevice, torch._C._cuda_getCurrentRawStream
@@ -181,23 +186,32 @@ def mx4_dequantize(q: Mx4Tensor, dtype=torch.bfloat16) -> torch.Tensor:
     return out
 
 
-def mx4_pack(q: Mx4Tensor) -> Mx4Weight:
+def mx4_pack(q: Mx4Tensor, out: Optional[Mx4Weight] = None) -> Mx4Weight:
     """Weights (m, n), or (experts, m, n), laid out for ``mx4_linear`` / ``mx4_grouped_linear``: once, when they are loaded.
-    The image has the size of codes and scales, rows rounded up to 128 and values to 256."""
+    The image has the size of codes and scales, rows rounded up to 128 and values to 256.  ``out``: a packed weight of the same
+    sizes, format and device, whose memory takes these weights in place of its own (captured graphs that read it then multiply by
+    them); what still reads it on another stream has to be waited for first."""
     fmt, rows, n, scales = _checked(q)
     if q.codes.dim() not in (2, 3):
         raise ValueError(f"glq_b200: weights are (m, n) or (experts, m, n), got codes of {tuple(q.codes.shape)}")
     experts, m = (q.codes.shape[0] if q.codes.dim() == 3 else None), q.codes.shape[-2]
     if rows == 0 or n == 0:
         raise ValueError(f"glq_b200: empty weights, codes of {tuple(q.codes.shape)}")
+    if out is not None and (out.__class__ is not Mx4Weight or not out._holds(q)):
+        raise ValueError(f"glq_b200: out is a packed {q.format} weight of {tuple(q.codes.shape[:-1]) + (n,)} on {q.codes.device}")
     codes, sc = q.codes.contiguous(), q.scales.contiguous()
     lib = _lib.load()
-    image = codes.new_empty((lib.glqb_mx4_image_bytes(fmt, experts or 1, m, n),))
+    image = codes.new_empty((lib.glqb_mx4_image_bytes(fmt, experts or 1, m, n),)) if out is None else out.image
     _call(codes.get_device(), "mx4_pack", lib.glqb_mx4_pack, codes.data_ptr(), sc.data_ptr(), fmt, experts or 1, m, n, image.data_ptr())
     t = q.tensor_scale
     if scales:
-        t = t.reshape(-1).expand(experts or 1).clone(memory_format=torch.contiguous_format)
-    return Mx4Weight(image, t, q.format, experts, m, n)
+        t = t.reshape(-1).expand(experts or 1)
+        if out is None:
+            t = t.clone(memory_format=torch.contiguous_format)
+        else:
+            with torch.inference_mode():          # (the weight's may have been made under it)
+                out.tensor_scale.copy_(t)
+    return Mx4Weight(image, t, q.format, experts, m, n) if out is None else out
 
 
 def _overlap(a, b):

@@ -856,3 +856,53 @@ def test_layer_that_goes_while_another_stream_reads_it():
     torch.cuda.synchronize()
     assert torch.equal(y, want[0])
     del junk
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_captured_layer_whose_weights_change(fmt):
+    """A graph goes on with the memory that it was captured with: the layer's weight of the day, packed by a forward or by `weight`."""
+    (layer, other), x, want = layers_and_input(fmt)
+    layer(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer(x)
+    held, at = layer.weight, layer.weight.image.data_ptr()
+    stored = {k: v.clone() for k, v in layer.state_dict().items()}
+    for state, right in ((other.state_dict(), want[1]), (stored, want[0]), (other.state_dict(), want[1])):
+        layer.load_state_dict(state)
+        assert torch.equal(layer(x), right)
+        assert layer.weight is held and held.image.data_ptr() == at
+        junk = torch.full_like(held.image, 0x55)
+        graph.replay()
+        assert torch.equal(y, right)
+        del junk
+    with torch.inference_mode():
+        layer.load_state_dict(stored)
+        layer.repack()
+        assert torch.equal(layer(x), want[0])
+    graph.replay()
+    assert layer.weight is held and torch.equal(y, want[0])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("experts", [None, 3])
+def test_packing_into_a_packed_weight(fmt, experts):
+    g = np.random.default_rng(17)
+    shape = (150, 328) if experts is None else (experts, 150, 328)
+
+    def stored():
+        q = ops.mx4_quantize(to_cuda(g.standard_normal(shape)), fmt)
+        return q if fmt == "mxfp4" or experts is None else q._replace(tensor_scale=torch.rand(experts, device="cuda"))
+
+    q, q2 = stored(), stored()
+    w, image = ops.mx4_pack(q), ops.mx4_pack(q2).image
+    at = w.image
+    assert ops.mx4_pack(q2, out=w) is w and w.image is at and torch.equal(at, image)
+    if fmt == "nvfp4":
+        assert torch.equal(w.tensor_scale, q2.tensor_scale.reshape(-1))
+    for bad in (q._replace(codes=q.codes[..., :149, :], scales=q.scales[..., :149, :]), ops.mx4_quantize(to_cuda(g.standard_normal((150, 320))), fmt),
+                ops.mx4_quantize(to_cuda(g.standard_normal(shape)), "nvfp4" if fmt == "mxfp4" else "mxfp4")):
+        with pytest.raises(ValueError, match="out is a packed"):
+            ops.mx4_pack(bad, out=w)
+    with pytest.raises(ValueError, match="out is a packed"):
+        ops.mx4_pack(q, out=w.image)

@@ -178,3 +178,28 @@ def test_layer_waits_for_its_packing_and_for_its_readers(monkeypatch):
         change()
         assert layer.weight is not None
         assert calls == ["all", "pack", "wait"], calls
+
+
+def test_layer_keeps_the_memory_of_its_packed_weight(monkeypatch):
+    """A captured graph holds the address of the packed weight: packed again, a layer offers the old one's memory, unless it has
+    gone to another device.  (The host's calls, without a GPU.)"""
+    import contextlib
+    import types
+    from glq_b200 import linear
+    offered = []
+
+    def pack(rows, out=None):
+        offered.append(out)
+        return out or types.SimpleNamespace(image=types.SimpleNamespace(device=rows.codes.device), tensor_scale=None, _holds=lambda rows: rows.cols == 64)
+
+    monkeypatch.setattr(linear.ops, "mx4_pack", pack)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: types.SimpleNamespace(synchronize=lambda: None, cuda_stream=7))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    layer = linear.Mx4Linear(64, 8)
+    first = layer.weight
+    for change in (lambda: layer.codes.add_(1), layer.half, layer.repack, lambda: layer.load_state_dict(layer.state_dict(), assign=True)):
+        change()
+        assert layer.weight is first and offered[-1] is first
+    layer.to("meta")
+    assert layer.weight is not first and offered[-1] is None
