@@ -189,7 +189,8 @@ _PACKING = threading.Lock()          # of layers of 4-bit weights: one host thre
 class Mx4Linear(nn.Module):
     """A linear layer whose weight is held in microscaled 4-bit floating point ("mxfp4" or "nvfp4"), as checkpoints store it:
     ``codes`` (out, ceil(in / 2)) and ``scales`` (out, ceil(in / block)) uint8, for "nvfp4" ``tensor_scale`` (fp32, one), ``bias``.
-    They are laid out for the products (``weight``) at the first forward, and again after they were loaded, moved or written.
+    They are laid out for the products (``weight``) at the first forward, and again after they were loaded, moved or written in
+    place (through ``buffer.data``: call ``repack``).
     ``quantize_input``: activations are brought to the format as well and 4-bit values are multiplied.  No counterpart in the
     reference.  There is no CPU path: on a CPU tensor ``forward`` raises."""
 
@@ -249,7 +250,9 @@ class Mx4Linear(nn.Module):
     def weight(self) -> "ops.Mx4Weight":
         """The packed weight (``ops.mx4_pack``), complete: the host has waited for the stream that packed it, so that any stream may
         read it.  Packed again it keeps its memory, so that captured graphs go on with the new weights; a layer that went to another
-        device has a new one, and has to be captured again.  Buffers created under inference mode do not count their changes: after writing to one in place, call ``repack``."""
+        device has a new one, and has to be captured again.  Changes are seen by the buffers' version counters, which do not count
+        writes through ``buffer.data`` (or memory shared with another library), nor any to buffers created under inference mode:
+        after such a write, call ``repack``, or the layer goes on with the weights that it has."""
         return self._ready()[2]
 
     def _ready(self):

@@ -906,3 +906,18 @@ def test_packing_into_a_packed_weight(fmt, experts):
             ops.mx4_pack(bad, out=w)
     with pytest.raises(ValueError, match="out is a packed"):
         ops.mx4_pack(q, out=w.image)
+
+
+def test_writes_that_move_no_version_counter_are_seen_after_repack():
+    (layer, other), x, want = layers_and_input()
+    layer(x)
+    layer.codes.data.copy_(other.codes)
+    layer.scales.data.copy_(other.scales)
+    layer.repack()
+    assert torch.equal(layer(x), want[1])
+    with torch.inference_mode():
+        layer.codes, layer.scales = layer.codes.clone(), layer.scales.clone()
+        assert torch.equal(layer(x), want[1])
+        layer.codes.zero_()
+        layer.repack()
+        assert not layer(x).any()
