@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
   bool ok = true;
 
   if (warp == 0) {
-    if (!PAIR || rank == 0) {
+    if ((!PAIR || rank == 0) && elect_one()) {
       Mx4Pos a, x, acc;
       const uint32_t x0 = smem_u32(x_base);
       for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
@@ -347,21 +347,18 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
         for (int k = 0; k < steps; ++k, a.add(1, R.a_stages), x.add(1, R.x_stages)) {
           if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) || !mbar_wait(&B.full_a[a.s], a.phase, &B.abort)) { ok = false; break; }
           tc_fence_after();
-          if (elect_one()) {
-            const uint32_t at = tmem_a + a.s * 64u, b = x0 + x.s * 2u * R.x_half;
-            const uint64_t d0 = umma_desc_sw128(b), d1 = umma_desc_sw128(b + R.x_half);
+          const uint32_t at = tmem_a + a.s * 64u, b = x0 + x.s * 2u * R.x_half;
+          const uint64_t d0 = umma_desc_sw128(b), d1 = umma_desc_sw128(b + R.x_half);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) umma16<PAIR>(d, at + 8u * j, d0 + 2u * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
+          for (int j = 0; j < 4; ++j) umma16<PAIR>(d, at + 8u * j, d0 + 2u * j, idesc, (k > 0 || j > 0) ? 1u : 0u);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) umma16<PAIR>(d, at + 32u + 8u * j, d1 + 2u * j, idesc, 1u);
-            commit<PAIR>(&B.empty_x[x.s]);
-            commit<PAIR>(&B.empty_a[a.s]);
-            if (k + 1 == steps) commit<PAIR>(&B.acc_full[acc.s]);
-          }
-          __syncwarp();
+          for (int j = 0; j < 4; ++j) umma16<PAIR>(d, at + 32u + 8u * j, d1 + 2u * j, idesc, 1u);
+          commit<PAIR>(&B.empty_x[x.s]);
+          commit<PAIR>(&B.empty_a[a.s]);
+          if (k + 1 == steps) commit<PAIR>(&B.acc_full[acc.s]);
         }
       }
-      if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
+      if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
     }
   } else if (warp == 1) {
     // (a box per lane: one thread that issues them in turn is late among the warps that decode)
@@ -371,7 +368,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       const int rows = PAIR ? cols_of(t) / 2 : t.rows, row0 = t.row0 + (PAIR ? rank * rows : 0), boxes = (rows + R.box_rows - 1) / R.box_rows;
       const int box = lane >> 1, half = lane & 1, to = half * R.x_half + box * R.box_rows * 128;
       for (int k = 0; k < steps; ++k, ++loads_x, x.add(1, R.x_stages)) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&B.empty_x[x.s], x.phase ^ 1u, &B.abort));
+        ok = mbar_wait_warp(&B.empty_x[x.s], x.phase ^ 1u, &B.abort);
         if (!ok) break;
         if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(&B.full_x[x.s], (uint32_t)((PAIR ? 4 : 2) * boxes * R.box_rows * 128));
         __syncwarp();
@@ -405,15 +402,18 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     // of a group's eight warps four take the first 64 values of a step, four the others; a warp the 32 rows of its quarter of tensor memory
     const int group = (warp - 8) >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t to = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + half * 32u;
+    // (A lane whose wait gave up goes on with what lies there, here and where results are drained, to the last tile: the instructions behind
+    // the wait are the whole warp's, and it can leave neither alone nor, without a vote, with the others.  32768 rows over 128 experts of 2048
+    // x 768: 121.5 us; with a vote per wait 123.4, with one per tile 122.9.  The other waits end at their next look at `abort`.)
     Mx4Pos a, w;
     a.add(group, R.a_stages);
-    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L)) {
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more(); t.next(L)) {
       int top = 0;
       if constexpr (FMT == GLQB_MX4_MXFP4) {
         top = J.tops[((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * MX4_ROWS + r] & 0xFF;
       }
       for (int k = group; k < steps + group; k += 2, w.add(1, G16_W_STAGES)) {
-        if (!mbar_wait(&B.full_w[w.s], w.phase, &B.abort)) { ok = false; break; }
+        if (!mbar_wait(&B.full_w[w.s], w.phase, &B.abort)) { ok = false; B.abort = 1; }
         const uint8_t* tile = w_base + w.s * TILE;
         uint32_t v[32];
         if (k < steps) {
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
         __syncwarp();
         if (lane == 0) mbar_arrive(&B.empty_w[w.s]);
         if (k < steps) {
-          if (!mbar_wait(&B.empty_a[a.s], a.phase ^ 1u, &B.abort)) { ok = false; break; }
+          if (!mbar_wait(&B.empty_a[a.s], a.phase ^ 1u, &B.abort)) { ok = false; B.abort = 1; }
           __syncwarp();
           tc_fence_after();
           tmem_st32(to + a.s * 64u, v);
@@ -463,11 +463,11 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     pdl_wait();                                    // (y may still be in use)
     mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
     Mx4Pos acc;
-    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more(); t.next(L), acc.add(1, 2)) {
       const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
       Mx4Factor f{1.0f, 1.0f};
       if (row < J.m) f = row_factor<FMT, T, false>(J, t.expert, row);
-      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; break; }
+      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; B.abort = 1; }
       __syncwarp();
       tc_fence_after();
       if (!PAIR || mt < J.m_tiles)
@@ -566,17 +566,17 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
   bool ok = true;
 
   if (warp == 0) {
-    Mx4Pos x, acc;
     if (!PAIR || rank == 0) {
-      for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
-        const int cols = (t.rows + 15) & ~15;
-        const uint32_t d = tmem + acc.s * C::MAX_TN;
-        if (!mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort)) { ok = false; break; }
-        tc_fence_after();
-        for (int k = 0; k < steps; ++k, x.add(1, stages)) {
-          if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) || (PAIR && !mbar_wait(&B.full_w[x.s], x.phase, &B.abort))) { ok = false; break; }
+      if (elect_one()) {
+        Mx4Pos x, acc;
+        for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
+          const int cols = (t.rows + 15) & ~15;
+          const uint32_t d = tmem + acc.s * C::MAX_TN;
+          if (!mbar_wait(&B.acc_empty[acc.s], acc.phase ^ 1u, &B.abort)) { ok = false; break; }
           tc_fence_after();
-          if (elect_one()) {
+          for (int k = 0; k < steps; ++k, x.add(1, stages)) {
+            if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort) || (PAIR && !mbar_wait(&B.full_w[x.s], x.phase, &B.abort))) { ok = false; break; }
+            tc_fence_after();
             const uint32_t w = smem_u32(base) + x.s * stage_bytes, xs = w + TILE, sc = xs + (own + 7) / 8 * 1024;
             const uint32_t sa = tmem + 2 * C::MAX_TN + x.s * C::SF_COLS, sb = sa + 4 * C::ATOMS;
             const uint64_t dws = scale_desc(w + MX4_CODE_BYTES), dxs = scale_desc(sc);
@@ -596,11 +596,11 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
             commit<PAIR>(&B.empty_x[x.s]);
             if (k + 1 == steps) commit<PAIR>(&B.acc_full[acc.s]);
           }
-          __syncwarp();
         }
+        if (!ok) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
       }
-      if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
     } else if (lane == 0) {
+      Mx4Pos x;
       for (int i = first; i < tiles && ok; i += step)
         for (int k = 0; k < steps; ++k, x.add(1, stages)) {
           if (!mbar_wait(&B.full_x[x.s], x.phase, &B.abort)) { ok = false; break; }
@@ -642,11 +642,11 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
     pdl_wait();                                    // (y may still be in use)
     mx4_clear_rest(J, L.eff, threadIdx.x - 128, 128);
     Mx4Pos acc;
-    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more() && ok; t.next(L), acc.add(1, 2)) {
+    for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more(); t.next(L), acc.add(1, 2)) {
       const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
       Mx4Factor f{1.0f, 1.0f};
       if (row < J.m) f = row_factor<FMT, __half, true>(J, t.expert, row);
-      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; break; }
+      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; B.abort = 1; }
       __syncwarp();
       tc_fence_after();
       if (!PAIR || mt < J.m_tiles)

@@ -1,6 +1,7 @@
 """Microscaled 4-bit floating point without a GPU: the oracle against itself, the ABI's structure, the refusals."""
 import ctypes
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -203,3 +204,46 @@ def test_layer_keeps_the_memory_of_its_packed_weight(monkeypatch):
         assert layer.weight is first and offered[-1] is first
     layer.to("meta")
     assert layer.weight is not first and offered[-1] is None
+
+
+def _source(name):
+    """C++ source without comments, and without the semicolons of loop heads and strings in calls."""
+    with open(os.path.join(ROOT, "glq_b200", "csrc", name)) as f:
+        text, depth, out = "\n".join(line.split("//")[0] for line in f.read().split("\n")), 0, []
+    for c in text:
+        depth += (c == "(") - (c == ")")
+        out.append(" " if c == ";" and depth else c)
+    return "".join(out)
+
+
+def _blocks_around(text, at):
+    """What stands in front of every brace that is open at a place of C++ source: the conditions and loops it is under."""
+    heads, depth = [], 0
+    for i in range(at, -1, -1):
+        if text[i] == "}":
+            depth += 1
+        elif text[i] == "{":
+            if depth:
+                depth -= 1
+            else:
+                start = max(text.rfind(c, 0, i) for c in ";{}")
+                heads.append(text[start + 1:i])
+    return heads
+
+
+def test_whole_warps_wait_with_one_outcome():
+    """A bounded wait gives up lane by lane.  Where it is a warp's, whose lanes go on to votes and matrix instructions together, either
+    its outcome is one for all of them, or no lane leaves its place by it; a wait that ends a loop is for blocks that a single lane runs."""
+    seen = 0
+    for name in ("glqb_mx4_gemm.cu", "glqb_mx4_mv.cu"):
+        text = _source(name)
+        at = text.find("mbar_wait(")
+        while at >= 0:
+            start = max(text.rfind(c, 0, at) for c in ";{}")
+            heads = [text[start + 1:at]] + _blocks_around(text, at)
+            line = text[at:text.find("\n", at)]
+            stays = not re.search(r"\b(break|continue|return)\b", line) and not any(re.search(r"\bok\b", h) for h in heads[1:])
+            assert stays or any("lane == 0" in h or "elect_one()" in h for h in heads), f"{name}: {text[at:at + 60]}"
+            seen += 1
+            at = text.find("mbar_wait(", at + 1)
+    assert seen >= 6
