@@ -87,6 +87,7 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 }
 template <bool PAIR>
 __device__ __forceinline__ void alloc_all(uint32_t* slot) {
+  __syncwarp();                                    // (thread 0 comes from the barriers)
   if constexpr (PAIR) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -240,11 +241,13 @@ __device__ __forceinline__ void drain_tile(const Mx4Job& J, const Mx4Walk& t, in
     uint32_t v[8];
     tmem_ld8(acc + (uint32_t)c0, v);
     tmem_ld_wait();
-    if (row >= J.m) continue;
-    const long long at = (long long)(t.row0 + c0) * J.y_stride + row;
+    if (row < J.m) {
+      const long long at = (long long)(t.row0 + c0) * J.y_stride + row;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c0 + i < t.rows) mx4_put(J, at + i * J.y_stride, __uint_as_float(v[i]) * f.a * f.b);
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < t.rows) mx4_put(J, at + i * J.y_stride, __uint_as_float(v[i]) * f.a * f.b);
+    }
+    __syncwarp();                                  // (the next load is the whole warp's)
   }
 }
 // The cluster's parts of a tile, added in rank order; the columns are shared out over the CTAs, then over their warps, a lane four rows

@@ -32,8 +32,18 @@ struct Mx4Job {
 };
 
 #ifdef __CUDACC__
+// (Each .aligned instruction wants all lanes of its warp: whoever comes here from loops of different lengths is gathered first.)
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_arrive() {      // (hands over nothing)
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {
   uint32_t a;

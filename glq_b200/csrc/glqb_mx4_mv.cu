@@ -120,7 +120,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
   uint32_t loads = 0;
   bool ok = true;
   Mx4Factor factor{1.0f, 1.0f};
-  if (J.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (J.split > 1) cluster_arrive();
 
   if (warp == MV4_WARPS) {
     if (lane == 0) {
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
       }
       if (J.split > 1) {
         // Each column of a shared tile has a CTA that adds it up: the parts go to its memory, part by part.
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // (all have begun)
+        cluster_wait();                                  // (all have begun)
         const int owned = (8 * NB + J.split - 1) / J.split;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -337,6 +337,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][e];
+      __syncwarp();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const int row = tile.mt * MX4_ROWS + (threadIdx.x & 127);
       if (row < J.m)
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
   }
   __syncwarp();
   if (J.split > 1) {                                     // (one tile per cluster)
-    if (first >= tiles || warp >= MV4_WARPS) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (first >= tiles || warp >= MV4_WARPS) cluster_wait();
     cluster_sync();
     if (first < tiles && warp < MV4_WARPS) {
       const Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles);

@@ -247,3 +247,25 @@ def test_whole_warps_wait_with_one_outcome():
             seen += 1
             at = text.find("mbar_wait(", at + 1)
     assert seen >= 6
+
+
+def test_instructions_of_whole_warps_are_reached_by_whole_warps():
+    """Cluster barriers gather their warp first; the loops that read tensor memory have no exit for single lanes, and lanes that store nothing
+    meet the others in front of the next read."""
+    text = {name: _source(name) for name in ("glqb_mx4_gemm.cu", "glqb_mx4_gemm.cuh", "glqb_mx4_mv.cu")}
+    seen = 0
+    for name, source in text.items():
+        for m in re.finditer(r"barrier\.cluster", source):
+            start = source.rfind("{", 0, m.start())
+            assert "__syncwarp" in source[start:m.start()], f"{name}: {source[m.start() - 80:m.start() + 60]}"
+            seen += 1
+    assert seen >= 4
+    gemm = text["glqb_mx4_gemm.cu"]
+    for name in ("drain_wide", "drain_tile"):
+        at = gemm.index(f"void {name}(")
+        body = gemm[at:gemm.index("template <", at)]
+        assert "tmem_ld" in body and "continue" not in body and "break" not in body
+    narrow = body[body.rindex("tmem_ld8"):]
+    assert narrow.index("mx4_put") < narrow.index("__syncwarp")
+    alloc = gemm[gemm.index("void alloc_all("):gemm.index("void dealloc_all(")]
+    assert alloc.index("__syncwarp") < alloc.index("tcgen05.alloc")
