@@ -13,8 +13,9 @@
 //
 // Operands are fp16, because two codes become fp16 in one instruction and bf16 in four (as bf16: 505 instructions per warp
 // for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  bf16 rows of x are brought to
-// fp16 on their way to shared memory, 256 values at a time, by the power of two that takes the largest finite one to 2^14 .. 2^15; the sums of a tile are multiplied back in
-// fp32.  Values of at least 2^-32 of the largest are exact, smaller ones off by at most 2^-40 of it.
+// fp16 on their way to shared memory, 256 values at a time, by the power of two that takes the largest finite one to 2^15 .. 2^16; the sums of a tile are multiplied back in
+// fp32.  (The largest bf16 number below 2^16 is 65280, which fp16 has.)  fp16 steps by 2^-24: values of at least 2^-32 of the largest are exact,
+// smaller ones off by at most 2^-25, 2^-40 of it.  Where the largest is below 2^-111 the power is 2^126, and every bf16 number exact.
 #include "glqb_mx4_gemm.cuh"
 #include "glqb_launch.h"
 #include <algorithm>
@@ -80,8 +81,8 @@ __device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
     }
     __syncwarp();
     top = __reduce_max_sync(0xFFFFFFFFu, top);
-    const int e = max((int)(top >> 7), 15);              // biased exponent of the largest; 2^(141 - e) takes it to 2^14
-    const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+    const int e = max((int)(top >> 7), 16);              // biased exponent of the largest; 2^(142 - e) takes it to 2^15
+    const float up = __uint_as_float((uint32_t)(269 - e) << 23);
     float f[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -91,7 +92,7 @@ __device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
     }
     auto pack = [](float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); };
     *reinterpret_cast<uint4*>(p) = make_uint4(pack(f[0], f[2]), pack(f[4], f[6]), pack(f[1], f[3]), pack(f[5], f[7]));
-    return __uint_as_float((uint32_t)(e - 14) << 23);
+    return __uint_as_float((uint32_t)(e - 15) << 23);
   }
 }
 

@@ -921,3 +921,32 @@ def test_writes_that_move_no_version_counter_are_seen_after_repack():
         layer.codes.zero_()
         layer.repack()
         assert not layer(x).any()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens", [1, 9, 16, 20, 70])
+def test_small_values_beside_large_ones(fmt, tokens):
+    """A weight row with one value reads one value of x.  In the form for few rows, where bf16 becomes fp16 under a power of two per 256 values,
+    it is exact from 2^-32 of the largest of them on, and below off by no more than 2^-40 of it; among more rows it is exact."""
+    g = np.random.default_rng(23)
+    n = 512
+    weight = ops.mx4_pack(ops.mx4_quantize(to_cuda(6.0 * np.eye(n)), fmt, torch.ones(1, device="cuda") if fmt == "nvfp4" else None))
+    tops = np.array([2.0 ** e for e in (0, 7, -100, -111, -112, 120)] + [255 * 2.0 ** e for e in (-7, 100, -119)] + [-(2.0 ** -126), 129 * 2.0 ** -7])
+    x = np.empty((tokens, n))
+    for r in range(tokens):
+        for half in (0, 256):
+            top = tops[(r + half // 256) % len(tops)]
+            v = g.integers(128, 256, 256) * 2.0 ** -8 * 2.0 ** g.integers(-46, 1, 256) * g.choice([-1, 1], 256) * abs(top)
+            v[1::16] = 129 * 2.0 ** -7 * 2.0 ** -32 * abs(top)
+            v[2::16] = 129 * 2.0 ** -7 * 2.0 ** -33 * abs(top)
+            v[::256] = top
+            x[r, half:half + 256] = v
+    xd = to_cuda(x, torch.bfloat16)
+    xv = host(xd).reshape(tokens, 2, 256)
+    y = host(ops.mx4_linear(xd, weight, out_dtype=torch.float32)).reshape(tokens, 2, 256)
+    top = np.abs(xv).max(-1, keepdims=True)
+    err = np.abs(y - 6.0 * xv)
+    # (6 x has ten bits: fp32 holds it, from 2^-149 on; the matrix instructions of more rows may take products below 2^-126 as zero)
+    few = tokens <= 32
+    low = 2.0 ** -149 if few else 2.0 ** -126
+    assert np.all(err <= np.where(np.abs(xv) >= 2.0 ** -32 * top, 0.0, 6.0 * 2.0 ** -40 * top if few else 0.0) + low)
