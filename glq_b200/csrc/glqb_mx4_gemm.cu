@@ -412,8 +412,12 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     a.add(group, R.a_stages);
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more(); t.next(L)) {
       int top = 0;
+      float up = 1.0f;
       if constexpr (FMT == GLQB_MX4_MXFP4) {
         top = J.tops[((long long)t.expert * J.m_tiles + min(row_tile(t), J.m_tiles - 1)) * MX4_ROWS + r] & 0xFF;
+        if constexpr (!__is_same(T, __half)) top = mx4_base(top);
+      } else if constexpr (!__is_same(T, __half)) {
+        up = mx4_pow2(126 + mx4_shift(J.w_scale[t.expert], MX4_BF16_MOST));
       }
       for (int k = group; k < steps + group; k += 2, w.add(1, G16_W_STAGES)) {
         if (!mbar_wait(&B.full_w[w.s], w.phase, &B.abort)) { ok = false; B.abort = 1; }
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
             const uint32_t words[4] = {q.x, q.y, q.z, q.w};
             uint32_t m0, m1;
             if constexpr (FMT == GLQB_MX4_MXFP4) m0 = m1 = mx4_multiplier<T>((sw >> (8 * u)) & 0xFFu, top);
-            else mx4_multipliers<T>((sw >> (16 * u)) & 0xFFFFu, m0, m1);
+            else mx4_multipliers<T>((sw >> (16 * u)) & 0xFFFFu, up, m0, m1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t p[4];

@@ -211,9 +211,11 @@ __device__ __forceinline__ void mx4_clear_rest(const Mx4Job& J, const int* eff, 
 // fp16: cvt takes two codes of a byte to fp16.  bf16 has no such instruction: the bits of a code are moved to sign, exponent and
 // first mantissa bit of a 16-bit number, where they read as the value times 2^-126, subnormals included.  One multiplication by
 // the scale then gives the operand exactly.  So that multiplier and operand stay in range, operands are
-//   MXFP4  value * 2^(s - top + 13) (fp16), value * 2^(s - top) (bf16), top the largest scale byte of the row
-//   NVFP4  value * s (fp16), value * s * 2^-7 (bf16)
-// and mx4_row_factor is what the sums are multiplied by.
+//   MXFP4  value * 2^(s - top + 13) (fp16), value * 2^(s - base) (bf16), top the largest scale byte of the row, base mx4_base(top)
+//   NVFP4  value * s (fp16), value * s * 2^k (bf16), k mx4_shift(t)
+// and mx4_row_factor is what the sums are multiplied by.  bf16 activations may be near the end of fp32's range: a sum must not leave it where the
+// result does not.  Operands are therefore no larger than the weights, down to where they are so small (6 * 2^-24, 2688 * 2^-31) that sums of 2^19
+// products stay in range whatever the activations are.
 //
 // bf16: the four pairs of a word, unscaled, r[i] holds values 2i and 2i + 1.  Logic and right shifts issue at half an instruction a
 // clock, and so do integer products (left shifts), on a pipe of their own.  Two of the pairs are therefore brought to bits 9:6 of
@@ -246,7 +248,13 @@ __device__ __forceinline__ void mx4_pairs(uint32_t w, uint32_t (&r)[4]) {
     mx4_pairs_bf16(w, r);
   }
 }
-// MXFP4: what a block's codes are multiplied by, in both halves
+// MXFP4: the scale byte that bf16 operands of a row are held relative to
+__device__ __forceinline__ int mx4_base(int top) { return top + min(24, max(0, 127 - top)); }
+// NVFP4: the power of two that a matrix's bf16 operands (or the sums of few rows) are multiplied by: that of t, between 2^-31 and 2^most
+__device__ __forceinline__ int mx4_shift(float t, int most) { return max(-31, min(most, (int)(__float_as_uint(t) >> 23 & 0xFFu) - 127)); }
+constexpr int MX4_BF16_MOST = -7;                              // (operands of up to 21: the multiplier, 448 * 2^(126 + k), is a bf16 number)
+__device__ __forceinline__ float mx4_pow2(int p) { return __uint_as_float((uint32_t)(p + 127) << 23); }      // -126 .. 127
+// MXFP4: what a block's codes are multiplied by, in both halves; `top`: what its row's operands are relative to
 template <typename T>
 __device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {
   const int d = (int)s - top;
@@ -255,9 +263,9 @@ __device__ __forceinline__ uint32_t mx4_multiplier(uint32_t s, int top) {
   else h = s == 255u ? 0x7FC0u : (uint32_t)max(d + 253, 0) << 7;
   return h | h << 16;
 }
-// NVFP4: the same of two neighbouring blocks, from their bytes
+// NVFP4: the same of two neighbouring blocks, from their bytes; `up` (bf16): 2^(126 + shift)
 template <typename T>
-__device__ __forceinline__ void mx4_multipliers(uint32_t two, uint32_t& m0, uint32_t& m1) {
+__device__ __forceinline__ void mx4_multipliers(uint32_t two, float up, uint32_t& m0, uint32_t& m1) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   if constexpr (__is_same(T, __half)) {
     const uint32_t b = (uint32_t)h.x | (uint32_t)h.y << 16;
@@ -266,7 +274,7 @@ __device__ __forceinline__ void mx4_multipliers(uint32_t two, uint32_t& m0, uint
   } else {
     const float2 f = __half22float2(__half2(h));
     float a = f.x, b = f.y;
-    mx4_mul_f32x2(a, b, 0x1p119f, 0x1p119f);
+    mx4_mul_f32x2(a, b, up, up);
     m0 = __byte_perm(__float_as_uint(a), 0, 0x3232);
     m1 = __byte_perm(__float_as_uint(b), 0, 0x3232);
   }
@@ -284,13 +292,16 @@ __device__ __forceinline__ uint32_t mx4_mul2(uint32_t a, uint32_t b) {
 struct Mx4Factor { float a, b; };     // two factors: 2^-127 and 2^127 have no single one
 template <typename T>
 __device__ __forceinline__ Mx4Factor mx4_power(uint32_t top) {          // MXFP4, from a row's entry in `tops`
-  const int p = (int)(top & 0xFFu) - (__is_same(T, __half) ? 140 : 127), h = p >> 1;
+  const int s = (int)(top & 0xFFu), p = __is_same(T, __half) ? s - 140 : mx4_base(s) - 127, h = p >> 1;
   return Mx4Factor{__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(p - h + 127) << 23)};
 }
+// NVFP4, sums that are held smaller by a power of two p: times p t, in an order that does not leave fp32's range on the way
+__device__ __forceinline__ Mx4Factor mx4_factor(float t, float p) { return t < 1.0f ? Mx4Factor{1.0f, t * p} : Mx4Factor{p, t}; }
 template <int FMT, typename T>
 __device__ __forceinline__ Mx4Factor mx4_row_factor(const Mx4Job& J, int expert, int row) {
   if constexpr (FMT == GLQB_MX4_MXFP4) return mx4_power<T>(J.tops[(long long)expert * J.m_tiles * MX4_ROWS + row]);
-  else return Mx4Factor{__is_same(T, __half) ? 1.0f : 128.0f, J.w_scale[expert]};
+  else if constexpr (__is_same(T, __half)) return Mx4Factor{1.0f, J.w_scale[expert]};
+  else return mx4_factor(J.w_scale[expert], mx4_pow2(-mx4_shift(J.w_scale[expert], MX4_BF16_MOST)));
 }
 #endif  // __CUDACC__
 

@@ -15,7 +15,11 @@
 // for 16 rows x 256 values, 256 rows over 128 experts of 1536 x 2048 70 us).  bf16 rows of x are brought to
 // fp16 on their way to shared memory, 256 values at a time, by the power of two that takes the largest finite one to 2^15 .. 2^16; the sums of a tile are multiplied back in
 // fp32.  (The largest bf16 number below 2^16 is 65280, which fp16 has.)  fp16 steps by 2^-24: values of at least 2^-32 of the largest are exact,
-// smaller ones off by at most 2^-25, 2^-40 of it.  Where the largest is below 2^-111 the power is 2^126, and every bf16 number exact.
+// smaller ones off by at most 2^-25, 2^-40 of it.  Where the largest is below 2^-94 the power is 2^109, and every bf16 number exact.
+//
+// A sum must not leave fp32's range where the result does not.  MXFP4 sums are relative to mx4_base; NVFP4 sums are multiplied, with the power that
+// brings a row of x back, by that of the matrix's scale (mx4_shift).  Nothing waits for the scale before a tile's first sums are there (eight
+// tokens of 14336 x 4096 14.9 us, without the power 14.7, with a wait at the start 15.5).
 #include "glqb_mx4_gemm.cuh"
 #include "glqb_launch.h"
 #include <algorithm>
@@ -25,12 +29,21 @@ namespace {
 
 constexpr int MV4_WARPS = 8;
 constexpr int MV4_X_ROW = MX4_K * 2 + 64;        // bytes of a row of x: two rows in different banks
-template <int FMT, int NB> struct Mv4 {
+template <int FMT, typename T, int NB> struct Mv4 {
   static constexpr int X = mx4_tile_bytes(FMT) + (FMT == GLQB_MX4_MXFP4 ? 2 * MX4_ROWS : 0);       // of a stage: weights, their rows' largest scales,
   static constexpr int X_SCALE = X + 8 * NB * MV4_X_ROW, STAGE = X_SCALE + 128;                    // x, what its sums are multiplied by
   static constexpr int STAGES = NB == 1 ? 4 : 3;                                                   // two CTAs per SM
   static constexpr int X_WARPS = 2 * NB, THREADS = (MV4_WARPS + 1 + X_WARPS) * 32;
+  static constexpr bool SHIFT = FMT == GLQB_MX4_NVFP4 && !__is_same(T, __half);                    // sums times a power of two of the matrix's scale
 };
+// A tile's factor, from the scale that was loaded at its start (used here first: moved in front of the sums it would be waited for there).
+template <bool SHIFT>
+__device__ __forceinline__ void settle_factor(Mx4Factor& f) {
+  if constexpr (SHIFT) {
+    asm volatile("" : "+f"(f.b));
+    f = mx4_factor(f.b, mx4_pow2(-mx4_shift(f.b, 0)));
+  }
+}
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -49,7 +62,8 @@ __device__ __forceinline__ void multipliers(uint32_t word, uint32_t pick, uint32
   m[0] = __byte_perm(b, 0, 0x1010);
   m[1] = __byte_perm(b, 0, 0x3232);
 }
-// MXFP4: 2^(scale - top) of a row's block j, from its word of scales.  PLAIN (all numbers, within 2^27 of the largest): the word holds scale - top + 127.
+// MXFP4: 2^(scale - top) of a row's block j, from its word of scales (top: mx4_base of the row's largest).  PLAIN (all numbers, within 2^27 of
+// the largest, which base is no more than 24 above): the word holds scale - top + 127.
 template <bool PLAIN>
 __device__ __forceinline__ float block_power(uint32_t word, int j, int top) {
   const int b = j & 3;
@@ -81,7 +95,7 @@ __device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
     }
     __syncwarp();
     top = __reduce_max_sync(0xFFFFFFFFu, top);
-    const int e = max((int)(top >> 7), 16);              // biased exponent of the largest; 2^(142 - e) takes it to 2^15
+    const int e = max((int)(top >> 7), 33);              // biased exponent of the largest; 2^(142 - e) takes it to 2^15
     const float up = __uint_as_float((uint32_t)(269 - e) << 23);
     float f[8];
 #pragma unroll
@@ -98,7 +112,7 @@ __device__ __forceinline__ float put8(uint8_t* p, const uint4& v) {
 
 template <int FMT, typename T, int NB>
 __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kernel(const __grid_constant__ Mx4Job J) {
-  using C = Mv4<FMT, NB>;
+  using C = Mv4<FMT, T, NB>;
   constexpr int TILE = mx4_tile_bytes(FMT), STAGE = C::STAGE, STAGES = C::STAGES;
   extern __shared__ __align__(128) uint8_t ring[];
   float* red = reinterpret_cast<float*>(ring + STAGES * STAGE);                      // [2][8 NB][128]
@@ -226,8 +240,8 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
             top[0] = tops[r];
             top[1] = tops[r + 8];
             plain = !__any_sync(0xFFFFFFFFu, ((top[0] | top[1]) & 256) != 0);
-            top[0] &= 255;
-            top[1] &= 255;
+            top[0] = mx4_base(top[0] & 255);
+            top[1] = mx4_base(top[1] & 255);
             f = mx4_power<__nv_bfloat16>(tops[threadIdx.x & 127]);
           }
         }
@@ -258,7 +272,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int a = 0; a < WORDS; ++a) sw[h][a] -= (uint32_t)(top[h] - 127) * 0x01010101u;       // (1 .. 127 in every byte)
+                for (int a = 0; a < WORDS; ++a) sw[h][a] -= (uint32_t)(top[h] - 127) * 0x01010101u;       // (76 .. 127 in every byte)
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -308,10 +322,16 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[n][e] = chain[n][0][e] + chain[n][1][e];
         }
+        float shift = 1.0f;
+        if constexpr (C::SHIFT) {
+          asm volatile("" : "+f"(f.b));
+          shift = fminf(fmaxf(__uint_as_float(__float_as_uint(f.b) & 0x7F800000u), 0x1p-31f), 1.0f);      // 2^mx4_shift(f.b, 0)
+        }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           float2 down = make_float2(1.0f, 1.0f);
           if constexpr (!__is_same(T, __half)) down = *reinterpret_cast<const float2*>(stage + C::X_SCALE + (n * 8 + 2 * t) * 4);
+          if constexpr (C::SHIFT) { down.x *= shift; down.y *= shift; }       // (at least 2^-140: exact)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(d[n][e], e & 1 ? down.y : down.x, acc[n][e]);
         }
@@ -340,6 +360,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
         for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * t + (e & 1)) * MX4_ROWS + r + 8 * (e >> 1)] = acc[n][e];
       __syncwarp();
       asm volatile("bar.sync 1, 256;" ::: "memory");
+      settle_factor<C::SHIFT>(f);
       const int row = tile.mt * MX4_ROWS + (threadIdx.x & 127);
       if (row < J.m)
         for (int c = threadIdx.x >> 7; c < tile.rows; c += 2)
@@ -352,6 +373,7 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
     if (first >= tiles || warp >= MV4_WARPS) cluster_wait();
     cluster_sync();
     if (first < tiles && warp < MV4_WARPS) {
+      settle_factor<C::SHIFT>(factor);
       const Mx4Walk t(L, J.experts, first, step, tiles, J.m_tiles);
       const int r = threadIdx.x & 127, row = t.mt * MX4_ROWS + r, owned = (8 * NB + J.split - 1) / J.split;
       if (row < J.m)
@@ -373,10 +395,10 @@ __global__ void __launch_bounds__((MV4_WARPS + 1 + 2 * NB) * 32, 2) mx4_mv_kerne
 
 template <int F, typename T, int NB>
 static size_t mv_smem(int experts) {
-  using C = Mv4<F, NB>;
+  using C = Mv4<F, T, NB>;
   return (size_t)C::STAGES * (C::STAGE + 16) + 2 * 8 * NB * MX4_ROWS * 4 + 8 + (size_t)(experts + 1) * 12;
 }
-int mx4_mv_clusters(int split) { return mx4_clusters(mx4_mv_kernel<GLQB_MX4_MXFP4, __half, 1>, Mv4<GLQB_MX4_MXFP4, 1>::THREADS, mv_smem<GLQB_MX4_MXFP4, __half, 1>(1), split); }
+int mx4_mv_clusters(int split) { return mx4_clusters(mx4_mv_kernel<GLQB_MX4_MXFP4, __half, 1>, Mv4<GLQB_MX4_MXFP4, __half, 1>::THREADS, mv_smem<GLQB_MX4_MXFP4, __half, 1>(1), split); }
 
 cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count, cudaStream_t stream) {
   const int nb = J.tn / 8;
@@ -386,7 +408,7 @@ cudaError_t mx4_mv_launch(int format, bool x_bf16, const Mx4Job& J, int sm_count
     using T = decltype(type);
     constexpr int F = decltype(fmt)::value, NB = decltype(blocks)::value;
     constexpr auto K = mx4_mv_kernel<F, T, NB>;
-    return mx4_launch<K>(K, grid, Mv4<F, NB>::THREADS, mv_smem<F, T, NB>(J.experts), J.split, stream, J);
+    return mx4_launch<K>(K, grid, Mv4<F, T, NB>::THREADS, mv_smem<F, T, NB>(J.experts), J.split, stream, J);
   };
   using M = std::integral_constant<int, GLQB_MX4_MXFP4>;
   using N = std::integral_constant<int, GLQB_MX4_NVFP4>;

@@ -950,3 +950,25 @@ def test_small_values_beside_large_ones(fmt, tokens):
     few = tokens <= 32
     low = 2.0 ** -149 if few else 2.0 ** -126
     assert np.all(err <= np.where(np.abs(xv) >= 2.0 ** -32 * top, 0.0, 6.0 * 2.0 ** -40 * top if few else 0.0) + low)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens,m", [(1, 200), (16, 200), (32, 130), (40, 200), (250, 200), (1700, 1100)])
+@pytest.mark.parametrize("small", [0, -20, -60, -100])
+def test_sums_that_stay_in_range(fmt, tokens, m, small):
+    """bf16 activations up to the largest there are, weights of any size below one: a sum leaves fp32's range only where the result does.
+    Activations times a power of two give the results times that power, bit for bit."""
+    g = np.random.default_rng(tokens)
+    n = 600
+    weight, w = make_weight(g, (m, n), fmt, spread=0.1)
+    if small:
+        dense = g.standard_normal((m, n)) * np.exp(g.standard_normal((m, 1)) * 0.1) / np.sqrt(n) * 2.0 ** small
+        q = ops.mx4_quantize(to_cuda(dense), fmt)
+        weight, w = ops.mx4_pack(q), host(ops.mx4_dequantize(q, torch.float32))
+    x = to_cuda(g.standard_normal((tokens, n)).clip(-3.9, 3.9), torch.bfloat16)
+    up = 125 if small else 122
+    y = ops.mx4_linear(x, weight, out_dtype=torch.float32)
+    z = ops.mx4_linear(x * 2.0 ** up, weight, out_dtype=torch.float32)
+    assert torch.isfinite(z).all()
+    check_product(z, host(x * 2.0 ** up), w, torch.float32)
+    assert torch.equal(z.double(), y.double() * 2.0 ** up) or small == -100
