@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     const int group = (warp - 8) >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const uint32_t to = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + half * 32u;
     // (A lane whose wait gave up goes on with what lies there, here and where results are drained, to the last tile: the instructions behind
-    // the wait are the whole warp's, and it can leave neither alone nor, without a vote, with the others.  32768 rows over 128 experts of 2048
-    // x 768: 121.5 us; with a vote per wait 123.4, with one per tile 122.9.  The other waits end at their next look at `abort`.)
+    // the wait are the whole warp's, and it can leave neither alone nor, without a vote, with the others; a vote per wait took 1.5 % of the time
+    // of 32768 rows over 128 experts of 2048 x 768, one per tile 1.  The other waits end at their next look at `abort`.)
     Mx4Pos a, w;
     a.add(group, R.a_stages);
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more(); t.next(L)) {
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
       Mx4Factor f{1.0f, 1.0f};
       if (row < J.m) f = row_factor<FMT, T, false>(J, t.expert, row);
-      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; B.abort = 1; }
+      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
       __syncwarp();
       tc_fence_after();
       if (!PAIR || mt < J.m_tiles)
@@ -483,7 +483,6 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       __syncwarp();
       if (lane == 0) arrive_first<PAIR>(&B.acc_empty[acc.s]);
     }
-    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
   }
   // ---- every thread arrives here, also after a wait gave up
   __syncwarp();
@@ -653,7 +652,7 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
       const int mt = row_tile(t), row = mt * MX4_ROWS + (warp & 3) * 32 + lane;
       Mx4Factor f{1.0f, 1.0f};
       if (row < J.m) f = row_factor<FMT, __half, true>(J, t.expert, row);
-      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { ok = false; B.abort = 1; }
+      if (!mbar_wait(&B.acc_full[acc.s], acc.phase, &B.abort)) { B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
       __syncwarp();
       tc_fence_after();
       if (!PAIR || mt < J.m_tiles)
@@ -662,7 +661,6 @@ __global__ void __launch_bounds__(G4_THREADS, 1) mx4_gemm4_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) arrive_first<PAIR>(&B.acc_empty[acc.s]);
     }
-    if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
   }
   // ---- every thread arrives here, also after a wait gave up
   __syncwarp();
