@@ -55,20 +55,19 @@ class Mx4Weight:
         return (self.format, self.in_features, self._index, lead) == (q.format, q.cols, q.codes.get_device(), tuple(q.codes.shape[:-1]))
 
 
-_get_device, _set_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_setDevice, torch._C._cuda_getCurrentRawStream
-
-
 def _call(index, what, fn, *args):
-    """fn(*args, current stream) with the tensors' device current: its kernels are launched there."""
-    before = _get_device()
+    """fn(*args, current stream) with the tensors' device current: its kernels are launched there.  (torch's names are looked up here: a
+    build of torch without CUDA has none of them, and imports this module all the same.)"""
+    cuda = torch._C
+    before = cuda._cuda_getDevice()
     if before == index:
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(*args, cuda._cuda_getCurrentRawStream(index))
     else:
-        _set_device(index)
+        cuda._cuda_setDevice(index)
         try:
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, cuda._cuda_getCurrentRawStream(index))
         finally:
-            _set_device(before)
+            cuda._cuda_setDevice(before)
     if rc:
         _lib.check(rc, what)
 

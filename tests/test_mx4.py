@@ -3,6 +3,7 @@ import ctypes
 import os
 import re
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -269,3 +270,15 @@ def test_instructions_of_whole_warps_are_reached_by_whole_warps():
     assert narrow.index("mx4_put") < narrow.index("__syncwarp")
     alloc = gemm[gemm.index("void alloc_all("):gemm.index("void dealloc_all(")]
     assert alloc.index("__syncwarp") < alloc.index("tcgen05.alloc")
+
+
+def test_modules_import_without_torchs_cuda_names():
+    """The host logic (checkpoints, loading, layers' buffers) is there with a build of torch that has no CUDA."""
+    code = ("import torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            "import glq_b200, glq_b200.ops, glq_b200.linear, glq_b200.loader, glq_b200.dropin, glq_b200.checkpoint\n"
+            "from glq_b200.linear import Mx4Linear\n"
+            "assert set(Mx4Linear(64, 8).state_dict()) == {'codes', 'scales'}\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
