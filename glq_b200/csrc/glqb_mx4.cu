@@ -500,6 +500,9 @@ int dequantize_launch(const uint8_t* codes, const uint8_t* scales, const float* 
   return mx4_launched("mx4_dequantize");
 }
 
+// Is an address a multiple of `bytes`?  (Kernels access values whole, and the images' bulk copies 16 bytes at a time: elsewhere they fault.)
+bool lies_on(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+size_t size_of(int dtype) { return dtype == GLQB_DT_F32 ? 4 : 2; }
 bool dtype_ok(int d) { return d == GLQB_DT_F16 || d == GLQB_DT_BF16 || d == GLQB_DT_F32; }
 bool format_ok(int f) { return f == GLQB_MX4_MXFP4 || f == GLQB_MX4_NVFP4; }
 
@@ -519,6 +522,7 @@ int glqb_mx4_quantize(const void* x, int32_t x_dtype, int64_t x_stride, int64_t 
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!x || !codes || !scales) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: null argument");
   if (x_stride < cols && rows > 1) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: rows of %d values %lld apart", cols, (long long)x_stride);
+  if (!lies_on(x, size_of(x_dtype)) || !lies_on(tensor_scale, 4) || !lies_on(own_scale, 4)) return mx4_fail(GLQB_E_INVALID, "mx4_quantize: values that are not aligned");
   const Mx4Rows q = rows_of(rows, cols, x_stride, format, true);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
@@ -534,6 +538,7 @@ int glqb_mx4_dequantize(const void* codes, const void* scales, const float* tens
   if (format == GLQB_MX4_NVFP4 && (!tensor_scale || rows_per_scale < 1)) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: nvfp4 needs tensor_scale");
   if (rows == 0 || cols == 0) return GLQB_OK;
   if (!codes || !scales || !out) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: null argument");
+  if (!lies_on(out, size_of(out_dtype)) || !lies_on(tensor_scale, 4)) return mx4_fail(GLQB_E_INVALID, "mx4_dequantize: values that are not aligned");
   const Mx4Rows q = rows_of(rows, cols, cols, format, format == GLQB_MX4_MXFP4 || rows_per_scale >= rows);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (format == GLQB_MX4_MXFP4)
@@ -552,7 +557,7 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
   if (!format_ok(format)) return mx4_fail(GLQB_E_INVALID, "mx4_pack: format %d", format);
   if (experts < 1 || m < 1 || n < 1 || m > MX4_MAX_SIZE || n > MX4_MAX_SIZE) return mx4_fail(GLQB_E_INVALID, "mx4_pack: %d x %d x %d", experts, m, n);
   if (!codes || !scales || !image) return mx4_fail(GLQB_E_INVALID, "mx4_pack: null argument");
-  if (reinterpret_cast<uintptr_t>(image) % 128) return mx4_fail(GLQB_E_INVALID, "mx4_pack: the image must be 128-byte aligned");
+  if (!lies_on(image, 128)) return mx4_fail(GLQB_E_INVALID, "mx4_pack: the image must be 128-byte aligned");
   const int mt = (m + MX4_ROWS - 1) / MX4_ROWS, kt = (n + MX4_K - 1) / MX4_K;
   const long long tiles = (long long)experts * mt * kt;
   if (tiles >= (1ll << 31) || experts > MX4_MAX_EXPERTS || (long long)experts * mt >= 1ll << 27)
@@ -660,6 +665,10 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
     return mx4_fail(GLQB_E_INVALID, "mx4_product: %lld rows of %d results are too many for one call", (long long)rows, w->m);
   if (!w->image || !x || !y || (w->format == GLQB_MX4_NVFP4 && !w->tensor_scale)) return mx4_fail(GLQB_E_INVALID, "mx4_product: null argument");
   if (rows > 1 && (x_stride < w->n || y_stride < w->m)) return mx4_fail(GLQB_E_INVALID, "mx4_product: rows overlap");
+  if (!lies_on(w->image, 128)) return mx4_fail(GLQB_E_INVALID, "mx4_product: the image must be 128-byte aligned");
+  if (!lies_on(workspace, 16)) return mx4_fail(GLQB_E_INVALID, "mx4_product: the workspace must be 16-byte aligned");
+  if (!lies_on(x, size_of(x_dtype)) || !lies_on(y, size_of(y_dtype)) || !lies_on(offsets, offsets_are_int64 ? 8 : 4) || !lies_on(w->tensor_scale, 4) || !lies_on(x_scale, 4))
+    return mx4_fail(GLQB_E_INVALID, "mx4_product: values that are not aligned");
   const Device* d = device();
   const Form f = form_of(w, rows, x_stride, x, quantize, d);
   if (workspace_bytes < f.bytes || (f.bytes && !workspace))

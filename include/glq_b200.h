@@ -298,7 +298,8 @@ size_t glqb_noalloc_scratch_bytes(void);
  *   GLQB_MX4_MXFP4  blocks of 32, the scale byte s stands for 2^(s - 127), 255 for NaN
  *   GLQB_MX4_NVFP4  blocks of 16, the scale byte is an e4m3 number (>= 0), times one fp32 number per tensor (or expert)
  * Stored rows: codes two to a byte, the even value in the low nibble, ceil(cols / 2) bytes; ceil(cols / block) scale bytes.
- * All entry points enqueue on `stream` and neither allocate nor synchronise, unless stated.
+ * All entry points enqueue on `stream` and neither allocate nor synchronise, unless stated.  Values, scales and offsets lie on
+ * multiples of their size, an image on 128 bytes, a workspace on 16; other addresses are refused.
  */
 #define GLQB_MX4_MXFP4 0
 #define GLQB_MX4_NVFP4 1

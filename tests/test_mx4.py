@@ -282,3 +282,31 @@ def test_modules_import_without_torchs_cuda_names():
             "assert set(Mx4Linear(64, 8).state_dict()) == {'codes', 'scales'}\n")
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
+
+
+def test_addresses_that_kernels_cannot_use_are_refused(lib):
+    """Before any CUDA call: an image or workspace that bulk copies cannot read, values that lie between their places."""
+    from glq_b200 import _lib
+    p = 1 << 20                                                 # never dereferenced: each call is refused
+
+    def refused(rc, text):
+        assert rc == -1 and text in lib.glqb_last_error().decode(), (rc, lib.glqb_last_error())
+
+    def product(w, x=p, xd=1, offsets=None, wide=0, q=0, xscale=None, y=p, yd=1, ws=None, size=0):
+        return lib.glqb_mx4_product(ctypes.byref(w), x, xd, 64, 40, offsets, wide, q, xscale, y, yd, 64, 0, 0, ws, size, None)
+
+    mx, nv = _lib.Mx4WeightDesc(p, None, 0, 1, 64, 64), _lib.Mx4WeightDesc(p, p, 1, 1, 64, 64)
+    for off in (16, 64, 1):
+        refused(product(_lib.Mx4WeightDesc(p + off, None, 0, 1, 64, 64)), "128-byte aligned")
+    for off in (1, 4, 8):
+        refused(product(mx, q=1, ws=p + off, size=1 << 20), "16-byte aligned")
+    for call in (lambda: product(mx, x=p + 1), lambda: product(mx, x=p + 2, xd=2, q=1, ws=p, size=1 << 20), lambda: product(mx, y=p + 1),
+                 lambda: product(mx, y=p + 2, yd=2), lambda: product(mx, offsets=p + 2), lambda: product(mx, offsets=p + 4, wide=1),
+                 lambda: product(_lib.Mx4WeightDesc(p, p + 2, 1, 1, 64, 64)), lambda: product(nv, q=1, xscale=p + 1, ws=p, size=1 << 20),
+                 lambda: lib.glqb_mx4_quantize(p + 1, 0, 32, 1, 32, 0, None, None, p, p, None),
+                 lambda: lib.glqb_mx4_quantize(p + 2, 2, 32, 1, 32, 0, None, None, p, p, None),
+                 lambda: lib.glqb_mx4_quantize(p, 0, 32, 1, 32, 1, p + 2, None, p, p, None),
+                 lambda: lib.glqb_mx4_quantize(p, 0, 32, 1, 32, 1, None, p + 1, p, p, None),
+                 lambda: lib.glqb_mx4_dequantize(p, p, None, 1, 1, 32, 0, p + 1, 0, None),
+                 lambda: lib.glqb_mx4_dequantize(p, p, p + 1, 1, 1, 32, 1, p, 0, None)):
+        refused(call(), "not aligned")
