@@ -20,6 +20,7 @@ from . import _lib
 
 _FORMATS = {"mxfp4": _lib.MX4_MXFP4, "nvfp4": _lib.MX4_NVFP4}
 _BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_MOST = 2 ** 31 - 1                 # values of a row
 _RAN_ON: set = set()                # devices whose status word a product may have set
 _DTYPES = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
 
@@ -96,6 +97,11 @@ def _dtype(dtype, what):
     return d
 
 
+def _counted(cols):
+    if cols > _MOST:
+        raise ValueError(f"glq_b200: rows of {cols} values: at most {_MOST} (the C ABI counts them in 32 bits)")
+
+
 def _scale_ptr(t, x, name, count=1):
     _same_device(t, x, name)
     if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous():
@@ -131,6 +137,7 @@ def mx4_quantize(x, format="mxfp4", tensor_scale=None) -> Mx4Tensor:
     if not shape:
         raise ValueError("glq_b200: x needs at least one dimension")
     cols, lead, some = shape[-1], shape[:-1], x.numel() > 0
+    _counted(cols)
     codes = _new(x, lead, (cols + 1) // 2, torch.uint8)
     scales = _new(x, lead, -(-cols // _BLOCK[format]), torch.uint8)
     given = own = None
@@ -160,6 +167,7 @@ def _checked(q: Mx4Tensor):
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not shape:
         raise ValueError("glq_b200: codes and scales are uint8 tensors of stored rows")
     lead = shape[:-1]
+    _counted(cols)
     if shape[-1] != (cols + 1) // 2 or scales.shape != lead + (-(-cols // _BLOCK[format]),):
         raise ValueError(f"glq_b200: codes {tuple(shape)} and scales {tuple(scales.shape)} are not {format} rows of {cols} values")
     count = 0
@@ -196,6 +204,8 @@ def mx4_pack(q: Mx4Tensor, out: Optional[Mx4Weight] = None) -> Mx4Weight:
     experts, m = (q.codes.shape[0] if q.codes.dim() == 3 else None), q.codes.shape[-2]
     if rows == 0 or n == 0:
         raise ValueError(f"glq_b200: empty weights, codes of {tuple(q.codes.shape)}")
+    if max(m, experts or 1) > _MOST:
+        raise ValueError(f"glq_b200: codes of {tuple(q.codes.shape)}: at most {_MOST} rows and experts")
     if out is not None and (out.__class__ is not Mx4Weight or not out._holds(q)):
         raise ValueError(f"glq_b200: out is a packed {q.format} weight of {tuple(q.codes.shape[:-1]) + (n,)} on {q.codes.device}")
     codes, sc = q.codes.contiguous(), q.scales.contiguous()

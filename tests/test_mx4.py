@@ -310,3 +310,21 @@ def test_addresses_that_kernels_cannot_use_are_refused(lib):
                  lambda: lib.glqb_mx4_dequantize(p, p, None, 1, 1, 32, 0, p + 1, 0, None),
                  lambda: lib.glqb_mx4_dequantize(p, p, p + 1, 1, 1, 32, 1, p, 0, None)):
         refused(call(), "not aligned")
+
+
+def test_rows_too_long_to_be_counted_are_refused(monkeypatch):
+    """Sizes pass a C interface of 32 bits, which would cut 2^32 + 32 values to 32 without a word.  (On tensors without memory.)"""
+    from glq_b200 import mx4, ops
+    monkeypatch.setattr(mx4, "_cuda", lambda t, name: None)
+    monkeypatch.setattr(mx4, "_call", lambda *a: pytest.fail("a call was made"))
+    for n in (2 ** 31, 2 ** 32 + 32):
+        with pytest.raises(ValueError, match="at most 2147483647"):
+            ops.mx4_quantize(torch.empty(n, dtype=torch.bfloat16, device="meta"))
+        q = ops.Mx4Tensor(torch.empty(1, n // 2, dtype=torch.uint8, device="meta"), torch.empty(1, n // 32, dtype=torch.uint8, device="meta"), "mxfp4", n)
+        for call in (ops.mx4_dequantize, ops.mx4_pack):
+            with pytest.raises(ValueError, match="at most 2147483647"):
+                call(q)
+        for lead in ((n,), (n, 1)):
+            q = ops.Mx4Tensor(torch.empty(*lead, 16, dtype=torch.uint8, device="meta"), torch.empty(*lead, 1, dtype=torch.uint8, device="meta"), "mxfp4", 32)
+            with pytest.raises(ValueError, match="at most 2147483647"):
+                ops.mx4_pack(q)
