@@ -270,15 +270,16 @@ class Mx4Linear(nn.Module):
                 return self._packed
             if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("glq_b200: the weight is packed at the first forward: run one before capturing a graph")
-            rows, stream, before = self._rows(), torch.cuda.current_stream(), self._packed
-            weight, packed_on = None, stream.cuda_stream
+            rows, before, weight = self._rows(), self._packed, None
             if before is not None:                # the same memory takes the new weights, behind whatever reads the old ones
                 torch.cuda.synchronize(before[2].image.device)
                 if before[2].image.device == self.codes.device and before[2]._holds(rows):
-                    weight, packed_on = before[2:]
+                    weight = before[2]
+            packed_on = before[3] if weight is not None else None
             weight = ops.mx4_pack(rows, out=weight)
+            stream = torch.cuda.current_stream()
             stream.synchronize()
-            self._packed = packed = (now, held, weight, packed_on)
+            self._packed = packed = (now, held, weight, stream.cuda_stream if packed_on is None else packed_on)
         return packed
 
     def repack(self) -> None:

@@ -328,3 +328,9 @@ def test_rows_too_long_to_be_counted_are_refused(monkeypatch):
             q = ops.Mx4Tensor(torch.empty(*lead, 16, dtype=torch.uint8, device="meta"), torch.empty(*lead, 1, dtype=torch.uint8, device="meta"), "mxfp4", 32)
             with pytest.raises(ValueError, match="at most 2147483647"):
                 ops.mx4_pack(q)
+
+
+def test_layer_on_the_host_has_no_packed_weight():
+    from glq_b200.linear import Mx4Linear
+    with pytest.raises(RuntimeError, match="codes must be a CUDA tensor"):
+        Mx4Linear(64, 8).weight
