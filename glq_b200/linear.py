@@ -226,6 +226,25 @@ class Mx4Linear(nn.Module):
             layer.bias = bias.detach().float()
         return layer
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        """Codes and scales are bytes, whatever one-byte type a checkpoint gives them (float8_e4m3fn, float8_e8m0fnu, int8): they are taken
+        as they lie, where a copy would convert their values.  Wider floating-point types are refused."""
+        state_dict = dict(state_dict)
+        for name in ("codes", "scales"):
+            t = state_dict.get(prefix + name)
+            if not isinstance(t, torch.Tensor) or t.dtype == torch.uint8:
+                continue
+            if t.element_size() == 1 and t.dtype != torch.bool:
+                state_dict[prefix + name] = t.view(torch.uint8)
+            elif t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+                error_msgs.append(f"{prefix}{name} holds {t.dtype} values, expected the stored bytes")
+                del state_dict[prefix + name]
+                strict = False
+        t = state_dict.get(prefix + "tensor_scale")
+        if isinstance(t, torch.Tensor) and t.dim() == 0:
+            state_dict[prefix + "tensor_scale"] = t.reshape(1)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
     def _apply(self, fn, *args, **kwargs):
         # (half() and bfloat16() are for activations: the tensor's scale and the bias stay fp32)
         kept = {name: t for name in ("tensor_scale", "bias") if (t := getattr(self, name)) is not None}

@@ -334,3 +334,29 @@ def test_layer_on_the_host_has_no_packed_weight():
     from glq_b200.linear import Mx4Linear
     with pytest.raises(RuntimeError, match="codes must be a CUDA tensor"):
         Mx4Linear(64, 8).weight
+
+
+@pytest.mark.parametrize("assign", [False, True])
+def test_layer_loads_bytes_of_any_one_byte_type(assign):
+    """Checkpoints give scales (and codes) types of their own; their bytes are what counts."""
+    from glq_b200.linear import Mx4Linear
+    g = np.random.default_rng(0)
+    for fmt, dtypes in (("nvfp4", (torch.uint8, torch.float8_e4m3fn, torch.int8)), ("mxfp4", (torch.uint8, torch.float8_e8m0fnu, torch.int8))):
+        scales = torch.from_numpy(g.integers(0, 127, (8, 64 // O.BLOCK[fmt]), dtype=np.uint8))
+        codes = torch.from_numpy(g.integers(0, 256, (8, 32), dtype=np.uint8))
+        for dtype in dtypes:
+            layer = Mx4Linear(64, 8, format=fmt)
+            state = {"codes": codes.view(torch.int8) if dtype == torch.int8 else codes, "scales": scales.view(dtype)}
+            if fmt == "nvfp4":
+                state["tensor_scale"] = torch.tensor(0.25)
+            kept = dict(state)
+            layer.load_state_dict(state, assign=assign)
+            assert layer.scales.dtype == layer.codes.dtype == torch.uint8
+            assert torch.equal(layer.scales, scales) and torch.equal(layer.codes, codes)
+            assert all(state[k] is kept[k] for k in kept)
+            if fmt == "nvfp4":
+                assert layer.tensor_scale.shape == (1,) and layer.tensor_scale.item() == 0.25
+        with pytest.raises(RuntimeError, match="scales holds torch.float32"):
+            Mx4Linear(64, 8, format=fmt).load_state_dict({"codes": codes, "scales": scales.float()}, strict=False)
+        with pytest.raises(RuntimeError, match="scales holds torch.float32"):
+            torch.nn.Sequential(Mx4Linear(64, 8, format=fmt)).load_state_dict({"0.codes": codes, "0.scales": scales.float()}, strict=False)
