@@ -223,7 +223,7 @@ class Mx4Linear(nn.Module):
         if format == "nvfp4":
             layer.tensor_scale = q.tensor_scale.clone()
         if bias is not None:
-            layer.bias = bias.detach().float()
+            layer.bias = bias.detach().to(layer.codes.device, torch.float32, copy=True)
         return layer
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):

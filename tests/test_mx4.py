@@ -360,3 +360,13 @@ def test_layer_loads_bytes_of_any_one_byte_type(assign):
             Mx4Linear(64, 8, format=fmt).load_state_dict({"codes": codes, "scales": scales.float()}, strict=False)
         with pytest.raises(RuntimeError, match="scales holds torch.float32"):
             torch.nn.Sequential(Mx4Linear(64, 8, format=fmt)).load_state_dict({"0.codes": codes, "0.scales": scales.float()}, strict=False)
+
+
+def test_layer_of_a_dense_weight_has_its_own_bias(monkeypatch):
+    """Loading into the layer must not write to the bias that it was made from."""
+    from glq_b200 import linear
+    monkeypatch.setattr(linear.ops, "mx4_quantize", lambda w, fmt: linear.ops.Mx4Tensor(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.uint8), fmt, 64))
+    bias = torch.nn.Parameter(torch.arange(8.0))
+    layer = linear.Mx4Linear.from_weight(torch.zeros(8, 64), bias)
+    layer.load_state_dict({**layer.state_dict(), "bias": torch.ones(8)})
+    assert torch.equal(bias.detach(), torch.arange(8.0)) and torch.equal(layer.bias, torch.ones(8)) and not layer.bias.requires_grad
