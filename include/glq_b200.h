@@ -333,8 +333,8 @@ int glqb_mx4_pack(const void* codes, const void* scales, int32_t format, int32_t
  * quantize: x is brought to the weights' format first, as glqb_mx4_quantize does (NVFP4: by *x_scale, or, with x_scale NULL, by the
  * scale of the experts' rows, offsets[0] up to the largest offset), and 4-bit values are multiplied.  Without it x is fp16 or bf16 and stays so.
  * Under 16-bit activations MXFP4 weights are multiplied relative to the largest scale of their row: a block whose scale lies more
- * than 2^36 below it may lose bits; few bf16 rows are multiplied as fp16 under a power of two per 256 values (exact from 2^-32 of the
- * largest of them on).  m and n up to 2^30, rows up to 2^31 - 2^16, (rows + experts) * ceil(m / 128) below 2^30.
+ * than 2^36 below it may lose bits (fp16 x); few bf16 rows are multiplied as fp16 under a power of two per 256 values (exact from 2^-32 of
+ * the largest of them on, below that off by at most 2^-40 of it).  m and n up to 2^30, rows up to 2^31 - 2^16, (rows + experts) * ceil(m / 128) below 2^30.
  * accumulate: y <- y + result, added before the rounding.  A bounded wait that gives up sets the device's status word. */
 size_t glqb_mx4_workspace_bytes(const GlqbMx4Weight* w, int64_t rows, int64_t x_stride, const void* x, int32_t quantize);
 int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int64_t x_stride, int64_t rows,
