@@ -289,12 +289,15 @@ class Mx4Linear(nn.Module):
                 return self._packed
             if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("glq_b200: the weight is packed at the first forward: run one before capturing a graph")
-            rows, before, weight = self._rows(), self._packed, None
-            if before is not None:                # the same memory takes the new weights, behind whatever reads the old ones
+            # behind whatever still writes the rows on another stream (what is packed is kept), or reads the old image, whose memory takes
+            # the new weights
+            rows, before, weight, packed_on = self._rows(), self._packed, None, None
+            if self.codes.is_cuda:
+                torch.cuda.synchronize(self.codes.device)
+            if before is not None and before[2].image.device != self.codes.device:
                 torch.cuda.synchronize(before[2].image.device)
-                if before[2].image.device == self.codes.device and before[2]._holds(rows):
-                    weight = before[2]
-            packed_on = before[3] if weight is not None else None
+            if before is not None and before[2].image.device == self.codes.device and before[2]._holds(rows):
+                weight, packed_on = before[2:]
             weight = ops.mx4_pack(rows, out=weight)
             stream = torch.cuda.current_stream()
             stream.synchronize()

@@ -972,3 +972,16 @@ def test_sums_that_stay_in_range(fmt, tokens, m, small):
     assert torch.isfinite(z).all()
     check_product(z, host(x * 2.0 ** up), w, torch.float32)
     assert torch.equal(z.double(), y.double() * 2.0 ** up) or small == -100
+
+
+def test_layer_whose_rows_another_stream_is_writing():
+    """The first forward packs what has been enqueued to be written, on whatever stream."""
+    (layer, other), x, want = layers_and_input()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(DELAY)
+        layer.load_state_dict(other.state_dict())
+    with torch.cuda.stream(b):
+        y = layer(x)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[1])

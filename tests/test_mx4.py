@@ -370,3 +370,34 @@ def test_layer_of_a_dense_weight_has_its_own_bias(monkeypatch):
     layer = linear.Mx4Linear.from_weight(torch.zeros(8, 64), bias)
     layer.load_state_dict({**layer.state_dict(), "bias": torch.ones(8)})
     assert torch.equal(bias.detach(), torch.arange(8.0)) and torch.equal(layer.bias, torch.ones(8)) and not layer.bias.requires_grad
+
+
+def test_layer_packs_behind_writes_on_other_streams(monkeypatch):
+    """What the first forward packs is kept: rows that another stream is still writing are waited for.  (The host's calls, without a GPU.)"""
+    import contextlib
+    import types
+    from glq_b200 import linear
+    calls = []
+
+    class Rows:
+        is_cuda, device, _version = True, torch.device("cuda:0"), 0
+        get_device = staticmethod(lambda: 0)
+        is_inference = staticmethod(lambda: False)
+
+    def pack(rows, out=None):
+        calls.append("pack")
+        return types.SimpleNamespace(image=types.SimpleNamespace(device=rows.codes.device), tensor_scale=None, _holds=lambda rows: True)
+
+    monkeypatch.setattr(linear.ops, "mx4_pack", pack)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: types.SimpleNamespace(synchronize=lambda: calls.append("wait"), cuda_stream=7))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: calls.append(str(device)))
+    layer = linear.Mx4Linear(64, 8)
+    del layer.codes, layer.scales
+    layer.codes, layer.scales = Rows(), Rows()
+    for _ in range(2):
+        assert layer.weight is layer.weight
+        assert calls == ["cuda:0", "pack", "wait"]
+        calls.clear()
+        layer.repack()
