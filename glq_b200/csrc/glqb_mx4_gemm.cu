@@ -408,8 +408,13 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
     // (A lane whose wait gave up goes on with what lies there, here and where results are drained, to the last tile: the instructions behind
     // the wait are the whole warp's, and it can leave neither alone nor, without a vote, with the others; a vote per wait took 1.5 % of the time
     // of 32768 rows over 128 experts of 2048 x 768, one per tile 1.  The other waits end at their next look at `abort`.)
+    // Groups take the CTA's steps in turn, counted over all its tiles: behind an odd number of them the other group begins.  A wait by parity
+    // holds only as long as the barrier is no further behind than the phase in front: a group's steps must not lie more than a_stages, two at
+    // least, apart.  (They did, by three, where each tile began with the first group: with two stages group 1 could write a stage
+    // that was not read yet.)
     Mx4Pos a, w;
     a.add(group, R.a_stages);
+    int mine = group;                              // of a tile's steps the even ones or the odd ones
     for (Mx4Walk t(L, J.experts, first, step, tiles, m_tiles); t.more(); t.next(L)) {
       int top = 0;
       float up = 1.0f;
@@ -419,12 +424,12 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
       } else if constexpr (!__is_same(T, __half)) {
         up = mx4_pow2(126 + mx4_shift(J.w_scale[t.expert], MX4_BF16_MOST));
       }
-      for (int k = group; k < steps + group; k += 2, w.add(1, G16_W_STAGES)) {
+      for (int k = mine; k < steps + mine; k += 2, w.add(1, G16_W_STAGES)) {
         if (!mbar_wait(&B.full_w[w.s], w.phase, &B.abort)) { ok = false; B.abort = 1; }
         const uint8_t* tile = w_base + w.s * TILE;
         uint32_t v[32];
         if (k < steps) {
-          const int c = group * 4 + half * 2;      // 16-byte units of a row: two of them
+          const int c = mine * 4 + half * 2;       // 16-byte units of a row: two of them
           const uint8_t* codes = tile + (r >> 3) * 1024 + (r & 7) * 128;
           const uint8_t* sc = tile + MX4_CODE_BYTES + (r & 31) * 16 + (r >> 5) * 4;
           uint32_t sw;
@@ -459,11 +464,7 @@ __global__ void __launch_bounds__(G16_THREADS, 1) mx4_gemm16_kernel(const __grid
           a.add(2, R.a_stages);
         }
       }
-      // (the place of the next tile's first step, or second: an odd number of steps puts the groups on the other one's)
-      if (steps & 1) {
-        if (group) a.add(1, R.a_stages);
-        else a.back(R.a_stages);
-      }
+      mine ^= steps & 1;
     }
     if (!ok) { B.abort = 1; if (lane == 0) atomicCAS(J.status, 0, (int)ST_GAVE_UP_PRODUCER); }
   } else if (warp >= 4) {

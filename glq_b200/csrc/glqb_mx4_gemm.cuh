@@ -171,10 +171,6 @@ struct Mx4Pos {                   // a place in a ring, and the parity of its ro
     s += d;
     while (s >= n) { s -= n; phase ^= 1u; }
   }
-  __device__ __forceinline__ void back(uint32_t n) {
-    if (s == 0) { s = n; phase ^= 1u; }
-    --s;
-  }
 };
 
 __device__ __forceinline__ void mx4_put(const Mx4Job& J, long long at, float v) {

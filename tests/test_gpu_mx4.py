@@ -985,3 +985,42 @@ def test_layer_whose_rows_another_stream_is_writing():
         y = layer(x)
     torch.cuda.synchronize()
     assert torch.equal(y, want[1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tokens,m,n", [(2042, 1680, 304), (1921, 1680, 304), (2300, 2500, 640), (1700, 2304, 136), (1537, 3000, 360), (190, 25000, 896)])
+def test_tiles_of_an_odd_number_of_steps(fmt, dtype, tokens, m, n):
+    """A CTA's second tile behind one of an odd number of steps, with activations that come late (caches emptied in front of every call): the same
+    bits every time, and the right ones."""
+    g = np.random.default_rng(tokens)
+    q = ops.mx4_quantize(to_cuda(g.standard_normal((m, n)) / np.sqrt(n)), fmt)
+    weight, w = ops.mx4_pack(q), host(ops.mx4_dequantize(q, torch.float32))
+    x = to_cuda(g.standard_normal((tokens, n)), DT[dtype])
+    junk = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    first = ops.mx4_linear(x, weight)
+    # (dequantised NVFP4 weights are rounded once, by 2^-24 of each)
+    check_product(first, host(x), w, DT[dtype])
+    for i in range(40):
+        junk.fill_(i)
+        assert torch.equal(ops.mx4_linear(x, weight), first), i
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("experts,per,m,n", [(40, 95, 600, 304), (16, 400, 1100, 384), (64, 90, 400, 136)])
+def test_experts_tiles_of_an_odd_number_of_steps(fmt, experts, per, m, n):
+    g = np.random.default_rng(experts)
+    weight, w = make_weight(g, (experts, m, n), fmt)
+    counts = g.multinomial(experts * per, g.dirichlet(np.full(experts, 3.0)))
+    x = to_cuda(g.standard_normal((int(counts.sum()), n)), torch.bfloat16)
+    off = counts_to_offsets(counts)
+    junk = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    first = ops.mx4_grouped_linear(x, weight, off)
+    at, xv = off.tolist(), host(x)
+    for e in range(experts):
+        if counts[e]:
+            check_product(first[at[e]:at[e + 1]], xv[at[e]:at[e + 1]], w[e], torch.bfloat16)
+    for i in range(40):
+        junk.fill_(i)
+        assert torch.equal(ops.mx4_grouped_linear(x, weight, off), first), i

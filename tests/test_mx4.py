@@ -401,3 +401,34 @@ def test_layer_packs_behind_writes_on_other_streams(monkeypatch):
         assert calls == ["cuda:0", "pack", "wait"]
         calls.clear()
         layer.repack()
+
+
+def _ring_is_safe(stages, steps, tiles, alternate):
+    """Two groups of warps fill a ring of `stages` in turn, one thread empties it in order.  A group waits for the round before by parity, which
+    a barrier two rounds behind answers with yes: the round before that must be known to be over, by what the group waited for last.
+    `alternate`: a group's steps are two apart over the tiles' borders; else each tile begins with the first group."""
+    for group in (0, 1):
+        over, g0 = -1, 0                                        # the last step known to be read (steps are read in order)
+        mine = group
+        for _ in range(tiles):
+            for k in range(mine, steps, 2):
+                g = g0 + k
+                if g - 2 * stages > over:
+                    return False
+                over = max(over, g - stages)
+            g0 += steps
+            if alternate:
+                mine ^= steps & 1
+    return True
+
+
+def test_groups_that_fill_a_ring_stay_within_what_parity_can_tell():
+    for steps in range(1, 12):
+        for stages in (2, 3, 4):                                # what two accumulators of up to 192, 160 and 128 columns leave
+            assert _ring_is_safe(stages, steps, 9, True)
+            assert _ring_is_safe(stages, steps, 9, False) == (stages > 2 or steps % 2 == 0 or steps == 1)
+    text = _source("glqb_mx4_gemm.cu")
+    loop = text[text.index("int mine = group"):]
+    assert re.search(r"for \(int k = mine  k < steps \+ mine  k \+= 2", loop) and re.search(r"mine \^= steps & 1;", loop)
+    assert "a.add(group, R.a_stages)" in text and "a.add(2, R.a_stages)" in loop and ".back(" not in text
+    assert "std::min(4, (512 - 2 * R.acc_cols) / 64)" in text.replace(" \n", " ")
