@@ -294,8 +294,8 @@ __device__ __forceinline__ void add_parts(const Mx4Job& J, const Mx4Walk& t, flo
 // With wide tiles what bounds one CTA is shared memory: of 128 bytes a clock, writing and reading the activations of 192 rows takes
 // 125 (2048 tokens of 14336 x 4096 317 us; without the loads 202).  Two CTAs therefore share a tile of 256 weight rows (PAIR): each
 // brings half of the activations, the first one's thread issues for both.  What is to arrive at the issuing thread comes from
-// both CTAs; what it releases goes to both.  2048 tokens of 14336 x 4096 167 us (1435 TFLOP/s; under the power limit 199), 32768 rows over 128
-// experts of 2048 x 768 117 (141).
+// both CTAs; what it releases goes to both.  2048 tokens of 14336 x 4096 171 us (1405 TFLOP/s; under the power limit 204), 32768 rows over 128
+// experts of 2048 x 768 117 (139).
 constexpr int G16_THREADS = 768, G16_W_STAGES = 3, G16_PRODUCERS = 8;
 
 struct Mx4Ring { int x_stages, box_rows, x_half, a_stages, acc_cols; };  // stages of x, rows per box, bytes of 64 values of a CTA's rows
