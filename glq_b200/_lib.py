@@ -33,7 +33,42 @@ EXPORTS = [
     "glqb_plan_set_comm",
     "glqb_mx4_quantize", "glqb_mx4_dequantize", "glqb_mx4_image_bytes", "glqb_mx4_pack", "glqb_mx4_workspace_bytes",
     "glqb_mx4_product", "glqb_mx4_status",
+    "glqb_rotary", "glqb_paged_append", "glqb_paged_attention_workspace_bytes", "glqb_paged_attention", "glqb_paged_status",
 ]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("pairs", C.c_int32), ("interleaved", C.c_int32), ("scale", C.c_float)]
+
+
+class PagedCacheDesc(C.Structure):
+    _fields_ = [
+        ("keys", C.c_void_p), ("values", C.c_void_p),
+        ("key_page", C.c_int64), ("key_row", C.c_int64), ("key_head", C.c_int64),
+        ("value_page", C.c_int64), ("value_row", C.c_int64), ("value_head", C.c_int64),
+        ("pages", C.c_int64), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [
+        ("key", C.c_void_p), ("value", C.c_void_p), ("query", C.c_void_p), ("query_out", C.c_void_p),
+        ("key_token", C.c_int64), ("key_head", C.c_int64), ("value_token", C.c_int64), ("value_head", C.c_int64),
+        ("query_token", C.c_int64), ("query_head", C.c_int64), ("query_out_token", C.c_int64), ("query_out_head", C.c_int64),
+        ("tokens", C.c_int64), ("slots", C.c_void_p), ("positions", C.c_void_p),
+        ("slots_are_int64", C.c_int32), ("positions_are_int64", C.c_int32), ("dtype", C.c_int32), ("heads", C.c_int32),
+    ]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [
+        ("query", C.c_void_p), ("out", C.c_void_p),
+        ("query_token", C.c_int64), ("query_head", C.c_int64), ("out_token", C.c_int64), ("out_head", C.c_int64),
+        ("tokens", C.c_int64), ("page_table", C.c_void_p), ("page_stride", C.c_int64), ("lengths", C.c_void_p), ("offsets", C.c_void_p),
+        ("lengths_are_int64", C.c_int32), ("offsets_are_int64", C.c_int32), ("sequences", C.c_int32), ("page_columns", C.c_int32),
+        ("heads", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("clear_rest", C.c_int32), ("max_query_len", C.c_int32),
+        ("scale", C.c_float),
+    ]
 
 
 class Mx4WeightDesc(C.Structure):
@@ -202,6 +237,16 @@ def load() -> C.CDLL:
     lib.glqb_mx4_product.restype = C.c_int
     lib.glqb_mx4_status.argtypes = [C.POINTER(i32)]
     lib.glqb_mx4_status.restype = C.c_int
+    lib.glqb_rotary.argtypes = [C.POINTER(RotaryDesc), vp, i32, i64, i64, vp, i64, i64, i64, i32, i32, vp, i32, vp]
+    lib.glqb_rotary.restype = C.c_int
+    lib.glqb_paged_append.argtypes = [C.POINTER(PagedCacheDesc), C.POINTER(PagedAppendDesc), C.POINTER(RotaryDesc), vp]
+    lib.glqb_paged_append.restype = C.c_int
+    lib.glqb_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedCacheDesc), C.POINTER(PagedAttentionDesc)]
+    lib.glqb_paged_attention_workspace_bytes.restype = sz
+    lib.glqb_paged_attention.argtypes = [C.POINTER(PagedCacheDesc), C.POINTER(PagedAttentionDesc), vp, sz, vp]
+    lib.glqb_paged_attention.restype = C.c_int
+    lib.glqb_paged_status.argtypes = [C.POINTER(i32)]
+    lib.glqb_paged_status.restype = C.c_int
     lib.glqb_last_error.argtypes = []
     lib.glqb_last_error.restype = C.c_char_p
     lib.glqb_version.argtypes = []

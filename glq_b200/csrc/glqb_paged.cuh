@@ -1,0 +1,222 @@
+// Attention over a paged cache: the job, how its work is shared out, and what its kernels have in common.
+#pragma once
+#include "glqb_internal.h"
+#include "glqb_ptx.cuh"
+#include "glqb_launch.h"
+#include <cuda.h>
+
+namespace glqb {
+
+constexpr int PA_PIECE = 64;         // most rows of a page that one copy brings
+constexpr int PA_STREAM_ROWS = 16, PA_STREAM_KEYS = 64;
+
+struct PagedJob {
+  const uint16_t* q;
+  void* out;
+  long long q_token, q_head, out_token, out_head;
+  const void *lengths, *offsets;
+  const int* pages;
+  long long page_stride;
+  int lengths_wide, offsets_wide, seqs, columns, page_log, tokens, heads, kv_heads, group, head_dim, causal, window, clear;
+  float scale_log2;                  // scale * log2(e): weights are powers of two
+  int most_keys;                     // columns * page size
+  int min_units;                     // key tiles that a CTA takes at least
+  bool out_wide;                     // rows of out lie on 8 bytes
+  float* part;                       // workspace: sums of items that several CTAs share, [CTA][2][rows][padded head_dim]
+  float2* part_ml;                   // their largest exponent and sum, [CTA][2][rows]
+  struct PagedPart* part_of;         // [CTA][2]
+  int* status;
+};
+// What a CTA left in the workspace: 0 the end, or the middle, of an item that another CTA began; 1 one that it began and did not end.
+struct PagedPart { int valid, ends, row0, rows, first, kv_head, queries, keys; };
+
+#ifdef __CUDACC__
+struct PagedSeq { int row0, queries, keys; };
+// Lengths and offsets are held to what there is, so that whatever they hold, nothing outside is read or written.
+__device__ __forceinline__ int pa_offset(const PagedJob& J, int i) {
+  if (!J.offsets) return min(i, J.tokens);
+  const long long o = J.offsets_wide ? reinterpret_cast<const long long*>(J.offsets)[i] : reinterpret_cast<const int*>(J.offsets)[i];
+  return (int)max(0ll, min((long long)J.tokens, o));
+}
+__device__ __forceinline__ PagedSeq pa_seq(const PagedJob& J, int i) {
+  PagedSeq s;
+  s.row0 = pa_offset(J, i);
+  s.queries = max(0, pa_offset(J, i + 1) - s.row0);
+  const long long n = J.lengths_wide ? reinterpret_cast<const long long*>(J.lengths)[i] : reinterpret_cast<const int*>(J.lengths)[i];
+  s.keys = (int)max(0ll, min((long long)J.most_keys, n));
+  return s;
+}
+// rows of an item are (query, head of the group) pairs, heads first
+__device__ __forceinline__ int pa_query(const PagedJob& J, int row) { return row / J.group; }
+// keys that query i sees: from .. to - 1
+__device__ __forceinline__ int pa_to(const PagedJob& J, const PagedSeq& s, int i) { return J.causal ? max(0, s.keys - s.queries + i + 1) : s.keys; }
+__device__ __forceinline__ int pa_from(const PagedJob& J, const PagedSeq& s, int i) {
+  return J.window ? max(0, s.keys - s.queries + i + 1 - J.window) : 0;
+}
+// An item: ROWS rows of one sequence and key head.  Its key tiles are [lo, hi): those that any of its rows sees, one at least, so that
+// every row is written.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int2 pa_tiles(const PagedJob& J, const PagedSeq& s, int qt) {
+  const int last = min(s.queries - 1, pa_query(J, min(s.queries * J.group, (qt + 1) * ROWS) - 1));
+  const int to = pa_to(J, s, last), from = min(pa_from(J, s, pa_query(J, qt * ROWS)), to);
+  const int lo = from / KEYS;
+  return make_int2(lo, max(lo + 1, (to + KEYS - 1) / KEYS));
+}
+template <int ROWS>
+__device__ __forceinline__ int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return (s.queries * J.group + ROWS - 1) / ROWS; }
+template <int ROWS, int KEYS>
+__device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq& s) {
+  const int n = pa_q_tiles<ROWS>(J, s);
+  long long sum = 0;
+  for (int qt = 0; qt < n; ++qt) {
+    const int2 t = pa_tiles<ROWS, KEYS>(J, s, qt);
+    sum += t.y - t.x;
+  }
+  return sum;
+}
+
+// Where a CTA's share of the work begins: item (seq, kv_head, q_tile), `skip` key tiles into it, `units` key tiles in all.
+struct PagedStart {
+  int seq, kv_head, q_tile, skip;
+  long long units;
+  long long warp_sum[32];
+};
+// The work is one list of key tiles: sequence after sequence, of each one key head after another, of each one row tile after another;
+// every CTA takes an equal run of it.  So batches of any lengths keep all SMs busy, and an item is cut only where a run ends.  Every
+// CTA counts the list itself: a thread some sequences, then a scan.  Called by all threads; ends with a block barrier.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
+  const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (J.seqs + threads - 1) / threads, first = min(J.seqs, (int)threadIdx.x * per), last = min(J.seqs, first + per);
+  long long own = 0;
+  for (int i = first; i < last; ++i) own += pa_units<ROWS, KEYS>(J, pa_seq(J, i)) * J.kv_heads;
+  long long sum = own;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long u = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+    if (lane >= d) sum += u;
+  }
+  if (lane == 31) S.warp_sum[warp] = sum;
+  if (threadIdx.x == 0) S.units = 0;
+  __syncthreads();
+  long long before = sum - own, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) before += S.warp_sum[w];
+    total += S.warp_sum[w];
+  }
+  const long long ctas = min((long long)gridDim.x, (total + J.min_units - 1) / J.min_units);
+  if ((long long)blockIdx.x < ctas) {
+    const long long begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+    if (begin >= before && begin < before + own) {
+      long long r = begin - before;
+      for (int i = first; i < last; ++i) {
+        const PagedSeq s = pa_seq(J, i);
+        const long long per_head = pa_units<ROWS, KEYS>(J, s);
+        if (r >= per_head * J.kv_heads) { r -= per_head * J.kv_heads; continue; }
+        S.seq = i;
+        S.kv_head = (int)(r / per_head);
+        r -= S.kv_head * per_head;
+        int qt = 0;
+        for (;; ++qt) {
+          const int2 t = pa_tiles<ROWS, KEYS>(J, s, qt);
+          if (r < t.y - t.x) break;
+          r -= t.y - t.x;
+        }
+        S.q_tile = qt;
+        S.skip = (int)r;
+        S.units = end - begin;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// A CTA's items one after the other, as its loading warp hands them to the others.
+struct PagedItem {
+  int more;                          // 0: no item, the CTA is done
+  int row0, queries, keys;           // the sequence
+  int seq, kv_head, first;           // first row of the item within the sequence's queries * group
+  int rows;                          // of it
+  int lo, hi;                        // key tiles of this CTA
+  int slot;                          // -1: the whole item; else its place in the workspace
+};
+template <int ROWS, int KEYS>
+struct PagedWalk {
+  PagedSeq s;
+  int seq, kv_head, qt, skip, q_tiles;
+  long long left;
+  PagedPart part[2];                 // what the CTA leaves in the workspace
+  __device__ __forceinline__ PagedWalk(const PagedJob& J, const PagedStart& S)
+      : seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(0), left(S.units) {
+    part[0] = part[1] = PagedPart{0, 1, 0, 0, 0, 0, 0, 0};
+    if (left > 0) { s = pa_seq(J, seq); q_tiles = pa_q_tiles<ROWS>(J, s); }
+  }
+  __device__ __forceinline__ PagedItem next(const PagedJob& J) {
+    PagedItem it{};
+    if (left <= 0) return it;
+    const int2 t = pa_tiles<ROWS, KEYS>(J, s, qt);
+    const int n = t.y - t.x, take = (int)min((long long)(n - skip), left);
+    it.more = 1;
+    it.row0 = s.row0;
+    it.queries = s.queries;
+    it.keys = s.keys;
+    it.seq = seq;
+    it.kv_head = kv_head;
+    it.first = qt * ROWS;
+    it.rows = min(ROWS, s.queries * J.group - it.first);
+    it.lo = t.x + skip;
+    it.hi = it.lo + take;
+    it.slot = take == n ? -1 : skip ? 0 : 1;
+    if (it.slot >= 0) part[it.slot] = PagedPart{1, skip + take == n, s.row0, it.rows, it.first, kv_head, s.queries, s.keys};
+    left -= take;
+    skip = 0;
+    if (++qt == q_tiles) {
+      qt = 0;
+      if (++kv_head == J.kv_heads) {
+        kv_head = 0;
+        if (left > 0) {
+          do { s = pa_seq(J, ++seq); } while (s.queries == 0 && seq + 1 < J.seqs);
+          q_tiles = pa_q_tiles<ROWS>(J, s);
+        }
+      }
+    }
+    return it;
+  }
+};
+__device__ __forceinline__ void pa_publish(const PagedJob& J, const PagedPart (&part)[2]) {
+  J.part_of[2 * blockIdx.x] = part[0];
+  J.part_of[2 * blockIdx.x + 1] = part[1];
+}
+
+// `rows` rows (PA_PIECE at most) x 64 values of one head of a page: coordinates (value, head, row, page)
+__device__ __forceinline__ void pa_load(void* dst, const CUtensorMap* map, int x, int head, int row, int page, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                   smem_u32(dst)),
+               "l"(map), "r"(x), "r"(head), "r"(row), "r"(page), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pa_pack(float a, float b) {
+  if constexpr (__is_same(T, __half)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// has one of two 16-bit values no finite value?
+template <typename T>
+__device__ __forceinline__ bool pa_not_finite(uint32_t two) {
+  constexpr uint32_t E = __is_same(T, __half) ? 0x7C00u : 0x7F80u;
+  return (two & E) == E || (two >> 16 & E) == E;
+}
+#endif  // __CUDACC__
+
+}  // namespace glqb

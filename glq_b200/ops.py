@@ -23,6 +23,7 @@ import torch
 from . import _lib
 from .mx4 import (Mx4Tensor, Mx4Weight, mx4_check_status, mx4_dequantize, mx4_grouped_linear, mx4_linear,  # noqa: F401
                   mx4_pack, mx4_quantize)
+from .paged import Rotary, paged_append, paged_attention, paged_check_status, rotary, rotary_table  # noqa: F401
 from .plan import LinearSpec, Plan, block_decompose
 
 DECODE_MAX_TOKENS = 64
@@ -142,6 +143,7 @@ def check_device_status() -> None:
         if hasattr(p, "check_status"):
             p.check_status()
     mx4_check_status()
+    paged_check_status()
 
 
 def clear_caches() -> None:

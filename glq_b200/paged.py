@@ -1,0 +1,327 @@
+"""Between a decoder's q/k/v and output projections: rotary positions, a paged cache of keys and values, attention over it.
+
+``rotary_table`` holds the frequencies of a model's rotary positions; ``rotary`` rotates heads by them, ``paged_append`` puts new keys
+(rotated on the way) and values into a paged cache and rotates their queries in the same launch, ``paged_attention`` lets queries, one of a
+sequence or a chunk of many, attend to what the cache holds.  A cache is a pair of tensors (pages, page_size, kv_heads, head_dim) of
+bf16 or fp16, in any order of strides with a head's values one behind the other; a page's number is its place in the first dimension.  The
+operators run on the current stream of their tensors' device, take a workspace from torch's allocator where they need one, read
+nothing back and can be captured into a CUDA graph.  They have no gradients.  No counterpart in the reference, which leaves attention to the
+framework that serves the model.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .mx4 import _call, _cuda, _dtype, _overlap, _same_device
+
+_RAN_ON: set = set()                # devices whose status word a call may have set
+_INTEGERS = (torch.int32, torch.int64)
+
+
+class Rotary:
+    """Frequencies of rotary positions (``rotary_table``): ``turns`` int64 (pairs,) on the device, the fraction of a turn that a pair makes per
+    position in units of 2^-64; ``scale`` on cosine and sine; ``interleaved``: neighbouring values make a pair, else values half of the
+    rotated part apart.  The attributes cannot be set."""
+    __slots__ = ("turns", "scale", "interleaved", "_desc", "_ref", "_index")
+
+    def __init__(self, turns, scale=1.0, interleaved=False):
+        _cuda(turns, "turns")
+        if turns.dtype != torch.int64 or turns.dim() != 1 or not turns.numel() or not turns.is_contiguous():
+            raise ValueError(f"glq_b200: turns must be int64 (pairs,), got {tuple(turns.shape)} of {turns.dtype}")
+        desc = _lib.RotaryDesc(turns.data_ptr(), turns.numel(), bool(interleaved), float(scale))
+        for name, value in zip(self.__slots__, (turns, float(scale), bool(interleaved), desc, C.byref(desc), turns.get_device())):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"glq_b200: {name} of a rotary table cannot be set")
+
+    @property
+    def dim(self) -> int:
+        """Values of a head that are rotated."""
+        return 2 * self.turns.numel()
+
+
+def _frequencies(dim, base, scaling):
+    """(radians per position of every pair, scale on cosine and sine), in 64 bits on the host."""
+    f = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if scaling is None:
+        return f, 1.0
+    kind = scaling.get("rope_type", scaling.get("type"))
+
+    def need(key):
+        if key not in scaling:
+            raise ValueError(f"glq_b200: {kind!r} rotary scaling needs {key!r}")
+        return scaling[key]
+
+    if kind == "default":
+        return f, 1.0
+    if kind not in ("linear", "llama3", "yarn"):
+        raise ValueError(f'glq_b200: rotary scaling is "linear", "llama3" or "yarn", not {kind!r}')
+    factor = float(need("factor"))
+    if kind == "linear":
+        return f / factor, 1.0
+    old = float(need("original_max_position_embeddings"))
+    if kind == "llama3":
+        # pairs that turn at least `high` times within the old context stay, those of at most `low` turns are stretched
+        low, high = float(need("low_freq_factor")), float(need("high_freq_factor"))
+        keep = ((old * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        return f / factor * (1 - keep) + f * keep, 1.0
+
+    def magnitude(mscale):
+        return 0.1 * mscale * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+    def pair(turns):          # the pair that makes so many turns within the old context
+        return dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    lo, hi = pair(float(scaling.get("beta_fast") or 32.0)), pair(float(scaling.get("beta_slow") or 1.0))
+    if scaling.get("truncate", True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, dim - 1)
+    stretched = ((torch.arange(dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+    scale = scaling.get("attention_factor")
+    if scale is None:
+        if scaling.get("mscale") and scaling.get("mscale_all_dim"):
+            scale = magnitude(scaling["mscale"]) / magnitude(scaling["mscale_all_dim"])
+        else:
+            scale = magnitude(1.0)
+    return f / factor * stretched + f * (1 - stretched), float(scale)
+
+
+def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv_freq=None, scale=None, device=None) -> Rotary:
+    """Frequencies base^(-2 i / dim) of ``dim`` rotated values (even), made once for a model.  ``scaling``: a dict as model
+    configurations hold it, "rope_type" "linear", "llama3" or "yarn" with its factors.  ``inv_freq``: radians per position of every pair, in
+    place of dim, base and scaling.  ``scale``: factor on cosine and sine in place of the scaling's own.  Frequencies are held in 64
+    bits: angles are exact to position * 2^-53 of the frequency given."""
+    own = 1.0
+    if inv_freq is not None:
+        if dim is not None and dim != 2 * inv_freq.numel() or scaling is not None:
+            raise ValueError("glq_b200: inv_freq comes in place of dim, base and scaling")
+        f = inv_freq.detach().to("cpu", torch.float64).reshape(-1)
+    else:
+        if dim is None or dim < 2 or dim % 2:
+            raise ValueError(f"glq_b200: an even number of values is rotated, not {dim}")
+        f, own = _frequencies(dim, base, scaling)
+    if not f.numel() or not bool(torch.isfinite(f).all()):
+        raise ValueError("glq_b200: frequencies must be finite")
+    # fractions of a turn in 2^-64, as signed integers (whole turns per position make no difference at whole positions)
+    whole = [int(math.ldexp(p, 64)) for p in ((f / (2 * math.pi)) % 1.0).tolist()]
+    turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in whole], dtype=torch.int64)
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise RuntimeError("glq_b200: a rotary table is used on a CUDA device (there is no CPU path)")
+    return Rotary(turns.to(device), own if scale is None else scale, interleaved)
+
+
+def _heads(x, name):
+    """x (tokens, heads, head_dim) with a head's values one behind the other."""
+    _cuda(x, name)
+    if x.dim() != 3:
+        raise ValueError(f"glq_b200: {name} is (tokens, heads, head_dim), got {tuple(x.shape)}")
+    return x if x.stride(2) == 1 or x.shape[2] <= 1 else x.contiguous()
+
+
+def _target(out, like, name):
+    """A given result: the shape, type and device of ``like``, no two values in one place."""
+    _same_device(out, like, name)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"glq_b200: {name} must be {tuple(like.shape)} of {like.dtype}, got {tuple(out.shape)} of {out.dtype}")
+    t, h, d = out.shape
+    (a, m), (b, n) = sorted(((out.stride(0), t), (out.stride(1), h)))
+    if d > 1 and out.stride(2) != 1 or m > 1 and a < d or n > 1 and b < d or m > 1 and n > 1 and b < a * (m - 1) + d:
+        raise ValueError(f"glq_b200: {name} needs a head's values one behind the other and rows that do not overlap, got strides {tuple(out.stride())}")
+
+
+def _result(x, out, name):
+    """Where the rotated x goes: a new tensor, or ``out``, which is x itself or lies apart from it."""
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _target(out, x, name)
+    if out.numel() and _overlap(x, out) and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+        raise ValueError(f"glq_b200: {name} overlaps its input without being it")
+    return out
+
+
+def _integers(t, x, name, count):
+    _same_device(t, x, name)
+    if t.dtype not in _INTEGERS or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+        raise ValueError(f"glq_b200: {name} must be {count} int32 or int64 values, got {tuple(t.shape)} of {t.dtype}")
+    return t.dtype is torch.int64
+
+
+def _check_table(table, x, head_dim):
+    if table.__class__ is not Rotary:
+        raise ValueError("glq_b200: table is what rotary_table returns")
+    if table._index != x.get_device():
+        raise ValueError(f"glq_b200: the rotary table is on {table.turns.device}, expected {x.device}")
+    if table.dim > head_dim:
+        raise ValueError(f"glq_b200: {table.dim} rotated values in heads of {head_dim}")
+
+
+def rotary(x, positions, table: Rotary, *, out=None) -> torch.Tensor:
+    """x (tokens, heads, head_dim) of bf16, fp16 or fp32 with the first ``table.dim`` values of every head rotated by its token's
+    position (int32 or int64, (tokens,); negative ones rotate back), computed in fp32 and rounded once; the other values as they are.
+    ``out``: where the result goes, x itself too."""
+    src = _heads(x, "x")
+    dt = _dtype(src.dtype, "x")
+    tokens, heads, dim = src.shape
+    _check_table(table, src, dim)
+    wide = _integers(positions, src, "positions", tokens)
+    out = _result(src, out, "out")
+    if tokens and heads:
+        _call(table._index, "rotary", _lib.load().glqb_rotary, table._ref, src.data_ptr(), dt, src.stride(0), src.stride(1), out.data_ptr(),
+              out.stride(0), out.stride(1), tokens, heads, dim, positions.data_ptr(), wide)
+    return out
+
+
+def _cache(keys, values):
+    """The C description of a cache, checked."""
+    _cuda(keys, "key_cache")
+    _same_device(values, keys, "value_cache")
+    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype:
+        raise ValueError(f"glq_b200: key_cache and value_cache are (pages, page_size, kv_heads, head_dim) of one type, got {tuple(keys.shape)} of {keys.dtype} and "
+                         f"{tuple(values.shape)} of {values.dtype}")
+    if keys.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"glq_b200: a cache is bf16 or fp16, not {keys.dtype}")
+    pages, size, heads, dim = keys.shape
+    if pages < 1 or heads < 1 or dim < 8 or dim > 128 or dim % 8 or size < 8 or size & (size - 1):
+        raise ValueError(f"glq_b200: a cache of {tuple(keys.shape)}: pages of a power of two rows, 8 at least, heads of a multiple of 8 values, 128 at most")
+    strides = []
+    for name, t in (("key_cache", keys), ("value_cache", values)):
+        s = t.stride()
+        if s[3] != 1 or t.data_ptr() & 15 or (s[0] & 7 and pages > 1) or s[1] & 7 or (s[2] & 7 and heads > 1):
+            raise ValueError(f"glq_b200: {name} must lie on 16 bytes, strides of 8 values, a head's values one behind the other; got strides {s}")
+        strides.append((s[0] if pages > 1 else 0, s[1], s[2] if heads > 1 else 0))
+    (kp, kr, kh), (vp, vr, vh) = strides
+    return _lib.PagedCacheDesc(keys.data_ptr(), values.data_ptr(), kp, kr, kh, vp, vr, vh, pages, size, heads, dim, _dtype(keys.dtype, "the cache"))
+
+
+def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, table: Optional[Rotary] = None, query=None, out=None):
+    """Puts the keys and values (tokens, kv_heads, head_dim) of new tokens into the cache, in place: token t's into row ``slots[t]`` =
+    page * page_size + row (int32 or int64); a slot outside the cache, -1 for one, leaves the cache alone, as for tokens that pad a batch.
+    The slots within the cache are all different.  With ``table`` and ``positions`` (tokens,) the keys are rotated on the way, and so is ``query``
+    (tokens, heads, head_dim) if it is given: to a new tensor or to ``out`` (the query itself too), which is returned.  Keys, values and
+    queries are of the cache's type, or fp32."""
+    desc = _cache(key_cache, value_cache)
+    key, value = _heads(key, "key"), _heads(value, "value")
+    _same_device(key, key_cache, "key")
+    _same_device(value, key, "value")
+    tokens = key.shape[0]
+    if key.shape != value.shape or key.shape[1:] != key_cache.shape[2:]:
+        raise ValueError(f"glq_b200: keys of {tuple(key.shape)} and values of {tuple(value.shape)} for a cache of {tuple(key_cache.shape)}")
+    if key.dtype != value.dtype or key.dtype not in (key_cache.dtype, torch.float32):
+        raise ValueError(f"glq_b200: keys and values are of the cache's type, {key_cache.dtype}, or fp32, got {key.dtype} and {value.dtype}")
+    slots_wide, positions_wide = _integers(slots, key, "slots", tokens), False
+    if (table is None) != (positions is None):
+        raise ValueError("glq_b200: table and positions come together")
+    if table is not None:
+        _check_table(table, key, key.shape[2])
+        positions_wide = _integers(positions, key, "positions", tokens)
+    if query is None:
+        if out is not None:
+            raise ValueError("glq_b200: out belongs to query")
+    else:
+        if table is None:
+            raise ValueError("glq_b200: query is here to be rotated: table and positions are needed")
+        query = _heads(query, "query")
+        _same_device(query, key, "query")
+        if query.shape[0] != tokens or query.shape[2] != key.shape[2] or query.dtype != key.dtype:
+            raise ValueError(f"glq_b200: queries of {tuple(query.shape)}, {query.dtype}, beside keys of {tuple(key.shape)}, {key.dtype}")
+        out = _result(query, out, "out")
+    for name, t in (("key", key), ("value", value), ("query", query), ("out", out)):
+        if t is not None and t.numel() and (_overlap(t, key_cache) or _overlap(t, value_cache)):
+            raise ValueError(f"glq_b200: {name} overlaps the cache")
+    for name, t in (("key", key), ("value", value)):
+        if out is not None and t.numel() and out.numel() and out is not query and _overlap(t, out):
+            raise ValueError(f"glq_b200: out overlaps {name}")
+    if tokens:
+        a = _lib.PagedAppendDesc(key.data_ptr(), value.data_ptr(), query.data_ptr() if query is not None else None, out.data_ptr() if out is not None else None,
+                                 key.stride(0), key.stride(1), value.stride(0), value.stride(1), *((query.stride(0), query.stride(1), out.stride(0), out.stride(1)) if query is not None else (0, 0, 0, 0)),
+                                 tokens, slots.data_ptr(), positions.data_ptr() if positions is not None else None, slots_wide, positions_wide, _dtype(key.dtype, "key"),
+                                 query.shape[1] if query is not None else 0)
+        _call(key.get_device(), "paged_append", _lib.load().glqb_paged_append, C.byref(desc), C.byref(a), table._ref if table is not None else None)
+    return out
+
+
+def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offsets=None, max_query_len=None, scale=None, causal=True, window=0, out=None):
+    """Attention of the newest tokens of every sequence over a paged cache that holds their keys and values already.
+
+    ``query`` (tokens, heads, head_dim) of the cache's type, the heads a multiple of the cache's: query head h reads key head
+    h // (heads // kv_heads).  ``lengths`` (sequences,): keys of every sequence, those of the new tokens among them, in the pages that
+    ``pages`` (sequences, columns) int32 names in order.  ``query_offsets`` (sequences + 1,): rows query_offsets[s] .. query_offsets[s + 1] - 1 are
+    the last ones of sequence s, ascending; None: one row per sequence.  A query sees the keys up to its own (``causal``, else all of its
+    sequence), of them the last ``window`` ones (0: all).  ``scale`` (positive): of the scores, head_dim ** -0.5 by default.
+    ``max_query_len``: what no sequence has more rows than, if the program knows it; the faster kernel is chosen by it.
+    Integers are int32 or int64 and stay on the device: lengths are held to 0 .. columns * page_size, offsets to 0 .. tokens; a page
+    outside the cache reads as zeros.  Rows that see no key are zero.  Rows of no sequence (in front of query_offsets[0], behind the last) are zero in a
+    new result and stay as they are in a given ``out``.  Sums and softmax in fp32, weights rounded to the cache's type for the product with the values, as
+    is the result; what lies in the cache where no query looks, NaN included, changes nothing.  The same call gives the same bits."""
+    desc = _cache(key_cache, value_cache)
+    query = _heads(query, "query")
+    _same_device(query, key_cache, "query")
+    tokens, heads, dim = query.shape
+    kv_heads = key_cache.shape[2]
+    if dim != key_cache.shape[3] or query.dtype != key_cache.dtype or heads < 1 or heads % kv_heads:
+        raise ValueError(f"glq_b200: queries of {tuple(query.shape)}, {query.dtype}, over a cache of {tuple(key_cache.shape)}, {key_cache.dtype}")
+    _same_device(pages, query, "pages")
+    if pages.dtype != torch.int32 or pages.dim() != 2 or (pages.shape[1] > 1 and pages.stride(1) != 1):
+        raise ValueError(f"glq_b200: pages must be int32 (sequences, columns), a row's entries one behind the other, got {tuple(pages.shape)} of {pages.dtype}")
+    seqs = pages.shape[0]
+    lengths_wide, offsets_wide = _integers(lengths, query, "lengths", seqs), False
+    if query_offsets is not None:
+        offsets_wide = _integers(query_offsets, query, "query_offsets", seqs + 1)
+    elif tokens != seqs:
+        raise ValueError(f"glq_b200: {tokens} queries of {seqs} sequences need query_offsets")
+    if max_query_len is None:
+        max_query_len = tokens if query_offsets is not None else 1
+    elif max_query_len < 0:
+        raise ValueError(f"glq_b200: max_query_len is {max_query_len}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"glq_b200: scale is a positive number, not {scale}")
+    window = int(window or 0)
+    if not 0 <= window < 2 ** 31:
+        raise ValueError(f"glq_b200: a window of {window} keys")
+    fresh = out is None
+    if fresh:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    else:
+        _target(out, query, "out")
+        if tokens and (_overlap(out, query) or _overlap(out, key_cache) or _overlap(out, value_cache)):
+            raise ValueError("glq_b200: out overlaps the queries or the cache")
+    if tokens:
+        if query.data_ptr() & 15 or query.stride(0) & 7 or query.stride(1) & 7:
+            query = query.clone(memory_format=torch.contiguous_format)
+        a = _lib.PagedAttentionDesc(query.data_ptr(), out.data_ptr(), query.stride(0), query.stride(1), out.stride(0), out.stride(1), tokens, pages.data_ptr(),
+                                    pages.stride(0), lengths.data_ptr(), query_offsets.data_ptr() if query_offsets is not None else None, lengths_wide,
+                                    offsets_wide, seqs, pages.shape[1], heads, bool(causal), window, fresh and query_offsets is not None, min(max_query_len, tokens), scale)
+        lib, index = _lib.load(), query.get_device()
+        size = _workspace(lib, index, desc, a)
+        ws = query.new_empty((size,), dtype=torch.uint8)
+        _call(index, "paged_attention", lib.glqb_paged_attention, C.byref(desc), C.byref(a), ws.data_ptr(), size)
+        _RAN_ON.add(index)
+    return out
+
+
+def _workspace(lib, index, desc, a):
+    """Bytes of workspace of a call; 0 from the library is a refusal, which the call itself words."""
+    cuda = torch._C
+    before = cuda._cuda_getDevice()
+    if before == index:
+        return lib.glqb_paged_attention_workspace_bytes(C.byref(desc), C.byref(a))
+    cuda._cuda_setDevice(index)
+    try:
+        return lib.glqb_paged_attention_workspace_bytes(C.byref(desc), C.byref(a))
+    finally:
+        cuda._cuda_setDevice(before)
+
+
+def paged_check_status() -> None:
+    """Synchronise the devices that attention ran on and raise RuntimeError (code GLQB_E_DEVICE) if a bounded wait in it gave up since
+    the last call: the results of that run are invalid."""
+    for index in sorted(_RAN_ON):
+        _call(index, "paged status", lambda stream: _lib.load().glqb_paged_status(None))

@@ -344,6 +344,71 @@ int glqb_mx4_product(const GlqbMx4Weight* w, const void* x, int32_t x_dtype, int
 /* Synchronising read of the current device's status word, which it clears: GLQB_E_DEVICE if a wait gave up since the last. */
 int glqb_mx4_status(int32_t* status_out);
 
+/*
+ * What lies between a decoder's q/k/v and output projections: rotary positions, a paged cache of keys and values, attention over it.
+ * No counterpart in the reference.  All entry points enqueue on `stream` and neither allocate nor synchronise, unless stated.
+ * Strides are counted in values; the values of a head lie one behind the other.
+ */
+
+/* Rotation of head values by a token's position: of the first 2 * pairs values of a head, values i and i + pairs (or 2 i and 2 i + 1:
+ * interleaved) make a pair, (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t) with t = 2 pi * position * turns[i] / 2^64.
+ * turns: device, one per pair, fractions of a turn per position as 64-bit integers: products wrap where whole turns do, so that
+ * the angle of any position is off by no more than position * 2^-65 turns.  The other values of a head stay as they are. */
+typedef struct GlqbRotary {
+  const int64_t* turns;
+  int32_t pairs, interleaved;
+  float scale;
+} GlqbRotary;
+/* `heads` heads of `tokens` tokens, x to out (out may be x with x's strides).  positions: device, one per token, int32 or int64. */
+int glqb_rotary(const GlqbRotary* r, const void* x, int32_t dtype, int64_t x_token, int64_t x_head, void* out, int64_t out_token, int64_t out_head,
+                int64_t tokens, int32_t heads, int32_t head_dim, const void* positions, int32_t positions_are_int64, void* stream);
+
+/* A cache of keys and values: `pages` pages of page_size rows (a power of two, 8 at least) of kv_heads heads, fp16 or bf16.  Addresses
+ * lie on 16 bytes, strides are multiples of 8 values, head_dim is a multiple of 8, 128 at most. */
+typedef struct GlqbPagedCache {
+  void *keys, *values;
+  int64_t key_page, key_row, key_head, value_page, value_row, value_head;
+  int64_t pages;
+  int32_t page_size, kv_heads, head_dim, dtype;
+} GlqbPagedCache;
+
+/* key and value (tokens, kv_heads, head_dim), fp32 or of the cache's type, into rows slots[t] (page * page_size + row) of the cache; a slot
+ * outside the cache, as a padding token's is, leaves it alone.  Slots within the cache are all different.  r: null, or the rotation of
+ * keys, and of `heads` heads of query to query_out (same type as key; query NULL: none), by positions. */
+typedef struct GlqbPagedAppend {
+  const void *key, *value, *query;
+  void* query_out;
+  int64_t key_token, key_head, value_token, value_head, query_token, query_head, query_out_token, query_out_head;
+  int64_t tokens;
+  const void *slots, *positions;
+  int32_t slots_are_int64, positions_are_int64, dtype, heads;
+} GlqbPagedAppend;
+int glqb_paged_append(const GlqbPagedCache* c, const GlqbPagedAppend* a, const GlqbRotary* r, void* stream);
+
+/* Attention of new tokens over a paged cache that holds their keys already.  Sequence s has lengths[s] keys, in the pages that row s of
+ * page_table (int32, page_stride apart, page_columns of them) names in order, and the queries offsets[s] .. offsets[s + 1] - 1
+ * (offsets NULL: one per sequence); the last query belongs to the last key.  A query sees the keys up to its own (causal; else all), of them
+ * the last `window` (0: all).  heads / kv_heads query heads share a key head.  out = softmax(scale * q k) v, rows without a visible key
+ * are zero.  All of this is read on the device: lengths are held to 0 .. page_columns * page_size, offsets to 0 .. tokens; a page outside
+ * the cache reads as zeros.  Rows of no sequence keep what out holds, or are zeroed with clear_rest.
+ * max_query_len: no sequence has more queries (a bound for the choice of the kernel; results do not depend on its truth).
+ * sequences up to 2^20, tokens * heads below 2^30, page_columns * page_size up to 2^30. */
+typedef struct GlqbPagedAttention {
+  const void* query;
+  void* out;
+  int64_t query_token, query_head, out_token, out_head;
+  int64_t tokens;
+  const int32_t* page_table;
+  int64_t page_stride;
+  const void *lengths, *offsets;
+  int32_t lengths_are_int64, offsets_are_int64, sequences, page_columns, heads, causal, window, clear_rest, max_query_len;
+  float scale;
+} GlqbPagedAttention;
+size_t glqb_paged_attention_workspace_bytes(const GlqbPagedCache* c, const GlqbPagedAttention* a);
+int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, void* workspace, size_t workspace_bytes, void* stream);
+/* Synchronising read of the current device's status word, which it clears: GLQB_E_DEVICE if a bounded wait gave up since the last. */
+int glqb_paged_status(int32_t* status_out);
+
 const char* glqb_last_error(void);
 const char* glqb_version(void);
 

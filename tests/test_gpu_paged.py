@@ -1,0 +1,438 @@
+"""Rotary positions, appending to a paged cache and attention over it on the GPU, against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import paged_oracle as O
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def nothing_gave_up():
+    yield
+    from glq_b200 import ops
+    ops.paged_check_status()
+
+
+def _gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *shape, dtype=BF):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def _close(y, ref, bound, what=""):
+    """Within the bound, and not a number exactly where the definition has none."""
+    y = y.double().cpu()
+    assert torch.equal(y.isnan(), ref.isnan()) and not y.isinf().any(), what
+    err = ((y - ref).abs() - bound).nan_to_num(0.0)
+    assert float(err.max()) <= 0, (what, float(err.max()), int(err.argmax()))
+
+
+def _freq(dim, base=10000.0):
+    return base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+
+
+# ---- rotary -------------------------------------------------------------------------------------------------------
+U = {BF: 2.0 ** -8, HF: 2.0 ** -11, F32: 2.0 ** -24}
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("tokens,heads,dim,rot", [(1, 20, 128, 128), (3, 5, 64, 32), (257, 3, 80, 40), (33, 2, 96, 24), (7, 1, 66, 30), (5000, 1, 8, 2), (2, 300, 256, 256)])
+def test_rotary(dtype, interleaved, tokens, heads, dim, rot):
+    from glq_b200 import ops
+    g = _gen(tokens + dim)
+    x = _randn(g, tokens, heads, dim, dtype=dtype)
+    pos = torch.randint(0, 1_000_000, (tokens,), generator=g, device="cuda")
+    pos = pos if tokens % 2 else pos.to(torch.int32)
+    y = ops.rotary(x, pos, ops.rotary_table(rot, interleaved=interleaved, scale=1.25))
+    ref, mag = O.rotate(x, pos, _freq(rot), 1.25, interleaved)
+    assert y.shape == x.shape and y.dtype == dtype
+    _close(y, ref, mag + (ref.abs() + mag) * U[dtype])
+    assert torch.equal(y[..., rot:], x[..., rot:])
+
+
+def test_rotary_far_positions_and_back():
+    from glq_b200 import ops
+    x = _randn(_gen(), 6, 4, 128, dtype=F32)
+    table = ops.rotary_table(128, base=5e6)
+    pos = torch.tensor([0, 1, 2 ** 24 + 1, 2 ** 31 - 1, 2 ** 40 + 12345, -7], device="cuda")
+    y = ops.rotary(x, pos, table)
+    # (a frequency in 64 bits is off by 2^-53 of itself: at 2^40 by 2^-13 turns; the reference takes the table's own turns)
+    ref = x.double().cpu().clone()
+    for i, t in enumerate(table.turns.cpu().tolist()):
+        for r, p in enumerate(pos.cpu().tolist()):
+            part = (t * p) % 2 ** 64
+            a = 2 * math.pi * (part - 2 ** 64 if part >= 2 ** 63 else part) / 2 ** 64
+            u, v = x[r, :, i].double().cpu(), x[r, :, i + 64].double().cpu()
+            ref[r, :, i], ref[r, :, i + 64] = u * math.cos(a) - v * math.sin(a), v * math.cos(a) + u * math.sin(a)
+    mag = (x.double().cpu()[..., :64].abs() + x.double().cpu()[..., 64:].abs()).repeat(1, 1, 2)
+    _close(y, ref, mag * 2.0 ** -20)
+    assert torch.equal(y[0], x[0])
+    _close(ops.rotary(y, -pos, table), x.double().cpu(), mag * 2.0 ** -18)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("off,width", [(0, 512), (64, 640), (1, 513), (3, 700)])
+def test_rotary_strides_alignment_and_in_place(dtype, off, width):
+    from glq_b200 import ops
+    g = _gen(off)
+    buf = _randn(g, 50, width, dtype=dtype)
+    x = torch.as_strided(buf.flatten()[off:], (49, 4, 96), (width, 128, 1))       # heads apart, rows of a wider matrix
+    pos, table = torch.arange(49, device="cuda"), ops.rotary_table(64)
+    want = ops.rotary(x.contiguous(), pos, table)
+    assert torch.equal(ops.rotary(x, pos, table), want)
+    out = torch.full_like(buf, 7.0)
+    into = torch.as_strided(out.flatten()[off:], x.shape, x.stride())
+    assert ops.rotary(x, pos, table, out=into) is into and torch.equal(into, want)
+    into.fill_(7.0)
+    assert bool((out == 7.0).all())                                               # nothing beside the rows was written
+    assert torch.equal(ops.rotary(x, pos, table, out=x), want) and torch.equal(x, want)
+    assert torch.equal(ops.rotary(x.transpose(1, 2).contiguous().transpose(1, 2), pos, table), ops.rotary(x, pos, table))
+
+
+# ---- append -------------------------------------------------------------------------------------------------------
+def _caches(g, pages, size, kv, dim, dtype, layout="rows"):
+    """A pair of caches: rows (pages, size, kv, dim), or heads first within a page, or both in one tensor."""
+    if layout == "rows":
+        return _randn(g, pages, size, kv, dim, dtype=dtype), _randn(g, pages, size, kv, dim, dtype=dtype)
+    if layout == "heads":
+        return tuple(_randn(g, pages, kv, size, dim, dtype=dtype).transpose(1, 2) for _ in range(2))
+    both = _randn(g, pages, 2, size, kv, dim + 8, dtype=dtype)
+    return both[:, 0, ..., :dim], both[:, 1, ..., :dim]
+
+
+@pytest.mark.parametrize("layout", ["rows", "heads", "both"])
+@pytest.mark.parametrize("source", ["own", "fp32"])
+@pytest.mark.parametrize("dtype,tokens,heads,kv,dim,size,rot", [(BF, 1, 16, 4, 128, 16, 128), (HF, 300, 6, 2, 64, 8, 32), (BF, 37, 5, 1, 72, 32, 36), (HF, 6000, 2, 2, 16, 64, 16)])
+def test_append(layout, source, dtype, tokens, heads, kv, dim, size, rot):
+    from glq_b200 import ops
+    g, kind = _gen(tokens), dtype if source == "own" else F32
+    pages = -(-tokens // size) + 5
+    keys, values = _caches(g, pages, size, kv, dim, dtype, layout)
+    before = keys.clone(), values.clone()
+    merged = _randn(g, tokens, (heads + 2 * kv) * dim, dtype=kind)                 # a q/k/v projection's result
+    q, k, v = (t.view(tokens, -1, dim) for t in merged.split([heads * dim, kv * dim, kv * dim], 1))
+    slots = torch.randperm(pages * size, generator=g, device="cuda")[:tokens]
+    slots[1::7] = -1
+    slots[2::11] = pages * size + 3
+    if tokens > 1:
+        slots[-1] = pages * size
+    slots = slots.to(torch.int32) if tokens % 2 else slots
+    pos, table = torch.randint(0, 100000, (tokens,), generator=g, device="cuda"), ops.rotary_table(rot, interleaved=layout == "heads")
+    y = ops.paged_append(k, v, keys, values, slots, positions=pos, table=table, query=q)
+    rk = ops.rotary(k, pos, table).to(dtype)
+    assert torch.equal(y, ops.rotary(q, pos, table))
+    for cache, old, new in ((keys, before[0], rk), (values, before[1], v.to(dtype))):
+        want = old.clone()
+        rows = [(t, int(s)) for t, s in enumerate(slots.tolist()) if 0 <= s < pages * size]
+        t, s = torch.tensor(rows, device="cuda").reshape(-1, 2).unbind(1)
+        want[s // size, s % size] = new[t]
+        assert torch.equal(cache, want)
+    # without rotation; the query in place
+    ops.paged_append(k, v, keys, values, slots)
+    assert all(torch.equal(keys[s // size, s % size], k[t].to(dtype)) for t, s in rows[:50])
+    want = ops.rotary(q, pos, table)
+    assert ops.paged_append(k, v, keys, values, slots, positions=pos, table=table, query=q, out=q) is q and torch.equal(q, want)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------
+def _batch(g, lengths, new, kv, heads, dim, size, dtype, layout="rows", spare=3, poison=True):
+    """(query, keys, values, pages, lengths, offsets): pages in any order; rows that hold no key are NaN, entries of the table
+    behind a sequence's pages far outside."""
+    used = [-(-max(n, 0) // size) for n in lengths]
+    total = sum(used) + spare
+    keys, values = _caches(g, total, size, kv, dim, dtype, layout)
+    order = torch.randperm(total, generator=torch.Generator().manual_seed(5)).tolist()
+    pages = torch.full((len(lengths), max(used + [1]) + 1), 1 << 30, dtype=torch.int32)
+    free = torch.ones(total, size, dtype=torch.bool)
+    at = 0
+    for i, n in enumerate(used):
+        pages[i, :n] = torch.tensor(order[at:at + n])
+        for j in range(n):
+            free[order[at + j], :min(size, lengths[i] - j * size)] = False
+        at += n
+    if poison:
+        for c in (keys, values):
+            c[free.cuda()] = math.nan
+    offsets = [0]
+    for n in new:
+        offsets.append(offsets[-1] + n)
+    query = _randn(g, offsets[-1], heads, dim, dtype=dtype)
+    return query, keys, values, pages.cuda(), torch.tensor(lengths, device="cuda"), torch.tensor(offsets, device="cuda")
+
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 500, 1000]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,kv,dim,size", [(4, 1, 128, 16), (6, 6, 64, 8), (10, 2, 72, 32), (16, 1, 128, 64), (40, 2, 96, 128), (3, 1, 8, 256)])
+def test_one_new_token(dtype, heads, kv, dim, size):
+    from glq_b200 import ops
+    q, k, v, pages, lengths, offsets = _batch(_gen(heads), LENGTHS, [1] * len(LENGTHS), kv, heads, dim, size, dtype)
+    y = ops.paged_attention(q, k, v, pages, lengths)
+    ref, bound = O.attend(q, k, v, pages, lengths, offsets)
+    _close(y, ref, bound)
+    assert not y[0].any()
+    assert torch.equal(y, ops.paged_attention(q, k, v, pages, lengths.to(torch.int32), query_offsets=offsets.to(torch.int32), max_query_len=1))
+
+
+CHUNKS = {          # lengths, new tokens
+    "one": ([300], [300]),
+    "behind": ([1000], [77]),
+    "mixed": ([0, 5, 130, 400, 64, 1, 700, 129], [0, 5, 1, 33, 64, 1, 2, 0]),
+    "fewer keys than queries": ([3, 0, 70], [10, 4, 200]),
+    "wide": ([600, 257], [513, 257]),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("mask", ["causal", "all", "window", "window of one", "all, window"])
+@pytest.mark.parametrize("name", sorted(CHUNKS))
+def test_chunks(dtype, mask, name):
+    from glq_b200 import ops
+    lengths, new = CHUNKS[name]
+    causal, window = not mask.startswith("all"), {"window": 37, "window of one": 1, "all, window": 50}.get(mask, 0)
+    for heads, kv, dim, size in ((4, 2, 128, 16), (5, 1, 64, 32)):
+        q, k, v, pages, n, offsets = _batch(_gen(len(name)), lengths, new, kv, heads, dim, size, dtype)
+        y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, causal=causal, window=window)
+        ref, bound = O.attend(q, k, v, pages, n, offsets, causal=causal, window=window)
+        _close(y, ref, bound, (heads, kv, dim, size))
+        assert torch.equal(y, ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, causal=causal, window=window))
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 200])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_what_a_query_does_not_see_changes_nothing(new, value):
+    """Infinities and NaN in keys and values behind a query's own position, in front of its window."""
+    from glq_b200 import ops
+    lengths, news = [230, 200 + new], [new, new]
+    q, k, v, pages, n, offsets = _batch(_gen(new), lengths, news, 2, 4, 128, 16, BF)
+    clean = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, window=90)
+    ref, bound = O.attend(q, k, v, pages, n, offsets, window=90)
+    _close(clean, ref, bound)
+    for i, bad in ((0, lengths[0] - 1), (0, 100), (1, lengths[1] - 1 - new // 2), (1, 3)):
+        page = pages[i, bad // 16]
+        kk, vv = k.clone(), v.clone()
+        kk[page, bad % 16], vv[page, bad % 16] = value, value
+        y = ops.paged_attention(q, kk, vv, pages, n, query_offsets=offsets, window=90)
+        for r in range(2 * new):
+            s, j = divmod(r, new)
+            at = lengths[s] - new + j
+            if s == i and at - 90 < bad <= at:
+                assert not torch.isfinite(y[r].float()).all() or value == -math.inf
+            else:
+                assert torch.equal(y[r], clean[r]) or (y[r].double().cpu() - ref[r]).abs().le(bound[r]).all(), (i, bad, r)
+
+
+def test_scores_without_a_softmax():
+    """A visible key of minus infinity alone, plus infinity, NaN: as the definition has it, not a number."""
+    from glq_b200 import ops
+    q = torch.ones(1, 1, 64, device="cuda", dtype=HF)
+    for value, length in ((-math.inf, 1), (math.inf, 5), (math.nan, 5)):
+        k, v = torch.ones(1, 8, 1, 64, device="cuda", dtype=HF), torch.ones(1, 8, 1, 64, device="cuda", dtype=HF)
+        k[0, 0] = value
+        y = ops.paged_attention(q, k, v, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([length], device="cuda"))
+        assert torch.isnan(y).all(), value
+    k[0, 0] = -math.inf                                                           # beside others: no weight
+    assert torch.equal(ops.paged_attention(q, k, v, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([5], device="cuda")), torch.ones_like(q))
+
+
+@pytest.mark.parametrize("new", [1, 2, 150])
+@pytest.mark.parametrize("layout", ["rows", "heads", "both"])
+def test_layouts_strides_and_given_results(layout, new):
+    from glq_b200 import ops
+    lengths, news = [400, 150, 222], [new, new, new]
+    q, k, v, pages, n, offsets = _batch(_gen(3), lengths, news, 2, 6, 96, 16, HF, layout)
+    want, bound = O.attend(q, k, v, pages, n, offsets)
+    y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets)
+    _close(y, want, bound)
+    for off, width in ((0, 600), (96, 800), (1, 577)):                             # rows of a merged projection, aligned and not
+        buf = torch.zeros(3 * new + 1, width, device="cuda", dtype=HF).flatten()
+        view = torch.as_strided(buf[off:], q.shape, (width, 96, 1))
+        view.copy_(q)
+        assert torch.equal(ops.paged_attention(view, k, v, pages, n, query_offsets=offsets), y)
+        big = torch.full((3 * new + 1, width), 7.0, device="cuda", dtype=HF)
+        out = torch.as_strided(big.flatten()[off:], q.shape, (width, 96, 1))
+        assert ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, out=out) is out and torch.equal(out, y)
+        out.fill_(7.0)
+        assert bool((big == 7.0).all())
+    assert torch.equal(ops.paged_attention(q.transpose(0, 1).contiguous().transpose(0, 1), k, v, pages, n, query_offsets=offsets), y)
+    table = torch.cat((pages, torch.full_like(pages, -1)), 1)[:, :pages.shape[1]]
+    assert table.stride(0) != table.shape[1] and torch.equal(ops.paged_attention(q, k, v, table, n, query_offsets=offsets), y)
+    half = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, scale=0.01)
+    _close(half, *O.attend(q, k, v, pages, n, offsets, scale=0.01))
+
+
+@pytest.mark.parametrize("rows", [60, 600])
+def test_rows_of_no_sequence(rows):
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(1), [50, 90], [20, 20], 1, 2, 64, 16, BF)
+    wide = torch.cat((q[:5], q, _randn(_gen(2), rows, 2, 64)))
+    y = ops.paged_attention(wide, k, v, pages, n, query_offsets=offsets + 5)
+    want = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets)
+    assert torch.equal(y[5:45], want) and not y[:5].any() and not y[45:].any()
+    out = torch.full_like(wide, 3.0)
+    ops.paged_attention(wide, k, v, pages, n, query_offsets=offsets + 5, out=out)
+    assert torch.equal(out[5:45], want) and bool((out[:5] == 3).all()) and bool((out[45:] == 3).all())
+    empty = ops.paged_attention(wide, k, v, pages[:0], n[:0], query_offsets=offsets[:1])
+    assert not empty.any()
+    assert ops.paged_attention(q[:0], k, v, pages, n, query_offsets=offsets * 0).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("new", [1, 90])
+def test_integers_that_make_no_sense_stay_in_bounds(new):
+    """Pages outside the cache read as zeros, lengths are held to the table, offsets to the rows."""
+    from glq_b200 import ops
+    lengths = [200, 300]
+    q, k, v, pages, n, offsets = _batch(_gen(4), lengths, [new, new], 1, 4, 128, 16, BF)
+    bad = pages.clone()
+    bad[0, 2], bad[0, 5], bad[1, 1] = -3, 10 ** 9, k.shape[0]
+    _close(ops.paged_attention(q, k, v, bad, n, query_offsets=offsets), *O.attend(q, k, v, bad, n, offsets))
+    most = bad.shape[1] * 16
+    far = torch.tensor([2 ** 40, -5], device="cuda")
+    _close(ops.paged_attention(q, k, v, bad, far, query_offsets=offsets), *O.attend(q, k, v, bad, torch.tensor([most, 0]), offsets))
+    for wild in ([0, 10 ** 12, 2 * new], [-5, new, 10 ** 9], [2 * new, new, 0], [10 ** 9, -7, 3]):
+        y = ops.paged_attention(q, k, v, pages, n, query_offsets=torch.tensor(wild, device="cuda"))
+        assert y.shape == q.shape
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new", [1, 4])
+def test_many_sequences(new):
+    from glq_b200 import ops
+    g = torch.Generator().manual_seed(8)
+    lengths = (torch.randint(0, 90, (1500,), generator=g) + new).tolist()
+    q, k, v, pages, n, offsets = _batch(_gen(6), lengths, [new] * 1500, 1, 2, 64, 16, BF, poison=False)
+    _close(ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=new), *O.attend(q, k, v, pages, n, offsets))
+
+
+def _reference(q, k, v, pages, length, scale):
+    """One sequence, one token, in 64 bits on the device."""
+    rows = k[pages].flatten(0, 1)[:length].double(), v[pages].flatten(0, 1)[:length].double()
+    g = q.shape[1] // k.shape[2]
+    z = torch.einsum("hd,nhd->hn", q[0].double(), rows[0].repeat_interleave(g, 1)) * scale
+    return torch.einsum("hn,nhd->hd", torch.softmax(z, -1), rows[1].repeat_interleave(g, 1))
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^32 bytes and 2^31 values, its last pages read and written."""
+    from glq_b200 import ops
+    pages, size, kv, dim = 140000, 32, 4, 128
+    keys, values = (torch.zeros(pages, size, kv, dim, device="cuda", dtype=BF) for _ in range(2))
+    assert keys.numel() > 2 ** 31
+    ids = torch.tensor([[pages - 1, 0, pages - 2, 70000]], dtype=torch.int32, device="cuda")
+    length = 100
+    g = _gen(2)
+    k, v, q = _randn(g, length, kv, dim), _randn(g, length, kv, dim), _randn(g, 1, 8, dim)
+    at = torch.arange(length, device="cuda")
+    ops.paged_append(k, v, keys, values, ids[0].long()[at // size] * size + at % size)
+    assert torch.equal(keys[ids[0].long()].flatten(0, 1)[:length], k) and torch.equal(values[pages - 1], v[:size])
+    y = ops.paged_attention(q, keys, values, ids, torch.tensor([length], device="cuda"))
+    ref = _reference(q, keys, values, ids[0].long(), length, dim ** -0.5)
+    assert (y[0].double() - ref).abs().max() <= 2.0 ** -7 * v.abs().max().double()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_long_context(dtype):
+    from glq_b200 import ops
+    size, length = 64, 70001
+    g = _gen(9)
+    n = -(-length // size)
+    keys, values = _randn(g, n, size, 2, 128, dtype=dtype), _randn(g, n, size, 2, 128, dtype=dtype)
+    pages = torch.randperm(n, generator=g, device="cuda").to(torch.int32)[None]
+    q = _randn(g, 1, 8, 128, dtype=dtype) * 3
+    y = ops.paged_attention(q, keys, values, pages, torch.tensor([length], device="cuda"))
+    ref = _reference(q, keys, values, pages[0].long(), length, 128 ** -0.5)
+    assert (y[0].double() - ref).abs().max() <= 2 * U[dtype] * values.abs().max().double()
+
+
+# ---- together -----------------------------------------------------------------------------------------------------
+def test_prompt_then_decoding_steps():
+    """A prompt in two chunks and decoding steps through append and attention, as a decoder runs them, against attention over the whole."""
+    from glq_b200 import ops
+    heads, kv, dim, size, steps = 8, 2, 128, 16, [40, 23, 1, 1, 1]
+    g = _gen(11)
+    total = sum(steps)
+    qkv = _randn(g, total, (heads + 2 * kv) * dim)
+    keys, values = (torch.full((9, size, kv, dim), math.nan, device="cuda", dtype=BF) for _ in range(2))
+    pages = torch.tensor([[7, 2, 5, 0, 8, 1]], dtype=torch.int32, device="cuda")
+    table = ops.rotary_table(dim, base=500000.0, scaling={"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 8192})
+    at = 0
+    for n in steps:
+        q, k, v = (t.view(n, -1, dim) for t in qkv[at:at + n].split([heads * dim, kv * dim, kv * dim], 1))
+        pos = torch.arange(at, at + n, device="cuda")
+        slots = pages[0].long()[pos // size] * size + pos % size
+        rq = ops.paged_append(k, v, keys, values, slots, positions=pos, table=table, query=q)
+        at += n
+        offsets = torch.tensor([0, n], device="cuda")
+        y = ops.paged_attention(rq, keys, values, pages, torch.tensor([at], device="cuda"), query_offsets=offsets, max_query_len=n)
+        _close(y, *O.attend(rq, keys, values, pages, [at], offsets))
+
+
+@pytest.mark.parametrize("new", [1, 130])
+def test_captured_and_replayed_with_other_contents(new):
+    """Two graphs of different batches over one cache, replayed in turn with other queries, lengths and pages in place."""
+    from glq_b200 import ops
+    batches = [_batch(_gen(s), lengths, [new] * len(lengths), 2, 8, 128, 16, BF) for s, lengths in ((1, [300, 200, 999]), (2, [777]))]
+    graphs = []
+    for q, k, v, pages, n, offsets in batches:
+        call = lambda: ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=new)
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()
+        graphs.append((graph, y))
+    for step in range(3):
+        for (q, k, v, pages, n, offsets), (graph, y) in zip(batches, graphs):
+            q.copy_(_randn(_gen(50 + step), *q.shape))
+            n.sub_(17)
+            graph.replay()
+        for (q, k, v, pages, n, offsets), (graph, y) in zip(batches, graphs):
+            want = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=new)
+            assert torch.equal(y, want)
+            ref, bound = O.attend(q, k, v, pages, n, offsets)
+            _close(y, ref, bound)
+
+
+def test_calls_on_several_streams_at_once():
+    from glq_b200 import ops
+    work = [_batch(_gen(s), [500 + 40 * s, 900], [new, new], 2, 8, 128, 16, BF) for s, new in enumerate((1, 1, 64, 200))]
+    want = [ops.paged_attention(q, k, v, p, n, query_offsets=o) for q, k, v, p, n, o in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for s, (q, k, v, p, n, o) in zip(streams, work):
+            with torch.cuda.stream(s):
+                got.append(ops.paged_attention(q, k, v, p, n, query_offsets=o))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals():
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(0), [50, 60], [1, 1], 2, 4, 64, 16, BF)
+    with pytest.raises(ValueError, match="over a cache"):
+        ops.paged_attention(q.half(), k, v, pages, n)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.paged_attention(q, k, v, pages, n, out=q)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.paged_attention(q, k, v, pages.cpu(), n)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.paged_attention(q, k, v, pages, n.cpu())
+    with pytest.raises(ValueError, match="16 bytes"):
+        ops.paged_attention(q, torch.as_strided(k.flatten()[1:], (k.shape[0] - 1, *k.shape[1:]), k.stride()), v[:-1], pages, n)
+    with pytest.raises(ValueError, match="overlaps the cache"):
+        ops.paged_append(k[0], v[0], k, v, torch.zeros(16, dtype=torch.int64, device="cuda"))
+    table = ops.rotary_table(64)
+    with pytest.raises(ValueError, match="positions"):
+        ops.rotary(q, torch.zeros(3, dtype=torch.int64, device="cuda"), table)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.rotary(q[:1], torch.zeros(1, dtype=torch.int64, device="cuda"), table, out=torch.as_strided(q, (1, 4, 64), (256, 64, 1), 8))

@@ -1,0 +1,310 @@
+"""Rotary positions, paged append and attention without a GPU: the oracle against itself, the ABI's structure, the refusals, the list of work."""
+import ctypes
+import math
+import os
+import subprocess
+
+import pytest
+import torch
+
+import paged_oracle as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from glq_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def test_oracle_rotates_by_the_angle():
+    x = torch.randn(3, 2, 8, dtype=torch.float64)
+    f = torch.tensor([1.0, 0.25], dtype=torch.float64)
+    pos = torch.tensor([0, 3, -2])
+    for interleaved in (False, True):
+        y, _ = O.rotate(x, pos, f, 1.0, interleaved)
+        a, b = ((0, 2), (1, 3)) if interleaved is False else ((0, 1), (2, 3))
+        for i, (u, v) in enumerate((a, b)):
+            z = torch.complex(x[..., u], x[..., v]) * torch.polar(torch.ones(3, dtype=torch.float64), pos * f[i])[:, None]
+            assert torch.allclose(y[..., u], z.real, atol=1e-14) and torch.allclose(y[..., v], z.imag, atol=1e-14)
+        assert torch.equal(y[0], x[0]) and torch.equal(y[..., 4:], x[..., 4:])
+
+
+def test_oracle_attention_is_softmax_over_what_is_seen():
+    g = torch.Generator().manual_seed(1)
+    keys, values = (torch.randn(3, 8, 1, 8, generator=g).half() for _ in range(2))
+    q = torch.randn(5, 2, 8, generator=g, dtype=torch.float64)
+    pages = torch.tensor([[2, 0]])
+    y, _ = O.attend(q, keys, values, pages, [11], [0, 5], window=4)
+    k, v = torch.cat((keys[2], keys[0]))[:11, 0].double(), torch.cat((values[2], values[0]))[:11, 0].double()
+    back = torch.arange(6, 11)[:, None] - torch.arange(11)[None]
+    z = torch.einsum("qhd,kd->hqk", q, k) / math.sqrt(8) + torch.where((back >= 0) & (back < 4), 0.0, -math.inf)
+    assert torch.allclose(y, torch.einsum("hqk,kd->qhd", torch.softmax(z, -1), v))
+
+
+def test_struct_layouts_match_header(tmp_path):
+    from glq_b200 import _lib
+    pairs = [("GlqbRotary", _lib.RotaryDesc), ("GlqbPagedCache", _lib.PagedCacheDesc), ("GlqbPagedAppend", _lib.PagedAppendDesc), ("GlqbPagedAttention", _lib.PagedAttentionDesc)]
+    lines = "".join(f'printf("%zu ", sizeof({c}));' + "".join(f'printf("%zu ", __builtin_offsetof({c}, {f[0]}));' for f in d._fields_) for c, d in pairs)
+    src, exe = tmp_path / "s.c", tmp_path / "s"
+    src.write_text('#include <stdio.h>\n#include "glq_b200.h"\nint main(){' + lines + "}")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    out = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert out == [v for _, d in pairs for v in [ctypes.sizeof(d)] + [getattr(d, f[0]).offset for f in d._fields_]]
+
+
+def test_c_entries_refuse_before_any_cuda_call(lib):
+    from glq_b200 import _lib
+    p = 4096                                                    # never dereferenced: each call is refused
+
+    def refused(rc, code, text):
+        assert rc == code and text in lib.glqb_last_error().decode(), (rc, lib.glqb_last_error())
+
+    def rotary(r=(p, 4, 0, 1.0), x=p, dt=1, out=p, tokens=2, heads=3, dim=64, pos=p):
+        return lib.glqb_rotary(ctypes.byref(_lib.RotaryDesc(*r)), x, dt, 192, 64, out, 192, 64, tokens, heads, dim, pos, 1, None)
+
+    refused(rotary(dt=3), -1, "dtype")
+    refused(rotary(tokens=-1), -1, "-1 tokens")
+    refused(rotary(dim=2000), -1, "2000 values")
+    refused(rotary(x=None), -1, "null")
+    refused(rotary(out=p + 1), -1, "aligned")
+    refused(rotary(r=(None, 4, 0, 1.0)), -1, "turns")
+    refused(rotary(r=(p, 33, 0, 1.0)), -1, "33 pairs")
+    refused(rotary(r=(p, 0, 0, 1.0)), -1, "0 pairs")
+    refused(rotary(pos=p + 4), -1, "aligned")
+    assert rotary(tokens=0) == 0 and rotary(heads=0) == 0
+
+    cache = dict(keys=p, values=p, key_page=2048, key_row=128, key_head=64, value_page=2048, value_row=128, value_head=64, pages=10, page_size=16, kv_heads=2, head_dim=64, dtype=1)
+
+    def append(r=(p, 4, 0, 1.0), c={}, **kw):
+        a = dict(key=p, value=p, key_token=128, key_head=64, value_token=128, value_head=64, tokens=3, slots=p, positions=p, slots_are_int64=1, positions_are_int64=1, dtype=1)
+        a.update(kw)
+        return lib.glqb_paged_append(ctypes.byref(_lib.PagedCacheDesc(**{**cache, **c})), ctypes.byref(_lib.PagedAppendDesc(**a)), ctypes.byref(_lib.RotaryDesc(*r)) if r else None, None)
+
+    def attention(ws=p, size=1 << 40, c={}, **kw):
+        a = dict(query=p, out=p, query_token=256, query_head=64, out_token=256, out_head=64, tokens=3, page_table=p, page_stride=4, lengths=p, offsets=None, sequences=3,
+                 page_columns=4, heads=4, causal=1, scale=0.1, max_query_len=1)
+        a.update(kw)
+        return lib.glqb_paged_attention(ctypes.byref(_lib.PagedCacheDesc(**{**cache, **c})), ctypes.byref(_lib.PagedAttentionDesc(**a)), ws, size, None)
+
+    for call in (append, attention):
+        refused(call(c=dict(dtype=2)), -1, "fp16 or bf16")
+        refused(call(c=dict(page_size=24)), -1, "24 rows")
+        refused(call(c=dict(page_size=4)), -1, "4 rows")
+        refused(call(c=dict(head_dim=136)), -1, "136 values")
+        refused(call(c=dict(head_dim=12)), -1, "12 values")
+        refused(call(c=dict(kv_heads=0)), -1, "0 heads")
+        refused(call(c=dict(pages=1 << 31)), -1, "pages")
+        refused(call(c=dict(values=None)), -1, "null")
+        refused(call(c=dict(key_row=124)), -1, "multiples of 8")
+        refused(call(c=dict(values=p + 8)), -1, "16 bytes")
+    refused(append(dtype=0), -1, "type")
+    refused(append(tokens=-1), -1, "-1 tokens")
+    refused(append(slots=None), -1, "null")
+    refused(append(query=p, query_out=p, heads=2, r=None), -1, "rotated")
+    refused(append(r=(p, 40, 0, 1.0)), -1, "40 pairs")
+    refused(append(value=p + 1), -1, "aligned")
+    assert append(tokens=0) == 0
+    refused(attention(heads=3), -1, "3 query heads")
+    refused(attention(tokens=1 << 29), -1, "too many")
+    refused(attention(sequences=(1 << 20) + 1), -1, "sequences")
+    refused(attention(page_columns=1 << 27), -1, "per sequence")
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        refused(attention(scale=scale), -1, "positive")
+    refused(attention(window=-1), -1, "window")
+    refused(attention(out=None), -1, "null")
+    refused(attention(lengths=None), -1, "null")
+    refused(attention(page_table=None), -1, "null")
+    refused(attention(query=p + 2), -1, "4 bytes")
+    refused(attention(ws=p + 4), -1, "aligned")
+    assert attention(tokens=0, out=None) == 0
+
+
+def _table(monkeypatch, dim=32, **kw):
+    """A rotary table on the host (its device is not looked at here)."""
+    from glq_b200 import paged
+    monkeypatch.setattr(paged, "_cuda", lambda t, name: None)
+    real = torch.device
+    monkeypatch.setattr(paged.torch, "device", lambda d: type("D", (), {"type": "cuda"})() if d == "cuda" else real(d))
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, *a, _to=torch.Tensor.to, **k: self if a and not isinstance(a[0], (str, torch.dtype, real)) else _to(self, *a, **k))
+    table = paged.rotary_table(dim, **kw)
+    monkeypatch.undo()
+    return table
+
+
+def test_table_holds_fractions_of_a_turn(monkeypatch):
+    t = _table(monkeypatch, 8, base=100.0)
+    for i, v in enumerate(t.turns.tolist()):
+        want = 100.0 ** (-2 * i / 8) / (2 * math.pi)
+        assert abs((v % 2 ** 64) / 2 ** 64 - want) <= 2.0 ** -52
+    assert t.dim == 8 and t.scale == 1.0 and not t.interleaved
+    # a frequency beyond a turn per position, and a negative one, wrap
+    t = _table(monkeypatch, None, inv_freq=torch.tensor([2 * math.pi * 3.75, -2 * math.pi * 0.25, 2 * math.pi * 0.5]))
+    for v, want in zip(t.turns.tolist(), (0.75, 0.75, 0.5)):
+        assert abs((v % 2 ** 64) / 2 ** 64 - want) < 1e-6
+    with pytest.raises(AttributeError, match="cannot be set"):
+        t.scale = 2.0
+
+
+@pytest.mark.parametrize("name,kw,dim", [("linear", dict(factor=4.0), 64), ("llama3", dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192), 128),
+                                         ("yarn", dict(factor=4.0, beta_fast=32.0, beta_slow=1.0, original_max_position_embeddings=32768), 128)])
+def test_scalings_of_long_contexts(monkeypatch, name, kw, dim):
+    base = 500000.0
+    t = _table(monkeypatch, dim, base=base, scaling={"rope_type": name, **kw})
+    got = [(v % 2 ** 64) / 2 ** 64 * 2 * math.pi for v in t.turns.tolist()]
+    for i, f in enumerate(got):
+        plain = base ** (-2 * i / dim)
+        if name == "linear":
+            want = plain / 4
+        else:
+            old, length = kw["original_max_position_embeddings"], 2 * math.pi / plain
+            if name == "llama3":
+                smooth = (old / length - 1.0) / 3.0
+                want = plain if length < old / 4 else plain / 8 if length > old else (1 - smooth) * plain / 8 + smooth * plain
+            else:
+                lo, hi = (dim * math.log(old / (r * 2 * math.pi)) / (2 * math.log(base)) for r in (32.0, 1.0))
+                ramp = min(1.0, max(0.0, (i - math.floor(lo)) / (math.ceil(hi) - math.floor(lo))))
+                want = plain / 4 * ramp + plain * (1 - ramp)
+        assert abs(f - want) <= 1e-12 * want + 1e-15, i
+    assert t.scale == pytest.approx(0.1 * math.log(4.0) + 1.0 if name == "yarn" else 1.0)
+
+
+def test_operators_refuse_host_tensors():
+    from glq_b200 import ops
+    x = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    c = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
+    n = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.rotary(x, n, None)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.paged_append(x[:, :2], x[:, :2], c, c, n)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.paged_attention(x, c, c, torch.zeros(2, 1, dtype=torch.int32), n)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.rotary_table(64, device="cpu")
+    for bad in (dict(dim=7), dict(dim=0), dict(), dict(dim=8, scaling={"rope_type": "other", "factor": 2.0}), dict(dim=8, scaling={"rope_type": "linear"}),
+                dict(dim=8, scaling={"rope_type": "yarn", "factor": 2.0}), dict(dim=8, inv_freq=torch.ones(3)), dict(inv_freq=torch.tensor([math.inf]))):
+        with pytest.raises(ValueError, match="glq_b200"):
+            ops.rotary_table(**bad)
+
+
+def test_operators_refuse_wrong_arguments(monkeypatch):
+    """The checks behind the one for the device, on host tensors; nothing is launched."""
+    from glq_b200 import ops, paged
+    table = _table(monkeypatch, 32)
+    big = _table(monkeypatch, 128)
+    monkeypatch.setattr(paged, "_cuda", lambda t, name: None)
+    monkeypatch.setattr(paged, "_same_device", lambda t, x, name: None)
+    launched = []
+    monkeypatch.setattr(paged, "_call", lambda *a: launched.append(a[1]))
+    monkeypatch.setattr(paged, "_workspace", lambda *a: 64)
+    bf = torch.bfloat16
+    x, n3 = torch.zeros(3, 4, 64, dtype=bf), torch.zeros(3, dtype=torch.int64)
+
+    def refuses(text, fn, *a, **kw):
+        with pytest.raises(ValueError, match=text):
+            fn(*a, **kw)
+
+    refuses("tokens, heads", ops.rotary, x[0], n3, table)
+    refuses("not torch.float64", ops.rotary, x.double(), n3, table)
+    refuses("rotary_table", ops.rotary, x, n3, None)
+    refuses("128 rotated values", ops.rotary, x, n3, big)
+    refuses("positions must be 3", ops.rotary, x, n3[:2], table)
+    refuses("positions must be 3", ops.rotary, x, n3.float(), table)
+    refuses("out must be", ops.rotary, x, n3, table, out=x[:2])
+    refuses("overlap", ops.rotary, x, n3, table, out=x[:1].expand(3, 4, 64))
+    refuses("without being it", ops.rotary, x, n3, table, out=torch.as_strided(x, x.shape, (64, 192, 1)))
+    y = torch.zeros(3, 64, 4, dtype=bf).transpose(1, 2)
+    refuses("one behind the other", ops.rotary, y, n3, table, out=y)
+
+    k, v = (torch.zeros(5, 16, 2, 64, dtype=bf) for _ in range(2))
+    new = torch.zeros(3, 2, 64, dtype=bf)
+    refuses("one type", ops.paged_append, new, new, k, v.half(), n3)
+    refuses("one type", ops.paged_append, new, new, k, v[:4], n3)
+    refuses("bf16 or fp16", ops.paged_append, new, new, k.float(), v.float(), n3)
+    refuses("power of two", ops.paged_append, new, new, k[:, :12], v[:, :12], n3)
+    refuses("multiple of 8", ops.paged_append, new[..., :12], new[..., :12], k[..., :12], v[..., :12], n3)
+    refuses("16 bytes", ops.paged_append, new, new, k.transpose(1, 3).contiguous().transpose(1, 3), v, n3)
+    refuses("for a cache of", ops.paged_append, new[:, :1], new[:, :1], k, v, n3)
+    refuses("for a cache of", ops.paged_append, new, new[:2], k, v, n3)
+    refuses("fp32", ops.paged_append, new.half(), new.half(), k, v, n3)
+    refuses("slots must be 3", ops.paged_append, new, new, k, v, n3[:1])
+    refuses("come together", ops.paged_append, new, new, k, v, n3, table=table)
+    refuses("come together", ops.paged_append, new, new, k, v, n3, positions=n3)
+    refuses("to be rotated", ops.paged_append, new, new, k, v, n3, query=x)
+    refuses("belongs to query", ops.paged_append, new, new, k, v, n3, out=x)
+    refuses("beside keys", ops.paged_append, new, new, k, v, n3, positions=n3, table=table, query=x.float())
+    refuses("beside keys", ops.paged_append, new, new, k, v, n3, positions=n3, table=table, query=x[:2])
+    refuses("128 rotated", ops.paged_append, new, new, k, v, n3, positions=n3, table=big)
+    refuses("out overlaps key", ops.paged_append, new, torch.zeros_like(new), k, v, n3, positions=n3, table=table, query=torch.zeros_like(new), out=new)
+    refuses("overlaps the cache", ops.paged_append, new, k[0, :3], k, v, n3)
+
+    pages = torch.zeros(3, 2, dtype=torch.int32)
+    ok = (x, k, v, pages, n3)
+    refuses("over a cache", ops.paged_attention, x.half(), *ok[1:])
+    refuses("over a cache", ops.paged_attention, x[:, :3], *ok[1:])
+    refuses("over a cache", ops.paged_attention, x[..., :32], *ok[1:])
+    refuses("pages must be int32", ops.paged_attention, x, k, v, pages.long(), n3)
+    refuses("pages must be int32", ops.paged_attention, x, k, v, pages.t().contiguous().t(), n3)
+    refuses("lengths must be 3", ops.paged_attention, x, k, v, pages, n3[:2])
+    refuses("query_offsets must be 4", ops.paged_attention, *ok, query_offsets=n3)
+    refuses("need query_offsets", ops.paged_attention, x, k, v, pages[:2], n3[:2])
+    refuses("max_query_len", ops.paged_attention, *ok, max_query_len=-1)
+    for scale in (0.0, -0.5, math.nan, math.inf):
+        refuses("positive", ops.paged_attention, *ok, scale=scale)
+    for window in (-1, 2 ** 31):
+        refuses("window", ops.paged_attention, *ok, window=window)
+    refuses("out must be", ops.paged_attention, *ok, out=x.half())
+    refuses("overlaps", ops.paged_attention, *ok, out=x)
+    assert not launched
+    ops.rotary(x, n3, table)
+    ops.paged_append(new, new, k, v, n3, positions=n3, table=table, query=x)
+    ops.paged_attention(*ok)
+    assert launched == ["rotary", "paged_append", "paged_attention"]
+
+
+def _model(lengths, new, group, kv_heads, rows, keys, ctas, min_units, causal=True, window=0):
+    """How attention's work is shared out: the list of key tiles, cut into runs.  [(cta, sequence, key head, row tile, lo, hi, slot)]"""
+    items = []
+    for s, (n, q) in enumerate(zip(lengths, new)):
+        for h in range(kv_heads):
+            for t in range(-(-q * group // rows)):
+                last = min(q - 1, (min(q * group, (t + 1) * rows) - 1) // group)
+                first = t * rows // group
+                to = max(0, n - q + last + 1) if causal else n
+                lo = min(to, max(0, n - q + first + 1 - window) if window else 0) // keys
+                items.append((s, h, t, lo, max(lo + 1, -(-to // keys))))
+    total = sum(i[4] - i[3] for i in items)
+    used = min(ctas, -(-total // min_units))
+    runs, out = [(total * c // used, total * (c + 1) // used) for c in range(used)], []
+    at = 0
+    for s, h, t, lo, hi in items:
+        for c, (a, b) in enumerate(runs):
+            x, y = max(a, at), min(b, at + hi - lo)
+            if x < y:
+                whole = x == at and y == at + hi - lo
+                out.append((c, s, h, t, lo + x - at, lo + y - at, -1 if whole else 1 if x == at else 0))
+        at += hi - lo
+    return items, out
+
+
+@pytest.mark.parametrize("lengths,new", [([4096], [1]), ([100, 3, 900, 0, 64], [1] * 5), ([700, 2], [650, 2]), ([5000], [5000])])
+@pytest.mark.parametrize("rows,keys,ctas,min_units", [(16, 64, 296, 1), (16, 64, 296, 2), (256, 128, 148, 1), (256, 128, 148, 4)])
+def test_runs_cover_the_work_and_parts_find_their_item(lengths, new, rows, keys, ctas, min_units):
+    """Every key tile is taken once, and the part that begins an item finds the others in slot 0 of the CTAs behind it, the last of them ending it."""
+    items, runs = _model(lengths, new, 4, 2, rows, keys, ctas, min_units)
+    slots = {}
+    for c, s, h, t, lo, hi, slot in runs:
+        if slot >= 0:
+            assert (c, slot) not in slots                        # a CTA leaves at most one part in either slot
+            slots[c, slot] = (s, h, t, lo, hi)
+    for s, h, t, lo, hi in items:
+        mine = [r for r in runs if r[1:4] == (s, h, t)]
+        assert mine[0][4] == lo and mine[-1][5] == hi and all(a[5] == b[4] for a, b in zip(mine, mine[1:]))
+        if len(mine) > 1:
+            c = mine[0][0]
+            assert slots[c, 1][:4] == (s, h, t, lo)
+            assert [r[0] for r in mine] == list(range(c, c + len(mine))) and all(r[6] == 0 for r in mine[1:])
+            assert all(slots[r[0], 0][4] < hi for r in mine[1:-1]) and slots[mine[-1][0], 0][4] == hi
