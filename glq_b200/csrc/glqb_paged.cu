@@ -49,9 +49,7 @@ __device__ __forceinline__ void to_floats(const Eight<T>& e, float (&v)[8]) {
     const uint32_t w[4] = {e.a.x, e.a.y, e.a.z, e.a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float2 f;
-      if constexpr (__is_same(T, __half)) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      const float2 f = pa_unpack<T>(w[i]);
       v[2 * i] = f.x;
       v[2 * i + 1] = f.y;
     }
@@ -68,11 +66,6 @@ __device__ __forceinline__ Eight<T> from_floats(const float (&v)[8]) {
   }
   return e;
 }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 __device__ __forceinline__ void rotate_neighbours(float (&v)[8], const float2* cs) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
@@ -156,13 +149,13 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
           const int a = J.interleaved ? 2 * u : u, b = J.interleaved ? a + 1 : u + J.pairs;
           const float2 f = cs[u];
           const float v = (float)src[a], w = (float)src[b];
-          dst[a] = from_float<TO>(v * f.x - w * f.y);
-          dst[b] = from_float<TO>(w * f.x + v * f.y);
+          dst[a] = pa_round<TO>(v * f.x - w * f.y);
+          dst[b] = pa_round<TO>(w * f.x + v * f.y);
         } else if (P.turn) {
-          dst[u + J.pairs] = from_float<TO>((float)src[u + J.pairs]);
+          dst[u + J.pairs] = pa_round<TO>((float)src[u + J.pairs]);
         } else {
-          dst[u] = from_float<TO>((float)src[u]);
-          if (u < J.pairs) dst[behind] = from_float<TO>((float)src[behind]);
+          dst[u] = pa_round<TO>((float)src[u]);
+          if (u < J.pairs) dst[behind] = pa_round<TO>((float)src[behind]);
         }
       }
     };
@@ -179,7 +172,6 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
 // that has grown by more than 2^8, which scales all weights of a row alike and leaves their precision as it is.  Weights are rounded to the values'
 // type for the product, as the tensor cores take them; sums stay in fp32.
 constexpr int ST_WARPS = 4, ST_THREADS = (ST_WARPS + 1) * 32, ST_ITEMS = 4;
-constexpr float PA_LAZY = 8.0f;
 template <int DP>
 struct StreamShape {
   static constexpr int HALF = PA_STREAM_KEYS * 128, K_BYTES = HALF * (DP / 64), STAGE = 2 * K_BYTES, STAGES = 96 * 1024 / STAGE;
@@ -206,28 +198,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ void store4(const PagedJob& J, long long at, int col, float4 v) {
-  T* p = reinterpret_cast<T*>(J.out) + at + col;
-  if (J.out_wide) {                                        // (head_dim is a multiple of 8: four columns are all there, or none)
-    *reinterpret_cast<uint2*>(p) = make_uint2(pa_pack<T>(v.x, v.y), pa_pack<T>(v.z, v.w));
-  } else {
-    p[0] = from_float<T>(v.x); p[1] = from_float<T>(v.y); p[2] = from_float<T>(v.z); p[3] = from_float<T>(v.w);
-  }
-}
-__device__ __forceinline__ long long out_row(const PagedJob& J, int row0, int kv_head, int row) {
-  const int i = pa_query(J, row);
-  return (long long)(row0 + i) * J.out_token + (long long)(kv_head * J.group + row - i * J.group) * J.out_head;
-}
-
-// What a row's sums are multiplied by.  Weights of nothing: a row that sees no key is zero; one that does has only scores of minus
-// infinity, which have no softmax.
-__device__ __forceinline__ float row_factor(const PagedJob& J, const PagedSeq& s, int row, float sum) {
-  if (sum != 0.0f) return 1.0f / sum;
-  const int i = pa_query(J, row);
-  return pa_to(J, s, i) > pa_from(J, s, i) ? NAN : 0.0f;
-}
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(ST_THREADS, 2)
 paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -445,9 +415,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
               for (int n = 0; n < STEPS * 2; ++n) {
                 uint32_t two;
                 asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(base + C::K_BYTES + (n / 8) * C::HALF + row * 128 + (((n % 8) ^ (row & 7)) << 4) + t4 * 4) : "memory");
-                float2 v;
-                if constexpr (__is_same(T, __half)) v = __half22float2(*reinterpret_cast<const __half2*>(&two));
-                else v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
+                const float2 v = pa_unpack<T>(two);
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
                   if (see[a]) { o[n][2 * a] += w[a] * v.x; o[n][2 * a + 1] += w[a] * v.y; }
@@ -495,8 +463,8 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
           v.x += f * u.x; v.y += f * u.y; v.z += f * u.z; v.w += f * u.w;
         }
         if (it.slot < 0) {
-          const float f = row_factor(J, seq, it.first + row, sum);
-          if (col < J.head_dim) store4<T>(J, out_row(J, it.row0, it.kv_head, it.first + row), col, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+          const float f = pa_row_factor(J, seq, it.first + row, sum);
+          if (col < J.head_dim) pa_store4<T>(J, pa_out_row(J, it.row0, it.kv_head, it.first + row), col, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
         } else {
           *reinterpret_cast<float4*>(J.part + (place + row) * DP + col) = v;
           if (col == 0) J.part_ml[place + row] = make_float2(most, sum);
@@ -527,7 +495,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
     const int first = pa_offset(J, 0), last = max(first, pa_offset(J, J.seqs)), rest = J.tokens - (last - first);
     for (int i = c; i < rest; i += gridDim.x) {
       T* p = reinterpret_cast<T*>(J.out) + (long long)(i < first ? i : i + last - first) * J.out_token;
-      for (int k = threadIdx.x; k < J.heads * J.head_dim; k += CB_WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = from_float<T>(0.0f);
+      for (int k = threadIdx.x; k < J.heads * J.head_dim; k += CB_WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
     }
   }
   const PagedPart lead = J.part_of[2 * c + 1];
@@ -595,8 +563,8 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
     }
   }
   if (row - row0 >= rows || col >= J.head_dim) return;
-  const float f = row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, sum);
-  store4<T>(J, out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+  const float f = pa_row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, sum);
+  pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -618,10 +586,6 @@ struct PagedDevice {
   std::atomic<int> sms{0};
   int* status = nullptr;
 };
-int pg_device_index() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
-}
 const PagedDevice* pg_device() {
   static PagedDevice known[64];
   static std::mutex building;
@@ -712,16 +676,18 @@ bool encode_cache(CUtensorMap* map, const GlqbPagedCache* c, const void* base, i
 
 // What a call launches and keeps in its workspace, by its sizes alone.
 struct PagedForm {
-  int rows, keys, dp, ctas;
+  bool tile;                        // on the tensor cores
+  int rows, dp, ctas;
   size_t ml, part_of, bytes;        // where the workspace's second and third part begin, and its size
 };
+// Rows of a sequence and key head up to which the streaming kernel runs.
+constexpr int PA_STREAM_MOST = 16;
 PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int sms) {
   PagedForm f;
-  (void)a;
-  f.rows = PA_STREAM_ROWS;
-  f.keys = PA_STREAM_KEYS;
+  f.tile = (long long)std::max(1, a->max_query_len) * (a->heads / c->kv_heads) > PA_STREAM_MOST;
+  f.rows = f.tile ? PA_TILE_ROWS : PA_STREAM_ROWS;
   f.dp = c->head_dim <= 64 ? 64 : 128;
-  f.ctas = 2 * sms;
+  f.ctas = f.tile ? sms : 2 * sms;
   f.ml = (size_t)f.ctas * 2 * f.rows * f.dp * sizeof(float);
   f.part_of = f.ml + (size_t)f.ctas * 2 * f.rows * sizeof(float2);
   f.bytes = f.part_of + (size_t)f.ctas * 2 * sizeof(PagedPart);
@@ -740,32 +706,12 @@ int check_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a) {
   return GLQB_OK;
 }
 
-template <auto K, typename... P, typename... A>
-cudaError_t paged_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
-  static std::atomic<bool> raised[64];   // per device: may the kernel have the shared memory it needs?
-  std::atomic<bool>& r = raised[pg_device_index()];
-  if (smem > 48 * 1024 && !r.load(std::memory_order_relaxed)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    r.store(true, std::memory_order_relaxed);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
 template <typename T, int DP>
 cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   using C = StreamShape<DP>;
   constexpr auto K = paged_stream_kernel<T, DP>;
-  cudaError_t e = paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
+  const cudaError_t e = f.tile ? paged_tile_launch(J, __is_same(T, __nv_bfloat16), mk, mv, f.ctas, stream)
+                               : paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
   if (e != cudaSuccess) return e;
   constexpr auto CB = paged_combine_kernel<T, DP>;
   return paged_launch<CB>(CB, dim3((unsigned)f.ctas, (unsigned)f.rows / 16), CB_WARPS * 32, 0, stream, J, f.ctas, f.rows);

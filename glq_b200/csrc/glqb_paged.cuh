@@ -3,12 +3,15 @@
 #include "glqb_internal.h"
 #include "glqb_ptx.cuh"
 #include "glqb_launch.h"
+#include <atomic>
 #include <cuda.h>
 
 namespace glqb {
 
 constexpr int PA_PIECE = 64;         // most rows of a page that one copy brings
-constexpr int PA_STREAM_ROWS = 16, PA_STREAM_KEYS = 64;
+constexpr int PA_STREAM_ROWS = 16, PA_STREAM_KEYS = 64;      // rows of an item, and keys of a tile: few rows,
+constexpr int PA_TILE_ROWS = 256, PA_TILE_KEYS = 128;        // and many
+constexpr float PA_LAZY = 8.0f;                              // a row's weights are relative to a score that its largest exceeds by no more
 
 struct PagedJob {
   const uint16_t* q;
@@ -211,6 +214,37 @@ __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+template <typename T> __device__ __forceinline__ T pa_round(float v) {
+  if constexpr (__is_same(T, float)) return v;
+  else if constexpr (__is_same(T, __half)) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+template <typename T>
+__device__ __forceinline__ float2 pa_unpack(uint32_t two) {
+  if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2*>(&two));
+  else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
+}
+// four columns of a row of the result
+template <typename T>
+__device__ __forceinline__ void pa_store4(const PagedJob& J, long long at, int col, float4 v) {
+  T* p = reinterpret_cast<T*>(J.out) + at + col;
+  if (J.out_wide) {                                        // (head_dim is a multiple of 8: four columns are all there, or none)
+    *reinterpret_cast<uint2*>(p) = make_uint2(pa_pack<T>(v.x, v.y), pa_pack<T>(v.z, v.w));
+  } else {
+    p[0] = pa_round<T>(v.x); p[1] = pa_round<T>(v.y); p[2] = pa_round<T>(v.z); p[3] = pa_round<T>(v.w);
+  }
+}
+__device__ __forceinline__ long long pa_out_row(const PagedJob& J, int row0, int kv_head, int row) {
+  const int i = pa_query(J, row);
+  return (long long)(row0 + i) * J.out_token + (long long)(kv_head * J.group + row - i * J.group) * J.out_head;
+}
+// What a row's sums are multiplied by.  Weights of nothing: a row that sees no key is zero; one that does has only scores of minus
+// infinity, which have no softmax.
+__device__ __forceinline__ float pa_row_factor(const PagedJob& J, const PagedSeq& s, int row, float sum) {
+  if (sum != 0.0f) return 1.0f / sum;
+  const int i = pa_query(J, row);
+  return pa_to(J, s, i) > pa_from(J, s, i) ? NAN : 0.0f;
+}
 // has one of two 16-bit values no finite value?
 template <typename T>
 __device__ __forceinline__ bool pa_not_finite(uint32_t two) {
@@ -218,5 +252,36 @@ __device__ __forceinline__ bool pa_not_finite(uint32_t two) {
   return (two & E) == E || (two >> 16 & E) == E;
 }
 #endif  // __CUDACC__
+
+inline int pg_device_index() {       // the current one, 0..63
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : 0;
+}
+// Chained to the kernel in front (launch_chained).
+template <auto K, typename... P, typename... A>
+inline cudaError_t paged_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+  static std::atomic<bool> raised[64];   // per device: may the kernel have the shared memory it needs?
+  std::atomic<bool>& r = raised[pg_device_index()];
+  if (smem > 48 * 1024 && !r.load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    r.store(true, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// ---- glqb_paged_tile.cu
+// Many rows, on the tensor cores: J's items are PA_TILE_ROWS x PA_TILE_KEYS, one CTA per SM.
+cudaError_t paged_tile_launch(const PagedJob& J, bool bf16, const CUtensorMap& keys, const CUtensorMap& values, int ctas, cudaStream_t stream);
 
 }  // namespace glqb
