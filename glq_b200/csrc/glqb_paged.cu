@@ -202,7 +202,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(ST_THREADS, 2)
 paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using C = StreamShape<DP>;
-  constexpr int ROWS = PA_STREAM_ROWS, KEYS = PA_STREAM_KEYS, STEPS = DP / 16;
+  constexpr int ROWS = PA_STREAM_ROWS, KEYS = PA_STREAM_KEYS, STEPS = DP / 16;      // (J.rows is ROWS)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   StreamShared& B = *reinterpret_cast<StreamShared*>(ring + C::STAGES * C::STAGE);
@@ -217,11 +217,11 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
   if (warp == ST_WARPS && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &map_v : &map_k)) : "memory");
   pdl_wait();
   pdl_trigger();
-  pa_start<ROWS, KEYS>(J, B.start);
+  pa_start<KEYS>(J, B.start);
   bool ok = true;
 
   if (warp == ST_WARPS) {
-    PagedWalk<ROWS, KEYS> walk(J, B.start);
+    PagedWalk<KEYS> walk(J, B.start);
     const int piece = min(1 << J.page_log, PA_PIECE), pieces = KEYS / piece, page_mask = (1 << J.page_log) - 1;
     uint32_t stage = 0, phase = 1, ip = 1, filled = 0;
     int is = 0;
@@ -481,11 +481,11 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
 }
 
 // ---- what several CTAs have of an item, together --------------------------------------------------
-// A block takes 16 rows of an item that CTA blockIdx.x began and did not end: its parts are that CTA's, then those of the CTAs behind it up
+// A block takes eight rows of an item that CTA blockIdx.x began and did not end: its parts are that CTA's, then those of the CTAs behind it up
 // to the one that ended the item.  A warp adds a row, several if there are few rows, each every n-th part; the order is the same in every call.
-constexpr int CB_WARPS = 16;
+constexpr int CB_WARPS = 8, CB_BATCH = 4;
 template <typename T, int DP>
-__global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas, int item_rows) {
+__global__ void __launch_bounds__(CB_WARPS * 32, 5) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas, int item_rows) {
   __shared__ float sums[CB_WARPS][DP];
   __shared__ float2 mls[CB_WARPS];
   pdl_wait();
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
     }
   }
   const PagedPart lead = J.part_of[2 * c + 1];
-  const int row0 = blockIdx.y * 16, rows = min(16, lead.rows - row0);
+  const int row0 = blockIdx.y * CB_WARPS, rows = min(CB_WARPS, lead.rows - row0);
   if (!lead.valid || rows <= 0) return;
   int parts = 1;
   for (;; parts += 32) {
@@ -514,29 +514,29 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float most = -INFINITY, sum = 0.0f;
   if (row - row0 < rows) {
-    for (int p0 = group; p0 < parts; p0 += 8 * groups) {
-      float2 ml[8];
-      float4 u[8];
+    for (int p0 = group; p0 < parts; p0 += CB_BATCH * groups) {
+      float2 ml[CB_BATCH];
+      float4 u[CB_BATCH];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < CB_BATCH; ++k) {
         const int p = p0 + k * groups;
         ml[k] = make_float2(-INFINITY, 0.0f);
         u[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (p < parts) {
-          const long long at = (p ? 2ll * (c + p) : 2ll * c + 1) * item_rows + row;
+          const long long at = (p ? 2ll * (c + p) : 2ll * c + 1) * item_rows + pa_place(J, row);
           ml[k] = J.part_ml[at];
           if (col < DP) u[k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
         }
       }
       float now = most;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) now = fmaxf(now, ml[k].x);
+      for (int k = 0; k < CB_BATCH; ++k) now = fmaxf(now, ml[k].x);
       const float f = now == -INFINITY ? 1.0f : pa_exp2(most - now);
       sum *= f;
       v.x *= f; v.y *= f; v.z *= f; v.w *= f;
       most = now;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < CB_BATCH; ++k) {
         if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;
         const float w = pa_exp2(ml[k].x - now);
         sum += w * ml[k].y;
@@ -674,6 +674,17 @@ bool encode_cache(CUtensorMap* map, const GlqbPagedCache* c, const void* base, i
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// heads that share a key head, of as many queries as make 128 rows
+bool encode_queries(CUtensorMap* map, const GlqbPagedCache* c, const GlqbPagedAttention* a) {
+  const int group = a->heads / c->kv_heads;
+  const cuuint64_t dims[3] = {(cuuint64_t)c->head_dim, (cuuint64_t)a->heads, (cuuint64_t)a->tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)(a->heads > 1 ? a->query_head * 2 : 16), (cuuint64_t)(a->tokens > 1 ? a->query_token * 2 : 16)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(128 / group)}, ones[3] = {1, 1, 1};
+  const EncodeTiled encode = encode_tiled();
+  return encode && encode(map, c->dtype == GLQB_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(a->query), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // What a call launches and keeps in its workspace, by its sizes alone.
 struct PagedForm {
   bool tile;                        // on the tensor cores
@@ -684,7 +695,8 @@ struct PagedForm {
 constexpr int PA_STREAM_MOST = 16;
 PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int sms) {
   PagedForm f;
-  f.tile = (long long)std::max(1, a->max_query_len) * (a->heads / c->kv_heads) > PA_STREAM_MOST;
+  const int group = a->heads / c->kv_heads;
+  f.tile = (long long)std::max(1, a->max_query_len) * group > PA_STREAM_MOST && group <= 128;
   f.rows = f.tile ? PA_TILE_ROWS : PA_STREAM_ROWS;
   f.dp = c->head_dim <= 64 ? 64 : 128;
   f.ctas = f.tile ? sms : 2 * sms;
@@ -707,14 +719,14 @@ int check_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a) {
 }
 
 template <typename T, int DP>
-cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   using C = StreamShape<DP>;
   constexpr auto K = paged_stream_kernel<T, DP>;
-  const cudaError_t e = f.tile ? paged_tile_launch(J, __is_same(T, __nv_bfloat16), mk, mv, f.ctas, stream)
+  const cudaError_t e = f.tile ? paged_tile_launch(J, __is_same(T, __nv_bfloat16), mq, mk, mv, f.ctas, stream)
                                : paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
   if (e != cudaSuccess) return e;
   constexpr auto CB = paged_combine_kernel<T, DP>;
-  return paged_launch<CB>(CB, dim3((unsigned)f.ctas, (unsigned)f.rows / 16), CB_WARPS * 32, 0, stream, J, f.ctas, f.rows);
+  return paged_launch<CB>(CB, dim3((unsigned)f.ctas, (unsigned)f.rows / CB_WARPS), CB_WARPS * 32, 0, stream, J, f.ctas, f.rows);
 }
 }  // namespace
 }  // namespace glqb
@@ -801,17 +813,19 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   if (const int rc = check_attention(c, a)) return rc;
   if (a->tokens == 0) return GLQB_OK;
   if (!a->query || !a->out || (a->sequences && (!a->lengths || (a->page_columns && !a->page_table)))) return pg_fail(GLQB_E_INVALID, "%s: null argument", what);
-  if (!lies_on(a->query, 4) || a->query_token % 2 || a->query_head % 2) return pg_fail(GLQB_E_INVALID, "%s: queries lie on 4 bytes", what);
+  if (!lies_on(a->query, 16) || a->query_token % 8 || a->query_head % 8 || a->query_token < 0 || a->query_head < 0 || a->query_token >= 1ll << 38 || a->query_head >= 1ll << 38)
+    return pg_fail(GLQB_E_INVALID, "%s: queries lie on 16 bytes, their strides are multiples of 8 values", what);
   if (!lies_on(a->out, 2) || !lies_on(a->page_table, 4) || !lies_on(a->lengths, a->lengths_are_int64 ? 8 : 4) || !lies_on(a->offsets, a->offsets_are_int64 ? 8 : 4))
     return pg_fail(GLQB_E_INVALID, "%s: values that are not aligned", what);
-  if (!lies_on(workspace, 16)) return pg_fail(GLQB_E_INVALID, "%s: the workspace must be 16-byte aligned", what);
+  if (!lies_on(workspace, 32)) return pg_fail(GLQB_E_INVALID, "%s: the workspace must be 32-byte aligned", what);
   const PagedDevice* d = pg_device();
   if (!d) return pg_fail(GLQB_E_CUDA, "%s: no device", what);
   const PagedForm f = paged_form(c, a, d->sms.load(std::memory_order_relaxed));
   if (workspace_bytes < f.bytes || !workspace) return pg_fail(GLQB_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, f.bytes);
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq = {};
   if (!encode_cache(&mk, c, c->keys, c->key_page, c->key_row, c->key_head) || !encode_cache(&mv, c, c->values, c->value_page, c->value_row, c->value_head))
     return pg_fail(GLQB_E_CUDA, "%s: cuTensorMapEncodeTiled refused the cache", what);
+  if (f.tile && !encode_queries(&mq, c, a)) return pg_fail(GLQB_E_CUDA, "%s: cuTensorMapEncodeTiled refused the queries", what);
   PagedJob J = {};
   J.q = (const uint16_t*)a->query;
   J.out = a->out;
@@ -838,16 +852,18 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.clear = a->clear_rest;
   J.scale_log2 = a->scale * 1.4426950408889634f;
   J.most_keys = a->page_columns * c->page_size;
-  J.min_units = 1;
+  J.min_units = f.tile ? 2 : 1;
+  J.rows = f.tile ? 128 / J.group * J.group * 2 : PA_STREAM_ROWS;
   J.out_wide = lies_on(a->out, 8) && a->out_token % 4 == 0 && a->out_head % 4 == 0;
+  J.out_sectors = lies_on(a->out, 32) && a->out_token % 16 == 0 && a->out_head % 16 == 0;
   J.part = (float*)workspace;
   J.part_ml = (float2*)((uint8_t*)workspace + f.ml);
   J.part_of = (PagedPart*)((uint8_t*)workspace + f.part_of);
   J.status = d->status;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   cudaError_t e;
-  if (c->dtype == GLQB_DT_F16) e = f.dp == 64 ? attention_launch<__half, 64>(J, f, mk, mv, stream) : attention_launch<__half, 128>(J, f, mk, mv, stream);
-  else e = f.dp == 64 ? attention_launch<__nv_bfloat16, 64>(J, f, mk, mv, stream) : attention_launch<__nv_bfloat16, 128>(J, f, mk, mv, stream);
+  if (c->dtype == GLQB_DT_F16) e = f.dp == 64 ? attention_launch<__half, 64>(J, f, mq, mk, mv, stream) : attention_launch<__half, 128>(J, f, mq, mk, mv, stream);
+  else e = f.dp == 64 ? attention_launch<__nv_bfloat16, 64>(J, f, mq, mk, mv, stream) : attention_launch<__nv_bfloat16, 128>(J, f, mq, mk, mv, stream);
   return pg_launched(what, e);
 }
 

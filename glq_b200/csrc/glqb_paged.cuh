@@ -10,7 +10,7 @@ namespace glqb {
 
 constexpr int PA_PIECE = 64;         // most rows of a page that one copy brings
 constexpr int PA_STREAM_ROWS = 16, PA_STREAM_KEYS = 64;      // rows of an item, and keys of a tile: few rows,
-constexpr int PA_TILE_ROWS = 256, PA_TILE_KEYS = 128;        // and many
+constexpr int PA_TILE_ROWS = 256, PA_TILE_KEYS = 128;        // and many (at most: whole queries)
 constexpr float PA_LAZY = 8.0f;                              // a row's weights are relative to a score that its largest exceeds by no more
 
 struct PagedJob {
@@ -24,7 +24,8 @@ struct PagedJob {
   float scale_log2;                  // scale * log2(e): weights are powers of two
   int most_keys;                     // columns * page size
   int min_units;                     // key tiles that a CTA takes at least
-  bool out_wide;                     // rows of out lie on 8 bytes
+  int rows;                          // of an item
+  bool out_wide, out_sectors;        // rows of out lie on 8, 32 bytes
   float* part;                       // workspace: sums of items that several CTAs share, [CTA][2][rows][padded head_dim]
   float2* part_ml;                   // their largest exponent and sum, [CTA][2][rows]
   struct PagedPart* part_of;         // [CTA][2]
@@ -56,23 +57,22 @@ __device__ __forceinline__ int pa_to(const PagedJob& J, const PagedSeq& s, int i
 __device__ __forceinline__ int pa_from(const PagedJob& J, const PagedSeq& s, int i) {
   return J.window ? max(0, s.keys - s.queries + i + 1 - J.window) : 0;
 }
-// An item: ROWS rows of one sequence and key head.  Its key tiles are [lo, hi): those that any of its rows sees, one at least, so that
+// An item: J.rows rows of one sequence and key head.  Its key tiles are [lo, hi): those that any of its rows sees, one at least, so that
 // every row is written.
-template <int ROWS, int KEYS>
+template <int KEYS>
 __device__ __forceinline__ int2 pa_tiles(const PagedJob& J, const PagedSeq& s, int qt) {
-  const int last = min(s.queries - 1, pa_query(J, min(s.queries * J.group, (qt + 1) * ROWS) - 1));
-  const int to = pa_to(J, s, last), from = min(pa_from(J, s, pa_query(J, qt * ROWS)), to);
+  const int last = min(s.queries - 1, pa_query(J, min(s.queries * J.group, (qt + 1) * J.rows) - 1));
+  const int to = pa_to(J, s, last), from = min(pa_from(J, s, pa_query(J, qt * J.rows)), to);
   const int lo = from / KEYS;
   return make_int2(lo, max(lo + 1, (to + KEYS - 1) / KEYS));
 }
-template <int ROWS>
-__device__ __forceinline__ int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return (s.queries * J.group + ROWS - 1) / ROWS; }
-template <int ROWS, int KEYS>
+__device__ __forceinline__ int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return (s.queries * J.group + J.rows - 1) / J.rows; }
+template <int KEYS>
 __device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq& s) {
-  const int n = pa_q_tiles<ROWS>(J, s);
+  const int n = pa_q_tiles(J, s);
   long long sum = 0;
   for (int qt = 0; qt < n; ++qt) {
-    const int2 t = pa_tiles<ROWS, KEYS>(J, s, qt);
+    const int2 t = pa_tiles<KEYS>(J, s, qt);
     sum += t.y - t.x;
   }
   return sum;
@@ -80,6 +80,7 @@ __device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq&
 
 // Where a CTA's share of the work begins: item (seq, kv_head, q_tile), `skip` key tiles into it, `units` key tiles in all.
 struct PagedStart {
+  PagedSeq s;
   int seq, kv_head, q_tile, skip;
   long long units;
   long long warp_sum[32];
@@ -87,12 +88,12 @@ struct PagedStart {
 // The work is one list of key tiles: sequence after sequence, of each one key head after another, of each one row tile after another;
 // every CTA takes an equal run of it.  So batches of any lengths keep all SMs busy, and an item is cut only where a run ends.  Every
 // CTA counts the list itself: a thread some sequences, then a scan.  Called by all threads; ends with a block barrier.
-template <int ROWS, int KEYS>
+template <int KEYS>
 __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
   const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (J.seqs + threads - 1) / threads, first = min(J.seqs, (int)threadIdx.x * per), last = min(J.seqs, first + per);
   long long own = 0;
-  for (int i = first; i < last; ++i) own += pa_units<ROWS, KEYS>(J, pa_seq(J, i)) * J.kv_heads;
+  for (int i = first; i < last; ++i) own += pa_units<KEYS>(J, pa_seq(J, i)) * J.kv_heads;
   long long sum = own;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -114,14 +115,15 @@ __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
       long long r = begin - before;
       for (int i = first; i < last; ++i) {
         const PagedSeq s = pa_seq(J, i);
-        const long long per_head = pa_units<ROWS, KEYS>(J, s);
+        const long long per_head = pa_units<KEYS>(J, s);
         if (r >= per_head * J.kv_heads) { r -= per_head * J.kv_heads; continue; }
+        S.s = s;
         S.seq = i;
         S.kv_head = (int)(r / per_head);
         r -= S.kv_head * per_head;
         int qt = 0;
         for (;; ++qt) {
-          const int2 t = pa_tiles<ROWS, KEYS>(J, s, qt);
+          const int2 t = pa_tiles<KEYS>(J, s, qt);
           if (r < t.y - t.x) break;
           r -= t.y - t.x;
         }
@@ -144,21 +146,21 @@ struct PagedItem {
   int lo, hi;                        // key tiles of this CTA
   int slot;                          // -1: the whole item; else its place in the workspace
 };
-template <int ROWS, int KEYS>
+template <int KEYS>
 struct PagedWalk {
   PagedSeq s;
   int seq, kv_head, qt, skip, q_tiles;
   long long left;
   PagedPart part[2];                 // what the CTA leaves in the workspace
   __device__ __forceinline__ PagedWalk(const PagedJob& J, const PagedStart& S)
-      : seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(0), left(S.units) {
+      : s(S.s), seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(0), left(S.units) {
     part[0] = part[1] = PagedPart{0, 1, 0, 0, 0, 0, 0, 0};
-    if (left > 0) { s = pa_seq(J, seq); q_tiles = pa_q_tiles<ROWS>(J, s); }
+    if (left > 0) q_tiles = pa_q_tiles(J, s);
   }
   __device__ __forceinline__ PagedItem next(const PagedJob& J) {
     PagedItem it{};
     if (left <= 0) return it;
-    const int2 t = pa_tiles<ROWS, KEYS>(J, s, qt);
+    const int2 t = pa_tiles<KEYS>(J, s, qt);
     const int n = t.y - t.x, take = (int)min((long long)(n - skip), left);
     it.more = 1;
     it.row0 = s.row0;
@@ -166,8 +168,8 @@ struct PagedWalk {
     it.keys = s.keys;
     it.seq = seq;
     it.kv_head = kv_head;
-    it.first = qt * ROWS;
-    it.rows = min(ROWS, s.queries * J.group - it.first);
+    it.first = qt * J.rows;
+    it.rows = min(J.rows, s.queries * J.group - it.first);
     it.lo = t.x + skip;
     it.hi = it.lo + take;
     it.slot = take == n ? -1 : skip ? 0 : 1;
@@ -180,13 +182,15 @@ struct PagedWalk {
         kv_head = 0;
         if (left > 0) {
           do { s = pa_seq(J, ++seq); } while (s.queries == 0 && seq + 1 < J.seqs);
-          q_tiles = pa_q_tiles<ROWS>(J, s);
+          q_tiles = pa_q_tiles(J, s);
         }
       }
     }
     return it;
   }
 };
+// A row's place among its item's parts in the workspace: tiles of many rows lie 128 apart
+__device__ __forceinline__ int pa_place(const PagedJob& J, int row) { return J.rows > PA_STREAM_ROWS && row >= J.rows / 2 ? row + 128 - J.rows / 2 : row; }
 __device__ __forceinline__ void pa_publish(const PagedJob& J, const PagedPart (&part)[2]) {
   J.part_of[2 * blockIdx.x] = part[0];
   J.part_of[2 * blockIdx.x + 1] = part[1];
@@ -281,7 +285,7 @@ inline cudaError_t paged_launch(void (*kernel)(P...), dim3 grid, int threads, si
 }
 
 // ---- glqb_paged_tile.cu
-// Many rows, on the tensor cores: J's items are PA_TILE_ROWS x PA_TILE_KEYS, one CTA per SM.
-cudaError_t paged_tile_launch(const PagedJob& J, bool bf16, const CUtensorMap& keys, const CUtensorMap& values, int ctas, cudaStream_t stream);
+// Many rows, on the tensor cores: one CTA per SM, items of two tiles of J.rows / 2 rows.  `queries`: boxes of 64 values x a group of heads x 128 / group tokens.
+cudaError_t paged_tile_launch(const PagedJob& J, bool bf16, const CUtensorMap& queries, const CUtensorMap& keys, const CUtensorMap& values, int ctas, cudaStream_t stream);
 
 }  // namespace glqb

@@ -1,12 +1,12 @@
 // Attention of many rows over a paged cache, on the tensor cores.
 //
-// An item is 256 rows (heads of a group that share a key head, times queries) of one sequence, as two tiles of 128, against tiles of 128
-// keys.  Scores S = Q K^T go to tensor memory; a thread has a row of them: four warps per tile take their largest, turn them into weights
+// An item is up to 256 rows (heads of a group that share a key head, times queries) of one sequence, as two tiles of the whole queries that 128
+// rows hold, against tiles of 128 keys.  Scores S = Q K^T go to tensor memory; a thread has a row of them: four warps per tile take their largest, turn them into weights
 // P = 2^(scale (S - reference)) in the values' type and put those back over the scores, as the operand from tensor memory of O += P V.  While
 // one tile's weights are formed, the tensor cores work for the other.  Tensor memory: 128 columns of scores and 128 of sums per tile, all of it.
 //
 // Warps 0-3 and 4-7: the tiles' weights, and their results; 8: one thread issues all MMAs; 9: TMA of keys and values (a stage is one tile
-// of either), and the list of items; 10 and 11: values of tiles that not every row sees.  Rows of values behind the sequence, or in front
+// of either), and the list of items; 10: values of tiles that not every row sees; 11: TMA of queries.  Rows of values behind the sequence, or in front
 // of its window, may hold anything, and a weight of nothing times NaN is NaN: those rows are set to zero in shared memory.  Rows that only some queries
 // see have to stay; where such a tile holds a value that is not finite, its product is left out of the MMAs and formed one row at a time.
 //
@@ -18,7 +18,7 @@ namespace glqb {
 namespace {
 
 constexpr int TL_THREADS = 384, TL_ITEMS = 4, TL_CHECKED = 6;
-constexpr int TL_MMA = 8, TL_LOAD = 9, TL_CHECK = 10, TL_CHECKERS = 2;
+constexpr int TL_MMA = 8, TL_LOAD = 9, TL_CHECK = 10, TL_QUERY = 11;
 template <int DP>
 struct TileShape {
   static constexpr int HALF = PA_TILE_KEYS * 128, STAGE = HALF * (DP / 64), Q_TILE = 128 * DP * 2, STAGES = DP == 64 ? 10 : 5;
@@ -30,8 +30,8 @@ struct TileShape {
 struct __align__(16) TileShared {
   PagedStart start;
   PagedItem item[TL_ITEMS];
-  uint64_t full[10], empty[10], item_full[TL_ITEMS], item_empty[TL_ITEMS], q_full[2], s_full[2], p_full[2], o_full[2], checked[TL_CHECKED], drain;
-  int odd[TL_CHECKED][TL_CHECKERS];
+  uint64_t full[10], empty[10], item_full[TL_ITEMS], item_empty[TL_ITEMS], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], checked[TL_CHECKED], drain;
+  int odd[TL_CHECKED];
   uint32_t tmem;
   int abort;
 };
@@ -69,45 +69,60 @@ template <int N> __device__ __forceinline__ void fewer_registers() { asm volatil
 // Is there a key in a tile that one of the rows first .. last (of the sequence's queries * group) does not see?
 __device__ __forceinline__ bool ragged(int key0, int all_from, int all_to) { return key0 < all_from || key0 + PA_TILE_KEYS > all_to; }
 
-// An item's rows of queries, as the operand of a tile: 128 rows, columns behind head_dim and rows behind the last zero.  16 lanes take a row.
-template <int DP>
-__device__ __forceinline__ void load_queries(const PagedJob& J, const PagedItem& it, int tile, int thread, uint4 (&v)[DP / 8]) {
-  constexpr int LANES = DP / 8;
-  const int col = thread % LANES * 8;
-#pragma unroll
-  for (int n = 0; n < DP / 8; ++n) {
-    const int r = tile * 128 + thread / LANES + n * (128 / LANES), row = it.first + r, i = pa_query(J, row);
-    v[n] = make_uint4(0, 0, 0, 0);
-    if (r < it.rows && col < J.head_dim)
-      v[n] = *reinterpret_cast<const uint4*>(J.q + (long long)(it.row0 + i) * J.q_token + (long long)(it.kv_head * J.group + row - i * J.group) * J.q_head + col);
-  }
+// `rows` rows x 64 values of queries: coordinates (value, head, token)
+__device__ __forceinline__ void load_queries(void* dst, const CUtensorMap* map, int x, int head, int token, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(map),
+               "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
+               : "memory");
 }
-template <int DP>
-__device__ __forceinline__ void store_queries(uint8_t* q, int thread, const uint4 (&v)[DP / 8]) {
-  constexpr int LANES = DP / 8;
-  const int chunk = thread % LANES;
-#pragma unroll
-  for (int n = 0; n < DP / 8; ++n) {
-    const int r = thread / LANES + n * (128 / LANES);
-    *reinterpret_cast<uint4*>(q + (chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = v[n];
-  }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// the largest of three; not a number if one of them is not
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 32 bytes at once
+__device__ __forceinline__ void store8(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+struct f2 { uint64_t v; };
+__device__ __forceinline__ f2 f2_of(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_to(f2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(TL_THREADS, 1)
-paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using C = TileShape<DP>;
-  constexpr int ROWS = PA_TILE_ROWS, KEYS = PA_TILE_KEYS;
+  constexpr int KEYS = PA_TILE_KEYS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* queries = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* ring = queries + 2 * C::Q_TILE;
   TileShared& B = *reinterpret_cast<TileShared*>(ring + C::STAGES * C::STAGE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&B.full[s], 1); mbar_init(&B.empty[s], 1); }
-    for (int s = 0; s < TL_ITEMS; ++s) { mbar_init(&B.item_full[s], 1); mbar_init(&B.item_empty[s], 9 + TL_CHECKERS); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&B.q_full[s], 4); mbar_init(&B.s_full[s], 1); mbar_init(&B.p_full[s], 4); mbar_init(&B.o_full[s], 1); }
-    for (int s = 0; s < TL_CHECKED; ++s) mbar_init(&B.checked[s], TL_CHECKERS);
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&B.full[s], 1); mbar_init(&B.empty[s], 2); }
+    for (int s = 0; s < TL_ITEMS; ++s) { mbar_init(&B.item_full[s], 1); mbar_init(&B.item_empty[s], 11); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&B.q_full[s], 1); mbar_init(&B.q_empty[s], 1); mbar_init(&B.s_full[s], 1); mbar_init(&B.p_full[s], 4); mbar_init(&B.o_full[s], 1); }
+    for (int s = 0; s < TL_CHECKED; ++s) mbar_init(&B.checked[s], 1);
     mbar_init(&B.drain, 1);
     B.abort = 0;
     fence_mbar_init();
@@ -117,11 +132,12 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
     tmem_alloc(&B.tmem, 512);
     tmem_relinquish();
   }
-  if (warp == TL_LOAD && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &map_v : &map_k)) : "memory");
+  if (warp == TL_LOAD && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 2 ? &map_q : lane ? &map_v : &map_k)) : "memory");
   tc_fence_before();
   pdl_wait();
   pdl_trigger();
-  pa_start<ROWS, KEYS>(J, B.start);                        // (ends with a block barrier)
+  pa_start<KEYS>(J, B.start);                        // (ends with a block barrier)
   tc_fence_after();
   const uint32_t tmem = B.tmem;
   volatile int* abort = &B.abort;
@@ -145,28 +161,21 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
     more_registers<200>();
     const int t = warp >> 2, thread = threadIdx.x & 127, quarter = warp & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, scores = tmem + lanes + (uint32_t)t * 128u, sums = tmem + lanes + C::SUMS + (uint32_t)t * 128u;
-    uint8_t* q = queries + t * C::Q_TILE;
     uint32_t s_phase = 0, o_phase = 0, n_checked = 0;
     const float c = J.scale_log2;
+    const int tile_rows = J.rows / 2;
     PagedItem it;
     ok = take(it);
-    uint4 qv[DP / 8];
-    bool mine = ok && it.more && t * 128 < it.rows;
-    if (mine) {
-      load_queries<DP>(J, it, t, thread, qv);
-      store_queries<DP>(q, thread, qv);
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B.q_full[t]);
-    }
     while (ok && it.more) {
       const PagedSeq seq{it.row0, it.queries, it.keys};
       const int i0 = pa_query(J, it.first), i1 = pa_query(J, it.first + it.rows - 1);
       const int item_from = pa_from(J, seq, i1), item_to = pa_to(J, seq, i0);
-      const int r = t * 128 + quarter * 32 + lane, row = it.first + min(r, it.rows - 1), i = pa_query(J, row);
+      // this thread's row (one behind the tile's last is computed as if it were that one, and not stored)
+      const bool mine = t * tile_rows < it.rows;
+      const int r = quarter * 32 + lane, row0 = it.first + (mine ? t * tile_rows : 0), rows = mine ? min(tile_rows, it.rows - t * tile_rows) : 1;
+      const int row = row0 + min(r, rows - 1), i = pa_query(J, row);
       const int from = pa_from(J, seq, i), to = pa_to(J, seq, i);
-      const int last = min(it.rows, t * 128 + 128) - 1;
-      const int all_from = pa_from(J, seq, pa_query(J, it.first + last)), all_to = pa_to(J, seq, pa_query(J, it.first + t * 128));
+      const int all_from = pa_from(J, seq, pa_query(J, row0 + rows - 1)), all_to = pa_to(J, seq, pa_query(J, row0));
       float m = -INFINITY, l = 0.0f;                       // (m: of scores without their scale)
       for (int tile = it.lo; tile < it.hi; ++tile) {
         const int key0 = tile * KEYS;
@@ -179,7 +188,8 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
 #pragma unroll
           for (int n = 0; n < 4; ++n) tmem_ld32(scores + n * 32u, s[n]);
           tmem_ld_wait();
-          if (ragged(key0, all_from, all_to)) {
+          const bool cut = ragged(key0, all_from, all_to);
+          if (cut) {
             const int lo = from - key0, hi = to - key0;
 #pragma unroll
             for (int n = 0; n < 4; ++n)
@@ -187,12 +197,15 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
               for (int k = 0; k < 32; ++k)
                 if (n * 32 + k < lo || n * 32 + k >= hi) s[n][k] = 0xFF800000u;
           }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float top[4];
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
+          for (int n = 0; n < 4; ++n) {
+            top[n] = __uint_as_float(s[n][0]);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) top[n] = fmaxf(top[n], __uint_as_float(s[n][k]));
-          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            for (int k = 1; k < 31; k += 2) top[n] = max3(top[n], __uint_as_float(s[n][k]), __uint_as_float(s[n][k + 1]));
+          }
+          // (not a number if a score is none: then the reference stays, and that score's weight says so)
+          const float most = max3(max3(top[0], top[1], __uint_as_float(s[0][31])), max3(top[2], top[3], __uint_as_float(s[1][31])), max3(__uint_as_float(s[2][31]), __uint_as_float(s[3][31]), top[0]));
           const bool grown = (most - m) * c > PA_LAZY;     // (from nothing: infinity; nothing from nothing: not a number, no)
           if (__any_sync(0xFFFFFFFFu, grown)) {
             const float now = fmaxf(m, most), f = now == -INFINITY ? 1.0f : pa_exp2((m - now) * c);
@@ -212,27 +225,31 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
             }
           }
           const float less = m == -INFINITY ? 0.0f : m * c;
-          float sum[4] = {};
-          uint32_t p[64];
+          const f2 c2 = f2_of(c, c), less2 = f2_of(-less, -less);
+          f2 sum[2] = {f2_of(l, 0.0f), f2_of(0.0f, 0.0f)};
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < 4; ++n) {
+            uint32_t p[16];
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float u = pa_exp2(fmaf(__uint_as_float(s[n][k]), c, -less)), v = pa_exp2(fmaf(__uint_as_float(s[n][k + 1]), c, -less));
-              sum[n] += u + v;
-              p[n * 16 + k / 2] = pa_pack<T>(u, v);
+            for (int k = 0; k < 16; ++k) {
+              float u, v;
+              f2_to(f2_fma(f2_of(__uint_as_float(s[n][2 * k]), __uint_as_float(s[n][2 * k + 1])), c2, less2), u, v);
+              u = pa_exp2(u);
+              v = pa_exp2(v);
+              sum[k & 1] = f2_add(sum[k & 1], f2_of(u, v));
+              p[k] = pa_pack<T>(u, v);
             }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st32(scores, p);
-          tmem_st32(scores + 32u, p + 32);
+            tmem_st16(scores + n * 16u, p);
+          }
+          float part[4];
+          f2_to(sum[0], part[0], part[1]);
+          f2_to(sum[1], part[2], part[3]);
+          l = (part[0] + part[1]) + (part[2] + part[3]);
           tmem_st_wait();
           if (check) {
             const uint32_t n = n_checked % TL_CHECKED;
             if (!mbar_wait_warp(&B.checked[n], n_checked / TL_CHECKED & 1u, abort)) { ok = false; break; }
-            int odd = 0;
-#pragma unroll
-            for (int k = 0; k < TL_CHECKERS; ++k) odd |= *(volatile int*)&B.odd[n][k];
-            if (odd) {
+            if (*(volatile int*)&B.odd[n]) {
               // a value that is not finite among those that only some rows see: this row's keys one at a time.  (The stage of the values: that
               // behind the keys', two stages per tile.)
               const uint32_t vs = (stage + 1u) % C::STAGES, base = smem_u32(ring) + vs * C::STAGE;
@@ -287,47 +304,42 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         advance();
       }
       if (!ok) break;
-      // the next item's queries, as soon as this one's products are done; then this one's results
-      PagedItem then;
-      if (!take(then)) { ok = false; break; }
-      const bool mine_then = then.more && t * 128 < then.rows;
-      if (mine_then) load_queries<DP>(J, then, t, thread, qv);
       if (mine) {
         if (!mbar_wait_warp(&B.o_full[t], o_phase, abort)) { ok = false; break; }
         o_phase ^= 1u;
         tc_fence_after();
-      }
-      if (mine_then) {
-        store_queries<DP>(q, thread, qv);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B.q_full[t]);
-      }
-      if (mine) {
-        const bool there = r < it.rows;
+        // A thread has a row: 32 bytes of it at once are whole sectors.  (8 bytes at once took 12,000 clocks per item.)
+        const bool there = r < rows;
         const float f = it.slot < 0 ? pa_row_factor(J, seq, row, l) : 1.0f;
-        const long long at = pa_out_row(J, it.row0, it.kv_head, row), place = (2ll * blockIdx.x + max(it.slot, 0)) * ROWS + r;
+        const long long at = pa_out_row(J, it.row0, it.kv_head, row), place = (2ll * blockIdx.x + max(it.slot, 0)) * PA_TILE_ROWS + t * 128 + r;
         if (it.slot >= 0 && there) J.part_ml[place] = make_float2(m * c, l);
 #pragma unroll 1
         for (int n = 0; n < DP / 32; ++n) {
           uint32_t o[32];
           tmem_ld32(sums + n * 32u, o);
           tmem_ld_wait();
-          if (there) {
+          if (there && it.slot >= 0) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 v = make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f, __uint_as_float(o[k + 3]) * f);
-              const int col = n * 32 + k;
-              if (it.slot >= 0) *reinterpret_cast<float4*>(J.part + place * DP + col) = v;
-              else if (col < J.head_dim) pa_store4<T>(J, at, col, v);
+            for (int k = 0; k < 32; k += 8) store8(J.part + place * DP + n * 32 + k, o + k);
+          } else if (there) {
+            if (J.out_sectors && n * 32 + 32 <= J.head_dim) {
+              uint32_t y[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = pa_pack<T>(__uint_as_float(o[2 * k]) * f, __uint_as_float(o[2 * k + 1]) * f);
+              store8(reinterpret_cast<uint16_t*>(J.out) + at + n * 32, y);
+              store8(reinterpret_cast<uint16_t*>(J.out) + at + n * 32 + 16, y + 8);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4)
+                if (n * 32 + k < J.head_dim)
+                  pa_store4<T>(J, at, n * 32 + k, make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f, __uint_as_float(o[k + 3]) * f));
             }
           }
           __syncwarp();
         }
         tc_fence_before();
       }
-      it = then;
-      mine = mine_then;
+      ok = take(it);
     }
     if (!ok && lane == 0) { *abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_EPILOGUE); }
   } else {
@@ -351,7 +363,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         if (!ok || !it.more) break;
         const PagedSeq seq{it.row0, it.queries, it.keys};
         const int item_from = pa_from(J, seq, pa_query(J, it.first + it.rows - 1)), item_to = pa_to(J, seq, pa_query(J, it.first));
-        const int tiles = it.rows > 128 ? 2 : 1;
+        const int tiles = it.rows > J.rows / 2 ? 2 : 1;
         ok = mbar_wait_warp(&B.full[stage], phase, abort);
         for (int t = 0; t < tiles && ok; ++t) {
           ok = mbar_wait_warp(&B.q_full[t], q_phase[t], abort);
@@ -359,7 +371,10 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
           q_phase[t] ^= 1u;
           tc_fence_after();
           scores_of(t, stage);
-          if (one) umma_commit(&B.s_full[t]);
+          if (one) {
+            umma_commit(&B.s_full[t]);
+            if (it.lo + 1 == it.hi) umma_commit(&B.q_empty[t]);
+          }
         }
         if (!ok) break;
         if (one) umma_commit(&B.empty[stage]);
@@ -382,8 +397,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
             ok = mbar_wait_warp(&B.checked[n], n_checked / TL_CHECKED & 1u, abort);
             if (!ok) break;
             ++n_checked;
-#pragma unroll
-            for (int k = 0; k < TL_CHECKERS; ++k) odd |= *(volatile int*)&B.odd[n][k];
+            odd = *(volatile int*)&B.odd[n];
           }
           for (int t = 0; t < tiles; ++t) {
             ok = mbar_wait_warp(&B.p_full[t], p_phase[t], abort);
@@ -398,7 +412,10 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
             }
             // (one thread's products run in the order they are issued in: the weights are read before new scores take their place)
             if (more) scores_of(t, ks);
-            if (one) umma_commit(more ? &B.s_full[t] : &B.o_full[t]);
+            if (one) {
+              umma_commit(more ? &B.s_full[t] : &B.o_full[t]);
+              if (more && tile + 2 == it.hi) umma_commit(&B.q_empty[t]);
+            }
           }
           if (!ok) break;
           if (one) {
@@ -416,7 +433,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         mbar_wait_warp(&B.drain, 0);
       }
     } else if (warp == TL_LOAD) {
-      PagedWalk<ROWS, KEYS> walk(J, B.start);
+      PagedWalk<KEYS> walk(J, B.start);
       const int piece = min(1 << J.page_log, PA_PIECE), pieces = KEYS / piece, page_mask = (1 << J.page_log) - 1;
       phase = 1;
       ip = 1;
@@ -457,9 +474,35 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
       // copies in flight land before the block ends
       if (!ok)
         for (uint32_t n = 1; n <= min(filled, (uint32_t)C::STAGES); ++n) mbar_wait(&B.full[(filled - n) % C::STAGES], (filled - n) / C::STAGES & 1u);
+    } else if (warp == TL_QUERY) {
+      uint32_t e_phase[2] = {1, 1}, issued[2] = {0, 0};
+      const int tile_rows = J.rows / 2;
+      PagedItem it;
+      for (;;) {
+        ok = take(it);
+        if (!ok || !it.more) break;
+        for (int t = 0; t < 2 && t * tile_rows < it.rows; ++t) {
+          if (!mbar_wait_warp(&B.q_empty[t], e_phase[t], abort)) { ok = false; break; }
+          e_phase[t] ^= 1u;
+          if (lane == 0) {
+            // (rows behind the sequence's last query are another's, or zeros behind the last token: they are computed and not stored)
+            mbar_expect_tx(&B.q_full[t], (uint32_t)tile_rows * DP * 2);
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h)
+              load_queries(queries + t * C::Q_TILE + h * (128 * 128), &map_q, h * 64, it.kv_head * J.group, it.row0 + pa_query(J, it.first + t * tile_rows), &B.q_full[t]);
+          }
+          __syncwarp();
+          ++issued[t];
+        }
+        if (!ok) break;
+      }
+      if (!ok) {
+        if (lane == 0) { *abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
+        for (int t = 0; t < 2; ++t)
+          if (issued[t]) mbar_wait(&B.q_full[t], (issued[t] - 1) & 1u);
+      }
     } else {
       // values of tiles that not every row sees
-      const int thread = (warp - TL_CHECK) * 32 + lane;
       uint32_t n_checked = 0;
       PagedItem it;
       for (;;) {
@@ -469,29 +512,38 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         const int i0 = pa_query(J, it.first), i1 = pa_query(J, it.first + it.rows - 1);
         const int item_from = pa_from(J, seq, i1), item_to = pa_to(J, seq, i0), any_from = pa_from(J, seq, i0), any_to = pa_to(J, seq, i1);
         for (int tile = it.lo; tile < it.hi; ++tile) {
-          advance();                                       // (the keys')
+          // Every stage is waited for and given back, also those with nothing to look at: a wait by parity takes a barrier that is two phases
+          // behind for ready, so a warp may not be ahead of the ring, nor the ring ahead of it.
+          if (!mbar_wait_warp(&B.full[stage], phase, abort)) { ok = false; break; }
+          if (lane == 0) mbar_arrive(&B.empty[stage]);
+          advance();
+          if (!mbar_wait_warp(&B.full[stage], phase, abort)) { ok = false; break; }
           if (ragged(tile * KEYS, item_from, item_to)) {
             const uint32_t n = n_checked % TL_CHECKED;
-            if (!mbar_wait_warp(&B.full[stage], phase, abort)) { ok = false; break; }
             bool odd = false;
-#pragma unroll 4
-            for (int k = thread; k < KEYS * (DP / 8); k += TL_CHECKERS * 32) {
-              const int key = tile * KEYS + k / (DP / 8), chunk = k % (DP / 8);
-              uint4* p = reinterpret_cast<uint4*>(ring + stage * C::STAGE + (chunk >> 3) * C::HALF + (k / (DP / 8)) * 128 + ((chunk & 7) << 4));
-              if (key < any_from || key >= any_to) {
-                *p = make_uint4(0, 0, 0, 0);
-              } else {
-                const uint4 v = *p;
-                odd = odd || pa_not_finite<T>(v.x) || pa_not_finite<T>(v.y) || pa_not_finite<T>(v.z) || pa_not_finite<T>(v.w);
+            uint8_t* values = ring + stage * C::STAGE;
+            const int first = any_from - tile * KEYS, last = any_to - tile * KEYS;
+#pragma unroll 1
+            for (int k0 = lane; k0 < KEYS * (DP / 8); k0 += 8 * 32) {
+              // (eight loads before the first store; 16 bytes of a row lie somewhere within its 128)
+              uint4 v[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4*>(values + (k0 + k * 32) * 16);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const int key = (k0 + k * 32) / 8 % KEYS;
+                if (key < first || key >= last) *reinterpret_cast<uint4*>(values + (k0 + k * 32) * 16) = make_uint4(0, 0, 0, 0);
+                else odd = odd || pa_not_finite<T>(v[k].x) || pa_not_finite<T>(v[k].y) || pa_not_finite<T>(v[k].z) || pa_not_finite<T>(v[k].w);
               }
             }
             odd = __any_sync(0xFFFFFFFFu, odd);
             fence_async_smem();
-            if (lane == 0) *(volatile int*)&B.odd[n][warp - TL_CHECK] = odd;
+            if (lane == 0) *(volatile int*)&B.odd[n] = odd;
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.checked[n]);
             ++n_checked;
           }
+          if (lane == 0) mbar_arrive(&B.empty[stage]);
           advance();
         }
         if (!ok) break;
@@ -510,18 +562,18 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
 }
 
 template <typename T, int DP>
-cudaError_t run(const PagedJob& J, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t stream) {
+cudaError_t run(const PagedJob& J, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t stream) {
   using C = TileShape<DP>;
   constexpr size_t SMEM = 1024 + 2 * C::Q_TILE + C::STAGES * C::STAGE + sizeof(TileShared);
   static_assert(SMEM <= 227 * 1024, "");
   static_assert(SMEM > 114 * 1024, "two CTAs on an SM would wait for each other's tensor memory");
   constexpr auto K = paged_tile_kernel<T, DP>;
-  return paged_launch<K>(K, dim3((unsigned)ctas), TL_THREADS, SMEM, stream, J, mk, mv);
+  return paged_launch<K>(K, dim3((unsigned)ctas), TL_THREADS, SMEM, stream, J, mq, mk, mv);
 }
 }  // namespace
 
-cudaError_t paged_tile_launch(const PagedJob& J, bool bf16, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t stream) {
-  if (J.head_dim <= 64) return bf16 ? run<__nv_bfloat16, 64>(J, mk, mv, ctas, stream) : run<__half, 64>(J, mk, mv, ctas, stream);
-  return bf16 ? run<__nv_bfloat16, 128>(J, mk, mv, ctas, stream) : run<__half, 128>(J, mk, mv, ctas, stream);
+cudaError_t paged_tile_launch(const PagedJob& J, bool bf16, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t stream) {
+  if (J.head_dim <= 64) return bf16 ? run<__nv_bfloat16, 64>(J, mq, mk, mv, ctas, stream) : run<__half, 64>(J, mq, mk, mv, ctas, stream);
+  return bf16 ? run<__nv_bfloat16, 128>(J, mq, mk, mv, ctas, stream) : run<__half, 128>(J, mq, mk, mv, ctas, stream);
 }
 }  // namespace glqb

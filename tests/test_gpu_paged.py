@@ -352,6 +352,38 @@ def test_long_context(dtype):
     assert (y[0].double() - ref).abs().max() <= 2 * U[dtype] * values.abs().max().double()
 
 
+def _reference_chunks(q, k, v, pages, lengths, offsets, window=0):
+    """Attention in 64 bits on the device, a sequence and key head at a time."""
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    g = q.shape[1] // k.shape[2]
+    for i, n in enumerate(lengths.tolist()):
+        a, b = int(offsets[i]), int(offsets[i + 1])
+        if a == b:
+            continue
+        ids = pages[i, :-(-n // k.shape[1])].long()
+        at, key = torch.arange(n - (b - a), n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+        seen = (key <= at) & ((key > at - window) if window else True)
+        for h in range(k.shape[2]):
+            z = torch.einsum("qgd,kd->gqk", q[a:b, h * g:(h + 1) * g].double(), k[ids][:, :, h].flatten(0, 1)[:n].double()) * q.shape[2] ** -0.5
+            p = torch.softmax(torch.where(seen, z, -math.inf), -1)
+            out[a:b, h * g:(h + 1) * g] = torch.einsum("gqk,kd->qgd", p, v[ids][:, :, h].flatten(0, 1)[:n].double())
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("window", [0, 1500])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (15, 3, 64)])
+@pytest.mark.parametrize("lengths,new", [([6000], [333]), ([2600], [2600]), ([5000, 17, 3000, 900, 2500, 64, 4000], [100, 17, 1, 300, 70, 1, 200])])
+def test_long_chunks(dtype, window, heads, kv, dim, lengths, new):
+    """Many key tiles per item, parts of items in several CTAs.  Values are normal: |out| <= max |v|, weights off by U each, the result by U."""
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(7), lengths, new, kv, heads, dim, 16, dtype, poison=False)
+    ref = _reference_chunks(q, k, v, pages, n, offsets, window)
+    for _ in range(3):
+        y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, window=window)
+        assert (y.double() - ref).abs().max() <= 2 * U[dtype] * v.abs().max().double()
+
+
 # ---- together -----------------------------------------------------------------------------------------------------
 def test_prompt_then_decoding_steps():
     """A prompt in two chunks and decoding steps through append and attention, as a decoder runs them, against attention over the whole."""

@@ -117,7 +117,8 @@ def test_c_entries_refuse_before_any_cuda_call(lib):
     refused(attention(out=None), -1, "null")
     refused(attention(lengths=None), -1, "null")
     refused(attention(page_table=None), -1, "null")
-    refused(attention(query=p + 2), -1, "4 bytes")
+    refused(attention(query=p + 8), -1, "16 bytes")
+    refused(attention(query_token=260), -1, "multiples of 8")
     refused(attention(ws=p + 4), -1, "aligned")
     assert attention(tokens=0, out=None) == 0
 
