@@ -481,16 +481,46 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
 }
 
 // ---- what several CTAs have of an item, together --------------------------------------------------
-// A block takes eight rows of an item that CTA blockIdx.x began and did not end: its parts are that CTA's, then those of the CTAs behind it up
-// to the one that ended the item.  A warp adds a row, several if there are few rows, each every n-th part; the order is the same in every call.
-constexpr int CB_WARPS = 8, CB_BATCH = 4;
-template <typename T, int DP>
-__global__ void __launch_bounds__(CB_WARPS * 32, 5) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas, int item_rows) {
-  __shared__ float sums[CB_WARPS][DP];
+// The parts of an item that CTA blockIdx.x began and did not end are that CTA's, then those of the CTAs behind it up to the one that ended
+// the item.  Of few rows (MANY false) a block has all: a row is several warps', each every n-th part, then together.  Of many rows there are few
+// parts: a block has 32 rows, a warp four of them at once.  The order is the same in every call.
+constexpr int CB_WARPS = 8, CB_ROWS = 32;
+struct Joined {
+  float4 v;
+  float most, sum;
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&u)[N]) {
+    float now = most;
+#pragma unroll
+    for (int k = 0; k < N; ++k) now = fmaxf(now, ml[k].x);
+    const float f = now == -INFINITY ? 1.0f : pa_exp2(most - now);
+    sum *= f;
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    most = now;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;        // (no key of its own: nothing in its sums)
+      const float w = pa_exp2(ml[k].x - now);
+      sum += w * ml[k].y;
+      v.x += w * u[k].x; v.y += w * u[k].y; v.z += w * u[k].z; v.w += w * u[k].w;
+    }
+  }
+};
+template <typename T, int DP, bool MANY>
+__global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
+  __shared__ float4 sums[CB_WARPS][DP / 4];
   __shared__ float2 mls[CB_WARPS];
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, col = lane * 4;
+  constexpr int PLACES = MANY ? PA_TILE_ROWS : PA_STREAM_ROWS, CB_BATCH = MANY ? 2 : 4;      // (parts of a row at once)
+  // (the first parts' ends are asked for before it is known whether this CTA has left a beginning)
+  const PagedPart lead = J.part_of[2 * c + 1];
+  auto ends = [&](int parts) {
+    const int at = c + parts + lane;
+    return __ballot_sync(0xFFFFFFFFu, at >= ctas || !J.part_of[2 * at].valid || J.part_of[2 * at].ends);
+  };
+  uint32_t end = ends(1);
   if (J.clear && blockIdx.y == 0) {
     const int first = pa_offset(J, 0), last = max(first, pa_offset(J, J.seqs)), rest = J.tokens - (last - first);
     for (int i = c; i < rest; i += gridDim.x) {
@@ -498,73 +528,87 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 5) paged_combine_kernel(const _
       for (int k = threadIdx.x; k < J.heads * J.head_dim; k += CB_WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
     }
   }
-  const PagedPart lead = J.part_of[2 * c + 1];
-  const int row0 = blockIdx.y * CB_WARPS, rows = min(CB_WARPS, lead.rows - row0);
-  if (!lead.valid || rows <= 0) return;
+  if (!lead.valid) return;
   int parts = 1;
-  for (;; parts += 32) {
-    const int at = c + parts + lane;
-    const bool end = at >= ctas || !J.part_of[2 * at].valid || J.part_of[2 * at].ends;
-    const uint32_t ends = __ballot_sync(0xFFFFFFFFu, end);
-    if (ends) { parts += __ffs(ends); break; }
-  }
-  int wide = 1;
-  while (wide < rows) wide <<= 1;
-  const int groups = CB_WARPS / wide, row = row0 + warp % wide, group = warp / wide, col = lane * 4;
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float most = -INFINITY, sum = 0.0f;
-  if (row - row0 < rows) {
-    for (int p0 = group; p0 < parts; p0 += CB_BATCH * groups) {
-      float2 ml[CB_BATCH];
-      float4 u[CB_BATCH];
+  while (!end) end = ends(parts += 32);
+  parts += __ffs(end);
+  auto part_at = [&](int p, int row) { return (p ? 2ll * (c + p) : 2ll * c + 1) * PLACES + pa_place(J, row); };
+  auto store = [&](int row, const Joined& j) {
+    if (col >= J.head_dim) return;
+    const float f = pa_row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, j.sum);
+    pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
+  };
+  if constexpr (MANY) {
+    Joined j[4];
 #pragma unroll
-      for (int k = 0; k < CB_BATCH; ++k) {
-        const int p = p0 + k * groups;
-        ml[k] = make_float2(-INFINITY, 0.0f);
-        u[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (p < parts) {
-          const long long at = (p ? 2ll * (c + p) : 2ll * c + 1) * item_rows + pa_place(J, row);
-          ml[k] = J.part_ml[at];
-          if (col < DP) u[k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
+    for (int n = 0; n < 4; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+    const int row0 = blockIdx.y * CB_ROWS + warp;
+    for (int p0 = 0; p0 < parts; p0 += CB_BATCH) {
+      float2 ml[4][CB_BATCH];
+      float4 u[4][CB_BATCH];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int k = 0; k < CB_BATCH; ++k) {
+          const int row = row0 + n * CB_WARPS;
+          ml[n][k] = make_float2(-INFINITY, 0.0f);
+          u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (p0 + k < parts && row < lead.rows) {
+            const long long at = part_at(p0 + k, row);
+            ml[n][k] = J.part_ml[at];
+            if (col < DP) u[n][k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
+          }
         }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) j[n].add(ml[n], u[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (row0 + n * CB_WARPS < lead.rows) store(row0 + n * CB_WARPS, j[n]);
+  } else {
+    const int row0 = blockIdx.y * CB_WARPS, rows = min(CB_WARPS, lead.rows - row0);
+    if (rows <= 0) return;
+    int wide = 1;
+    while (wide < rows) wide <<= 1;
+    const int groups = CB_WARPS / wide, row = row0 + warp % wide, group = warp / wide;
+    Joined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+    if (row - row0 < rows)
+      for (int p0 = group; p0 < parts; p0 += CB_BATCH * groups) {
+        float2 ml[CB_BATCH];
+        float4 u[CB_BATCH];
+#pragma unroll
+        for (int k = 0; k < CB_BATCH; ++k) {
+          const int p = p0 + k * groups;
+          ml[k] = make_float2(-INFINITY, 0.0f);
+          u[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (p < parts) {
+            const long long at = part_at(p, row);
+            ml[k] = J.part_ml[at];
+            if (col < DP) u[k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
+          }
+        }
+        j.add(ml, u);
       }
-      float now = most;
+    if (groups > 1) {
+      if (lane == 0) mls[warp] = make_float2(j.most, j.sum);
+      if (col < DP) sums[warp][lane] = j.v;
+      __syncthreads();
+      if (group > 0) return;
+      j = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+      for (int k0 = 0; k0 < groups; k0 += CB_BATCH) {
+        float2 ml[CB_BATCH];
+        float4 u[CB_BATCH];
 #pragma unroll
-      for (int k = 0; k < CB_BATCH; ++k) now = fmaxf(now, ml[k].x);
-      const float f = now == -INFINITY ? 1.0f : pa_exp2(most - now);
-      sum *= f;
-      v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-      most = now;
-#pragma unroll
-      for (int k = 0; k < CB_BATCH; ++k) {
-        if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;
-        const float w = pa_exp2(ml[k].x - now);
-        sum += w * ml[k].y;
-        v.x += w * u[k].x; v.y += w * u[k].y; v.z += w * u[k].z; v.w += w * u[k].w;
+        for (int k = 0; k < CB_BATCH; ++k) {
+          const bool there = k0 + k < groups;
+          ml[k] = there ? mls[warp + (k0 + k) * wide] : make_float2(-INFINITY, 0.0f);
+          u[k] = there && col < DP ? sums[warp + (k0 + k) * wide][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        j.add(ml, u);
       }
     }
+    if (row - row0 < rows) store(row, j);
   }
-  if (groups > 1) {
-    if (lane == 0) mls[warp] = make_float2(most, sum);
-    if (col < DP) *reinterpret_cast<float4*>(&sums[warp][col]) = v;
-    __syncthreads();
-    if (group > 0) return;
-    float now = most;
-    for (int k = 1; k < groups; ++k) now = fmaxf(now, mls[warp + k * wide].x);
-    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    sum = 0.0f;
-    for (int k = 0; k < groups; ++k) {
-      const float2 ml = mls[warp + k * wide];
-      if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-      const float w = pa_exp2(ml.x - now);
-      const float4 u = col < DP ? *reinterpret_cast<const float4*>(&sums[warp + k * wide][col]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      sum += w * ml.y;
-      v.x += w * u.x; v.y += w * u.y; v.z += w * u.z; v.w += w * u.w;
-    }
-  }
-  if (row - row0 >= rows || col >= J.head_dim) return;
-  const float f = pa_row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, sum);
-  pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -693,6 +737,8 @@ struct PagedForm {
 };
 // Rows of a sequence and key head up to which the streaming kernel runs.
 constexpr int PA_STREAM_MOST = 16;
+// What beginning an item costs a CTA of either kernel, in its key tiles.
+constexpr int PA_STREAM_BEGIN = 2, PA_TILE_BEGIN = 2;
 PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int sms) {
   PagedForm f;
   const int group = a->heads / c->kv_heads;
@@ -721,12 +767,15 @@ int check_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a) {
 template <typename T, int DP>
 cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   using C = StreamShape<DP>;
+  const int most_rows = PA_STREAM_ROWS;
   constexpr auto K = paged_stream_kernel<T, DP>;
   const cudaError_t e = f.tile ? paged_tile_launch(J, __is_same(T, __nv_bfloat16), mq, mk, mv, f.ctas, stream)
                                : paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
   if (e != cudaSuccess) return e;
-  constexpr auto CB = paged_combine_kernel<T, DP>;
-  return paged_launch<CB>(CB, dim3((unsigned)f.ctas, (unsigned)f.rows / CB_WARPS), CB_WARPS * 32, 0, stream, J, f.ctas, f.rows);
+  constexpr auto FEW = paged_combine_kernel<T, DP, false>;
+  constexpr auto MANY = paged_combine_kernel<T, DP, true>;
+  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS * 32, 0, stream, J, f.ctas)
+                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas, (unsigned)((std::min(PA_STREAM_ROWS, most_rows) + CB_WARPS - 1) / CB_WARPS)), CB_WARPS * 32, 0, stream, J, f.ctas);
 }
 }  // namespace
 }  // namespace glqb
@@ -852,7 +901,8 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.clear = a->clear_rest;
   J.scale_log2 = a->scale * 1.4426950408889634f;
   J.most_keys = a->page_columns * c->page_size;
-  J.min_units = f.tile ? 2 : 1;
+  J.begin = f.tile ? PA_TILE_BEGIN : PA_STREAM_BEGIN;
+  J.min_units = J.begin + (f.tile ? 2 : 1);
   J.rows = f.tile ? 128 / J.group * J.group * 2 : PA_STREAM_ROWS;
   J.out_wide = lies_on(a->out, 8) && a->out_token % 4 == 0 && a->out_head % 4 == 0;
   J.out_sectors = lies_on(a->out, 32) && a->out_token % 16 == 0 && a->out_head % 16 == 0;

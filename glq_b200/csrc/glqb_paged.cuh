@@ -23,8 +23,9 @@ struct PagedJob {
   int lengths_wide, offsets_wide, seqs, columns, page_log, tokens, heads, kv_heads, group, head_dim, causal, window, clear;
   float scale_log2;                  // scale * log2(e): weights are powers of two
   int most_keys;                     // columns * page size
-  int min_units;                     // key tiles that a CTA takes at least
+  int min_units;                     // units that a CTA takes at least
   int rows;                          // of an item
+  int begin;                         // what beginning an item costs, in key tiles
   bool out_wide, out_sectors;        // rows of out lie on 8, 32 bytes
   float* part;                       // workspace: sums of items that several CTAs share, [CTA][2][rows][padded head_dim]
   float2* part_ml;                   // their largest exponent and sum, [CTA][2][rows]
@@ -73,20 +74,20 @@ __device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq&
   long long sum = 0;
   for (int qt = 0; qt < n; ++qt) {
     const int2 t = pa_tiles<KEYS>(J, s, qt);
-    sum += t.y - t.x;
+    sum += t.y - t.x + J.begin;
   }
   return sum;
 }
 
-// Where a CTA's share of the work begins: item (seq, kv_head, q_tile), `skip` key tiles into it, `units` key tiles in all.
+// Where a CTA's share of the work begins: item (seq, kv_head, q_tile), `skip` units into it, `units` units in all.
 struct PagedStart {
   PagedSeq s;
   int seq, kv_head, q_tile, skip;
   long long units;
   long long warp_sum[32];
 };
-// The work is one list of key tiles: sequence after sequence, of each one key head after another, of each one row tile after another;
-// every CTA takes an equal run of it.  So batches of any lengths keep all SMs busy, and an item is cut only where a run ends.  Every
+// The work is one list of units: sequence after sequence, of each one key head after another, of each one row tile after another, of each such item
+// J.begin units for its beginning and one per key tile; every CTA takes an equal run of it.  So batches of any lengths keep all SMs busy, and an item is cut only where a run ends.  Every
 // CTA counts the list itself: a thread some sequences, then a scan.  Called by all threads; ends with a block barrier.
 template <int KEYS>
 __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
@@ -124,8 +125,8 @@ __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
         int qt = 0;
         for (;; ++qt) {
           const int2 t = pa_tiles<KEYS>(J, s, qt);
-          if (r < t.y - t.x) break;
-          r -= t.y - t.x;
+          if (r < t.y - t.x + J.begin) break;
+          r -= t.y - t.x + J.begin;
         }
         S.q_tile = qt;
         S.skip = (int)r;
@@ -159,30 +160,34 @@ struct PagedWalk {
   }
   __device__ __forceinline__ PagedItem next(const PagedJob& J) {
     PagedItem it{};
-    if (left <= 0) return it;
-    const int2 t = pa_tiles<KEYS>(J, s, qt);
-    const int n = t.y - t.x, take = (int)min((long long)(n - skip), left);
-    it.more = 1;
-    it.row0 = s.row0;
-    it.queries = s.queries;
-    it.keys = s.keys;
-    it.seq = seq;
-    it.kv_head = kv_head;
-    it.first = qt * J.rows;
-    it.rows = min(J.rows, s.queries * J.group - it.first);
-    it.lo = t.x + skip;
-    it.hi = it.lo + take;
-    it.slot = take == n ? -1 : skip ? 0 : 1;
-    if (it.slot >= 0) part[it.slot] = PagedPart{1, skip + take == n, s.row0, it.rows, it.first, kv_head, s.queries, s.keys};
-    left -= take;
-    skip = 0;
-    if (++qt == q_tiles) {
-      qt = 0;
-      if (++kv_head == J.kv_heads) {
-        kv_head = 0;
-        if (left > 0) {
-          do { s = pa_seq(J, ++seq); } while (s.queries == 0 && seq + 1 < J.seqs);
-          q_tiles = pa_q_tiles(J, s);
+    while (left > 0 && !it.more) {
+      const int2 t = pa_tiles<KEYS>(J, s, qt);
+      const int n = t.y - t.x, take = (int)min((long long)(n + J.begin - skip), left);
+      const int from = max(0, skip - J.begin), to = max(0, skip + take - J.begin);
+      if (from < to) {                   // (a run that ends before the first tile leaves the item to the next CTA)
+        it.more = 1;
+        it.row0 = s.row0;
+        it.queries = s.queries;
+        it.keys = s.keys;
+        it.seq = seq;
+        it.kv_head = kv_head;
+        it.first = qt * J.rows;
+        it.rows = min(J.rows, s.queries * J.group - it.first);
+        it.lo = t.x + from;
+        it.hi = t.x + to;
+        it.slot = to - from == n ? -1 : from ? 0 : 1;
+        if (it.slot >= 0) part[it.slot] = PagedPart{1, to == n, s.row0, it.rows, it.first, kv_head, s.queries, s.keys};
+      }
+      left -= take;
+      skip = 0;
+      if (++qt == q_tiles) {
+        qt = 0;
+        if (++kv_head == J.kv_heads) {
+          kv_head = 0;
+          if (left > 0) {
+            do { s = pa_seq(J, ++seq); } while (s.queries == 0 && seq + 1 < J.seqs);
+            q_tiles = pa_q_tiles(J, s);
+          }
         }
       }
     }

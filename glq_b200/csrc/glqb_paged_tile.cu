@@ -18,7 +18,7 @@ namespace glqb {
 namespace {
 
 constexpr int TL_THREADS = 384, TL_ITEMS = 4, TL_CHECKED = 6;
-constexpr int TL_MMA = 8, TL_LOAD = 9, TL_CHECK = 10, TL_QUERY = 11;
+constexpr int TL_MMA = 8, TL_LOAD = 9, TL_QUERY = 11;      // (10 checks values)
 template <int DP>
 struct TileShape {
   static constexpr int HALF = PA_TILE_KEYS * 128, STAGE = HALF * (DP / 64), Q_TILE = 128 * DP * 2, STAGES = DP == 64 ? 10 : 5;
@@ -108,6 +108,23 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   return r;
 }
 
+// Weights of 32 scores: to tensor memory in the values' type, their sum to `sum`.
+template <typename T>
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], f2 c, f2 less, f2 (&sum)[2], uint32_t taddr) {
+  uint32_t p[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const f2 x = f2_fma(f2_of(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c, less);
+    float u, v;
+    f2_to(x, u, v);
+    u = pa_exp2(u);
+    v = pa_exp2(v);
+    sum[k & 1] = f2_add(sum[k & 1], f2_of(u, v));
+    p[k] = pa_pack<T>(u, v);
+  }
+  tmem_st16(taddr, p);
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(TL_THREADS, 1)
 paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -159,7 +176,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
 
   if (warp < TL_MMA) {
     more_registers<200>();
-    const int t = warp >> 2, thread = threadIdx.x & 127, quarter = warp & 3;
+    const int t = warp >> 2, quarter = warp & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, scores = tmem + lanes + (uint32_t)t * 128u, sums = tmem + lanes + C::SUMS + (uint32_t)t * 128u;
     uint32_t s_phase = 0, o_phase = 0, n_checked = 0;
     const float c = J.scale_log2;
@@ -206,7 +223,8 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
           }
           // (not a number if a score is none: then the reference stays, and that score's weight says so)
           const float most = max3(max3(top[0], top[1], __uint_as_float(s[0][31])), max3(top[2], top[3], __uint_as_float(s[1][31])), max3(__uint_as_float(s[2][31]), __uint_as_float(s[3][31]), top[0]));
-          const bool grown = (most - m) * c > PA_LAZY;     // (from nothing: infinity; nothing from nothing: not a number, no)
+          // (from nothing: infinity; nothing from nothing: not a number, no.  What a row without a query holds decides nothing for its warp's others.)
+          const bool grown = r < rows && (most - m) * c > PA_LAZY;
           if (__any_sync(0xFFFFFFFFu, grown)) {
             const float now = fmaxf(m, most), f = now == -INFINITY ? 1.0f : pa_exp2((m - now) * c);
             m = now;
@@ -229,17 +247,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
           f2 sum[2] = {f2_of(l, 0.0f), f2_of(0.0f, 0.0f)};
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            uint32_t p[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float u, v;
-              f2_to(f2_fma(f2_of(__uint_as_float(s[n][2 * k]), __uint_as_float(s[n][2 * k + 1])), c2, less2), u, v);
-              u = pa_exp2(u);
-              v = pa_exp2(v);
-              sum[k & 1] = f2_add(sum[k & 1], f2_of(u, v));
-              p[k] = pa_pack<T>(u, v);
-            }
-            tmem_st16(scores + n * 16u, p);
+            weights<T>(s[n], c2, less2, sum, scores + n * 16u);
           }
           float part[4];
           f2_to(sum[0], part[0], part[1]);
@@ -520,23 +528,25 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
           if (!mbar_wait_warp(&B.full[stage], phase, abort)) { ok = false; break; }
           if (ragged(tile * KEYS, item_from, item_to)) {
             const uint32_t n = n_checked % TL_CHECKED;
-            bool odd = false;
-            uint8_t* values = ring + stage * C::STAGE;
-            const int first = any_from - tile * KEYS, last = any_to - tile * KEYS;
+            // (rows of 128 bytes, per 64 values; their 16-byte pieces lie somewhere within them.  Eight loads at once, and no branch.)
+            uint32_t largest = 0u;
+            const int first = min(KEYS, max(0, any_from - tile * KEYS)), last = max(first, min(KEYS, any_to - tile * KEYS));
 #pragma unroll 1
-            for (int k0 = lane; k0 < KEYS * (DP / 8); k0 += 8 * 32) {
-              // (eight loads before the first store; 16 bytes of a row lie somewhere within its 128)
-              uint4 v[8];
+            for (int h = 0; h < DP / 64; ++h) {
+              uint4* values = reinterpret_cast<uint4*>(ring + stage * C::STAGE + h * C::HALF);
+              for (int k = lane; k < first * 8; k += 32) values[k] = make_uint4(0, 0, 0, 0);
+              for (int k = last * 8 + lane; k < KEYS * 8; k += 32) values[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+              for (int k0 = first * 8; k0 < last * 8; k0 += 8 * 32) {
+                uint4 v[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4*>(values + (k0 + k * 32) * 16);
+                for (int k = 0; k < 8; ++k) v[k] = values[min(k0 + k * 32 + lane, last * 8 - 1)];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const int key = (k0 + k * 32) / 8 % KEYS;
-                if (key < first || key >= last) *reinterpret_cast<uint4*>(values + (k0 + k * 32) * 16) = make_uint4(0, 0, 0, 0);
-                else odd = odd || pa_not_finite<T>(v[k].x) || pa_not_finite<T>(v[k].y) || pa_not_finite<T>(v[k].z) || pa_not_finite<T>(v[k].w);
+                for (int k = 0; k < 8; ++k)
+                  largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v[k].x & 0x7FFF7FFFu, v[k].y & 0x7FFF7FFFu), __vmaxu2(v[k].z & 0x7FFF7FFFu, v[k].w & 0x7FFF7FFFu)));
               }
             }
-            odd = __any_sync(0xFFFFFFFFu, odd);
+            const bool odd = __any_sync(0xFFFFFFFFu, pa_not_finite<T>(largest));
             fence_async_smem();
             if (lane == 0) *(volatile int*)&B.odd[n] = odd;
             __syncwarp();

@@ -17,10 +17,12 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .mx4 import _call, _cuda, _dtype, _overlap, _same_device
+from .mx4 import _DTYPES, _call, _cuda, _dtype, _same_device
 
 _RAN_ON: set = set()                # devices whose status word a call may have set
 _INTEGERS = (torch.int32, torch.int64)
+_CACHE_TYPES = {t: _DTYPES[t] for t in (torch.bfloat16, torch.float16)}
+_NONE = (0, 0)                      # strides of what is not there
 
 
 class Rotary:
@@ -118,39 +120,71 @@ def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv
 
 
 def _heads(x, name):
-    """x (tokens, heads, head_dim) with a head's values one behind the other."""
+    """x (tokens, heads, head_dim) with a head's values one behind the other, its strides, and its span: the addresses from its first value to
+    behind its last."""
     _cuda(x, name)
-    if x.dim() != 3:
-        raise ValueError(f"glq_b200: {name} is (tokens, heads, head_dim), got {tuple(x.shape)}")
-    return x if x.stride(2) == 1 or x.shape[2] <= 1 else x.contiguous()
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"glq_b200: {name} is (tokens, heads, head_dim), got {tuple(shape)}")
+    stride = x.stride()
+    if stride[2] != 1 and shape[2] > 1:
+        x = x.contiguous()
+        stride = x.stride()
+    return x, shape, stride, _span(x, shape, stride)
 
 
-def _target(out, like, name):
-    """A given result: the shape, type and device of ``like``, no two values in one place."""
-    _same_device(out, like, name)
-    if out.shape != like.shape or out.dtype != like.dtype:
-        raise ValueError(f"glq_b200: {name} must be {tuple(like.shape)} of {like.dtype}, got {tuple(out.shape)} of {out.dtype}")
-    t, h, d = out.shape
-    (a, m), (b, n) = sorted(((out.stride(0), t), (out.stride(1), h)))
-    if d > 1 and out.stride(2) != 1 or m > 1 and a < d or n > 1 and b < d or m > 1 and n > 1 and b < a * (m - 1) + d:
-        raise ValueError(f"glq_b200: {name} needs a head's values one behind the other and rows that do not overlap, got strides {tuple(out.stride())}")
+def _span(x, shape, stride):
+    first, last = x.data_ptr(), 1
+    for n, s in zip(shape, stride):
+        if n == 0:
+            return first, first
+        last += (n - 1) * s
+    return first, first + last * x.element_size()
 
 
-def _result(x, out, name):
-    """Where the rotated x goes: a new tensor, or ``out``, which is x itself or lies apart from it."""
+def _result(out, x, shape, stride, span, name):
+    """Where a tensor's result goes, its strides and span: a new tensor, or the given ``out``, which has x's shape, type and device, no two
+    values in one place, and is x itself or lies apart from it."""
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _target(out, x, name)
-    if out.numel() and _overlap(x, out) and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+        t, h, d = shape
+        return torch.empty_strided(shape, (h * d, d, 1), dtype=x.dtype, device=x.device), (h * d, d, 1), None
+    _same_device(out, x, name)
+    if out.shape != shape or out.dtype != x.dtype:
+        raise ValueError(f"glq_b200: {name} must be {tuple(shape)} of {x.dtype}, got {tuple(out.shape)} of {out.dtype}")
+    t, h, d = shape
+    own = out.stride()
+    (a, m), (b, n) = sorted(((own[0], t), (own[1], h)))
+    if d > 1 and own[2] != 1 or m > 1 and a < d or n > 1 and b < d or m > 1 and n > 1 and b < a * (m - 1) + d:
+        raise ValueError(f"glq_b200: {name} needs a head's values one behind the other and rows that do not overlap, got strides {own}")
+    at = _span(out, shape, own)
+    if _meet(span, at) and not (span[0] == at[0] and own == stride) and _rows_meet(span, shape, stride, at, shape, own, x):
         raise ValueError(f"glq_b200: {name} overlaps its input without being it")
-    return out
+    return out, own, at
+
+
+def _meet(a, b):
+    """Do two spans have an address in common?"""
+    return a[0] < b[1] and b[0] < a[1]
+
+
+def _rows_meet(a, shape, stride, b, other, own, x):
+    """The same of rows: those of one wider matrix (parts of a merged projection) lie within each other's span and may be apart all the same."""
+    if not _meet(a, b):
+        return False
+    step, size = stride[0], x.element_size()
+    long, wide = ((s[1] - 1) * t[1] + s[2] for s, t in ((shape, stride), (other, own)))
+    if step != own[0] or shape[0] < 2 or long > step or wide > step:
+        return True
+    apart = (b[0] - a[0]) % (step * size)
+    return apart < long * size or apart + wide * size > step * size
 
 
 def _integers(t, x, name, count):
     _same_device(t, x, name)
-    if t.dtype not in _INTEGERS or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
-        raise ValueError(f"glq_b200: {name} must be {count} int32 or int64 values, got {tuple(t.shape)} of {t.dtype}")
-    return t.dtype is torch.int64
+    dtype = t.dtype
+    if dtype not in _INTEGERS or t.shape != (count,) or not t.is_contiguous():
+        raise ValueError(f"glq_b200: {name} must be {count} int32 or int64 values, got {tuple(t.shape)} of {dtype}")
+    return dtype is torch.int64
 
 
 def _check_table(table, x, head_dim):
@@ -166,38 +200,40 @@ def rotary(x, positions, table: Rotary, *, out=None) -> torch.Tensor:
     """x (tokens, heads, head_dim) of bf16, fp16 or fp32 with the first ``table.dim`` values of every head rotated by its token's
     position (int32 or int64, (tokens,); negative ones rotate back), computed in fp32 and rounded once; the other values as they are.
     ``out``: where the result goes, x itself too."""
-    src = _heads(x, "x")
-    dt = _dtype(src.dtype, "x")
-    tokens, heads, dim = src.shape
-    _check_table(table, src, dim)
-    wide = _integers(positions, src, "positions", tokens)
-    out = _result(src, out, "out")
+    x, shape, stride, span = _heads(x, "x")
+    dt = _dtype(x.dtype, "x")
+    tokens, heads, dim = shape
+    _check_table(table, x, dim)
+    wide = _integers(positions, x, "positions", tokens)
+    out, own, _ = _result(out, x, shape, stride, span, "out")
     if tokens and heads:
-        _call(table._index, "rotary", _lib.load().glqb_rotary, table._ref, src.data_ptr(), dt, src.stride(0), src.stride(1), out.data_ptr(),
-              out.stride(0), out.stride(1), tokens, heads, dim, positions.data_ptr(), wide)
+        _call(table._index, "rotary", _lib.load().glqb_rotary, table._ref, span[0], dt, stride[0], stride[1], out.data_ptr(), own[0], own[1], tokens, heads, dim,
+              positions.data_ptr(), wide)
     return out
 
 
 def _cache(keys, values):
-    """The C description of a cache, checked."""
+    """The C description of a cache, checked, its shape, and the spans of its two tensors."""
     _cuda(keys, "key_cache")
     _same_device(values, keys, "value_cache")
-    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype:
+    shape, dtype = keys.shape, keys.dtype
+    if len(shape) != 4 or values.shape != shape or values.dtype != dtype:
         raise ValueError(f"glq_b200: key_cache and value_cache are (pages, page_size, kv_heads, head_dim) of one type, got {tuple(keys.shape)} of {keys.dtype} and "
                          f"{tuple(values.shape)} of {values.dtype}")
-    if keys.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"glq_b200: a cache is bf16 or fp16, not {keys.dtype}")
-    pages, size, heads, dim = keys.shape
+    kind = _CACHE_TYPES.get(dtype)
+    if kind is None:
+        raise ValueError(f"glq_b200: a cache is bf16 or fp16, not {dtype}")
+    pages, size, heads, dim = shape
     if pages < 1 or heads < 1 or dim < 8 or dim > 128 or dim % 8 or size < 8 or size & (size - 1):
-        raise ValueError(f"glq_b200: a cache of {tuple(keys.shape)}: pages of a power of two rows, 8 at least, heads of a multiple of 8 values, 128 at most")
-    strides = []
-    for name, t in (("key_cache", keys), ("value_cache", values)):
-        s = t.stride()
-        if s[3] != 1 or t.data_ptr() & 15 or (s[0] & 7 and pages > 1) or s[1] & 7 or (s[2] & 7 and heads > 1):
+        raise ValueError(f"glq_b200: a cache of {tuple(shape)}: pages of a power of two rows, 8 at least, heads of a multiple of 8 values, 128 at most")
+    ks, vs = keys.stride(), values.stride()
+    kspan, vspan = _span(keys, shape, ks), _span(values, shape, vs)
+    for name, s, at in (("key_cache", ks, kspan), ("value_cache", vs, vspan)):
+        if s[3] != 1 or at[0] & 15 or (s[0] & 7 and pages > 1) or s[1] & 7 or (s[2] & 7 and heads > 1):
             raise ValueError(f"glq_b200: {name} must lie on 16 bytes, strides of 8 values, a head's values one behind the other; got strides {s}")
-        strides.append((s[0] if pages > 1 else 0, s[1], s[2] if heads > 1 else 0))
-    (kp, kr, kh), (vp, vr, vh) = strides
-    return _lib.PagedCacheDesc(keys.data_ptr(), values.data_ptr(), kp, kr, kh, vp, vr, vh, pages, size, heads, dim, _dtype(keys.dtype, "the cache"))
+    desc = _lib.PagedCacheDesc(kspan[0], vspan[0], ks[0] if pages > 1 else 0, ks[1], ks[2] if heads > 1 else 0, vs[0] if pages > 1 else 0, vs[1], vs[2] if heads > 1 else 0, pages,
+                               size, heads, dim, kind)
+    return desc, shape, dtype, kspan, vspan
 
 
 def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, table: Optional[Rotary] = None, query=None, out=None):
@@ -206,44 +242,46 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
     The slots within the cache are all different.  With ``table`` and ``positions`` (tokens,) the keys are rotated on the way, and so is ``query``
     (tokens, heads, head_dim) if it is given: to a new tensor or to ``out`` (the query itself too), which is returned.  Keys, values and
     queries are of the cache's type, or fp32."""
-    desc = _cache(key_cache, value_cache)
-    key, value = _heads(key, "key"), _heads(value, "value")
+    desc, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
+    key, shape, ks, at_key = _heads(key, "key")
+    value, value_shape, vs, at_value = _heads(value, "value")
     _same_device(key, key_cache, "key")
     _same_device(value, key, "value")
-    tokens = key.shape[0]
-    if key.shape != value.shape or key.shape[1:] != key_cache.shape[2:]:
-        raise ValueError(f"glq_b200: keys of {tuple(key.shape)} and values of {tuple(value.shape)} for a cache of {tuple(key_cache.shape)}")
-    if key.dtype != value.dtype or key.dtype not in (key_cache.dtype, torch.float32):
-        raise ValueError(f"glq_b200: keys and values are of the cache's type, {key_cache.dtype}, or fp32, got {key.dtype} and {value.dtype}")
-    slots_wide, positions_wide = _integers(slots, key, "slots", tokens), False
+    tokens, kv_heads, dim = shape
+    if value_shape != shape or kv_heads != cache[2] or dim != cache[3]:
+        raise ValueError(f"glq_b200: keys of {tuple(shape)} and values of {tuple(value_shape)} for a cache of {tuple(cache)}")
+    kind = key.dtype
+    if value.dtype != kind or (kind != dtype and kind != torch.float32):
+        raise ValueError(f"glq_b200: keys and values are of the cache's type, {dtype}, or fp32, got {kind} and {value.dtype}")
+    slots_wide, positions_wide, at_positions, turn = _integers(slots, key, "slots", tokens), False, None, None
     if (table is None) != (positions is None):
         raise ValueError("glq_b200: table and positions come together")
     if table is not None:
-        _check_table(table, key, key.shape[2])
-        positions_wide = _integers(positions, key, "positions", tokens)
+        _check_table(table, key, dim)
+        positions_wide, at_positions, turn = _integers(positions, key, "positions", tokens), positions.data_ptr(), table._ref
+    heads, at_query, at_out, qs, os = 0, None, None, _NONE, _NONE
     if query is None:
         if out is not None:
             raise ValueError("glq_b200: out belongs to query")
     else:
         if table is None:
             raise ValueError("glq_b200: query is here to be rotated: table and positions are needed")
-        query = _heads(query, "query")
+        given = out is not None
+        query, query_shape, qs, at_query = _heads(query, "query")
         _same_device(query, key, "query")
-        if query.shape[0] != tokens or query.shape[2] != key.shape[2] or query.dtype != key.dtype:
-            raise ValueError(f"glq_b200: queries of {tuple(query.shape)}, {query.dtype}, beside keys of {tuple(key.shape)}, {key.dtype}")
-        out = _result(query, out, "out")
-    for name, t in (("key", key), ("value", value), ("query", query), ("out", out)):
-        if t is not None and t.numel() and (_overlap(t, key_cache) or _overlap(t, value_cache)):
+        heads = query_shape[1]
+        if query_shape[0] != tokens or query_shape[2] != dim or query.dtype != kind:
+            raise ValueError(f"glq_b200: queries of {tuple(query_shape)}, {query.dtype}, beside keys of {tuple(shape)}, {kind}")
+        out, os, at_out = _result(out, query, query_shape, qs, at_query, "out")
+        if given and (_rows_meet(at_key, shape, ks, at_out, query_shape, os, key) or _rows_meet(at_value, shape, vs, at_out, query_shape, os, key)):
+            raise ValueError("glq_b200: out overlaps key or value")
+    for name, at in (("key", at_key), ("value", at_value), ("query", at_query), ("out", at_out)):
+        if at is not None and (_meet(at, kspan) or _meet(at, vspan)):
             raise ValueError(f"glq_b200: {name} overlaps the cache")
-    for name, t in (("key", key), ("value", value)):
-        if out is not None and t.numel() and out.numel() and out is not query and _overlap(t, out):
-            raise ValueError(f"glq_b200: out overlaps {name}")
     if tokens:
-        a = _lib.PagedAppendDesc(key.data_ptr(), value.data_ptr(), query.data_ptr() if query is not None else None, out.data_ptr() if out is not None else None,
-                                 key.stride(0), key.stride(1), value.stride(0), value.stride(1), *((query.stride(0), query.stride(1), out.stride(0), out.stride(1)) if query is not None else (0, 0, 0, 0)),
-                                 tokens, slots.data_ptr(), positions.data_ptr() if positions is not None else None, slots_wide, positions_wide, _dtype(key.dtype, "key"),
-                                 query.shape[1] if query is not None else 0)
-        _call(key.get_device(), "paged_append", _lib.load().glqb_paged_append, C.byref(desc), C.byref(a), table._ref if table is not None else None)
+        a = _lib.PagedAppendDesc(at_key[0], at_value[0], at_query[0] if at_query is not None else None, out.data_ptr() if out is not None else None, ks[0], ks[1], vs[0], vs[1], qs[0],
+                                 qs[1], os[0], os[1], tokens, slots.data_ptr(), at_positions, slots_wide, positions_wide, _DTYPES[kind], heads)
+        _call(key.get_device(), "paged_append", _lib.load().glqb_paged_append, C.byref(desc), C.byref(a), turn)
     return out
 
 
@@ -260,20 +298,20 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
     outside the cache reads as zeros.  Rows that see no key are zero.  Rows of no sequence (in front of query_offsets[0], behind the last) are zero in a
     new result and stay as they are in a given ``out``.  Sums and softmax in fp32, weights rounded to the cache's type for the product with the values, as
     is the result; what lies in the cache where no query looks, NaN included, changes nothing.  The same call gives the same bits."""
-    desc = _cache(key_cache, value_cache)
-    query = _heads(query, "query")
+    desc, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
+    query, shape, qs, span = _heads(query, "query")
     _same_device(query, key_cache, "query")
-    tokens, heads, dim = query.shape
-    kv_heads = key_cache.shape[2]
-    if dim != key_cache.shape[3] or query.dtype != key_cache.dtype or heads < 1 or heads % kv_heads:
-        raise ValueError(f"glq_b200: queries of {tuple(query.shape)}, {query.dtype}, over a cache of {tuple(key_cache.shape)}, {key_cache.dtype}")
+    tokens, heads, dim = shape
+    if dim != cache[3] or query.dtype != dtype or heads < 1 or heads % cache[2]:
+        raise ValueError(f"glq_b200: queries of {tuple(shape)}, {query.dtype}, over a cache of {tuple(cache)}, {dtype}")
     _same_device(pages, query, "pages")
-    if pages.dtype != torch.int32 or pages.dim() != 2 or (pages.shape[1] > 1 and pages.stride(1) != 1):
-        raise ValueError(f"glq_b200: pages must be int32 (sequences, columns), a row's entries one behind the other, got {tuple(pages.shape)} of {pages.dtype}")
-    seqs = pages.shape[0]
-    lengths_wide, offsets_wide = _integers(lengths, query, "lengths", seqs), False
+    table = pages.shape
+    if pages.dtype != torch.int32 or len(table) != 2 or (table[1] > 1 and pages.stride(1) != 1):
+        raise ValueError(f"glq_b200: pages must be int32 (sequences, columns), a row's entries one behind the other, got {tuple(table)} of {pages.dtype}")
+    seqs = table[0]
+    lengths_wide, offsets_wide, at_offsets = _integers(lengths, query, "lengths", seqs), False, None
     if query_offsets is not None:
-        offsets_wide = _integers(query_offsets, query, "query_offsets", seqs + 1)
+        offsets_wide, at_offsets = _integers(query_offsets, query, "query_offsets", seqs + 1), query_offsets.data_ptr()
     elif tokens != seqs:
         raise ValueError(f"glq_b200: {tokens} queries of {seqs} sequences need query_offsets")
     if max_query_len is None:
@@ -287,35 +325,31 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
     if not 0 <= window < 2 ** 31:
         raise ValueError(f"glq_b200: a window of {window} keys")
     fresh = out is None
-    if fresh:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    else:
-        _target(out, query, "out")
-        if tokens and (_overlap(out, query) or _overlap(out, key_cache) or _overlap(out, value_cache)):
-            raise ValueError("glq_b200: out overlaps the queries or the cache")
+    out, os, at_out = _result(out, query, shape, qs, span, "out")
+    if not fresh and (_meet(at_out, span) or _meet(at_out, kspan) or _meet(at_out, vspan)):
+        raise ValueError("glq_b200: out overlaps the queries or the cache")
     if tokens:
-        if query.data_ptr() & 15 or query.stride(0) & 7 or query.stride(1) & 7:
+        if span[0] & 15 or qs[0] & 7 or qs[1] & 7:
             query = query.clone(memory_format=torch.contiguous_format)
-        a = _lib.PagedAttentionDesc(query.data_ptr(), out.data_ptr(), query.stride(0), query.stride(1), out.stride(0), out.stride(1), tokens, pages.data_ptr(),
-                                    pages.stride(0), lengths.data_ptr(), query_offsets.data_ptr() if query_offsets is not None else None, lengths_wide,
-                                    offsets_wide, seqs, pages.shape[1], heads, bool(causal), window, fresh and query_offsets is not None, min(max_query_len, tokens), scale)
-        lib, index = _lib.load(), query.get_device()
-        size = _workspace(lib, index, desc, a)
-        ws = query.new_empty((size,), dtype=torch.uint8)
-        _call(index, "paged_attention", lib.glqb_paged_attention, C.byref(desc), C.byref(a), ws.data_ptr(), size)
+            qs = query.stride()
+        a = _lib.PagedAttentionDesc(query.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], tokens, pages.data_ptr(), pages.stride(0), lengths.data_ptr(), at_offsets, lengths_wide,
+                                    offsets_wide, seqs, table[1], heads, bool(causal), window, fresh and at_offsets is not None, min(max_query_len, tokens), scale)
+        lib, index, cache_ref, ref = _lib.load(), query.get_device(), C.byref(desc), C.byref(a)
+        size = _workspace(lib, index, cache_ref, ref)
+        _call(index, "paged_attention", lib.glqb_paged_attention, cache_ref, ref, query.new_empty((size,), dtype=torch.uint8).data_ptr(), size)
         _RAN_ON.add(index)
     return out
 
 
-def _workspace(lib, index, desc, a):
+def _workspace(lib, index, cache, call):
     """Bytes of workspace of a call; 0 from the library is a refusal, which the call itself words."""
     cuda = torch._C
     before = cuda._cuda_getDevice()
     if before == index:
-        return lib.glqb_paged_attention_workspace_bytes(C.byref(desc), C.byref(a))
+        return lib.glqb_paged_attention_workspace_bytes(cache, call)
     cuda._cuda_setDevice(index)
     try:
-        return lib.glqb_paged_attention_workspace_bytes(C.byref(desc), C.byref(a))
+        return lib.glqb_paged_attention_workspace_bytes(cache, call)
     finally:
         cuda._cuda_setDevice(before)
 

@@ -241,6 +241,14 @@ def test_operators_refuse_wrong_arguments(monkeypatch):
     refuses("128 rotated", ops.paged_append, new, new, k, v, n3, positions=n3, table=big)
     refuses("out overlaps key", ops.paged_append, new, torch.zeros_like(new), k, v, n3, positions=n3, table=table, query=torch.zeros_like(new), out=new)
     refuses("overlaps the cache", ops.paged_append, new, k[0, :3], k, v, n3)
+    # parts of a merged projection lie between each other's rows: they may be rotated in place, but not onto one another
+    merged = torch.zeros(3, 8, 64, dtype=bf)
+    q, kk, vv = merged[:, :4], merged[:, 4:6], merged[:, 6:]
+    assert ops.paged_append(kk, vv, k, v, n3, positions=n3, table=table, query=q, out=q) is q and launched.pop() == "paged_append"
+    assert ops.rotary(merged[:, :2], n3, table, out=merged[:, 5:7]) is not None and launched.pop() == "rotary"
+    refuses("out overlaps key", ops.paged_append, merged[:, 3:5], vv, k, v, n3, positions=n3, table=table, query=q, out=q)
+    refuses("out overlaps key", ops.paged_append, kk, merged[:, 1:3], k, v, n3, positions=n3, table=table, query=q, out=q)
+    refuses("without being it", ops.rotary, merged[:, :2], n3, table, out=merged[:, 1:3])
 
     pages = torch.zeros(3, 2, dtype=torch.int32)
     ok = (x, k, v, pages, n3)
