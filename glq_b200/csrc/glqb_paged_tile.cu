@@ -80,6 +80,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                : "memory");
 }
+// the n lowest bits
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 // the largest of three; not a number if one of them is not
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -207,12 +209,14 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
           tmem_ld_wait();
           const bool cut = ragged(key0, all_from, all_to);
           if (cut) {
-            const int lo = from - key0, hi = to - key0;
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < 4; ++n) {
+              // (a bit per key)
+              const uint32_t seen = below(to - key0 - n * 32) & ~below(from - key0 - n * 32);
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (n * 32 + k < lo || n * 32 + k >= hi) s[n][k] = 0xFF800000u;
+                if (!(seen >> k & 1u)) s[n][k] = 0xFF800000u;
+            }
           }
           float top[4];
 #pragma unroll
@@ -321,30 +325,33 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         const float f = it.slot < 0 ? pa_row_factor(J, seq, row, l) : 1.0f;
         const long long at = pa_out_row(J, it.row0, it.kv_head, row), place = (2ll * blockIdx.x + max(it.slot, 0)) * PA_TILE_ROWS + t * 128 + r;
         if (it.slot >= 0 && there) J.part_ml[place] = make_float2(m * c, l);
-#pragma unroll 1
-        for (int n = 0; n < DP / 32; ++n) {
-          uint32_t o[32];
-          tmem_ld32(sums + n * 32u, o);
-          tmem_ld_wait();
-          if (there && it.slot >= 0) {
+        uint32_t o[DP / 32][32];
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) store8(J.part + place * DP + n * 32 + k, o + k);
-          } else if (there) {
+        for (int n = 0; n < DP / 32; ++n) tmem_ld32(sums + n * 32u, o[n]);
+        tmem_ld_wait();
+        if (there && it.slot >= 0) {
+#pragma unroll
+          for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) store8(J.part + place * DP + n * 32 + k, o[n] + k);
+        } else if (there) {
+#pragma unroll
+          for (int n = 0; n < DP / 32; ++n) {
             if (J.out_sectors && n * 32 + 32 <= J.head_dim) {
               uint32_t y[16];
 #pragma unroll
-              for (int k = 0; k < 16; ++k) y[k] = pa_pack<T>(__uint_as_float(o[2 * k]) * f, __uint_as_float(o[2 * k + 1]) * f);
+              for (int k = 0; k < 16; ++k) y[k] = pa_pack<T>(__uint_as_float(o[n][2 * k]) * f, __uint_as_float(o[n][2 * k + 1]) * f);
               store8(reinterpret_cast<uint16_t*>(J.out) + at + n * 32, y);
               store8(reinterpret_cast<uint16_t*>(J.out) + at + n * 32 + 16, y + 8);
             } else {
 #pragma unroll
               for (int k = 0; k < 32; k += 4)
                 if (n * 32 + k < J.head_dim)
-                  pa_store4<T>(J, at, n * 32 + k, make_float4(__uint_as_float(o[k]) * f, __uint_as_float(o[k + 1]) * f, __uint_as_float(o[k + 2]) * f, __uint_as_float(o[k + 3]) * f));
+                  pa_store4<T>(J, at, n * 32 + k, make_float4(__uint_as_float(o[n][k]) * f, __uint_as_float(o[n][k + 1]) * f, __uint_as_float(o[n][k + 2]) * f, __uint_as_float(o[n][k + 3]) * f));
             }
           }
-          __syncwarp();
         }
+        __syncwarp();
         tc_fence_before();
       }
       ok = take(it);
