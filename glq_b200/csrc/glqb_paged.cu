@@ -166,12 +166,13 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
 
 // ---- attention of few rows ------------------------------------------------------------------------
 // Sixteen rows (heads of a group that share a key head, times queries) against tiles of 64 keys: what bounds it is reading the cache.
-// A loading warp brings tiles by TMA into a ring, a page's rows per copy, under the 128-byte swizzle; four warps multiply, each 16
+// Two warps bring tiles of keys and of values by TMA into a ring, a page's rows per copy, under the 128-byte swizzle (a copy takes its warp 80 clocks, a tile of four
+// pages 1300 where one warp brings both); four warps multiply, each 16
 // keys of every tile for itself (mma.sync: with so few rows the tensor cores are idle either way), with a running maximum and sum of its own, and add up when
 // the item ends.  Scores are scale * log2(e) * q k, weights 2^(score - reference): the reference follows the largest score only when
 // that has grown by more than 2^8, which scales all weights of a row alike and leaves their precision as it is.  Weights are rounded to the values'
 // type for the product, as the tensor cores take them; sums stay in fp32.
-constexpr int ST_WARPS = 4, ST_THREADS = (ST_WARPS + 1) * 32, ST_ITEMS = 4;
+constexpr int ST_WARPS = 4, ST_THREADS = (ST_WARPS + 2) * 32, ST_ITEMS = 4;
 template <int DP>
 struct StreamShape {
   static constexpr int HALF = PA_STREAM_KEYS * 128, K_BYTES = HALF * (DP / 64), STAGE = 2 * K_BYTES, STAGES = 96 * 1024 / STAGE;
@@ -208,8 +209,8 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
   StreamShared& B = *reinterpret_cast<StreamShared*>(ring + C::STAGES * C::STAGE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&B.full[s], 1); mbar_init(&B.empty[s], ST_WARPS); }
-    for (int s = 0; s < ST_ITEMS; ++s) { mbar_init(&B.item_full[s], 1); mbar_init(&B.item_empty[s], ST_WARPS); }
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&B.full[s], 2); mbar_init(&B.empty[s], ST_WARPS); }
+    for (int s = 0; s < ST_ITEMS; ++s) { mbar_init(&B.item_full[s], 1); mbar_init(&B.item_empty[s], ST_WARPS + 1); }
     for (int s = 0; s < 2; ++s) mbar_init(&B.joined[s], ST_WARPS);
     B.abort = 0;
     fence_mbar_init();
@@ -220,17 +221,24 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
   pa_start<KEYS>(J, B.start);
   bool ok = true;
 
-  if (warp == ST_WARPS) {
+  if (warp >= ST_WARPS) {
+    // the first of the two makes the list of items, the second one takes it from there, as the others do
+    const bool values = warp > ST_WARPS;
+    const CUtensorMap* map = values ? &map_v : &map_k;
     PagedWalk<KEYS> walk(J, B.start);
     const int piece = min(1 << J.page_log, PA_PIECE), pieces = KEYS / piece, page_mask = (1 << J.page_log) - 1;
-    uint32_t stage = 0, phase = 1, ip = 1, filled = 0;
+    uint32_t stage = 0, phase = 1, ip = values ? 0 : 1, filled = 0;
     int is = 0;
     auto advance = [&] { ++filled; if (++stage == C::STAGES) { stage = 0; phase ^= 1u; } };
     for (;;) {
-      const PagedItem it = walk.next(J);
-      ok = ok && mbar_wait_warp(&B.item_empty[is], ip, &B.abort);
+      PagedItem it;
+      if (!values) it = walk.next(J);
+      ok = ok && mbar_wait_warp(values ? &B.item_full[is] : &B.item_empty[is], ip, &B.abort);
       if (!ok) break;
-      if (lane == 0) { B.item[is] = it; mbar_arrive(&B.item_full[is]); }
+      if (values) it = B.item[is];
+      else if (lane == 0) B.item[is] = it;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(values ? &B.item_empty[is] : &B.item_full[is]);
       if (!it.more) break;
       if (++is == ST_ITEMS) { is = 0; ip ^= 1u; }
       const int* table = J.pages + (long long)it.seq * J.page_stride;
@@ -239,16 +247,13 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
         int page = 0;
         if (lane < here) page = table[(tile * KEYS + lane * piece) >> J.page_log];
         if (!mbar_wait_warp(&B.empty[stage], phase, &B.abort)) { ok = false; break; }
-        uint8_t* at = ring + stage * C::STAGE;
-        if (lane == 0) mbar_expect_tx(&B.full[stage], (uint32_t)(here * piece) * (DP * 4));
+        uint8_t* at = ring + stage * C::STAGE + (values ? C::K_BYTES : 0);
+        if (lane == 0) mbar_expect_tx(&B.full[stage], (uint32_t)(here * piece) * (DP * 2));
         __syncwarp();
         if (lane < here) {
           const int row = (tile * KEYS + lane * piece) & page_mask;
 #pragma unroll
-          for (int h = 0; h < DP / 64; ++h) {
-            pa_load(at + h * C::HALF + lane * piece * 128, &map_k, h * 64, it.kv_head, row, page, &B.full[stage]);
-            pa_load(at + C::K_BYTES + h * C::HALF + lane * piece * 128, &map_v, h * 64, it.kv_head, row, page, &B.full[stage]);
-          }
+          for (int h = 0; h < DP / 64; ++h) pa_load(at + h * C::HALF + lane * piece * 128, map, h * 64, it.kv_head, row, page, &B.full[stage]);
         }
         __syncwarp();
         advance();
@@ -261,9 +266,9 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
     }
     if (lane == 0) {
       if (!ok) { *(volatile int*)&B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
-      pa_publish(J, walk.part);
+      if (!values) pa_publish(J, walk.part);
     }
-    // copies in flight land before the block ends
+    // copies in flight land before the block ends (a stage that the other of the two did not fill does not: the wait is bounded)
     if (!ok)
       for (uint32_t n = 1; n <= min(filled, (uint32_t)C::STAGES); ++n) mbar_wait(&B.full[(filled - n) % C::STAGES], (filled - n) / C::STAGES & 1u);
   } else {
@@ -484,7 +489,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
 // The parts of an item that CTA blockIdx.x began and did not end are that CTA's, then those of the CTAs behind it up to the one that ended
 // the item.  Of few rows (MANY false) a block has all: a row is several warps', each every n-th part, then together.  Of many rows there are few
 // parts: a block has 32 rows, a warp four of them at once.  The order is the same in every call.
-constexpr int CB_WARPS = 8, CB_ROWS = 32;
+constexpr int CB_ROWS = 32;
 struct Joined {
   float4 v;
   float most, sum;
@@ -506,10 +511,12 @@ struct Joined {
     }
   }
 };
+template <bool MANY> constexpr int CB_WARPS = MANY ? 8 : 16;
 template <typename T, int DP, bool MANY>
-__global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
-  __shared__ float4 sums[CB_WARPS][DP / 4];
-  __shared__ float2 mls[CB_WARPS];
+__global__ void __launch_bounds__(CB_WARPS<MANY> * 32) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
+  constexpr int WARPS = CB_WARPS<MANY>;
+  __shared__ float4 sums[WARPS][DP / 4];
+  __shared__ float2 mls[WARPS];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, col = lane * 4;
@@ -525,7 +532,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
     const int first = pa_offset(J, 0), last = max(first, pa_offset(J, J.seqs)), rest = J.tokens - (last - first);
     for (int i = c; i < rest; i += gridDim.x) {
       T* p = reinterpret_cast<T*>(J.out) + (long long)(i < first ? i : i + last - first) * J.out_token;
-      for (int k = threadIdx.x; k < J.heads * J.head_dim; k += CB_WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
+      for (int k = threadIdx.x; k < J.heads * J.head_dim; k += WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
     }
   }
   if (!lead.valid) return;
@@ -550,7 +557,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int k = 0; k < CB_BATCH; ++k) {
-          const int row = row0 + n * CB_WARPS;
+          const int row = row0 + n * WARPS;
           ml[n][k] = make_float2(-INFINITY, 0.0f);
           u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           if (p0 + k < parts && row < lead.rows) {
@@ -564,15 +571,14 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      if (row0 + n * CB_WARPS < lead.rows) store(row0 + n * CB_WARPS, j[n]);
+      if (row0 + n * WARPS < lead.rows) store(row0 + n * WARPS, j[n]);
   } else {
-    const int row0 = blockIdx.y * CB_WARPS, rows = min(CB_WARPS, lead.rows - row0);
-    if (rows <= 0) return;
+    const int rows = min(WARPS, lead.rows);                // (an item has 16 at most)
     int wide = 1;
     while (wide < rows) wide <<= 1;
-    const int groups = CB_WARPS / wide, row = row0 + warp % wide, group = warp / wide;
+    const int groups = WARPS / wide, row = warp % wide, group = warp / wide;
     Joined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-    if (row - row0 < rows)
+    if (row < rows)
       for (int p0 = group; p0 < parts; p0 += CB_BATCH * groups) {
         float2 ml[CB_BATCH];
         float4 u[CB_BATCH];
@@ -607,7 +613,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
         j.add(ml, u);
       }
     }
-    if (row - row0 < rows) store(row, j);
+    if (row < rows) store(row, j);
   }
 }
 
@@ -767,15 +773,14 @@ int check_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a) {
 template <typename T, int DP>
 cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   using C = StreamShape<DP>;
-  const int most_rows = PA_STREAM_ROWS;
   constexpr auto K = paged_stream_kernel<T, DP>;
   const cudaError_t e = f.tile ? paged_tile_launch(J, __is_same(T, __nv_bfloat16), mq, mk, mv, f.ctas, stream)
                                : paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
   if (e != cudaSuccess) return e;
   constexpr auto FEW = paged_combine_kernel<T, DP, false>;
   constexpr auto MANY = paged_combine_kernel<T, DP, true>;
-  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS * 32, 0, stream, J, f.ctas)
-                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas, (unsigned)((std::min(PA_STREAM_ROWS, most_rows) + CB_WARPS - 1) / CB_WARPS)), CB_WARPS * 32, 0, stream, J, f.ctas);
+  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS<true> * 32, 0, stream, J, f.ctas)
+                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas), CB_WARPS<false> * 32, 0, stream, J, f.ctas);
 }
 }  // namespace
 }  // namespace glqb

@@ -82,56 +82,85 @@ __device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq&
 // Where a CTA's share of the work begins: item (seq, kv_head, q_tile), `skip` units into it, `units` units in all.
 struct PagedStart {
   PagedSeq s;
-  int seq, kv_head, q_tile, skip;
+  int seq, kv_head, q_tile, skip, q_tiles;
+  int2 tiles;                        // the item's
   long long units;
   long long warp_sum[32];
 };
+// quotient of numbers >= 0 (a division of 64 bits takes some hundred clocks)
+__device__ __forceinline__ long long pa_div(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
+// The item that unit r of a sequence's belongs to.
+template <int KEYS>
+__device__ __forceinline__ void pa_place_start(const PagedJob& J, PagedStart& S, int seq, const PagedSeq& s, long long per_head, long long r, long long units) {
+  S.s = s;
+  S.seq = seq;
+  S.kv_head = (int)pa_div(r, per_head);
+  r -= S.kv_head * per_head;
+  int qt = 0;
+  int2 t;
+  for (;; ++qt) {
+    t = pa_tiles<KEYS>(J, s, qt);
+    if (r < t.y - t.x + J.begin) break;
+    r -= t.y - t.x + J.begin;
+  }
+  S.q_tile = qt;
+  S.q_tiles = pa_q_tiles(J, s);
+  S.tiles = t;
+  S.skip = (int)r;
+  S.units = units;
+}
 // The work is one list of units: sequence after sequence, of each one key head after another, of each one row tile after another, of each such item
 // J.begin units for its beginning and one per key tile; every CTA takes an equal run of it.  So batches of any lengths keep all SMs busy, and an item is cut only where a run ends.  Every
-// CTA counts the list itself: a thread some sequences, then a scan.  Called by all threads; ends with a block barrier.
+// CTA counts the list itself: a thread some sequences, then a scan; up to 32 sequences are one warp's.  Called by all threads; ends with a block barrier.
 template <int KEYS>
 __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
   const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (J.seqs + threads - 1) / threads, first = min(J.seqs, (int)threadIdx.x * per), last = min(J.seqs, first + per);
-  long long own = 0;
-  for (int i = first; i < last; ++i) own += pa_units<KEYS>(J, pa_seq(J, i)) * J.kv_heads;
+  const bool small = J.seqs <= 32;
+  if (threadIdx.x == 0) S.units = 0;
+  if (small && warp > 0) {
+    __syncthreads();
+    return;
+  }
+  const int per = small ? 1 : (J.seqs + threads - 1) / threads, first = min(J.seqs, (int)threadIdx.x * per), last = min(J.seqs, first + per);
+  PagedSeq s{0, 0, 0};
+  long long own = 0, per_head = 0;
+  for (int i = first; i < last; ++i) {
+    s = pa_seq(J, i);
+    per_head = pa_units<KEYS>(J, s);
+    own += per_head * J.kv_heads;
+  }
   long long sum = own;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const long long u = __shfl_up_sync(0xFFFFFFFFu, sum, d);
     if (lane >= d) sum += u;
   }
-  if (lane == 31) S.warp_sum[warp] = sum;
-  if (threadIdx.x == 0) S.units = 0;
-  __syncthreads();
   long long before = sum - own, total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += S.warp_sum[w];
-    total += S.warp_sum[w];
+  if (small) {
+    total = __shfl_sync(0xFFFFFFFFu, sum, 31);
+  } else {
+    if (lane == 31) S.warp_sum[warp] = sum;
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) before += S.warp_sum[w];
+      total += S.warp_sum[w];
+    }
   }
-  const long long ctas = min((long long)gridDim.x, (total + J.min_units - 1) / J.min_units);
+  const long long ctas = min((long long)gridDim.x, pa_div(total + J.min_units - 1, J.min_units));
   if ((long long)blockIdx.x < ctas) {
-    const long long begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+    const long long begin = pa_div(total * blockIdx.x, ctas), end = pa_div(total * (blockIdx.x + 1), ctas);
     if (begin >= before && begin < before + own) {
       long long r = begin - before;
-      for (int i = first; i < last; ++i) {
-        const PagedSeq s = pa_seq(J, i);
-        const long long per_head = pa_units<KEYS>(J, s);
-        if (r >= per_head * J.kv_heads) { r -= per_head * J.kv_heads; continue; }
-        S.s = s;
-        S.seq = i;
-        S.kv_head = (int)(r / per_head);
-        r -= S.kv_head * per_head;
-        int qt = 0;
-        for (;; ++qt) {
-          const int2 t = pa_tiles<KEYS>(J, s, qt);
-          if (r < t.y - t.x + J.begin) break;
-          r -= t.y - t.x + J.begin;
+      if (per == 1) {
+        pa_place_start<KEYS>(J, S, first, s, per_head, r, end - begin);
+      } else {
+        for (int i = first; i < last; ++i) {
+          s = pa_seq(J, i);
+          per_head = pa_units<KEYS>(J, s);
+          if (r >= per_head * J.kv_heads) { r -= per_head * J.kv_heads; continue; }
+          pa_place_start<KEYS>(J, S, i, s, per_head, r, end - begin);
+          break;
         }
-        S.q_tile = qt;
-        S.skip = (int)r;
-        S.units = end - begin;
-        break;
       }
     }
   }
@@ -151,17 +180,16 @@ template <int KEYS>
 struct PagedWalk {
   PagedSeq s;
   int seq, kv_head, qt, skip, q_tiles;
+  int2 t;                            // the item's key tiles
   long long left;
   PagedPart part[2];                 // what the CTA leaves in the workspace
   __device__ __forceinline__ PagedWalk(const PagedJob& J, const PagedStart& S)
-      : s(S.s), seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(0), left(S.units) {
+      : s(S.s), seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(S.q_tiles), t(S.tiles), left(S.units) {
     part[0] = part[1] = PagedPart{0, 1, 0, 0, 0, 0, 0, 0};
-    if (left > 0) q_tiles = pa_q_tiles(J, s);
   }
   __device__ __forceinline__ PagedItem next(const PagedJob& J) {
     PagedItem it{};
     while (left > 0 && !it.more) {
-      const int2 t = pa_tiles<KEYS>(J, s, qt);
       const int n = t.y - t.x, take = (int)min((long long)(n + J.begin - skip), left);
       const int from = max(0, skip - J.begin), to = max(0, skip + take - J.begin);
       if (from < to) {                   // (a run that ends before the first tile leaves the item to the next CTA)
@@ -190,6 +218,7 @@ struct PagedWalk {
           }
         }
       }
+      if (left > 0) t = pa_tiles<KEYS>(J, s, qt);
     }
     return it;
   }
