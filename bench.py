@@ -510,12 +510,12 @@ def run_moe_bench(name, D: Dist, args, steps, tokens=None):
 # --------------------------------------------------------------------------------------------------
 # dependent chain through the operator layer, and the latency of one linear
 # --------------------------------------------------------------------------------------------------
-def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False):
+def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False, context=0):
     """Batch-1 decode where every projection consumes the previous output, through glq_b200.ops (the calls a
     drop-in user makes), captured in one CUDA graph: per layer  qkv(h) -> o(attention stand-in) -> residual ->
     gate/up(h) -> silu(gate) * up -> down -> residual.  SmolLM3-3B shapes, trellis 4 bpw.  The attention itself
-    is replaced by a shape-correct stand-in (the first 2048 of the qkv outputs), the metric counts the linears'
-    compressed bytes.  Tensor parallel ranks all-reduce after o and down (fp32), as a served model does."""
+    is replaced by a shape-correct stand-in (the first 2048 of the qkv outputs), or, with `context` keys, computed: rotary
+    positions, append to a paged cache and attention over it.  The metric counts the linears' compressed bytes.  Tensor parallel ranks all-reduce after o and down (fp32), as a served model does."""
     import torch
     import torch.distributed as dist
     from glq_b200 import ops, synth, tp
@@ -555,6 +555,23 @@ def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False):
     ei = torch.empty(0, dtype=torch.int16, device=dev)
     eh = torch.empty(0, dtype=torch.float16, device=dev)
 
+    if context:
+        # a cache of the layer's own per layer, its pages in any order; the new token is the last of `context`
+        head_dim, page_size = 128, 16
+        heads, kv_heads = shapes["q"][0] // head_dim, shapes["k"][0] // head_dim
+        n_pages = -(-context // page_size)
+        caches = [[torch.randn(n_pages, page_size, kv_heads, head_dim, device=dev, generator=gen).to(torch.bfloat16) for _ in range(2)] for _ in Ls]
+        pages = torch.randperm(n_pages, device=dev, generator=gen).to(torch.int32)[None]
+        position = torch.tensor([context - 1], device=dev)
+        slot = pages[0, (context - 1) // page_size].long().reshape(1) * page_size + (context - 1) % page_size
+        lengths = torch.tensor([context], device=dev)
+        rotary = ops.rotary_table(head_dim, base=500000.0, device=dev)
+
+    def attend(qkv, cache):
+        q, k, v = (t.view(1, -1, head_dim) for t in qkv.split([heads * head_dim, kv_heads * head_dim, kv_heads * head_dim], 1))
+        q = ops.paged_append(k, v, *cache, slot, positions=position, table=rotary, query=q)
+        return ops.paged_attention(q, *cache, pages, lengths).view(1, -1)
+
     def lin(L, x, **kw):
         if e8:
             tail = []
@@ -574,9 +591,12 @@ def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False):
 
     def forward(h0_):
         h = h0_.clone()
-        for d, w1, w2 in zip(Ls, norm1, norm2):
+        for i, (d, w1, w2) in enumerate(zip(Ls, norm1, norm2)):
             qkv = shards(h, (d["q"], d["k"], d["v"]), w1)             # RMSNorm + q/k/v: one launch
-            a = qkv[:, :d["q"].m]                                     # attention stand-in: a view, (1, 2048 / world)
+            if context:
+                a = attend(qkv, caches[i])                            # rotation + append: one launch; attention: two
+            else:
+                a = qkv[:, :d["q"].m]                                 # attention stand-in: a view, (1, 2048 / world)
             if world == 1:
                 lin(d["o"], a, accumulate_into=h)                     # o projection + residual add: one launch
             elif comm is not None:
@@ -620,14 +640,15 @@ def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False):
     hbm, tens, kind = measured_peaks()
     total_bytes = D.sum_int(code_bytes)[0]
     gbs = total_bytes / (ms * 1e-3) / 1e9
-    glq_launches = sum(p.launches for p in ops._PLAN_CACHE.values() if hasattr(p, "launches"))
+    glq_launches = sum(p.launches for p in ops._PLAN_CACHE.values() if hasattr(p, "launches")) + (3 * n_layers if context else 0)
     model = ("decoder layers of the 62-layer dense shape (hidden 5376, intermediate 21504), E8 shell 2 / 3 / 3 stages" if dense62 else
              "Llama-3-8B decoder layers, E8 shell two-stage (4 bpw)" if e8 else "SmolLM3-3B decoder layers, trellis 4 bpw")
     rec = {"workload": "decode_chain_62l" if dense62 else "decode_chain_e8" if e8 else "decode_chain", "metric": METRIC, "value": gbs, "unit": "GB/s", "ms_per_step": ms, "n_gpus": world,
            "us_per_layer": ms * 1e3 / n_layers, "us_per_linear": ms * 1e3 / (7 * n_layers),
            "config": f"{n_layers} {model}, batch 1, every projection consumes the previous "
                      f"output through glq_b200.ops: per layer RMSNorm + q/k/v, o + residual, RMSNorm + gate/up, "
-                     f"silu(gate) * up + down + residual as four calls (attention replaced by a view of the q output; "
+                     f"silu(gate) * up + down + residual as four calls ("
+                     f"{f'rotary positions, append to a paged cache and attention over {context} keys as two' if context else 'attention replaced by a view of the q output'}; "
                      f"{'one CUDA graph' if graph is not None else 'eager launches'}); "
                      f"{total_bytes / 1e6:.0f} MB of codes per step, larger than L2"
                      + ((f"; tp{world}: o and down summed over the ranks inside their decode kernels (glq_b200.comm)" if comm is not None
@@ -635,6 +656,7 @@ def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False):
            "e2e": {"value": total_bytes / (ms_e2e * 1e-3) / 1e9, "unit": "GB/s", "h2d_bytes_per_step": h0.numel() * 2,
                    "d2h_bytes_per_step": out.numel() * 2},
            "gpu_launches": glq_launches * steps, "glq_launches_per_layer": glq_launches / n_layers,
+           **({"context": context, "kv_bytes_per_step": 2 * n_layers * context * kv_heads * head_dim * 2} if context else {}),
            "roofline": {"bound": "hbm", "kernel": ("whole chain: e8_fused_kernel for the launches of up to 16 MB of indices, rht_in + e8_mv(_smem)_kernel + rht_out above" if e8 else
                                                   "whole chain: 4 trellis_fused_kernel<4,0> launches (+ 1 rht_in_kernel for down) per layer")
                                                  + " for its 7 linears, norms, activation and residual adds",
@@ -858,6 +880,8 @@ def main():
     ap.add_argument("--tokens", type=int, default=None)
     ap.add_argument("--layers", type=int, default=None,
                     help="decoder layers to build (default: per workload); smaller values are for profiler captures only")
+    ap.add_argument("--context", type=int, default=0,
+                    help="decode_chain workloads: keys of the sequence; attention over a paged cache of them in place of the stand-in")
     args = ap.parse_args()
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
@@ -886,7 +910,8 @@ def main():
         if kind == "chain":
             dense62 = name == "decode_chain_62l"
             e8 = name == "decode_chain_e8" or dense62
-            return run_chain_bench(D, args, n_steps, layers or (62 if dense62 else 32 if e8 else 36), e8=e8, dense62=dense62)
+            return run_chain_bench(D, args, n_steps, layers or (62 if dense62 else 32 if e8 else 36), e8=e8, dense62=dense62,
+                                   context=args.context if args.workload.startswith("decode_chain") else 0)
         return run_linear_latency(D, args)
 
     if args.workload != "decode_trellis_sweep":

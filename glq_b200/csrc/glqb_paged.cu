@@ -41,6 +41,18 @@ template <typename T> struct Eight;                      // eight values as they
 template <> struct Eight<float> { float4 a, b; };
 template <> struct Eight<__half> { uint4 a; };
 template <> struct Eight<__nv_bfloat16> { uint4 a; };
+// (read once: the first to leave L2, where what is written should stay.  4096 tokens appended: 27.7 us, 24.6 so)
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p) {
+  Eight<T> e;
+  if constexpr (__is_same(T, float)) {
+    e.a = __ldcs(reinterpret_cast<const float4*>(p));
+    e.b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  } else {
+    e.a = __ldcs(reinterpret_cast<const uint4*>(p));
+  }
+  return e;
+}
 template <typename T>
 __device__ __forceinline__ void to_floats(const Eight<T>& e, float (&v)[8]) {
   if constexpr (__is_same(T, float)) {
@@ -66,10 +78,10 @@ __device__ __forceinline__ Eight<T> from_floats(const float (&v)[8]) {
   }
   return e;
 }
-__device__ __forceinline__ void rotate_neighbours(float (&v)[8], const float2* cs) {
+__device__ __forceinline__ void rotate_neighbours(float (&v)[8], const float2* cs, int step) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    const float2 f = cs[j / 2];
+    const float2 f = cs[j / 2 * step];
     const float a = v[j];
     v[j] = a * f.x - v[j + 1] * f.y;
     v[j + 1] = v[j + 1] * f.x + a * f.y;
@@ -79,20 +91,23 @@ __device__ __forceinline__ void rotate_neighbours(float (&v)[8], const float2* c
 // TI: queries, keys and values as they come; TC: the cache's type (queries keep theirs).  WIDE: all pieces are whole and lie on 16 bytes.
 template <typename TI, typename TC, bool WIDE>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid_constant__ RotJob J) {
-  extern __shared__ float2 turn_of[];                    // [token][pair]: cosine and sine
+  // Cosine and sine by token and pair; of WIDE units pairs p, p + 8, .. lie one behind the other, so that the units of neighbouring lanes are in
+  // different banks (8191 tokens x 40 heads: 34 us in the order of the pairs, 30 so).
+  extern __shared__ float2 turn_of[];
   __shared__ long long row_of[ROT_TOKENS];                      // row of the cache of each token, -1: none
   pdl_wait();
   pdl_trigger();
   const int block = blockIdx.x / J.head_blocks, head0 = (blockIdx.x % J.head_blocks) * J.block_heads;
   const long long token0 = (long long)block * J.per_block;
   const int n = (int)min((long long)J.per_block, J.tokens - token0), heads = min(J.block_heads, J.heads - head0);
+  const int eighths = (J.pairs + 7) / 8, sines = WIDE ? eighths * 8 : J.pairs;
   for (int i = threadIdx.x; i < n * J.pairs; i += ROT_THREADS) {
     const int t = i / J.pairs, p = i - t * J.pairs;
     const long long pos = J.positions_wide ? reinterpret_cast<const long long*>(J.positions)[token0 + t] : reinterpret_cast<const int*>(J.positions)[token0 + t];
     // the fraction of a turn, as a signed 64-bit number: whole turns are what the product loses
     float s, c;
     sincospif((float)(long long)((unsigned long long)pos * J.turns[p]) * 0x1p-63f, &s, &c);
-    turn_of[i] = make_float2(c * J.scale, s * J.scale);
+    turn_of[t * sines + (WIDE ? (p & 7) * eighths + (p >> 3) : p)] = make_float2(c * J.scale, s * J.scale);
   }
   if (J.slots && threadIdx.x < n) {
     const long long s = J.slots_wide ? reinterpret_cast<const long long*>(J.slots)[token0 + threadIdx.x] : reinterpret_cast<const int*>(J.slots)[token0 + threadIdx.x];
@@ -116,7 +131,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
     } else {
       at = (token0 + t) * P.dst_token + h * P.dst_head;
     }
-    const float2* cs = turn_of + t * J.pairs;
+    const float2* cs = turn_of + t * sines;
     auto run = [&](auto type) {
       using TO = decltype(type);
       TO* dst = reinterpret_cast<TO*>(P.dst) + at;
@@ -125,20 +140,20 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
         const int first = apart ? u * 8 : u * 16, second = apart ? first + J.pairs : first + 8;
         const bool two = second < J.head_dim;
         float x[8], y[8];
-        const Eight<TI> ex = *reinterpret_cast<const Eight<TI>*>(src + first), ey = two ? *reinterpret_cast<const Eight<TI>*>(src + second) : Eight<TI>{};
+        const Eight<TI> ex = load_eight(src + first), ey = two ? load_eight(src + second) : Eight<TI>{};
         to_floats<TI>(ex, x);
         to_floats<TI>(ey, y);
         if (apart) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float2 f = cs[first + j];
+            const float2 f = cs[j * eighths + u];
             const float v = x[j];
             x[j] = v * f.x - y[j] * f.y;
             y[j] = y[j] * f.x + v * f.y;
           }
         } else if (P.turn && J.interleaved) {
-          if (first < 2 * J.pairs) rotate_neighbours(x, cs + first / 2);
-          if (second < 2 * J.pairs) rotate_neighbours(y, cs + second / 2);
+          if (first < 2 * J.pairs) rotate_neighbours(x, cs + u, eighths);
+          if (second < 2 * J.pairs) rotate_neighbours(y, cs + 4 * eighths + u, eighths);
         }
         *reinterpret_cast<Eight<TO>*>(dst + first) = from_floats<TO>(x);
         if (two) *reinterpret_cast<Eight<TO>*>(dst + second) = from_floats<TO>(y);
@@ -681,7 +696,7 @@ int rotary_launch(RotJob& J, int sms, cudaStream_t stream, const char* what) {
   J.head_mul = mul(J.block_heads);
   const long long grid = (J.tokens + J.per_block - 1) / J.per_block * J.head_blocks;
   if (grid > INT_MAX) return pg_fail(GLQB_E_INVALID, "%s: %lld tokens of %d heads are too many for one call", what, J.tokens, J.heads);
-  const size_t smem = (size_t)J.per_block * J.pairs * sizeof(float2);
+  const size_t smem = (size_t)J.per_block * ((J.pairs + 7) / 8 * 8) * sizeof(float2);
   return pg_launched(what, wide ? launch_chained(true, rotary_append_kernel<TI, TC, true>, (int)grid, ROT_THREADS, smem, stream, J)
                                 : launch_chained(true, rotary_append_kernel<TI, TC, false>, (int)grid, ROT_THREADS, smem, stream, J));
 }

@@ -119,10 +119,13 @@ def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv
     return Rotary(turns.to(device), own if scale is None else scale, interleaved)
 
 
-def _heads(x, name):
-    """x (tokens, heads, head_dim) with a head's values one behind the other, its strides, and its span: the addresses from its first value to
-    behind its last."""
-    _cuda(x, name)
+def _heads(x, name, index=None):
+    """x (tokens, heads, head_dim) with a head's values one behind the other, its shape, strides and span: the addresses from its first value to
+    behind its last.  On the device ``index`` if that is given."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        _cuda(x, name)
+    if index is not None and x.get_device() != index:
+        raise ValueError(f"glq_b200: {name} is on {x.device}, expected cuda:{index}")
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"glq_b200: {name} is (tokens, heads, head_dim), got {tuple(shape)}")
@@ -134,12 +137,13 @@ def _heads(x, name):
 
 
 def _span(x, shape, stride):
-    first, last = x.data_ptr(), 1
+    first = x.data_ptr()
+    if 0 in shape:
+        return first, first
+    last = 1
     for n, s in zip(shape, stride):
-        if n == 0:
-            return first, first
         last += (n - 1) * s
-    return first, first + last * x.element_size()
+    return first, first + last * x.itemsize
 
 
 def _result(out, x, shape, stride, span, name):
@@ -147,7 +151,8 @@ def _result(out, x, shape, stride, span, name):
     values in one place, and is x itself or lies apart from it."""
     if out is None:
         t, h, d = shape
-        return torch.empty_strided(shape, (h * d, d, 1), dtype=x.dtype, device=x.device), (h * d, d, 1), None
+        stride = (h * d, d, 1)
+        return torch.empty_strided(shape, stride, dtype=x.dtype, device=x.device), stride, None
     _same_device(out, x, name)
     if out.shape != shape or out.dtype != x.dtype:
         raise ValueError(f"glq_b200: {name} must be {tuple(shape)} of {x.dtype}, got {tuple(out.shape)} of {out.dtype}")
@@ -171,7 +176,7 @@ def _rows_meet(a, shape, stride, b, other, own, x):
     """The same of rows: those of one wider matrix (parts of a merged projection) lie within each other's span and may be apart all the same."""
     if not _meet(a, b):
         return False
-    step, size = stride[0], x.element_size()
+    step, size = stride[0], x.itemsize
     long, wide = ((s[1] - 1) * t[1] + s[2] for s, t in ((shape, stride), (other, own)))
     if step != own[0] or shape[0] < 2 or long > step or wide > step:
         return True
@@ -179,8 +184,12 @@ def _rows_meet(a, shape, stride, b, other, own, x):
     return apart < long * size or apart + wide * size > step * size
 
 
-def _integers(t, x, name, count):
-    _same_device(t, x, name)
+def _integers(t, index, name, count):
+    """Are they int64 (else int32)?"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _cuda(t, name)
+    if t.get_device() != index:
+        raise ValueError(f"glq_b200: {name} is on {t.device}, expected cuda:{index}")
     dtype = t.dtype
     if dtype not in _INTEGERS or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"glq_b200: {name} must be {count} int32 or int64 values, got {tuple(t.shape)} of {dtype}")
@@ -204,7 +213,7 @@ def rotary(x, positions, table: Rotary, *, out=None) -> torch.Tensor:
     dt = _dtype(x.dtype, "x")
     tokens, heads, dim = shape
     _check_table(table, x, dim)
-    wide = _integers(positions, x, "positions", tokens)
+    wide = _integers(positions, table._index, "positions", tokens)
     out, own, _ = _result(out, x, shape, stride, span, "out")
     if tokens and heads:
         _call(table._index, "rotary", _lib.load().glqb_rotary, table._ref, span[0], dt, stride[0], stride[1], out.data_ptr(), own[0], own[1], tokens, heads, dim,
@@ -226,14 +235,18 @@ def _cache(keys, values):
     pages, size, heads, dim = shape
     if pages < 1 or heads < 1 or dim < 8 or dim > 128 or dim % 8 or size < 8 or size & (size - 1):
         raise ValueError(f"glq_b200: a cache of {tuple(shape)}: pages of a power of two rows, 8 at least, heads of a multiple of 8 values, 128 at most")
-    ks, vs = keys.stride(), values.stride()
-    kspan, vspan = _span(keys, shape, ks), _span(values, shape, vs)
-    for name, s, at in (("key_cache", ks, kspan), ("value_cache", vs, vspan)):
-        if s[3] != 1 or at[0] & 15 or (s[0] & 7 and pages > 1) or s[1] & 7 or (s[2] & 7 and heads > 1):
-            raise ValueError(f"glq_b200: {name} must lie on 16 bytes, strides of 8 values, a head's values one behind the other; got strides {s}")
-    desc = _lib.PagedCacheDesc(kspan[0], vspan[0], ks[0] if pages > 1 else 0, ks[1], ks[2] if heads > 1 else 0, vs[0] if pages > 1 else 0, vs[1], vs[2] if heads > 1 else 0, pages,
-                               size, heads, dim, kind)
-    return desc, shape, dtype, kspan, vspan
+    (kp, kr, kh, kd), (vp, vr, vh, vd) = keys.stride(), values.stride()
+    if pages == 1:
+        kp = vp = 0
+    if heads == 1:
+        kh = vh = 0
+    first, other = keys.data_ptr(), values.data_ptr()
+    if kd != 1 or vd != 1 or (first | other) & 15 or (kp | kr | kh | vp | vr | vh) & 7:
+        raise ValueError(f"glq_b200: key_cache and value_cache must lie on 16 bytes, strides of 8 values, a head's values one behind the other; got strides {keys.stride()} and "
+                         f"{values.stride()}")
+    desc = _lib.PagedCacheDesc(first, other, kp, kr, kh, vp, vr, vh, pages, size, heads, dim, kind)
+    pages, size, heads = pages - 1, size - 1, heads - 1
+    return (desc, shape, dtype, (first, first + 2 * (pages * kp + size * kr + heads * kh + dim)), (other, other + 2 * (pages * vp + size * vr + heads * vh + dim)))
 
 
 def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, table: Optional[Rotary] = None, query=None, out=None):
@@ -243,22 +256,21 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
     (tokens, heads, head_dim) if it is given: to a new tensor or to ``out`` (the query itself too), which is returned.  Keys, values and
     queries are of the cache's type, or fp32."""
     desc, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
-    key, shape, ks, at_key = _heads(key, "key")
-    value, value_shape, vs, at_value = _heads(value, "value")
-    _same_device(key, key_cache, "key")
-    _same_device(value, key, "value")
+    index = key_cache.get_device()
+    key, shape, ks, at_key = _heads(key, "key", index)
+    value, value_shape, vs, at_value = _heads(value, "value", index)
     tokens, kv_heads, dim = shape
     if value_shape != shape or kv_heads != cache[2] or dim != cache[3]:
         raise ValueError(f"glq_b200: keys of {tuple(shape)} and values of {tuple(value_shape)} for a cache of {tuple(cache)}")
     kind = key.dtype
     if value.dtype != kind or (kind != dtype and kind != torch.float32):
         raise ValueError(f"glq_b200: keys and values are of the cache's type, {dtype}, or fp32, got {kind} and {value.dtype}")
-    slots_wide, positions_wide, at_positions, turn = _integers(slots, key, "slots", tokens), False, None, None
+    slots_wide, positions_wide, at_positions, turn = _integers(slots, index, "slots", tokens), False, None, None
     if (table is None) != (positions is None):
         raise ValueError("glq_b200: table and positions come together")
     if table is not None:
         _check_table(table, key, dim)
-        positions_wide, at_positions, turn = _integers(positions, key, "positions", tokens), positions.data_ptr(), table._ref
+        positions_wide, at_positions, turn = _integers(positions, index, "positions", tokens), positions.data_ptr(), table._ref
     heads, at_query, at_out, qs, os = 0, None, None, _NONE, _NONE
     if query is None:
         if out is not None:
@@ -267,8 +279,7 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
         if table is None:
             raise ValueError("glq_b200: query is here to be rotated: table and positions are needed")
         given = out is not None
-        query, query_shape, qs, at_query = _heads(query, "query")
-        _same_device(query, key, "query")
+        query, query_shape, qs, at_query = _heads(query, "query", index)
         heads = query_shape[1]
         if query_shape[0] != tokens or query_shape[2] != dim or query.dtype != kind:
             raise ValueError(f"glq_b200: queries of {tuple(query_shape)}, {query.dtype}, beside keys of {tuple(shape)}, {kind}")
@@ -276,12 +287,12 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
         if given and (_rows_meet(at_key, shape, ks, at_out, query_shape, os, key) or _rows_meet(at_value, shape, vs, at_out, query_shape, os, key)):
             raise ValueError("glq_b200: out overlaps key or value")
     for name, at in (("key", at_key), ("value", at_value), ("query", at_query), ("out", at_out)):
-        if at is not None and (_meet(at, kspan) or _meet(at, vspan)):
+        if at is not None and (at[0] < kspan[1] and kspan[0] < at[1] or at[0] < vspan[1] and vspan[0] < at[1]):
             raise ValueError(f"glq_b200: {name} overlaps the cache")
     if tokens:
         a = _lib.PagedAppendDesc(at_key[0], at_value[0], at_query[0] if at_query is not None else None, out.data_ptr() if out is not None else None, ks[0], ks[1], vs[0], vs[1], qs[0],
                                  qs[1], os[0], os[1], tokens, slots.data_ptr(), at_positions, slots_wide, positions_wide, _DTYPES[kind], heads)
-        _call(key.get_device(), "paged_append", _lib.load().glqb_paged_append, C.byref(desc), C.byref(a), turn)
+        _call(index, "paged_append", _lib.load().glqb_paged_append, C.byref(desc), C.byref(a), turn)
     return out
 
 
@@ -299,27 +310,29 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
     new result and stay as they are in a given ``out``.  Sums and softmax in fp32, weights rounded to the cache's type for the product with the values, as
     is the result; what lies in the cache where no query looks, NaN included, changes nothing.  The same call gives the same bits."""
     desc, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
-    query, shape, qs, span = _heads(query, "query")
-    _same_device(query, key_cache, "query")
+    index = key_cache.get_device()
+    query, shape, qs, span = _heads(query, "query", index)
     tokens, heads, dim = shape
     if dim != cache[3] or query.dtype != dtype or heads < 1 or heads % cache[2]:
         raise ValueError(f"glq_b200: queries of {tuple(shape)}, {query.dtype}, over a cache of {tuple(cache)}, {dtype}")
-    _same_device(pages, query, "pages")
+    if not isinstance(pages, torch.Tensor) or pages.get_device() != index:
+        _same_device(pages, query, "pages")
     table = pages.shape
-    if pages.dtype != torch.int32 or len(table) != 2 or (table[1] > 1 and pages.stride(1) != 1):
+    if pages.dtype != torch.int32 or len(table) != 2 or (pages.stride(1) != 1 and table[1] > 1):
         raise ValueError(f"glq_b200: pages must be int32 (sequences, columns), a row's entries one behind the other, got {tuple(table)} of {pages.dtype}")
     seqs = table[0]
-    lengths_wide, offsets_wide, at_offsets = _integers(lengths, query, "lengths", seqs), False, None
+    lengths_wide, offsets_wide, at_offsets = _integers(lengths, index, "lengths", seqs), False, None
     if query_offsets is not None:
-        offsets_wide, at_offsets = _integers(query_offsets, query, "query_offsets", seqs + 1), query_offsets.data_ptr()
+        offsets_wide, at_offsets = _integers(query_offsets, index, "query_offsets", seqs + 1), query_offsets.data_ptr()
     elif tokens != seqs:
         raise ValueError(f"glq_b200: {tokens} queries of {seqs} sequences need query_offsets")
     if max_query_len is None:
         max_query_len = tokens if query_offsets is not None else 1
     elif max_query_len < 0:
         raise ValueError(f"glq_b200: max_query_len is {max_query_len}")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
+    if scale is None:
+        scale = dim ** -0.5
+    elif not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"glq_b200: scale is a positive number, not {scale}")
     window = int(window or 0)
     if not 0 <= window < 2 ** 31:
@@ -334,9 +347,10 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
             qs = query.stride()
         a = _lib.PagedAttentionDesc(query.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], tokens, pages.data_ptr(), pages.stride(0), lengths.data_ptr(), at_offsets, lengths_wide,
                                     offsets_wide, seqs, table[1], heads, bool(causal), window, fresh and at_offsets is not None, min(max_query_len, tokens), scale)
-        lib, index, cache_ref, ref = _lib.load(), query.get_device(), C.byref(desc), C.byref(a)
+        lib, cache_ref, ref = _lib.load(), C.byref(desc), C.byref(a)
         size = _workspace(lib, index, cache_ref, ref)
-        _call(index, "paged_attention", lib.glqb_paged_attention, cache_ref, ref, query.new_empty((size,), dtype=torch.uint8).data_ptr(), size)
+        ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=query.device)
+        _call(index, "paged_attention", lib.glqb_paged_attention, cache_ref, ref, ws.data_ptr(), size)
         _RAN_ON.add(index)
     return out
 
