@@ -503,8 +503,9 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
 // ---- what several CTAs have of an item, together --------------------------------------------------
 // The parts of an item that CTA blockIdx.x began and did not end are that CTA's, then those of the CTAs behind it up to the one that ended
 // the item.  Of few rows (MANY false) a block has all: a row is several warps', each every n-th part, then together.  Of many rows there are few
-// parts: a block has 32 rows, a warp four of them at once.  The order is the same in every call.
-constexpr int CB_ROWS = 32;
+// parts: a block has half of them, a warp two at once.  (All blocks are there at once then.  With 32 rows to a block of eight warps they came in four
+// waves: 11 us behind 50 of the products, 24 sequences of mixed lengths.)  The order is the same in every call.
+constexpr int CB_ROWS = 128, CB_WARPS = 16;
 struct Joined {
   float4 v;
   float most, sum;
@@ -526,10 +527,9 @@ struct Joined {
     }
   }
 };
-template <bool MANY> constexpr int CB_WARPS = MANY ? 8 : 16;
 template <typename T, int DP, bool MANY>
-__global__ void __launch_bounds__(CB_WARPS<MANY> * 32) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
-  constexpr int WARPS = CB_WARPS<MANY>;
+__global__ void __launch_bounds__(CB_WARPS * 32, 2) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
+  constexpr int WARPS = CB_WARPS;
   __shared__ float4 sums[WARPS][DP / 4];
   __shared__ float2 mls[WARPS];
   pdl_wait();
@@ -561,32 +561,34 @@ __global__ void __launch_bounds__(CB_WARPS<MANY> * 32) paged_combine_kernel(cons
     pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
   };
   if constexpr (MANY) {
-    Joined j[4];
+    const int last = min(lead.rows, (int)(blockIdx.y + 1) * CB_ROWS);
+    for (int row0 = blockIdx.y * CB_ROWS + warp; row0 < last; row0 += 2 * WARPS) {
+      Joined j[2];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-    const int row0 = blockIdx.y * CB_ROWS + warp;
-    for (int p0 = 0; p0 < parts; p0 += CB_BATCH) {
-      float2 ml[4][CB_BATCH];
-      float4 u[4][CB_BATCH];
+      for (int n = 0; n < 2; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+      for (int p0 = 0; p0 < parts; p0 += CB_BATCH) {
+        float2 ml[2][CB_BATCH];
+        float4 u[2][CB_BATCH];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int k = 0; k < CB_BATCH; ++k) {
-          const int row = row0 + n * WARPS;
-          ml[n][k] = make_float2(-INFINITY, 0.0f);
-          u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (p0 + k < parts && row < lead.rows) {
-            const long long at = part_at(p0 + k, row);
-            ml[n][k] = J.part_ml[at];
-            if (col < DP) u[n][k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
+          for (int k = 0; k < CB_BATCH; ++k) {
+            const int row = row0 + n * WARPS;
+            ml[n][k] = make_float2(-INFINITY, 0.0f);
+            u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (p0 + k < parts && row < last) {
+              const long long at = part_at(p0 + k, row);
+              ml[n][k] = J.part_ml[at];
+              if (col < DP) u[n][k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
+            }
           }
-        }
 #pragma unroll
-      for (int n = 0; n < 4; ++n) j[n].add(ml[n], u[n]);
+        for (int n = 0; n < 2; ++n) j[n].add(ml[n], u[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        if (row0 + n * WARPS < last) store(row0 + n * WARPS, j[n]);
     }
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (row0 + n * WARPS < lead.rows) store(row0 + n * WARPS, j[n]);
   } else {
     const int rows = min(WARPS, lead.rows);                // (an item has 16 at most)
     int wide = 1;
@@ -759,7 +761,7 @@ struct PagedForm {
 // Rows of a sequence and key head up to which the streaming kernel runs.
 constexpr int PA_STREAM_MOST = 16;
 // What beginning an item costs a CTA of either kernel, in its key tiles.
-constexpr int PA_STREAM_BEGIN = 2, PA_TILE_BEGIN = 2;
+constexpr int PA_STREAM_BEGIN = 2, PA_TILE_BEGIN = 2, PA_TILE_BEGIN_64 = 4;      // (heads of up to 64 values: shorter products)
 PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int sms) {
   PagedForm f;
   const int group = a->heads / c->kv_heads;
@@ -794,8 +796,8 @@ cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtens
   if (e != cudaSuccess) return e;
   constexpr auto FEW = paged_combine_kernel<T, DP, false>;
   constexpr auto MANY = paged_combine_kernel<T, DP, true>;
-  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS<true> * 32, 0, stream, J, f.ctas)
-                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas), CB_WARPS<false> * 32, 0, stream, J, f.ctas);
+  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS * 32, 0, stream, J, f.ctas)
+                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas), CB_WARPS * 32, 0, stream, J, f.ctas);
 }
 }  // namespace
 }  // namespace glqb
@@ -921,7 +923,7 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.clear = a->clear_rest;
   J.scale_log2 = a->scale * 1.4426950408889634f;
   J.most_keys = a->page_columns * c->page_size;
-  J.begin = f.tile ? PA_TILE_BEGIN : PA_STREAM_BEGIN;
+  J.begin = !f.tile ? PA_STREAM_BEGIN : f.dp == 64 ? PA_TILE_BEGIN_64 : PA_TILE_BEGIN;
   J.min_units = J.begin + (f.tile ? 2 : 1);
   J.rows = f.tile ? 128 / J.group * J.group * 2 : PA_STREAM_ROWS;
   J.out_wide = lies_on(a->out, 8) && a->out_token % 4 == 0 && a->out_head % 4 == 0;
