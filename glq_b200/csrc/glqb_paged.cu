@@ -503,9 +503,10 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
 // ---- what several CTAs have of an item, together --------------------------------------------------
 // The parts of an item that CTA blockIdx.x began and did not end are that CTA's, then those of the CTAs behind it up to the one that ended
 // the item.  Of few rows (MANY false) a block has all: a row is several warps', each every n-th part, then together.  Of many rows there are few
-// parts: a block has half of them, a warp two at once.  (All blocks are there at once then.  With 32 rows to a block of eight warps they came in four
-// waves: 11 us behind 50 of the products, 24 sequences of mixed lengths.)  The order is the same in every call.
-constexpr int CB_ROWS = 128, CB_WARPS = 16;
+// parts: a block has 16 rows, a warp two at once.  The order is the same in every call.  Bound by latency: a block reads what a CTA has left, then two rows'
+// parts.  (24 sequences of mixed lengths: 7 us behind 49 of the products; 128 rows to a block of 16 warps 9, 32 rows to one of eight, four at once, 11.)
+constexpr int CB_ROWS = 16;
+template <bool MANY> constexpr int CB_WARPS = MANY ? 8 : 16;
 struct Joined {
   float4 v;
   float most, sum;
@@ -528,8 +529,8 @@ struct Joined {
   }
 };
 template <typename T, int DP, bool MANY>
-__global__ void __launch_bounds__(CB_WARPS * 32, 2) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
-  constexpr int WARPS = CB_WARPS;
+__global__ void __launch_bounds__(CB_WARPS<MANY> * 32, MANY ? 4 : 2) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
+  constexpr int WARPS = CB_WARPS<MANY>;
   __shared__ float4 sums[WARPS][DP / 4];
   __shared__ float2 mls[WARPS];
   pdl_wait();
@@ -561,8 +562,9 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) paged_combine_kernel(const _
     pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
   };
   if constexpr (MANY) {
-    const int last = min(lead.rows, (int)(blockIdx.y + 1) * CB_ROWS);
-    for (int row0 = blockIdx.y * CB_ROWS + warp; row0 < last; row0 += 2 * WARPS) {
+    static_assert(CB_ROWS == 2 * WARPS, "");
+    const int row0 = blockIdx.y * CB_ROWS + warp, last = min(lead.rows, (int)(blockIdx.y + 1) * CB_ROWS);
+    if (row0 < last) {
       Joined j[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
@@ -796,8 +798,8 @@ cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtens
   if (e != cudaSuccess) return e;
   constexpr auto FEW = paged_combine_kernel<T, DP, false>;
   constexpr auto MANY = paged_combine_kernel<T, DP, true>;
-  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS * 32, 0, stream, J, f.ctas)
-                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas), CB_WARPS * 32, 0, stream, J, f.ctas);
+  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS<true> * 32, 0, stream, J, f.ctas)
+                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas), CB_WARPS<false> * 32, 0, stream, J, f.ctas);
 }
 }  // namespace
 }  // namespace glqb
