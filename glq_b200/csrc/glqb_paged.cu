@@ -913,7 +913,6 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.pages = a->page_table;
   J.page_stride = a->page_stride;
   J.seqs = a->sequences;
-  J.columns = a->page_columns;
   while (1 << J.page_log < c->page_size) ++J.page_log;
   J.tokens = (int)a->tokens;
   J.heads = a->heads;

@@ -20,7 +20,7 @@ struct PagedJob {
   const void *lengths, *offsets;
   const int* pages;
   long long page_stride;
-  int lengths_wide, offsets_wide, seqs, columns, page_log, tokens, heads, kv_heads, group, head_dim, causal, window, clear;
+  int lengths_wide, offsets_wide, seqs, page_log, tokens, heads, kv_heads, group, head_dim, causal, window, clear;
   float scale_log2;                  // scale * log2(e): weights are powers of two
   int most_keys;                     // columns * page size
   int min_units;                     // units that a CTA takes at least

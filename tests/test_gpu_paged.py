@@ -285,6 +285,31 @@ def test_rows_of_no_sequence(rows):
     assert ops.paged_attention(q[:0], k, v, pages, n, query_offsets=offsets * 0).shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("heads,kv,new", [(160, 1, 1), (160, 1, 3), (258, 2, 2), (128, 1, 5), (64, 1, 40), (7, 1, 100)])
+def test_wide_groups_of_heads(heads, kv, new):
+    """Up to 128 heads that share a key head are a tile's, more are the streaming kernel's."""
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(heads), [150, 70 + new], [new, new], kv, heads, 64, 16, HF)
+    y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=new)
+    _close(y, *O.attend(q, k, v, pages, n, offsets))
+
+
+def test_no_pages_at_all():
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(3), [50, 90], [3, 40], 1, 2, 64, 16, BF)
+    for longest in (1, 40):
+        y = ops.paged_attention(q, k, v, pages[:, :0], n, query_offsets=offsets, max_query_len=longest)
+        assert not y.any()
+
+
+@pytest.mark.parametrize("longest", [0, 1, 4, 16, 300])
+def test_bound_of_the_queries_changes_the_kernel_alone(longest):
+    """max_query_len chooses the kernel; results are right whatever it says."""
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(8), [300, 40, 77], [130, 1, 20], 2, 8, 128, 32, BF)
+    _close(ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=longest), *O.attend(q, k, v, pages, n, offsets))
+
+
 @pytest.mark.parametrize("new", [1, 90])
 def test_integers_that_make_no_sense_stay_in_bounds(new):
     """Pages outside the cache read as zeros, lengths are held to the table, offsets to the rows."""
