@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GLQB_LIB_PATH") or os.path.join(_HERE, "libglq_b200.so")
@@ -125,6 +126,17 @@ class LinearDesc(C.Structure):
     ]
 
 
+def _packer(desc):
+    """struct.Struct.pack for a description's fields: a fifth of what its constructor takes."""
+    codes = {C.c_void_p: "Q", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    s = struct.Struct("=" + "".join(codes[t] for _, t in desc._fields_) + "x" * (C.sizeof(desc) - sum(C.sizeof(t) for _, t in desc._fields_)))
+    if s.size != C.sizeof(desc):
+        raise RuntimeError(f"glq_b200: {desc.__name__} has gaps between its fields")
+    return s.pack
+
+
+pack_cache, pack_append, pack_attention = _packer(PagedCacheDesc), _packer(PagedAppendDesc), _packer(PagedAttentionDesc)
+
 _lib = None
 
 
@@ -237,13 +249,14 @@ def load() -> C.CDLL:
     lib.glqb_mx4_product.restype = C.c_int
     lib.glqb_mx4_status.argtypes = [C.POINTER(i32)]
     lib.glqb_mx4_status.restype = C.c_int
-    lib.glqb_rotary.argtypes = [C.POINTER(RotaryDesc), vp, i32, i64, i64, vp, i64, i64, i64, i32, i32, vp, i32, vp]
+    # (descriptions go as a structure or as its packed bytes)
+    lib.glqb_rotary.argtypes = [vp, vp, i32, i64, i64, vp, i64, i64, i64, i32, i32, vp, i32, vp]
     lib.glqb_rotary.restype = C.c_int
-    lib.glqb_paged_append.argtypes = [C.POINTER(PagedCacheDesc), C.POINTER(PagedAppendDesc), C.POINTER(RotaryDesc), vp]
+    lib.glqb_paged_append.argtypes = [vp, vp, vp, vp]
     lib.glqb_paged_append.restype = C.c_int
-    lib.glqb_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedCacheDesc), C.POINTER(PagedAttentionDesc)]
+    lib.glqb_paged_attention_workspace_bytes.argtypes = [vp, vp]
     lib.glqb_paged_attention_workspace_bytes.restype = sz
-    lib.glqb_paged_attention.argtypes = [C.POINTER(PagedCacheDesc), C.POINTER(PagedAttentionDesc), vp, sz, vp]
+    lib.glqb_paged_attention.argtypes = [vp, vp, vp, sz, vp]
     lib.glqb_paged_attention.restype = C.c_int
     lib.glqb_paged_status.argtypes = [C.POINTER(i32)]
     lib.glqb_paged_status.restype = C.c_int

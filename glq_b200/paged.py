@@ -28,24 +28,19 @@ _NONE = (0, 0)                      # strides of what is not there
 class Rotary:
     """Frequencies of rotary positions (``rotary_table``): ``turns`` int64 (pairs,) on the device, the fraction of a turn that a pair makes per
     position in units of 2^-64; ``scale`` on cosine and sine; ``interleaved``: neighbouring values make a pair, else values half of the
-    rotated part apart.  The attributes cannot be set."""
-    __slots__ = ("turns", "scale", "interleaved", "_desc", "_ref", "_index")
+    rotated part apart; ``dim``: values of a head that are rotated.  The attributes cannot be set."""
+    __slots__ = ("turns", "scale", "interleaved", "dim", "_desc", "_ref", "_index")
 
     def __init__(self, turns, scale=1.0, interleaved=False):
         _cuda(turns, "turns")
         if turns.dtype != torch.int64 or turns.dim() != 1 or not turns.numel() or not turns.is_contiguous():
             raise ValueError(f"glq_b200: turns must be int64 (pairs,), got {tuple(turns.shape)} of {turns.dtype}")
         desc = _lib.RotaryDesc(turns.data_ptr(), turns.numel(), bool(interleaved), float(scale))
-        for name, value in zip(self.__slots__, (turns, float(scale), bool(interleaved), desc, C.byref(desc), turns.get_device())):
+        for name, value in zip(self.__slots__, (turns, float(scale), bool(interleaved), 2 * turns.numel(), desc, C.byref(desc), turns.get_device())):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
         raise AttributeError(f"glq_b200: {name} of a rotary table cannot be set")
-
-    @property
-    def dim(self) -> int:
-        """Values of a head that are rotated."""
-        return 2 * self.turns.numel()
 
 
 def _frequencies(dim, base, scaling):
@@ -119,13 +114,23 @@ def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv
     return Rotary(turns.to(device), own if scale is None else scale, interleaved)
 
 
+def _device_of(x, name, index=None):
+    """The device a tensor is on, which is ``index`` if that is given.  (One call instead of three: -1 is the host's, others have none.)"""
+    try:
+        own = x.get_device()
+    except AttributeError:
+        own = -1
+    if own < 0:
+        _cuda(x, name)
+    if index is not None and own != index:
+        raise ValueError(f"glq_b200: {name} is on {x.device}, expected cuda:{index}")
+    return own
+
+
 def _heads(x, name, index=None):
     """x (tokens, heads, head_dim) with a head's values one behind the other, its shape, strides and span: the addresses from its first value to
     behind its last.  On the device ``index`` if that is given."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        _cuda(x, name)
-    if index is not None and x.get_device() != index:
-        raise ValueError(f"glq_b200: {name} is on {x.device}, expected cuda:{index}")
+    _device_of(x, name, index)
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"glq_b200: {name} is (tokens, heads, head_dim), got {tuple(shape)}")
@@ -138,12 +143,10 @@ def _heads(x, name, index=None):
 
 def _span(x, shape, stride):
     first = x.data_ptr()
-    if 0 in shape:
+    t, h, d = shape
+    if not (t and h and d):
         return first, first
-    last = 1
-    for n, s in zip(shape, stride):
-        last += (n - 1) * s
-    return first, first + last * x.itemsize
+    return first, first + ((t - 1) * stride[0] + (h - 1) * stride[1] + d) * x.itemsize
 
 
 def _result(out, x, shape, stride, span, name):
@@ -151,8 +154,8 @@ def _result(out, x, shape, stride, span, name):
     values in one place, and is x itself or lies apart from it."""
     if out is None:
         t, h, d = shape
-        stride = (h * d, d, 1)
-        return torch.empty_strided(shape, stride, dtype=x.dtype, device=x.device), stride, None
+        own = (h * d, d, 1)
+        return torch.empty_like(x) if stride == own else torch.empty_strided(shape, own, dtype=x.dtype, device=x.device), own, None
     _same_device(out, x, name)
     if out.shape != shape or out.dtype != x.dtype:
         raise ValueError(f"glq_b200: {name} must be {tuple(shape)} of {x.dtype}, got {tuple(out.shape)} of {out.dtype}")
@@ -186,21 +189,18 @@ def _rows_meet(a, shape, stride, b, other, own, x):
 
 def _integers(t, index, name, count):
     """Are they int64 (else int32)?"""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _cuda(t, name)
-    if t.get_device() != index:
-        raise ValueError(f"glq_b200: {name} is on {t.device}, expected cuda:{index}")
+    _device_of(t, name, index)
     dtype = t.dtype
     if dtype not in _INTEGERS or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"glq_b200: {name} must be {count} int32 or int64 values, got {tuple(t.shape)} of {dtype}")
     return dtype is torch.int64
 
 
-def _check_table(table, x, head_dim):
+def _check_table(table, index, head_dim):
     if table.__class__ is not Rotary:
         raise ValueError("glq_b200: table is what rotary_table returns")
-    if table._index != x.get_device():
-        raise ValueError(f"glq_b200: the rotary table is on {table.turns.device}, expected {x.device}")
+    if table._index != index:
+        raise ValueError(f"glq_b200: the rotary table is on {table.turns.device}, expected cuda:{index}")
     if table.dim > head_dim:
         raise ValueError(f"glq_b200: {table.dim} rotated values in heads of {head_dim}")
 
@@ -212,7 +212,7 @@ def rotary(x, positions, table: Rotary, *, out=None) -> torch.Tensor:
     x, shape, stride, span = _heads(x, "x")
     dt = _dtype(x.dtype, "x")
     tokens, heads, dim = shape
-    _check_table(table, x, dim)
+    _check_table(table, x.get_device(), dim)
     wide = _integers(positions, table._index, "positions", tokens)
     out, own, _ = _result(out, x, shape, stride, span, "out")
     if tokens and heads:
@@ -222,9 +222,9 @@ def rotary(x, positions, table: Rotary, *, out=None) -> torch.Tensor:
 
 
 def _cache(keys, values):
-    """The C description of a cache, checked, its shape, and the spans of its two tensors."""
-    _cuda(keys, "key_cache")
-    _same_device(values, keys, "value_cache")
+    """The C description of a cache, checked, its device, shape, type, and the spans of its two tensors."""
+    index = _device_of(keys, "key_cache")
+    _device_of(values, "value_cache", index)
     shape, dtype = keys.shape, keys.dtype
     if len(shape) != 4 or values.shape != shape or values.dtype != dtype:
         raise ValueError(f"glq_b200: key_cache and value_cache are (pages, page_size, kv_heads, head_dim) of one type, got {tuple(keys.shape)} of {keys.dtype} and "
@@ -244,9 +244,9 @@ def _cache(keys, values):
     if kd != 1 or vd != 1 or (first | other) & 15 or (kp | kr | kh | vp | vr | vh) & 7:
         raise ValueError(f"glq_b200: key_cache and value_cache must lie on 16 bytes, strides of 8 values, a head's values one behind the other; got strides {keys.stride()} and "
                          f"{values.stride()}")
-    desc = _lib.PagedCacheDesc(first, other, kp, kr, kh, vp, vr, vh, pages, size, heads, dim, kind)
+    desc = _lib.pack_cache(first, other, kp, kr, kh, vp, vr, vh, pages, size, heads, dim, kind)
     pages, size, heads = pages - 1, size - 1, heads - 1
-    return (desc, shape, dtype, (first, first + 2 * (pages * kp + size * kr + heads * kh + dim)), (other, other + 2 * (pages * vp + size * vr + heads * vh + dim)))
+    return (desc, index, shape, dtype, (first, first + 2 * (pages * kp + size * kr + heads * kh + dim)), (other, other + 2 * (pages * vp + size * vr + heads * vh + dim)))
 
 
 def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, table: Optional[Rotary] = None, query=None, out=None):
@@ -255,8 +255,7 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
     The slots within the cache are all different.  With ``table`` and ``positions`` (tokens,) the keys are rotated on the way, and so is ``query``
     (tokens, heads, head_dim) if it is given: to a new tensor or to ``out`` (the query itself too), which is returned.  Keys, values and
     queries are of the cache's type, or fp32."""
-    desc, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
-    index = key_cache.get_device()
+    desc, index, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
     key, shape, ks, at_key = _heads(key, "key", index)
     value, value_shape, vs, at_value = _heads(value, "value", index)
     tokens, kv_heads, dim = shape
@@ -265,11 +264,11 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
     kind = key.dtype
     if value.dtype != kind or (kind != dtype and kind != torch.float32):
         raise ValueError(f"glq_b200: keys and values are of the cache's type, {dtype}, or fp32, got {kind} and {value.dtype}")
-    slots_wide, positions_wide, at_positions, turn = _integers(slots, index, "slots", tokens), False, None, None
+    slots_wide, positions_wide, at_positions, turn = _integers(slots, index, "slots", tokens), False, 0, None
     if (table is None) != (positions is None):
         raise ValueError("glq_b200: table and positions come together")
     if table is not None:
-        _check_table(table, key, dim)
+        _check_table(table, index, dim)
         positions_wide, at_positions, turn = _integers(positions, index, "positions", tokens), positions.data_ptr(), table._ref
     heads, at_query, at_out, qs, os = 0, None, None, _NONE, _NONE
     if query is None:
@@ -290,9 +289,9 @@ def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, t
         if at is not None and (at[0] < kspan[1] and kspan[0] < at[1] or at[0] < vspan[1] and vspan[0] < at[1]):
             raise ValueError(f"glq_b200: {name} overlaps the cache")
     if tokens:
-        a = _lib.PagedAppendDesc(at_key[0], at_value[0], at_query[0] if at_query is not None else None, out.data_ptr() if out is not None else None, ks[0], ks[1], vs[0], vs[1], qs[0],
+        a = _lib.pack_append(at_key[0], at_value[0], at_query[0] if at_query is not None else 0, out.data_ptr() if out is not None else 0, ks[0], ks[1], vs[0], vs[1], qs[0],
                                  qs[1], os[0], os[1], tokens, slots.data_ptr(), at_positions, slots_wide, positions_wide, _DTYPES[kind], heads)
-        _call(index, "paged_append", _lib.load().glqb_paged_append, C.byref(desc), C.byref(a), turn)
+        _call(index, "paged_append", _lib.load().glqb_paged_append, desc, a, turn)
     return out
 
 
@@ -309,19 +308,17 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
     outside the cache reads as zeros.  Rows that see no key are zero.  Rows of no sequence (in front of query_offsets[0], behind the last) are zero in a
     new result and stay as they are in a given ``out``.  Sums and softmax in fp32, weights rounded to the cache's type for the product with the values, as
     is the result; what lies in the cache where no query looks, NaN included, changes nothing.  The same call gives the same bits."""
-    desc, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
-    index = key_cache.get_device()
+    desc, index, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)
     query, shape, qs, span = _heads(query, "query", index)
     tokens, heads, dim = shape
     if dim != cache[3] or query.dtype != dtype or heads < 1 or heads % cache[2]:
         raise ValueError(f"glq_b200: queries of {tuple(shape)}, {query.dtype}, over a cache of {tuple(cache)}, {dtype}")
-    if not isinstance(pages, torch.Tensor) or pages.get_device() != index:
-        _same_device(pages, query, "pages")
+    _device_of(pages, "pages", index)
     table = pages.shape
     if pages.dtype != torch.int32 or len(table) != 2 or (pages.stride(1) != 1 and table[1] > 1):
         raise ValueError(f"glq_b200: pages must be int32 (sequences, columns), a row's entries one behind the other, got {tuple(table)} of {pages.dtype}")
     seqs = table[0]
-    lengths_wide, offsets_wide, at_offsets = _integers(lengths, index, "lengths", seqs), False, None
+    lengths_wide, offsets_wide, at_offsets = _integers(lengths, index, "lengths", seqs), False, 0
     if query_offsets is not None:
         offsets_wide, at_offsets = _integers(query_offsets, index, "query_offsets", seqs + 1), query_offsets.data_ptr()
     elif tokens != seqs:
@@ -345,12 +342,12 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
         if span[0] & 15 or qs[0] & 7 or qs[1] & 7:
             query = query.clone(memory_format=torch.contiguous_format)
             qs = query.stride()
-        a = _lib.PagedAttentionDesc(query.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], tokens, pages.data_ptr(), pages.stride(0), lengths.data_ptr(), at_offsets, lengths_wide,
-                                    offsets_wide, seqs, table[1], heads, bool(causal), window, fresh and at_offsets is not None, min(max_query_len, tokens), scale)
-        lib, cache_ref, ref = _lib.load(), C.byref(desc), C.byref(a)
-        size = _workspace(lib, index, cache_ref, ref)
+        a = _lib.pack_attention(query.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], tokens, pages.data_ptr(), pages.stride(0), lengths.data_ptr(), at_offsets, lengths_wide,
+                                    offsets_wide, seqs, table[1], heads, bool(causal), window, fresh and query_offsets is not None, min(max_query_len, tokens), scale)
+        lib = _lib.load()
+        size = _workspace(lib, index, desc, a)
         ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=query.device)
-        _call(index, "paged_attention", lib.glqb_paged_attention, cache_ref, ref, ws.data_ptr(), size)
+        _call(index, "paged_attention", lib.glqb_paged_attention, desc, a, ws.data_ptr(), size)
         _RAN_ON.add(index)
     return out
 

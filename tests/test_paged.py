@@ -55,6 +55,13 @@ def test_struct_layouts_match_header(tmp_path):
     assert out == [v for _, d in pairs for v in [ctypes.sizeof(d)] + [getattr(d, f[0]).offset for f in d._fields_]]
 
 
+def test_packed_descriptions_are_the_structures():
+    from glq_b200 import _lib
+    for desc, pack in ((_lib.PagedCacheDesc, _lib.pack_cache), (_lib.PagedAppendDesc, _lib.pack_append), (_lib.PagedAttentionDesc, _lib.pack_attention)):
+        values = [0.5 if t is ctypes.c_float else 3 + i for i, (_, t) in enumerate(desc._fields_)]
+        assert pack(*values) == bytes(desc(*values))
+
+
 def test_c_entries_refuse_before_any_cuda_call(lib):
     from glq_b200 import _lib
     p = 4096                                                    # never dereferenced: each call is refused
@@ -198,6 +205,7 @@ def test_operators_refuse_wrong_arguments(monkeypatch):
     big = _table(monkeypatch, 128)
     monkeypatch.setattr(paged, "_cuda", lambda t, name: None)
     monkeypatch.setattr(paged, "_same_device", lambda t, x, name: None)
+    monkeypatch.setattr(paged, "_device_of", lambda t, name, index=None: -1)
     launched = []
     monkeypatch.setattr(paged, "_call", lambda *a: launched.append(a[1]))
     monkeypatch.setattr(paged, "_workspace", lambda *a: 64)
