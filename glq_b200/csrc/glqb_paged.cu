@@ -2,6 +2,7 @@
 #include "glqb_paged.cuh"
 #include <algorithm>
 #include <atomic>
+#include <chrono>
 #include <climits>
 #include <cmath>
 #include <cstdarg>
@@ -12,6 +13,7 @@ namespace glqb {
 namespace {
 
 __device__ int g_paged_status;      // 0, or what gave up (ST_GAVE_UP_*): calls have no plan to keep it in
+__device__ unsigned g_paged_gave_up; // how often
 
 // ---- rotation and append --------------------------------------------------------------------------
 // Heads of every token, in up to three parts (queries, keys, values).  One pass: a thread moves two pieces of eight values, those that
@@ -214,6 +216,28 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// parts of a row, added up
+struct Joined {
+  float4 v;
+  float most, sum;
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&u)[N]) {
+    float now = most;
+#pragma unroll
+    for (int k = 0; k < N; ++k) now = fmaxf(now, ml[k].x);
+    const float f = now == -INFINITY ? 1.0f : pa_exp2(most - now);
+    sum *= f;
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    most = now;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;        // (no key of its own: nothing in its sums)
+      const float w = pa_exp2(ml[k].x - now);
+      sum += w * ml[k].y;
+      v.x += w * u[k].x; v.y += w * u[k].y; v.z += w * u[k].z; v.w += w * u[k].w;
+    }
+  }
+};
 template <typename T, int DP>
 __global__ void __launch_bounds__(ST_THREADS, 2)
 paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -240,7 +264,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
     // the first of the two makes the list of items, the second one takes it from there, as the others do
     const bool values = warp > ST_WARPS;
     const CUtensorMap* map = values ? &map_v : &map_k;
-    PagedWalk<KEYS> walk(J, B.start);
+    PagedWalk<KEYS, true> walk(J, B.start);
     const int piece = min(1 << J.page_log, PA_PIECE), pieces = KEYS / piece, page_mask = (1 << J.page_log) - 1;
     uint32_t stage = 0, phase = 1, ip = values ? 0 : 1, filled = 0;
     int is = 0;
@@ -280,14 +304,21 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
       advance();
     }
     if (lane == 0) {
-      if (!ok) { *(volatile int*)&B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); }
-      if (!values) pa_publish(J, walk.part);
+      if (!ok) { *(volatile int*)&B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_LOADER); atomicAdd(J.gave_up, 1u); }
     }
     // copies in flight land before the block ends (a stage that the other of the two did not fill does not: the wait is bounded)
     if (!ok)
       for (uint32_t n = 1; n <= min(filled, (uint32_t)C::STAGES); ++n) mbar_wait(&B.full[(filled - n) % C::STAGES], (filled - n) / C::STAGES & 1u);
   } else {
     const int g = lane >> 2, t4 = lane & 3;
+    const unsigned long long tag = (J.tag + *(volatile unsigned*)J.gave_up * 0x9E3779B97F4A7ull) & ((1ull << 52) - 1) | 1ull;
+    if (J.clear) {
+      const int first = pa_offset(J, 0), last = max(first, pa_offset(J, J.seqs)), rest = J.tokens - (last - first);
+      for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+        T* p = reinterpret_cast<T*>(J.out) + (long long)(i < first ? i : i + last - first) * J.out_token;
+        for (int k = threadIdx.x; k < J.heads * J.head_dim; k += ST_WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
+      }
+    }
     uint32_t stage = 0, phase = 0, ip = 0, turn = 0;
     int is = 0;
     auto advance = [&] { if (++stage == C::STAGES) { stage = 0; phase ^= 1u; } };
@@ -301,6 +332,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
       if (lane == 0) mbar_arrive(&B.item_empty[is]);
       if (!it.more) break;
       if (++is == ST_ITEMS) { is = 0; ip ^= 1u; }
+      if (lane == 0 && it.slot >= 0 && warp * (128 / DP) < it.rows) pa_open(J.tickets + it.begun_by * ST_WARPS + warp, tag);
       // queries as fragments: rows g and g + 8
       uint32_t q[STEPS][4];
       int to[2], from[2];
@@ -492,51 +524,58 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
       }
       __syncwarp();
       if (lane == 0) { mbar_arrive(&B.joined[1]); mbar_arrive(&B.empty[stage]); }
+      // An item that several CTAs have a part of: a warp has the same rows in each.  The last to arrive adds them up, all from the workspace, in the
+      // order of the CTAs.  (In a launch of its own behind this one: one token of 4096 keys FIXME us, 12.2.)
+      if (it.slot >= 0 && warp * (128 / DP) < it.rows) {
+        __threadfence();
+        __syncwarp();
+        int last = 0;
+        if (lane == 0) last = pa_arrive(J.tickets + it.begun_by * ST_WARPS + warp, it.parts);
+        if (__shfl_sync(0xFFFFFFFFu, last, 0)) {
+          __threadfence();
+          for (int i = threadIdx.x; i < it.rows * (DP / 4); i += ST_WARPS * 32) {
+            const int row = i / (DP / 4), col = i % (DP / 4) * 4;
+            Joined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+            for (int p0 = 0; p0 < it.parts; p0 += 8) {
+              float2 ml[8];
+              float4 u[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.0f);
+                u[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (p0 + k < it.parts) {
+                  const long long at = (2ll * (it.begun_by + p0 + k) + (p0 + k == 0)) * ROWS + row;
+                  ml[k] = __ldcg(J.part_ml + at);
+                  u[k] = __ldcg(reinterpret_cast<const float4*>(J.part + at * DP + col));
+                }
+              }
+              j.add(ml, u);
+            }
+            const float f = pa_row_factor(J, seq, it.first + row, j.sum);
+            if (col < J.head_dim) pa_store4<T>(J, pa_out_row(J, it.row0, it.kv_head, it.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
+          }
+          __syncwarp();
+        }
+      }
       if (!mbar_wait_warp(&B.joined[1], turn, &B.abort)) { ok = false; break; }       // (ml is read)
       turn ^= 1u;
       advance();
     }
-    if (!ok && lane == 0) { *(volatile int*)&B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); }
+    if (!ok && lane == 0) { *(volatile int*)&B.abort = 1; atomicCAS(J.status, 0, (int)ST_GAVE_UP_MMA); atomicAdd(J.gave_up, 1u); }
   }
 }
 
-// ---- what several CTAs have of an item, together --------------------------------------------------
+// ---- what several CTAs have of an item of many rows, together -------------------------------------
 // The parts of an item that CTA blockIdx.x began and did not end are that CTA's, then those of the CTAs behind it up to the one that ended
-// the item.  Of few rows (MANY false) a block has all: a row is several warps', each every n-th part, then together.  Of many rows there are few
-// parts: a block has 16 rows, a warp two at once.  The order is the same in every call.  Bound by latency: a block reads what a CTA has left, then two rows'
-// parts.  (24 sequences of mixed lengths: 7 us behind 49 of the products; 128 rows to a block of 16 warps 9, 32 rows to one of eight, four at once, 11.)
-constexpr int CB_ROWS = 16;
-template <bool MANY> constexpr int CB_WARPS = MANY ? 8 : 16;
-struct Joined {
-  float4 v;
-  float most, sum;
-  template <int N>
-  __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&u)[N]) {
-    float now = most;
-#pragma unroll
-    for (int k = 0; k < N; ++k) now = fmaxf(now, ml[k].x);
-    const float f = now == -INFINITY ? 1.0f : pa_exp2(most - now);
-    sum *= f;
-    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-    most = now;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;        // (no key of its own: nothing in its sums)
-      const float w = pa_exp2(ml[k].x - now);
-      sum += w * ml[k].y;
-      v.x += w * u[k].x; v.y += w * u[k].y; v.z += w * u[k].z; v.w += w * u[k].w;
-    }
-  }
-};
-template <typename T, int DP, bool MANY>
-__global__ void __launch_bounds__(CB_WARPS<MANY> * 32, MANY ? 4 : 2) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
-  constexpr int WARPS = CB_WARPS<MANY>;
-  __shared__ float4 sums[WARPS][DP / 4];
-  __shared__ float2 mls[WARPS];
+// the item.  A block has 16 rows, a warp two at once.  The order is the same in every call.  Bound by latency: a block reads what a CTA has left, then two
+// rows' parts.  (24 sequences of mixed lengths: 7 us behind 49 of the products; 128 rows to a block of 16 warps 9, 32 rows to one of eight, four at once, 11.
+// One CTA could not do it in the first kernel, as it does with few rows: 256 rows of 18 CTAs are 2.4 MB.)
+constexpr int CB_WARPS = 8, CB_ROWS = 2 * CB_WARPS, CB_BATCH = 2;
+template <typename T, int DP>
+__global__ void __launch_bounds__(CB_WARPS * 32, 4) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, col = lane * 4;
-  constexpr int PLACES = MANY ? PA_TILE_ROWS : PA_STREAM_ROWS, CB_BATCH = MANY ? 2 : 4;      // (parts of a row at once)
   // (the first parts' ends are asked for before it is known whether this CTA has left a beginning)
   const PagedPart lead = J.part_of[2 * c + 1];
   auto ends = [&](int parts) {
@@ -548,92 +587,46 @@ __global__ void __launch_bounds__(CB_WARPS<MANY> * 32, MANY ? 4 : 2) paged_combi
     const int first = pa_offset(J, 0), last = max(first, pa_offset(J, J.seqs)), rest = J.tokens - (last - first);
     for (int i = c; i < rest; i += gridDim.x) {
       T* p = reinterpret_cast<T*>(J.out) + (long long)(i < first ? i : i + last - first) * J.out_token;
-      for (int k = threadIdx.x; k < J.heads * J.head_dim; k += WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
+      for (int k = threadIdx.x; k < J.heads * J.head_dim; k += CB_WARPS * 32) p[k / J.head_dim * J.out_head + k % J.head_dim] = pa_round<T>(0.0f);
     }
   }
   if (!lead.valid) return;
   int parts = 1;
   while (!end) end = ends(parts += 32);
   parts += __ffs(end);
-  auto part_at = [&](int p, int row) { return (p ? 2ll * (c + p) : 2ll * c + 1) * PLACES + pa_place(J, row); };
+  auto part_at = [&](int p, int row) { return (p ? 2ll * (c + p) : 2ll * c + 1) * PA_TILE_ROWS + pa_place(J, row); };
   auto store = [&](int row, const Joined& j) {
     if (col >= J.head_dim) return;
     const float f = pa_row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, j.sum);
     pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
   };
-  if constexpr (MANY) {
-    static_assert(CB_ROWS == 2 * WARPS, "");
-    const int row0 = blockIdx.y * CB_ROWS + warp, last = min(lead.rows, (int)(blockIdx.y + 1) * CB_ROWS);
-    if (row0 < last) {
-      Joined j[2];
+  const int row0 = blockIdx.y * CB_ROWS + warp, last = min(lead.rows, (int)(blockIdx.y + 1) * CB_ROWS);
+  if (row0 >= last) return;
+  Joined j[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-      for (int p0 = 0; p0 < parts; p0 += CB_BATCH) {
-        float2 ml[2][CB_BATCH];
-        float4 u[2][CB_BATCH];
+  for (int n = 0; n < 2; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  for (int p0 = 0; p0 < parts; p0 += CB_BATCH) {
+    float2 ml[2][CB_BATCH];
+    float4 u[2][CB_BATCH];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int k = 0; k < CB_BATCH; ++k) {
-            const int row = row0 + n * WARPS;
-            ml[n][k] = make_float2(-INFINITY, 0.0f);
-            u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (p0 + k < parts && row < last) {
-              const long long at = part_at(p0 + k, row);
-              ml[n][k] = J.part_ml[at];
-              if (col < DP) u[n][k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
-            }
-          }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) j[n].add(ml[n], u[n]);
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-        if (row0 + n * WARPS < last) store(row0 + n * WARPS, j[n]);
-    }
-  } else {
-    const int rows = min(WARPS, lead.rows);                // (an item has 16 at most)
-    int wide = 1;
-    while (wide < rows) wide <<= 1;
-    const int groups = WARPS / wide, row = warp % wide, group = warp / wide;
-    Joined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-    if (row < rows)
-      for (int p0 = group; p0 < parts; p0 += CB_BATCH * groups) {
-        float2 ml[CB_BATCH];
-        float4 u[CB_BATCH];
-#pragma unroll
-        for (int k = 0; k < CB_BATCH; ++k) {
-          const int p = p0 + k * groups;
-          ml[k] = make_float2(-INFINITY, 0.0f);
-          u[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (p < parts) {
-            const long long at = part_at(p, row);
-            ml[k] = J.part_ml[at];
-            if (col < DP) u[k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
-          }
+      for (int k = 0; k < CB_BATCH; ++k) {
+        const int row = row0 + n * CB_WARPS;
+        ml[n][k] = make_float2(-INFINITY, 0.0f);
+        u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p0 + k < parts && row < last) {
+          const long long at = part_at(p0 + k, row);
+          ml[n][k] = J.part_ml[at];
+          if (col < DP) u[n][k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
         }
-        j.add(ml, u);
       }
-    if (groups > 1) {
-      if (lane == 0) mls[warp] = make_float2(j.most, j.sum);
-      if (col < DP) sums[warp][lane] = j.v;
-      __syncthreads();
-      if (group > 0) return;
-      j = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-      for (int k0 = 0; k0 < groups; k0 += CB_BATCH) {
-        float2 ml[CB_BATCH];
-        float4 u[CB_BATCH];
 #pragma unroll
-        for (int k = 0; k < CB_BATCH; ++k) {
-          const bool there = k0 + k < groups;
-          ml[k] = there ? mls[warp + (k0 + k) * wide] : make_float2(-INFINITY, 0.0f);
-          u[k] = there && col < DP ? sums[warp + (k0 + k) * wide][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        j.add(ml, u);
-      }
-    }
-    if (row < rows) store(row, j);
+    for (int n = 0; n < 2; ++n) j[n].add(ml[n], u[n]);
   }
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+    if (row0 + n * CB_WARPS < last) store(row0 + n * CB_WARPS, j[n]);
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -654,6 +647,7 @@ size_t size_of(int d) { return d == GLQB_DT_F32 ? 4 : 2; }
 struct PagedDevice {
   std::atomic<int> sms{0};
   int* status = nullptr;
+  unsigned* gave_up = nullptr;
 };
 const PagedDevice* pg_device() {
   static PagedDevice known[64];
@@ -664,7 +658,8 @@ const PagedDevice* pg_device() {
     int n = 0;
     if (d.sms.load(std::memory_order_relaxed) == 0) {
       if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, pg_device_index()) != cudaSuccess || n < 1 ||
-          cudaGetSymbolAddress(reinterpret_cast<void**>(&d.status), g_paged_status) != cudaSuccess)
+          cudaGetSymbolAddress(reinterpret_cast<void**>(&d.status), g_paged_status) != cudaSuccess ||
+          cudaGetSymbolAddress(reinterpret_cast<void**>(&d.gave_up), g_paged_gave_up) != cudaSuccess)
         return nullptr;
       d.sms.store(n, std::memory_order_release);
     }
@@ -754,6 +749,15 @@ bool encode_queries(CUtensorMap* map, const GlqbPagedCache* c, const GlqbPagedAt
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A call's tag: 52 bits of the splitmix64 sequence (Steele, Lea and Flood 2014), which starts anywhere.
+unsigned long long next_tag() {
+  static std::atomic<unsigned long long> state{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() ^ (unsigned long long)reinterpret_cast<uintptr_t>(&state) << 20};
+  unsigned long long z = state.fetch_add(0x9E3779B97F4A7C15ull) + 0x9E3779B97F4A7C15ull;
+  z = (z ^ z >> 30) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ z >> 27) * 0x94D049BB133111EBull;
+  return (z ^ z >> 31) >> 12;
+}
+
 // What a call launches and keeps in its workspace, by its sizes alone.
 struct PagedForm {
   bool tile;                        // on the tensor cores
@@ -773,7 +777,8 @@ PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int s
   f.ctas = f.tile ? sms : 2 * sms;
   f.ml = (size_t)f.ctas * 2 * f.rows * f.dp * sizeof(float);
   f.part_of = f.ml + (size_t)f.ctas * 2 * f.rows * sizeof(float2);
-  f.bytes = f.part_of + (size_t)f.ctas * 2 * sizeof(PagedPart);
+  // (many rows: what the CTAs leave; few: tickets)
+  f.bytes = f.part_of + (size_t)f.ctas * (f.tile ? 2 * sizeof(PagedPart) : ST_WARPS * sizeof(unsigned long long));
   return f;
 }
 int check_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a) {
@@ -793,13 +798,11 @@ template <typename T, int DP>
 cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   using C = StreamShape<DP>;
   constexpr auto K = paged_stream_kernel<T, DP>;
-  const cudaError_t e = f.tile ? paged_tile_launch(J, __is_same(T, __nv_bfloat16), mq, mk, mv, f.ctas, stream)
-                               : paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
+  if (!f.tile) return paged_launch<K>(K, dim3((unsigned)f.ctas), ST_THREADS, C::STAGES * C::STAGE + sizeof(StreamShared) + 1024, stream, J, mk, mv);
+  const cudaError_t e = paged_tile_launch(J, __is_same(T, __nv_bfloat16), mq, mk, mv, f.ctas, stream);
   if (e != cudaSuccess) return e;
-  constexpr auto FEW = paged_combine_kernel<T, DP, false>;
-  constexpr auto MANY = paged_combine_kernel<T, DP, true>;
-  return f.tile ? paged_launch<MANY>(MANY, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS<true> * 32, 0, stream, J, f.ctas)
-                : paged_launch<FEW>(FEW, dim3((unsigned)f.ctas), CB_WARPS<false> * 32, 0, stream, J, f.ctas);
+  constexpr auto CB = paged_combine_kernel<T, DP>;
+  return paged_launch<CB>(CB, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS * 32, 0, stream, J, f.ctas);
 }
 }  // namespace
 }  // namespace glqb
@@ -932,7 +935,10 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.part = (float*)workspace;
   J.part_ml = (float2*)((uint8_t*)workspace + f.ml);
   J.part_of = (PagedPart*)((uint8_t*)workspace + f.part_of);
+  J.tickets = (unsigned long long*)((uint8_t*)workspace + f.part_of);
+  J.tag = next_tag();
   J.status = d->status;
+  J.gave_up = d->gave_up;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   cudaError_t e;
   if (c->dtype == GLQB_DT_F16) e = f.dp == 64 ? attention_launch<__half, 64>(J, f, mq, mk, mv, stream) : attention_launch<__half, 128>(J, f, mq, mk, mv, stream);

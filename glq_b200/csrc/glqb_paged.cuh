@@ -29,7 +29,10 @@ struct PagedJob {
   bool out_wide, out_sectors;        // rows of out lie on 8, 32 bytes
   float* part;                       // workspace: sums of items that several CTAs share, [CTA][2][rows][padded head_dim]
   float2* part_ml;                   // their largest exponent and sum, [CTA][2][rows]
-  struct PagedPart* part_of;         // [CTA][2]
+  struct PagedPart* part_of;         // many rows: [CTA][2]
+  unsigned long long* tickets;       // few rows: [CTA that begins an item][warp], see pa_open
+  unsigned long long tag;            // this call's
+  unsigned* gave_up;                 // device: waits that gave up so far
   int* status;
 };
 // What a CTA left in the workspace: 0 the end, or the middle, of an item that another CTA began; 1 one that it began and did not end.
@@ -84,7 +87,8 @@ struct PagedStart {
   PagedSeq s;
   int seq, kv_head, q_tile, skip, q_tiles;
   int2 tiles;                        // the item's
-  long long units;
+  int ctas;                          // that have a share
+  long long units, at, total;        // units: of this share, which begins at unit `at`
   long long warp_sum[32];
 };
 // quotient of numbers >= 0 (a division of 64 bits takes some hundred clocks)
@@ -151,6 +155,9 @@ __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
     const long long begin = pa_div(total * blockIdx.x, ctas), end = pa_div(total * (blockIdx.x + 1), ctas);
     if (begin >= before && begin < before + own) {
       long long r = begin - before;
+      S.at = begin;
+      S.total = total;
+      S.ctas = (int)ctas;
       if (per == 1) {
         pa_place_start<KEYS>(J, S, first, s, per_head, r, end - begin);
       } else {
@@ -175,18 +182,22 @@ struct PagedItem {
   int rows;                          // of it
   int lo, hi;                        // key tiles of this CTA
   int slot;                          // -1: the whole item; else its place in the workspace
+  int begun_by, parts;               // CTA that has its beginning, CTAs that have a part (JOIN)
 };
-template <int KEYS>
+template <int KEYS, bool JOIN>
 struct PagedWalk {
   PagedSeq s;
   int seq, kv_head, qt, skip, q_tiles;
   int2 t;                            // the item's key tiles
-  long long left;
+  int ctas;
+  long long left, at, total;
   PagedPart part[2];                 // what the CTA leaves in the workspace
   __device__ __forceinline__ PagedWalk(const PagedJob& J, const PagedStart& S)
-      : s(S.s), seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(S.q_tiles), t(S.tiles), left(S.units) {
+      : s(S.s), seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(S.q_tiles), t(S.tiles), ctas(S.ctas), left(S.units), at(S.at), total(S.total) {
     part[0] = part[1] = PagedPart{0, 1, 0, 0, 0, 0, 0, 0};
   }
+  // the CTA that has unit u: the last c with total * c / ctas <= u
+  __device__ __forceinline__ int cta_of(long long u) const { return (int)pa_div((u + 1) * ctas - 1, total); }
   __device__ __forceinline__ PagedItem next(const PagedJob& J) {
     PagedItem it{};
     while (left > 0 && !it.more) {
@@ -204,9 +215,15 @@ struct PagedWalk {
         it.lo = t.x + from;
         it.hi = t.x + to;
         it.slot = to - from == n ? -1 : from ? 0 : 1;
+        if (JOIN && it.slot >= 0) {
+          const long long first = at - skip + J.begin;
+          it.begun_by = cta_of(first);
+          it.parts = cta_of(first + n - 1) - it.begun_by + 1;
+        }
         if (it.slot >= 0) part[it.slot] = PagedPart{1, to == n, s.row0, it.rows, it.first, kv_head, s.queries, s.keys};
       }
       left -= take;
+      at += take;
       skip = 0;
       if (++qt == q_tiles) {
         qt = 0;
@@ -223,6 +240,21 @@ struct PagedWalk {
     return it;
   }
 };
+// A ticket counts the parts of an item that are there.  It is the call's tag (52 bits) and a number (12), so that nothing has to be cleared in
+// front of a call: whoever is to arrive at it opens it first, which sets it to (tag, 0) if it has another tag, whatever the memory held
+// before.  The last to arrive leaves it cleared, as a captured call that is replayed has the same tag again.  Tags are numbers of a 52-bit sequence that
+// starts anywhere; a launch whose waits gave up, which may leave tickets behind, moves the tags of those after it (J.gave_up).  (Counting by
+// compare and swap alone: 37 CTAs that arrive together took 15 us.)
+__device__ __forceinline__ void pa_open(unsigned long long* ticket, unsigned long long tag) {
+  const unsigned long long old = *(volatile unsigned long long*)ticket;
+  if (old >> 12 != tag) atomicCAS(ticket, old, tag << 12);         // (where that fails, another has opened it)
+}
+// true for the last of `parts`
+__device__ __forceinline__ bool pa_arrive(unsigned long long* ticket, int parts) {
+  const bool last = (int)(atomicAdd(ticket, 1ull) & 4095u) + 1 == parts;
+  if (last) *(volatile unsigned long long*)ticket = 0ull;
+  return last;
+}
 // A row's place among its item's parts in the workspace: tiles of many rows lie 128 apart
 __device__ __forceinline__ int pa_place(const PagedJob& J, int row) { return J.rows > PA_STREAM_ROWS && row >= J.rows / 2 ? row + 128 - J.rows / 2 : row; }
 __device__ __forceinline__ void pa_publish(const PagedJob& J, const PagedPart (&part)[2]) {

@@ -448,7 +448,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         mbar_wait_warp(&B.drain, 0);
       }
     } else if (warp == TL_LOAD) {
-      PagedWalk<KEYS> walk(J, B.start);
+      PagedWalk<KEYS, false> walk(J, B.start);
       const int piece = min(1 << J.page_log, PA_PIECE), pieces = KEYS / piece, page_mask = (1 << J.page_log) - 1;
       phase = 1;
       ip = 1;
