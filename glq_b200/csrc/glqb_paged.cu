@@ -930,6 +930,8 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.begin = !f.tile ? PA_STREAM_BEGIN : f.dp == 64 ? PA_TILE_BEGIN_64 : PA_TILE_BEGIN;
   J.min_units = J.begin + (f.tile ? 2 : 1);
   J.rows = f.tile ? 128 / J.group * J.group * 2 : PA_STREAM_ROWS;
+  J.by_group = pa_divisor(J.group);
+  J.by_rows = pa_divisor(J.rows);
   J.out_wide = lies_on(a->out, 8) && a->out_token % 4 == 0 && a->out_head % 4 == 0;
   J.out_sectors = lies_on(a->out, 32) && a->out_token % 16 == 0 && a->out_head % 16 == 0;
   J.part = (float*)workspace;

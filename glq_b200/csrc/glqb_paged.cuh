@@ -13,6 +13,17 @@ constexpr int PA_STREAM_ROWS = 16, PA_STREAM_KEYS = 64;      // rows of an item,
 constexpr int PA_TILE_ROWS = 256, PA_TILE_KEYS = 128;        // and many (at most: whole queries)
 constexpr float PA_LAZY = 8.0f;                              // a row's weights are relative to a score that its largest exceeds by no more
 
+// Division of 0 .. 2^31 - 1 by one number: q = n * mul >> shift, mul = ceil(2^(31 + l) / d), l = ceil(log2 d) (Granlund and Montgomery 1994).
+struct PagedDivisor {
+  uint32_t mul;
+  int shift;
+};
+inline PagedDivisor pa_divisor(int d) {
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  return PagedDivisor{(uint32_t)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
+}
+
 struct PagedJob {
   const uint16_t* q;
   void* out;
@@ -25,6 +36,7 @@ struct PagedJob {
   int most_keys;                     // columns * page size
   int min_units;                     // units that a CTA takes at least
   int rows;                          // of an item
+  PagedDivisor by_group, by_rows;
   int begin;                         // what beginning an item costs, in key tiles
   bool out_wide, out_sectors;        // rows of out lie on 8, 32 bytes
   float* part;                       // workspace: sums of items that several CTAs share, [CTA][2][rows][padded head_dim]
@@ -55,7 +67,8 @@ __device__ __forceinline__ PagedSeq pa_seq(const PagedJob& J, int i) {
   return s;
 }
 // rows of an item are (query, head of the group) pairs, heads first
-__device__ __forceinline__ int pa_query(const PagedJob& J, int row) { return row / J.group; }
+__device__ __forceinline__ int pa_over(int n, const PagedDivisor& d) { return (int)((unsigned long long)(uint32_t)n * d.mul >> d.shift); }
+__device__ __forceinline__ int pa_query(const PagedJob& J, int row) { return pa_over(row, J.by_group); }
 // keys that query i sees: from .. to - 1
 __device__ __forceinline__ int pa_to(const PagedJob& J, const PagedSeq& s, int i) { return J.causal ? max(0, s.keys - s.queries + i + 1) : s.keys; }
 __device__ __forceinline__ int pa_from(const PagedJob& J, const PagedSeq& s, int i) {
@@ -70,7 +83,7 @@ __device__ __forceinline__ int2 pa_tiles(const PagedJob& J, const PagedSeq& s, i
   const int lo = from / KEYS;
   return make_int2(lo, max(lo + 1, (to + KEYS - 1) / KEYS));
 }
-__device__ __forceinline__ int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return (s.queries * J.group + J.rows - 1) / J.rows; }
+__device__ __forceinline__ int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return pa_over(s.queries * J.group + J.rows - 1, J.by_rows); }
 template <int KEYS>
 __device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq& s) {
   const int n = pa_q_tiles(J, s);
