@@ -594,7 +594,7 @@ def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False, 
         for i, (d, w1, w2) in enumerate(zip(Ls, norm1, norm2)):
             qkv = shards(h, (d["q"], d["k"], d["v"]), w1)             # RMSNorm + q/k/v: one launch
             if context:
-                a = attend(qkv, caches[i])                            # rotation + append: one launch; attention: two
+                a = attend(qkv, caches[i])                            # rotation + append: one launch; attention: one
             else:
                 a = qkv[:, :d["q"].m]                                 # attention stand-in: a view, (1, 2048 / world)
             if world == 1:
@@ -640,7 +640,7 @@ def run_chain_bench(D: Dist, args, steps, n_layers=36, e8=False, dense62=False, 
     hbm, tens, kind = measured_peaks()
     total_bytes = D.sum_int(code_bytes)[0]
     gbs = total_bytes / (ms * 1e-3) / 1e9
-    glq_launches = sum(p.launches for p in ops._PLAN_CACHE.values() if hasattr(p, "launches")) + (3 * n_layers if context else 0)
+    glq_launches = sum(p.launches for p in ops._PLAN_CACHE.values() if hasattr(p, "launches")) + (2 * n_layers if context else 0)
     model = ("decoder layers of the 62-layer dense shape (hidden 5376, intermediate 21504), E8 shell 2 / 3 / 3 stages" if dense62 else
              "Llama-3-8B decoder layers, E8 shell two-stage (4 bpw)" if e8 else "SmolLM3-3B decoder layers, trellis 4 bpw")
     rec = {"workload": "decode_chain_62l" if dense62 else "decode_chain_e8" if e8 else "decode_chain", "metric": METRIC, "value": gbs, "unit": "GB/s", "ms_per_step": ms, "n_gpus": world,

@@ -182,9 +182,11 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
 }
 
 // ---- attention of few rows ------------------------------------------------------------------------
-// Sixteen rows (heads of a group that share a key head, times queries) against tiles of 64 keys: what bounds it is reading the cache.
-// Two warps bring tiles of keys and of values by TMA into a ring, a page's rows per copy, under the 128-byte swizzle (a copy takes its warp 80 clocks, a tile of four
-// pages 1300 where one warp brings both); four warps multiply, each 16
+// Sixteen rows (heads of a group that share a key head, times queries) against tiles of 64 keys: what bounds it is reading the cache.  One token of
+// 131072 keys, fp16, 8 key heads of 128 values: 537 MB in 90.5 us, 5.93 TB/s; 64 sequences of up to 8192: 1.11 GB in 169 to 173 us, 6.4 to 6.6 TB/s.  Small calls are
+// latency: one token of 4096 keys, 8.4 MB over 4 key heads, 11.5 us.
+// Two warps bring tiles of keys and of values by TMA into a ring, a page's rows per copy, under the 128-byte swizzle (one warp that brings both was
+// what a tile of four pages waited for); four warps multiply, each 16
 // keys of every tile for itself (mma.sync: with so few rows the tensor cores are idle either way), with a running maximum and sum of its own, and add up when
 // the item ends.  Scores are scale * log2(e) * q k, weights 2^(score - reference): the reference follows the largest score only when
 // that has grown by more than 2^8, which scales all weights of a row alike and leaves their precision as it is.  Weights are rounded to the values'
@@ -352,9 +354,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
             q[s][a + 2 * b] = there && col < J.head_dim ? *reinterpret_cast<const uint32_t*>(src + col) : 0u;
           }
       }
-      // keys that all rows see, and that any does
-      const int i0 = pa_query(J, it.first), i1 = pa_query(J, it.first + it.rows - 1);
-      const int all_from = pa_from(J, seq, i1), all_to = pa_to(J, seq, i0), any_from = pa_from(J, seq, i0), any_to = pa_to(J, seq, i1);
+      const int all_from = it.all_from, all_to = it.all_to, any_from = it.any_from, any_to = it.any_to;
       float o[STEPS * 2][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
       for (int tile = it.lo; tile < it.hi; ++tile) {
         if (!mbar_wait_warp(&B.full[stage], phase, &B.abort)) { ok = false; break; }
@@ -525,7 +525,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
       __syncwarp();
       if (lane == 0) { mbar_arrive(&B.joined[1]); mbar_arrive(&B.empty[stage]); }
       // An item that several CTAs have a part of: a warp has the same rows in each.  The last to arrive adds them up, all from the workspace, in the
-      // order of the CTAs.  (In a launch of its own behind this one: one token of 4096 keys FIXME us, 12.2.)
+      // order of the CTAs.  (In a launch of its own behind this one: 64 sequences of up to 8192 keys 178 us, 173 so.)
       if (it.slot >= 0 && warp * (128 / DP) < it.rows) {
         __threadfence();
         __syncwarp();
@@ -764,10 +764,14 @@ struct PagedForm {
   int rows, dp, ctas;
   size_t ml, part_of, bytes;        // where the workspace's second and third part begin, and its size
 };
-// Rows of a sequence and key head up to which the streaming kernel runs.
+// Rows of a sequence and key head up to which the streaming kernel runs: those of one of its items.  More rows are several items, that read the cache once
+// each.  64 sequences of 2048 keys, 8 key heads of 128 values, streaming / on the tensor cores: 8 rows 91 / 110 us, 16 95 / 112, 24 171 / 113, 32 172 / 114,
+// 64 331 / 116; one sequence of 16384: 8 rows 21 / 27, 16 29 / 28, 64 41 / 29.
 constexpr int PA_STREAM_MOST = 16;
-// What beginning an item costs a CTA of either kernel, in its key tiles.
-constexpr int PA_STREAM_BEGIN = 2, PA_TILE_BEGIN = 2, PA_TILE_BEGIN_64 = 4;      // (heads of up to 64 values: shorter products)
+// What beginning an item costs a CTA of either kernel, in its key tiles.  (Of 1, 2 and 4: one token of 4096 keys 11.9, 11.5, 12.2 us; prompt of 2048
+// tokens 59.0, 57.1, 58.5; of 8192 489, 471, 481.  Heads of 64 values, of 2, 4 and 6: 24 sequences of mixed lengths 54.9, 53.6, 52.4; prompt of 2048
+// tokens 54 to 58, 60, 60.)
+constexpr int PA_STREAM_BEGIN = 2, PA_TILE_BEGIN = 2;
 PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int sms) {
   PagedForm f;
   const int group = a->heads / c->kv_heads;
@@ -927,7 +931,7 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.clear = a->clear_rest;
   J.scale_log2 = a->scale * 1.4426950408889634f;
   J.most_keys = a->page_columns * c->page_size;
-  J.begin = !f.tile ? PA_STREAM_BEGIN : f.dp == 64 ? PA_TILE_BEGIN_64 : PA_TILE_BEGIN;
+  J.begin = f.tile ? PA_TILE_BEGIN : PA_STREAM_BEGIN;
   J.min_units = J.begin + (f.tile ? 2 : 1);
   J.rows = f.tile ? 128 / J.group * J.group * 2 : PA_STREAM_ROWS;
   J.by_group = pa_divisor(J.group);

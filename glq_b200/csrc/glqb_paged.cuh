@@ -194,6 +194,8 @@ struct PagedItem {
   int seq, kv_head, first;           // first row of the item within the sequence's queries * group
   int rows;                          // of it
   int lo, hi;                        // key tiles of this CTA
+  int all_from, all_to;              // keys that all rows see: all_from .. all_to - 1
+  int any_from, any_to;              // and that any row does
   int slot;                          // -1: the whole item; else its place in the workspace
   int begun_by, parts;               // CTA that has its beginning, CTAs that have a part (JOIN)
 };
@@ -227,6 +229,11 @@ struct PagedWalk {
         it.rows = min(J.rows, s.queries * J.group - it.first);
         it.lo = t.x + from;
         it.hi = t.x + to;
+        const int i0 = pa_query(J, it.first), i1 = pa_query(J, it.first + it.rows - 1);
+        it.all_from = pa_from(J, s, i1);
+        it.all_to = pa_to(J, s, i0);
+        it.any_from = pa_from(J, s, i0);
+        it.any_to = pa_to(J, s, i1);
         it.slot = to - from == n ? -1 : from ? 0 : 1;
         if (JOIN && it.slot >= 0) {
           const long long first = at - skip + J.begin;

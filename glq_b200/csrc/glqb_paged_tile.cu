@@ -10,8 +10,11 @@
 // of its window, may hold anything, and a weight of nothing times NaN is NaN: those rows are set to zero in shared memory.  Rows that only some queries
 // see have to stay; where such a tile holds a value that is not finite, its product is left out of the MMAs and formed one row at a time.
 //
-// What bounds it: of a tile of 128 x 128, the exponentials take 1024 clocks of the special-function units and the two products 1024 of the tensor
-// pipe (head_dim 128).
+// What bounds it: the exponentials of 256 rows x 128 keys take 2048 clocks of the special-function units, 16 a clock, and the two products 2048 of the tensor pipe (head_dim
+// 128).  Either would be enough for 2048 from tile to tile; it takes 3300, as each half of the rows goes its way scores, weights, product, scores, and
+// what its warps do beside the exponentials has to hide behind the other half.  32 heads over 8, bf16: a prompt of 8192 tokens 464 to 471 us
+// (1165 to 1185 TFLOP/s), 512 tokens behind 16384 keys 127 us (1095).  Two halves rather than one tile of 128 rows: then neither unit has work while the other does.
+// Five stages of 32 KB for keys and values (head_dim 128) are what 64 KB of queries leave of shared memory.
 #include "glqb_paged.cuh"
 
 namespace glqb {
@@ -187,8 +190,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
     ok = take(it);
     while (ok && it.more) {
       const PagedSeq seq{it.row0, it.queries, it.keys};
-      const int i0 = pa_query(J, it.first), i1 = pa_query(J, it.first + it.rows - 1);
-      const int item_from = pa_from(J, seq, i1), item_to = pa_to(J, seq, i0);
+      const int item_from = it.all_from, item_to = it.all_to;
       // this thread's row (one behind the tile's last is computed as if it were that one, and not stored)
       const bool mine = t * tile_rows < it.rows;
       const int r = quarter * 32 + lane, row0 = it.first + (mine ? t * tile_rows : 0), rows = mine ? min(tile_rows, it.rows - t * tile_rows) : 1;
@@ -376,8 +378,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
       for (;;) {
         ok = take(it);
         if (!ok || !it.more) break;
-        const PagedSeq seq{it.row0, it.queries, it.keys};
-        const int item_from = pa_from(J, seq, pa_query(J, it.first + it.rows - 1)), item_to = pa_to(J, seq, pa_query(J, it.first));
+        const int item_from = it.all_from, item_to = it.all_to;
         const int tiles = it.rows > J.rows / 2 ? 2 : 1;
         ok = mbar_wait_warp(&B.full[stage], phase, abort);
         for (int t = 0; t < tiles && ok; ++t) {
@@ -523,9 +524,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
       for (;;) {
         ok = take(it);
         if (!ok || !it.more) break;
-        const PagedSeq seq{it.row0, it.queries, it.keys};
-        const int i0 = pa_query(J, it.first), i1 = pa_query(J, it.first + it.rows - 1);
-        const int item_from = pa_from(J, seq, i1), item_to = pa_to(J, seq, i0), any_from = pa_from(J, seq, i0), any_to = pa_to(J, seq, i1);
+        const int item_from = it.all_from, item_to = it.all_to, any_from = it.any_from, any_to = it.any_to;
         for (int tile = it.lo; tile < it.hi; ++tile) {
           // Every stage is waited for and given back, also those with nothing to look at: a wait by parity takes a barrier that is two phases
           // behind for ready, so a warp may not be ahead of the ring, nor the ring ahead of it.

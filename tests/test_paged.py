@@ -282,8 +282,9 @@ def test_operators_refuse_wrong_arguments(monkeypatch):
     assert launched == ["rotary", "paged_append", "paged_attention"]
 
 
-def _model(lengths, new, group, kv_heads, rows, keys, ctas, min_units, causal=True, window=0):
-    """How attention's work is shared out: the list of key tiles, cut into runs.  [(cta, sequence, key head, row tile, lo, hi, slot)]"""
+def _model(lengths, new, group, kv_heads, rows, keys, ctas, begin, least, causal=True, window=0):
+    """How attention's work is shared out: a list of units, `begin` for an item and one per key tile of it, cut into equal runs, of `least`
+    units if there are as many.  The items as (sequence, key head, row tile, lo, hi) and what the CTAs have of them as (cta, item, lo, hi, slot, begun_by, parts)."""
     items = []
     for s, (n, q) in enumerate(zip(lengths, new)):
         for h in range(kv_heads):
@@ -293,35 +294,42 @@ def _model(lengths, new, group, kv_heads, rows, keys, ctas, min_units, causal=Tr
                 to = max(0, n - q + last + 1) if causal else n
                 lo = min(to, max(0, n - q + first + 1 - window) if window else 0) // keys
                 items.append((s, h, t, lo, max(lo + 1, -(-to // keys))))
-    total = sum(i[4] - i[3] for i in items)
-    used = min(ctas, -(-total // min_units))
-    runs, out = [(total * c // used, total * (c + 1) // used) for c in range(used)], []
-    at = 0
-    for s, h, t, lo, hi in items:
-        for c, (a, b) in enumerate(runs):
-            x, y = max(a, at), min(b, at + hi - lo)
+    total = sum(i[4] - i[3] + begin for i in items)
+    used = min(ctas, -(-total // least))
+    cta_of = lambda u: ((u + 1) * used - 1) // total
+    out, at = [], 0
+    for i, (s, h, t, lo, hi) in enumerate(items):
+        for c in range(cta_of(at), cta_of(at + begin + hi - lo - 1) + 1):
+            x = max(0, total * c // used - at - begin)
+            y = min(hi - lo, total * (c + 1) // used - at - begin)
             if x < y:
-                whole = x == at and y == at + hi - lo
-                out.append((c, s, h, t, lo + x - at, lo + y - at, -1 if whole else 1 if x == at else 0))
-        at += hi - lo
+                slot = -1 if y - x == hi - lo else 0 if x else 1
+                first = at + begin
+                out.append((c, i, lo + x, lo + y, slot, cta_of(first), cta_of(first + hi - lo - 1) - cta_of(first) + 1))
+        at += begin + hi - lo
     return items, out
 
 
-@pytest.mark.parametrize("lengths,new", [([4096], [1]), ([100, 3, 900, 0, 64], [1] * 5), ([700, 2], [650, 2]), ([5000], [5000])])
-@pytest.mark.parametrize("rows,keys,ctas,min_units", [(16, 64, 296, 1), (16, 64, 296, 2), (256, 128, 148, 1), (256, 128, 148, 4)])
-def test_runs_cover_the_work_and_parts_find_their_item(lengths, new, rows, keys, ctas, min_units):
-    """Every key tile is taken once, and the part that begins an item finds the others in slot 0 of the CTAs behind it, the last of them ending it."""
-    items, runs = _model(lengths, new, 4, 2, rows, keys, ctas, min_units)
-    slots = {}
-    for c, s, h, t, lo, hi, slot in runs:
+@pytest.mark.parametrize("lengths,new", [([4096], [1]), ([100, 3, 900, 0, 64], [1] * 5), ([700, 2], [650, 2]), ([5000], [5000]), ([31, 64, 1] * 50, [1] * 150)])
+@pytest.mark.parametrize("rows,keys,ctas,begin,least", [(16, 64, 296, 2, 3), (256, 128, 148, 2, 4), (16, 64, 7, 2, 3), (256, 128, 5, 0, 1)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_runs_cover_the_work_and_parts_find_their_item(lengths, new, rows, keys, ctas, begin, least, window):
+    """Every key tile is taken once.  Of an item that is cut, the CTA that all take for its first leaves its part in slot 1 and the others, the CTAs behind
+    it without a gap, theirs in slot 0; all know how many they are."""
+    items, runs = _model(lengths, new, 4, 2, rows, keys, ctas, begin, least, window=window)
+    slots, cut = set(), set()
+    for c, i, lo, hi, slot, begun_by, parts in runs:
         if slot >= 0:
             assert (c, slot) not in slots                        # a CTA leaves at most one part in either slot
-            slots[c, slot] = (s, h, t, lo, hi)
-    for s, h, t, lo, hi in items:
-        mine = [r for r in runs if r[1:4] == (s, h, t)]
-        assert mine[0][4] == lo and mine[-1][5] == hi and all(a[5] == b[4] for a, b in zip(mine, mine[1:]))
-        if len(mine) > 1:
-            c = mine[0][0]
-            assert slots[c, 1][:4] == (s, h, t, lo)
-            assert [r[0] for r in mine] == list(range(c, c + len(mine))) and all(r[6] == 0 for r in mine[1:])
-            assert all(slots[r[0], 0][4] < hi for r in mine[1:-1]) and slots[mine[-1][0], 0][4] == hi
+            slots.add((c, slot))
+    for i, (s, h, t, lo, hi) in enumerate(items):
+        mine = [r for r in runs if r[1] == i]
+        assert mine[0][2] == lo and mine[-1][3] == hi and all(a[3] == b[2] for a, b in zip(mine, mine[1:]))
+        if len(mine) == 1:
+            assert mine[0][4] == -1
+            continue
+        assert [r[4] for r in mine] == [1] + [0] * (len(mine) - 1)
+        assert [r[0] for r in mine] == list(range(mine[0][0], mine[0][0] + len(mine)))
+        assert all(r[5] == mine[0][0] and r[6] == len(mine) for r in mine)
+        assert mine[0][0] not in cut                             # (a ticket is that CTA's: one item that it begins and does not end)
+        cut.add(mine[0][0])
