@@ -1,6 +1,7 @@
 // Rotary positions, appending to a paged cache, and attention of few rows over one: between a decoder's q/k/v and output projections.
 #include "glqb_paged.cuh"
 #include <algorithm>
+#include <utility>
 #include <atomic>
 #include <chrono>
 #include <climits>
@@ -713,6 +714,17 @@ int check_cache(const GlqbPagedCache* c, const char* what) {
   for (const int64_t s : strides)
     if (s < 0 || s % 8 || s >= 1ll << 38) return pg_fail(GLQB_E_INVALID, "%s: a cache's strides are multiples of 8 values", what);
   if (!lies_on(c->keys, 16) || !lies_on(c->values, 16)) return pg_fail(GLQB_E_INVALID, "%s: a cache lies on 16 bytes", what);
+  // no two rows in one place: each stride passes what the smaller ones reach over
+  for (int i = 0; i < 6; i += 3) {
+    std::pair<int64_t, int64_t> by[3] = {{strides[i], c->pages}, {strides[i + 1], c->page_size}, {strides[i + 2], c->kv_heads}};
+    std::sort(by, by + 3);
+    __int128 reach = c->head_dim;
+    for (const auto& d : by)
+      if (d.second > 1) {
+        if (d.first < reach) return pg_fail(GLQB_E_INVALID, "%s: rows of a cache overlap", what);
+        reach += (__int128)d.first * (d.second - 1);
+      }
+  }
   return GLQB_OK;
 }
 
@@ -927,7 +939,7 @@ int glqb_paged_attention(const GlqbPagedCache* c, const GlqbPagedAttention* a, v
   J.group = a->heads / c->kv_heads;
   J.head_dim = c->head_dim;
   J.causal = a->causal;
-  J.window = a->window;
+  J.window = a->window < 1 << 30 ? a->window : 0;        // (no sequence has more keys; so position - window stays within 32 bits)
   J.clear = a->clear_rest;
   J.scale_log2 = a->scale * 1.4426950408889634f;
   J.most_keys = a->page_columns * c->page_size;

@@ -339,7 +339,7 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
     if not fresh and (_meet(at_out, span) or _meet(at_out, kspan) or _meet(at_out, vspan)):
         raise ValueError("glq_b200: out overlaps the queries or the cache")
     if tokens:
-        if span[0] & 15 or qs[0] & 7 or qs[1] & 7:
+        if span[0] & 15 or qs[0] & 7 or qs[1] & 7 or not (qs[0] and qs[1]):          # (strides of 0: expanded)
             query = query.clone(memory_format=torch.contiguous_format)
             qs = query.stride()
         a = _lib.pack_attention(query.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], tokens, pages.data_ptr(), pages.stride(0), lengths.data_ptr(), at_offsets, lengths_wide,

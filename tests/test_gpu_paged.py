@@ -1,5 +1,6 @@
 """Rotary positions, appending to a paged cache and attention over it on the GPU, against the definitions in 64 bits."""
 import math
+import os
 
 import pytest
 import torch
@@ -292,6 +293,62 @@ def test_wide_groups_of_heads(heads, kv, new):
     q, k, v, pages, n, offsets = _batch(_gen(heads), [150, 70 + new], [new, new], kv, heads, 64, 16, HF)
     y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=new)
     _close(y, *O.attend(q, k, v, pages, n, offsets))
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_expanded_queries(new):
+    from glq_b200 import ops
+    _, k, v, pages, n, offsets = _batch(_gen(new), [90, 150], [new, new], 2, 4, 64, 16, BF)
+    one = _randn(_gen(3), 1, 4, 64, dtype=BF)
+    for q in (one.expand(2 * new, 4, 64), _randn(_gen(4), 2 * new, 1, 64, dtype=BF).expand(2 * new, 4, 64)):
+        y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=new)
+        ref, bound = O.attend(q, k, v, pages, n, offsets)
+        _close(y, ref, bound)
+        assert torch.equal(y, ops.paged_attention(q.contiguous(), k, v, pages, n, query_offsets=offsets, max_query_len=new))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new", [2, 60])
+def test_windows_wider_than_any_sequence(new, causal):
+    """Of sequences that are shorter than their queries too, where position - window is far below the first key."""
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(new), [1, new // 2, 300], [new] * 3, 2, 4, 64, 16, HF)
+    want = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, causal=causal)
+    _close(want, *O.attend(q, k, v, pages, n, offsets, causal=causal))
+    for window in (400, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1):
+        assert torch.equal(want, ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, causal=causal, window=window))
+
+
+FIRST = """
+import torch
+from glq_b200 import ops
+table = ops.rotary_table(64)
+k, v = (torch.zeros(8, 16, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+x = torch.randn(NEW, 8, 64, dtype=torch.bfloat16, device="cuda")
+at = torch.arange(NEW, device="cuda")
+pages = torch.arange(8, device="cuda", dtype=torch.int32)[None]
+n, offsets = torch.tensor([NEW], device="cuda"), torch.tensor([0, NEW], device="cuda")
+def step():
+    q = ops.paged_append(x[:, 4:6], x[:, 6:], k, v, at, positions=at, table=table, query=x[:, :4])
+    return ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, max_query_len=NEW)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = step()
+graph.replay()
+assert torch.equal(y, step()) and y.abs().sum() > 0
+ops.check_device_status()
+print("right")
+"""
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_first_call_of_a_process_is_captured(new):
+    import subprocess
+    import sys
+    run = subprocess.run([sys.executable, "-c", FIRST.replace("NEW", str(new))], capture_output=True, text=True, timeout=300,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert run.returncode == 0 and "right" in run.stdout, run.stderr[-2000:]
 
 
 def test_no_pages_at_all():

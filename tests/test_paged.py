@@ -107,6 +107,8 @@ def test_c_entries_refuse_before_any_cuda_call(lib):
         refused(call(c=dict(values=None)), -1, "null")
         refused(call(c=dict(key_row=124)), -1, "multiples of 8")
         refused(call(c=dict(values=p + 8)), -1, "16 bytes")
+        for wrong in (dict(key_page=0), dict(value_row=0), dict(key_head=56), dict(value_row=64), dict(key_page=2040), dict(key_page=128, key_row=1024)):
+            refused(call(c=wrong), -1, "overlap")
     refused(append(dtype=0), -1, "type")
     refused(append(tokens=-1), -1, "-1 tokens")
     refused(append(slots=None), -1, "null")
@@ -280,6 +282,13 @@ def test_operators_refuse_wrong_arguments(monkeypatch):
     ops.paged_append(new, new, k, v, n3, positions=n3, table=table, query=x)
     ops.paged_attention(*ok)
     assert launched == ["rotary", "paged_append", "paged_attention"]
+    # expanded queries go to the device as copies, which every kernel can read
+    packed = []
+    real = paged._lib.pack_attention
+    monkeypatch.setattr(paged._lib, "pack_attention", lambda *a: packed.append(a[2:4]) or real(*a))
+    ops.paged_attention(x[:, :1].expand(3, 4, 64), *ok[1:])
+    ops.paged_attention(x[:1].expand(3, 4, 64), *ok[1:])
+    assert packed == [(256, 64)] * 2
 
 
 def _model(lengths, new, group, kv_heads, rows, keys, ctas, begin, least, causal=True, window=0):
