@@ -219,25 +219,32 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// parts of a row, added up
+// parts of a row, added up: 4 Q of its values
+template <int Q>
 struct Joined {
-  float4 v;
+  float4 v[Q];
   float most, sum;
+  __device__ __forceinline__ Joined() : most(-INFINITY), sum(0.0f) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   template <int N>
-  __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&u)[N]) {
+  __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&u)[N][Q]) {
     float now = most;
 #pragma unroll
     for (int k = 0; k < N; ++k) now = fmaxf(now, ml[k].x);
     const float f = now == -INFINITY ? 1.0f : pa_exp2(most - now);
     sum *= f;
-    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) { v[q].x *= f; v[q].y *= f; v[q].z *= f; v[q].w *= f; }
     most = now;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;        // (no key of its own: nothing in its sums)
       const float w = pa_exp2(ml[k].x - now);
       sum += w * ml[k].y;
-      v.x += w * u[k].x; v.y += w * u[k].y; v.z += w * u[k].z; v.w += w * u[k].w;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) { v[q].x += w * u[k][q].x; v[q].y += w * u[k][q].y; v[q].z += w * u[k][q].z; v[q].w += w * u[k][q].w; }
     }
   }
 };
@@ -536,24 +543,24 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
           __threadfence();
           for (int i = threadIdx.x; i < it.rows * (DP / 4); i += ST_WARPS * 32) {
             const int row = i / (DP / 4), col = i % (DP / 4) * 4;
-            Joined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+            Joined<1> j;
             for (int p0 = 0; p0 < it.parts; p0 += 8) {
               float2 ml[8];
-              float4 u[8];
+              float4 u[8][1];
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 ml[k] = make_float2(-INFINITY, 0.0f);
-                u[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                u[k][0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (p0 + k < it.parts) {
                   const long long at = (2ll * (it.begun_by + p0 + k) + (p0 + k == 0)) * ROWS + row;
                   ml[k] = __ldcg(J.part_ml + at);
-                  u[k] = __ldcg(reinterpret_cast<const float4*>(J.part + at * DP + col));
+                  u[k][0] = __ldcg(reinterpret_cast<const float4*>(J.part + at * DP + col));
                 }
               }
               j.add(ml, u);
             }
             const float f = pa_row_factor(J, seq, it.first + row, j.sum);
-            if (col < J.head_dim) pa_store4<T>(J, pa_out_row(J, it.row0, it.kv_head, it.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
+            if (col < J.head_dim) pa_store4<T>(J, pa_out_row(J, it.row0, it.kv_head, it.first + row), col, make_float4(j.v[0].x * f, j.v[0].y * f, j.v[0].z * f, j.v[0].w * f));
           }
           __syncwarp();
         }
@@ -568,15 +575,17 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
 
 // ---- what several CTAs have of an item of many rows, together -------------------------------------
 // The parts of an item that CTA blockIdx.x began and did not end are that CTA's, then those of the CTAs behind it up to the one that ended
-// the item.  A block has 16 rows, a warp two at once.  The order is the same in every call.  Bound by latency: a block reads what a CTA has left, then two
-// rows' parts.  (24 sequences of mixed lengths: 7 us behind 49 of the products; 128 rows to a block of 16 warps 9, 32 rows to one of eight, four at once, 11.
+// the item.  A lane has 16 values of one row, a warp 32 rows, whose parts it reads a kilobyte at once.  The order is the same in every call.  Bound by latency and by
+// blocks that wait for others to end: what a CTA has left, then the parts.  (Parts with a row's values one behind the other, a warp for two rows: prompt of 2048
+// tokens 58.5 us, 52.1 so, 24 sequences of mixed lengths 55.0, 49.3; blocks of eight warps 52.8 and 49.4, three parts at once 53.9 and 50.1, one 53.5 and 51.0.
 // One CTA could not do it in the first kernel, as it does with few rows: 256 rows of 18 CTAs are 2.4 MB.)
-constexpr int CB_WARPS = 8, CB_ROWS = 2 * CB_WARPS, CB_BATCH = 2;
+constexpr int CB_WARPS = 4, CB_BATCH = 2;
+constexpr int cb_blocks(int dp) { return PA_TILE_ROWS / 32 * (dp / 16) / CB_WARPS; }        // of an item
 template <typename T, int DP>
-__global__ void __launch_bounds__(CB_WARPS * 32, 4) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
+__global__ void __launch_bounds__(CB_WARPS * 32, 6) paged_combine_kernel(const __grid_constant__ PagedJob J, int ctas) {
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, col = lane * 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
   // (the first parts' ends are asked for before it is known whether this CTA has left a beginning)
   const PagedPart lead = J.part_of[2 * c + 1];
   auto ends = [&](int parts) {
@@ -595,39 +604,42 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 4) paged_combine_kernel(const _
   int parts = 1;
   while (!end) end = ends(parts += 32);
   parts += __ffs(end);
-  auto part_at = [&](int p, int row) { return (p ? 2ll * (c + p) : 2ll * c + 1) * PA_TILE_ROWS + pa_place(J, row); };
-  auto store = [&](int row, const Joined& j) {
-    if (col >= J.head_dim) return;
-    const float f = pa_row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, j.sum);
-    pa_store4<T>(J, pa_out_row(J, lead.row0, lead.kv_head, lead.first + row), col, make_float4(j.v.x * f, j.v.y * f, j.v.z * f, j.v.w * f));
-  };
-  const int row0 = blockIdx.y * CB_ROWS + warp, last = min(lead.rows, (int)(blockIdx.y + 1) * CB_ROWS);
-  if (row0 >= last) return;
-  Joined j[2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) j[n] = Joined{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  const int task = (int)blockIdx.y * CB_WARPS + warp, col = task % (DP / 16) * 16, r = task / (DP / 16) * 32 + lane;      // (r: 128 to a half)
+  const int half = J.rows / 2, row = r < 128 ? r : half + r - 128;
+  if ((r & 127) >= half || row >= lead.rows || col >= J.head_dim) return;
+  Joined<4> j;
   for (int p0 = 0; p0 < parts; p0 += CB_BATCH) {
-    float2 ml[2][CB_BATCH];
-    float4 u[2][CB_BATCH];
+    float2 ml[CB_BATCH];
+    float4 u[CB_BATCH][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int k = 0; k < CB_BATCH; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-      for (int k = 0; k < CB_BATCH; ++k) {
-        const int row = row0 + n * CB_WARPS;
-        ml[n][k] = make_float2(-INFINITY, 0.0f);
-        u[n][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (p0 + k < parts && row < last) {
-          const long long at = part_at(p0 + k, row);
-          ml[n][k] = J.part_ml[at];
-          if (col < DP) u[n][k] = *reinterpret_cast<const float4*>(J.part + at * DP + col);
-        }
+      for (int q = 0; q < 4; ++q) u[k][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p0 + k < parts) {
+        const int slot = 2 * (c + p0 + k) + (p0 + k == 0);
+        ml[k] = J.part_ml[(long long)slot * PA_TILE_ROWS + r];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) load8(J.part + pa_part_at<DP>(slot, r, col / 8 + q), u[k][2 * q], u[k][2 * q + 1]);
       }
-#pragma unroll
-    for (int n = 0; n < 2; ++n) j[n].add(ml[n], u[n]);
+    }
+    j.add(ml, u);
   }
+  const float f = pa_row_factor(J, PagedSeq{lead.row0, lead.queries, lead.keys}, lead.first + row, j.sum);
+  const long long at = pa_out_row(J, lead.row0, lead.kv_head, lead.first + row);
+  if (J.out_sectors && col + 16 <= J.head_dim) {
+    uint32_t y[8];
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
-    if (row0 + n * CB_WARPS < last) store(row0 + n * CB_WARPS, j[n]);
+    for (int q = 0; q < 4; ++q) {
+      y[2 * q] = pa_pack<T>(j.v[q].x * f, j.v[q].y * f);
+      y[2 * q + 1] = pa_pack<T>(j.v[q].z * f, j.v[q].w * f);
+    }
+    store8(reinterpret_cast<uint16_t*>(J.out) + at + col, y);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (col + 4 * q < J.head_dim) pa_store4<T>(J, at, col + 4 * q, make_float4(j.v[q].x * f, j.v[q].y * f, j.v[q].z * f, j.v[q].w * f));
+  }
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -818,7 +830,7 @@ cudaError_t attention_launch(const PagedJob& J, const PagedForm& f, const CUtens
   const cudaError_t e = paged_tile_launch(J, __is_same(T, __nv_bfloat16), mq, mk, mv, f.ctas, stream);
   if (e != cudaSuccess) return e;
   constexpr auto CB = paged_combine_kernel<T, DP>;
-  return paged_launch<CB>(CB, dim3((unsigned)f.ctas, PA_TILE_ROWS / CB_ROWS), CB_WARPS * 32, 0, stream, J, f.ctas);
+  return paged_launch<CB>(CB, dim3((unsigned)f.ctas, cb_blocks(DP)), CB_WARPS * 32, 0, stream, J, f.ctas);
 }
 }  // namespace
 }  // namespace glqb

@@ -275,8 +275,19 @@ __device__ __forceinline__ bool pa_arrive(unsigned long long* ticket, int parts)
   if (last) *(volatile unsigned long long*)ticket = 0ull;
   return last;
 }
-// A row's place among its item's parts in the workspace: tiles of many rows lie 128 apart
-__device__ __forceinline__ int pa_place(const PagedJob& J, int row) { return J.rows > PA_STREAM_ROWS && row >= J.rows / 2 ? row + 128 - J.rows / 2 : row; }
+// 32 bytes at once
+__device__ __forceinline__ void store8(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void load8(const float* p, float4& a, float4& b) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w), "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "l"(p) : "memory");
+}
+// Where eight values of a row are in a part of many rows: row r (128 to a half), values 8 g and up.  A warp that has 32 rows writes, and reads, a
+// kilobyte of them at once.
+template <int DP>
+__device__ __forceinline__ long long pa_part_at(int slot, int r, int g) {
+  return (long long)slot * PA_TILE_ROWS * DP + (((r >> 7) * (DP / 8) + g) * 128 + (r & 127)) * 8;
+}
 __device__ __forceinline__ void pa_publish(const PagedJob& J, const PagedPart (&part)[2]) {
   J.part_of[2 * blockIdx.x] = part[0];
   J.part_of[2 * blockIdx.x + 1] = part[1];

@@ -91,10 +91,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 32 bytes at once
-__device__ __forceinline__ void store8(void* p, const uint32_t* r) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
 struct f2 { uint64_t v; };
 __device__ __forceinline__ f2 f2_of(float a, float b) {
   f2 r;
@@ -325,8 +321,8 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
         // A thread has a row: 32 bytes of it at once are whole sectors.  (8 bytes at once took 12,000 clocks per item.)
         const bool there = r < rows;
         const float f = it.slot < 0 ? pa_row_factor(J, seq, row, l) : 1.0f;
-        const long long at = pa_out_row(J, it.row0, it.kv_head, row), place = (2ll * blockIdx.x + max(it.slot, 0)) * PA_TILE_ROWS + t * 128 + r;
-        if (it.slot >= 0 && there) J.part_ml[place] = make_float2(m * c, l);
+        const long long at = pa_out_row(J, it.row0, it.kv_head, row);
+        if (it.slot >= 0 && there) J.part_ml[(2ll * blockIdx.x + it.slot) * PA_TILE_ROWS + t * 128 + r] = make_float2(m * c, l);
         uint32_t o[DP / 32][32];
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n) tmem_ld32(sums + n * 32u, o[n]);
@@ -335,7 +331,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
 #pragma unroll
           for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) store8(J.part + place * DP + n * 32 + k, o[n] + k);
+            for (int k = 0; k < 32; k += 8) store8(J.part + pa_part_at<DP>(2 * blockIdx.x + it.slot, t * 128 + r, n * 4 + k / 8), o[n] + k);
         } else if (there) {
 #pragma unroll
           for (int n = 0; n < DP / 32; ++n) {
