@@ -12,8 +12,8 @@
 //
 // What bounds it: the exponentials of 256 rows x 128 keys take 2048 clocks of the special-function units, 16 a clock, and the two products 2048 of the tensor pipe (head_dim
 // 128).  Either would be enough for 2048 from tile to tile; it takes 3300, as each half of the rows goes its way scores, weights, product, scores, and
-// what its warps do beside the exponentials has to hide behind the other half.  32 heads over 8, bf16: a prompt of 8192 tokens 464 to 471 us
-// (1165 to 1185 TFLOP/s), 512 tokens behind 16384 keys 127 us (1095).  Two halves rather than one tile of 128 rows: then neither unit has work while the other does.
+// what its warps do beside the exponentials has to hide behind the other half.  32 heads over 8, bf16: a prompt of 8192 tokens 464 us
+// (1185 TFLOP/s), 512 tokens behind 16384 keys 124 us (1125), with the parts joined.  Two halves rather than one tile of 128 rows: then neither unit has work while the other does.
 // Five stages of 32 KB for keys and values (head_dim 128) are what 64 KB of queries leave of shared memory.
 #include "glqb_paged.cuh"
 
