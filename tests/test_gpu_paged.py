@@ -467,6 +467,22 @@ def test_long_chunks(dtype, window, heads, kv, dim, lengths, new):
 
 
 # ---- together -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 72), (6, 2, 8), (5, 1, 120), (3, 3, 40), (20, 1, 96)])
+@pytest.mark.parametrize("lengths,new", [([1700], [60]), ([900, 64, 1300, 5], [300, 1, 17, 5])])
+def test_items_of_several_parts_in_heads_of_any_width(dtype, heads, kv, dim, lengths, new):
+    """Results whose rows begin on 32 bytes, and in between."""
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(dim), lengths, new, kv, heads, dim, 16, dtype)
+    ref, bound = O.attend(q, k, v, pages, n, offsets)
+    y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets)
+    _close(y, ref, bound)
+    wide = torch.zeros(q.shape[0], heads, dim + 4, dtype=dtype, device="cuda")
+    out = wide[:, :, :dim]
+    ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, out=out)
+    assert torch.equal(out, y) and not wide[:, :, dim:].any()
+
+
 def test_prompt_then_decoding_steps():
     """A prompt in two chunks and decoding steps through append and attention, as a decoder runs them, against attention over the whole."""
     from glq_b200 import ops
