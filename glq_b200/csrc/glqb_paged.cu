@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
 // keys of every tile for itself (mma.sync: with so few rows the tensor cores are idle either way), with a running maximum and sum of its own, and add up when
 // the item ends.  Scores are scale * log2(e) * q k, weights 2^(score - reference): the reference follows the largest score only when
 // that has grown by more than 2^8, which scales all weights of a row alike and leaves their precision as it is.  Weights are rounded to the values'
-// type for the product, as the tensor cores take them; sums stay in fp32.
+// type for the product, as the tensor cores take them (fp16 ones are 2^7 larger: pa_up); sums stay in fp32.
 constexpr int ST_WARPS = 4, ST_THREADS = (ST_WARPS + 2) * 32, ST_ITEMS = 4;
 template <int DP>
 struct StreamShape {
@@ -410,7 +410,7 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
             }
           }
 #pragma unroll
-          for (int a = 0; a < 2; ++a) less[a] = m[a] == -INFINITY ? 0.0f : m[a];
+          for (int a = 0; a < 2; ++a) less[a] = m[a] == -INFINITY ? 0.0f : m[a] - pa_up<T>();
           uint32_t p[4];
 #pragma unroll
           for (int n = 0; n < 2; ++n)

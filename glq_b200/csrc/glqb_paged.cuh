@@ -325,6 +325,10 @@ __device__ __forceinline__ float2 pa_unpack(uint32_t two) {
   if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2*>(&two));
   else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
 }
+// Weights are 2^(score - reference + this), of which a row's sums, its parts and their sums all have the factor, so that the quotient loses it.  fp16's
+// smallest number is 2^-24: without it what weighs 2^-25 of a row's strongest key is nothing in the sum over the values and something in the sum that divides it
+// (131,071 such keys beside a strong one: 0.4 % of the result).  PA_LAZY more is 2^15, of at most 65,504.  bf16 has fp32's exponents.
+template <typename T> __device__ __forceinline__ constexpr float pa_up() { return __is_same(T, __half) ? 7.0f : 0.0f; }
 // four columns of a row of the result
 template <typename T>
 __device__ __forceinline__ void pa_store4(const PagedJob& J, long long at, int col, float4 v) {

@@ -244,7 +244,7 @@ paged_tile_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ CU
               }
             }
           }
-          const float less = m == -INFINITY ? 0.0f : m * c;
+          const float less = m == -INFINITY ? 0.0f : m * c - pa_up<T>();
           const f2 c2 = f2_of(c, c), less2 = f2_of(-less, -less);
           f2 sum[2] = {f2_of(l, 0.0f), f2_of(0.0f, 0.0f)};
 #pragma unroll

@@ -566,3 +566,76 @@ def test_refusals():
         ops.rotary(q, torch.zeros(3, dtype=torch.int64, device="cuda"), table)
     with pytest.raises(ValueError, match="overlaps"):
         ops.rotary(q[:1], torch.zeros(1, dtype=torch.int64, device="cuda"), table, out=torch.as_strided(q, (1, 4, 64), (256, 64, 1), 8))
+
+
+# ---- weights far below a row's largest ----------------------------------------------------------------------------
+def _within(y, q, k, v, pages, lengths, offsets, window=0, what=""):
+    """Each value against 64 bits on the device, within what its own weights allow.  A weight is rounded by U of itself or, of fp16's
+    subnormal numbers, by half a step: weights are held as 2^7 times those relative to a score that is no larger than the row's
+    largest, so 2^-25 is 2^-32 of the largest at most (bf16 has fp32's exponents).  The result is rounded by U.  In fp32: scores with
+    `dim` products and sums, 2^-23 each where the tensor cores cut off, in a weight and in their sum; no sum is longer than the
+    keys, a step of it off by 2^-24 of what it has, in the values' sum and in the weights'."""
+    g, dtype = q.shape[1] // k.shape[2], v.dtype
+    floor = 2.0 ** -32 if dtype == HF else 0.0
+    worst = -math.inf
+    for i, n in enumerate(lengths.tolist()):
+        a, b = int(offsets[i]), int(offsets[i + 1])
+        ids = pages[i, :-(-n // k.shape[1])].long()
+        at, key = torch.arange(n - (b - a), n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+        seen = (key <= at) & ((key > at - window) if window else True)
+        for h in range(k.shape[2]):
+            kk, vv = (c[ids][:, :, h].flatten(0, 1)[:n].double() for c in (k, v))
+            qq, own = q[a:b, h * g:(h + 1) * g].double(), y[a:b, h * g:(h + 1) * g].double()
+            scale = q.shape[2] ** -0.5
+            z = torch.where(seen, torch.einsum("qgd,kd->gqk", qq, kk) * scale, -math.inf)
+            weight = torch.exp(z - z.amax(-1, keepdim=True))
+            total = weight.sum(-1).transpose(0, 1)[..., None]
+            ref, reach, far = (torch.einsum("gqk,kd->qgd", w, x) / total for w, x in ((weight, vv), (weight, vv.abs()), (seen.expand(g, -1, -1).double(), vv.abs())))
+            size = torch.einsum("qgd,kd->gqk", qq.abs(), kk.abs()).masked_fill(~seen, 0.0).amax(-1).transpose(0, 1)[..., None] * scale
+            fp32 = 2 * size * (q.shape[2] + 4) * 2.0 ** -23 + 2 * n * 2.0 ** -24 + 2.0 ** -19
+            bound = (U[dtype] + fp32) * reach + floor * far + U[dtype] * (ref.abs() + (U[dtype] + fp32) * reach + floor * far)
+            worst = max(worst, float(((own - ref).abs() - bound).max()))
+            assert bool(torch.isfinite(own).all()) and bool(((own - ref).abs() <= bound).all()), (what, i, h, worst)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("new", [1, 9])
+@pytest.mark.parametrize("seqs", [1, 300])
+@pytest.mark.parametrize("strong", [0, 70000, -10])
+@pytest.mark.parametrize("below", [14.0, 20.0, 24.4, 25.4, 28.0])
+def test_one_strong_key_and_many_weak_ones(dtype, new, seqs, strong, below):
+    """One key has most of a row's weight and values of 0, 131,071 others 2^-below of it each and values of 1: theirs is the result, up to 0.9.
+    Of one sequence each CTA has some keys, of 300 (that name the same pages) all or half of an item's."""
+    from glq_b200 import ops
+    n, dim, size = 131072, 64, 64
+    k = torch.zeros(n // size, size, 1, dim, device="cuda", dtype=dtype)
+    v = torch.ones_like(k)
+    k.view(n, dim)[strong, 0] = below * math.log(2.0)
+    v.view(n, dim)[strong] = 0.0
+    q = torch.zeros(seqs * new, 4, dim, device="cuda", dtype=dtype)
+    q[..., 0] = math.sqrt(dim)                                                     # (scores are the keys' first values)
+    pages = torch.randperm(n // size, generator=_gen(1), device="cuda").to(torch.int32)[None]
+    k[pages[0].long()], v[pages[0].long()] = k.clone(), v.clone()
+    lengths, offsets = torch.full((seqs,), n, device="cuda"), torch.arange(seqs + 1, device="cuda") * new
+    y = ops.paged_attention(q, k, v, pages.expand(seqs, -1), lengths, query_offsets=offsets, max_query_len=new)
+    for i in sorted({0, 1 % seqs, seqs // 4, seqs // 2, seqs - 1}):
+        mine = y[i * new:(i + 1) * new]
+        _within(mine, q[:new], k, v, pages, lengths[:1], offsets[:2], what=(i, float(mine.float().mean())))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("new", [1, 9])
+@pytest.mark.parametrize("above", [3.0, 7.9, 8.1, 15.9, 40.0])
+def test_scores_that_grow_along_the_keys(dtype, new, above):
+    """Later keys' weights are up to 2^above of the first one's: within the type, however far the reference lags behind."""
+    from glq_b200 import ops
+    n, dim = 5000, 64
+    g = _gen(int(above))
+    k, v = torch.zeros(1, 8192, 1, dim, device="cuda", dtype=dtype), _randn(g, 1, 8192, 1, dim, dtype=dtype)
+    step = torch.where(torch.arange(8192, device="cuda") % 3000 < 1500, 0.0, above * math.log(2.0))
+    k[0, :, 0, 0] = step.to(dtype)
+    q = torch.zeros(new, 4, dim, device="cuda", dtype=dtype)
+    q[..., 0] = math.sqrt(dim)
+    pages, lengths, offsets = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([n], device="cuda"), torch.tensor([0, new], device="cuda")
+    y = ops.paged_attention(q, k, v, pages, lengths, query_offsets=offsets, max_query_len=new)
+    _within(y, q, k, v, pages, lengths, offsets)
