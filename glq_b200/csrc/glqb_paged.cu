@@ -740,6 +740,41 @@ int check_cache(const GlqbPagedCache* c, const char* what) {
   return GLQB_OK;
 }
 
+// Is |at + sum of e_i strides[i]| below `dim` for some |e_i| < counts[i]?  Strides pass what the ones behind them reach over, so that of each two e come into question.
+bool rows_meet(__int128 at, const std::pair<int64_t, int64_t>* by, int n, int dim) {
+  if (n == 0) return at < dim && at > -dim;
+  const __int128 s = by->first, most = by->second - 1;
+  const __int128 low = -(at >= 0 ? (at + s - 1) / s : at / s);       // floor(-at / s)
+  for (__int128 e = low; e <= low + 1; ++e)
+    if (e >= -most && e <= most && rows_meet(at + e * s, by + 1, n - 1, dim)) return true;
+  return false;
+}
+// Have keys and values (check_cache) an address in common?  They may lie between one another, as those of one tensor do.
+bool caches_meet(const GlqbPagedCache* c) {
+  const __int128 at = ((__int128) reinterpret_cast<intptr_t>(c->values) - reinterpret_cast<intptr_t>(c->keys)) / 2;
+  const int64_t k[3] = {c->key_page, c->key_row, c->key_head}, v[3] = {c->value_page, c->value_row, c->value_head}, n[3] = {c->pages, c->page_size, c->kv_heads};
+  std::pair<int64_t, int64_t> by[3];
+  int used = 0;
+  bool alike = true;
+  __int128 k_page = c->head_dim, v_page = c->head_dim;               // what a page reaches over
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] < 2) continue;
+    alike = alike && k[i] == v[i];
+    by[used++] = {k[i], n[i]};
+    if (i) k_page += (__int128)k[i] * (n[i] - 1), v_page += (__int128)v[i] * (n[i] - 1);
+  }
+  if (alike) {
+    std::sort(by, by + used, [](const auto& a, const auto& b) { return a.first > b.first; });
+    return rows_meet(at, by, used, c->head_dim);
+  }
+  const __int128 all = (__int128)(c->pages - 1);
+  if (at >= k_page + all * k[0] || at + v_page + all * v[0] <= 0) return false;
+  // rows or heads in another order: apart if whole pages are
+  if (c->pages < 2 || k[0] != v[0] || k_page > k[0] || v_page > k[0]) return true;
+  const __int128 r = (at % k[0] + k[0]) % k[0];
+  return r < k_page || r + v_page > k[0];
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
@@ -880,6 +915,7 @@ int glqb_paged_append(const GlqbPagedCache* c, const GlqbPagedAppend* a, const G
     return pg_fail(GLQB_E_INVALID, "%s: values that are not aligned", what);
   if (r)
     if (const int rc = check_rotary(r, c->head_dim, a->positions, a->positions_are_int64, what)) return rc;
+  if (caches_meet(c)) return pg_fail(GLQB_E_INVALID, "%s: keys and values of the cache share addresses", what);
   const PagedDevice* d = pg_device();
   if (!d) return pg_fail(GLQB_E_CUDA, "%s: no device", what);
   RotJob J = {};

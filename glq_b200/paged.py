@@ -252,7 +252,7 @@ def _cache(keys, values):
 def paged_append(key, value, key_cache, value_cache, slots, *, positions=None, table: Optional[Rotary] = None, query=None, out=None):
     """Puts the keys and values (tokens, kv_heads, head_dim) of new tokens into the cache, in place: token t's into row ``slots[t]`` =
     page * page_size + row (int32 or int64); a slot outside the cache, -1 for one, leaves the cache alone, as for tokens that pad a batch.
-    The slots within the cache are all different.  With ``table`` and ``positions`` (tokens,) the keys are rotated on the way, and so is ``query``
+    The slots within the cache are all different, and keys and values do not share addresses (they may lie between one another's, as in one tensor).  With ``table`` and ``positions`` (tokens,) the keys are rotated on the way, and so is ``query``
     (tokens, heads, head_dim) if it is given: to a new tensor or to ``out`` (the query itself too), which is returned.  Keys, values and
     queries are of the cache's type, or fp32."""
     desc, index, cache, dtype, kspan, vspan = _cache(key_cache, value_cache)

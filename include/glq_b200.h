@@ -373,7 +373,8 @@ typedef struct GlqbPagedCache {
 } GlqbPagedCache;
 
 /* key and value (tokens, kv_heads, head_dim), fp32 or of the cache's type, into rows slots[t] (page * page_size + row) of the cache; a slot
- * outside the cache, as a padding token's is, leaves it alone.  Slots within the cache are all different.  r: null, or the rotation of
+ * outside the cache, as a padding token's is, leaves it alone.  Slots within the cache are all different, and so are the addresses of its
+ * keys and values (in one tensor they may lie between one another).  r: null, or the rotation of
  * keys, and of `heads` heads of query to query_out (same type as key; query NULL: none), by positions. */
 typedef struct GlqbPagedAppend {
   const void *key, *value, *query;

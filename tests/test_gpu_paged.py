@@ -639,3 +639,15 @@ def test_scores_that_grow_along_the_keys(dtype, new, above):
     pages, lengths, offsets = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([n], device="cuda"), torch.tensor([0, new], device="cuda")
     y = ops.paged_attention(q, k, v, pages, lengths, query_offsets=offsets, max_query_len=new)
     _within(y, q, k, v, pages, lengths, offsets)
+
+
+def test_keys_and_values_in_one_place():
+    """Attention may read one tensor as both; append may not write it as both."""
+    from glq_b200 import ops
+    q, k, _, pages, n, offsets = _batch(_gen(2), [50, 60], [1, 20], 2, 4, 64, 16, BF)
+    _close(ops.paged_attention(q, k, k, pages, n, query_offsets=offsets), *O.attend(q, k, k, pages, n, offsets))
+    new, slots, before = k[:1, 0].clone(), torch.zeros(1, dtype=torch.int64, device="cuda"), k.clone()
+    for values in (k, torch.as_strided(k.flatten()[64:], (k.shape[0] - 1, *k.shape[1:]), k.stride())):
+        with pytest.raises(RuntimeError, match="share addresses"):
+            ops.paged_append(new, new, k[:len(values)], values, slots)
+    assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))

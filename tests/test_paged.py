@@ -132,6 +132,48 @@ def test_c_entries_refuse_before_any_cuda_call(lib):
     assert attention(tokens=0, out=None) == 0
 
 
+def _append_refusal(lib, keys, values, key_strides, value_strides, pages, size, heads, dim):
+    """What a call says of caches at these addresses.  It has too many tokens for a launch, wherever it runs."""
+    from glq_b200 import _lib
+    cache = _lib.PagedCacheDesc(keys, values, *key_strides, *value_strides, pages, size, heads, dim, 1)
+    a = _lib.PagedAppendDesc(key=4096, value=4096, key_token=128, key_head=64, value_token=128, value_head=64, tokens=1 << 40, slots=4096, slots_are_int64=1, dtype=1)
+    assert lib.glqb_paged_append(ctypes.byref(cache), ctypes.byref(a), None, None) < 0
+    return lib.glqb_last_error().decode()
+
+
+def test_append_refuses_keys_and_values_in_one_place(lib):
+    """Two threads would write each value.  Against every address of both, for keys and values that lie between one another in all manners."""
+    import itertools
+    import random
+    rng = random.Random(3)
+    p, found = 1 << 40, {True: 0, False: 0}
+
+    def taken(strides, counts, dim, at):
+        return {at + sum(i * s for i, s in zip(ix, strides)) + e for ix in itertools.product(*(range(n) for n in counts)) for e in range(dim)}
+
+    for trial in range(600):
+        counts, dim = (rng.randint(1, 3), 8, rng.randint(1, 3)), rng.choice([8, 16])
+        order, strides, reach = rng.sample(range(3), 3), [0, 0, 0], dim
+        for i in order:
+            strides[i] = reach + 8 * rng.choice([0, 0, 1, dim // 8, reach // 8])
+            reach = strides[i] * (counts[i] - 1) + reach if counts[i] > 1 else reach
+        shift = 8 * rng.randint(-reach // 8 - 2, reach // 8 + 2) if rng.random() < 0.6 else rng.choice(strides) - rng.choice([0, 0, 8]) * rng.choice([-1, 1])
+        shift = shift // 8 * 8
+        mine = taken(strides, counts, dim, 0)
+        meet = any(a + shift in mine for a in mine)
+        said = _append_refusal(lib, p, p + 2 * shift, strides, strides, *counts, dim)
+        assert ("share" in said) == meet, (counts, dim, strides, shift, said)
+        found[meet] += 1
+    assert min(found.values()) > 100
+    # of different strides: pages that lie beside one another's, or caches that do
+    rows, heads = (4096, 128, 64), (4096, 64, 1024)
+    for shift, meet in ((2048, False), (-2048, False), (2048 + 4096 * 3, False), (1024, True), (-1024, True), (0, True), (4096 * 10, False), (4096 * 9 + 2048, False), (4096 * 9 - 64, True), (-4096 * 10, False)):
+        assert ("share" in _append_refusal(lib, p, p + 2 * shift, rows, heads, 10, 16, 2, 64)) == meet, shift
+    far = (1 << 37, 128, 64)                                      # (addresses beyond 64 bits)
+    assert "share" in _append_refusal(lib, p, p + 64, far, far, (1 << 31) - 1, 16, 2, 64)
+    assert "share" not in _append_refusal(lib, p, p + 4096, far, far, (1 << 31) - 1, 16, 2, 64)
+
+
 def _table(monkeypatch, dim=32, **kw):
     """A rotary table on the host (its device is not looked at here)."""
     from glq_b200 import paged
