@@ -530,6 +530,8 @@ paged_stream_kernel(const __grid_constant__ PagedJob J, const __grid_constant__ 
           if (col == 0) J.part_ml[place + row] = make_float2(most, sum);
         }
       }
+      // (the sums lie where the next tile is copied to: ordinary stores are ordered before copies by this alone, not by the barrier)
+      fence_async_smem();
       __syncwarp();
       if (lane == 0) { mbar_arrive(&B.joined[1]); mbar_arrive(&B.empty[stage]); }
       // An item that several CTAs have a part of: a warp has the same rows in each.  The last to arrive adds them up, all from the workspace, in the

@@ -651,3 +651,20 @@ def test_keys_and_values_in_one_place():
         with pytest.raises(RuntimeError, match="share addresses"):
             ops.paged_append(new, new, k[:len(values)], values, slots)
     assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 128), (HF, 64)])
+def test_items_follow_one_another_in_a_ring(dtype, dim):
+    """Each CTA of the streaming kernel has many items of every number of tiles, so that a ring's stages hold keys, then sums, then keys again."""
+    from glq_b200 import ops
+    seqs = 3000
+    g = torch.Generator().manual_seed(4)
+    lengths = torch.randint(1, 700, (seqs,), generator=g).tolist()
+    q, k, v, _, n, offsets = _batch(_gen(5), [64 * 16], [seqs], 2, 8, dim, 16, dtype, poison=False)
+    pages = torch.randint(0, k.shape[0], (seqs, 44), generator=g).to(torch.int32).cuda()
+    lengths = torch.tensor(lengths, device="cuda")
+    y = ops.paged_attention(q, k, v, pages, lengths)
+    for _ in range(5):
+        assert torch.equal(y, ops.paged_attention(q, k, v, pages, lengths))
+    some = torch.arange(0, seqs, 37, device="cuda")
+    _within(y[some], q[some], k, v, pages[some], lengths[some], torch.arange(len(some) + 1, device="cuda"))
