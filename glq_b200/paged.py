@@ -301,8 +301,8 @@ def paged_attention(query, key_cache, value_cache, pages, lengths, *, query_offs
     ``query`` (tokens, heads, head_dim) of the cache's type, the heads a multiple of the cache's: query head h reads key head
     h // (heads // kv_heads).  ``lengths`` (sequences,): keys of every sequence, those of the new tokens among them, in the pages that
     ``pages`` (sequences, columns) int32 names in order.  ``query_offsets`` (sequences + 1,): rows query_offsets[s] .. query_offsets[s + 1] - 1 are
-    the last ones of sequence s, ascending; None: one row per sequence.  A query sees the keys up to its own (``causal``, else all of its
-    sequence), of them the last ``window`` ones (0: all).  ``scale`` (positive): of the scores, head_dim ** -0.5 by default.
+    the last ones of sequence s, ascending; None: one row per sequence.  A query sees the keys up to its own (``causal``, else to its
+    sequence's last), from ``window`` - 1 in front of its own on (0: from the first).  ``scale`` (positive): of the scores, head_dim ** -0.5 by default.
     ``max_query_len``: what no sequence has more rows than, if the program knows it; the faster kernel is chosen by it.
     Integers are int32 or int64 and stay on the device: lengths are held to 0 .. columns * page_size, offsets to 0 .. tokens; a page
     outside the cache reads as zeros.  Rows that see no key are zero.  Rows of no sequence (in front of query_offsets[0], behind the last) are zero in a

@@ -388,8 +388,8 @@ int glqb_paged_append(const GlqbPagedCache* c, const GlqbPagedAppend* a, const G
 
 /* Attention of new tokens over a paged cache that holds their keys already.  Sequence s has lengths[s] keys, in the pages that row s of
  * page_table (int32, page_stride apart, page_columns of them) names in order, and the queries offsets[s] .. offsets[s + 1] - 1
- * (offsets NULL: one per sequence); the last query belongs to the last key.  A query sees the keys up to its own (causal; else all), of them
- * the last `window` (0: all).  heads / kv_heads query heads share a key head.  out = softmax(scale * q k) v, rows without a visible key
+ * (offsets NULL: one per sequence); the last query belongs to the last key.  A query sees the keys up to its own (causal; else to the sequence's
+ * last), from window - 1 in front of its own on (0: from the first).  heads / kv_heads query heads share a key head.  out = softmax(scale * q k) v, rows without a visible key
  * are zero.  All of this is read on the device: lengths are held to 0 .. page_columns * page_size, offsets to 0 .. tokens; a page outside
  * the cache reads as zeros.  Rows of no sequence keep what out holds, or are zeroed with clear_rest.
  * max_query_len: no sequence has more queries (a bound for the choice of the kernel; results do not depend on its truth).

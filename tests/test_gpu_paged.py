@@ -668,3 +668,20 @@ def test_items_follow_one_another_in_a_ring(dtype, dim):
         assert torch.equal(y, ops.paged_attention(q, k, v, pages, lengths))
     some = torch.arange(0, seqs, 37, device="cuda")
     _within(y[some], q[some], k, v, pages[some], lengths[some], torch.arange(len(some) + 1, device="cuda"))
+
+
+@pytest.mark.parametrize("new", [3, 100])
+def test_window_without_causal_begins_in_front_of_the_query(new):
+    """Scores of 0: a query's result is the mean of the values from window - 1 keys in front of its own to the sequence's last."""
+    from glq_b200 import ops
+    n, window = 1000, 50
+    k, v = torch.zeros(1, 1024, 1, 64, device="cuda", dtype=BF), torch.zeros(1, 1024, 1, 64, device="cuda", dtype=BF)
+    pages, lengths, offsets = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([n], device="cuda"), torch.tensor([0, new], device="cuda")
+    for key in (n - new - window, n - new - window + 1, n - window, n - 1):
+        v.zero_()
+        v[0, key] = 1.0
+        y = ops.paged_attention(torch.ones(new, 8, 64, device="cuda", dtype=BF), k, v, pages, lengths, query_offsets=offsets, causal=False, window=window)
+        for i, at in enumerate(range(n - new, n)):
+            first = at - window + 1
+            want = 1.0 / (n - first) if key >= first else 0.0
+            assert (y[i].double() - want).abs().max() <= 2.0 ** -7 * want, (i, key)
