@@ -93,7 +93,7 @@ def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv
     """Frequencies base^(-2 i / dim) of ``dim`` rotated values (even), made once for a model.  ``scaling``: a dict as model
     configurations hold it, "rope_type" "linear", "llama3" or "yarn" with its factors.  ``inv_freq``: radians per position of every pair, in
     place of dim, base and scaling.  ``scale``: factor on cosine and sine in place of the scaling's own.  Frequencies are held in 64
-    bits: angles are exact to position * 2^-53 of the frequency given."""
+    bits: an angle is off by position * (2^-52 of the frequency given + 2^-65 of a turn) at most, and by 2^-26 of a turn where it becomes fp32."""
     own = 1.0
     if inv_freq is not None:
         if dim is not None and dim != 2 * inv_freq.numel() or scaling is not None:
@@ -105,9 +105,11 @@ def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv
         f, own = _frequencies(dim, base, scaling)
     if not f.numel() or not bool(torch.isfinite(f).all()):
         raise ValueError("glq_b200: frequencies must be finite")
-    # fractions of a turn in 2^-64, as signed integers (whole turns per position make no difference at whole positions)
-    whole = [int(math.ldexp(p, 64)) for p in ((f / (2 * math.pi)) % 1.0).tolist()]
-    turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in whole], dtype=torch.int64)
+    # fractions of a turn in 2^-64, as signed integers, the nearest ones (whole turns per position make no difference at whole positions; half a
+    # turn is the same forth and back)
+    turns = f / (2 * math.pi)
+    turns = [round(math.ldexp(p, 64)) for p in (turns - turns.round()).tolist()]
+    turns = torch.tensor([t - 2 ** 64 if t == 2 ** 63 else t for t in turns], dtype=torch.int64)
     device = torch.device("cuda" if device is None else device)
     if device.type != "cuda":
         raise RuntimeError("glq_b200: a rotary table is used on a CUDA device (there is no CPU path)")

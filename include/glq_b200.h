@@ -353,7 +353,7 @@ int glqb_mx4_status(int32_t* status_out);
 /* Rotation of head values by a token's position: of the first 2 * pairs values of a head, values i and i + pairs (or 2 i and 2 i + 1:
  * interleaved) make a pair, (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t) with t = 2 pi * position * turns[i] / 2^64.
  * turns: device, one per pair, fractions of a turn per position as 64-bit integers: products wrap where whole turns do, so that
- * the angle of any position is off by no more than position * 2^-65 turns.  The other values of a head stay as they are. */
+ * an angle is off by position times what turns[i] is (2^-65 of a turn where it is the nearest integer), and by 2^-26 of a turn where it becomes fp32.  The other values of a head stay as they are. */
 typedef struct GlqbRotary {
   const int64_t* turns;
   int32_t pairs, interleaved;

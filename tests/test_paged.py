@@ -200,6 +200,16 @@ def test_table_holds_fractions_of_a_turn(monkeypatch):
         t.scale = 2.0
 
 
+def test_table_is_rounded(monkeypatch):
+    """Of slow pairs, whose frequency's 53 bits end below 2^-64 turns, the nearest number of units is held."""
+    from fractions import Fraction
+    f = torch.tensor([2.0 ** -40 * 1.7, 2.0 ** -50 * 1.3, -2.0 ** -45 * 1.1, 2.0 ** -66, 1.0], dtype=torch.float64)
+    t = _table(monkeypatch, None, inv_freq=f)
+    for v, p in zip(t.turns.tolist(), (f / (2 * math.pi)).tolist()):
+        off = (v - Fraction(p) * 2 ** 64) % 2 ** 64
+        assert min(off, 2 ** 64 - off) <= Fraction(1, 2), (v, p)
+
+
 @pytest.mark.parametrize("name,kw,dim", [("linear", dict(factor=4.0), 64), ("llama3", dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192), 128),
                                          ("yarn", dict(factor=4.0, beta_fast=32.0, beta_slow=1.0, original_max_position_embeddings=32768), 128)])
 def test_scalings_of_long_contexts(monkeypatch, name, kw, dim):
