@@ -89,9 +89,9 @@ def _frequencies(dim, base, scaling):
     return f / factor * stretched + f * (1 - stretched), float(scale)
 
 
-def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv_freq=None, scale=None, device=None) -> Rotary:
+def rotary_table(dim=None, *, base=None, scaling=None, interleaved=False, inv_freq=None, scale=None, device=None) -> Rotary:
     """Frequencies base^(-2 i / dim) of ``dim`` rotated values (even), made once for a model.  ``scaling``: a dict as model
-    configurations hold it, "rope_type" "linear", "llama3" or "yarn" with its factors.  ``inv_freq``: radians per position of every pair, in
+    configurations hold it, "rope_type" "linear", "llama3" or "yarn" with its factors.  ``base``: its "rope_theta" by default, else 10000.  ``inv_freq``: radians per position of every pair, in
     place of dim, base and scaling.  ``scale``: factor on cosine and sine in place of the scaling's own.  Frequencies are held in 64
     bits: an angle is off by position * (2^-52 of the frequency given + 2^-65 of a turn) at most, and by 2^-26 of a turn where it becomes fp32."""
     own = 1.0
@@ -102,6 +102,8 @@ def rotary_table(dim=None, *, base=10000.0, scaling=None, interleaved=False, inv
     else:
         if dim is None or dim < 2 or dim % 2:
             raise ValueError(f"glq_b200: an even number of values is rotated, not {dim}")
+        if base is None:
+            base = (scaling or {}).get("rope_theta") or 10000.0
         f, own = _frequencies(dim, base, scaling)
     if not f.numel() or not bool(torch.isfinite(f).all()):
         raise ValueError("glq_b200: frequencies must be finite")

@@ -210,6 +210,17 @@ def test_table_is_rounded(monkeypatch):
         assert min(off, 2 ** 64 - off) <= Fraction(1, 2), (v, p)
 
 
+def test_base_in_the_scaling(monkeypatch):
+    """Configurations may hold a model's base beside its scaling: it is taken where no other is given."""
+    plain = _table(monkeypatch, 64, base=500000.0).turns
+    assert torch.equal(_table(monkeypatch, 64, scaling={"rope_type": "default", "rope_theta": 500000.0}).turns, plain)
+    assert torch.equal(_table(monkeypatch, 64, base=500000, scaling={"rope_type": "default", "rope_theta": 500000.0}).turns, plain)
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    assert torch.equal(_table(monkeypatch, 64, scaling={**yarn, "rope_theta": 5e5}).turns, _table(monkeypatch, 64, base=5e5, scaling=yarn).turns)
+    assert torch.equal(_table(monkeypatch, 64, scaling=yarn).turns, _table(monkeypatch, 64, base=10000.0, scaling=yarn).turns)
+    assert torch.equal(_table(monkeypatch, 64, base=10000.0, scaling={**yarn, "rope_theta": 5e5}).turns, _table(monkeypatch, 64, scaling=yarn).turns)
+
+
 @pytest.mark.parametrize("name,kw,dim", [("linear", dict(factor=4.0), 64), ("llama3", dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192), 128),
                                          ("yarn", dict(factor=4.0, beta_fast=32.0, beta_slow=1.0, original_max_position_embeddings=32768), 128)])
 def test_scalings_of_long_contexts(monkeypatch, name, kw, dim):
