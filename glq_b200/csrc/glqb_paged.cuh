@@ -134,6 +134,7 @@ __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
   const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool small = J.seqs <= 32;
   if (threadIdx.x == 0) S.units = 0;
+  __syncwarp();                                          // (another lane of this warp may have a share to write there)
   if (small && warp > 0) {
     __syncthreads();
     return;
