@@ -34,7 +34,7 @@ struct PagedJob {
   int lengths_wide, offsets_wide, seqs, page_log, tokens, heads, kv_heads, group, head_dim, causal, window, clear;
   float scale_log2;                  // scale * log2(e): weights are powers of two
   int most_keys;                     // columns * page size
-  int min_units;                     // units that a CTA takes at least
+  int min_units;                     // units of a share where the grid has more CTAs than there is work for (about: shares are equal)
   int rows;                          // of an item
   PagedDivisor by_group, by_rows;
   int begin;                         // what beginning an item costs, in key tiles
@@ -51,14 +51,16 @@ struct PagedJob {
 struct PagedPart { int valid, ends, row0, rows, first, kv_head, queries, keys; };
 
 #ifdef __CUDACC__
+// How work is shared out is arithmetic that the host can do as well, to look at it.
+#define GLQB_LIST __host__ __device__ __forceinline__
 struct PagedSeq { int row0, queries, keys; };
 // Lengths and offsets are held to what there is, so that whatever they hold, nothing outside is read or written.
-__device__ __forceinline__ int pa_offset(const PagedJob& J, int i) {
+GLQB_LIST int pa_offset(const PagedJob& J, int i) {
   if (!J.offsets) return min(i, J.tokens);
   const long long o = J.offsets_wide ? reinterpret_cast<const long long*>(J.offsets)[i] : reinterpret_cast<const int*>(J.offsets)[i];
   return (int)max(0ll, min((long long)J.tokens, o));
 }
-__device__ __forceinline__ PagedSeq pa_seq(const PagedJob& J, int i) {
+GLQB_LIST PagedSeq pa_seq(const PagedJob& J, int i) {
   PagedSeq s;
   s.row0 = pa_offset(J, i);
   s.queries = max(0, pa_offset(J, i + 1) - s.row0);
@@ -67,25 +69,25 @@ __device__ __forceinline__ PagedSeq pa_seq(const PagedJob& J, int i) {
   return s;
 }
 // rows of an item are (query, head of the group) pairs, heads first
-__device__ __forceinline__ int pa_over(int n, const PagedDivisor& d) { return (int)((unsigned long long)(uint32_t)n * d.mul >> d.shift); }
-__device__ __forceinline__ int pa_query(const PagedJob& J, int row) { return pa_over(row, J.by_group); }
+GLQB_LIST int pa_over(int n, const PagedDivisor& d) { return (int)((unsigned long long)(uint32_t)n * d.mul >> d.shift); }
+GLQB_LIST int pa_query(const PagedJob& J, int row) { return pa_over(row, J.by_group); }
 // keys that query i sees: from .. to - 1
-__device__ __forceinline__ int pa_to(const PagedJob& J, const PagedSeq& s, int i) { return J.causal ? max(0, s.keys - s.queries + i + 1) : s.keys; }
-__device__ __forceinline__ int pa_from(const PagedJob& J, const PagedSeq& s, int i) {
+GLQB_LIST int pa_to(const PagedJob& J, const PagedSeq& s, int i) { return J.causal ? max(0, s.keys - s.queries + i + 1) : s.keys; }
+GLQB_LIST int pa_from(const PagedJob& J, const PagedSeq& s, int i) {
   return J.window ? max(0, s.keys - s.queries + i + 1 - J.window) : 0;
 }
 // An item: J.rows rows of one sequence and key head.  Its key tiles are [lo, hi): those that any of its rows sees, one at least, so that
 // every row is written.
 template <int KEYS>
-__device__ __forceinline__ int2 pa_tiles(const PagedJob& J, const PagedSeq& s, int qt) {
+GLQB_LIST int2 pa_tiles(const PagedJob& J, const PagedSeq& s, int qt) {
   const int last = min(s.queries - 1, pa_query(J, min(s.queries * J.group, (qt + 1) * J.rows) - 1));
   const int to = pa_to(J, s, last), from = min(pa_from(J, s, pa_query(J, qt * J.rows)), to);
   const int lo = from / KEYS;
   return make_int2(lo, max(lo + 1, (to + KEYS - 1) / KEYS));
 }
-__device__ __forceinline__ int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return pa_over(s.queries * J.group + J.rows - 1, J.by_rows); }
+GLQB_LIST int pa_q_tiles(const PagedJob& J, const PagedSeq& s) { return pa_over(s.queries * J.group + J.rows - 1, J.by_rows); }
 template <int KEYS>
-__device__ __forceinline__ long long pa_units(const PagedJob& J, const PagedSeq& s) {
+GLQB_LIST long long pa_units(const PagedJob& J, const PagedSeq& s) {
   const int n = pa_q_tiles(J, s);
   long long sum = 0;
   for (int qt = 0; qt < n; ++qt) {
@@ -105,10 +107,16 @@ struct PagedStart {
   long long warp_sum[32];
 };
 // quotient of numbers >= 0 (a division of 64 bits takes some hundred clocks)
-__device__ __forceinline__ long long pa_div(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
+GLQB_LIST long long pa_div(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
+// CTAs that have a share of `total` units, and where that of CTA c begins: the one behind it begins where it ends.
+GLQB_LIST long long pa_ctas(const PagedJob& J, long long total, int grid) {
+  const long long n = pa_div(total + J.min_units - 1, J.min_units);
+  return n < grid ? n : grid;
+}
+GLQB_LIST long long pa_begin(long long total, long long ctas, long long c) { return pa_div(total * c, ctas); }
 // The item that unit r of a sequence's belongs to.
 template <int KEYS>
-__device__ __forceinline__ void pa_place_start(const PagedJob& J, PagedStart& S, int seq, const PagedSeq& s, long long per_head, long long r, long long units) {
+GLQB_LIST void pa_place_start(const PagedJob& J, PagedStart& S, int seq, const PagedSeq& s, long long per_head, long long r, long long units) {
   S.s = s;
   S.seq = seq;
   S.kv_head = (int)pa_div(r, per_head);
@@ -164,9 +172,9 @@ __device__ __forceinline__ void pa_start(const PagedJob& J, PagedStart& S) {
       total += S.warp_sum[w];
     }
   }
-  const long long ctas = min((long long)gridDim.x, pa_div(total + J.min_units - 1, J.min_units));
+  const long long ctas = pa_ctas(J, total, (int)gridDim.x);
   if ((long long)blockIdx.x < ctas) {
-    const long long begin = pa_div(total * blockIdx.x, ctas), end = pa_div(total * (blockIdx.x + 1), ctas);
+    const long long begin = pa_begin(total, ctas, blockIdx.x), end = pa_begin(total, ctas, blockIdx.x + 1);
     if (begin >= before && begin < before + own) {
       long long r = begin - before;
       S.at = begin;
@@ -208,13 +216,13 @@ struct PagedWalk {
   int ctas;
   long long left, at, total;
   PagedPart part[2];                 // what the CTA leaves in the workspace
-  __device__ __forceinline__ PagedWalk(const PagedJob& J, const PagedStart& S)
+  GLQB_LIST PagedWalk(const PagedJob& J, const PagedStart& S)
       : s(S.s), seq(S.seq), kv_head(S.kv_head), qt(S.q_tile), skip(S.skip), q_tiles(S.q_tiles), t(S.tiles), ctas(S.ctas), left(S.units), at(S.at), total(S.total) {
     part[0] = part[1] = PagedPart{0, 1, 0, 0, 0, 0, 0, 0};
   }
   // the CTA that has unit u: the last c with total * c / ctas <= u
-  __device__ __forceinline__ int cta_of(long long u) const { return (int)pa_div((u + 1) * ctas - 1, total); }
-  __device__ __forceinline__ PagedItem next(const PagedJob& J) {
+  GLQB_LIST int cta_of(long long u) const { return (int)pa_div((u + 1) * ctas - 1, total); }
+  GLQB_LIST PagedItem next(const PagedJob& J) {
     PagedItem it{};
     while (left > 0 && !it.more) {
       const int n = t.y - t.x, take = (int)min((long long)(n + J.begin - skip), left);

@@ -405,3 +405,51 @@ def test_runs_cover_the_work_and_parts_find_their_item(lengths, new, rows, keys,
         assert all(r[5] == mine[0][0] and r[6] == len(mine) for r in mine)
         assert mine[0][0] not in cut                             # (a ticket is that CTA's: one item that it begins and does not end)
         cut.add(mine[0][0])
+
+
+@pytest.fixture(scope="module")
+def the_list(tmp_path_factory):
+    """The kernels' own list of work, built for the host."""
+    from glq_b200 import build
+    out = str(tmp_path_factory.mktemp("list") / "list.so")
+    res = subprocess.run([build._nvcc(), *build.NVCC_FLAGS, "-O1", "-I", build.CSRC, "-I", os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "paged_list.cu"), "-o", out],
+                         capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    fn = ctypes.CDLL(out).paged_list
+
+    def rows(lengths, new, group, kv_heads, rows, keys, grid, begin, least, causal=True, window=0):
+        offsets = [sum(new[:i]) for i in range(len(new) + 1)]
+        numbers, most = (ctypes.c_int * (14 << 16))(), 1 << 16
+        n = fn((ctypes.c_longlong * len(lengths))(*lengths), (ctypes.c_longlong * len(offsets))(*offsets), len(lengths), offsets[-1], 1 << 30, group, kv_heads, rows, keys, grid, begin,
+               least, int(causal), window, numbers, most)
+        assert 0 <= n < most
+        return [tuple(numbers[14 * i:14 * i + 14]) for i in range(n)]
+
+    return rows
+
+
+@pytest.mark.parametrize("lengths,new", [([4096], [1]), ([100, 3, 900, 0, 64], [1] * 5), ([700, 2], [650, 2]), ([5000], [5000]), ([31, 64, 1] * 50, [1] * 150),
+                                         ([0, 5, 130, 400, 64, 1, 700, 129], [0, 5, 1, 33, 64, 1, 2, 0]), ([3, 0, 70], [10, 4, 200]), ([9], [0])])
+@pytest.mark.parametrize("rows,keys,ctas,begin,least", [(16, 64, 296, 2, 3), (240, 128, 148, 2, 4), (256, 128, 148, 2, 4), (16, 64, 7, 2, 3), (256, 128, 5, 0, 1)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 200), (False, 0), (False, 30)])
+def test_kernels_share_work_as_the_model_does(the_list, lengths, new, rows, keys, ctas, begin, least, causal, window):
+    """Item for item, and that no query of an item sees a key outside its tiles."""
+    group = 5 if rows == 240 else 4
+    items, runs = _model(lengths, new, group, 2, rows, keys, ctas, begin, least, causal, window) if sum(new) else ([], [])
+    got = the_list(lengths, new, group, 2, rows, keys, ctas, begin, least, causal, window)
+    assert len(got) == len(runs)
+    covered = {}
+    for (c, i, lo, hi, slot, begun_by, parts), row in zip(sorted(runs), got):
+        s, h, t, first_tile, last_tile = items[i]
+        assert row[:3] == (c, s, h) and row[3] == t * rows and row[4] == min(rows, new[s] * group - t * rows) and row[5:8] == (lo, hi, slot)
+        assert slot < 0 or row[8:10] == (begun_by, parts)
+        # keys of the item's first and last query
+        ends = []
+        for q in (row[3] // group, (row[3] + row[4] - 1) // group):
+            at = lengths[s] - new[s] + q
+            ends.append((max(0, at + 1 - window) if window else 0, max(0, at + 1) if causal else lengths[s]))
+        (f0, t0), (f1, t1) = ends
+        assert row[10:] == (f1, t0, f0, t1)
+        assert t1 <= f0 or first_tile * keys <= f0 and t1 <= last_tile * keys
+        covered.setdefault(i, []).append((lo, hi))
+    assert len(covered) == len(items)
