@@ -569,14 +569,15 @@ def test_refusals():
 
 
 # ---- weights far below a row's largest ----------------------------------------------------------------------------
-def _within(y, q, k, v, pages, lengths, offsets, window=0, what=""):
+def _within(y, q, k, v, pages, lengths, offsets, window=0, what="", chain=None):
     """Each value against 64 bits on the device, within what its own weights allow.  A weight is rounded by U of itself or, of fp16's
     subnormal numbers, by half a step: weights are held as 2^7 times those relative to a score that is no larger than the row's
-    largest, so 2^-25 is 2^-32 of the largest at most (bf16 has fp32's exponents).  The result is rounded by U.  In fp32: scores with
+    largest, so 2^-25 is 2^-32 of the largest at most (bf16 has fp32's exponents).  The result is rounded by U of itself or, below 2^-14 in fp16, where
+    numbers are multiples of 2^-24, by 2^-25.  In fp32: scores with
     `dim` products and sums, 2^-23 each where the tensor cores cut off, in a weight and in their sum; no sum is longer than the
-    keys, a step of it off by 2^-24 of what it has, in the values' sum and in the weights'."""
+    keys (or ``chain``), a step of it off by 2^-24 of what it has, in the values' sum and in the weights'."""
     g, dtype = q.shape[1] // k.shape[2], v.dtype
-    floor = 2.0 ** -32 if dtype == HF else 0.0
+    floor, least = (2.0 ** -32, 2.0 ** -25) if dtype == HF else (0.0, 0.0)
     worst = -math.inf
     for i, n in enumerate(lengths.tolist()):
         a, b = int(offsets[i]), int(offsets[i + 1])
@@ -592,8 +593,8 @@ def _within(y, q, k, v, pages, lengths, offsets, window=0, what=""):
             total = weight.sum(-1).transpose(0, 1)[..., None]
             ref, reach, far = (torch.einsum("gqk,kd->qgd", w, x) / total for w, x in ((weight, vv), (weight, vv.abs()), (seen.expand(g, -1, -1).double(), vv.abs())))
             size = torch.einsum("qgd,kd->gqk", qq.abs(), kk.abs()).masked_fill(~seen, 0.0).amax(-1).transpose(0, 1)[..., None] * scale
-            fp32 = 2 * size * (q.shape[2] + 4) * 2.0 ** -23 + 2 * n * 2.0 ** -24 + 2.0 ** -19
-            bound = (U[dtype] + fp32) * reach + floor * far + U[dtype] * (ref.abs() + (U[dtype] + fp32) * reach + floor * far)
+            fp32 = 2 * size * (q.shape[2] + 4) * 2.0 ** -23 + 2 * (chain or n) * 2.0 ** -24 + 2.0 ** -19
+            bound = (U[dtype] + fp32) * reach + floor * far + U[dtype] * (ref.abs() + (U[dtype] + fp32) * reach + floor * far) + least
             worst = max(worst, float(((own - ref).abs() - bound).max()))
             assert bool(torch.isfinite(own).all()) and bool(((own - ref).abs() <= bound).all()), (what, i, h, worst)
 
@@ -685,3 +686,74 @@ def test_window_without_causal_begins_in_front_of_the_query(new):
             first = at - window + 1
             want = 1.0 / (n - first) if key >= first else 0.0
             assert (y[i].double() - want).abs().max() <= 2.0 ** -7 * want, (i, key)
+
+
+def _told_apart(v, pages, size):
+    """Values (pages, rows, heads, dim) that are 0 but in one column, which 64 keys of a sequence have in turn: the results' columns say what each 64 keys gave, and one
+    that is lost or counted twice is an eighth of a column at least of 70,000 keys, where bounds are a hundredth."""
+    key = torch.arange(pages.numel() * size, device=v.device)
+    column = torch.zeros(v.shape[0] * size, dtype=torch.long, device=v.device)
+    column[pages.long().flatten()[key // size] * size + key % size] = key // 64 % v.shape[3]
+    only = (column[:, None] == torch.arange(v.shape[3], device=v.device)).view(v.shape[0], size, 1, -1)
+    return ((v.abs() + 0.5) * only).to(v.dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kv,group,new", [(2, 4, 1), (1, 2, 1), (2, 4, 20)])
+def test_long_context_value_by_value(dtype, kv, group, new):
+    """148 CTAs at least have a share each: 2 * 70,001 keys are less than 1024 for one, and as many parts as
+    CTAs are joined."""
+    from glq_b200 import ops
+    size, length = 64, 70001
+    g = _gen(19)
+    n = -(-length // size)
+    keys, values = _randn(g, n, size, kv, 128, dtype=dtype), _randn(g, n, size, kv, 128, dtype=dtype)
+    pages = torch.randperm(n, generator=g, device="cuda").to(torch.int32)[None]
+    q, values = _randn(g, new, kv * group, 128, dtype=dtype), _told_apart(values, pages, size)
+    lengths, offsets = torch.tensor([length], device="cuda"), torch.tensor([0, new], device="cuda")
+    y = ops.paged_attention(q, keys, values, pages, lengths, query_offsets=offsets, max_query_len=new)
+    _within(y, q, keys, values, pages, lengths, offsets, chain=1024 + 296)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("window", [0, 1500])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (15, 3, 64)])
+@pytest.mark.parametrize("lengths,new", [([6000], [333]), ([2600], [2600]), ([5000, 17, 3000, 900, 2500, 64, 4000], [100, 17, 1, 300, 70, 1, 200])])
+def test_long_chunks_value_by_value(dtype, window, heads, kv, dim, lengths, new):
+    from glq_b200 import ops
+    q, k, v, pages, n, offsets = _batch(_gen(17), lengths, new, kv, heads, dim, 16, dtype, poison=False)
+    for i, length in enumerate(lengths):
+        mine = pages[i, :-(-length // 16)]
+        v[mine.long()] = _told_apart(v, mine, 16)[mine.long()]
+    y = ops.paged_attention(q, k, v, pages, n, query_offsets=offsets, window=window)
+    _within(y, q, k, v, pages, n, offsets, window)
+
+
+WITHOUT_CHAINING = """
+import torch
+from glq_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(3)
+rand = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)
+table, k, v = ops.rotary_table(64), rand(40, 16, 2, 64), rand(40, 16, 2, 64)
+pages = torch.randperm(40, generator=g, device="cuda").to(torch.int32)[None]
+for new, total in ((200, 200), (1, 201), (40, 241), (1, 242)):
+    x, at = rand(new, 8, 64), torch.arange(total - new, total, device="cuda")
+    q = ops.paged_append(x[:, 4:6], x[:, 6:], k, v, pages[0].long()[at // 16] * 16 + at % 16, positions=at, table=table, query=x[:, :4])
+    assert torch.equal(q, ops.rotary(x[:, :4], at, table))
+    y = ops.paged_attention(q, k, v, pages, torch.tensor([total], device="cuda"), query_offsets=torch.tensor([0, new], device="cuda"), max_query_len=new)
+    print(new, y.view(torch.int16).long().sum().item(), k.view(torch.int16).long().sum().item())
+ops.check_device_status()
+"""
+
+
+def test_launches_that_are_not_chained():
+    """GLQB_PDL=0, which is read once in a process: the same bits."""
+    import subprocess
+    import sys
+    said = []
+    for value in ("1", "0"):
+        run = subprocess.run([sys.executable, "-c", WITHOUT_CHAINING], capture_output=True, text=True, timeout=300, env={**os.environ, "GLQB_PDL": value},
+                             cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+        assert run.returncode == 0, run.stderr[-2000:]
+        said.append(run.stdout)
+    assert said[0] == said[1] and said[0].count("\n") == 4
