@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_append_kernel(const __grid
 
 // ---- attention of few rows ------------------------------------------------------------------------
 // Sixteen rows (heads of a group that share a key head, times queries) against tiles of 64 keys: what bounds it is reading the cache.  One token of
-// 131072 keys, fp16, 8 key heads of 128 values: 537 MB in 90.5 us, 5.93 TB/s; 64 sequences of up to 8192: 1.11 GB in 169 to 173 us, 6.4 to 6.6 TB/s.  Small calls are
+// 131072 keys, fp16, 8 key heads of 128 values: 537 MB in 91.4 us, 5.87 TB/s; 64 sequences of up to 8192: 1.11 GB in 173 to 175 us, 6.4 TB/s.  Small calls are
 // latency: one token of 4096 keys, 8.4 MB over 4 key heads, 11.5 us.
 // Two warps bring tiles of keys and of values by TMA into a ring, a page's rows per copy, under the 128-byte swizzle (one warp that brings both was
 // what a tile of four pages waited for); four warps multiply, each 16
@@ -826,12 +826,12 @@ struct PagedForm {
   size_t ml, part_of, bytes;        // where the workspace's second and third part begin, and its size
 };
 // Rows of a sequence and key head up to which the streaming kernel runs: those of one of its items.  More rows are several items, that read the cache once
-// each.  64 sequences of 2048 keys, 8 key heads of 128 values, streaming / on the tensor cores: 8 rows 91 / 110 us, 16 95 / 112, 24 171 / 113, 32 172 / 114,
-// 64 331 / 116; one sequence of 16384: 8 rows 21 / 27, 16 29 / 28, 64 41 / 29.
+// each.  64 sequences of 2048 keys, 8 key heads of 128 values, streaming / on the tensor cores: 8 rows 93 / 109 us, 16 98 / 112, 24 175 / 112, 32 176 / 113,
+// 64 337 / 114; one sequence of 16384: 8 rows 21 / 27, 16 29 / 27, 24 29 / 27, 64 41 / 28.
 constexpr int PA_STREAM_MOST = 16;
-// What beginning an item costs a CTA of either kernel, in its key tiles.  (Of 1, 2 and 4: one token of 4096 keys 11.9, 11.5, 12.2 us; prompt of 2048
-// tokens 59.0, 57.1, 58.5; of 8192 489, 471, 481.  Heads of 64 values, of 2, 4 and 6: 24 sequences of mixed lengths 54.9, 53.6, 52.4; prompt of 2048
-// tokens 54 to 58, 60, 60.)
+// What beginning an item costs a CTA of either kernel, in its key tiles.  (Of 1, 2, 4 and 6: one token of 4096 keys 11.8, 11.5, 12.1, 13.4 us, of 512 8.7, 9.2, 10.4,
+// 11.9; 64 sequences of up to 1024 39.1, 34.1, 33.4, 34.1, of up to 8192 174.6, 173.0, 173.3, 174.8; prompt of 2048 tokens 53.5, 51.5, 52.9, 55.1; of 8192 493, 468, 474, 486.  Heads of 64 values, two
+// processes each, which differ by more: 24 sequences of mixed lengths 49, 49, 49, 48; prompt of 2048 tokens 42 and 48, 44 and 51, 45 and 48, 49 and 51.)
 constexpr int PA_STREAM_BEGIN = 2, PA_TILE_BEGIN = 2;
 PagedForm paged_form(const GlqbPagedCache* c, const GlqbPagedAttention* a, int sms) {
   PagedForm f;

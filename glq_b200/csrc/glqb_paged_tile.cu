@@ -12,8 +12,8 @@
 //
 // What bounds it: the exponentials of 256 rows x 128 keys take 2048 clocks of the special-function units, 16 a clock, and the two products 2048 of the tensor pipe (head_dim
 // 128).  Either would be enough for 2048 from tile to tile; it takes 3300, as each half of the rows goes its way scores, weights, product, scores, and
-// what its warps do beside the exponentials has to hide behind the other half.  32 heads over 8, bf16: a prompt of 8192 tokens 464 us
-// (1185 TFLOP/s), 512 tokens behind 16384 keys 124 us (1125), with the parts joined.  Two halves rather than one tile of 128 rows: then neither unit has work while the other does.
+// what its warps do beside the exponentials has to hide behind the other half.  32 heads over 8, bf16: a prompt of 8192 tokens 467 us
+// (1178 TFLOP/s), 512 tokens behind 16384 keys 125 us (1120), with the parts joined.  Two halves rather than one tile of 128 rows: then neither unit has work while the other does.
 // Five stages of 32 KB for keys and values (head_dim 128) are what 64 KB of queries leave of shared memory.
 #include "glqb_paged.cuh"
 
@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t tile_idesc(int bf16, int cols, int turned) {
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Is there a key in a tile that one of the rows first .. last (of the sequence's queries * group) does not see?
+// Is there a key in the tile from key0 on that is not one of all_from .. all_to - 1, those that all rows see?
 __device__ __forceinline__ bool ragged(int key0, int all_from, int all_to) { return key0 < all_from || key0 + PA_TILE_KEYS > all_to; }
 
 // `rows` rows x 64 values of queries: coordinates (value, head, token)
